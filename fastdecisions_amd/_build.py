@@ -1,9 +1,10 @@
-"""Build the gfx950 kernel library ``libfd_kernels.so`` in-tree with hipcc.
+"""Build the gfx950 kernel libraries ``libfd_kernels.so`` and ``libfd_cache.so`` in-tree with hipcc.
 
 Each source is compiled to an object of its own (hipcc, ``--offload-arch=gfx950``,
 ``-ffp-contract=off`` so every fp32 operation rounds where the source says it
-does, packed-fp32 instructions disabled), then linked into one shared library
-whose exported symbols are exactly the C ABI of ``include/fd_kernels.h``.
+does, packed-fp32 instructions disabled), then linked into shared libraries
+whose exported symbols are exactly the C ABIs of ``include/fd_kernels.h`` and
+``include/fd_cache.h`` (what continues a request from its caches).
 """
 from __future__ import annotations
 
@@ -18,9 +19,13 @@ PKG_DIR = Path(__file__).resolve().parent
 CSRC = PKG_DIR / "csrc"
 LIB_NAME = "libfd_kernels.so"
 LIB_PATH = PKG_DIR / LIB_NAME
+CACHE_LIB_NAME = "libfd_cache.so"
+CACHE_LIB_PATH = PKG_DIR / CACHE_LIB_NAME
 OFFLOAD_ARCH = "gfx950"
 
 SOURCES = ["fd_abi.cpp", "add_rmsnorm.hip", "packed_conv.hip", "gqa_fwd.hip", "gated_delta.hip", "gate_transform.hip", "attn_prologue.hip", "slot_readout.hip", "gated_norm.hip", "hbm_copy.hip"]
+
+CACHE_SOURCES = ["cache_abi.cpp", "paged_kv.hip", "paged_gqa.hip"]
 
 COMMON_FLAGS = [
     "-O3",
@@ -56,16 +61,15 @@ def _run(cmd: list[str]) -> None:
 
 
 def build(verbose: bool = False, jobs: int = 4) -> Path:
-    """Compile every source and link ``libfd_kernels.so``; returns its path."""
+    """Compile every source and link both libraries; returns ``libfd_kernels.so``'s path."""
     cc = hipcc()
     objdir = PKG_DIR / "_build"
     objdir.mkdir(exist_ok=True)
+    libs = [(LIB_PATH, SOURCES), (CACHE_LIB_PATH, CACHE_SOURCES)]
     cmds = []
-    objs = []
-    for src in SOURCES:
+    objs = {src: objdir / (src.rsplit(".", 1)[0] + ".o") for _, sources in libs for src in sources}
+    for src, obj in objs.items():
         path = CSRC / src
-        obj = objdir / (src.rsplit(".", 1)[0] + ".o")
-        objs.append(obj)
         cmd = [cc, *COMMON_FLAGS]
         if src.endswith(".hip"):
             cmd += ["-x", "hip", *DEVICE_FLAGS]
@@ -85,13 +89,14 @@ def build(verbose: bool = False, jobs: int = 4) -> Path:
         for cmd, out in failed:
             sys.stderr.write(" ".join(cmd) + "\n" + out + "\n")
         raise RuntimeError(f"{len(failed)} kernel source(s) failed to compile")
-    tmp = LIB_PATH.with_suffix(".so.tmp")
-    link = [cc, f"--offload-arch={OFFLOAD_ARCH}", "-shared", "-fPIC", "-o", str(tmp), *map(str, objs),
-            "-Wl,--no-undefined", "-Wl,-soname," + LIB_NAME]
-    if verbose:
-        print(" ".join(link), flush=True)
-    _run(link)
-    os.replace(tmp, LIB_PATH)
+    for lib_path, sources in libs:
+        tmp = lib_path.with_suffix(".so.tmp")
+        link = [cc, f"--offload-arch={OFFLOAD_ARCH}", "-shared", "-fPIC", "-o", str(tmp), *(str(objs[s]) for s in sources),
+                "-Wl,--no-undefined", "-Wl,-soname," + lib_path.name]
+        if verbose:
+            print(" ".join(link), flush=True)
+        _run(link)
+        os.replace(tmp, lib_path)
     return LIB_PATH
 
 

@@ -1,0 +1,96 @@
+// What the kernels of the paged cache share: the host's checks of an
+// fd_paged_cache and the device's way from (request, key) to memory.
+#pragma once
+
+#include "../../include/fd_cache.h"
+#include <initializer_list>
+
+#include "fd_common.h"
+
+namespace {
+
+// One of K and V as the kernels see it.
+struct PagedSide {
+  unsigned char* base;
+  uint8_t* scale;
+  int64_t page, head, row;      // strides in bytes
+  int64_t s_page, s_head;
+};
+
+struct PagedView {
+  PagedSide k, v;
+  const int32_t* table;
+  const int32_t* lens;
+  int64_t table_stride;
+  int n_pages, max_pages, shift;  // page_size == 1 << shift
+};
+
+inline int fill_view(const char* what, const fd_paged_cache* c, bool needs_lens, PagedView* out) {
+  FD_REQUIRE(c != nullptr, FD_ERR_INVALID_ARGUMENT, "%s: the cache must be non-null", what);
+  FD_REQUIRE(c->k && c->v && c->page_table && (c->cache_lens || !needs_lens), FD_ERR_INVALID_ARGUMENT,
+             "%s: the cache's tensors, page table and lengths must be non-null", what);
+  FD_REQUIRE(c->head_dim == 64 || c->head_dim == 128 || c->head_dim == 256, FD_ERR_UNSUPPORTED,
+             "%s: head_dim must be 64, 128 or 256 (got %d)", what, c->head_dim);
+  FD_REQUIRE(c->page_size >= 16 && c->page_size <= 256 && (c->page_size & (c->page_size - 1)) == 0,
+             FD_ERR_UNSUPPORTED, "%s: page_size must be a power of two in [16, 256] (got %d)", what, c->page_size);
+  FD_REQUIRE(c->dtype == FD_DTYPE_BF16 || c->dtype == FD_DTYPE_E4M3, FD_ERR_INVALID_ARGUMENT,
+             "%s: the cache's dtype must be FD_DTYPE_BF16 or FD_DTYPE_E4M3", what);
+  FD_REQUIRE(c->n_pages >= 1 && c->max_pages >= 1 && c->kv_heads >= 1, FD_ERR_INVALID_ARGUMENT,
+             "%s: n_pages, max_pages and kv_heads must be >= 1", what);
+  FD_REQUIRE(static_cast<int64_t>(c->max_pages) * c->page_size < (1LL << 30), FD_ERR_UNSUPPORTED,
+             "%s: a request holds fewer than 2^30 keys", what);
+  const bool fp8 = c->dtype == FD_DTYPE_E4M3;
+  FD_REQUIRE(!fp8 || (c->k_scale && c->v_scale), FD_ERR_INVALID_ARGUMENT, "%s: an E4M3 cache needs its scales", what);
+  const int64_t elem = fp8 ? 1 : 2;
+  for (const int64_t* s : {c->k_strides, c->v_strides}) {
+    FD_REQUIRE(s[0] * elem % 16 == 0 && s[1] * elem % 16 == 0 && s[2] * elem % 16 == 0, FD_ERR_ALIGNMENT,
+               "%s: the cache's rows must be 16-byte aligned", what);
+    FD_REQUIRE(s[2] >= 0 && s[2] < (1 << 20), FD_ERR_UNSUPPORTED, "%s: cache row strides must be in [0, 2^20)", what);
+  }
+  FD_REQUIRE(fd_aligned16(c->k) && fd_aligned16(c->v), FD_ERR_ALIGNMENT, "%s: the cache must be 16-byte aligned", what);
+  auto side = [&](void* p, uint8_t* sc, const int64_t* st, const int64_t* ss) {
+    return PagedSide{static_cast<unsigned char*>(p), sc, st[0] * elem, st[1] * elem, st[2] * elem, ss[0], ss[1]};
+  };
+  out->k = side(c->k, c->k_scale, c->k_strides, c->k_scale_strides);
+  out->v = side(c->v, c->v_scale, c->v_strides, c->v_scale_strides);
+  out->table = c->page_table;
+  out->lens = c->cache_lens;
+  out->table_stride = c->table_stride;
+  out->n_pages = c->n_pages;
+  out->max_pages = c->max_pages;
+  out->shift = __builtin_ctz(static_cast<unsigned>(c->page_size));
+  return FD_OK;
+}
+
+// New tokens [start, end) of the T axis of request r, clamped to [0, seq_len]: a
+// malformed offset table cannot move an access outside the tensors.
+__device__ __forceinline__ void request_rows(const int32_t* cu, int r, int seq_len, int* start, int* end) {
+  if (cu == nullptr) {
+    *start = 0;
+    *end = seq_len;
+  } else {
+    *start = min(max(cu[r], 0), seq_len);
+    *end = min(max(cu[r + 1], *start), seq_len);
+  }
+}
+
+__device__ __forceinline__ int request_keys(const PagedView& c, int r) {
+  return min(max(c.lens[r], 0), c.max_pages << c.shift);
+}
+
+// The request of packed row t (the last one that starts at or before it), or -1
+// for a row behind the last request.
+__device__ __forceinline__ int request_of(const int32_t* cu, int n_seqs, int t) {
+  int lo = 0, hi = n_seqs;  // cu[lo] <= t < cu[hi], where the table is well formed
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (cu[mid] <= t) lo = mid;
+    else hi = mid;
+  }
+  return cu[lo] <= t && t < cu[lo + 1] ? lo : -1;
+}
+
+// Scale byte -> 2^(byte - 127).
+__device__ __forceinline__ float scale_of(uint32_t byte) { return __uint_as_float(byte << 23); }
+
+}  // namespace

@@ -1,0 +1,753 @@
+// Grouped-query attention of new tokens over a paged key/value cache, gfx950
+// (bf16 MFMA, fp32 softmax; bf16 or e4m3 pages).
+//
+// The rows of one KV head are the (token, query head of its group) pairs of a
+// request, token by token: row p is token p / G, head p % G.  A row sees the
+// keys up to its token's position.  An item of work is one tile of rows of one
+// (request, KV head) against one range of its keys:
+//
+//   few rows   32 rows, 4 wavefronts that each take every fourth block of 32
+//              keys into LDS of their own: no barrier in the loop, the cache
+//              streams through at the rate of the memory.  Single tokens.
+//   pieces     128 rows, wavefronts share the staged key tiles.  Long suffixes.
+//
+// Key ranges are sized on the device: the lengths are there, and a grid sized by
+// the longest possible request would be mostly empty.  Every workgroup sums the
+// row tiles times key tiles of all requests and cuts every request into ranges
+// of c tiles, c = total / workers, so items are alike whatever the mix of
+// lengths; the host only bounds their number (workers + row tiles).  Items of a
+// split row tile leave (o, max, denominator) in the workspace and
+// paged_gqa_join_kernel joins them.
+//
+// The tile mathematics are those of the uncached kernel (gqa_tile.h): scores
+// transposed (S^T = K Q^T) on v_mfma_f32_32x32x16_bf16, so a lane owns one row's
+// scores; P feeds P V from registers; V^T comes from transposing LDS reads.
+// E4M3 rows are turned into bf16 (code times power-of-two scale: exact) on their
+// way into LDS, so both cache types share everything behind the staging.
+#include <type_traits>
+
+#include "gqa_tile.h"
+#include "paged_common.h"
+
+namespace {
+
+constexpr int kNumXcd = 8;
+
+// RB row blocks of 32 rows and KS key parts of a tile per workgroup, NB 32-key
+// blocks per wavefront and tile.
+template <int D_, bool FP8_, int RB_, int KS_, int NB_>
+struct Shape {
+  static constexpr int D = D_, RB = RB_, KS = KS_, NB = NB_;
+  static constexpr bool FP8 = FP8_;
+  static constexpr bool kPrivate = RB == 1;             // wavefronts stage their own keys
+  static constexpr int kWaves = RB * KS;
+  static constexpr int kThreads = 64 * kWaves;
+  static constexpr int kRows = 32 * RB;
+  static constexpr int kKeys = 32 * KS * NB;            // keys of a tile
+  static constexpr int CR = D / 8;                      // 16-byte chunks of a bf16 row
+  static constexpr int kTileBytes = kKeys * CR * 16;    // K or V
+  static constexpr int kStages = kPrivate ? 1 : 2;
+  static constexpr int kStageBytes = 2 * kTileBytes * kStages;
+  // epilogue: every key part's rows, padded, and their (max, denominator)
+  static constexpr int kRowFloats = D + 4;
+  static constexpr int kEpilogueBytes = KS * kRows * (kRowFloats + 2) * 4;
+  static constexpr int kSmemBytes = kStageBytes > kEpilogueBytes ? kStageBytes : kEpilogueBytes;
+  // 1 KiB copies of a bf16 K (or V) tile per wavefront, and the rows of each
+  static constexpr int kCopies = kTileBytes / 1024 / kWaves;
+  static constexpr int kCopyRows = 1024 / (2 * D);
+  // loads of 16 codes per lane of an E4M3 tile per wavefront, and their rows
+  static constexpr int kLoads = kKeys * D / 1024 / kWaves;
+  static constexpr int kLoadRows = 1024 / D;
+  static_assert(kCopies >= 1 && kLoads >= 1, "a tile gives every wavefront a whole copy");
+  static_assert(kSmemBytes <= 160 * 1024, "LDS");
+};
+
+struct PagedArgs {
+  PagedView c;
+  const uint16_t* q;
+  const uint16_t* gate;
+  uint16_t* o;
+  int64_t qs[3], gs[3], os[3];  // b, h, t
+  const int32_t* cu;
+  int n_req, seq_len, group, kv_heads;
+  int workers, min_tiles;       // key ranges: at least min_tiles tiles, about `workers` items
+  int max_items;                // items the grid and the workspace hold
+  float scale_log2;
+  float* part;                  // per item: rows x D of o, then rows x 2 of (max, denominator)
+};
+
+// The work of one (request, row tile, KV head, key range).
+struct Item {
+  int req, head, rtile, range;
+  int row0, rows;               // first row of the tile, rows of the request
+  int start, n_new, len;        // new tokens on the T axis, keys
+  int tiles;                    // key tiles of a range
+  int base, n_rtiles, n_ranges; // first item of the request; its row tiles and key ranges
+};
+
+__device__ __forceinline__ int wave_scan(int v, int lane) {  // inclusive
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int u = __shfl_up(v, d);
+    if (lane >= d) v += u;
+  }
+  return v;
+}
+
+// Finds work item `want(total items)` (JOIN: row tile, whatever its ranges).  One wavefront
+// looks at 64 requests at a time; false if there is no such item.
+template <int ROWS, int KEYS, bool JOIN, typename Want>
+__device__ __forceinline__ bool find_item(const PagedArgs& a, int lane, Want want, Item* it) {
+  auto sizes = [&](int r, int* start, int* n_new, int* len, int* rt, int* kt) {
+    *start = *n_new = *len = *rt = *kt = 0;
+    if (r < a.n_req) {
+      int end;
+      request_rows(a.cu, r, a.seq_len, start, &end);
+      *n_new = end - *start;
+      *len = request_keys(a.c, r);
+      *rt = static_cast<int>((static_cast<int64_t>(*n_new) * a.group + ROWS - 1) / ROWS);
+      *kt = (*len + KEYS - 1) / KEYS;
+    }
+  };
+  int start, n_new, len, rt, kt;
+  int64_t work = 0;
+  for (int r0 = 0; r0 < a.n_req; r0 += 64) {
+    sizes(r0 + lane, &start, &n_new, &len, &rt, &kt);
+    work += static_cast<int64_t>(rt) * kt;
+  }
+#pragma unroll
+  for (int d = 32; d >= 1; d >>= 1) work += __shfl_xor(work, d);
+  const int64_t per = (work * a.kv_heads + a.workers - 1) / a.workers;
+  const int tiles = static_cast<int>(per > a.min_tiles ? per : a.min_tiles);
+  int total = 0;
+  if (a.n_req > 64) {
+    for (int r0 = 0; r0 < a.n_req; r0 += 64) {
+      sizes(r0 + lane, &start, &n_new, &len, &rt, &kt);
+      int n = rt * (JOIN ? 1 : max((kt + tiles - 1) / tiles, 1)) * a.kv_heads;
+#pragma unroll
+      for (int d = 32; d >= 1; d >>= 1) n += __shfl_xor(n, d);
+      total += n;
+    }
+  }
+  int at = a.n_req > 64 ? want(total) : 0;
+  if (a.n_req > 64 && (at < 0 || at >= total)) return false;
+  int base = 0, before = 0;  // items of the requests before r0 (all ranges), and in terms of `at`
+  for (int r0 = 0; r0 < a.n_req; r0 += 64) {
+    sizes(r0 + lane, &start, &n_new, &len, &rt, &kt);
+    const int ranges = max((kt + tiles - 1) / tiles, 1);
+    const int all = rt * ranges * a.kv_heads;
+    const int mine = JOIN ? rt * a.kv_heads : all;
+    const int incl = wave_scan(mine, lane);
+    const int incl_all = JOIN ? wave_scan(all, lane) : incl;
+    if (a.n_req <= 64) {
+      total = __shfl(incl, 63);
+      at = want(total);
+      if (at < 0 || at >= total) return false;
+    }
+    const uint64_t past = __builtin_amdgcn_ballot_w64(before + incl > at);
+    if (past != 0) {
+      const int l = __builtin_ctzll(past);
+      it->req = r0 + l;
+      const int r_all = __shfl(all, l);
+      const int k = at - (before + __shfl(incl, l) - __shfl(mine, l));  // within the request
+      it->base = base + __shfl(incl_all, l) - r_all;
+      it->n_rtiles = __shfl(rt, l);
+      it->n_ranges = __shfl(ranges, l);
+      it->start = __shfl(start, l);
+      it->n_new = __shfl(n_new, l);
+      it->len = __shfl(len, l);
+      it->tiles = tiles;
+      it->rtile = k % it->n_rtiles;  // row tiles of a key range one after the other: they share its keys
+      const int hr = k / it->n_rtiles;
+      it->range = JOIN ? 0 : hr % it->n_ranges;
+      it->head = JOIN ? hr : hr / it->n_ranges;
+      it->row0 = it->rtile * ROWS;
+      it->rows = it->n_new * a.group;
+      return true;
+    }
+    before += __shfl(incl, 63);
+    base += __shfl(incl_all, 63);
+  }
+  return false;
+}
+
+// Keys that the last row of the tile sees (the tile's keys).
+template <int ROWS>
+__device__ __forceinline__ int keys_of_tile(const PagedArgs& a, const Item& it) {
+  const int last = min(it.row0 + ROWS, it.rows) - 1;
+  return max(0, min(it.len, it.len - it.n_new + last / a.group + 1));
+}
+
+template <int ROWS>
+__device__ __forceinline__ int64_t part_floats(int D) {
+  return static_cast<int64_t>(ROWS) * (D + 2);
+}
+
+// out = acc * inv (* sigmoid(gate)), four features of a row.
+__device__ __forceinline__ void store4(const PagedArgs& a, const Item& it, int row, int d, f32x4_t acc, float inv) {
+  const int p = it.row0 + row;
+  const int token = p / a.group;
+  const int head = it.head * a.group + (p - token * a.group);
+  const int b = a.cu == nullptr ? it.req : 0;
+  const int64_t t = it.start + token;
+  f32x4_t v = acc * inv;
+  if (a.gate != nullptr) {
+    const bf16x4_t g4 = *reinterpret_cast<const bf16x4_t*>(a.gate + b * a.gs[0] + head * a.gs[1] + t * a.gs[2] + d);
+    const f32x4_t g = __builtin_convertvector(g4, f32x4_t);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = v[e] / (1.0f + __expf(-g[e]));
+  }
+  *reinterpret_cast<bf16x4_t*>(a.o + b * a.os[0] + head * a.os[1] + t * a.os[2] + d) = __builtin_convertvector(v, bf16x4_t);
+}
+
+// An index that is the same in all lanes, in a scalar register.
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
+// p[i] for a uniform i, by a scalar load: a vector load here would make the compiler wait for
+// the copies in flight.  Nothing writes the page table while the kernel runs.
+__device__ __forceinline__ int scalar_load(const int32_t* p, int i) {
+  return reinterpret_cast<const __attribute__((address_space(4))) int32_t*>(reinterpret_cast<uintptr_t>(p))[i];
+}
+
+__device__ __forceinline__ void wait_lds_reads() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void wait_copies() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+
+template <class S>
+__global__ __launch_bounds__(S::kThreads) void paged_gqa_kernel(PagedArgs a) {
+  constexpr int D = S::D, CR = S::CR, kKk = D / 16, kNdb = D / 32;
+  __shared__ __attribute__((aligned(1024))) unsigned char smem[S::kSmemBytes];
+  const int tid = threadIdx.x;
+  const int lane = tid & 63;
+  const int wave = uniform(tid >> 6);
+  const int rb = wave % S::RB;   // row block
+  const int kp = wave / S::RB;   // key part
+  const int col = lane & 31, half = lane >> 5;
+
+  Item it;
+  {
+    // XCD x takes one contiguous run of the items: row tiles that share keys meet in one L2
+    const int b = blockIdx.x;
+    auto want = [&](int total) {
+      const int per = (total + kNumXcd - 1) / kNumXcd;
+      const int i = b / kNumXcd;
+      return i < per ? (b % kNumXcd) * per + i : -1;
+    };
+    if (!find_item<S::kRows, S::kKeys, false>(a, lane, want, &it)) return;
+  }
+  it.req = uniform(it.req), it.head = uniform(it.head), it.rtile = uniform(it.rtile), it.range = uniform(it.range);
+  it.row0 = uniform(it.row0), it.rows = uniform(it.rows), it.start = uniform(it.start), it.n_new = uniform(it.n_new);
+  it.len = uniform(it.len), it.tiles = uniform(it.tiles), it.base = uniform(it.base);
+  it.n_rtiles = uniform(it.n_rtiles), it.n_ranges = uniform(it.n_ranges);
+  const int kend = uniform(keys_of_tile<S::kRows>(a, it));
+  const int nt_all = (kend + S::kKeys - 1) / S::kKeys;
+  const int t0 = it.range * it.tiles;
+  if (it.range > 0 && t0 >= nt_all) return;  // nothing of this range is visible to the tile's rows
+  const int nt = min(it.tiles, nt_all - t0);  // 0 where no key is visible at all
+  const bool split = nt_all > it.tiles;
+  // where a part goes; the workspace has a place for every item of a well-formed offset table
+  const int slot = it.base + (it.head * it.n_ranges + it.range) * it.n_rtiles + it.rtile;
+  if (slot < 0 || slot >= a.max_items) return;
+
+  // ---- this lane's row
+  const int p = it.row0 + rb * 32 + col;
+  const int pc = min(p, it.rows - 1);  // rows behind the last one repeat it and are not stored
+  const int token = pc / a.group;
+  const int pos = it.len - it.n_new + token;
+  bf16x8_t qf[kKk];
+  {
+    const int b = a.cu == nullptr ? it.req : 0;
+    const int head = it.head * a.group + (pc - token * a.group);
+    const uint16_t* qp = a.q + b * a.qs[0] + head * a.qs[1] + static_cast<int64_t>(it.start + token) * a.qs[2] + half * 8;
+#pragma unroll
+    for (int kk = 0; kk < kKk; ++kk) qf[kk] = *reinterpret_cast<const bf16x8_t*>(qp + kk * 16);
+  }
+  const bool has_rows = it.row0 + rb * 32 < it.rows;
+  const int pos_min = uniform(it.len - it.n_new + min(it.row0 + rb * 32, it.rows - 1) / a.group);
+  const int pos_max = uniform(it.len - it.n_new + min(it.row0 + rb * 32 + 31, it.rows - 1) / a.group);
+
+  const int32_t* table = a.c.table + it.req * a.c.table_stride;
+  const int page_mask = (1 << a.c.shift) - 1;
+  // keys on no page: any in this item?
+  bool absent = false;
+  if (nt > 0) {
+    const int first = (t0 * S::kKeys) >> a.c.shift;
+    const int last = (min((t0 + nt) * S::kKeys, kend) - 1) >> a.c.shift;
+    bool bad = false;
+    for (int i = first + lane; i <= last; i += 64)
+      bad |= static_cast<unsigned>(table[i]) >= static_cast<unsigned>(a.c.n_pages);
+    absent = __builtin_amdgcn_ballot_w64(bad) != 0;
+  }
+  // Page of a key below kend; keys on no page read page 0 and are masked.
+  auto page_of = [&](int key) {
+    const int page = scalar_load(table, key >> a.c.shift);
+    return static_cast<unsigned>(page) < static_cast<unsigned>(a.c.n_pages) ? page : 0;
+  };
+
+  const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_void_t*)smem));
+  // ---- staging.  Rows past kend repeat row kend - 1; the mask discards them.
+  // bf16: copy g of a tile brings rows g * kCopyRows .. of it, one page's, to 1 KiB of LDS.
+  auto copy_side = [&](const PagedSide& c, int tile, uint32_t lds, bool is_v) {
+#pragma unroll
+    for (int i = 0; i < S::kCopies; ++i) {
+      const int g = S::kPrivate ? wave * S::kCopies + i : i * S::kWaves + wave;
+      const int row0 = uniform(g * S::kCopyRows);
+      const int key0 = uniform(min(tile * S::kKeys + row0, kend - 1));
+      const unsigned char* base = c.base + page_of(key0) * c.page + it.head * c.head;
+      const int lrow = row0 + lane / CR;  // of the tile
+      const int key = min(tile * S::kKeys + lrow, kend - 1);
+      const int chunk = (lane % CR) ^ (is_v ? swz_v<CR>(lrow) : swz_k<CR>(lrow));
+      const uint32_t off = static_cast<uint32_t>((key & page_mask) * static_cast<int>(c.row) + chunk * 16);
+      copy_to_lds(base, off, lds + static_cast<uint32_t>(g * 1024));
+    }
+  };
+  // e4m3: 16 codes per lane into registers, later converted and stored as bf16
+  struct Codes {
+    uint4 w[S::FP8 ? S::kLoads : 1];
+    uint32_t s[S::FP8 ? S::kLoads : 1];
+  };
+  constexpr int kLanesRow = D / 16;
+  auto load_side = [&](const PagedSide& c, int tile, Codes& x) {
+#pragma unroll
+    for (int i = 0; i < S::kLoads; ++i) {
+      const int g = S::kPrivate ? wave * S::kLoads + i : i * S::kWaves + wave;
+      const int row0 = uniform(g * S::kLoadRows);
+      const int key0 = uniform(min(tile * S::kKeys + row0, kend - 1));
+      const int page = page_of(key0);
+      const int key = min(tile * S::kKeys + row0 + lane / kLanesRow, kend - 1) & page_mask;
+      const unsigned char* base = c.base + page * c.page + it.head * c.head;
+      x.w[i] = *reinterpret_cast<const uint4*>(base + static_cast<uint32_t>(key * static_cast<int>(c.row) + (lane % kLanesRow) * 16));
+      x.s[i] = *(c.scale + page * c.s_page + it.head * c.s_head + static_cast<uint32_t>(key));
+    }
+  };
+  auto store_side = [&](const Codes& x, unsigned char* lds, bool is_v) {
+#pragma unroll
+    for (int i = 0; i < S::kLoads; ++i) {
+      const int g = S::kPrivate ? wave * S::kLoads + i : i * S::kWaves + wave;
+      const int row = g * S::kLoadRows + lane / kLanesRow;
+      const float s = scale_of(x.s[i]);
+      const uint32_t w[4] = {x.w[i].x, x.w[i].y, x.w[i].z, x.w[i].w};
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        uint32_t b[4];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int code = static_cast<int>(w[2 * h + e]);
+          const auto f0 = __builtin_amdgcn_cvt_pk_f32_fp8(code, false);
+          const auto f1 = __builtin_amdgcn_cvt_pk_f32_fp8(code, true);
+          b[2 * e] = fd_pack2(f0[0] * s, f0[1] * s);
+          b[2 * e + 1] = fd_pack2(f1[0] * s, f1[1] * s);
+        }
+        const int chunk = ((lane % kLanesRow) * 2 + h) ^ (is_v ? swz_v<CR>(row) : swz_k<CR>(row));
+        *reinterpret_cast<uint4*>(lds + row * CR * 16 + chunk * 16) = uint4{b[0], b[1], b[2], b[3]};
+      }
+    }
+  };
+
+  f32x16_t o[kNdb];
+#pragma unroll
+  for (int db = 0; db < kNdb; ++db) o[db] = f32x16_t{};
+  float m_run = -__builtin_inff();  // running maximum (log2 units), may lag the true one by 8
+  float l_run = 0.0f;               // this lane's part of the denominator
+
+  // ---- one 32-key block from LDS: scores, softmax, then P V.  `row0` is the block's
+  // first row within the staged tile, kb0 its first key.
+  const int grp = lane >> 4, li = lane & 15;
+  bf16x8_t pb[2];
+  auto scores = [&](const unsigned char* kt, int row0, int kb0) {
+    f32x16_t s = f32x16_t{};
+    const int row = row0 + sigma(col);
+#pragma unroll
+    for (int kk = 0; kk < kKk; ++kk) {
+      const bf16x8_t kf = *reinterpret_cast<const bf16x8_t*>(kt + row * CR * 16 + (((2 * kk + half) ^ swz_k<CR>(row)) * 16));
+      s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qf[kk], s, 0, 0, 0);
+    }
+    if (kb0 + 31 > pos_min || absent) {
+      bool there[2] = {true, true};
+      if (absent) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int key = min(kb0 + 16 * j, kend - 1);
+          there[j] = static_cast<unsigned>(scalar_load(table, uniform(key >> a.c.shift))) < static_cast<unsigned>(a.c.n_pages);
+        }
+      }
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int key = kb0 + (r >> 3) * 16 + half * 8 + (r & 7);
+        if (key > pos || !there[r >> 3]) s[r] = -__builtin_inff();
+      }
+    }
+    float mx = s[0];
+#pragma unroll
+    for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[r]);
+    mx = half_max(mx) * a.scale_log2;
+    const bool grow = mx > m_run + 8.0f;
+    const float m_new = grow ? mx : m_run;
+    const float alpha = grow ? __builtin_amdgcn_exp2f(m_run - m_new) : 1.0f;
+    const float m_sub = m_new == -__builtin_inff() ? 0.0f : m_new;  // nothing seen so far: p = 0
+    m_run = m_new;
+    if (__builtin_amdgcn_ballot_w64(grow) != 0) {
+#pragma unroll
+      for (int db = 0; db < kNdb; ++db) o[db] *= alpha;
+    }
+    float psum = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      f32x8_t pv;
+#pragma unroll
+      for (int r = 0; r < 8; ++r) pv[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[8 * j + r], a.scale_log2, -m_sub));
+      pb[j] = __builtin_convertvector(pv, bf16x8_t);
+      // the denominator takes the rounded p: its error then cancels where a few keys carry the row
+      const f32x8_t pr = __builtin_convertvector(pb[j], f32x8_t);
+#pragma unroll
+      for (int r = 0; r < 8; ++r) psum += pr[r];
+    }
+    l_run = l_run * alpha + psum;
+  };
+  auto p_v = [&](const unsigned char* vt, int row0, int kb0) {
+    // a block with masked keys: their values must not reach a row as 0 * NaN or 0 * inf
+    const bool guard = kb0 + 31 > pos_min || absent;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+#pragma unroll
+      for (int db = 0; db < kNdb; ++db) {
+        const int dim = db * 32 + 16 * (grp & 1) + 4 * (li & 3);
+        const int row = row0 + 16 * j + 8 * (grp >> 1) + (li >> 2);
+        const unsigned char* vp = vt + row * CR * 16 + (((dim >> 3) ^ swz_v<CR>(row)) * 16) + (dim & 7) * 2;
+        v4i16_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16_t*)vp);
+        v4i16_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16_t*)(vp + 4 * CR * 16));
+        if (guard) {
+          short e[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+          bool odd = false;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) odd |= (e[i] & 0x7f80) == 0x7f80;
+          if (__builtin_amdgcn_ballot_w64(odd) != 0) {
+            // This lane holds V[key 16 j + 8 half + i][32 db + col]: infinities and NaN leave the
+            // product and are added by hand to the rows that see them.
+#pragma unroll 1
+            for (int i = 0; i < 8; ++i) {
+              const float x = (e[i] & 0x7f80) == 0x7f80 ? fd_bf16_to_f32(static_cast<uint16_t>(e[i])) : 0.0f;
+              float pi = 0.0f;
+#pragma unroll
+              for (int u = 0; u < 8; ++u) pi = u == i ? static_cast<float>(pb[j][u]) : pi;
+#pragma unroll 1
+              for (int h = 0; h < 2; ++h) {
+                const float ph = __shfl(pi, h * 32 + col);  // this lane's row, key 16 j + 8 h + i
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                  const int d = (r & 3) + 8 * (r >> 2) + 4 * half;  // feature of o[db][r]
+                  const float xd = __shfl(x, h * 32 + d);
+                  if (xd != 0.0f && ph != 0.0f) o[db][r] += ph * xd;
+                }
+              }
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              if ((lo[i] & 0x7f80) == 0x7f80) lo[i] = 0;
+              if ((hi[i] & 0x7f80) == 0x7f80) hi[i] = 0;
+            }
+          }
+        }
+        const short __attribute__((ext_vector_type(8))) vv = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+        o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, vv), pb[j], o[db], 0, 0, 0);
+      }
+    }
+  };
+
+  unsigned char* const k_lds = smem;
+  unsigned char* const v_lds = smem + S::kTileBytes * S::kStages;
+  if constexpr (S::kPrivate) {
+    // ---- every wavefront walks its own blocks: tile t's rows wave * 32 .. + 31.  K and V of a
+    // block have one buffer each; the next K is copied during the softmax and P V, the next V
+    // during the next scores.
+    const int row0 = wave * 32;
+    const int mine = max(0, min(nt, (kend - t0 * S::kKeys - row0 + S::kKeys - 1) / S::kKeys));
+    if constexpr (!S::FP8) {
+      if (mine > 0) {
+        copy_side(a.c.k, t0, lds0, false);
+        copy_side(a.c.v, t0, lds0 + S::kTileBytes, true);
+      }
+      for (int t = 0; t < mine; ++t) {
+        const int kb0 = (t0 + t) * S::kKeys + row0;
+        wait_copies<S::kCopies>();  // K has landed, V may be in flight
+        scores(k_lds, row0, kb0);
+        wait_lds_reads();
+        if (t + 1 < mine) {
+          copy_side(a.c.k, t0 + t + 1, lds0, false);
+          wait_copies<S::kCopies>();  // V has landed, the next K may be in flight
+        } else {
+          wait_copies<0>();
+        }
+        p_v(v_lds, row0, kb0);
+        wait_lds_reads();
+        if (t + 1 < mine) copy_side(a.c.v, t0 + t + 1, lds0 + S::kTileBytes, true);
+      }
+    } else {
+      Codes ck, cv;
+      if (mine > 0) {
+        load_side(a.c.k, t0, ck);
+        load_side(a.c.v, t0, cv);
+      }
+      for (int t = 0; t < mine; ++t) {
+        const int kb0 = (t0 + t) * S::kKeys + row0;
+        store_side(ck, k_lds, false);
+        if (t + 1 < mine) load_side(a.c.k, t0 + t + 1, ck);
+        scores(k_lds, row0, kb0);
+        store_side(cv, v_lds, true);
+        if (t + 1 < mine) load_side(a.c.v, t0 + t + 1, cv);
+        p_v(v_lds, row0, kb0);
+      }
+    }
+  } else {
+    // ---- shared tiles, two stages: tile t + 1 arrives while tile t is worked on
+    auto work_on = [&](int t, int buf) {
+#pragma unroll
+      for (int nb = 0; nb < S::NB; ++nb) {
+        const int row0 = (kp * S::NB + nb) * 32;
+        const int kb0 = (t0 + t) * S::kKeys + row0;
+        if (has_rows && kb0 <= pos_max) {
+          scores(k_lds + buf * S::kTileBytes, row0, kb0);
+          p_v(v_lds + buf * S::kTileBytes, row0, kb0);
+        }
+      }
+    };
+    if constexpr (!S::FP8) {
+      auto copy_tile = [&](int t, int buf) {
+        copy_side(a.c.k, t0 + t, lds0 + static_cast<uint32_t>(buf * S::kTileBytes), false);
+        copy_side(a.c.v, t0 + t, lds0 + static_cast<uint32_t>((S::kStages + buf) * S::kTileBytes), true);
+      };
+      if (nt > 0) copy_tile(0, 0);
+      for (int t = 0; t < nt; ++t) {
+        wait_copies<0>();
+        wait_lds_reads();  // of tile t - 1: its stage is copied over next
+        __syncthreads();
+        if (t + 1 < nt) copy_tile(t + 1, (t + 1) & 1);
+        work_on(t, t & 1);
+      }
+    } else {
+      Codes ck, cv;
+      if (nt > 0) {
+        load_side(a.c.k, t0, ck);
+        load_side(a.c.v, t0, cv);
+      }
+      for (int t = 0; t < nt; ++t) {
+        // the other stage is being read by the wavefronts still at tile t - 1
+        store_side(ck, k_lds + (t & 1) * S::kTileBytes, false);
+        store_side(cv, v_lds + (t & 1) * S::kTileBytes, true);
+        if (t + 1 < nt) {
+          load_side(a.c.k, t0 + t + 1, ck);
+          load_side(a.c.v, t0 + t + 1, cv);
+        }
+        __syncthreads();
+        work_on(t, t & 1);
+      }
+    }
+  }
+
+  // ---- join the key parts through LDS, row by row, then store the rows or leave the item's part
+  __syncthreads();  // the stages are free
+  float* const rowsf = reinterpret_cast<float*>(smem);
+  float* const ml = rowsf + S::KS * S::kRows * S::kRowFloats;
+  {
+    const int at = kp * S::kRows + rb * 32 + col;
+    float* dst = rowsf + at * S::kRowFloats;
+#pragma unroll
+    for (int db = 0; db < kNdb; ++db)
+#pragma unroll
+      for (int r4 = 0; r4 < 4; ++r4)
+        *reinterpret_cast<f32x4_t*>(dst + db * 32 + r4 * 8 + half * 4) =
+            f32x4_t{o[db][r4 * 4], o[db][r4 * 4 + 1], o[db][r4 * 4 + 2], o[db][r4 * 4 + 3]};
+    const float l = half_sum(l_run);
+    if (half == 0) {
+      ml[at * 2] = m_run;
+      ml[at * 2 + 1] = l;
+    }
+  }
+  __syncthreads();
+  const int rows = min(S::kRows, it.rows - it.row0);
+  float* const part = a.part + slot * part_floats<S::kRows>(D);
+  for (int i = tid; i < rows * (D / 4); i += S::kThreads) {
+    const int row = i / (D / 4), d = (i % (D / 4)) * 4;
+    float m = ml[row * 2];
+#pragma unroll
+    for (int s = 1; s < S::KS; ++s) m = fmaxf(m, ml[(s * S::kRows + row) * 2]);
+    const float m_sub = m == -__builtin_inff() ? 0.0f : m;
+    f32x4_t acc = {0.0f, 0.0f, 0.0f, 0.0f};
+    float l = 0.0f;
+#pragma unroll
+    for (int s = 0; s < S::KS; ++s) {
+      const int at = s * S::kRows + row;
+      const float w = __builtin_amdgcn_exp2f(ml[at * 2] - m_sub);
+      l += ml[at * 2 + 1] * w;
+      acc += *reinterpret_cast<const f32x4_t*>(rowsf + at * S::kRowFloats + d) * w;
+    }
+    if (!split) {
+      store4(a, it, row, d, acc, l == 0.0f ? 0.0f : 1.0f / l);
+    } else {
+      *reinterpret_cast<f32x4_t*>(part + row * D + d) = acc;
+      if (d == 0) {
+        part[S::kRows * D + row * 2] = m;
+        part[S::kRows * D + row * 2 + 1] = l;
+      }
+    }
+  }
+}
+
+// Joins the key ranges of every split row tile and stores its rows.
+template <class S>
+__global__ __launch_bounds__(256) void paged_gqa_join_kernel(PagedArgs a) {
+  constexpr int D = S::D;
+  Item it;
+  const int b = blockIdx.x;
+  if (!find_item<S::kRows, S::kKeys, true>(a, threadIdx.x & 63, [&](int) { return b; }, &it)) return;
+  const int nt_all = (keys_of_tile<S::kRows>(a, it) + S::kKeys - 1) / S::kKeys;
+  const int ranges = (nt_all + it.tiles - 1) / it.tiles;
+  if (ranges <= 1) return;  // its one item has stored the rows
+  const int slot = it.base + it.head * it.n_ranges * it.n_rtiles + it.rtile;
+  if (slot < 0 || slot + (ranges - 1) * static_cast<int64_t>(it.n_rtiles) >= a.max_items) return;
+  const int rows = min(S::kRows, it.rows - it.row0);
+  const int64_t step = it.n_rtiles * part_floats<S::kRows>(D);  // from one range's part to the next one's
+  const float* const part = a.part + slot * part_floats<S::kRows>(D);
+  for (int i = threadIdx.x; i < rows * (D / 4); i += 256) {
+    const int row = i / (D / 4), d = (i % (D / 4)) * 4;
+    float m = -__builtin_inff();
+    for (int s = 0; s < ranges; ++s) m = fmaxf(m, part[s * step + S::kRows * D + row * 2]);
+    const float m_sub = m == -__builtin_inff() ? 0.0f : m;
+    f32x4_t acc = {0.0f, 0.0f, 0.0f, 0.0f};
+    float l = 0.0f;
+    for (int s = 0; s < ranges; ++s) {
+      const float* ps = part + s * step;
+      const float w = __builtin_amdgcn_exp2f(ps[S::kRows * D + row * 2] - m_sub);
+      l += ps[S::kRows * D + row * 2 + 1] * w;
+      acc += *reinterpret_cast<const f32x4_t*>(ps + row * D + d) * w;
+    }
+    store4(a, it, row, d, acc, l == 0.0f ? 0.0f : 1.0f / l);
+  }
+}
+
+template <int D, bool FP8>
+using Few = Shape<D, FP8, 1, 4, 1>;
+template <int D, bool FP8>
+using Piece = Shape<D, FP8, 4, D == 256 ? 1 : 2, D == 64 ? 2 : 1>;
+
+// Items, row tiles and workspace of a call, whatever the lengths turn out to be.
+struct Plan {
+  bool few;
+  int rows, keys, workers, min_tiles;
+  int64_t items, rtiles, bytes;
+  bool may_split;
+};
+
+Plan plan_of(int64_t requests, int64_t tokens, int group, int kv_heads, int head_dim, int64_t max_keys, int max_seqlen) {
+  Plan p;
+  p.few = static_cast<int64_t>(max_seqlen) * group <= 32;
+  p.rows = p.few ? Few<64, false>::kRows : Piece<64, false>::kRows;
+  p.keys = p.few ? Few<64, false>::kKeys
+                 : head_dim == 64 ? Piece<64, false>::kKeys : head_dim == 128 ? Piece<128, false>::kKeys : Piece<256, false>::kKeys;
+  p.workers = p.few ? 1024 : 512;
+  p.min_tiles = 256 / p.keys;
+  // a request's last row tile may be partly empty, its last key range too
+  p.rtiles = kv_heads * (tokens * group / p.rows + requests);
+  p.items = p.workers + p.rtiles;
+  p.may_split = max_keys > static_cast<int64_t>(p.min_tiles) * p.keys;
+  p.bytes = p.may_split ? p.items * p.rows * (head_dim + 2) * 4 : 0;
+  return p;
+}
+
+template <class S, class Join>
+void launch(const PagedArgs& a, const Plan& p, hipStream_t s) {
+  static_assert(S::kRows == Join::kRows && S::kKeys == Join::kKeys, "one way of cutting the work");
+  const int64_t blocks = (p.items + kNumXcd - 1) / kNumXcd * kNumXcd;
+  hipLaunchKernelGGL((paged_gqa_kernel<S>), dim3(static_cast<unsigned>(blocks)), dim3(S::kThreads), 0, s, a);
+  if (p.may_split)
+    hipLaunchKernelGGL((paged_gqa_join_kernel<Join>), dim3(static_cast<unsigned>(p.rtiles)), dim3(256), 0, s, a);
+}
+
+template <int D>
+void launch_dim(const PagedArgs& a, const Plan& p, bool fp8, hipStream_t s) {
+  if (p.few) {
+    if (fp8) launch<Few<D, true>, Few<D, false>>(a, p, s);
+    else launch<Few<D, false>, Few<D, false>>(a, p, s);
+  } else {
+    if (fp8) launch<Piece<D, true>, Piece<D, false>>(a, p, s);
+    else launch<Piece<D, false>, Piece<D, false>>(a, p, s);
+  }
+}
+
+int check_sizes(const char* what, int batch, int q_heads, int kv_heads, int seq_len, int n_seqs, int max_seqlen) {
+  FD_REQUIRE(batch >= 0 && seq_len >= 0 && q_heads >= 1 && kv_heads >= 1 && q_heads % kv_heads == 0 && n_seqs >= 0,
+             FD_ERR_INVALID_ARGUMENT, "%s: sizes must be >= 0 and q_heads a multiple of kv_heads >= 1", what);
+  FD_REQUIRE(n_seqs == 0 || batch == 1, FD_ERR_INVALID_ARGUMENT, "%s: cu_seqlens requires batch == 1", what);
+  FD_REQUIRE(max_seqlen >= 0 && max_seqlen <= seq_len, FD_ERR_INVALID_ARGUMENT,
+             "%s: max_seqlen must be in [0, seq_len]", what);
+  FD_REQUIRE(static_cast<int64_t>(batch) * seq_len * q_heads < (1LL << 30), FD_ERR_UNSUPPORTED,
+             "%s: batch * seq_len * q_heads must be below 2^30", what);
+  return FD_OK;
+}
+
+}  // namespace
+
+extern "C" int64_t fd_paged_gqa_workspace_bytes(int batch, int q_heads, int kv_heads, int seq_len, int head_dim,
+                                                int page_size, int max_pages, int n_seqs, int max_seqlen) {
+  static const char* what = "fd_paged_gqa_workspace_bytes";
+  if (int rc = check_sizes(what, batch, q_heads, kv_heads, seq_len, n_seqs, max_seqlen)) return rc;
+  FD_REQUIRE(head_dim == 64 || head_dim == 128 || head_dim == 256, FD_ERR_UNSUPPORTED,
+             "%s: head_dim must be 64, 128 or 256 (got %d)", what, head_dim);
+  FD_REQUIRE(page_size >= 1 && max_pages >= 1, FD_ERR_INVALID_ARGUMENT, "%s: page_size and max_pages must be >= 1", what);
+  return plan_of(n_seqs > 0 ? n_seqs : batch, static_cast<int64_t>(batch) * seq_len, q_heads / kv_heads, kv_heads,
+                 head_dim, static_cast<int64_t>(max_pages) * page_size, max_seqlen).bytes;
+}
+
+extern "C" int fd_paged_gqa_fwd(const void* q, const fd_paged_cache* cache, const void* gate, void* out,
+                                const int64_t q_strides[4], const int64_t gate_strides[4], const int64_t out_strides[4],
+                                int batch, int q_heads, int seq_len, float scale, const int32_t* cu_seqlens, int n_seqs,
+                                int max_seqlen, void* workspace, int64_t workspace_bytes, void* stream) {
+  static const char* what = "fd_paged_gqa_fwd";
+  FD_REQUIRE(q && out && q_strides && out_strides && (!gate || gate_strides), FD_ERR_INVALID_ARGUMENT,
+             "%s: tensors and strides must be non-null", what);
+  PagedArgs a;
+  if (int rc = fill_view(what, cache, true, &a.c)) return rc;
+  FD_REQUIRE((cu_seqlens != nullptr) == (n_seqs > 0), FD_ERR_INVALID_ARGUMENT,
+             "%s: cu_seqlens and n_seqs >= 1 come together", what);
+  if (int rc = check_sizes(what, batch, q_heads, cache->kv_heads, seq_len, n_seqs, max_seqlen)) return rc;
+  FD_REQUIRE(scale > 0.0f && scale < 1e30f, FD_ERR_INVALID_ARGUMENT, "%s: scale must be positive", what);
+  auto rows_ok = [](const void* p, const int64_t* s) {
+    return fd_aligned16(p) && s[3] == 1 && s[0] % 8 == 0 && s[1] % 8 == 0 && s[2] % 8 == 0;
+  };
+  FD_REQUIRE(rows_ok(q, q_strides) && rows_ok(out, out_strides) && (!gate || rows_ok(gate, gate_strides)),
+             FD_ERR_ALIGNMENT, "%s: rows must be contiguous and 16-byte aligned", what);
+  const int requests = n_seqs > 0 ? n_seqs : batch;
+  if (requests == 0 || seq_len == 0) return FD_OK;
+  const Plan p = plan_of(requests, static_cast<int64_t>(batch) * seq_len, q_heads / cache->kv_heads, cache->kv_heads,
+                         cache->head_dim, static_cast<int64_t>(cache->max_pages) * cache->page_size, max_seqlen);
+  FD_REQUIRE(p.items < (1LL << 30), FD_ERR_UNSUPPORTED, "%s: problem too large", what);
+  FD_REQUIRE(p.bytes == 0 || (workspace && fd_aligned16(workspace) && workspace_bytes >= p.bytes),
+             FD_ERR_INVALID_ARGUMENT, "%s: the workspace must be 16-byte aligned and hold %lld bytes", what,
+             static_cast<long long>(p.bytes));
+  a.q = static_cast<const uint16_t*>(q);
+  a.gate = static_cast<const uint16_t*>(gate);
+  a.o = static_cast<uint16_t*>(out);
+  for (int i = 0; i < 3; ++i) {
+    a.qs[i] = q_strides[i];
+    a.gs[i] = gate ? gate_strides[i] : 0;
+    a.os[i] = out_strides[i];
+  }
+  a.cu = cu_seqlens;
+  a.n_req = requests;
+  a.seq_len = seq_len;
+  a.group = q_heads / cache->kv_heads;
+  a.kv_heads = cache->kv_heads;
+  a.workers = p.workers;
+  a.min_tiles = p.min_tiles;
+  a.max_items = static_cast<int>(p.items);
+  a.scale_log2 = scale * 1.4426950408889634f;
+  a.part = static_cast<float*>(workspace);
+  const bool fp8 = cache->dtype == FD_DTYPE_E4M3;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (cache->head_dim == 64) launch_dim<64>(a, p, fp8, s);
+  else if (cache->head_dim == 128) launch_dim<128>(a, p, fp8, s);
+  else launch_dim<256>(a, p, fp8, s);
+  return fd_check_launch(what);
+}

@@ -1,0 +1,135 @@
+/*
+ * fd_cache.h — C ABI of libfd_cache.so: the gfx950 kernels that continue a
+ * request from its caches (paged keys/values, conv state, delta-rule state).
+ *
+ *   fd_paged_kv_write     keys and values of new tokens into a paged cache (bf16, or e4m3 quantised on the way)
+ *   fd_paged_kv_read      the pages back as dense bf16 keys and values
+ *   fd_paged_gqa_fwd      causal grouped-query attention of the new tokens over the paged cache
+ *   fd_gated_delta_step   the gated delta rule token by token, from and into its fp32 state
+ *   fd_packed_conv_state  the packed causal conv + activation continued from its state
+ *
+ * They serve what the reference's prefix cache serves (ref: src/decider/shared_prefix.py:
+ * keys/values, conv state and recurrent state of a prefix, continued by suffixes).
+ *
+ * Conventions as in fd_kernels.h: device pointers, bf16 as raw 16-bit storage, work
+ * enqueued on `stream`, no allocation, no synchronisation, FD_OK or a negative FD_ERR_*
+ * code, with the message in fd_cache_last_error() (of the calling thread).
+ */
+#ifndef FD_CACHE_H
+#define FD_CACHE_H
+
+#include "fd_kernels.h"
+
+#ifdef __cplusplus
+extern "C" {
+#endif
+
+#define FD_CACHE_ABI_VERSION 1
+
+/* Cache element type besides FD_DTYPE_BF16: OCP 8-bit floats with 4 exponent and 3 mantissa bits. */
+#define FD_DTYPE_E4M3 2
+
+FD_API int fd_cache_abi_version(void);
+
+/* Message describing the last failed call of this library on this thread ("" if none). */
+FD_API const char* fd_cache_last_error(void);
+
+/*
+ * A paged key/value cache and the requests' view of it.
+ *
+ *   k, v      [n_pages, kv_heads, page_size, head_dim] of dtype (FD_DTYPE_BF16 or FD_DTYPE_E4M3);
+ *             strides {page, head, row} in elements, head_dim contiguous
+ *   k_scale, v_scale  with FD_DTYPE_E4M3: [n_pages, kv_heads, page_size] bytes, strides {page, head},
+ *             rows contiguous; byte b stands for the scale 2^(b - 127), b in [1, 254], and a cached
+ *             value is its code times that scale.  NULL with FD_DTYPE_BF16
+ *   page_table  [requests, max_pages] int32 on the device, rows table_stride elements apart: key j of
+ *             request r is row j % page_size of page page_table[r][j / page_size].  An entry outside
+ *             [0, n_pages) is no page: its keys are not there (not written, read as zeros, not visible)
+ *   cache_lens  [requests] int32 on the device: the keys of each request, the new tokens of the call
+ *             included (clamped to [0, max_pages * page_size]); the last n new tokens of request r are
+ *             its keys cache_lens[r] - n .. cache_lens[r] - 1.  Not used by fd_paged_kv_read
+ *
+ * Limits: head_dim 64, 128 or 256; page_size a power of two in [16, 256]; cache rows and
+ * tensors 16-byte aligned; row strides below 2^20 elements.
+ */
+typedef struct fd_paged_cache {
+  void* k;
+  void* v;
+  uint8_t* k_scale;
+  uint8_t* v_scale;
+  int64_t k_strides[3];
+  int64_t v_strides[3];
+  int64_t k_scale_strides[2];
+  int64_t v_scale_strides[2];
+  const int32_t* page_table;
+  int64_t table_stride;
+  const int32_t* cache_lens;
+  int32_t n_pages;
+  int32_t page_size;
+  int32_t max_pages;
+  int32_t kv_heads;
+  int32_t head_dim;
+  int32_t dtype;
+} fd_paged_cache;
+
+/*
+ * Writes the keys and values of new tokens into their pages.
+ *
+ *   k, v  [batch, kv_heads, seq_len, head_dim] bf16, strides {b, h, t, d} in elements (d contiguous)
+ * Without cu_seqlens request r is batch row r with seq_len new tokens.  With cu_seqlens (device
+ * int32[n_seqs + 1], non-decreasing from 0) batch is 1 and request r's new tokens are
+ * [cu_seqlens[r], cu_seqlens[r + 1]) of the T axis; tokens behind the last request are ignored.
+ *
+ * FD_DTYPE_E4M3: per (token, head) the scale is the smallest 2^E with max|x| <= 448 * 2^E over the
+ * row's finite values (E >= -126; 2^0 for a row of zeros), the code is x / 2^E rounded to nearest
+ * even; an infinity becomes +-448 * 2^E, a NaN stays NaN.  Powers of two keep the division and the way
+ * back exact, so a value is off by at most half a step of its code.
+ * A page that two requests of a call write must not be shared between them at the same rows.
+ */
+FD_API int fd_paged_kv_write(const void* k, const void* v, const int64_t k_strides[4], const int64_t v_strides[4],
+                             const fd_paged_cache* cache, int batch, int seq_len, const int32_t* cu_seqlens,
+                             int n_seqs, void* stream);
+
+/*
+ * The first cu_seqlens[r + 1] - cu_seqlens[r] keys and values of every request r as dense bf16 rows
+ * [cu_seqlens[r], cu_seqlens[r + 1]) of k_out and v_out [kv_heads, total, head_dim] (strides {h, t};
+ * d contiguous).  Keys past the page table or on no page are zeros; rows behind the last request are
+ * left as they were.  cache_lens is not used.
+ */
+FD_API int fd_paged_kv_read(const fd_paged_cache* cache, void* k_out, void* v_out, const int64_t k_strides[2],
+                            const int64_t v_strides[2], int64_t total, const int32_t* cu_seqlens, int n_seqs,
+                            void* stream);
+
+/*
+ * Causal grouped-query attention of the new tokens of every request over its paged cache, which
+ * holds their own keys and values already (fd_paged_kv_write).  New token i of n of request r sees
+ * the keys 0 .. cache_lens[r] - n + i; a row that sees no key is zeros.  fp32 softmax; probabilities
+ * are rounded to bf16 before the P V product, the denominator sums the rounded ones.
+ *
+ *   q, out  [batch, q_heads, seq_len, head_dim] bf16, strides {b, h, t, d}; query head h reads key
+ *           head h / (q_heads / kv_heads)
+ *   gate    NULL, or logically like out: out = attention * sigmoid(gate), rounded to bf16 once
+ *   cu_seqlens, n_seqs  as in fd_paged_kv_write; rows of out behind the last request are left as
+ *           they were
+ *   max_seqlen  (host) the longest request's new tokens (seq_len without cu_seqlens).  It chooses the
+ *           kernel by the rows of a key head and bounds nothing: longer requests are computed too
+ *   workspace  fd_paged_gqa_workspace_bytes(...) bytes, 16-byte aligned.  Long key ranges are split
+ *           over workgroups, whose parts a second launch joins, both on `stream`: calls that may
+ *           overlap need workspaces of their own
+ * A row's last bits depend on how the call splits its keys, which follows from all requests' lengths.
+ * Masked or absent keys never reach a row, not even as NaN or infinities.
+ */
+FD_API int fd_paged_gqa_fwd(const void* q, const fd_paged_cache* cache, const void* gate, void* out,
+                            const int64_t q_strides[4], const int64_t gate_strides[4], const int64_t out_strides[4],
+                            int batch, int q_heads, int seq_len, float scale, const int32_t* cu_seqlens, int n_seqs,
+                            int max_seqlen, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Workspace of fd_paged_gqa_fwd for these sizes, or a negative FD_ERR_* code. */
+FD_API int64_t fd_paged_gqa_workspace_bytes(int batch, int q_heads, int kv_heads, int seq_len, int head_dim,
+                                            int page_size, int max_pages, int n_seqs, int max_seqlen);
+
+#ifdef __cplusplus
+}
+#endif
+
+#endif /* FD_CACHE_H */
