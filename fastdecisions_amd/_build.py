@@ -25,7 +25,7 @@ OFFLOAD_ARCH = "gfx950"
 
 SOURCES = ["fd_abi.cpp", "add_rmsnorm.hip", "packed_conv.hip", "gqa_fwd.hip", "gated_delta.hip", "gate_transform.hip", "attn_prologue.hip", "slot_readout.hip", "gated_norm.hip", "hbm_copy.hip"]
 
-CACHE_SOURCES = ["cache_abi.cpp", "paged_kv.hip", "paged_gqa.hip"]
+CACHE_SOURCES = ["cache_abi.cpp", "paged_kv.hip", "paged_gqa.hip", "delta_step.hip", "conv_state.hip"]
 
 COMMON_FLAGS = [
     "-O3",

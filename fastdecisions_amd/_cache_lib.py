@@ -38,6 +38,8 @@ SIGNATURES = {
     "fd_paged_kv_read": (_i, [_cache, _p, _p, _i64s, _i64s, _i64, _p, _i, _p]),
     "fd_paged_gqa_fwd": (_i, [_p, _cache, _p, _p, _i64s, _i64s, _i64s, _i, _i, _i, _f, _p, _i, _i, _p, _i64, _p]),
     "fd_paged_gqa_workspace_bytes": (_i64, [_i] * 9),
+    "fd_gated_delta_step": (_i, [_p] * 8 + [_i, _p] + [_i] * 6 + [_f, _i, _i, _p, _i, _p]),
+    "fd_packed_conv_state": (_i, [_p, _i64, _p, _p, _p, _p, _i, _p, _p, _p, _p] + [_i] * 5 + [_p, _i, _i, _p]),
 }
 
 _LIB = None
@@ -65,6 +67,29 @@ def check(name: str, code: int) -> None:
         raise _lib.KernelError(name, code, lib().fd_cache_last_error().decode(errors="replace"))
 
 
-def strides(t: torch.Tensor, n: int) -> ctypes.Array:
-    """The first n strides of t in elements."""
-    return (_i64 * n)(*t.stride()[:n])
+def check_states(state, state_out, state_indices, requests: int, shape: tuple, dtype, device) -> tuple[int, int | None]:
+    """Validate a state pool ``[n, *shape]``, where it is written and the rows requests own in it;
+    returns (rows of the pool, pointer of the indices)."""
+    for name, t in (("state", state), ("state_out", state_out)):
+        if t is not None and (t.ndim != len(shape) + 1 or t.shape[1:] != shape or t.dtype != dtype
+                              or t.device != device or not t.is_contiguous() or t.data_ptr() % 16):
+            raise ValueError(f"{name} must be a contiguous, 16-byte aligned {dtype} tensor [n, "
+                             f"{', '.join(map(str, shape))}] on the inputs' device")
+    if state is not None and state_out is not None:
+        if state.shape != state_out.shape:
+            raise ValueError("state and state_out must have one shape")
+        a, b, size = state.data_ptr(), state_out.data_ptr(), state.numel() * state.element_size()
+        if a != b and abs(a - b) < size:
+            raise ValueError("state and state_out must be the same memory or not overlap")
+    pool = state if state is not None else state_out
+    n_pool = 0 if pool is None else pool.shape[0]
+    if state_indices is None:
+        if pool is not None and n_pool != requests:
+            raise ValueError(f"Without state_indices the state has one row for each of the {requests} requests")
+        return n_pool, None
+    if pool is None or n_pool < 1:
+        raise ValueError("state_indices need a state")
+    if (state_indices.shape != (requests,) or state_indices.dtype != torch.int32 or state_indices.device != device
+            or not state_indices.is_contiguous()):
+        raise ValueError(f"state_indices must be a contiguous int32 vector [{requests}] on the inputs' device")
+    return n_pool, state_indices.data_ptr()

@@ -22,12 +22,15 @@ Differences a caller can see:
   (``fd_gated_delta_norm_fwd``: the delta rule's rows pass through the
   workspace): the result equals ``gated_rms_norm`` of the plain output, bit
   for bit; z is a ``[B, T, Hv, Dv]`` bf16 view.
+
+``recurrent_gated_delta_rule`` is the rule token by token from and into kept
+states (``fd_gated_delta_step``), for requests that grow by a few tokens.
 """
 from __future__ import annotations
 
 import torch
 
-from . import _lib
+from . import _cache_lib, _lib
 
 
 def workspace_bytes(batch: int, seq_len: int, v_heads: int, n_seqs: int = 0) -> int:
@@ -38,22 +41,9 @@ def workspace_bytes(batch: int, seq_len: int, v_heads: int, n_seqs: int = 0) -> 
     return int(n)
 
 
-def chunk_gated_delta_rule(
-    query: torch.Tensor,
-    key: torch.Tensor,
-    value: torch.Tensor,
-    g: torch.Tensor,
-    beta: torch.Tensor,
-    chunk_size: int = 64,
-    initial_state: torch.Tensor | None = None,
-    output_final_state: bool = False,
-    use_qk_l2norm_in_kernel: bool = False,
-    *,
-    scale: float | None = None,
-    cu_seqlens: torch.Tensor | None = None,
-    norm: tuple | None = None,
-    **kwargs,
-):
+def _check_rows(query, key, value, g, beta, cu_seqlens):
+    """What both forms of the rule ask of their inputs; returns
+    (B, T, Hk, Hv, Dk, Dv, cu_seqlens pointer, n_seqs, states)."""
     if not value.is_cuda:
         raise ValueError("value must be on CUDA")
     if query.ndim != 4 or key.ndim != 4 or value.ndim != 4:
@@ -64,8 +54,6 @@ def chunk_gated_delta_rule(
         raise ValueError("query and key must match, and value must share their [B, T]")
     if Dk != 128 or Dv != 128:
         raise ValueError("head dims must be 128")
-    if chunk_size != 64:
-        raise ValueError("chunk_size must be 64")
     if Hv % Hk:
         raise ValueError(f"value heads ({Hv}) must be a multiple of key heads ({Hk})")
     for name, t in (("query", query), ("key", key), ("value", value)):
@@ -91,6 +79,28 @@ def chunk_gated_delta_rule(
         n_seqs = cu_seqlens.numel() - 1
         cu_ptr = cu_seqlens.data_ptr()
         n_states = n_seqs
+    return B, T, Hk, Hv, Dk, Dv, cu_ptr, n_seqs, n_states
+
+
+def chunk_gated_delta_rule(
+    query: torch.Tensor,
+    key: torch.Tensor,
+    value: torch.Tensor,
+    g: torch.Tensor,
+    beta: torch.Tensor,
+    chunk_size: int = 64,
+    initial_state: torch.Tensor | None = None,
+    output_final_state: bool = False,
+    use_qk_l2norm_in_kernel: bool = False,
+    *,
+    scale: float | None = None,
+    cu_seqlens: torch.Tensor | None = None,
+    norm: tuple | None = None,
+    **kwargs,
+):
+    B, T, Hk, Hv, Dk, Dv, cu_ptr, n_seqs, n_states = _check_rows(query, key, value, g, beta, cu_seqlens)
+    if chunk_size != 64:
+        raise ValueError("chunk_size must be 64")
     state_shape = (n_states, Hv, Dk, Dv)
     if initial_state is not None:
         if initial_state.shape != state_shape or initial_state.device != value.device:
@@ -121,6 +131,60 @@ def chunk_gated_delta_rule(
                 query.data_ptr(), key.data_ptr(), value.data_ptr(), g.data_ptr(), beta.data_ptr(), *norm_args,
                 float(norm_eps), out.data_ptr(), *tail))
     return out, final
+
+
+def recurrent_gated_delta_rule(
+    query: torch.Tensor,
+    key: torch.Tensor,
+    value: torch.Tensor,
+    g: torch.Tensor,
+    beta: torch.Tensor,
+    initial_state: torch.Tensor | None = None,
+    output_final_state: bool = False,
+    use_qk_l2norm_in_kernel: bool = False,
+    *,
+    scale: float | None = None,
+    cu_seqlens: torch.Tensor | None = None,
+    state_indices: torch.Tensor | None = None,
+    state_out: torch.Tensor | None = None,
+):
+    """The rule token by token (``fd_gated_delta_step``), as transformers'
+    ``torch_recurrent_gated_delta_rule`` with the same arguments: the form for the few new
+    tokens of requests whose states are kept.  Inputs as ``chunk_gated_delta_rule``'s;
+    returns ``(out, final state or None)``.
+
+    * ``cu_seqlens`` packs requests of unequal length (B == 1), each from its own state;
+    * ``state_out`` receives the final states (it may be ``initial_state`` itself);
+    * ``state_indices`` (int32 ``[requests]``): ``initial_state`` is a pool of fp32 states of
+      which request r owns row ``state_indices[r]``; the final states are written to
+      ``state_out``, by default the pool itself, which is returned.  An index that is no row of
+      the pool, or that an earlier request of the call names already, is no state: its request
+      starts from zeros and keeps nothing;
+    * q and k are normalised in fp32 (``chunk_gated_delta_rule`` rounds them to bf16 after it,
+      as transformers does on bf16 tensors), and nothing is rounded before the output."""
+    B, T, Hk, Hv, Dk, Dv, cu_ptr, n_seqs, n_states = _check_rows(query, key, value, g, beta, cu_seqlens)
+    if initial_state is not None and state_indices is None:
+        if initial_state.shape != (n_states, Hv, Dk, Dv) or initial_state.device != value.device:
+            raise ValueError(f"initial_state must be {[n_states, Hv, Dk, Dv]} on value's device")
+        if state_out is not initial_state:
+            initial_state = initial_state.to(torch.float32).contiguous()
+    if scale is None:
+        scale = 1.0 / Dk ** 0.5
+    with _lib.on_device(value.device):
+        if state_out is None:
+            if state_indices is not None:
+                state_out = initial_state
+            elif output_final_state:
+                state_out = torch.empty((n_states, Hv, Dk, Dv), device=value.device, dtype=torch.float32)
+        n_pool, indices = _cache_lib.check_states(initial_state, state_out, state_indices, n_states, (Hv, Dk, Dv),
+                                                  torch.float32, value.device)
+        out = torch.empty((B, T, Hv, Dv), device=value.device, dtype=torch.bfloat16)
+        beta_dtype = _lib.FD_DTYPE_F32 if beta.dtype == torch.float32 else _lib.FD_DTYPE_BF16
+        _cache_lib.check("fd_gated_delta_step", _cache_lib.lib().fd_gated_delta_step(
+            query.data_ptr(), key.data_ptr(), value.data_ptr(), g.data_ptr(), beta.data_ptr(), out.data_ptr(),
+            _lib.ptr(initial_state), _lib.ptr(state_out), n_pool, indices, B, T, Hk, Hv, Dk, Dv, float(scale),
+            beta_dtype, int(bool(use_qk_l2norm_in_kernel)), cu_ptr, n_seqs, _lib.stream_handle(value.device)))
+    return out, state_out
 
 
 _NORM_W_DTYPES = {torch.bfloat16: _lib.FD_DTYPE_BF16, torch.float32: _lib.FD_DTYPE_F32}

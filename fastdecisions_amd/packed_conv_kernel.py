@@ -13,12 +13,15 @@ Keyword extensions (defaults reproduce the reference exactly): ``bias``,
 splits, ``activation`` (``"silu"`` or ``None``) and ``cu_seqlens`` for packed
 variable-length batches (B == 1), where the causal window restarts at every
 request start so no request reads another's tokens.
+
+``prep_qkv_state`` continues requests from the conv state of their earlier
+tokens (``fd_packed_conv_state``).
 """
 from __future__ import annotations
 
 import torch
 
-from . import _lib
+from . import _cache_lib, _lib
 
 _ACTIVATIONS = {"silu": _lib.FD_ACT_SILU, None: _lib.FD_ACT_NONE}
 
@@ -153,3 +156,42 @@ def prep_qkv_gates(
             _PARAM_DTYPES[dt_bias.dtype], decay.data_ptr(), beta.data_ptr(), H,
             _lib.stream_handle(input_qkv.device)))
     return q, k, v, decay, beta
+
+
+def prep_qkv_state(
+    input_qkv: torch.Tensor,
+    weight: torch.Tensor,
+    conv_state: torch.Tensor,
+    bias: torch.Tensor | None = None,
+    *,
+    key_dim: int | None = None,
+    value_dim: int | None = None,
+    head_k_dim: int = 128,
+    head_v_dim: int = 128,
+    activation: str | None = "silu",
+    cu_seqlens: torch.Tensor | None = None,
+    state_indices: torch.Tensor | None = None,
+    state_out: torch.Tensor | None = None,
+):
+    """``prep_qkv`` of requests that continue: the taps before a request's first new token read
+    its ``conv_state`` ``[n, W - 1, C]`` (bf16, the last W - 1 inputs, oldest first), which then
+    holds its last W - 1 inputs.  A request fed in pieces from zeros gets the bits of the request
+    in one piece.  The state is updated in place, or written to ``state_out``; ``state_indices``
+    (int32 ``[requests]``) says which row of it a request owns, as in
+    ``recurrent_gated_delta_rule``.  W is 2 to 4; other arguments, results and errors as
+    ``prep_qkv``."""
+    B, T, key_dim, value_dim, row_stride, width, cu_ptr, n_seqs = _check_conv(
+        input_qkv, weight, bias, key_dim, value_dim, head_k_dim, head_v_dim, activation, cu_seqlens)
+    if width < 2:
+        raise ValueError("A conv of one tap has no state")
+    if state_out is None:
+        state_out = conv_state
+    n_pool, indices = _cache_lib.check_states(conv_state, state_out, state_indices, n_seqs or B,
+                                              (width - 1, input_qkv.shape[2]), torch.bfloat16, input_qkv.device)
+    with _lib.on_device(input_qkv.device):
+        q, k, v = _alloc_qkv(input_qkv, B, T, key_dim, value_dim, head_k_dim, head_v_dim)
+        _cache_lib.check("fd_packed_conv_state", _cache_lib.lib().fd_packed_conv_state(
+            input_qkv.data_ptr(), row_stride, weight.data_ptr(), _lib.ptr(bias), conv_state.data_ptr(),
+            state_out.data_ptr(), n_pool, indices, q.data_ptr(), k.data_ptr(), v.data_ptr(), B, T, key_dim, value_dim,
+            width, cu_ptr, n_seqs, _ACTIVATIONS[activation], _lib.stream_handle(input_qkv.device)))
+    return q, k, v

@@ -128,6 +128,50 @@ FD_API int fd_paged_gqa_fwd(const void* q, const fd_paged_cache* cache, const vo
 FD_API int64_t fd_paged_gqa_workspace_bytes(int batch, int q_heads, int kv_heads, int seq_len, int head_dim,
                                             int page_size, int max_pages, int n_seqs, int max_seqlen);
 
+/*
+ * The gated delta rule of the Gated-DeltaNet layers token by token (transformers'
+ * torch_recurrent_gated_delta_rule), for the few new tokens of requests whose state is kept.
+ * fd_gated_delta_fwd is the form for whole prompts and long pieces.
+ *
+ *   q, k  [batch, seq_len, k_heads, 128], v, out [batch, seq_len, v_heads, 128] bf16 contiguous
+ *   g     [batch, seq_len, v_heads] fp32; beta likewise, of beta_dtype (FD_DTYPE_BF16 or FD_DTYPE_F32)
+ *   state, state_out  [n_pool, v_heads, 128, 128] fp32 contiguous (key dimension first), or NULL (state:
+ *         zeros, state_out: not kept).  They may be the same memory; otherwise they do not overlap
+ *   state_indices  device int32[requests]: request r's state is row state_indices[r] of both; NULL:
+ *         row r.  An index outside [0, n_pool), or one that an earlier request of the call names
+ *         already, is no state: that request starts from zeros and keeps nothing
+ * Requests: batch rows, or with cu_seqlens (batch 1) [cu_seqlens[r], cu_seqlens[r + 1]); a request
+ * without new tokens hands its state on, rows of out behind the last request are left as they were.
+ * With l2norm_qk q and k rows are divided by sqrt(sum of squares + 1e-6).  All arithmetic in fp32
+ * without intermediate rounding (fd_gated_delta_fwd rounds the normalised q and k to bf16, as
+ * transformers' l2norm does on bf16 tensors); out is rounded once.
+ *
+ * Limits: head dims 128; v_heads % k_heads == 0; 16-byte aligned pointers.
+ */
+FD_API int fd_gated_delta_step(const void* q, const void* k, const void* v, const float* g, const void* beta,
+                               void* out, const float* state, float* state_out, int n_pool,
+                               const int32_t* state_indices, int batch, int seq_len, int k_heads, int v_heads,
+                               int head_k_dim, int head_v_dim, float scale, int beta_dtype, int l2norm_qk,
+                               const int32_t* cu_seqlens, int n_seqs, void* stream);
+
+/*
+ * fd_packed_conv_strided_fwd continued from a state: the taps before a request's first new token
+ * read its state, the last width - 1 inputs before it (oldest first), and state_out receives the
+ * last width - 1 inputs after its new tokens.  Values as fd_packed_conv_fwd: a request fed in
+ * pieces from a zero state gets the bits of the request in one piece.
+ *
+ *   state, state_out  [n_pool, width - 1, C] bf16 contiguous, C = 2 * key_dim + value_dim; the same
+ *         memory, or without overlap
+ *   state_indices, requests, rows behind the last request  as in fd_gated_delta_step
+ *
+ * Limits: width in [2, 4]; key_dim and value_dim multiples of 8; 16-byte aligned pointers;
+ * x_row_stride a multiple of 8, at least C.
+ */
+FD_API int fd_packed_conv_state(const void* x, int64_t x_row_stride, const void* weight, const void* bias,
+                                const void* state, void* state_out, int n_pool, const int32_t* state_indices,
+                                void* q, void* k, void* v, int batch, int seq_len, int key_dim, int value_dim,
+                                int width, const int32_t* cu_seqlens, int n_seqs, int activation, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

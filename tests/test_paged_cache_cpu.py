@@ -127,3 +127,52 @@ def test_tensors_that_do_not_fit_are_refused():
         paged_gqa_attention(x, k, k, table, lens, scale=-1.0)
     with pytest.raises(ValueError, match="cu_seqlens requires batch size 1"):
         paged_gqa_attention(x.expand(2, -1, -1, -1), k, k, table, lens, cu_seqlens=torch.zeros(3, dtype=torch.int32))
+
+
+def test_state_operators_refuse_bad_arguments():
+    lib = _cache_lib.lib()
+    inv, align, uns = _lib.FD_ERR_INVALID_ARGUMENT, _lib.FD_ERR_ALIGNMENT, _lib.FD_ERR_UNSUPPORTED
+
+    def step(**kw):
+        a = dict(q=FAKE, out=FAKE, s=FAKE, so=FAKE, pool=2, idx=None, B=2, T=1, hk=2, hv=4, dk=128, dv=128, bd=0, cu=None,
+                 n=0) | kw
+        return lib.fd_gated_delta_step(a["q"], FAKE, FAKE, FAKE, FAKE, a["out"], a["s"], a["so"], a["pool"], a["idx"],
+                                       a["B"], a["T"], a["hk"], a["hv"], a["dk"], a["dv"], 0.1, a["bd"], 1, a["cu"], a["n"],
+                                       None)
+    assert step(q=None) == inv and step(hv=3) == inv and step(dk=64) == uns and step(bd=2) == inv
+    assert step(pool=1) == inv and step(pool=0, idx=FAKE) == inv and step(so=FAKE + 4) == align
+    assert step(cu=FAKE) == inv and step(n=2) == inv and step(cu=FAKE, n=2, B=2) == inv
+    assert step(B=1 << 16, T=1 << 15, pool=1 << 16) == uns and step(B=0) == _lib.FD_OK
+
+    def conv(**kw):
+        a = dict(x=FAKE, row=384, s=FAKE, so=FAKE, pool=2, idx=None, B=2, T=1, kd=128, vd=128, W=4, cu=None, n=0, act=1) | kw
+        return lib.fd_packed_conv_state(a["x"], a["row"], FAKE, None, a["s"], a["so"], a["pool"], a["idx"], FAKE, FAKE, FAKE,
+                                        a["B"], a["T"], a["kd"], a["vd"], a["W"], a["cu"], a["n"], a["act"], None)
+    assert conv(x=None) == inv and conv(s=None) == inv and conv(kd=12) == inv and conv(W=1) == uns and conv(W=5) == uns
+    assert conv(row=380) == align and conv(row=376) == align and conv(x=FAKE + 2) == align and conv(act=3) == inv
+    assert conv(pool=1) == inv and conv(cu=FAKE) == inv and conv(n=1) == inv and conv(B=0) == _lib.FD_OK
+
+
+def test_states_that_do_not_fit_are_refused():
+    check = lambda *a: _cache_lib.check_states(*a, (2, 4), torch.float32, torch.device("cpu"))
+    s, idx = torch.zeros((3, 2, 4)), torch.zeros(2, dtype=torch.int32)
+    assert check(s, s, None, 3) == (3, None) and check(s, None, idx, 2)[0] == 3 and check(None, None, None, 5) == (0, None)
+    for bad in ((s, s, None, 2), (s[:, :1], None, None, 3), (s.double(), None, None, 3), (s, s[:2], None, 3),
+                (s.transpose(1, 2).contiguous().transpose(1, 2), None, None, 3), (None, None, idx, 2),
+                (s, None, idx.long(), 2), (s, None, idx, 3)):
+        with pytest.raises(ValueError):
+            check(*bad)
+    big = torch.zeros((6, 2, 4))
+    with pytest.raises(ValueError, match="overlap"):
+        check(big[:4], big[2:], None, 4)
+
+
+def test_tensors_of_the_host_are_refused():
+    from fastdecisions_amd.gated_delta_kernel import recurrent_gated_delta_rule
+    from fastdecisions_amd.packed_conv_kernel import prep_qkv_state
+    x = torch.zeros((1, 1, 2, 128), dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="must be on CUDA"):
+        recurrent_gated_delta_rule(x, x, x, torch.zeros((1, 1, 2)), torch.zeros((1, 1, 2)))
+    with pytest.raises(ValueError, match="must be on CUDA"):
+        prep_qkv_state(torch.zeros((1, 1, 384), dtype=torch.bfloat16), torch.zeros((384, 4), dtype=torch.bfloat16),
+                       torch.zeros((1, 3, 384), dtype=torch.bfloat16))
