@@ -6,8 +6,8 @@
 // keys up to its token's position.  An item of work is one tile of rows of one
 // (request, KV head) against one range of its keys:
 //
-//   few rows   32 rows, 4 wavefronts that each take every fourth block of 32
-//              keys into LDS of their own: no barrier in the loop, the cache
+//   few rows   16 or 32 rows, 4 wavefronts that each take every fourth block of
+//              32 keys into LDS of their own: no barrier in the loop, the cache
 //              streams through at the rate of the memory.  Single tokens.
 //   pieces     128 rows, wavefronts share the staged key tiles.  Long suffixes.
 //
@@ -19,11 +19,10 @@
 // split row tile leave (o, max, denominator) in the workspace and
 // paged_gqa_join_kernel joins them.
 //
-// The tile mathematics are those of the uncached kernel (gqa_tile.h): scores
-// transposed (S^T = K Q^T) on v_mfma_f32_32x32x16_bf16, so a lane owns one row's
-// scores; P feeds P V from registers; V^T comes from transposing LDS reads.
-// E4M3 rows are turned into bf16 (code times power-of-two scale: exact) on their
-// way into LDS, so both cache types share everything behind the staging.
+// In both, scores are computed transposed (S^T = K Q^T on MFMA), with the K rows
+// permuted so that a lane's scores are those of the 8 consecutive keys whose
+// probabilities it must supply to P V: P never leaves registers, and V^T comes
+// from transposing LDS reads.
 #include <type_traits>
 
 #include "gqa_tile.h"
@@ -33,20 +32,43 @@ namespace {
 
 constexpr int kNumXcd = 8;
 
-// RB row blocks of 32 rows and KS key parts of a tile per workgroup, NB 32-key
-// blocks per wavefront and tile.
+// Few rows: NR blocks of 16 rows; every wavefront stages blocks of 32 keys of its own.
+template <int D_, bool FP8_, int NR_>
+struct Few {
+  static constexpr int D = D_, NR = NR_;
+  static constexpr bool FP8 = FP8_;
+  static constexpr int kWaves = 4;
+  static constexpr int kThreads = 64 * kWaves;
+  static constexpr int kRows = 16 * NR;
+  static constexpr int kKeys = 32 * kWaves;             // keys of a tile: a block of each wavefront
+  static constexpr int kRowBytes = FP8 ? D : 2 * D;     // of a cached row, staged as it is
+  static constexpr int kBlockBytes = 32 * kRowBytes;    // K or V of a block
+  static constexpr int kScaleBytes = FP8 ? 256 : 0;     // 32 K scales and 32 V scales, a word each
+  static constexpr int kStageBytes = 2 * kBlockBytes + kScaleBytes;
+  static constexpr int kStages = kBlockBytes >= 8192 ? 1 : 8192 / kBlockBytes;
+  static constexpr int kCopies = kBlockBytes / 1024;    // copy instructions of a block's K (or V)
+  static constexpr int kCopyRows = 1024 / kRowBytes;
+  static constexpr int kKGroup = kCopies + (FP8 ? 1 : 0);  // with the scales
+  static constexpr int kRowFloats = D + 4;
+  static constexpr int kEpilogueBytes = kWaves * kRows * (kRowFloats + 2) * 4;
+  static constexpr int kLoopBytes = kWaves * kStages * kStageBytes;
+  static constexpr int kSmemBytes = kLoopBytes > kEpilogueBytes ? kLoopBytes : kEpilogueBytes;
+  static constexpr int kPerCu = kSmemBytes > 80 * 1024 ? 1 : 2;  // workgroups that a CU's LDS holds
+};
+
+// Pieces: RB row blocks of 32 rows and KS key parts of a tile per workgroup, NB 32-key blocks per
+// wavefront and tile.
 template <int D_, bool FP8_, int RB_, int KS_, int NB_>
 struct Shape {
   static constexpr int D = D_, RB = RB_, KS = KS_, NB = NB_;
   static constexpr bool FP8 = FP8_;
-  static constexpr bool kPrivate = RB == 1;             // wavefronts stage their own keys
   static constexpr int kWaves = RB * KS;
   static constexpr int kThreads = 64 * kWaves;
   static constexpr int kRows = 32 * RB;
   static constexpr int kKeys = 32 * KS * NB;            // keys of a tile
   static constexpr int CR = D / 8;                      // 16-byte chunks of a bf16 row
   static constexpr int kTileBytes = kKeys * CR * 16;    // K or V
-  static constexpr int kStages = kPrivate ? 1 : 2;
+  static constexpr int kStages = 2;
   static constexpr int kStageBytes = 2 * kTileBytes * kStages;
   // epilogue: every key part's rows, padded, and their (max, denominator)
   static constexpr int kRowFloats = D + 4;
@@ -85,12 +107,14 @@ struct Item {
   int base, n_rtiles, n_ranges; // first item of the request; its row tiles and key ranges
 };
 
-__device__ __forceinline__ int wave_scan(int v, int lane) {  // inclusive
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int u = __shfl_up(v, d);
-    if (lane >= d) v += u;
-  }
+// Inclusive sums over the lanes, on DPP: within rows of 16 lanes, then a row's last lane into the next row(s).
+__device__ __forceinline__ int wave_scan(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);  // row_shr:1
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row_bcast:15 into rows 1 and 3
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // row_bcast:31 into rows 2 and 3
   return v;
 }
 
@@ -109,38 +133,37 @@ __device__ __forceinline__ bool find_item(const PagedArgs& a, int lane, Want wan
       *kt = (*len + KEYS - 1) / KEYS;
     }
   };
+  auto at_lane = [](int v, int l) { return __builtin_amdgcn_readlane(v, l); };
   int start, n_new, len, rt, kt;
   int64_t work = 0;
   for (int r0 = 0; r0 < a.n_req; r0 += 64) {
     sizes(r0 + lane, &start, &n_new, &len, &rt, &kt);
-    work += static_cast<int64_t>(rt) * kt;
+    const int64_t w = static_cast<int64_t>(rt) * kt;  // below 2^49: summed in two parts
+    work += at_lane(wave_scan(static_cast<int>(w & 0xffffff)), 63);
+    work += static_cast<int64_t>(at_lane(wave_scan(static_cast<int>(w >> 24)), 63)) << 24;
   }
-#pragma unroll
-  for (int d = 32; d >= 1; d >>= 1) work += __shfl_xor(work, d);
   const int64_t per = (work * a.kv_heads + a.workers - 1) / a.workers;
   const int tiles = static_cast<int>(per > a.min_tiles ? per : a.min_tiles);
-  int total = 0;
+  auto ranges_of = [&](int k) { return max((k + tiles - 1) / tiles, 1); };
+  int total = 0, at = 0;
   if (a.n_req > 64) {
     for (int r0 = 0; r0 < a.n_req; r0 += 64) {
       sizes(r0 + lane, &start, &n_new, &len, &rt, &kt);
-      int n = rt * (JOIN ? 1 : max((kt + tiles - 1) / tiles, 1)) * a.kv_heads;
-#pragma unroll
-      for (int d = 32; d >= 1; d >>= 1) n += __shfl_xor(n, d);
-      total += n;
+      total += at_lane(wave_scan(rt * (JOIN ? 1 : ranges_of(kt)) * a.kv_heads), 63);
     }
+    at = want(total);
+    if (at < 0 || at >= total) return false;
   }
-  int at = a.n_req > 64 ? want(total) : 0;
-  if (a.n_req > 64 && (at < 0 || at >= total)) return false;
   int base = 0, before = 0;  // items of the requests before r0 (all ranges), and in terms of `at`
   for (int r0 = 0; r0 < a.n_req; r0 += 64) {
-    sizes(r0 + lane, &start, &n_new, &len, &rt, &kt);
-    const int ranges = max((kt + tiles - 1) / tiles, 1);
+    if (a.n_req > 64) sizes(r0 + lane, &start, &n_new, &len, &rt, &kt);
+    const int ranges = ranges_of(kt);
     const int all = rt * ranges * a.kv_heads;
     const int mine = JOIN ? rt * a.kv_heads : all;
-    const int incl = wave_scan(mine, lane);
-    const int incl_all = JOIN ? wave_scan(all, lane) : incl;
+    const int incl = wave_scan(mine);
+    const int incl_all = JOIN ? wave_scan(all) : incl;
     if (a.n_req <= 64) {
-      total = __shfl(incl, 63);
+      total = at_lane(incl, 63);
       at = want(total);
       if (at < 0 || at >= total) return false;
     }
@@ -148,14 +171,13 @@ __device__ __forceinline__ bool find_item(const PagedArgs& a, int lane, Want wan
     if (past != 0) {
       const int l = __builtin_ctzll(past);
       it->req = r0 + l;
-      const int r_all = __shfl(all, l);
-      const int k = at - (before + __shfl(incl, l) - __shfl(mine, l));  // within the request
-      it->base = base + __shfl(incl_all, l) - r_all;
-      it->n_rtiles = __shfl(rt, l);
-      it->n_ranges = __shfl(ranges, l);
-      it->start = __shfl(start, l);
-      it->n_new = __shfl(n_new, l);
-      it->len = __shfl(len, l);
+      const int k = at - (before + at_lane(incl, l) - at_lane(mine, l));  // within the request
+      it->base = base + at_lane(incl_all, l) - at_lane(all, l);
+      it->n_rtiles = at_lane(rt, l);
+      it->n_ranges = at_lane(ranges, l);
+      it->start = at_lane(start, l);
+      it->n_new = at_lane(n_new, l);
+      it->len = at_lane(len, l);
       it->tiles = tiles;
       it->rtile = k % it->n_rtiles;  // row tiles of a key range one after the other: they share its keys
       const int hr = k / it->n_rtiles;
@@ -165,8 +187,8 @@ __device__ __forceinline__ bool find_item(const PagedArgs& a, int lane, Want wan
       it->rows = it->n_new * a.group;
       return true;
     }
-    before += __shfl(incl, 63);
-    base += __shfl(incl_all, 63);
+    before += at_lane(incl, 63);
+    base += at_lane(incl_all, 63);
   }
   return false;
 }
@@ -215,6 +237,430 @@ __device__ __forceinline__ void wait_copies() {
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
 
+// Block b's item and the keys its rows see; false if there is none or none of its range's keys is seen.
+struct Job {
+  Item it;
+  int kend, t0, nt, slot;  // keys seen; first tile, tiles, and place of the item
+  bool split;
+};
+template <class S>
+__device__ __forceinline__ bool open_job(const PagedArgs& a, int lane, Job* j) {
+  Item it;
+  // XCD x takes one contiguous run of the items: row tiles that share keys meet in one L2
+  const int b = blockIdx.x;
+  auto want = [&](int total) {
+    const int per = (total + kNumXcd - 1) / kNumXcd;
+    const int i = b / kNumXcd;
+    return i < per ? (b % kNumXcd) * per + i : -1;
+  };
+  if (!find_item<S::kRows, S::kKeys, false>(a, lane, want, &it)) return false;
+  it.req = uniform(it.req), it.head = uniform(it.head), it.rtile = uniform(it.rtile), it.range = uniform(it.range);
+  it.row0 = uniform(it.row0), it.rows = uniform(it.rows), it.start = uniform(it.start), it.n_new = uniform(it.n_new);
+  it.len = uniform(it.len), it.tiles = uniform(it.tiles), it.base = uniform(it.base);
+  it.n_rtiles = uniform(it.n_rtiles), it.n_ranges = uniform(it.n_ranges);
+  j->it = it;
+  j->kend = uniform(keys_of_tile<S::kRows>(a, it));
+  const int nt_all = (j->kend + S::kKeys - 1) / S::kKeys;
+  j->t0 = it.range * it.tiles;
+  if (it.range > 0 && j->t0 >= nt_all) return false;
+  j->nt = min(it.tiles, nt_all - j->t0);  // 0 where no key is visible at all
+  j->split = nt_all > it.tiles;
+  // where a part goes; the workspace has a place for every item of a well-formed offset table
+  j->slot = it.base + (it.head * it.n_ranges + it.range) * it.n_rtiles + it.rtile;
+  return j->slot >= 0 && j->slot < a.max_items;
+}
+
+// Is any key of the job's tiles on no page?
+template <class S>
+__device__ __forceinline__ bool any_absent(const PagedArgs& a, const Job& j, const int32_t* table, int lane) {
+  if (j.nt <= 0) return false;
+  const int first = (j.t0 * S::kKeys) >> a.c.shift;
+  const int last = (min((j.t0 + j.nt) * S::kKeys, j.kend) - 1) >> a.c.shift;
+  bool bad = false;
+  for (int i = first + lane; i <= last; i += 64)
+    bad |= static_cast<unsigned>(table[i]) >= static_cast<unsigned>(a.c.n_pages);
+  return __builtin_amdgcn_ballot_w64(bad) != 0;
+}
+
+// The key parts' rows in LDS (S::kRowFloats apart) and their (max, denominator), joined row by row: stored, or
+// left as the item's part.
+template <class S, int PARTS>
+__device__ __forceinline__ void close_job(const PagedArgs& a, const Job& j, const float* rowsf, const float* ml) {
+  constexpr int D = S::D;
+  const int rows = min(S::kRows, j.it.rows - j.it.row0);
+  float* const part = a.part + j.slot * part_floats<S::kRows>(D);
+  for (int i = threadIdx.x; i < rows * (D / 4); i += S::kThreads) {
+    const int row = i / (D / 4), d = (i % (D / 4)) * 4;
+    float m = ml[row * 2];
+#pragma unroll
+    for (int s = 1; s < PARTS; ++s) m = fmaxf(m, ml[(s * S::kRows + row) * 2]);
+    const float m_sub = m == -__builtin_inff() ? 0.0f : m;
+    f32x4_t acc = {0.0f, 0.0f, 0.0f, 0.0f};
+    float l = 0.0f;
+#pragma unroll
+    for (int s = 0; s < PARTS; ++s) {
+      const int at = s * S::kRows + row;
+      const float w = __builtin_amdgcn_exp2f(ml[at * 2] - m_sub);
+      l += ml[at * 2 + 1] * w;
+      acc += *reinterpret_cast<const f32x4_t*>(rowsf + at * S::kRowFloats + d) * w;
+    }
+    if (!j.split) {
+      store4(a, j.it, row, d, acc, l == 0.0f ? 0.0f : 1.0f / l);
+    } else {
+      *reinterpret_cast<f32x4_t*>(part + row * D + d) = acc;
+      if (d == 0) {
+        part[S::kRows * D + row * 2] = m;
+        part[S::kRows * D + row * 2 + 1] = l;
+      }
+    }
+  }
+}
+
+// ---------------------------------------------------------------- few rows
+
+// Key (within a 32-key block) that row m of the block's score MFMA a supplies: lane group g then
+// holds the scores of keys 8 g .. 8 g + 7, those whose P it supplies as the B operand of P V.
+__device__ __forceinline__ int sigma16(int a, int m) { return 8 * (m >> 2) + 4 * a + (m & 3); }
+
+// Chunk swizzles of the staged rows (physical chunk = logical chunk ^ f(row)), such that rows read
+// together lie in different banks: 16 permuted rows at one chunk for K; for V the 4 (bf16, chunk
+// pairs) or 8 (codes) rows of a transposing read and the next lane group's.
+template <int ROW_BYTES>
+constexpr int kRowShift = ROW_BYTES >= 256 ? 0 : ROW_BYTES == 128 ? 1 : 2;
+template <int ROW_BYTES>
+__device__ __forceinline__ int few_swz_k(int row) {
+  return ((row & 3) | ((row >> 3) & 3) << 2) >> kRowShift<ROW_BYTES>;
+}
+template <int ROW_BYTES, bool FP8>
+__device__ __forceinline__ int few_swz_v(int row) {
+  if constexpr (FP8) return ((row & 7) | ((row >> 3) & 1) << 3) >> kRowShift<ROW_BYTES>;
+  else return 2 * (((row & 3) | ((row >> 3) & 1) << 2) >> kRowShift<ROW_BYTES>);
+}
+
+// Eight codes as bf16, scale 1 (exact).
+__device__ __forceinline__ bf16x8_t codes_to_bf16(uint32_t lo, uint32_t hi) {
+  typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+  const bf16x2_t a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, false);
+  const bf16x2_t b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, true);
+  const bf16x2_t c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, false);
+  const bf16x2_t d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, true);
+  return bf16x8_t{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+
+// Half-word i (uniform) of four words.
+__device__ __forceinline__ uint32_t half_of(uint32_t a, uint32_t b, uint32_t c, uint32_t d, int i) {
+  const uint32_t w = i < 2 ? a : i < 4 ? b : i < 6 ? c : d;
+  return (i & 1) ? w >> 16 : w & 0xffffu;
+}
+
+// One byte per lane, zero-extended, to a word of LDS at lds + 4 * lane.
+__device__ __forceinline__ void byte_to_lds(const uint8_t* p, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_ubyte %0, off" ::"v"(p), "s"(lds) : "memory", "m0");
+}
+
+// A block of 32 keys costs a wavefront 16 (NR) MFMAs of 16x16x32 and, at the memory's rate, several
+// times as long to arrive, so what counts is that copies are always in flight: rows go to LDS as they
+// are (codes are converted where they are read, scales multiply scores and probabilities), K and V
+// of kStages blocks each, the next K leaving as soon as a block's scores have read theirs, the next
+// V as soon as P V has.
+template <class S>
+__global__ __launch_bounds__(S::kThreads, S::kPerCu) void paged_gqa_few_kernel(PagedArgs a) {
+  constexpr int D = S::D, NR = S::NR, RBY = S::kRowBytes, kKk = D / 32, kNdb = D / 16, NS = S::kStages;
+  constexpr bool FP8 = S::FP8;
+  __shared__ __attribute__((aligned(1024))) unsigned char smem[S::kSmemBytes];
+  const int tid = threadIdx.x;
+  const int lane = tid & 63;
+  const int wave = uniform(tid >> 6);
+  const int grp = lane >> 4, li = lane & 15;
+
+  Job job;
+  if (!open_job<S>(a, lane, &job)) return;
+  const Item& it = job.it;
+  const int kend = job.kend;
+  const int32_t* const table = a.c.table + it.req * a.c.table_stride;
+
+  // ---- copies.  Block j of this wavefront: keys first + 128 j .. + 31; rows past kend repeat row kend - 1 (the
+  // mask discards them).  Its two halves of 16 keys lie on a page each.
+  const int first = job.t0 * S::kKeys + wave * 32;
+  const int mine = max(0, min(job.nt, (kend - first + S::kKeys - 1) / S::kKeys));
+  struct Pages {
+    int p[2];
+  };
+  auto pages_of = [&](int j) {
+    Pages x;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int key = uniform(max(min(first + j * S::kKeys + 16 * h, kend - 1), 0));
+      const int page = scalar_load(table, key >> a.c.shift);
+      x.p[h] = static_cast<unsigned>(page) < static_cast<unsigned>(a.c.n_pages) ? page : 0;
+    }
+    return x;
+  };
+  const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_void_t*)smem)) +
+                        static_cast<uint32_t>(wave * NS * S::kStageBytes);
+  const unsigned char* const stage0 = smem + wave * NS * S::kStageBytes;
+  const int page_mask = (1 << a.c.shift) - 1;
+  constexpr int kChunks = RBY / 16;
+  auto copy_side = [&](const PagedSide& c, const Pages& pg, int j, uint32_t lds, bool is_v) {
+    const int kb0 = first + j * S::kKeys;
+#pragma unroll
+    for (int i = 0; i < S::kCopies; ++i) {
+      const int row = i * S::kCopyRows + lane / kChunks;
+      const int page = pg.p[i * S::kCopyRows / 16];
+      const unsigned char* base = c.base + page * c.page + it.head * c.head;
+      const int chunk = (lane % kChunks) ^ (is_v ? few_swz_v<RBY, FP8>(row) : few_swz_k<RBY>(row));
+      const int key = min(kb0 + row, kend - 1) & page_mask;
+      copy_to_lds(base, static_cast<uint32_t>(key * static_cast<int>(c.row) + chunk * 16), lds + static_cast<uint32_t>(i * 1024));
+    }
+  };
+  auto copy_k = [&](const Pages& pg, int j) {
+    const uint32_t lds = lds0 + static_cast<uint32_t>((j & (NS - 1)) * S::kStageBytes);
+    copy_side(a.c.k, pg, j, lds, false);
+    if constexpr (FP8) {
+      const int row = lane & 31;
+      const int key = min(first + j * S::kKeys + row, kend - 1) & page_mask;
+      const int page = row < 16 ? pg.p[0] : pg.p[1];
+      const PagedSide& c = lane < 32 ? a.c.k : a.c.v;
+      byte_to_lds(c.scale + page * c.s_page + it.head * c.s_head + key, lds + 2 * S::kBlockBytes);
+    }
+  };
+  auto copy_v = [&](const Pages& pg, int j) {
+    copy_side(a.c.v, pg, j, lds0 + static_cast<uint32_t>((j & (NS - 1)) * S::kStageBytes + S::kBlockBytes), true);
+  };
+
+  // ---- this lane's rows (li of each block of 16)
+  int pos[NR];
+  bf16x8_t qf[NR][kKk];
+#pragma unroll
+  for (int n = 0; n < NR; ++n) {
+    const int p = min(it.row0 + n * 16 + li, it.rows - 1);  // rows behind the last one repeat it and are not stored
+    const int token = p / a.group;
+    pos[n] = it.len - it.n_new + token;
+    const int b = a.cu == nullptr ? it.req : 0;
+    const int head = it.head * a.group + (p - token * a.group);
+    const uint16_t* qp = a.q + b * a.qs[0] + head * a.qs[1] + static_cast<int64_t>(it.start + token) * a.qs[2] + grp * 8;
+#pragma unroll
+    for (int kk = 0; kk < kKk; ++kk) qf[n][kk] = *reinterpret_cast<const bf16x8_t*>(qp + kk * 32);
+  }
+  const int pos_min = uniform(it.len - it.n_new + it.row0 / a.group);
+  const bool absent = any_absent<S>(a, job, table, lane);
+
+  f32x4_t o[NR][kNdb];
+  float m_run[NR], l_run[NR];
+#pragma unroll
+  for (int n = 0; n < NR; ++n) {
+    m_run[n] = -__builtin_inff();  // running maximum (log2 units), may lag the true one by 8
+    l_run[n] = 0.0f;               // this lane's part of the denominator
+#pragma unroll
+    for (int db = 0; db < kNdb; ++db) o[n][db] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+  }
+  bf16x8_t pb[NR];
+
+  auto scores = [&](int j) {
+    const unsigned char* const st = stage0 + (j & (NS - 1)) * S::kStageBytes;
+    const int kb0 = first + j * S::kKeys;
+    f32x4_t s[NR][2];
+#pragma unroll
+    for (int n = 0; n < NR; ++n) s[n][0] = s[n][1] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int row = sigma16(h, li);
+      const int swz = few_swz_k<RBY>(row);
+#pragma unroll
+      for (int kk = 0; kk < kKk; ++kk) {
+        bf16x8_t kf;
+        if constexpr (FP8) {
+          const uint2 w = *reinterpret_cast<const uint2*>(st + row * RBY + ((2 * kk + (grp >> 1)) ^ swz) * 16 + 8 * (grp & 1));
+          kf = codes_to_bf16(w.x, w.y);
+        } else {
+          kf = *reinterpret_cast<const bf16x8_t*>(st + row * RBY + ((4 * kk + grp) ^ swz) * 16);
+        }
+#pragma unroll
+        for (int n = 0; n < NR; ++n) s[n][h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[n][kk], s[n][h], 0, 0, 0);
+      }
+    }
+    float ks[8], vs[8];
+    if constexpr (FP8) {
+      const uint4* const sc = reinterpret_cast<const uint4*>(st + 2 * S::kBlockBytes);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint4 kw = sc[2 * grp + h], vw = sc[8 + 2 * grp + h];
+        const uint32_t ku[4] = {kw.x, kw.y, kw.z, kw.w}, vu[4] = {vw.x, vw.y, vw.z, vw.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          ks[4 * h + e] = scale_of(ku[e]);
+          vs[4 * h + e] = scale_of(vu[e]);
+        }
+      }
+    }
+    const bool masked = kb0 + 31 > pos_min || absent;
+    bool there = true;
+    if (absent) {
+      bool t[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int key = uniform(min(kb0 + 16 * h, kend - 1));
+        t[h] = static_cast<unsigned>(scalar_load(table, key >> a.c.shift)) < static_cast<unsigned>(a.c.n_pages);
+      }
+      there = grp < 2 ? t[0] : t[1];
+    }
+#pragma unroll
+    for (int n = 0; n < NR; ++n) {
+      float x[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        x[e] = s[n][e >> 2][e & 3];
+        if constexpr (FP8) x[e] *= ks[e];
+      }
+      if (masked) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (kb0 + 8 * grp + e > pos[n] || !there) x[e] = -__builtin_inff();
+      }
+      float mx = x[0];
+#pragma unroll
+      for (int e = 1; e < 8; ++e) mx = fmaxf(mx, x[e]);
+      mx = fd_xor_max<32>(fd_xor_max<16>(mx)) * a.scale_log2;
+      const bool grow = mx > m_run[n] + 8.0f;
+      const float m_new = grow ? mx : m_run[n];
+      const float alpha = grow ? __builtin_amdgcn_exp2f(m_run[n] - m_new) : 1.0f;
+      const float m_sub = m_new == -__builtin_inff() ? 0.0f : m_new;  // nothing seen so far: p = 0
+      m_run[n] = m_new;
+      if (__builtin_amdgcn_ballot_w64(grow) != 0) {
+#pragma unroll
+        for (int db = 0; db < kNdb; ++db) o[n][db] *= alpha;
+      }
+      f32x8_t pv;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) pv[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[e], a.scale_log2, -m_sub));
+      pb[n] = __builtin_convertvector(pv, bf16x8_t);
+      // the denominator takes the rounded p: its error then cancels where a few keys carry the row
+      f32x8_t pr = __builtin_convertvector(pb[n], f32x8_t);
+      float psum = 0.0f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) psum += pr[e];
+      l_run[n] = l_run[n] * alpha + psum;
+      if constexpr (FP8) {  // V's scales go to P: a power of two changes no rounding
+#pragma unroll
+        for (int e = 0; e < 8; ++e) pr[e] = masked && pr[e] == 0.0f ? 0.0f : pr[e] * vs[e];
+        pb[n] = __builtin_convertvector(pr, bf16x8_t);
+      }
+    }
+  };
+
+  auto p_v = [&](int j) {
+    const unsigned char* const st = stage0 + (j & (NS - 1)) * S::kStageBytes + S::kBlockBytes;
+    // a block with masked keys: their values must not reach a row as 0 * NaN or 0 * inf
+    const bool guard = first + j * S::kKeys + 31 > pos_min || absent;
+#pragma unroll
+    for (int db = 0; db < kNdb; ++db) {
+      bf16x8_t vf;  // V[key 8 grp + i][16 db + li]
+      if constexpr (FP8) {
+        typedef int v2i_t __attribute__((ext_vector_type(2)));
+        typedef __attribute__((address_space(3))) v2i_t lds_v2i_t;
+        const int row = 8 * grp + (li >> 1);
+        const v2i_t w = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+            (lds_v2i_t*)(st + row * RBY + (db ^ few_swz_v<RBY, true>(row)) * 16 + 8 * (li & 1)));
+        vf = codes_to_bf16(static_cast<uint32_t>(w[0]), static_cast<uint32_t>(w[1]));
+      } else {
+        const int row = 8 * grp + (li >> 2);
+        const unsigned char* vp = st + row * RBY + ((2 * db + ((li & 3) >> 1)) ^ few_swz_v<RBY, false>(row)) * 16 + 8 * (li & 1);
+        const v4i16_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16_t*)vp);
+        const v4i16_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16_t*)(vp + 4 * RBY));
+        const short __attribute__((ext_vector_type(8))) vv = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+        vf = __builtin_bit_cast(bf16x8_t, vv);
+      }
+      if (guard) {
+        typedef short i16x8_t __attribute__((ext_vector_type(8)));
+        i16x8_t e = __builtin_bit_cast(i16x8_t, vf);
+        bool odd = false;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) odd |= (e[i] & 0x7f80) == 0x7f80;
+        if (__builtin_amdgcn_ballot_w64(odd) != 0) {
+          // infinities and NaN leave the product and are added by hand to the rows that see them
+          typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
+          const u32x4_t ew = __builtin_bit_cast(u32x4_t, vf);
+#pragma unroll 1
+          for (int i = 0; i < 8; ++i) {
+            const uint32_t bits = half_of(ew[0], ew[1], ew[2], ew[3], i);
+            const float x = (bits & 0x7f80u) == 0x7f80u ? fd_bf16_to_f32(bits) : 0.0f;
+#pragma unroll
+            for (int n = 0; n < NR; ++n) {
+              const u32x4_t pw = __builtin_bit_cast(u32x4_t, pb[n]);
+              const float pi = fd_bf16_to_f32(half_of(pw[0], pw[1], pw[2], pw[3], i));
+#pragma unroll 1
+              for (int g = 0; g < 4; ++g) {
+                const float pg = __shfl(pi, 16 * g + li);  // this lane's row, key 8 g + i
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                  const float xd = __shfl(x, 16 * g + 4 * grp + r);  // feature of o[n][db][r]
+                  if (xd != 0.0f && pg != 0.0f) o[n][db][r] += pg * xd;
+                }
+              }
+            }
+          }
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if ((e[i] & 0x7f80) == 0x7f80) e[i] = 0;
+          vf = __builtin_bit_cast(bf16x8_t, e);
+        }
+      }
+#pragma unroll
+      for (int n = 0; n < NR; ++n) o[n][db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pb[n], o[n][db], 0, 0, 0);
+    }
+  };
+
+  // ---- the loop: copies in the queue, oldest first, at block j's scores: K(j) V(j) .. K(j + NS - 1) V(j + NS - 1)
+  constexpr int kBoth = S::kKGroup + S::kCopies;
+#pragma unroll
+  for (int j = 0; j < NS; ++j) {
+    if (j < mine) {
+      const Pages pg = pages_of(j);
+      copy_k(pg, j);
+      copy_v(pg, j);
+    }
+  }
+  Pages next = pages_of(NS);
+  for (int j = 0; j < mine; ++j) {
+    const bool more = j + NS < mine;
+    if (more || j + NS == mine) wait_copies<S::kCopies + (NS - 1) * kBoth>();  // K(j) has landed
+    else wait_copies<0>();
+    scores(j);
+    wait_lds_reads();
+    if (more) {
+      copy_k(next, j + NS);
+      wait_copies<(NS - 1) * kBoth + S::kKGroup>();  // V(j) has landed
+    } else {
+      wait_copies<0>();
+    }
+    p_v(j);
+    wait_lds_reads();
+    if (more) copy_v(next, j + NS);
+    next = pages_of(j + NS + 1);
+  }
+
+  // ---- join the wavefronts' keys
+  __syncthreads();  // the stages are free
+  float* const rowsf = reinterpret_cast<float*>(smem);
+  float* const ml = rowsf + S::kWaves * S::kRows * S::kRowFloats;
+#pragma unroll
+  for (int n = 0; n < NR; ++n) {
+    const int at = wave * S::kRows + n * 16 + li;
+#pragma unroll
+    for (int db = 0; db < kNdb; ++db)
+      *reinterpret_cast<f32x4_t*>(rowsf + at * S::kRowFloats + db * 16 + 4 * grp) = o[n][db];
+    const float l = fd_xor_sum<32>(fd_xor_sum<16>(l_run[n]));
+    if (grp == 0) {
+      ml[at * 2] = m_run[n];
+      ml[at * 2 + 1] = l;
+    }
+  }
+  __syncthreads();
+  close_job<S, S::kWaves>(a, job, rowsf, ml);
+}
+
+// ---------------------------------------------------------------- pieces
+
 template <class S>
 __global__ __launch_bounds__(S::kThreads) void paged_gqa_kernel(PagedArgs a) {
   constexpr int D = S::D, CR = S::CR, kKk = D / 16, kNdb = D / 32;
@@ -226,30 +672,10 @@ __global__ __launch_bounds__(S::kThreads) void paged_gqa_kernel(PagedArgs a) {
   const int kp = wave / S::RB;   // key part
   const int col = lane & 31, half = lane >> 5;
 
-  Item it;
-  {
-    // XCD x takes one contiguous run of the items: row tiles that share keys meet in one L2
-    const int b = blockIdx.x;
-    auto want = [&](int total) {
-      const int per = (total + kNumXcd - 1) / kNumXcd;
-      const int i = b / kNumXcd;
-      return i < per ? (b % kNumXcd) * per + i : -1;
-    };
-    if (!find_item<S::kRows, S::kKeys, false>(a, lane, want, &it)) return;
-  }
-  it.req = uniform(it.req), it.head = uniform(it.head), it.rtile = uniform(it.rtile), it.range = uniform(it.range);
-  it.row0 = uniform(it.row0), it.rows = uniform(it.rows), it.start = uniform(it.start), it.n_new = uniform(it.n_new);
-  it.len = uniform(it.len), it.tiles = uniform(it.tiles), it.base = uniform(it.base);
-  it.n_rtiles = uniform(it.n_rtiles), it.n_ranges = uniform(it.n_ranges);
-  const int kend = uniform(keys_of_tile<S::kRows>(a, it));
-  const int nt_all = (kend + S::kKeys - 1) / S::kKeys;
-  const int t0 = it.range * it.tiles;
-  if (it.range > 0 && t0 >= nt_all) return;  // nothing of this range is visible to the tile's rows
-  const int nt = min(it.tiles, nt_all - t0);  // 0 where no key is visible at all
-  const bool split = nt_all > it.tiles;
-  // where a part goes; the workspace has a place for every item of a well-formed offset table
-  const int slot = it.base + (it.head * it.n_ranges + it.range) * it.n_rtiles + it.rtile;
-  if (slot < 0 || slot >= a.max_items) return;
+  Job job;
+  if (!open_job<S>(a, lane, &job)) return;
+  const Item& it = job.it;
+  const int kend = job.kend, t0 = job.t0, nt = job.nt;
 
   // ---- this lane's row
   const int p = it.row0 + rb * 32 + col;
@@ -270,16 +696,7 @@ __global__ __launch_bounds__(S::kThreads) void paged_gqa_kernel(PagedArgs a) {
 
   const int32_t* table = a.c.table + it.req * a.c.table_stride;
   const int page_mask = (1 << a.c.shift) - 1;
-  // keys on no page: any in this item?
-  bool absent = false;
-  if (nt > 0) {
-    const int first = (t0 * S::kKeys) >> a.c.shift;
-    const int last = (min((t0 + nt) * S::kKeys, kend) - 1) >> a.c.shift;
-    bool bad = false;
-    for (int i = first + lane; i <= last; i += 64)
-      bad |= static_cast<unsigned>(table[i]) >= static_cast<unsigned>(a.c.n_pages);
-    absent = __builtin_amdgcn_ballot_w64(bad) != 0;
-  }
+  const bool absent = any_absent<S>(a, job, table, lane);
   // Page of a key below kend; keys on no page read page 0 and are masked.
   auto page_of = [&](int key) {
     const int page = scalar_load(table, key >> a.c.shift);
@@ -292,7 +709,7 @@ __global__ __launch_bounds__(S::kThreads) void paged_gqa_kernel(PagedArgs a) {
   auto copy_side = [&](const PagedSide& c, int tile, uint32_t lds, bool is_v) {
 #pragma unroll
     for (int i = 0; i < S::kCopies; ++i) {
-      const int g = S::kPrivate ? wave * S::kCopies + i : i * S::kWaves + wave;
+      const int g = i * S::kWaves + wave;
       const int row0 = uniform(g * S::kCopyRows);
       const int key0 = uniform(min(tile * S::kKeys + row0, kend - 1));
       const unsigned char* base = c.base + page_of(key0) * c.page + it.head * c.head;
@@ -312,7 +729,7 @@ __global__ __launch_bounds__(S::kThreads) void paged_gqa_kernel(PagedArgs a) {
   auto load_side = [&](const PagedSide& c, int tile, Codes& x) {
 #pragma unroll
     for (int i = 0; i < S::kLoads; ++i) {
-      const int g = S::kPrivate ? wave * S::kLoads + i : i * S::kWaves + wave;
+      const int g = i * S::kWaves + wave;
       const int row0 = uniform(g * S::kLoadRows);
       const int key0 = uniform(min(tile * S::kKeys + row0, kend - 1));
       const int page = page_of(key0);
@@ -325,7 +742,7 @@ __global__ __launch_bounds__(S::kThreads) void paged_gqa_kernel(PagedArgs a) {
   auto store_side = [&](const Codes& x, unsigned char* lds, bool is_v) {
 #pragma unroll
     for (int i = 0; i < S::kLoads; ++i) {
-      const int g = S::kPrivate ? wave * S::kLoads + i : i * S::kWaves + wave;
+      const int g = i * S::kWaves + wave;
       const int row = g * S::kLoadRows + lane / kLanesRow;
       const float s = scale_of(x.s[i]);
       const uint32_t w[4] = {x.w[i].x, x.w[i].y, x.w[i].z, x.w[i].w};
@@ -458,49 +875,7 @@ __global__ __launch_bounds__(S::kThreads) void paged_gqa_kernel(PagedArgs a) {
 
   unsigned char* const k_lds = smem;
   unsigned char* const v_lds = smem + S::kTileBytes * S::kStages;
-  if constexpr (S::kPrivate) {
-    // ---- every wavefront walks its own blocks: tile t's rows wave * 32 .. + 31.  K and V of a
-    // block have one buffer each; the next K is copied during the softmax and P V, the next V
-    // during the next scores.
-    const int row0 = wave * 32;
-    const int mine = max(0, min(nt, (kend - t0 * S::kKeys - row0 + S::kKeys - 1) / S::kKeys));
-    if constexpr (!S::FP8) {
-      if (mine > 0) {
-        copy_side(a.c.k, t0, lds0, false);
-        copy_side(a.c.v, t0, lds0 + S::kTileBytes, true);
-      }
-      for (int t = 0; t < mine; ++t) {
-        const int kb0 = (t0 + t) * S::kKeys + row0;
-        wait_copies<S::kCopies>();  // K has landed, V may be in flight
-        scores(k_lds, row0, kb0);
-        wait_lds_reads();
-        if (t + 1 < mine) {
-          copy_side(a.c.k, t0 + t + 1, lds0, false);
-          wait_copies<S::kCopies>();  // V has landed, the next K may be in flight
-        } else {
-          wait_copies<0>();
-        }
-        p_v(v_lds, row0, kb0);
-        wait_lds_reads();
-        if (t + 1 < mine) copy_side(a.c.v, t0 + t + 1, lds0 + S::kTileBytes, true);
-      }
-    } else {
-      Codes ck, cv;
-      if (mine > 0) {
-        load_side(a.c.k, t0, ck);
-        load_side(a.c.v, t0, cv);
-      }
-      for (int t = 0; t < mine; ++t) {
-        const int kb0 = (t0 + t) * S::kKeys + row0;
-        store_side(ck, k_lds, false);
-        if (t + 1 < mine) load_side(a.c.k, t0 + t + 1, ck);
-        scores(k_lds, row0, kb0);
-        store_side(cv, v_lds, true);
-        if (t + 1 < mine) load_side(a.c.v, t0 + t + 1, cv);
-        p_v(v_lds, row0, kb0);
-      }
-    }
-  } else {
+  {
     // ---- shared tiles, two stages: tile t + 1 arrives while tile t is worked on
     auto work_on = [&](int t, int buf) {
 #pragma unroll
@@ -566,36 +941,12 @@ __global__ __launch_bounds__(S::kThreads) void paged_gqa_kernel(PagedArgs a) {
     }
   }
   __syncthreads();
-  const int rows = min(S::kRows, it.rows - it.row0);
-  float* const part = a.part + slot * part_floats<S::kRows>(D);
-  for (int i = tid; i < rows * (D / 4); i += S::kThreads) {
-    const int row = i / (D / 4), d = (i % (D / 4)) * 4;
-    float m = ml[row * 2];
-#pragma unroll
-    for (int s = 1; s < S::KS; ++s) m = fmaxf(m, ml[(s * S::kRows + row) * 2]);
-    const float m_sub = m == -__builtin_inff() ? 0.0f : m;
-    f32x4_t acc = {0.0f, 0.0f, 0.0f, 0.0f};
-    float l = 0.0f;
-#pragma unroll
-    for (int s = 0; s < S::KS; ++s) {
-      const int at = s * S::kRows + row;
-      const float w = __builtin_amdgcn_exp2f(ml[at * 2] - m_sub);
-      l += ml[at * 2 + 1] * w;
-      acc += *reinterpret_cast<const f32x4_t*>(rowsf + at * S::kRowFloats + d) * w;
-    }
-    if (!split) {
-      store4(a, it, row, d, acc, l == 0.0f ? 0.0f : 1.0f / l);
-    } else {
-      *reinterpret_cast<f32x4_t*>(part + row * D + d) = acc;
-      if (d == 0) {
-        part[S::kRows * D + row * 2] = m;
-        part[S::kRows * D + row * 2 + 1] = l;
-      }
-    }
-  }
+  close_job<S, S::KS>(a, job, rowsf, ml);
 }
 
-// Joins the key ranges of every split row tile and stores its rows.
+// Joins the key ranges of every split row tile and stores its rows, kJoinRows of them per workgroup.
+constexpr int kJoinRows = 16;
+
 template <class S>
 __global__ __launch_bounds__(256) void paged_gqa_join_kernel(PagedArgs a) {
   constexpr int D = S::D;
@@ -607,34 +958,53 @@ __global__ __launch_bounds__(256) void paged_gqa_join_kernel(PagedArgs a) {
   if (ranges <= 1) return;  // its one item has stored the rows
   const int slot = it.base + it.head * it.n_ranges * it.n_rtiles + it.rtile;
   if (slot < 0 || slot + (ranges - 1) * static_cast<int64_t>(it.n_rtiles) >= a.max_items) return;
-  const int rows = min(S::kRows, it.rows - it.row0);
+  const int row_end = min(min(S::kRows, it.rows - it.row0), static_cast<int>(blockIdx.y + 1) * kJoinRows);
   const int64_t step = it.n_rtiles * part_floats<S::kRows>(D);  // from one range's part to the next one's
   const float* const part = a.part + slot * part_floats<S::kRows>(D);
-  for (int i = threadIdx.x; i < rows * (D / 4); i += 256) {
-    const int row = i / (D / 4), d = (i % (D / 4)) * 4;
-    float m = -__builtin_inff();
-    for (int s = 0; s < ranges; ++s) m = fmaxf(m, part[s * step + S::kRows * D + row * 2]);
-    const float m_sub = m == -__builtin_inff() ? 0.0f : m;
+  constexpr int kLanes = D / 4;  // of a row
+  for (int row = blockIdx.y * kJoinRows + threadIdx.x / kLanes; row < row_end; row += 256 / kLanes) {
+    const int d = (threadIdx.x % kLanes) * 4;
+    // four ranges at a time: their loads are in flight together
+    float m = -__builtin_inff(), l = 0.0f;
     f32x4_t acc = {0.0f, 0.0f, 0.0f, 0.0f};
-    float l = 0.0f;
-    for (int s = 0; s < ranges; ++s) {
-      const float* ps = part + s * step;
-      const float w = __builtin_amdgcn_exp2f(ps[S::kRows * D + row * 2] - m_sub);
-      l += ps[S::kRows * D + row * 2 + 1] * w;
-      acc += *reinterpret_cast<const f32x4_t*>(ps + row * D + d) * w;
+    for (int s0 = 0; s0 < ranges; s0 += 4) {
+      float ms[4], ls[4];
+      f32x4_t os[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const float* ps = part + min(s0 + u, ranges - 1) * step;
+        ms[u] = ps[S::kRows * D + row * 2];
+        ls[u] = ps[S::kRows * D + row * 2 + 1];
+        os[u] = *reinterpret_cast<const f32x4_t*>(ps + row * D + d);
+      }
+      float top = m;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        if (s0 + u >= ranges) ms[u] = -__builtin_inff(), ls[u] = 0.0f, os[u] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+        top = fmaxf(top, ms[u]);
+      }
+      const float sub = top == -__builtin_inff() ? 0.0f : top;
+      const float keep = __builtin_amdgcn_exp2f(m - sub);
+      l *= keep;
+      acc *= keep;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const float w = __builtin_amdgcn_exp2f(ms[u] - sub);
+        l += ls[u] * w;
+        acc += os[u] * w;
+      }
+      m = top;
     }
     store4(a, it, row, d, acc, l == 0.0f ? 0.0f : 1.0f / l);
   }
 }
 
 template <int D, bool FP8>
-using Few = Shape<D, FP8, 1, 4, 1>;
-template <int D, bool FP8>
 using Piece = Shape<D, FP8, 4, D == 256 ? 1 : 2, D == 64 ? 2 : 1>;
 
-// Items, row tiles and workspace of a call, whatever the lengths turn out to be.
+// The kernel of a call, and its items, row tiles and workspace, whatever the lengths turn out to be.
 struct Plan {
-  bool few;
+  int few;  // blocks of 16 rows of the few-rows kernel, 0: pieces
   int rows, keys, workers, min_tiles;
   int64_t items, rtiles, bytes;
   bool may_split;
@@ -642,11 +1012,12 @@ struct Plan {
 
 Plan plan_of(int64_t requests, int64_t tokens, int group, int kv_heads, int head_dim, int64_t max_keys, int max_seqlen) {
   Plan p;
-  p.few = static_cast<int64_t>(max_seqlen) * group <= 32;
-  p.rows = p.few ? Few<64, false>::kRows : Piece<64, false>::kRows;
-  p.keys = p.few ? Few<64, false>::kKeys
+  const int64_t rows = static_cast<int64_t>(max_seqlen) * group;
+  p.few = rows <= 16 ? 1 : rows <= 32 ? 2 : 0;
+  p.rows = p.few ? 16 * p.few : Piece<64, false>::kRows;
+  p.keys = p.few ? Few<64, false, 1>::kKeys
                  : head_dim == 64 ? Piece<64, false>::kKeys : head_dim == 128 ? Piece<128, false>::kKeys : Piece<256, false>::kKeys;
-  p.workers = p.few ? 1024 : 512;
+  p.workers = p.few ? 1024 : 256;
   p.min_tiles = 256 / p.keys;
   // a request's last row tile may be partly empty, its last key range too
   p.rtiles = kv_heads * (tokens * group / p.rows + requests);
@@ -656,24 +1027,26 @@ Plan plan_of(int64_t requests, int64_t tokens, int group, int kv_heads, int head
   return p;
 }
 
-template <class S, class Join>
-void launch(const PagedArgs& a, const Plan& p, hipStream_t s) {
-  static_assert(S::kRows == Join::kRows && S::kKeys == Join::kKeys, "one way of cutting the work");
+template <class S, typename K>
+void launch(K kernel, const PagedArgs& a, const Plan& p, hipStream_t s) {
   const int64_t blocks = (p.items + kNumXcd - 1) / kNumXcd * kNumXcd;
-  hipLaunchKernelGGL((paged_gqa_kernel<S>), dim3(static_cast<unsigned>(blocks)), dim3(S::kThreads), 0, s, a);
+  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(S::kThreads), 0, s, a);
   if (p.may_split)
-    hipLaunchKernelGGL((paged_gqa_join_kernel<Join>), dim3(static_cast<unsigned>(p.rtiles)), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((paged_gqa_join_kernel<S>), dim3(static_cast<unsigned>(p.rtiles), (S::kRows + kJoinRows - 1) / kJoinRows),
+                       dim3(256), 0, s, a);
+}
+
+template <int D, bool FP8>
+void launch_as(const PagedArgs& a, const Plan& p, hipStream_t s) {
+  if (p.few == 1) launch<Few<D, false, 1>>(paged_gqa_few_kernel<Few<D, FP8, 1>>, a, p, s);
+  else if (p.few == 2) launch<Few<D, false, 2>>(paged_gqa_few_kernel<Few<D, FP8, 2>>, a, p, s);
+  else launch<Piece<D, false>>(paged_gqa_kernel<Piece<D, FP8>>, a, p, s);
 }
 
 template <int D>
 void launch_dim(const PagedArgs& a, const Plan& p, bool fp8, hipStream_t s) {
-  if (p.few) {
-    if (fp8) launch<Few<D, true>, Few<D, false>>(a, p, s);
-    else launch<Few<D, false>, Few<D, false>>(a, p, s);
-  } else {
-    if (fp8) launch<Piece<D, true>, Piece<D, false>>(a, p, s);
-    else launch<Piece<D, false>, Piece<D, false>>(a, p, s);
-  }
+  if (fp8) launch_as<D, true>(a, p, s);
+  else launch_as<D, false>(a, p, s);
 }
 
 int check_sizes(const char* what, int batch, int q_heads, int kv_heads, int seq_len, int n_seqs, int max_seqlen) {
