@@ -27,6 +27,10 @@ SOURCES = ["fd_abi.cpp", "add_rmsnorm.hip", "packed_conv.hip", "gqa_fwd.hip", "g
 
 CACHE_SOURCES = ["cache_abi.cpp", "paged_kv.hip", "paged_gqa.hip", "delta_step.hip", "conv_state.hip"]
 
+# Accumulators of a kernel with more than 256 registers in either half of the register file: without
+# it the compiler puts them all in the accumulation half and copies scores over for every softmax.
+EXTRA_FLAGS = {"paged_gqa.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
+
 COMMON_FLAGS = [
     "-O3",
     "-std=c++17",
@@ -72,7 +76,7 @@ def build(verbose: bool = False, jobs: int = 4) -> Path:
         path = CSRC / src
         cmd = [cc, *COMMON_FLAGS]
         if src.endswith(".hip"):
-            cmd += ["-x", "hip", *DEVICE_FLAGS]
+            cmd += ["-x", "hip", *DEVICE_FLAGS, *EXTRA_FLAGS.get(src, [])]
         else:
             cmd += ["-x", "c++", "-D__HIP_PLATFORM_AMD__", f"-I{rocm_path()}/include"]
         cmd += ["-c", str(path), "-o", str(obj)]

@@ -56,24 +56,22 @@ struct Few {
   static constexpr int kPerCu = kSmemBytes > 80 * 1024 ? 1 : 2;  // workgroups that a CU's LDS holds
 };
 
-// Pieces: RB row blocks of 32 rows and KS key parts of a tile per workgroup, NB 32-key blocks per
-// wavefront and tile.
-template <int D_, bool FP8_, int RB_, int KS_, int NB_>
-struct Shape {
-  static constexpr int D = D_, RB = RB_, KS = KS_, NB = NB_;
+// Pieces: RW row wavefronts of NB blocks of 32 rows, times KS key parts of a tile.
+template <int D_, bool FP8_, int RW_, int NB_, int KS_>
+struct Piece {
+  static constexpr int D = D_, RW = RW_, NB = NB_, KS = KS_;
   static constexpr bool FP8 = FP8_;
-  static constexpr int kWaves = RB * KS;
+  static constexpr int kWaves = RW * KS;
   static constexpr int kThreads = 64 * kWaves;
-  static constexpr int kRows = 32 * RB;
-  static constexpr int kKeys = 32 * KS * NB;            // keys of a tile
-  static constexpr int CR = D / 8;                      // 16-byte chunks of a bf16 row
+  static constexpr int kRows = 32 * RW * NB;
+  static constexpr int kKeys = 32 * KS;                 // keys of a tile
+  static constexpr int CR = D / 8;                      // 16-byte chunks of a staged (bf16) row
   static constexpr int kTileBytes = kKeys * CR * 16;    // K or V
-  static constexpr int kStages = 2;
-  static constexpr int kStageBytes = 2 * kTileBytes * kStages;
-  // epilogue: every key part's rows, padded, and their (max, denominator)
-  static constexpr int kRowFloats = D + 4;
+  static constexpr int kStages = 4;
+  static constexpr int kRowFloats = D + 4;              // epilogue rows, padded
   static constexpr int kEpilogueBytes = KS * kRows * (kRowFloats + 2) * 4;
-  static constexpr int kSmemBytes = kStageBytes > kEpilogueBytes ? kStageBytes : kEpilogueBytes;
+  static constexpr int kLoopBytes = 2 * kStages * kTileBytes;
+  static constexpr int kSmemBytes = kLoopBytes > kEpilogueBytes ? kLoopBytes : kEpilogueBytes;
   // 1 KiB copies of a bf16 K (or V) tile per wavefront, and the rows of each
   static constexpr int kCopies = kTileBytes / 1024 / kWaves;
   static constexpr int kCopyRows = 1024 / (2 * D);
@@ -337,14 +335,24 @@ __device__ __forceinline__ int few_swz_v(int row) {
   else return 2 * (((row & 3) | ((row >> 3) & 1) << 2) >> kRowShift<ROW_BYTES>);
 }
 
-// Eight codes as bf16, scale 1 (exact).
-__device__ __forceinline__ bf16x8_t codes_to_bf16(uint32_t lo, uint32_t hi) {
+// Eight codes times a power of two as bf16 (exact).
+__device__ __forceinline__ bf16x8_t codes_to_bf16(uint32_t lo, uint32_t hi, float scale = 1.0f) {
   typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
-  const bf16x2_t a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, false);
-  const bf16x2_t b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, true);
-  const bf16x2_t c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, false);
-  const bf16x2_t d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, true);
+  const bf16x2_t a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, false);
+  const bf16x2_t b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, true);
+  const bf16x2_t c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, false);
+  const bf16x2_t d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, true);
   return bf16x8_t{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+
+// x plus the eight bf16 of p.
+__device__ __forceinline__ float sum8(bf16x8_t p, float x) {
+  typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+  const bf16x2_t one = {static_cast<__bf16>(1.0f), static_cast<__bf16>(1.0f)};
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    x = __builtin_amdgcn_fdot2_f32_bf16(bf16x2_t{p[2 * i], p[2 * i + 1]}, one, x, false);
+  return x;
 }
 
 // Half-word i (uniform) of four words.
@@ -661,15 +669,43 @@ __global__ __launch_bounds__(S::kThreads, S::kPerCu) void paged_gqa_few_kernel(P
 
 // ---------------------------------------------------------------- pieces
 
+// Runs f(u) for the softmax pieces u (8 per row block) that go behind MFMA m of a phase of NB * STEPS MFMAs.
+template <int NB, int STEPS, typename F>
+__device__ __forceinline__ void pieces(int m, F f) {
+  constexpr int kAll = 8 * NB, kMfma = NB * STEPS;
+  if constexpr (kAll >= kMfma) {
+#pragma unroll
+    for (int u = 0; u < kAll / kMfma; ++u) f(m * (kAll / kMfma) + u);
+  } else {
+    if (m % (kMfma / kAll) == 0) f(m / (kMfma / kAll));
+  }
+}
+
+// A wavefront owns NB blocks of 32 rows and every KS-th block of 32 keys.  With two row blocks an
+// operand read from LDS feeds two MFMAs: with one, the 4 SIMDs' operand reads (1 KiB per 32-cycle
+// MFMA each) alone would take all of LDS's 128 bytes per cycle.  One wavefront per SIMD: 128 rows
+// of 128 features are 128 registers of O^T and 64 of Q.
+//
+// Tiles that all rows see whole run in a pipelined loop without masks; the rest (the new tokens' own
+// tiles, and everything of a request with absent pages) in a plain one.  A pipelined step t has two
+// phases with one barrier between them:
+//   A: the score MFMAs of tile t + 1; between them the second half of tile t's softmax and the reads
+//      of tile t's V operands
+//   B: the P V MFMAs of tile t; between them the first half of tile t + 1's softmax and the reads of
+//      tile t + 2's K operands
+// so that the softmax's VALU and exp work runs under both halves of the MFMAs and every operand is
+// read a phase before it is used.  Four LDS stages: bf16 tiles are copied three steps ahead (asm copies,
+// counted by hand), codes are loaded into registers three steps ahead and stored as bf16 two ahead.
 template <class S>
-__global__ __launch_bounds__(S::kThreads) void paged_gqa_kernel(PagedArgs a) {
-  constexpr int D = S::D, CR = S::CR, kKk = D / 16, kNdb = D / 32;
+__global__ __launch_bounds__(S::kThreads) void paged_gqa_piece_kernel(PagedArgs a) {
+  constexpr int D = S::D, NB = S::NB, CR = S::CR, kNdb = D / 32, kSteps = D / 16, kAhead = 4;
+  constexpr bool FP8 = S::FP8;
   __shared__ __attribute__((aligned(1024))) unsigned char smem[S::kSmemBytes];
   const int tid = threadIdx.x;
   const int lane = tid & 63;
   const int wave = uniform(tid >> 6);
-  const int rb = wave % S::RB;   // row block
-  const int kp = wave / S::RB;   // key part
+  const int rw = wave % S::RW;   // row wavefront
+  const int kp = wave / S::RW;   // key part
   const int col = lane & 31, half = lane >> 5;
 
   Job job;
@@ -677,247 +713,421 @@ __global__ __launch_bounds__(S::kThreads) void paged_gqa_kernel(PagedArgs a) {
   const Item& it = job.it;
   const int kend = job.kend, t0 = job.t0, nt = job.nt;
 
-  // ---- this lane's row
-  const int p = it.row0 + rb * 32 + col;
-  const int pc = min(p, it.rows - 1);  // rows behind the last one repeat it and are not stored
-  const int token = pc / a.group;
-  const int pos = it.len - it.n_new + token;
-  bf16x8_t qf[kKk];
-  {
+  // ---- this lane's rows: col of each of the wavefront's row blocks
+  int pos[NB];
+  bf16x8_t qf[NB][kSteps];
+#pragma unroll
+  for (int n = 0; n < NB; ++n) {
+    const int p = min(it.row0 + (rw * NB + n) * 32 + col, it.rows - 1);  // rows behind the last repeat it, not stored
+    const int token = p / a.group;
+    pos[n] = it.len - it.n_new + token;
     const int b = a.cu == nullptr ? it.req : 0;
-    const int head = it.head * a.group + (pc - token * a.group);
+    const int head = it.head * a.group + (p - token * a.group);
     const uint16_t* qp = a.q + b * a.qs[0] + head * a.qs[1] + static_cast<int64_t>(it.start + token) * a.qs[2] + half * 8;
 #pragma unroll
-    for (int kk = 0; kk < kKk; ++kk) qf[kk] = *reinterpret_cast<const bf16x8_t*>(qp + kk * 16);
+    for (int kk = 0; kk < kSteps; ++kk) qf[n][kk] = *reinterpret_cast<const bf16x8_t*>(qp + kk * 16);
   }
-  const bool has_rows = it.row0 + rb * 32 < it.rows;
-  const int pos_min = uniform(it.len - it.n_new + min(it.row0 + rb * 32, it.rows - 1) / a.group);
-  const int pos_max = uniform(it.len - it.n_new + min(it.row0 + rb * 32 + 31, it.rows - 1) / a.group);
-
-  const int32_t* table = a.c.table + it.req * a.c.table_stride;
+  const int32_t* const table = a.c.table + it.req * a.c.table_stride;
   const int page_mask = (1 << a.c.shift) - 1;
   const bool absent = any_absent<S>(a, job, table, lane);
-  // Page of a key below kend; keys on no page read page 0 and are masked.
-  auto page_of = [&](int key) {
-    const int page = scalar_load(table, key >> a.c.shift);
-    return static_cast<unsigned>(page) < static_cast<unsigned>(a.c.n_pages) ? page : 0;
-  };
+  // tiles [0, n_full) of the job are seen whole by every row of the workgroup
+  const int pos_first = uniform(it.len - it.n_new + it.row0 / a.group);
+  const int n_full = absent ? 0 : max(0, min(nt, (pos_first + 1) / S::kKeys - t0));
 
+  // ---- staging.  The kMoveRows rows of a copy (or load) lie on one page: its address is a scalar base plus
+  // a lane offset that depends on no tile.  Tiles that reach past kend repeat row kend - 1 there (the mask
+  // discards it).
   const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_void_t*)smem));
-  // ---- staging.  Rows past kend repeat row kend - 1; the mask discards them.
-  // bf16: copy g of a tile brings rows g * kCopyRows .. of it, one page's, to 1 KiB of LDS.
-  auto copy_side = [&](const PagedSide& c, int tile, uint32_t lds, bool is_v) {
+  unsigned char* const k_lds = smem;
+  unsigned char* const v_lds = smem + S::kStages * S::kTileBytes;
+  constexpr int kMoves = FP8 ? S::kLoads : S::kCopies;  // per wavefront and side
+  constexpr int kMoveRows = FP8 ? S::kLoadRows : S::kCopyRows;
+  constexpr int kLanesRow = 64 / kMoveRows;             // lanes of a row, 16 bytes each
+  const int lrow = lane / kLanesRow;
+  struct Pages {
+    int p[kMoves];
+  };
+  auto move_row = [&](int i) { return (i * S::kWaves + wave) * kMoveRows; };  // first row of move i within a tile
+  auto pages_of = [&](int t) {
+    Pages x;
 #pragma unroll
-    for (int i = 0; i < S::kCopies; ++i) {
-      const int g = i * S::kWaves + wave;
-      const int row0 = uniform(g * S::kCopyRows);
-      const int key0 = uniform(min(tile * S::kKeys + row0, kend - 1));
-      const unsigned char* base = c.base + page_of(key0) * c.page + it.head * c.head;
-      const int lrow = row0 + lane / CR;  // of the tile
-      const int key = min(tile * S::kKeys + lrow, kend - 1);
-      const int chunk = (lane % CR) ^ (is_v ? swz_v<CR>(lrow) : swz_k<CR>(lrow));
-      const uint32_t off = static_cast<uint32_t>((key & page_mask) * static_cast<int>(c.row) + chunk * 16);
-      copy_to_lds(base, off, lds + static_cast<uint32_t>(g * 1024));
+    for (int i = 0; i < kMoves; ++i) {
+      const int key = uniform(max(min((t0 + t) * S::kKeys + move_row(i), kend - 1), 0));
+      const int page = scalar_load(table, key >> a.c.shift);
+      x.p[i] = static_cast<unsigned>(page) < static_cast<unsigned>(a.c.n_pages) ? page : 0;
+    }
+    return x;
+  };
+  // first row of move i of tile t on its page, and this lane's row from there
+  auto first_row = [&](int t, int i) { return uniform(min((t0 + t) * S::kKeys + move_row(i), kend - 1)) & page_mask; };
+  auto lane_row = [&](auto whole_c, int t, int i) {
+    if constexpr (decltype(whole_c)::value) return lrow;
+    else return max(0, min(lrow, kend - 1 - ((t0 + t) * S::kKeys + move_row(i))));
+  };
+  auto copy_tile = [&](auto whole_c, const Pages& pg, int t, int buf) {
+#pragma unroll
+    for (int v = 0; v < 2; ++v) {
+      const PagedSide& c = v ? a.c.v : a.c.k;
+#pragma unroll
+      for (int i = 0; i < S::kCopies; ++i) {
+        const unsigned char* base = c.base + pg.p[i] * c.page + it.head * c.head + first_row(t, i) * c.row;
+        const int row = move_row(i) + lrow;
+        const int chunk = (lane % CR) ^ (v ? swz_v<CR>(row) : swz_k<CR>(row));
+        copy_to_lds(base, static_cast<uint32_t>(lane_row(whole_c, t, i) * static_cast<int>(c.row) + chunk * 16),
+                    lds0 + static_cast<uint32_t>((v * S::kStages + buf) * S::kTileBytes + (i * S::kWaves + wave) * 1024));
+      }
     }
   };
-  // e4m3: 16 codes per lane into registers, later converted and stored as bf16
   struct Codes {
-    uint4 w[S::FP8 ? S::kLoads : 1];
-    uint32_t s[S::FP8 ? S::kLoads : 1];
+    uint4 w[FP8 ? 2 * S::kLoads : 1];
+    uint32_t s[FP8 ? 2 * S::kLoads : 1];
   };
-  constexpr int kLanesRow = D / 16;
-  auto load_side = [&](const PagedSide& c, int tile, Codes& x) {
+  auto load_tile = [&](auto whole_c, const Pages& pg, int t, Codes& x) {
 #pragma unroll
     for (int i = 0; i < S::kLoads; ++i) {
-      const int g = i * S::kWaves + wave;
-      const int row0 = uniform(g * S::kLoadRows);
-      const int key0 = uniform(min(tile * S::kKeys + row0, kend - 1));
-      const int page = page_of(key0);
-      const int key = min(tile * S::kKeys + row0 + lane / kLanesRow, kend - 1) & page_mask;
-      const unsigned char* base = c.base + page * c.page + it.head * c.head;
-      x.w[i] = *reinterpret_cast<const uint4*>(base + static_cast<uint32_t>(key * static_cast<int>(c.row) + (lane % kLanesRow) * 16));
-      x.s[i] = *(c.scale + page * c.s_page + it.head * c.s_head + static_cast<uint32_t>(key));
+      const uint32_t row = static_cast<uint32_t>(lane_row(whole_c, t, i));
+#pragma unroll
+      for (int v = 0; v < 2; ++v) {
+        const PagedSide& c = v ? a.c.v : a.c.k;
+        const unsigned char* base = c.base + pg.p[i] * c.page + it.head * c.head + first_row(t, i) * c.row;
+        x.w[2 * i + v] = *reinterpret_cast<const uint4*>(base + (row * static_cast<uint32_t>(c.row) + (lane % kLanesRow) * 16));
+        x.s[2 * i + v] = (c.scale + pg.p[i] * c.s_page + it.head * c.s_head + first_row(t, i))[row];
+      }
     }
   };
-  auto store_side = [&](const Codes& x, unsigned char* lds, bool is_v) {
+  auto store_tile = [&](const Codes& x, int buf) {
 #pragma unroll
     for (int i = 0; i < S::kLoads; ++i) {
-      const int g = i * S::kWaves + wave;
-      const int row = g * S::kLoadRows + lane / kLanesRow;
-      const float s = scale_of(x.s[i]);
-      const uint32_t w[4] = {x.w[i].x, x.w[i].y, x.w[i].z, x.w[i].w};
+      const int row = move_row(i) + lrow;
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        uint32_t b[4];
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int code = static_cast<int>(w[2 * h + e]);
-          const auto f0 = __builtin_amdgcn_cvt_pk_f32_fp8(code, false);
-          const auto f1 = __builtin_amdgcn_cvt_pk_f32_fp8(code, true);
-          b[2 * e] = fd_pack2(f0[0] * s, f0[1] * s);
-          b[2 * e + 1] = fd_pack2(f1[0] * s, f1[1] * s);
-        }
-        const int chunk = ((lane % kLanesRow) * 2 + h) ^ (is_v ? swz_v<CR>(row) : swz_k<CR>(row));
-        *reinterpret_cast<uint4*>(lds + row * CR * 16 + chunk * 16) = uint4{b[0], b[1], b[2], b[3]};
+      for (int v = 0; v < 2; ++v) {
+        const float s = scale_of(x.s[2 * i + v]);
+        unsigned char* const dst = (v ? v_lds : k_lds) + buf * S::kTileBytes + row * CR * 16;
+        const int swz = v ? swz_v<CR>(row) : swz_k<CR>(row);
+        const uint4 w = x.w[2 * i + v];
+        *reinterpret_cast<bf16x8_t*>(dst + (((lane % kLanesRow) * 2) ^ swz) * 16) = codes_to_bf16(w.x, w.y, s);
+        *reinterpret_cast<bf16x8_t*>(dst + (((lane % kLanesRow) * 2 + 1) ^ swz) * 16) = codes_to_bf16(w.z, w.w, s);
       }
     }
   };
 
-  f32x16_t o[kNdb];
+  f32x16_t o[NB][kNdb];
+  float m_run[NB], l_run[NB];
 #pragma unroll
-  for (int db = 0; db < kNdb; ++db) o[db] = f32x16_t{};
-  float m_run = -__builtin_inff();  // running maximum (log2 units), may lag the true one by 8
-  float l_run = 0.0f;               // this lane's part of the denominator
+  for (int n = 0; n < NB; ++n) {
+    m_run[n] = -__builtin_inff();  // running maximum (log2 units), may lag the true one by 8
+    l_run[n] = 0.0f;               // this lane's part of the denominator
+#pragma unroll
+    for (int db = 0; db < kNdb; ++db) o[n][db] = f32x16_t{};
+  }
 
-  // ---- one 32-key block from LDS: scores, softmax, then P V.  `row0` is the block's
-  // first row within the staged tile, kb0 its first key.
+  // ---- operand addresses within a tile.  K: row kp * 32 + sigma(col), chunk 2 kk + half.  V^T of O
+  // block db: two transposing reads (keys + 0..3, + 4..7) per 16-key slice.
   const int grp = lane >> 4, li = lane & 15;
-  bf16x8_t pb[2];
-  auto scores = [&](const unsigned char* kt, int row0, int kb0) {
-    f32x16_t s = f32x16_t{};
-    const int row = row0 + sigma(col);
+  int k_rd[kSteps], v_rd[kNdb];
 #pragma unroll
-    for (int kk = 0; kk < kKk; ++kk) {
-      const bf16x8_t kf = *reinterpret_cast<const bf16x8_t*>(kt + row * CR * 16 + (((2 * kk + half) ^ swz_k<CR>(row)) * 16));
-      s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qf[kk], s, 0, 0, 0);
-    }
-    if (kb0 + 31 > pos_min || absent) {
-      bool there[2] = {true, true};
-      if (absent) {
+  for (int kk = 0; kk < kSteps; ++kk) {
+    const int row = kp * 32 + sigma(col);
+    k_rd[kk] = row * CR * 16 + (((2 * kk + half) ^ swz_k<CR>(row)) * 16);
+  }
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const int key = min(kb0 + 16 * j, kend - 1);
-          there[j] = static_cast<unsigned>(scalar_load(table, uniform(key >> a.c.shift))) < static_cast<unsigned>(a.c.n_pages);
-        }
-      }
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int key = kb0 + (r >> 3) * 16 + half * 8 + (r & 7);
-        if (key > pos || !there[r >> 3]) s[r] = -__builtin_inff();
-      }
-    }
-    float mx = s[0];
-#pragma unroll
-    for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[r]);
-    mx = half_max(mx) * a.scale_log2;
-    const bool grow = mx > m_run + 8.0f;
-    const float m_new = grow ? mx : m_run;
-    const float alpha = grow ? __builtin_amdgcn_exp2f(m_run - m_new) : 1.0f;
-    const float m_sub = m_new == -__builtin_inff() ? 0.0f : m_new;  // nothing seen so far: p = 0
-    m_run = m_new;
-    if (__builtin_amdgcn_ballot_w64(grow) != 0) {
-#pragma unroll
-      for (int db = 0; db < kNdb; ++db) o[db] *= alpha;
-    }
-    float psum = 0.0f;
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      f32x8_t pv;
-#pragma unroll
-      for (int r = 0; r < 8; ++r) pv[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[8 * j + r], a.scale_log2, -m_sub));
-      pb[j] = __builtin_convertvector(pv, bf16x8_t);
-      // the denominator takes the rounded p: its error then cancels where a few keys carry the row
-      const f32x8_t pr = __builtin_convertvector(pb[j], f32x8_t);
-#pragma unroll
-      for (int r = 0; r < 8; ++r) psum += pr[r];
-    }
-    l_run = l_run * alpha + psum;
+  for (int db = 0; db < kNdb; ++db) {
+    const int dim = db * 32 + 16 * (grp & 1) + 4 * (li & 3);
+    const int row = kp * 32 + 8 * (grp >> 1) + (li >> 2);
+    v_rd[db] = row * CR * 16 + (((dim >> 3) ^ swz_v<CR>(row)) * 16) + (dim & 7) * 2;
+  }
+  bf16x8_t kf[kAhead];               // K operands a few MFMAs ahead
+  v4i16_t vlo[kSteps], vhi[kSteps];  // V operands of a tile; MFMA i: slice i / kNdb, O block i % kNdb
+  auto read_k = [&](int buf, int kk) {
+    kf[kk % kAhead] = *reinterpret_cast<const bf16x8_t*>(k_lds + buf * S::kTileBytes + k_rd[kk]);
   };
-  auto p_v = [&](const unsigned char* vt, int row0, int kb0) {
-    // a block with masked keys: their values must not reach a row as 0 * NaN or 0 * inf
-    const bool guard = kb0 + 31 > pos_min || absent;
+  auto read_v = [&](int buf, int i) {
+    const unsigned char* vt = v_lds + buf * S::kTileBytes + v_rd[i % kNdb] + (i / kNdb) * 16 * CR * 16;
+    vlo[i] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16_t*)vt);
+    vhi[i] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16_t*)(vt + 4 * CR * 16));
+  };
+  auto v_operand = [&](int i) {
+    const short __attribute__((ext_vector_type(8))) vv = {vlo[i][0], vlo[i][1], vlo[i][2], vlo[i][3],
+                                                          vhi[i][0], vhi[i][1], vhi[i][2], vhi[i][3]};
+    return __builtin_bit_cast(bf16x8_t, vv);
+  };
+
+  // ---- softmax of a row block's scores, in pieces that fit behind one MFMA each: maximum and first half
+  // of the probabilities (head), second half, rounding and denominator (tail)
+  float p[NB][16], alpha[NB], m_sub[NB], mx[NB];
+  bf16x8_t pb[NB][2];
+  bool grow[NB];
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
+  for (int n = 0; n < NB; ++n) alpha[n] = 1.0f, m_sub[n] = 0.0f, mx[n] = 0.0f, grow[n] = false;
+  auto exps = [&](int n, const f32x16_t& s, int r0) {
 #pragma unroll
-      for (int db = 0; db < kNdb; ++db) {
-        const int dim = db * 32 + 16 * (grp & 1) + 4 * (li & 3);
-        const int row = row0 + 16 * j + 8 * (grp >> 1) + (li >> 2);
-        const unsigned char* vp = vt + row * CR * 16 + (((dim >> 3) ^ swz_v<CR>(row)) * 16) + (dim & 7) * 2;
-        v4i16_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16_t*)vp);
-        v4i16_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16_t*)(vp + 4 * CR * 16));
-        if (guard) {
-          short e[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-          bool odd = false;
+    for (int r = r0; r < r0 + 2; ++r) {
+      p[n][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], a.scale_log2, -m_sub[n]));
+      asm volatile("" : "+v"(p[n][r]));  // computed here, not sunk towards its use in P V
+    }
+  };
+  auto head = [&](int n, int k, const f32x16_t& s) {
+    if (k == 0) {
+      mx[n] = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
 #pragma unroll
-          for (int i = 0; i < 8; ++i) odd |= (e[i] & 0x7f80) == 0x7f80;
-          if (__builtin_amdgcn_ballot_w64(odd) != 0) {
-            // This lane holds V[key 16 j + 8 half + i][32 db + col]: infinities and NaN leave the
-            // product and are added by hand to the rows that see them.
-#pragma unroll 1
-            for (int i = 0; i < 8; ++i) {
-              const float x = (e[i] & 0x7f80) == 0x7f80 ? fd_bf16_to_f32(static_cast<uint16_t>(e[i])) : 0.0f;
-              float pi = 0.0f;
+      for (int r = 4; r < 8; ++r) mx[n] = fmaxf(mx[n], s[r]);
+    } else if (k == 1) {
 #pragma unroll
-              for (int u = 0; u < 8; ++u) pi = u == i ? static_cast<float>(pb[j][u]) : pi;
-#pragma unroll 1
-              for (int h = 0; h < 2; ++h) {
-                const float ph = __shfl(pi, h * 32 + col);  // this lane's row, key 16 j + 8 h + i
+      for (int r = 8; r < 16; ++r) mx[n] = fmaxf(mx[n], s[r]);
+    } else if (k == 2) {
+      mx[n] = half_max(mx[n]) * a.scale_log2;
+      grow[n] = mx[n] > m_run[n] + 8.0f;
+      const float m_new = grow[n] ? mx[n] : m_run[n];
+      alpha[n] = grow[n] ? __builtin_amdgcn_exp2f(m_run[n] - m_new) : 1.0f;
+      m_sub[n] = m_new == -__builtin_inff() ? 0.0f : m_new;  // nothing seen so far: p = 0
+      m_run[n] = m_new;
+    } else if (k < 7) {
+      exps(n, s, 2 * (k - 3));
+    }
+  };
+  auto round8 = [&](int n, int j) {
+    pb[n][j] = __builtin_convertvector(f32x8_t{p[n][8 * j], p[n][8 * j + 1], p[n][8 * j + 2], p[n][8 * j + 3], p[n][8 * j + 4],
+                                               p[n][8 * j + 5], p[n][8 * j + 6], p[n][8 * j + 7]}, bf16x8_t);
+    asm volatile("" : "+v"(pb[n][j]));
+  };
+  auto tail = [&](int n, int k, const f32x16_t& s) {
+    if (k < 4) {
+      exps(n, s, 8 + 2 * k);
+    } else if (k == 4) {
+      round8(n, 0);
+    } else if (k == 5) {
+      round8(n, 1);
+    } else if (k == 6) {
+      // the denominator takes the rounded p: its error then cancels where a few keys carry the row
+      l_run[n] = sum8(pb[n][1], sum8(pb[n][0], l_run[n] * alpha[n]));
+      asm volatile("" : "+v"(l_run[n]));
+    }
+  };
+  auto rescale = [&]() {
 #pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                  const int d = (r & 3) + 8 * (r >> 2) + 4 * half;  // feature of o[db][r]
-                  const float xd = __shfl(x, h * 32 + d);
-                  if (xd != 0.0f && ph != 0.0f) o[db][r] += ph * xd;
-                }
-              }
+    for (int n = 0; n < NB; ++n) {
+      if (__builtin_amdgcn_ballot_w64(grow[n]) != 0) {
+#pragma unroll
+        for (int db = 0; db < kNdb; ++db) o[n][db] *= alpha[n];
+      }
+    }
+  };
+
+  const std::true_type whole{};
+  const std::false_type part{};
+  Codes codes;
+  if (n_full > 0) {
+    f32x16_t sA[NB], sB[NB];
+    Pages next;
+    // Prologue: tiles 0 and 1 landed (Q too), tile 2 on its way; scores of tile 0 and the head of its softmax.
+    if constexpr (!FP8) {
+      copy_tile(whole, pages_of(0), 0, 0);
+      if (n_full > 1) copy_tile(whole, pages_of(1), 1, 1);
+      next = pages_of(2);
+      wait_copies<0>();
+#pragma unroll
+      for (int n = 0; n < NB; ++n)
+#pragma unroll
+        for (int kk = 0; kk < kSteps; ++kk) asm volatile("" : "+v"(qf[n][kk]));  // the compiler's own loads end here
+      if (n_full > 2) copy_tile(whole, next, 2, 2);
+    } else {
+      load_tile(part, pages_of(0), 0, codes);
+      next = pages_of(1);
+      store_tile(codes, 0);
+      load_tile(part, next, 1, codes);  // (tiles behind the last whole one may reach past kend)
+      next = pages_of(2);
+      store_tile(codes, 1);
+      load_tile(part, next, 2, codes);
+    }
+    next = pages_of(3);
+    __syncthreads();
+#pragma unroll
+    for (int n = 0; n < NB; ++n) sA[n] = f32x16_t{};
+#pragma unroll
+    for (int kk = 0; kk < kSteps; ++kk) {
+      read_k(0, kk);
+#pragma unroll
+      for (int n = 0; n < NB; ++n) sA[n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[kk % kAhead], qf[n][kk], sA[n], 0, 0, 0);
+    }
+    if (n_full > 1) {
+#pragma unroll
+      for (int kk = 0; kk < kAhead; ++kk) read_k(1, kk);
+    }
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+      for (int k = 0; k < 8; ++k) head(n, k, sA[n]);
+
+    // BUF = t % 4; LAST: no tile t + 1
+    auto step = [&](auto last_c, int t, int BUF, f32x16_t (&sc)[NB], f32x16_t (&sn)[NB]) {
+      constexpr bool LAST = decltype(last_c)::value;
+      const bool issued = !LAST && t + 3 < n_full;
+      if constexpr (!LAST) {
+        if constexpr (FP8) {
+          if (t + 2 < n_full) store_tile(codes, (BUF + 2) & 3);
+          if (issued) load_tile(whole, next, t + 3, codes);
+        } else {
+          if (issued) copy_tile(whole, next, t + 3, (BUF + 3) & 3);
+        }
+        next = pages_of(t + 4);
+      }
+      // ---- phase A
+      __builtin_amdgcn_sched_barrier(0);
+      if constexpr (!LAST) {
+#pragma unroll
+        for (int n = 0; n < NB; ++n)
+#pragma unroll
+          for (int kk = 0; kk < kSteps; ++kk) asm volatile("" : "+a"(qf[n][kk]));
+#pragma unroll
+        for (int n = 0; n < NB; ++n) sn[n] = f32x16_t{};
+#pragma unroll
+        for (int kk = 0; kk < kSteps; ++kk) {
+#pragma unroll
+          for (int n = 0; n < NB; ++n) {
+            sn[n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[kk % kAhead], qf[n][kk], sn[n], 0, 0, 0);
+            if (n == NB - 1) {
+              if (kk + kAhead < kSteps) read_k((BUF + 1) & 3, kk + kAhead);
+              read_v(BUF, kk);
             }
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              if ((lo[i] & 0x7f80) == 0x7f80) lo[i] = 0;
-              if ((hi[i] & 0x7f80) == 0x7f80) hi[i] = 0;
-            }
+            pieces<NB, kSteps>(kk * NB + n, [&](int u) { tail(u % NB, u / NB, sc[u % NB]); });
+            __builtin_amdgcn_sched_barrier(0);
           }
         }
-        const short __attribute__((ext_vector_type(8))) vv = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-        o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, vv), pb[j], o[db], 0, 0, 0);
-      }
-    }
-  };
-
-  unsigned char* const k_lds = smem;
-  unsigned char* const v_lds = smem + S::kTileBytes * S::kStages;
-  {
-    // ---- shared tiles, two stages: tile t + 1 arrives while tile t is worked on
-    auto work_on = [&](int t, int buf) {
+      } else {
 #pragma unroll
-      for (int nb = 0; nb < S::NB; ++nb) {
-        const int row0 = (kp * S::NB + nb) * 32;
-        const int kb0 = (t0 + t) * S::kKeys + row0;
-        if (has_rows && kb0 <= pos_max) {
-          scores(k_lds + buf * S::kTileBytes, row0, kb0);
-          p_v(v_lds + buf * S::kTileBytes, row0, kb0);
+        for (int i = 0; i < kSteps; ++i) read_v(BUF, i);
+#pragma unroll
+        for (int n = 0; n < NB; ++n)
+#pragma unroll
+          for (int k = 0; k < 8; ++k) tail(n, k, sc[n]);
+      }
+      rescale();  // by tile t's alpha: phase B moves it on to tile t + 1
+      if constexpr (!LAST) {
+        if constexpr (!FP8) {
+          if (issued) wait_copies<2 * S::kCopies>();  // all but this step's: tile t + 2 has landed
+          else wait_copies<0>();
+        }
+        wait_lds_reads();  // the V operands have arrived, their stage is free after the barrier
+        __syncthreads();
+      }
+      // ---- phase B
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int i = 0; i < kSteps; ++i) {
+#pragma unroll
+        for (int n = 0; n < NB; ++n) {
+          o[n][i % kNdb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v_operand(i), pb[n][i / kNdb], o[n][i % kNdb], 0, 0, 0);
+          if constexpr (!LAST) {
+            if (n == 0 && i >= kSteps - kAhead) read_k((BUF + 2) & 3, i - (kSteps - kAhead));
+            pieces<NB, kSteps>(i * NB + n, [&](int u) { head(u % NB, u / NB, sn[u % NB]); });
+          }
+          __builtin_amdgcn_sched_barrier(0);
         }
       }
     };
-    if constexpr (!S::FP8) {
-      auto copy_tile = [&](int t, int buf) {
-        copy_side(a.c.k, t0 + t, lds0 + static_cast<uint32_t>(buf * S::kTileBytes), false);
-        copy_side(a.c.v, t0 + t, lds0 + static_cast<uint32_t>((S::kStages + buf) * S::kTileBytes), true);
-      };
-      if (nt > 0) copy_tile(0, 0);
-      for (int t = 0; t < nt; ++t) {
-        wait_copies<0>();
-        wait_lds_reads();  // of tile t - 1: its stage is copied over next
-        __syncthreads();
-        if (t + 1 < nt) copy_tile(t + 1, (t + 1) & 1);
-        work_on(t, t & 1);
-      }
+    const std::false_type mid{};
+    const std::true_type last{};
+    const int n1 = n_full - 1;
+    int t = 0;
+    for (; t + 4 <= n1; t += 4) {
+      step(mid, t, 0, sA, sB);
+      step(mid, t + 1, 1, sB, sA);
+      step(mid, t + 2, 2, sA, sB);
+      step(mid, t + 3, 3, sB, sA);
+    }
+    if (t < n1) step(mid, t, 0, sA, sB);
+    if (t + 1 < n1) step(mid, t + 1, 1, sB, sA);
+    if (t + 2 < n1) step(mid, t + 2, 2, sA, sB);
+    if (n1 & 1) {
+#pragma unroll
+      for (int n = 0; n < NB; ++n) sA[n] = sB[n];
+    }
+    step(last, n1, n1 & 3, sA, sB);
+  }
+
+  // ---- the other tiles, one at a time: copied, masked, and with values of masked keys kept out
+#pragma unroll 1
+  for (int t = n_full; t < nt; ++t) {
+    __syncthreads();  // every wavefront has read the tile before
+    if constexpr (FP8) {
+      load_tile(part, pages_of(t), t, codes);
+      store_tile(codes, 0);
     } else {
-      Codes ck, cv;
-      if (nt > 0) {
-        load_side(a.c.k, t0, ck);
-        load_side(a.c.v, t0, cv);
+      copy_tile(part, pages_of(t), t, 0);
+      wait_copies<0>();
+    }
+    __syncthreads();
+    const int kb0 = (t0 + t) * S::kKeys + kp * 32;
+    bool there[2] = {true, true};
+    if (absent) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int key = uniform(min(kb0 + 16 * j, kend - 1));
+        there[j] = static_cast<unsigned>(scalar_load(table, key >> a.c.shift)) < static_cast<unsigned>(a.c.n_pages);
       }
-      for (int t = 0; t < nt; ++t) {
-        // the other stage is being read by the wavefronts still at tile t - 1
-        store_side(ck, k_lds + (t & 1) * S::kTileBytes, false);
-        store_side(cv, v_lds + (t & 1) * S::kTileBytes, true);
-        if (t + 1 < nt) {
-          load_side(a.c.k, t0 + t + 1, ck);
-          load_side(a.c.v, t0 + t + 1, cv);
+    }
+    f32x16_t s[NB];
+#pragma unroll
+    for (int n = 0; n < NB; ++n) s[n] = f32x16_t{};
+#pragma unroll
+    for (int kk = 0; kk < kSteps; ++kk) {
+      read_k(0, kk);
+#pragma unroll
+      for (int n = 0; n < NB; ++n) s[n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[kk % kAhead], qf[n][kk], s[n], 0, 0, 0);
+    }
+#pragma unroll
+    for (int n = 0; n < NB; ++n) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int key = kb0 + (r >> 3) * 16 + half * 8 + (r & 7);
+        if (key > pos[n] || !there[r >> 3]) s[n][r] = -__builtin_inff();
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) head(n, k, s[n]);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) tail(n, k, s[n]);
+    }
+    rescale();
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) {
+      const int j = i / kNdb, db = i % kNdb;
+      read_v(0, i);
+      bf16x8_t vf = v_operand(i);  // V[key 16 j + 8 half + e][32 db + col]
+      typedef short i16x8_t __attribute__((ext_vector_type(8)));
+      typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
+      i16x8_t e = __builtin_bit_cast(i16x8_t, vf);
+      bool odd = false;
+#pragma unroll
+      for (int u = 0; u < 8; ++u) odd |= (e[u] & 0x7f80) == 0x7f80;
+      if (__builtin_amdgcn_ballot_w64(odd) != 0) {
+        // infinities and NaN leave the product (0 times one is NaN) and are added by hand to the rows that see them
+        const u32x4_t ew = __builtin_bit_cast(u32x4_t, vf);
+#pragma unroll 1
+        for (int u = 0; u < 8; ++u) {
+          const uint32_t bits = half_of(ew[0], ew[1], ew[2], ew[3], u);
+          const float x = (bits & 0x7f80u) == 0x7f80u ? fd_bf16_to_f32(bits) : 0.0f;
+#pragma unroll
+          for (int n = 0; n < NB; ++n) {
+            const u32x4_t pw = __builtin_bit_cast(u32x4_t, pb[n][j]);
+            const float pu = fd_bf16_to_f32(half_of(pw[0], pw[1], pw[2], pw[3], u));
+#pragma unroll 1
+            for (int h = 0; h < 2; ++h) {
+              const float ph = __shfl(pu, h * 32 + col);  // this lane's row, key 16 j + 8 h + u
+#pragma unroll
+              for (int r = 0; r < 16; ++r) {
+                const float xd = __shfl(x, h * 32 + (r & 3) + 8 * (r >> 2) + 4 * half);  // feature of o[n][db][r]
+                if (xd != 0.0f && ph != 0.0f) o[n][db][r] += ph * xd;
+              }
+            }
+          }
         }
-        __syncthreads();
-        work_on(t, t & 1);
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+          if ((e[u] & 0x7f80) == 0x7f80) e[u] = 0;
+        vf = __builtin_bit_cast(bf16x8_t, e);
       }
+#pragma unroll
+      for (int n = 0; n < NB; ++n) o[n][db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pb[n][j], o[n][db], 0, 0, 0);
     }
   }
 
@@ -925,18 +1135,19 @@ __global__ __launch_bounds__(S::kThreads) void paged_gqa_kernel(PagedArgs a) {
   __syncthreads();  // the stages are free
   float* const rowsf = reinterpret_cast<float*>(smem);
   float* const ml = rowsf + S::KS * S::kRows * S::kRowFloats;
-  {
-    const int at = kp * S::kRows + rb * 32 + col;
+#pragma unroll
+  for (int n = 0; n < NB; ++n) {
+    const int at = kp * S::kRows + (rw * NB + n) * 32 + col;
     float* dst = rowsf + at * S::kRowFloats;
 #pragma unroll
     for (int db = 0; db < kNdb; ++db)
 #pragma unroll
       for (int r4 = 0; r4 < 4; ++r4)
         *reinterpret_cast<f32x4_t*>(dst + db * 32 + r4 * 8 + half * 4) =
-            f32x4_t{o[db][r4 * 4], o[db][r4 * 4 + 1], o[db][r4 * 4 + 2], o[db][r4 * 4 + 3]};
-    const float l = half_sum(l_run);
+            f32x4_t{o[n][db][r4 * 4], o[n][db][r4 * 4 + 1], o[n][db][r4 * 4 + 2], o[n][db][r4 * 4 + 3]};
+    const float l = half_sum(l_run[n]);
     if (half == 0) {
-      ml[at * 2] = m_run;
+      ml[at * 2] = m_run[n];
       ml[at * 2 + 1] = l;
     }
   }
@@ -999,8 +1210,9 @@ __global__ __launch_bounds__(256) void paged_gqa_join_kernel(PagedArgs a) {
   }
 }
 
+// 128 rows: two row blocks per wavefront up to 128 features; at 256 one (registers)
 template <int D, bool FP8>
-using Piece = Shape<D, FP8, 4, D == 256 ? 1 : 2, D == 64 ? 2 : 1>;
+using PieceOf = std::conditional_t<D == 256, Piece<D, FP8, 4, 1, 1>, Piece<D, FP8, 2, 2, 2>>;
 
 // The kernel of a call, and its items, row tiles and workspace, whatever the lengths turn out to be.
 struct Plan {
@@ -1014,9 +1226,9 @@ Plan plan_of(int64_t requests, int64_t tokens, int group, int kv_heads, int head
   Plan p;
   const int64_t rows = static_cast<int64_t>(max_seqlen) * group;
   p.few = rows <= 16 ? 1 : rows <= 32 ? 2 : 0;
-  p.rows = p.few ? 16 * p.few : Piece<64, false>::kRows;
+  p.rows = p.few ? 16 * p.few : PieceOf<64, false>::kRows;
   p.keys = p.few ? Few<64, false, 1>::kKeys
-                 : head_dim == 64 ? Piece<64, false>::kKeys : head_dim == 128 ? Piece<128, false>::kKeys : Piece<256, false>::kKeys;
+                 : head_dim == 64 ? PieceOf<64, false>::kKeys : head_dim == 128 ? PieceOf<128, false>::kKeys : PieceOf<256, false>::kKeys;
   p.workers = p.few ? 1024 : 256;
   p.min_tiles = 256 / p.keys;
   // a request's last row tile may be partly empty, its last key range too
@@ -1040,7 +1252,7 @@ template <int D, bool FP8>
 void launch_as(const PagedArgs& a, const Plan& p, hipStream_t s) {
   if (p.few == 1) launch<Few<D, false, 1>>(paged_gqa_few_kernel<Few<D, FP8, 1>>, a, p, s);
   else if (p.few == 2) launch<Few<D, false, 2>>(paged_gqa_few_kernel<Few<D, FP8, 2>>, a, p, s);
-  else launch<Piece<D, false>>(paged_gqa_kernel<Piece<D, FP8>>, a, p, s);
+  else launch<PieceOf<D, false>>(paged_gqa_piece_kernel<PieceOf<D, FP8>>, a, p, s);
 }
 
 template <int D>
