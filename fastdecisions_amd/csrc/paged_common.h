@@ -37,8 +37,8 @@ inline int fill_view(const char* what, const fd_paged_cache* c, bool needs_lens,
              "%s: the cache's dtype must be FD_DTYPE_BF16 or FD_DTYPE_E4M3", what);
   FD_REQUIRE(c->n_pages >= 1 && c->max_pages >= 1 && c->kv_heads >= 1, FD_ERR_INVALID_ARGUMENT,
              "%s: n_pages, max_pages and kv_heads must be >= 1", what);
-  FD_REQUIRE(static_cast<int64_t>(c->max_pages) * c->page_size < (1LL << 30), FD_ERR_UNSUPPORTED,
-             "%s: a request holds fewer than 2^30 keys", what);
+  FD_REQUIRE(static_cast<int64_t>(c->max_pages) * c->page_size < (1LL << 27), FD_ERR_UNSUPPORTED,
+             "%s: a request holds fewer than 2^27 keys", what);
   const bool fp8 = c->dtype == FD_DTYPE_E4M3;
   FD_REQUIRE(!fp8 || (c->k_scale && c->v_scale), FD_ERR_INVALID_ARGUMENT, "%s: an E4M3 cache needs its scales", what);
   const int64_t elem = fp8 ? 1 : 2;

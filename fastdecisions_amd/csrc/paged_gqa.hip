@@ -31,6 +31,7 @@
 namespace {
 
 constexpr int kNumXcd = 8;
+constexpr int kCus = 256;
 
 // Few rows: NR blocks of 16 rows; every wavefront stages blocks of 32 keys of its own.
 template <int D_, bool FP8_, int NR_>
@@ -90,9 +91,10 @@ struct PagedArgs {
   int64_t qs[3], gs[3], os[3];  // b, h, t
   const int32_t* cu;
   int n_req, seq_len, group, kv_heads;
-  int workers, min_tiles;       // key ranges: at least min_tiles tiles, about `workers` items
+  int slots, min_tiles, overhead;  // workgroups that run at once; tiles of a range at least, and that one costs besides
   int max_items;                // items the grid and the workspace hold
   float scale_log2;
+  int32_t* range_tiles;         // the key tiles of a range, for the joining kernel; null where nothing is split
   float* part;                  // per item: rows x D of o, then rows x 2 of (max, denominator)
 };
 
@@ -116,8 +118,65 @@ __device__ __forceinline__ int wave_scan(int v) {
   return v;
 }
 
+// p[i] for a uniform i, by a scalar load: a vector load here would make the compiler wait for
+// the copies in flight.  Nothing writes the page table while the kernel runs.
+__device__ __forceinline__ int scalar_load(const int32_t* p, int i) {
+  return reinterpret_cast<const __attribute__((address_space(4))) int32_t*>(reinterpret_cast<uintptr_t>(p))[i];
+}
+
+// An index that is the same in all lanes, in a scalar register.
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
+template <typename T>
+__device__ __forceinline__ T ceil_div(T a, T b) {
+  return (a + b - 1) / b;
+}
+
+// ceil(x / c) for x and c up to 2^22: a reciprocal whose error is put right by one step.
+__device__ __forceinline__ int tiles_over(int x, int c) {
+  const int y = x + c - 1;
+  int q = static_cast<int>(static_cast<float>(y) * __builtin_amdgcn_rcpf(static_cast<float>(c)));
+  const int r = y - q * c;
+  return q + (r >= c ? 1 : 0) - (r < 0 ? 1 : 0);
+}
+
+// The key tiles of a range, for up to 64 requests of rt row tiles and kt key tiles (a lane each) and
+// `work` tile pairs in all heads.  A range of c tiles gives sum rt ceil(kt / c) heads items; the smallest
+// c whose items fit m times the workgroups that run at once takes about m (c + overhead) tiles of time,
+// and the better of m = 1 .. kMaxRounds is taken (a few items more than workgroups would cost a whole
+// round: six suffixes, 344 items of 35 tiles on 256 CUs, 107 us, 232 of 42: see the figures below).
+constexpr int kMaxRounds = 2;
+__device__ __forceinline__ int best_range(const PagedArgs& a, int rt, int kt, int64_t work) {
+  auto items = [&](int c) { return __builtin_amdgcn_readlane(wave_scan(rt * max(tiles_over(kt, c), 1)), 63) * a.kv_heads; };
+  const float longest = fd_xor_max<32>(fd_xor_max<16>(fd_xor_max<8>(fd_xor_max<4>(fd_xor_max<2>(fd_xor_max<1>(static_cast<float>(kt)))))));
+  const int top = max(uniform(static_cast<int>(longest)) + 1, a.min_tiles);
+  int best = top, cost = 0x7fffffff;
+  for (int m = 1; m <= kMaxRounds; ++m) {
+    const int fit = m * a.slots;
+    const int64_t share = max(static_cast<int64_t>(a.min_tiles), ceil_div(work, static_cast<int64_t>(fit)));
+    if (share >= top || items(top) > fit) continue;
+    int lo = static_cast<int>(share);
+    if (items(lo) > fit) {  // items(hi) <= fit < items(lo)
+      int hi = top;
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (items(mid) > fit) lo = mid;
+        else hi = mid;
+      }
+      lo = hi;
+    }
+    const int now = m * (lo + a.overhead);
+    if (now < cost) {
+      cost = now;
+      best = lo;
+    }
+    if (lo == a.min_tiles) break;
+  }
+  return best;
+}
+
 // Finds work item `want(total items)` (JOIN: row tile, whatever its ranges).  One wavefront
-// looks at 64 requests at a time; false if there is no such item.
+// looks at 64 requests at a time; false if there is no such item.  Beyond 64 requests ranges are a round's share.
 template <int ROWS, int KEYS, bool JOIN, typename Want>
 __device__ __forceinline__ bool find_item(const PagedArgs& a, int lane, Want want, Item* it) {
   auto sizes = [&](int r, int* start, int* n_new, int* len, int* rt, int* kt) {
@@ -133,16 +192,27 @@ __device__ __forceinline__ bool find_item(const PagedArgs& a, int lane, Want wan
   };
   auto at_lane = [](int v, int l) { return __builtin_amdgcn_readlane(v, l); };
   int start, n_new, len, rt, kt;
-  int64_t work = 0;
-  for (int r0 = 0; r0 < a.n_req; r0 += 64) {
-    sizes(r0 + lane, &start, &n_new, &len, &rt, &kt);
-    const int64_t w = static_cast<int64_t>(rt) * kt;  // below 2^49: summed in two parts
-    work += at_lane(wave_scan(static_cast<int>(w & 0xffffff)), 63);
-    work += static_cast<int64_t>(at_lane(wave_scan(static_cast<int>(w >> 24)), 63)) << 24;
+  int tiles;
+  if constexpr (JOIN) {
+    tiles = scalar_load(a.range_tiles, 0);  // what the items' kernel worked with
+    if (a.n_req <= 64) sizes(lane, &start, &n_new, &len, &rt, &kt);
+  } else {
+    int64_t work = 0;
+    for (int r0 = 0; r0 < a.n_req; r0 += 64) {
+      sizes(r0 + lane, &start, &n_new, &len, &rt, &kt);
+      const int64_t w = static_cast<int64_t>(rt) * kt;  // below 2^49: summed in two parts
+      work += at_lane(wave_scan(static_cast<int>(w & 0xffffff)), 63);
+      work += static_cast<int64_t>(at_lane(wave_scan(static_cast<int>(w >> 24)), 63)) << 24;
+    }
+    if (a.n_req <= 64) {
+      tiles = best_range(a, rt, kt, work * a.kv_heads);
+    } else {
+      const int64_t share = ceil_div(work * a.kv_heads, static_cast<int64_t>(kMaxRounds * a.slots));
+      tiles = static_cast<int>(min(max(static_cast<int64_t>(a.min_tiles), share), static_cast<int64_t>(1 << 22)));
+    }
+    if (a.range_tiles != nullptr && blockIdx.x == 0 && threadIdx.x == 0) *a.range_tiles = tiles;
   }
-  const int64_t per = (work * a.kv_heads + a.workers - 1) / a.workers;
-  const int tiles = static_cast<int>(per > a.min_tiles ? per : a.min_tiles);
-  auto ranges_of = [&](int k) { return max((k + tiles - 1) / tiles, 1); };
+  auto ranges_of = [&](int k) { return max(tiles_over(k, tiles), 1); };
   int total = 0, at = 0;
   if (a.n_req > 64) {
     for (int r0 = 0; r0 < a.n_req; r0 += 64) {
@@ -176,7 +246,7 @@ __device__ __forceinline__ bool find_item(const PagedArgs& a, int lane, Want wan
       it->start = at_lane(start, l);
       it->n_new = at_lane(n_new, l);
       it->len = at_lane(len, l);
-      it->tiles = tiles;
+      it->tiles = max(ceil_div(at_lane(kt, l), it->n_ranges), 1);  // a request's ranges are alike
       it->rtile = k % it->n_rtiles;  // row tiles of a key range one after the other: they share its keys
       const int hr = k / it->n_rtiles;
       it->range = JOIN ? 0 : hr % it->n_ranges;
@@ -218,15 +288,6 @@ __device__ __forceinline__ void store4(const PagedArgs& a, const Item& it, int r
     for (int e = 0; e < 4; ++e) v[e] = v[e] / (1.0f + __expf(-g[e]));
   }
   *reinterpret_cast<bf16x4_t*>(a.o + b * a.os[0] + head * a.os[1] + t * a.os[2] + d) = __builtin_convertvector(v, bf16x4_t);
-}
-
-// An index that is the same in all lanes, in a scalar register.
-__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
-
-// p[i] for a uniform i, by a scalar load: a vector load here would make the compiler wait for
-// the copies in flight.  Nothing writes the page table while the kernel runs.
-__device__ __forceinline__ int scalar_load(const int32_t* p, int i) {
-  return reinterpret_cast<const __attribute__((address_space(4))) int32_t*>(reinterpret_cast<uintptr_t>(p))[i];
 }
 
 __device__ __forceinline__ void wait_lds_reads() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
@@ -1214,10 +1275,12 @@ __global__ __launch_bounds__(256) void paged_gqa_join_kernel(PagedArgs a) {
 template <int D, bool FP8>
 using PieceOf = std::conditional_t<D == 256, Piece<D, FP8, 4, 1, 1>, Piece<D, FP8, 2, 2, 2>>;
 
+constexpr int kHeaderBytes = 256;  // of the workspace: range_tiles
+
 // The kernel of a call, and its items, row tiles and workspace, whatever the lengths turn out to be.
 struct Plan {
   int few;  // blocks of 16 rows of the few-rows kernel, 0: pieces
-  int rows, keys, workers, min_tiles;
+  int rows, keys, slots, min_tiles;
   int64_t items, rtiles, bytes;
   bool may_split;
 };
@@ -1229,13 +1292,13 @@ Plan plan_of(int64_t requests, int64_t tokens, int group, int kv_heads, int head
   p.rows = p.few ? 16 * p.few : PieceOf<64, false>::kRows;
   p.keys = p.few ? Few<64, false, 1>::kKeys
                  : head_dim == 64 ? PieceOf<64, false>::kKeys : head_dim == 128 ? PieceOf<128, false>::kKeys : PieceOf<256, false>::kKeys;
-  p.workers = p.few ? 1024 : 256;
+  p.slots = kCus * (p.few ? 2 : 1);
   p.min_tiles = 256 / p.keys;
   // a request's last row tile may be partly empty, its last key range too
   p.rtiles = kv_heads * (tokens * group / p.rows + requests);
-  p.items = p.workers + p.rtiles;
+  p.items = kMaxRounds * p.slots + p.rtiles;
   p.may_split = max_keys > static_cast<int64_t>(p.min_tiles) * p.keys;
-  p.bytes = p.may_split ? p.items * p.rows * (head_dim + 2) * 4 : 0;
+  p.bytes = p.may_split ? kHeaderBytes + p.items * p.rows * (head_dim + 2) * 4 : 0;
   return p;
 }
 
@@ -1324,11 +1387,13 @@ extern "C" int fd_paged_gqa_fwd(const void* q, const fd_paged_cache* cache, cons
   a.seq_len = seq_len;
   a.group = q_heads / cache->kv_heads;
   a.kv_heads = cache->kv_heads;
-  a.workers = p.workers;
+  a.slots = p.slots;
   a.min_tiles = p.min_tiles;
+  a.overhead = p.few ? 2 : 4;
   a.max_items = static_cast<int>(p.items);
   a.scale_log2 = scale * 1.4426950408889634f;
-  a.part = static_cast<float*>(workspace);
+  a.range_tiles = p.may_split ? static_cast<int32_t*>(workspace) : nullptr;
+  a.part = p.may_split ? static_cast<float*>(workspace) + kHeaderBytes / 4 : nullptr;
   const bool fp8 = cache->dtype == FD_DTYPE_E4M3;
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (cache->head_dim == 64) launch_dim<64>(a, p, fp8, s);

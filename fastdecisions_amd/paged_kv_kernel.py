@@ -70,8 +70,8 @@ def check_cache(k_cache, v_cache, page_table, cache_lens, k_scale, v_scale, requ
     if (page_table.ndim != 2 or page_table.dtype != torch.int32 or page_table.device != k_cache.device
             or page_table.shape[0] != requests or page_table.shape[1] < 1 or page_table.stride(1) != 1):
         raise ValueError(f"page_table must be int32 [{requests}, max_pages] on the cache's device, its rows contiguous")
-    if page_table.shape[1] * page_size >= 1 << 30:
-        raise ValueError("A request holds fewer than 2^30 keys")
+    if page_table.shape[1] * page_size >= 1 << 27:
+        raise ValueError("A request holds fewer than 2^27 keys")
     if cache_lens is not None:
         if (cache_lens.shape != (requests,) or cache_lens.dtype != torch.int32 or cache_lens.device != k_cache.device
                 or not cache_lens.is_contiguous()):
