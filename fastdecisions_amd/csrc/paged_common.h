@@ -45,7 +45,8 @@ inline int fill_view(const char* what, const fd_paged_cache* c, bool needs_lens,
   for (const int64_t* s : {c->k_strides, c->v_strides}) {
     FD_REQUIRE(s[0] * elem % 16 == 0 && s[1] * elem % 16 == 0 && s[2] * elem % 16 == 0, FD_ERR_ALIGNMENT,
                "%s: the cache's rows must be 16-byte aligned", what);
-    FD_REQUIRE(s[2] >= 0 && s[2] < (1 << 20), FD_ERR_UNSUPPORTED, "%s: cache row strides must be in [0, 2^20)", what);
+    FD_REQUIRE(s[2] >= 0 && s[2] < (1 << 20) && s[0] >= 0 && s[0] < (1LL << 35), FD_ERR_UNSUPPORTED,
+               "%s: cache row strides must be in [0, 2^20), page strides in [0, 2^35)", what);
   }
   FD_REQUIRE(fd_aligned16(c->k) && fd_aligned16(c->v), FD_ERR_ALIGNMENT, "%s: the cache must be 16-byte aligned", what);
   auto side = [&](void* p, uint8_t* sc, const int64_t* st, const int64_t* ss) {

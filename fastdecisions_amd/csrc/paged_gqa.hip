@@ -809,67 +809,78 @@ __global__ __launch_bounds__(S::kThreads) void paged_gqa_piece_kernel(PagedArgs 
     int p[kMoves];
   };
   auto move_row = [&](int i) { return (i * S::kWaves + wave) * kMoveRows; };  // first row of move i within a tile
-  auto pages_of = [&](int t) {
+  // WHOLE: a tile of the job without absent pages that ends before kend
+  auto pages_of = [&](auto whole_c, int t) {
     Pages x;
 #pragma unroll
     for (int i = 0; i < kMoves; ++i) {
       const int key = uniform(max(min((t0 + t) * S::kKeys + move_row(i), kend - 1), 0));
       const int page = scalar_load(table, key >> a.c.shift);
-      x.p[i] = static_cast<unsigned>(page) < static_cast<unsigned>(a.c.n_pages) ? page : 0;
+      x.p[i] = decltype(whole_c)::value || static_cast<unsigned>(page) < static_cast<unsigned>(a.c.n_pages) ? page : 0;
     }
     return x;
   };
   // first row of move i of tile t on its page, and this lane's row from there
-  auto first_row = [&](int t, int i) { return uniform(min((t0 + t) * S::kKeys + move_row(i), kend - 1)) & page_mask; };
+  auto first_row = [&](auto whole_c, int t, int i) {
+    const int key = (t0 + t) * S::kKeys + move_row(i);
+    return uniform(decltype(whole_c)::value ? key : min(key, kend - 1)) & page_mask;
+  };
   auto lane_row = [&](auto whole_c, int t, int i) {
     if constexpr (decltype(whole_c)::value) return lrow;
     else return max(0, min(lrow, kend - 1 - ((t0 + t) * S::kKeys + move_row(i))));
   };
+  // K (v = 0) and V of this head; pages lie a multiple of 16 bytes apart, 32 bits of it
+  const unsigned char* const head_base[2] = {a.c.k.base + it.head * a.c.k.head, a.c.v.base + it.head * a.c.v.head};
+  const uint32_t page16[2] = {static_cast<uint32_t>(a.c.k.page >> 4), static_cast<uint32_t>(a.c.v.page >> 4)};
+  const uint32_t row_bytes[2] = {static_cast<uint32_t>(a.c.k.row), static_cast<uint32_t>(a.c.v.row)};
+  auto move_base = [&](int v, int page, int row) {
+    return head_base[v] + ((static_cast<uint64_t>(page16[v]) * static_cast<uint32_t>(page)) << 4) +
+           static_cast<uint32_t>(row) * row_bytes[v];
+  };
+  auto copy_piece = [&](auto whole_c, const Pages& pg, int t, int buf, int i, int v) {
+    const int row = move_row(i) + lrow;
+    const int chunk = (lane % CR) ^ (v ? swz_v<CR>(row) : swz_k<CR>(row));
+    copy_to_lds(move_base(v, pg.p[i], first_row(whole_c, t, i)),
+                static_cast<uint32_t>(lane_row(whole_c, t, i)) * row_bytes[v] + static_cast<uint32_t>(chunk * 16),
+                lds0 + static_cast<uint32_t>((v * S::kStages + buf) * S::kTileBytes + (i * S::kWaves + wave) * 1024));
+  };
   auto copy_tile = [&](auto whole_c, const Pages& pg, int t, int buf) {
 #pragma unroll
-    for (int v = 0; v < 2; ++v) {
-      const PagedSide& c = v ? a.c.v : a.c.k;
+    for (int i = 0; i < S::kCopies; ++i)
 #pragma unroll
-      for (int i = 0; i < S::kCopies; ++i) {
-        const unsigned char* base = c.base + pg.p[i] * c.page + it.head * c.head + first_row(t, i) * c.row;
-        const int row = move_row(i) + lrow;
-        const int chunk = (lane % CR) ^ (v ? swz_v<CR>(row) : swz_k<CR>(row));
-        copy_to_lds(base, static_cast<uint32_t>(lane_row(whole_c, t, i) * static_cast<int>(c.row) + chunk * 16),
-                    lds0 + static_cast<uint32_t>((v * S::kStages + buf) * S::kTileBytes + (i * S::kWaves + wave) * 1024));
-      }
-    }
+      for (int v = 0; v < 2; ++v) copy_piece(whole_c, pg, t, buf, i, v);
   };
   struct Codes {
     uint4 w[FP8 ? 2 * S::kLoads : 1];
     uint32_t s[FP8 ? 2 * S::kLoads : 1];
   };
+  auto load_piece = [&](auto whole_c, const Pages& pg, int t, Codes& x, int i, int v) {
+    const PagedSide& c = v ? a.c.v : a.c.k;
+    const uint32_t row = static_cast<uint32_t>(lane_row(whole_c, t, i));
+    const int first = first_row(whole_c, t, i);
+    x.w[2 * i + v] = *reinterpret_cast<const uint4*>(move_base(v, pg.p[i], first) + (row * row_bytes[v] + (lane % kLanesRow) * 16));
+    x.s[2 * i + v] = (c.scale + pg.p[i] * c.s_page + it.head * c.s_head + first)[row];
+  };
+  auto store_piece = [&](const Codes& x, int buf, int i, int v) {
+    const int row = move_row(i) + lrow;
+    const float s = scale_of(x.s[2 * i + v]);
+    unsigned char* const dst = (v ? v_lds : k_lds) + buf * S::kTileBytes + row * CR * 16;
+    const int swz = v ? swz_v<CR>(row) : swz_k<CR>(row);
+    const uint4 w = x.w[2 * i + v];
+    *reinterpret_cast<bf16x8_t*>(dst + (((lane % kLanesRow) * 2) ^ swz) * 16) = codes_to_bf16(w.x, w.y, s);
+    *reinterpret_cast<bf16x8_t*>(dst + (((lane % kLanesRow) * 2 + 1) ^ swz) * 16) = codes_to_bf16(w.z, w.w, s);
+  };
   auto load_tile = [&](auto whole_c, const Pages& pg, int t, Codes& x) {
 #pragma unroll
-    for (int i = 0; i < S::kLoads; ++i) {
-      const uint32_t row = static_cast<uint32_t>(lane_row(whole_c, t, i));
+    for (int i = 0; i < S::kLoads; ++i)
 #pragma unroll
-      for (int v = 0; v < 2; ++v) {
-        const PagedSide& c = v ? a.c.v : a.c.k;
-        const unsigned char* base = c.base + pg.p[i] * c.page + it.head * c.head + first_row(t, i) * c.row;
-        x.w[2 * i + v] = *reinterpret_cast<const uint4*>(base + (row * static_cast<uint32_t>(c.row) + (lane % kLanesRow) * 16));
-        x.s[2 * i + v] = (c.scale + pg.p[i] * c.s_page + it.head * c.s_head + first_row(t, i))[row];
-      }
-    }
+      for (int v = 0; v < 2; ++v) load_piece(whole_c, pg, t, x, i, v);
   };
   auto store_tile = [&](const Codes& x, int buf) {
 #pragma unroll
-    for (int i = 0; i < S::kLoads; ++i) {
-      const int row = move_row(i) + lrow;
+    for (int i = 0; i < S::kLoads; ++i)
 #pragma unroll
-      for (int v = 0; v < 2; ++v) {
-        const float s = scale_of(x.s[2 * i + v]);
-        unsigned char* const dst = (v ? v_lds : k_lds) + buf * S::kTileBytes + row * CR * 16;
-        const int swz = v ? swz_v<CR>(row) : swz_k<CR>(row);
-        const uint4 w = x.w[2 * i + v];
-        *reinterpret_cast<bf16x8_t*>(dst + (((lane % kLanesRow) * 2) ^ swz) * 16) = codes_to_bf16(w.x, w.y, s);
-        *reinterpret_cast<bf16x8_t*>(dst + (((lane % kLanesRow) * 2 + 1) ^ swz) * 16) = codes_to_bf16(w.z, w.w, s);
-      }
-    }
+      for (int v = 0; v < 2; ++v) store_piece(x, buf, i, v);
   };
 
   f32x16_t o[NB][kNdb];
@@ -895,7 +906,7 @@ __global__ __launch_bounds__(S::kThreads) void paged_gqa_piece_kernel(PagedArgs 
   for (int db = 0; db < kNdb; ++db) {
     const int dim = db * 32 + 16 * (grp & 1) + 4 * (li & 3);
     const int row = kp * 32 + 8 * (grp >> 1) + (li >> 2);
-    v_rd[db] = row * CR * 16 + (((dim >> 3) ^ swz_v<CR>(row)) * 16) + (dim & 7) * 2;
+    v_rd[db] = S::kStages * S::kTileBytes + row * CR * 16 + (((dim >> 3) ^ swz_v<CR>(row)) * 16) + (dim & 7) * 2;
   }
   bf16x8_t kf[kAhead];               // K operands a few MFMAs ahead
   v4i16_t vlo[kSteps], vhi[kSteps];  // V operands of a tile; MFMA i: slice i / kNdb, O block i % kNdb
@@ -903,7 +914,7 @@ __global__ __launch_bounds__(S::kThreads) void paged_gqa_piece_kernel(PagedArgs 
     kf[kk % kAhead] = *reinterpret_cast<const bf16x8_t*>(k_lds + buf * S::kTileBytes + k_rd[kk]);
   };
   auto read_v = [&](int buf, int i) {
-    const unsigned char* vt = v_lds + buf * S::kTileBytes + v_rd[i % kNdb] + (i / kNdb) * 16 * CR * 16;
+    const unsigned char* vt = smem + buf * S::kTileBytes + v_rd[i % kNdb] + (i / kNdb) * 16 * CR * 16;
     vlo[i] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16_t*)vt);
     vhi[i] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16_t*)(vt + 4 * CR * 16));
   };
@@ -928,13 +939,10 @@ __global__ __launch_bounds__(S::kThreads) void paged_gqa_piece_kernel(PagedArgs 
     }
   };
   auto head = [&](int n, int k, const f32x16_t& s) {
-    if (k == 0) {
-      mx[n] = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
+    if (k < 2) {
+      if (k == 0) mx[n] = s[0];
 #pragma unroll
-      for (int r = 4; r < 8; ++r) mx[n] = fmaxf(mx[n], s[r]);
-    } else if (k == 1) {
-#pragma unroll
-      for (int r = 8; r < 16; ++r) mx[n] = fmaxf(mx[n], s[r]);
+      for (int r = k == 0 ? 1 : 9; r < (k == 0 ? 9 : 16); ++r) mx[n] = fmaxf(mx[n], s[r]);
     } else if (k == 2) {
       mx[n] = half_max(mx[n]) * a.scale_log2;
       grow[n] = mx[n] > m_run[n] + 8.0f;
@@ -982,9 +990,9 @@ __global__ __launch_bounds__(S::kThreads) void paged_gqa_piece_kernel(PagedArgs 
     Pages next;
     // Prologue: tiles 0 and 1 landed (Q too), tile 2 on its way; scores of tile 0 and the head of its softmax.
     if constexpr (!FP8) {
-      copy_tile(whole, pages_of(0), 0, 0);
-      if (n_full > 1) copy_tile(whole, pages_of(1), 1, 1);
-      next = pages_of(2);
+      copy_tile(whole, pages_of(whole, 0), 0, 0);
+      if (n_full > 1) copy_tile(whole, pages_of(whole, 1), 1, 1);
+      next = pages_of(whole, 2);
       wait_copies<0>();
 #pragma unroll
       for (int n = 0; n < NB; ++n)
@@ -992,15 +1000,15 @@ __global__ __launch_bounds__(S::kThreads) void paged_gqa_piece_kernel(PagedArgs 
         for (int kk = 0; kk < kSteps; ++kk) asm volatile("" : "+v"(qf[n][kk]));  // the compiler's own loads end here
       if (n_full > 2) copy_tile(whole, next, 2, 2);
     } else {
-      load_tile(part, pages_of(0), 0, codes);
-      next = pages_of(1);
+      load_tile(part, pages_of(whole, 0), 0, codes);
+      next = pages_of(whole, 1);
       store_tile(codes, 0);
       load_tile(part, next, 1, codes);  // (tiles behind the last whole one may reach past kend)
-      next = pages_of(2);
+      next = pages_of(whole, 2);
       store_tile(codes, 1);
       load_tile(part, next, 2, codes);
     }
-    next = pages_of(3);
+    next = pages_of(whole, 3);
     __syncthreads();
 #pragma unroll
     for (int n = 0; n < NB; ++n) sA[n] = f32x16_t{};
@@ -1023,15 +1031,17 @@ __global__ __launch_bounds__(S::kThreads) void paged_gqa_piece_kernel(PagedArgs 
     auto step = [&](auto last_c, int t, int BUF, f32x16_t (&sc)[NB], f32x16_t (&sn)[NB]) {
       constexpr bool LAST = decltype(last_c)::value;
       const bool issued = !LAST && t + 3 < n_full;
-      if constexpr (!LAST) {
+      // the moves of a step, one behind every kMoveEvery-th score MFMA: their scalar arithmetic is issued while
+      // the matrix core works
+      constexpr int kMoveEvery = NB * kSteps / (2 * kMoves);
+      auto move_piece = [&](int u) {
         if constexpr (FP8) {
-          if (t + 2 < n_full) store_tile(codes, (BUF + 2) & 3);
-          if (issued) load_tile(whole, next, t + 3, codes);
+          if (t + 2 < n_full) store_piece(codes, (BUF + 2) & 3, u / 2, u % 2);
+          if (issued) load_piece(whole, next, t + 3, codes, u / 2, u % 2);
         } else {
-          if (issued) copy_tile(whole, next, t + 3, (BUF + 3) & 3);
+          if (issued) copy_piece(whole, next, t + 3, (BUF + 3) & 3, u / 2, u % 2);
         }
-        next = pages_of(t + 4);
-      }
+      };
       // ---- phase A
       __builtin_amdgcn_sched_barrier(0);
       if constexpr (!LAST) {
@@ -1051,6 +1061,7 @@ __global__ __launch_bounds__(S::kThreads) void paged_gqa_piece_kernel(PagedArgs 
               read_v(BUF, kk);
             }
             pieces<NB, kSteps>(kk * NB + n, [&](int u) { tail(u % NB, u / NB, sc[u % NB]); });
+            if ((kk * NB + n) % kMoveEvery == 0) move_piece((kk * NB + n) / kMoveEvery);
             __builtin_amdgcn_sched_barrier(0);
           }
         }
@@ -1070,6 +1081,7 @@ __global__ __launch_bounds__(S::kThreads) void paged_gqa_piece_kernel(PagedArgs 
         }
         wait_lds_reads();  // the V operands have arrived, their stage is free after the barrier
         __syncthreads();
+        next = pages_of(whole, t + 4);
       }
       // ---- phase B
       __builtin_amdgcn_sched_barrier(0);
@@ -1111,10 +1123,10 @@ __global__ __launch_bounds__(S::kThreads) void paged_gqa_piece_kernel(PagedArgs 
   for (int t = n_full; t < nt; ++t) {
     __syncthreads();  // every wavefront has read the tile before
     if constexpr (FP8) {
-      load_tile(part, pages_of(t), t, codes);
+      load_tile(part, pages_of(part, t), t, codes);
       store_tile(codes, 0);
     } else {
-      copy_tile(part, pages_of(t), t, 0);
+      copy_tile(part, pages_of(part, t), t, 0);
       wait_copies<0>();
     }
     __syncthreads();

@@ -50,7 +50,8 @@ FD_API const char* fd_cache_last_error(void);
  *             its keys cache_lens[r] - n .. cache_lens[r] - 1.  Not used by fd_paged_kv_read
  *
  * Limits: head_dim 64, 128 or 256; page_size a power of two in [16, 256]; cache rows and
- * tensors 16-byte aligned; row strides below 2^20 elements; max_pages * page_size < 2^27.
+ * tensors 16-byte aligned; row strides below 2^20 and page strides below 2^35 elements;
+ * max_pages * page_size < 2^27.
  */
 typedef struct fd_paged_cache {
   void* k;
