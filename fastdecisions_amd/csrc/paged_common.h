@@ -48,6 +48,9 @@ inline int fill_view(const char* what, const fd_paged_cache* c, bool needs_lens,
     FD_REQUIRE(s[2] >= 0 && s[2] < (1 << 20) && s[0] >= 0 && s[0] < (1LL << 35), FD_ERR_UNSUPPORTED,
                "%s: cache row strides must be in [0, 2^20), page strides in [0, 2^35)", what);
   }
+  FD_REQUIRE(!fp8 || (c->k_scale_strides[0] >= 0 && c->k_scale_strides[0] < (1LL << 31) && c->v_scale_strides[0] >= 0 &&
+                      c->v_scale_strides[0] < (1LL << 31)),
+             FD_ERR_UNSUPPORTED, "%s: scale page strides must be in [0, 2^31)", what);
   FD_REQUIRE(fd_aligned16(c->k) && fd_aligned16(c->v), FD_ERR_ALIGNMENT, "%s: the cache must be 16-byte aligned", what);
   auto side = [&](void* p, uint8_t* sc, const int64_t* st, const int64_t* ss) {
     return PagedSide{static_cast<unsigned char*>(p), sc, st[0] * elem, st[1] * elem, st[2] * elem, ss[0], ss[1]};

@@ -833,6 +833,8 @@ __global__ __launch_bounds__(S::kThreads) void paged_gqa_piece_kernel(PagedArgs 
   const unsigned char* const head_base[2] = {a.c.k.base + it.head * a.c.k.head, a.c.v.base + it.head * a.c.v.head};
   const uint32_t page16[2] = {static_cast<uint32_t>(a.c.k.page >> 4), static_cast<uint32_t>(a.c.v.page >> 4)};
   const uint32_t row_bytes[2] = {static_cast<uint32_t>(a.c.k.row), static_cast<uint32_t>(a.c.v.row)};
+  const uint8_t* const scale_base[2] = {a.c.k.scale + it.head * a.c.k.s_head, a.c.v.scale + it.head * a.c.v.s_head};
+  const uint32_t scale_page[2] = {static_cast<uint32_t>(a.c.k.s_page), static_cast<uint32_t>(a.c.v.s_page)};
   auto move_base = [&](int v, int page, int row) {
     return head_base[v] + ((static_cast<uint64_t>(page16[v]) * static_cast<uint32_t>(page)) << 4) +
            static_cast<uint32_t>(row) * row_bytes[v];
@@ -855,11 +857,10 @@ __global__ __launch_bounds__(S::kThreads) void paged_gqa_piece_kernel(PagedArgs 
     uint32_t s[FP8 ? 2 * S::kLoads : 1];
   };
   auto load_piece = [&](auto whole_c, const Pages& pg, int t, Codes& x, int i, int v) {
-    const PagedSide& c = v ? a.c.v : a.c.k;
     const uint32_t row = static_cast<uint32_t>(lane_row(whole_c, t, i));
     const int first = first_row(whole_c, t, i);
     x.w[2 * i + v] = *reinterpret_cast<const uint4*>(move_base(v, pg.p[i], first) + (row * row_bytes[v] + (lane % kLanesRow) * 16));
-    x.s[2 * i + v] = (c.scale + pg.p[i] * c.s_page + it.head * c.s_head + first)[row];
+    x.s[2 * i + v] = (scale_base[v] + static_cast<uint64_t>(scale_page[v]) * static_cast<uint32_t>(pg.p[i]) + first)[row];
   };
   auto store_piece = [&](const Codes& x, int buf, int i, int v) {
     const int row = move_row(i) + lrow;
@@ -1045,6 +1046,9 @@ __global__ __launch_bounds__(S::kThreads) void paged_gqa_piece_kernel(PagedArgs 
       // ---- phase A
       __builtin_amdgcn_sched_barrier(0);
       if constexpr (!LAST) {
+        // the pages are waited for here, not where they were asked for; Q stays in the accumulation half
+#pragma unroll
+        for (int i = 0; i < kMoves; ++i) asm volatile("" : "+s"(next.p[i]));
 #pragma unroll
         for (int n = 0; n < NB; ++n)
 #pragma unroll
