@@ -166,24 +166,30 @@ def recurrent_gated_delta_rule(
     if initial_state is not None and state_indices is None:
         if initial_state.shape != (n_states, Hv, Dk, Dv) or initial_state.device != value.device:
             raise ValueError(f"initial_state must be {[n_states, Hv, Dk, Dv]} on value's device")
-        if state_out is not initial_state:
+        if initial_state.dtype != torch.float32 or not initial_state.is_contiguous():
+            if state_out is initial_state:
+                raise ValueError("A state that is updated in place must be contiguous float32")
             initial_state = initial_state.to(torch.float32).contiguous()
-    if scale is None:
-        scale = 1.0 / Dk ** 0.5
-    with _lib.on_device(value.device):
-        if state_out is None:
-            if state_indices is not None:
-                state_out = initial_state
-            elif output_final_state:
-                state_out = torch.empty((n_states, Hv, Dk, Dv), device=value.device, dtype=torch.float32)
-        n_pool, indices = _cache_lib.check_states(initial_state, state_out, state_indices, n_states, (Hv, Dk, Dv),
-                                                  torch.float32, value.device)
-        out = torch.empty((B, T, Hv, Dv), device=value.device, dtype=torch.bfloat16)
-        beta_dtype = _lib.FD_DTYPE_F32 if beta.dtype == torch.float32 else _lib.FD_DTYPE_BF16
-        _cache_lib.check("fd_gated_delta_step", _cache_lib.lib().fd_gated_delta_step(
-            query.data_ptr(), key.data_ptr(), value.data_ptr(), g.data_ptr(), beta.data_ptr(), out.data_ptr(),
-            _lib.ptr(initial_state), _lib.ptr(state_out), n_pool, indices, B, T, Hk, Hv, Dk, Dv, float(scale),
-            beta_dtype, int(bool(use_qk_l2norm_in_kernel)), cu_ptr, n_seqs, _lib.stream_handle(value.device)))
+    device = value.get_device()
+    if _cache_lib.current_device() != device:
+        with torch.cuda.device(device):
+            return recurrent_gated_delta_rule(query, key, value, g, beta, initial_state, output_final_state,
+                                              use_qk_l2norm_in_kernel, scale=scale, cu_seqlens=cu_seqlens,
+                                              state_indices=state_indices, state_out=state_out)
+    if state_out is None:
+        if state_indices is not None:
+            state_out = initial_state
+        elif output_final_state:
+            state_out = torch.empty((n_states, Hv, Dk, Dv), device=value.device, dtype=torch.float32)
+    n_pool, indices = _cache_lib.check_states(initial_state, state_out, state_indices, n_states, (Hv, Dk, Dv),
+                                              torch.float32, value.device)
+    out = torch.empty_like(value)
+    beta_dtype = _lib.FD_DTYPE_F32 if beta.dtype == torch.float32 else _lib.FD_DTYPE_BF16
+    _cache_lib.check("fd_gated_delta_step", _cache_lib.lib().fd_gated_delta_step(
+        query.data_ptr(), key.data_ptr(), value.data_ptr(), g.data_ptr(), beta.data_ptr(), out.data_ptr(),
+        _lib.ptr(initial_state), _lib.ptr(state_out), n_pool, indices, B, T, Hk, Hv, Dk, Dv,
+        1.0 / Dk ** 0.5 if scale is None else float(scale), beta_dtype, int(bool(use_qk_l2norm_in_kernel)), cu_ptr,
+        n_seqs, _cache_lib.raw_stream(device)))
     return out, state_out
 
 

@@ -188,10 +188,15 @@ def prep_qkv_state(
         state_out = conv_state
     n_pool, indices = _cache_lib.check_states(conv_state, state_out, state_indices, n_seqs or B,
                                               (width - 1, input_qkv.shape[2]), torch.bfloat16, input_qkv.device)
-    with _lib.on_device(input_qkv.device):
-        q, k, v = _alloc_qkv(input_qkv, B, T, key_dim, value_dim, head_k_dim, head_v_dim)
-        _cache_lib.check("fd_packed_conv_state", _cache_lib.lib().fd_packed_conv_state(
-            input_qkv.data_ptr(), row_stride, weight.data_ptr(), _lib.ptr(bias), conv_state.data_ptr(),
-            state_out.data_ptr(), n_pool, indices, q.data_ptr(), k.data_ptr(), v.data_ptr(), B, T, key_dim, value_dim,
-            width, cu_ptr, n_seqs, _ACTIVATIONS[activation], _lib.stream_handle(input_qkv.device)))
+    device = input_qkv.get_device()
+    if _cache_lib.current_device() != device:
+        with torch.cuda.device(device):
+            return prep_qkv_state(input_qkv, weight, conv_state, bias, key_dim=key_dim, value_dim=value_dim,
+                                  head_k_dim=head_k_dim, head_v_dim=head_v_dim, activation=activation,
+                                  cu_seqlens=cu_seqlens, state_indices=state_indices, state_out=state_out)
+    q, k, v = _alloc_qkv(input_qkv, B, T, key_dim, value_dim, head_k_dim, head_v_dim)
+    _cache_lib.check("fd_packed_conv_state", _cache_lib.lib().fd_packed_conv_state(
+        input_qkv.data_ptr(), row_stride, weight.data_ptr(), _lib.ptr(bias), conv_state.data_ptr(),
+        state_out.data_ptr(), n_pool, indices, q.data_ptr(), k.data_ptr(), v.data_ptr(), B, T, key_dim, value_dim,
+        width, cu_ptr, n_seqs, _ACTIVATIONS[activation], _cache_lib.raw_stream(device)))
     return q, k, v

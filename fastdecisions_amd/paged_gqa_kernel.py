@@ -20,12 +20,22 @@ The cache's layout is described in ``paged_kv_kernel``.
 """
 from __future__ import annotations
 
-import ctypes
+from functools import lru_cache
 
 import torch
 
-from . import _cache_lib, _lib
-from .paged_kv_kernel import check_cache, check_cu_seqlens
+from . import _cache_lib
+from .paged_kv_kernel import check_cache, check_cu_seqlens, check_rows
+
+
+@lru_cache(maxsize=4096)
+def workspace_bytes(batch: int, q_heads: int, kv_heads: int, seq_len: int, head_dim: int, page_size: int,
+                    max_pages: int, n_seqs: int, max_seqlen: int) -> int:
+    """Device workspace of a call of these sizes (``fd_paged_gqa_workspace_bytes``)."""
+    nbytes = _cache_lib.lib().fd_paged_gqa_workspace_bytes(batch, q_heads, kv_heads, seq_len, head_dim, page_size,
+                                                           max_pages, n_seqs, max_seqlen)
+    _cache_lib.check("fd_paged_gqa_workspace_bytes", nbytes)
+    return nbytes
 
 
 def paged_gqa_attention(
@@ -42,44 +52,45 @@ def paged_gqa_attention(
     max_seqlen: int | None = None,
     gate: torch.Tensor | None = None,
 ) -> torch.Tensor:
-    if q.ndim != 4:
+    shape = q.shape
+    if len(shape) != 4:
         raise ValueError("Q must be four-dimensional")
-    batch, q_heads, seq_len, dim = q.shape
+    batch, q_heads, seq_len, dim = shape
     if min(batch, q_heads, seq_len) < 1:
         raise ValueError("Batch, head counts and sequence length must be positive")
-    if k_cache.ndim != 4 or q_heads % k_cache.shape[1] or dim != k_cache.shape[3]:
+    if k_cache.ndim != 4:
+        raise ValueError("k_cache and v_cache must be [n_pages, Hkv, page_size, D] of one shape")
+    _, kv_heads, page_size, cache_dim = k_cache.shape
+    if kv_heads < 1 or q_heads % kv_heads or dim != cache_dim:
         raise ValueError("Q must have the cache's head dimension and a multiple of its heads")
-    for name, t in (("Q", q), ("gate", gate)):
-        if t is None:
-            continue
-        if t.shape != q.shape or t.dtype != torch.bfloat16 or t.device != k_cache.device:
-            raise ValueError(f"{name} must be BF16, shaped like Q, on the cache's device")
-        sb, sh, st, sd = t.stride()
-        if sd != 1 or t.data_ptr() % 16 or (sb | sh | st) % 8:
-            raise ValueError(f"{name} rows must be contiguous and 16-byte aligned")
     if batch * seq_len * q_heads >= 1 << 30:
         raise ValueError("B * T * Hq must be below 2^30")
-    cu_ptr, n_seqs = check_cu_seqlens(cu_seqlens, batch, k_cache.device)
-    if max_seqlen is None or n_seqs == 0:
-        max_seqlen = seq_len
-    if not 0 <= int(max_seqlen) <= seq_len:
-        raise ValueError("max_seqlen must lie in [0, T]")
     if scale is None:
         scale = dim ** -0.5
-    if not 0.0 < scale < 1e30:
+    elif not 0.0 < scale < 1e30:
         raise ValueError("scale must be positive")
     if cache_lens is None:
         raise ValueError("cache_lens is required")
+    device = k_cache.get_device()
+    cu_ptr, n_seqs = check_cu_seqlens(cu_seqlens, batch, device)
+    if max_seqlen is None or n_seqs == 0:
+        max_seqlen = seq_len
+    elif not 0 <= int(max_seqlen) <= seq_len:
+        raise ValueError("max_seqlen must lie in [0, T]")
     cache = check_cache(k_cache, v_cache, page_table, cache_lens, k_scale, v_scale, n_seqs or batch)
-    with _lib.on_device(q.device):
-        out = torch.empty((batch, seq_len, q_heads, dim), device=q.device, dtype=q.dtype).permute(0, 2, 1, 3)
-        lib = _cache_lib.lib()
-        nbytes = lib.fd_paged_gqa_workspace_bytes(batch, q_heads, cache.kv_heads, seq_len, dim, cache.page_size,
-                                                  cache.max_pages, n_seqs, int(max_seqlen))
-        _cache_lib.check("fd_paged_gqa_workspace_bytes", nbytes)
-        work = torch.empty(nbytes, device=q.device, dtype=torch.uint8) if nbytes > 0 else None
-        _cache_lib.check("fd_paged_gqa_fwd", lib.fd_paged_gqa_fwd(
-            q.data_ptr(), ctypes.byref(cache), _lib.ptr(gate), out.data_ptr(), _lib.strides4(q),
-            None if gate is None else _lib.strides4(gate), _lib.strides4(out), batch, q_heads, seq_len, float(scale),
-            cu_ptr, n_seqs, int(max_seqlen), _lib.ptr(work), nbytes, _lib.stream_handle(q.device)))
+    q_ptr, q_strides = check_rows("Q", q, shape, device)
+    g_ptr, g_strides = (None, None) if gate is None else check_rows("gate", gate, shape, device)
+    if _cache_lib.current_device() != device:
+        with torch.cuda.device(device):
+            return paged_gqa_attention(q, k_cache, v_cache, page_table, cache_lens, k_scale=k_scale, v_scale=v_scale,
+                                       scale=scale, cu_seqlens=cu_seqlens, max_seqlen=max_seqlen, gate=gate)
+    strides = (seq_len * q_heads * dim, dim, q_heads * dim, 1)
+    out = torch.empty_strided(shape, strides, device=q.device, dtype=q.dtype)
+    nbytes = workspace_bytes(batch, q_heads, kv_heads, seq_len, dim, page_size, page_table.shape[1], n_seqs,
+                             int(max_seqlen))
+    work = torch.empty(nbytes, device=q.device, dtype=torch.uint8) if nbytes > 0 else None
+    _cache_lib.check("fd_paged_gqa_fwd", _cache_lib.lib().fd_paged_gqa_fwd(
+        q_ptr, cache, g_ptr, out.data_ptr(), q_strides, g_strides, _cache_lib.pack4(*strides), batch, q_heads, seq_len,
+        float(scale), cu_ptr, n_seqs, int(max_seqlen), None if work is None else work.data_ptr(), nbytes,
+        _cache_lib.raw_stream(device)))
     return out

@@ -232,7 +232,7 @@ def test_rows_behind_the_last_request_stay():
     q = make_q([80], 16, 128, 11)
     out = torch.full((1, 80, 16, 128), 7.0, dtype=torch.bfloat16, device="cuda").transpose(1, 2)
     cu, lens_t = ints([0, 3, 53]), ints(lens)
-    cache = check_cache(c["k"], c["v"], c["table"], lens_t, None, None, 2)
+    cache = _cache_lib.PagedCache.from_buffer_copy(check_cache(c["k"], c["v"], c["table"], lens_t, None, None, 2))
     lib = _cache_lib.lib()
     size = lib.fd_paged_gqa_workspace_bytes(1, 16, 4, 80, 128, 16, cache.max_pages, 2, 50)
     work = torch.empty(size, dtype=torch.uint8, device="cuda")
@@ -404,7 +404,7 @@ def test_read_back(heads, dim, page, fp8):
             assert torch.equal(got[0, :, at[r]:at[r] + m], want), (name, r)
             assert (got[0, :, at[r] + m:at[r + 1]] == 0).all()
     out = torch.full((total + 5, heads, dim), 3.0, dtype=torch.bfloat16, device="cuda")
-    cache = check_cache(c["k"], c["v"], c["table"], None, c["ks"], c["vs"], len(ask))
+    cache = _cache_lib.PagedCache.from_buffer_copy(check_cache(c["k"], c["v"], c["table"], None, c["ks"], c["vs"], len(ask)))
     s2 = (ctypes.c_int64 * 2)(dim, heads * dim)
     cu = ints(at)
     _cache_lib.check("fd_paged_kv_read", _cache_lib.lib().fd_paged_kv_read(
