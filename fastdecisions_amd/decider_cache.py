@@ -1,0 +1,238 @@
+"""Caches of decider requests: score many questions over one prefix, feed prompts in pieces, extend by tokens.
+
+The reference computes a shared prefix once and forks its cache per question (keys and values,
+conv state, recurrent state; ref: src/decider/shared_prefix.py:157-200).  ``DeciderCache`` holds
+the caches of up to ``requests`` requests of one model:
+
+* attention layers — a pool of pages of keys and values, bf16 or e4m3 with a power-of-two scale
+  per token and head (``paged_kv_kernel``); a request holds pages, not a range, so a fork shares
+  its parent's whole pages and copies the last, partly filled one;
+* Gated-DeltaNet layers — the conv's last inputs and the fp32 state of the delta rule, a row of a
+  pool per request.
+
+Use (``model`` with every HIP kernel installed, inference mode)::
+
+    cache = DeciderCache(model.shape, requests=64, tokens=200_000)
+    prefix = cache.open()
+    model.hidden(ids, cache=cache.step([prefix], [ids.shape[1]]))       # fill, in one or more pieces
+    forks = [cache.fork(prefix) for _ in questions]
+    step = cache.step(forks, lengths)                                   # one packed row [1, sum(lengths)]
+    logits = model(packed_ids, cache=step)
+
+A step reserves its pages and counts its tokens when it is made; run each step once, in order.
+``CacheStep.again`` makes the next step of the same shape in the same device tensors, so a
+captured forward over a step can be replayed token after token.
+"""
+from __future__ import annotations
+
+from dataclasses import dataclass, field
+
+import torch
+
+from .model import DeciderShape
+
+
+@dataclass
+class CacheStep:
+    """New tokens of some requests, packed into one row: what the cached layers need of them."""
+    cache: "DeciderCache"
+    slots: list[int]
+    new: list[int]
+    cu_seqlens: torch.Tensor      # int32 [n + 1]
+    cache_lens: torch.Tensor      # int32 [n], the new tokens included
+    state_indices: torch.Tensor   # int32 [n]
+    page_table: torch.Tensor      # int32 [n, max_pages]
+    positions: torch.Tensor       # int32 [1, total]
+    buffer: torch.Tensor = field(repr=False)
+
+    @property
+    def max_new(self) -> int:
+        return max(self.new)
+
+    @property
+    def last_rows(self) -> list[int]:
+        """Row of every request's last new token in the packed row."""
+        rows, at = [], 0
+        for n in self.new:
+            at += n
+            rows.append(at - 1)
+        return rows
+
+    def again(self) -> "CacheStep":
+        """The next step of the same requests with as many new tokens each, in the same device tensors."""
+        self.buffer.copy_(self.cache._reserve(self.slots, self.new))
+        return self
+
+
+class DeciderCache:
+    def __init__(self, shape: DeciderShape, *, requests: int, tokens: int, max_tokens: int | None = None,
+                 page_size: int = 64, kv_dtype: torch.dtype = torch.bfloat16, device="cuda"):
+        """``tokens``: cached tokens of all requests together (rounded up to pages, plus one partly filled
+        page per request); ``max_tokens``: of one request (default ``tokens``)."""
+        if requests < 1 or tokens < 1:
+            raise ValueError("requests and tokens must be positive")
+        if page_size not in (16, 32, 64, 128, 256):
+            raise ValueError("page_size must be a power of two in [16, 256]")
+        if kv_dtype not in (torch.bfloat16, torch.float8_e4m3fn):
+            raise ValueError("kv_dtype must be bfloat16 or float8_e4m3fn")
+        max_tokens = tokens if max_tokens is None else max_tokens
+        self.shape, self.page_size, self.kv_dtype, self.device = shape, page_size, kv_dtype, torch.device(device)
+        self.requests = requests
+        self.max_pages = -(-max_tokens // page_size)
+        self.n_pages = -(-tokens // page_size) + requests
+        layers = range(shape.num_hidden_layers)
+        attention = [i for i in layers if (i + 1) % shape.full_attention_interval == 0]
+        linear = [i for i in layers if (i + 1) % shape.full_attention_interval]
+        self._attention = {layer: i for i, layer in enumerate(attention)}
+        self._linear = {layer: i for i, layer in enumerate(linear)}
+        kv = (len(attention), self.n_pages, shape.num_key_value_heads, page_size, shape.head_dim)
+        self.k = torch.zeros(kv, dtype=kv_dtype, device=self.device)
+        self.v = torch.zeros_like(self.k)
+        self.k_scale = self.v_scale = None
+        if kv_dtype == torch.float8_e4m3fn:
+            self.k_scale = torch.full(kv[:4], 127, dtype=torch.uint8, device=self.device)
+            self.v_scale = self.k_scale.clone()
+        heads, dim = shape.linear_num_heads, shape.linear_head_dim
+        self.conv = torch.zeros((len(linear), requests, shape.conv_kernel - 1, 3 * heads * dim), dtype=torch.bfloat16,
+                                device=self.device)
+        self.delta = torch.zeros((len(linear), requests, heads, dim, dim), dtype=torch.float32, device=self.device)
+        self._free_slots = list(range(requests))[::-1]
+        self._free_pages = list(range(self.n_pages))[::-1]
+        self._users = [0] * self.n_pages              # requests that hold a page
+        self._pages: dict[int, list[int]] = {}        # of an open request
+        self._lens: dict[int, int] = {}
+
+    # ---- requests
+
+    def open(self) -> int:
+        """A new, empty request; its number."""
+        if not self._free_slots:
+            raise RuntimeError(f"All {self.requests} requests of the cache are open")
+        slot = self._free_slots.pop()
+        self.conv[:, slot].zero_()
+        self.delta[:, slot].zero_()
+        self._pages[slot], self._lens[slot] = [], 0
+        return slot
+
+    def fork(self, parent: int) -> int:
+        """A new request that continues where ``parent`` stands: whole pages shared, the rest copied."""
+        self._check([parent])
+        n, pages = self._lens[parent], self._pages[parent]
+        whole = n // self.page_size
+        if not self._free_slots:
+            raise RuntimeError(f"All {self.requests} requests of the cache are open")
+        if whole < len(pages) and not self._free_pages:
+            raise RuntimeError("The cache has no free page")
+        slot = self._free_slots.pop()
+        own = pages[:whole]
+        for page in own:
+            self._users[page] += 1
+        if whole < len(pages):
+            page = self._take()
+            for t in (self.k, self.v, self.k_scale, self.v_scale):
+                if t is not None:
+                    t.view(torch.uint8)[:, page] = t.view(torch.uint8)[:, pages[whole]]
+            own = own + [page]
+        self.conv[:, slot] = self.conv[:, parent]
+        self.delta[:, slot] = self.delta[:, parent]
+        self._pages[slot], self._lens[slot] = list(own), n
+        return slot
+
+    def close(self, slot: int) -> None:
+        """End a request; pages nobody else holds become free."""
+        self._check([slot])
+        for page in self._pages.pop(slot):
+            self._users[page] -= 1
+            if self._users[page] == 0:
+                self._free_pages.append(page)
+        del self._lens[slot]
+        self._free_slots.append(slot)
+
+    def length(self, slot: int) -> int:
+        self._check([slot])
+        return self._lens[slot]
+
+    # ---- steps
+
+    def step(self, slots: list[int], new: list[int]) -> CacheStep:
+        """``new[i]`` (>= 1) further tokens of request ``slots[i]``, packed in this order into one row."""
+        slots, new = list(slots), [int(n) for n in new]
+        if len(slots) != len(new) or not slots or min(new) < 1:
+            raise ValueError("A step takes one or more requests and a positive number of new tokens of each")
+        buffer = self._reserve(slots, new).to(self.device)
+        n, total = len(slots), sum(new)
+        cu, lens, idx, table, pos = buffer.split([n + 1, n, n, n * self.max_pages, total])
+        return CacheStep(self, slots, new, cu, lens, idx, table.view(n, self.max_pages), pos.view(1, total), buffer)
+
+    def _check(self, slots) -> None:
+        for slot in slots:
+            if slot not in self._lens:
+                raise ValueError(f"{slot} is no open request of the cache")
+
+    def _take(self) -> int:
+        page = self._free_pages.pop()
+        self._users[page] = 1
+        return page
+
+    def _reserve(self, slots, new) -> torch.Tensor:
+        """Pages for the new tokens; the step's device tensors as one host tensor."""
+        self._check(slots)
+        if len(set(slots)) != len(slots):
+            raise ValueError("A request appears once in a step")
+        need = []
+        for slot, n in zip(slots, new):
+            pages = -(-(self._lens[slot] + n) // self.page_size)
+            if pages > self.max_pages:
+                raise RuntimeError(f"Request {slot} would pass the cache's {self.max_pages * self.page_size} tokens per request")
+            need.append(pages - len(self._pages[slot]))
+        if sum(need) > len(self._free_pages):
+            raise RuntimeError(f"The cache has {len(self._free_pages)} free pages, the step needs {sum(need)}")
+        cu, lens, table, pos = [0], [], [], []
+        for slot, n, pages in zip(slots, new, need):
+            held = self._lens[slot]
+            self._pages[slot] += [self._take() for _ in range(pages)]
+            self._lens[slot] = held + n
+            cu.append(cu[-1] + n)
+            lens.append(held + n)
+            table += self._pages[slot] + [-1] * (self.max_pages - len(self._pages[slot]))
+            pos += range(held, held + n)
+        return torch.tensor(cu + lens + list(slots) + table + pos, dtype=torch.int32)
+
+    # ---- what the layers see
+
+    def attention_layer(self, layer: int):
+        """(k, v, k_scale, v_scale) of an attention layer's cache."""
+        i = self._attention[layer]
+        scales = (None, None) if self.k_scale is None else (self.k_scale[i], self.v_scale[i])
+        return self.k[i], self.v[i], *scales
+
+    def linear_layer(self, layer: int):
+        """(conv state pool, delta state pool) of a Gated-DeltaNet layer."""
+        i = self._linear[layer]
+        return self.conv[i], self.delta[i]
+
+    def read(self, slot: int, layer: int):
+        """Keys and values [1, Hkv, length, D] (bf16) that an attention layer has cached of a request."""
+        from .cached_ops import paged_kv_read_op
+        self._check([slot])
+        n, pages = self._lens[slot], self._pages[slot]
+        k, v, k_scale, v_scale = self.attention_layer(layer)
+        table = torch.tensor([pages or [-1]], dtype=torch.int32).to(self.device)
+        cu = torch.tensor([0, n], dtype=torch.int32).to(self.device)
+        return paged_kv_read_op(k, v, table, cu, n, k_scale, v_scale)
+
+
+def cached_layers_ready(core) -> bool:
+    """True when every layer's cached forward can run: attention and Gated-DeltaNet patched, the delta
+    rule's heads 128 wide."""
+    for layer in core.layers:
+        attention, linear = getattr(layer, "self_attn", None), getattr(layer, "linear_attn", None)
+        if attention is not None and not (hasattr(attention, "_native_gqa_original_forward")
+                                          and attention.head_dim in (64, 128, 256)):
+            return False
+        if linear is not None and not (
+                hasattr(linear, "_packed_original_forward") and getattr(linear, "_fd_gated_delta", False)
+                and linear.key_dim == linear.value_dim and linear.head_k_dim == linear.head_v_dim == 128
+                and linear.conv1d.bias is None and linear.activation == "silu" and 2 <= linear.conv_kernel_size <= 4):
+            return False
+    return True

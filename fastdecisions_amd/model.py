@@ -91,15 +91,27 @@ class DeciderModel(nn.Module):
 
     def hidden(self, ids: torch.Tensor, *, cu_seqlens: torch.Tensor | None = None,
                segments: list[tuple[int, int]] | None = None, max_seqlen: int | None = None,
-               final_norm: bool = True) -> torch.Tensor:
+               final_norm: bool = True, cache=None) -> torch.Tensor:
         """Final normed hidden states [B, T, H] (the residual stream before the final
         norm with ``final_norm=False``).  For packed requests pass ``cu_seqlens``
-        (device int32), ``segments`` (host (start, end) pairs) and ``max_seqlen``."""
+        (device int32), ``segments`` (host (start, end) pairs) and ``max_seqlen``.
+        With ``cache`` (a ``CacheStep`` of a ``DeciderCache``) ids [1, total] are the step's new
+        tokens, which continue its requests; it needs every HIP kernel installed."""
         core = self.core
         h = core.embed_tokens(ids)
         B, T = ids.shape
         kwargs = {}
-        if cu_seqlens is None:
+        if cache is not None:
+            from .decider_cache import cached_layers_ready
+            from .persistent_residual_rms import chain_ready
+            if cu_seqlens is not None or ids.shape != cache.positions.shape:
+                raise ValueError(f"A step's ids are [1, {cache.positions.shape[1]}], without cu_seqlens")
+            if not (chain_ready(core, h) and cached_layers_ready(core)):
+                raise RuntimeError("The cached forward needs every HIP kernel (install_hip_kernels(model)), bf16 "
+                                   "weights on the GPU and no gradients")
+            pos = cache.positions
+            kwargs = dict(fd_cache=cache)
+        elif cu_seqlens is None:
             pos = torch.arange(T, device=ids.device)[None].expand(B, T)
         else:
             if B != 1 or segments is None or max_seqlen is None:

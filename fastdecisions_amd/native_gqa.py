@@ -116,6 +116,38 @@ def _fused_forward(self, hidden_states, position_embeddings, cu_seqlens, max_seq
     return self.o_proj(out.transpose(1, 2).reshape(*shape, -1)), None
 
 
+def _cached_forward(self, hidden_states, position_embeddings, step):
+    """The attention layer over a paged cache: ``hidden_states`` [1, total, hidden] are the step's new tokens,
+    whose keys and values are written before the attention reads everything their requests hold."""
+    from .cached_ops import paged_gqa_op, paged_kv_write_op
+    shape = hidden_states.shape[:-1]
+    d = self.head_dim
+    if hasattr(self, "_fd_qkv_weight"):
+        proj = F.linear(hidden_states, self._fd_qkv_weight)
+        nq, nk = self.q_proj.weight.shape[0], self.k_proj.weight.shape[0]
+        qg, kp, v = proj[..., :nq], proj[..., nq:nq + nk], proj[..., nq + nk:]
+    else:
+        qg, kp, v = self.q_proj(hidden_states), self.k_proj(hidden_states), self.v_proj(hidden_states)
+    qg = qg.view(*shape, -1, 2 * d)  # per head: query | gate
+    kp = kp.view(*shape, -1, d)
+    v = v.view(*shape, -1, d).transpose(1, 2)
+    if getattr(self, "_fd_attn_fused", False) and _fusable(self, position_embeddings):
+        cos, sin = position_embeddings
+        q, k = attn_prologue(qg[..., :d], kp, self.q_norm.weight, self.k_norm.weight, cos.contiguous(),
+                             sin.contiguous(), float(self.q_norm.eps))
+        q, k = q.transpose(1, 2), k.transpose(1, 2)
+    else:
+        from transformers.models.qwen3_5.modeling_qwen3_5 import apply_rotary_pos_emb
+        q = self.q_norm(qg[..., :d].contiguous()).transpose(1, 2)
+        k = self.k_norm(kp.contiguous()).transpose(1, 2)
+        q, k = (t.contiguous() for t in apply_rotary_pos_emb(q, k, *position_embeddings))
+    k_cache, v_cache, k_scale, v_scale = step.cache.attention_layer(self.layer_idx)
+    paged_kv_write_op(k, v, k_cache, v_cache, step.page_table, step.cache_lens, k_scale, v_scale, step.cu_seqlens)
+    out = paged_gqa_op(q, k_cache, v_cache, step.page_table, step.cache_lens, k_scale, v_scale,
+                       qg[..., d:].transpose(1, 2), step.cu_seqlens, step.max_new)
+    return self.o_proj(out.transpose(1, 2).reshape(*shape, -1)), None
+
+
 def plain_causal(mask, t: int) -> bool:
     """True when ``mask`` adds nothing to the in-kernel causal mask over ``t`` tokens: None, a boolean
     mask equal to the lower triangle, or an additive mask that is 0 on and below the diagonal and
@@ -142,7 +174,10 @@ def candidate_forward(self, hidden_states, position_embeddings, attention_mask=N
     (ref: experiments/native_gqa/bench_native_gqa_model.py:43-56).  The causal
     mask is applied in-kernel, so the kernel runs only when ``attention_mask`` adds
     nothing to it (``plain_causal``); any other mask (padding, segments, a bias)
-    runs the original forward, which applies it."""
+    runs the original forward, which applies it.  With ``fd_cache`` (a ``CacheStep``) the tokens continue
+    requests of a ``DeciderCache``."""
+    if kwargs.get("fd_cache") is not None:
+        return _cached_forward(self, hidden_states, position_embeddings, kwargs["fd_cache"])
     if (past_key_values is not None or self.training or torch.is_grad_enabled()
             or not hidden_states.is_cuda or hidden_states.dtype != torch.bfloat16
             or self.head_dim not in (64, 128, 256)
