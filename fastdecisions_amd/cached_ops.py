@@ -1,4 +1,4 @@
-"""Torch ops of the cache operators: one node each under ``torch.compile``, capturable in a HIP graph.
+"""Torch ops of the cache operators (``fastdecisions_cache::``): one node each under ``torch.compile``, capturable in a HIP graph.
 
 They wrap ``paged_kv_write``, ``paged_kv_read`` (``paged_kv_kernel``), ``paged_gqa_attention``
 (``paged_gqa_kernel``), ``prep_qkv_state`` (``packed_conv_kernel``) and
@@ -16,7 +16,7 @@ from .paged_gqa_kernel import paged_gqa_attention
 from .paged_kv_kernel import paged_kv_read, paged_kv_write
 
 
-@torch.library.custom_op("fastdecisions::paged_kv_write", mutates_args=("k_cache", "v_cache", "k_scale", "v_scale"),
+@torch.library.custom_op("fastdecisions_cache::paged_kv_write", mutates_args=("k_cache", "v_cache", "k_scale", "v_scale"),
                          device_types="cuda")
 def paged_kv_write_op(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
                       page_table: torch.Tensor, cache_lens: torch.Tensor, k_scale: Optional[torch.Tensor],
@@ -30,7 +30,7 @@ def _paged_kv_write_fake(key, value, k_cache, v_cache, page_table, cache_lens, k
     return None
 
 
-@torch.library.custom_op("fastdecisions::paged_kv_read", mutates_args=(), device_types="cuda")
+@torch.library.custom_op("fastdecisions_cache::paged_kv_read", mutates_args=(), device_types="cuda")
 def paged_kv_read_op(k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor, cu_seqlens: torch.Tensor,
                      total: int, k_scale: Optional[torch.Tensor],
                      v_scale: Optional[torch.Tensor]) -> tuple[torch.Tensor, torch.Tensor]:
@@ -43,7 +43,7 @@ def _paged_kv_read_fake(k_cache, v_cache, page_table, cu_seqlens, total, k_scale
     return tuple(k_cache.new_empty((1, total, h, d), dtype=torch.bfloat16).transpose(1, 2) for _ in range(2))
 
 
-@torch.library.custom_op("fastdecisions::paged_gqa", mutates_args=(), device_types="cuda")
+@torch.library.custom_op("fastdecisions_cache::paged_gqa", mutates_args=(), device_types="cuda")
 def paged_gqa_op(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor,
                  cache_lens: torch.Tensor, k_scale: Optional[torch.Tensor], v_scale: Optional[torch.Tensor],
                  gate: Optional[torch.Tensor], cu_seqlens: Optional[torch.Tensor], max_seqlen: int) -> torch.Tensor:
@@ -57,7 +57,7 @@ def _paged_gqa_fake(q, k_cache, v_cache, page_table, cache_lens, k_scale, v_scal
     return q.new_empty((b, t, h, d)).permute(0, 2, 1, 3)
 
 
-@torch.library.custom_op("fastdecisions::packed_conv_state", mutates_args=("conv_state",), device_types="cuda")
+@torch.library.custom_op("fastdecisions_cache::packed_conv_state", mutates_args=("conv_state",), device_types="cuda")
 def packed_conv_state_op(x: torch.Tensor, weight: torch.Tensor, conv_state: torch.Tensor,
                          cu_seqlens: Optional[torch.Tensor],
                          state_indices: Optional[torch.Tensor]) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
@@ -71,7 +71,7 @@ def _packed_conv_state_fake(x, weight, conv_state, cu_seqlens, state_indices):
     return tuple(x.new_empty(shape) for _ in range(3))
 
 
-@torch.library.custom_op("fastdecisions::gated_delta_step", mutates_args=("state",), device_types="cuda")
+@torch.library.custom_op("fastdecisions_cache::gated_delta_step", mutates_args=("state",), device_types="cuda")
 def gated_delta_step_op(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tensor, beta: torch.Tensor,
                         state: torch.Tensor, cu_seqlens: Optional[torch.Tensor],
                         state_indices: torch.Tensor) -> torch.Tensor:
