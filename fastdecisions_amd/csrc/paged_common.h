@@ -3,22 +3,18 @@
 #pragma once
 
 #include "../../include/fd_cache.h"
-#include <initializer_list>
-
 #include "fd_common.h"
 
 namespace {
 
-// One of K and V as the kernels see it.
-struct PagedSide {
-  unsigned char* base;
-  uint8_t* scale;
+// A cache as the kernels see it: K and V (and their scales) lie at the same offsets of two pools.
+struct PagedView {
+  unsigned char* k;
+  unsigned char* v;
+  uint8_t* k_scale;
+  uint8_t* v_scale;
   int64_t page, head, row;      // strides in bytes
   int64_t s_page, s_head;
-};
-
-struct PagedView {
-  PagedSide k, v;
   const int32_t* table;
   const int32_t* lens;
   int64_t table_stride;
@@ -42,21 +38,27 @@ inline int fill_view(const char* what, const fd_paged_cache* c, bool needs_lens,
   const bool fp8 = c->dtype == FD_DTYPE_E4M3;
   FD_REQUIRE(!fp8 || (c->k_scale && c->v_scale), FD_ERR_INVALID_ARGUMENT, "%s: an E4M3 cache needs its scales", what);
   const int64_t elem = fp8 ? 1 : 2;
-  for (const int64_t* s : {c->k_strides, c->v_strides}) {
-    FD_REQUIRE(s[0] * elem % 16 == 0 && s[1] * elem % 16 == 0 && s[2] * elem % 16 == 0, FD_ERR_ALIGNMENT,
-               "%s: the cache's rows must be 16-byte aligned", what);
-    FD_REQUIRE(s[2] >= 0 && s[2] < (1 << 20) && s[0] >= 0 && s[0] < (1LL << 35), FD_ERR_UNSUPPORTED,
-               "%s: cache row strides must be in [0, 2^20), page strides in [0, 2^35)", what);
-  }
-  FD_REQUIRE(!fp8 || (c->k_scale_strides[0] >= 0 && c->k_scale_strides[0] < (1LL << 31) && c->v_scale_strides[0] >= 0 &&
-                      c->v_scale_strides[0] < (1LL << 31)),
-             FD_ERR_UNSUPPORTED, "%s: scale page strides must be in [0, 2^31)", what);
+  const int64_t* st = c->k_strides;
+  const int64_t* ss = c->k_scale_strides;
+  FD_REQUIRE(st[0] == c->v_strides[0] && st[1] == c->v_strides[1] && st[2] == c->v_strides[2] &&
+                 (!fp8 || (ss[0] == c->v_scale_strides[0] && ss[1] == c->v_scale_strides[1])),
+             FD_ERR_UNSUPPORTED, "%s: the strides of K and V must be the same", what);
+  FD_REQUIRE(st[0] * elem % 16 == 0 && st[1] * elem % 16 == 0 && st[2] * elem % 16 == 0, FD_ERR_ALIGNMENT,
+             "%s: the cache's rows must be 16-byte aligned", what);
+  FD_REQUIRE(st[2] >= 0 && st[2] < (1 << 20) && st[0] >= 0 && st[0] < (1LL << 35), FD_ERR_UNSUPPORTED,
+             "%s: cache row strides must be in [0, 2^20), page strides in [0, 2^35)", what);
+  FD_REQUIRE(!fp8 || (ss[0] >= 0 && ss[0] < (1LL << 31)), FD_ERR_UNSUPPORTED,
+             "%s: scale page strides must be in [0, 2^31)", what);
   FD_REQUIRE(fd_aligned16(c->k) && fd_aligned16(c->v), FD_ERR_ALIGNMENT, "%s: the cache must be 16-byte aligned", what);
-  auto side = [&](void* p, uint8_t* sc, const int64_t* st, const int64_t* ss) {
-    return PagedSide{static_cast<unsigned char*>(p), sc, st[0] * elem, st[1] * elem, st[2] * elem, ss[0], ss[1]};
-  };
-  out->k = side(c->k, c->k_scale, c->k_strides, c->k_scale_strides);
-  out->v = side(c->v, c->v_scale, c->v_strides, c->v_scale_strides);
+  out->k = static_cast<unsigned char*>(c->k);
+  out->v = static_cast<unsigned char*>(c->v);
+  out->k_scale = c->k_scale;
+  out->v_scale = c->v_scale;
+  out->page = st[0] * elem;
+  out->head = st[1] * elem;
+  out->row = st[2] * elem;
+  out->s_page = ss[0];
+  out->s_head = ss[1];
   out->table = c->page_table;
   out->lens = c->cache_lens;
   out->table_stride = c->table_stride;

@@ -120,8 +120,12 @@ __device__ __forceinline__ int wave_scan(int v) {
 
 // p[i] for a uniform i, by a scalar load: a vector load here would make the compiler wait for
 // the copies in flight.  Nothing writes the page table while the kernel runs.
+// i is not negative and 4 i fits 32 bits.
 __device__ __forceinline__ int scalar_load(const int32_t* p, int i) {
-  return reinterpret_cast<const __attribute__((address_space(4))) int32_t*>(reinterpret_cast<uintptr_t>(p))[i];
+  typedef const __attribute__((address_space(4))) char const_char;
+  typedef const __attribute__((address_space(4))) int32_t const_i32;
+  const uint32_t at = static_cast<uint32_t>(i) * 4u;
+  return *reinterpret_cast<const_i32*>(reinterpret_cast<const_char*>(reinterpret_cast<uintptr_t>(p)) + at);
 }
 
 // An index that is the same in all lanes, in a scalar register.
@@ -170,7 +174,7 @@ __device__ __forceinline__ int best_range(const PagedArgs& a, int rt, int kt, in
       cost = now;
       best = lo;
     }
-    if (lo == a.min_tiles) break;
+    if (lo == a.min_tiles || 8 * lo <= 9 * share) break;  // one round within an eighth of an even share: no better two
   }
   return best;
 }
@@ -470,32 +474,39 @@ __global__ __launch_bounds__(S::kThreads, S::kPerCu) void paged_gqa_few_kernel(P
   const unsigned char* const stage0 = smem + wave * NS * S::kStageBytes;
   const int page_mask = (1 << a.c.shift) - 1;
   constexpr int kChunks = RBY / 16;
-  auto copy_side = [&](const PagedSide& c, const Pages& pg, int j, uint32_t lds, bool is_v) {
+  const unsigned char* const head_base[2] = {a.c.k + it.head * a.c.head, a.c.v + it.head * a.c.head};
+  auto copy_side = [&](const Pages& pg, int j, int v) {
     const int kb0 = first + j * S::kKeys;
+    const uint32_t lds = lds0 + static_cast<uint32_t>((j & (NS - 1)) * S::kStageBytes + v * S::kBlockBytes);
 #pragma unroll
     for (int i = 0; i < S::kCopies; ++i) {
       const int row = i * S::kCopyRows + lane / kChunks;
-      const int page = pg.p[i * S::kCopyRows / 16];
-      const unsigned char* base = c.base + page * c.page + it.head * c.head;
-      const int chunk = (lane % kChunks) ^ (is_v ? few_swz_v<RBY, FP8>(row) : few_swz_k<RBY>(row));
+      const int chunk = (lane % kChunks) ^ (v ? few_swz_v<RBY, FP8>(row) : few_swz_k<RBY>(row));
       const int key = min(kb0 + row, kend - 1) & page_mask;
-      copy_to_lds(base, static_cast<uint32_t>(key * static_cast<int>(c.row) + chunk * 16), lds + static_cast<uint32_t>(i * 1024));
+      copy_to_lds(head_base[v] + pg.p[i * S::kCopyRows / 16] * a.c.page,
+                  static_cast<uint32_t>(key * static_cast<int>(a.c.row) + chunk * 16), lds + static_cast<uint32_t>(i * 1024));
     }
   };
   auto copy_k = [&](const Pages& pg, int j) {
-    const uint32_t lds = lds0 + static_cast<uint32_t>((j & (NS - 1)) * S::kStageBytes);
-    copy_side(a.c.k, pg, j, lds, false);
+    copy_side(pg, j, 0);
     if constexpr (FP8) {
       const int row = lane & 31;
       const int key = min(first + j * S::kKeys + row, kend - 1) & page_mask;
       const int page = row < 16 ? pg.p[0] : pg.p[1];
-      const PagedSide& c = lane < 32 ? a.c.k : a.c.v;
-      byte_to_lds(c.scale + page * c.s_page + it.head * c.s_head + key, lds + 2 * S::kBlockBytes);
+      byte_to_lds((lane < 32 ? a.c.k_scale : a.c.v_scale) + page * a.c.s_page + it.head * a.c.s_head + key,
+                  lds0 + static_cast<uint32_t>((j & (NS - 1)) * S::kStageBytes + 2 * S::kBlockBytes));
     }
   };
-  auto copy_v = [&](const Pages& pg, int j) {
-    copy_side(a.c.v, pg, j, lds0 + static_cast<uint32_t>((j & (NS - 1)) * S::kStageBytes + S::kBlockBytes), true);
-  };
+  auto copy_v = [&](const Pages& pg, int j) { copy_side(pg, j, 1); };
+  // the first blocks leave at once; Q and the table are loaded behind them
+#pragma unroll
+  for (int j = 0; j < NS; ++j) {
+    if (j < mine) {
+      const Pages pg = pages_of(j);
+      copy_k(pg, j);
+      copy_v(pg, j);
+    }
+  }
 
   // ---- this lane's rows (li of each block of 16)
   int pos[NR];
@@ -681,14 +692,6 @@ __global__ __launch_bounds__(S::kThreads, S::kPerCu) void paged_gqa_few_kernel(P
 
   // ---- the loop: copies in the queue, oldest first, at block j's scores: K(j) V(j) .. K(j + NS - 1) V(j + NS - 1)
   constexpr int kBoth = S::kKGroup + S::kCopies;
-#pragma unroll
-  for (int j = 0; j < NS; ++j) {
-    if (j < mine) {
-      const Pages pg = pages_of(j);
-      copy_k(pg, j);
-      copy_v(pg, j);
-    }
-  }
   Pages next = pages_of(NS);
   for (int j = 0; j < mine; ++j) {
     const bool more = j + NS < mine;
@@ -809,13 +812,14 @@ __global__ __launch_bounds__(S::kThreads) void paged_gqa_piece_kernel(PagedArgs 
     int p[kMoves];
   };
   auto move_row = [&](int i) { return (i * S::kWaves + wave) * kMoveRows; };  // first row of move i within a tile
-  // WHOLE: a tile of the job without absent pages that ends before kend
+  // whole: tiles of [0, n_full), all of whose pages are there
   auto pages_of = [&](auto whole_c, int t) {
     Pages x;
+    const int first = (t0 + (decltype(whole_c)::value ? min(t, n_full - 1) : t)) * S::kKeys;
 #pragma unroll
     for (int i = 0; i < kMoves; ++i) {
-      const int key = uniform(max(min((t0 + t) * S::kKeys + move_row(i), kend - 1), 0));
-      const int page = scalar_load(table, key >> a.c.shift);
+      const int key = first + move_row(i);
+      const int page = scalar_load(table, uniform(decltype(whole_c)::value ? key : max(min(key, kend - 1), 0)) >> a.c.shift);
       x.p[i] = decltype(whole_c)::value || static_cast<unsigned>(page) < static_cast<unsigned>(a.c.n_pages) ? page : 0;
     }
     return x;
@@ -829,21 +833,18 @@ __global__ __launch_bounds__(S::kThreads) void paged_gqa_piece_kernel(PagedArgs 
     if constexpr (decltype(whole_c)::value) return lrow;
     else return max(0, min(lrow, kend - 1 - ((t0 + t) * S::kKeys + move_row(i))));
   };
-  // K (v = 0) and V of this head; pages lie a multiple of 16 bytes apart, 32 bits of it
-  const unsigned char* const head_base[2] = {a.c.k.base + it.head * a.c.k.head, a.c.v.base + it.head * a.c.v.head};
-  const uint32_t page16[2] = {static_cast<uint32_t>(a.c.k.page >> 4), static_cast<uint32_t>(a.c.v.page >> 4)};
-  const uint32_t row_bytes[2] = {static_cast<uint32_t>(a.c.k.row), static_cast<uint32_t>(a.c.v.row)};
-  const uint8_t* const scale_base[2] = {a.c.k.scale + it.head * a.c.k.s_head, a.c.v.scale + it.head * a.c.v.s_head};
-  const uint32_t scale_page[2] = {static_cast<uint32_t>(a.c.k.s_page), static_cast<uint32_t>(a.c.v.s_page)};
-  auto move_base = [&](int v, int page, int row) {
-    return head_base[v] + ((static_cast<uint64_t>(page16[v]) * static_cast<uint32_t>(page)) << 4) +
-           static_cast<uint32_t>(row) * row_bytes[v];
+  // K (v = 0) and V of this head, at one offset; pages lie a multiple of 16 bytes apart, 32 bits of it
+  const unsigned char* const head_base[2] = {a.c.k + it.head * a.c.head, a.c.v + it.head * a.c.head};
+  const uint32_t page16 = static_cast<uint32_t>(a.c.page >> 4), row_bytes = static_cast<uint32_t>(a.c.row);
+  const uint8_t* const scale_base[2] = {a.c.k_scale + it.head * a.c.s_head, a.c.v_scale + it.head * a.c.s_head};
+  auto move_offset = [&](int page, int row) {
+    return ((static_cast<uint64_t>(page16) * static_cast<uint32_t>(page)) << 4) + static_cast<uint32_t>(row) * row_bytes;
   };
   auto copy_piece = [&](auto whole_c, const Pages& pg, int t, int buf, int i, int v) {
     const int row = move_row(i) + lrow;
     const int chunk = (lane % CR) ^ (v ? swz_v<CR>(row) : swz_k<CR>(row));
-    copy_to_lds(move_base(v, pg.p[i], first_row(whole_c, t, i)),
-                static_cast<uint32_t>(lane_row(whole_c, t, i)) * row_bytes[v] + static_cast<uint32_t>(chunk * 16),
+    copy_to_lds(head_base[v] + move_offset(pg.p[i], first_row(whole_c, t, i)),
+                static_cast<uint32_t>(lane_row(whole_c, t, i)) * row_bytes + static_cast<uint32_t>(chunk * 16),
                 lds0 + static_cast<uint32_t>((v * S::kStages + buf) * S::kTileBytes + (i * S::kWaves + wave) * 1024));
   };
   auto copy_tile = [&](auto whole_c, const Pages& pg, int t, int buf) {
@@ -859,8 +860,8 @@ __global__ __launch_bounds__(S::kThreads) void paged_gqa_piece_kernel(PagedArgs 
   auto load_piece = [&](auto whole_c, const Pages& pg, int t, Codes& x, int i, int v) {
     const uint32_t row = static_cast<uint32_t>(lane_row(whole_c, t, i));
     const int first = first_row(whole_c, t, i);
-    x.w[2 * i + v] = *reinterpret_cast<const uint4*>(move_base(v, pg.p[i], first) + (row * row_bytes[v] + (lane % kLanesRow) * 16));
-    x.s[2 * i + v] = (scale_base[v] + static_cast<uint64_t>(scale_page[v]) * static_cast<uint32_t>(pg.p[i]) + first)[row];
+    x.w[2 * i + v] = *reinterpret_cast<const uint4*>(head_base[v] + move_offset(pg.p[i], first) + (row * row_bytes + (lane % kLanesRow) * 16));
+    x.s[2 * i + v] = (scale_base[v] + static_cast<uint64_t>(static_cast<uint32_t>(a.c.s_page)) * static_cast<uint32_t>(pg.p[i]) + first)[row];
   };
   auto store_piece = [&](const Codes& x, int buf, int i, int v) {
     const int row = move_row(i) + lrow;

@@ -86,9 +86,8 @@ __global__ __launch_bounds__(kThreads) void paged_kv_write_kernel(WriteArgs a) {
     if (pos >= 0 && pos < len) page = a.c.table[r * a.c.table_stride + (pos >> a.c.shift)];
   }
   live = static_cast<unsigned>(page) < static_cast<unsigned>(a.c.n_pages);
-  const PagedSide& c = side == 0 ? a.c.k : a.c.v;
   const int at = pos & ((1 << a.c.shift) - 1);
-  unsigned char* dst = c.base + page * c.page + head * c.head + at * c.row;
+  unsigned char* dst = (side == 0 ? a.c.k : a.c.v) + page * a.c.page + head * a.c.head + at * a.c.row;
   if constexpr (!FP8) {
     if (live) *reinterpret_cast<uint4*>(dst + li * 16) = w;
   } else {
@@ -119,7 +118,7 @@ __global__ __launch_bounds__(kThreads) void paged_kv_write_kernel(WriteArgs a) {
     code.y = static_cast<uint32_t>(hi);
     if (live) {
       *reinterpret_cast<uint2*>(dst + li * 8) = code;
-      if (li == 0) c.scale[page * c.s_page + head * c.s_head + at] = static_cast<uint8_t>(byte);
+      if (li == 0) (side == 0 ? a.c.k_scale : a.c.v_scale)[page * a.c.s_page + head * a.c.s_head + at] = static_cast<uint8_t>(byte);
     }
   }
 }
@@ -147,15 +146,14 @@ __global__ __launch_bounds__(kThreads) void paged_kv_read_kernel(ReadArgs a) {
   const int key = static_cast<int>(t) - max(a.cu[r], 0);
   const int slot = key >> a.c.shift, at = key & ((1 << a.c.shift) - 1);
   const int page = slot < a.c.max_pages ? a.c.table[r * a.c.table_stride + slot] : -1;
-  const PagedSide& c = side == 0 ? a.c.k : a.c.v;
   uint4 w = {0, 0, 0, 0};
   if (static_cast<unsigned>(page) < static_cast<unsigned>(a.c.n_pages)) {
-    const unsigned char* src = c.base + page * c.page + head * c.head + at * c.row;
+    const unsigned char* src = (side == 0 ? a.c.k : a.c.v) + page * a.c.page + head * a.c.head + at * a.c.row;
     if constexpr (!FP8) {
       w = *reinterpret_cast<const uint4*>(src + li * 16);
     } else {
       const uint2 code = *reinterpret_cast<const uint2*>(src + li * 8);
-      const float s = scale_of(c.scale[page * c.s_page + head * c.s_head + at]);
+      const float s = scale_of((side == 0 ? a.c.k_scale : a.c.v_scale)[page * a.c.s_page + head * a.c.s_head + at]);
       typedef float f32x2_t __attribute__((ext_vector_type(2)));
       const f32x2_t f0 = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(code.x), false);
       const f32x2_t f1 = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(code.x), true);

@@ -5,7 +5,7 @@ forks it per question (ref: src/decider/shared_prefix.py); here a cache is a poo
 pages that requests hold through a page table:
 
 * ``k_cache``, ``v_cache`` — logical ``[n_pages, Hkv, page_size, D]`` (any strides with a
-  contiguous feature dimension), bf16 or ``torch.float8_e4m3fn``; D 64, 128 or 256,
+  contiguous feature dimension, the same for both), bf16 or ``torch.float8_e4m3fn``; D 64, 128 or 256,
   page_size a power of two in [16, 256];
 * ``k_scale``, ``v_scale`` — for an e4m3 cache, uint8 ``[n_pages, Hkv, page_size]``: byte b
   stands for 2^(b - 127), and a cached value is its code times that;
@@ -54,19 +54,21 @@ def check_cache(k_cache, v_cache, page_table, cache_lens, k_scale, v_scale, requ
         raise ValueError("The cache needs at least one page and one head")
     fp8 = dtype == _E4M3
     k_ptr, v_ptr = k_cache.data_ptr(), v_cache.data_ptr()
-    kp, kh, kr, kd = k_cache.stride()
-    vp, vh, vr, vd = v_cache.stride()
-    if (kd != 1 or vd != 1 or (k_ptr | v_ptr) % 16 or (kp | kh | kr | vp | vh | vr) % (16 if fp8 else 8)
-            or max(kr, vr) >= 1 << 20):
+    strides = k_cache.stride()
+    if v_cache.stride() != strides:
+        raise ValueError("k_cache and v_cache must have the same strides")
+    sp, sh, sr, sd = strides
+    if sd != 1 or (k_ptr | v_ptr) % 16 or (sp | sh | sr) % (16 if fp8 else 8) or sr >= 1 << 20:
         raise ValueError("Cache rows must be contiguous and 16-byte aligned")
-    ks = vs = ksp = ksh = vsp = vsh = 0
+    ks = vs = ssp = ssh = 0
     if fp8:
         for t in (k_scale, v_scale):
             if (t is None or t.shape != shape[:3] or t.dtype != _UINT8 or t.get_device() != device or t.stride(2) != 1):
                 raise ValueError("An e4m3 cache needs k_scale and v_scale: uint8 [n_pages, Hkv, page_size] on its device")
         ks, vs = k_scale.data_ptr(), v_scale.data_ptr()
-        ksp, ksh, _ = k_scale.stride()
-        vsp, vsh, _ = v_scale.stride()
+        if v_scale.stride() != k_scale.stride():
+            raise ValueError("k_scale and v_scale must have the same strides")
+        ssp, ssh, _ = k_scale.stride()
     elif k_scale is not None or v_scale is not None:
         raise ValueError("A BF16 cache has no scales")
     max_pages = page_table.shape[-1]
@@ -82,7 +84,7 @@ def check_cache(k_cache, v_cache, page_table, cache_lens, k_scale, v_scale, requ
                 or not cache_lens.is_contiguous()):
             raise ValueError(f"cache_lens must be a contiguous int32 vector [{requests}] on the cache's device")
         lens = cache_lens.data_ptr()
-    return _cache_lib.pack_cache(k_ptr, v_ptr, ks, vs, kp, kh, kr, vp, vh, vr, ksp, ksh, vsp, vsh, page_table.data_ptr(),
+    return _cache_lib.pack_cache(k_ptr, v_ptr, ks, vs, sp, sh, sr, sp, sh, sr, ssp, ssh, ssp, ssh, page_table.data_ptr(),
                                  table_stride[0], lens, n_pages, page_size, max_pages, heads, dim,
                                  _cache_lib.FD_DTYPE_E4M3 if fp8 else _lib.FD_DTYPE_BF16)
 

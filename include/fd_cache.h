@@ -38,7 +38,7 @@ FD_API const char* fd_cache_last_error(void);
  * A paged key/value cache and the requests' view of it.
  *
  *   k, v      [n_pages, kv_heads, page_size, head_dim] of dtype (FD_DTYPE_BF16 or FD_DTYPE_E4M3);
- *             strides {page, head, row} in elements, head_dim contiguous
+ *             strides {page, head, row} in elements, head_dim contiguous; those of k and v the same
  *   k_scale, v_scale  with FD_DTYPE_E4M3: [n_pages, kv_heads, page_size] bytes, strides {page, head},
  *             rows contiguous; byte b stands for the scale 2^(b - 127), b in [1, 254], and a cached
  *             value is its code times that scale.  NULL with FD_DTYPE_BF16

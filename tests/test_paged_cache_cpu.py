@@ -59,8 +59,12 @@ def cache(**kw):
     (dict(page_size=48), "UNSUPPORTED"), (dict(page_size=512), "UNSUPPORTED"), (dict(dtype=7), "INVALID_ARGUMENT"),
     (dict(dtype=2), "INVALID_ARGUMENT"), (dict(n_pages=0), "INVALID_ARGUMENT"), (dict(max_pages=0), "INVALID_ARGUMENT"),
     (dict(max_pages=1 << 27), "UNSUPPORTED"), (dict(k=FAKE + 8), "ALIGNMENT"),
-    (dict(k_strides=(ctypes.c_int64 * 3)(4, 16 * 128, 128)), "ALIGNMENT"),
-    (dict(v_strides=(ctypes.c_int64 * 3)(8192, 2048, 1 << 20)), "UNSUPPORTED")])
+    (dict(k_strides=(ctypes.c_int64 * 3)(4, 16 * 128, 128), v_strides=(ctypes.c_int64 * 3)(4, 16 * 128, 128)), "ALIGNMENT"),
+    (dict(k_strides=(ctypes.c_int64 * 3)(8192, 2048, 1 << 20), v_strides=(ctypes.c_int64 * 3)(8192, 2048, 1 << 20)),
+     "UNSUPPORTED"),
+    (dict(k_strides=(ctypes.c_int64 * 3)(1 << 35, 2048, 128), v_strides=(ctypes.c_int64 * 3)(1 << 35, 2048, 128)),
+     "UNSUPPORTED"),
+    (dict(v_strides=(ctypes.c_int64 * 3)(8192, 2048, 256)), "UNSUPPORTED")])
 def test_a_bad_cache_is_refused(change, code):
     lib = _cache_lib.lib()
     want = getattr(_lib, "FD_ERR_" + code)
