@@ -94,7 +94,7 @@ struct PagedArgs {
   int slots, min_tiles, overhead;  // workgroups that run at once; tiles of a range at least, and that one costs besides
   int max_items;                // items the grid and the workspace hold
   float scale_log2;
-  int32_t* range_tiles;         // the key tiles of a range, for the joining kernel; null where nothing is split
+  int32_t* range_tiles;         // the key tiles of a range, for the joining kernel; null where nothing can be split
   float* part;                  // per item: rows x D of o, then rows x 2 of (max, denominator)
 };
 
@@ -198,7 +198,8 @@ __device__ __forceinline__ bool find_item(const PagedArgs& a, int lane, Want wan
   int start, n_new, len, rt, kt;
   int tiles;
   if constexpr (JOIN) {
-    tiles = scalar_load(a.range_tiles, 0);  // what the items' kernel worked with
+    tiles = scalar_load(a.range_tiles, 0);  // what the items' kernel worked with, 0: it split nothing
+    if (tiles == 0) return false;
     if (a.n_req <= 64) sizes(lane, &start, &n_new, &len, &rt, &kt);
   } else {
     int64_t work = 0;
@@ -214,7 +215,14 @@ __device__ __forceinline__ bool find_item(const PagedArgs& a, int lane, Want wan
       const int64_t share = ceil_div(work * a.kv_heads, static_cast<int64_t>(kMaxRounds * a.slots));
       tiles = static_cast<int>(min(max(static_cast<int64_t>(a.min_tiles), share), static_cast<int64_t>(1 << 22)));
     }
-    if (a.range_tiles != nullptr && blockIdx.x == 0 && threadIdx.x == 0) *a.range_tiles = tiles;
+    if (a.range_tiles != nullptr && blockIdx.x == 0) {
+      bool split = false;
+      for (int r0 = 0; r0 < a.n_req; r0 += 64) {
+        if (a.n_req > 64) sizes(r0 + lane, &start, &n_new, &len, &rt, &kt);
+        split |= __builtin_amdgcn_ballot_w64(kt > tiles) != 0;
+      }
+      if (threadIdx.x == 0) *a.range_tiles = split ? tiles : 0;
+    }
   }
   auto ranges_of = [&](int k) { return max(tiles_over(k, tiles), 1); };
   int total = 0, at = 0;
@@ -775,7 +783,7 @@ __global__ __launch_bounds__(S::kThreads) void paged_gqa_piece_kernel(PagedArgs 
   Job job;
   if (!open_job<S>(a, lane, &job)) return;
   const Item& it = job.it;
-  const int kend = job.kend, t0 = job.t0, nt = job.nt;
+  const int kend = job.kend, t0 = uniform(job.t0), nt = uniform(job.nt);
 
   // ---- this lane's rows: col of each of the wavefront's row blocks
   int pos[NB];
@@ -796,7 +804,7 @@ __global__ __launch_bounds__(S::kThreads) void paged_gqa_piece_kernel(PagedArgs 
   const bool absent = any_absent<S>(a, job, table, lane);
   // tiles [0, n_full) of the job are seen whole by every row of the workgroup
   const int pos_first = uniform(it.len - it.n_new + it.row0 / a.group);
-  const int n_full = absent ? 0 : max(0, min(nt, (pos_first + 1) / S::kKeys - t0));
+  const int n_full = uniform(absent ? 0 : max(0, min(nt, (pos_first + 1) / S::kKeys - t0)));
 
   // ---- staging.  The kMoveRows rows of a copy (or load) lie on one page: its address is a scalar base plus
   // a lane offset that depends on no tile.  Tiles that reach past kend repeat row kend - 1 there (the mask
@@ -987,6 +995,18 @@ __global__ __launch_bounds__(S::kThreads) void paged_gqa_piece_kernel(PagedArgs 
   const std::true_type whole{};
   const std::false_type part{};
   Codes codes;
+  // The tiles behind the whole ones go to stage t % 4 too; the first of them (three, or one of codes) leave
+  // before the pipelined loop's last step.
+  constexpr int kAheadTiles = 3;
+  auto ahead = [&]() {
+    if constexpr (FP8) {
+      if (n_full < nt) load_tile(part, pages_of(part, n_full), n_full, codes);
+    } else {
+#pragma unroll
+      for (int u = 0; u < kAheadTiles; ++u)
+        if (n_full + u < nt) copy_tile(part, pages_of(part, n_full + u), n_full + u, (n_full + u) & 3);
+    }
+  };
   if (n_full > 0) {
     f32x16_t sA[NB], sB[NB];
     Pages next;
@@ -1120,21 +1140,29 @@ __global__ __launch_bounds__(S::kThreads) void paged_gqa_piece_kernel(PagedArgs 
 #pragma unroll
       for (int n = 0; n < NB; ++n) sA[n] = sB[n];
     }
+    ahead();  // every stage but tile n1's is free since the last barrier
     step(last, n1, n1 & 3, sA, sB);
+  } else {
+    ahead();
   }
 
-  // ---- the other tiles, one at a time: copied, masked, and with values of masked keys kept out
+  // ---- the other tiles: masked, and with values of masked keys kept out
 #pragma unroll 1
   for (int t = n_full; t < nt; ++t) {
-    __syncthreads();  // every wavefront has read the tile before
+    const bool early = t < n_full + kAheadTiles;  // copied ahead
+    const int buf = FP8 || early ? t & 3 : 0;
     if constexpr (FP8) {
-      load_tile(part, pages_of(part, t), t, codes);
-      store_tile(codes, 0);
-    } else {
-      copy_tile(part, pages_of(part, t), t, 0);
+      store_tile(codes, buf);  // (the stages being read are those of tiles t - 1 and earlier)
+      if (t + 1 < nt) load_tile(part, pages_of(part, t + 1), t + 1, codes);
+      __syncthreads();
+    } else if (!early || t == n_full) {
+      if (!early) {
+        __syncthreads();  // every wavefront has read the tile before
+        copy_tile(part, pages_of(part, t), t, 0);
+      }
       wait_copies<0>();
+      __syncthreads();
     }
-    __syncthreads();
     const int kb0 = (t0 + t) * S::kKeys + kp * 32;
     bool there[2] = {true, true};
     if (absent) {
@@ -1149,7 +1177,7 @@ __global__ __launch_bounds__(S::kThreads) void paged_gqa_piece_kernel(PagedArgs 
     for (int n = 0; n < NB; ++n) s[n] = f32x16_t{};
 #pragma unroll
     for (int kk = 0; kk < kSteps; ++kk) {
-      read_k(0, kk);
+      read_k(buf, kk);
 #pragma unroll
       for (int n = 0; n < NB; ++n) s[n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[kk % kAhead], qf[n][kk], s[n], 0, 0, 0);
     }
@@ -1169,7 +1197,7 @@ __global__ __launch_bounds__(S::kThreads) void paged_gqa_piece_kernel(PagedArgs 
 #pragma unroll
     for (int i = 0; i < kSteps; ++i) {
       const int j = i / kNdb, db = i % kNdb;
-      read_v(0, i);
+      read_v(buf, i);
       bf16x8_t vf = v_operand(i);  // V[key 16 j + 8 half + e][32 db + col]
       typedef short i16x8_t __attribute__((ext_vector_type(8)));
       typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
