@@ -31,7 +31,7 @@
 namespace {
 
 constexpr int kNumXcd = 8;
-constexpr int kCus = 256;
+constexpr int kCus = 256;  // a power of two (slots_log2)
 
 // Few rows: NR blocks of 16 rows; every wavefront stages blocks of 32 keys of its own.
 template <int D_, bool FP8_, int NR_>
@@ -91,7 +91,8 @@ struct PagedArgs {
   int64_t qs[3], gs[3], os[3];  // b, h, t
   const int32_t* cu;
   int n_req, seq_len, group, kv_heads;
-  int slots, min_tiles, overhead;  // workgroups that run at once; tiles of a range at least, and that one costs besides
+  uint32_t group_magic;         // ceil(2^24 / group)
+  int slots_log2, min_tiles, overhead;  // workgroups that run at once; tiles of a range at least, and that one costs besides
   int max_items;                // items the grid and the workspace hold
   float scale_log2;
   int32_t* range_tiles;         // the key tiles of a range, for the joining kernel; null where nothing can be split
@@ -102,6 +103,7 @@ struct PagedArgs {
 struct Item {
   int req, head, rtile, range;
   int row0, rows;               // first row of the tile, rows of the request
+  int token0, rem0;             // row0 / group and row0 % group
   int start, n_new, len;        // new tokens on the T axis, keys
   int tiles;                    // key tiles of a range
   int base, n_rtiles, n_ranges; // first item of the request; its row tiles and key ranges
@@ -131,11 +133,6 @@ __device__ __forceinline__ int scalar_load(const int32_t* p, int i) {
 // An index that is the same in all lanes, in a scalar register.
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
-template <typename T>
-__device__ __forceinline__ T ceil_div(T a, T b) {
-  return (a + b - 1) / b;
-}
-
 // ceil(x / c) for x and c up to 2^22: a reciprocal whose error is put right by one step.
 __device__ __forceinline__ int tiles_over(int x, int c) {
   const int y = x + c - 1;
@@ -150,14 +147,15 @@ __device__ __forceinline__ int tiles_over(int x, int c) {
 // and the better of m = 1 .. kMaxRounds is taken (a few items more than workgroups would cost a whole
 // round: six suffixes, 344 items of 35 tiles on 256 CUs, 107 us, 232 of 42: see the figures below).
 constexpr int kMaxRounds = 2;
+static_assert(kMaxRounds == 2, "m << slots_log2 and >> (slots_log2 + m - 1) are the same for m = 1 and 2");
 __device__ __forceinline__ int best_range(const PagedArgs& a, int rt, int kt, int64_t work) {
   auto items = [&](int c) { return __builtin_amdgcn_readlane(wave_scan(rt * max(tiles_over(kt, c), 1)), 63) * a.kv_heads; };
   const float longest = fd_xor_max<32>(fd_xor_max<16>(fd_xor_max<8>(fd_xor_max<4>(fd_xor_max<2>(fd_xor_max<1>(static_cast<float>(kt)))))));
   const int top = max(uniform(static_cast<int>(longest)) + 1, a.min_tiles);
   int best = top, cost = 0x7fffffff;
   for (int m = 1; m <= kMaxRounds; ++m) {
-    const int fit = m * a.slots;
-    const int64_t share = max(static_cast<int64_t>(a.min_tiles), ceil_div(work, static_cast<int64_t>(fit)));
+    const int fit = m << a.slots_log2;
+    const int64_t share = max(static_cast<int64_t>(a.min_tiles), (work + fit - 1) >> (a.slots_log2 + m - 1));
     if (share >= top || items(top) > fit) continue;
     int lo = static_cast<int>(share);
     if (items(lo) > fit) {  // items(hi) <= fit < items(lo)
@@ -212,7 +210,8 @@ __device__ __forceinline__ bool find_item(const PagedArgs& a, int lane, Want wan
     if (a.n_req <= 64) {
       tiles = best_range(a, rt, kt, work * a.kv_heads);
     } else {
-      const int64_t share = ceil_div(work * a.kv_heads, static_cast<int64_t>(kMaxRounds * a.slots));
+      const int log2 = a.slots_log2 + 1;  // of kMaxRounds rounds
+      const int64_t share = (work * a.kv_heads + (1LL << log2) - 1) >> log2;
       tiles = static_cast<int>(min(max(static_cast<int64_t>(a.min_tiles), share), static_cast<int64_t>(1 << 22)));
     }
     if (a.range_tiles != nullptr && blockIdx.x == 0) {
@@ -258,13 +257,15 @@ __device__ __forceinline__ bool find_item(const PagedArgs& a, int lane, Want wan
       it->start = at_lane(start, l);
       it->n_new = at_lane(n_new, l);
       it->len = at_lane(len, l);
-      it->tiles = max(ceil_div(at_lane(kt, l), it->n_ranges), 1);  // a request's ranges are alike
+      it->tiles = max(tiles_over(at_lane(kt, l), it->n_ranges), 1);  // a request's ranges are alike
       it->rtile = k % it->n_rtiles;  // row tiles of a key range one after the other: they share its keys
       const int hr = k / it->n_rtiles;
       it->range = JOIN ? 0 : hr % it->n_ranges;
       it->head = JOIN ? hr : hr / it->n_ranges;
       it->row0 = it->rtile * ROWS;
       it->rows = it->n_new * a.group;
+      it->token0 = it->row0 / a.group;
+      it->rem0 = it->row0 - it->token0 * a.group;
       return true;
     }
     before += at_lane(incl, 63);
@@ -273,11 +274,16 @@ __device__ __forceinline__ bool find_item(const PagedArgs& a, int lane, Want wan
   return false;
 }
 
+// Token (from the tile's first one on) of row `row` of a tile: (rem0 + row) / group, below 2^24 / group.
+__device__ __forceinline__ int token_of(const PagedArgs& a, const Item& it, int row) {
+  return static_cast<int>((static_cast<uint32_t>(it.rem0 + row) * a.group_magic) >> 24);
+}
+
 // Keys that the last row of the tile sees (the tile's keys).
 template <int ROWS>
 __device__ __forceinline__ int keys_of_tile(const PagedArgs& a, const Item& it) {
-  const int last = min(it.row0 + ROWS, it.rows) - 1;
-  return max(0, min(it.len, it.len - it.n_new + last / a.group + 1));
+  const int last = min(ROWS, it.rows - it.row0) - 1;
+  return max(0, min(it.len, it.len - it.n_new + it.token0 + token_of(a, it, last) + 1));
 }
 
 template <int ROWS>
@@ -287,11 +293,10 @@ __device__ __forceinline__ int64_t part_floats(int D) {
 
 // out = acc * inv (* sigmoid(gate)), four features of a row.
 __device__ __forceinline__ void store4(const PagedArgs& a, const Item& it, int row, int d, f32x4_t acc, float inv) {
-  const int p = it.row0 + row;
-  const int token = p / a.group;
-  const int head = it.head * a.group + (p - token * a.group);
+  const int local = token_of(a, it, row);
+  const int head = it.head * a.group + (it.rem0 + row - local * a.group);
   const int b = a.cu == nullptr ? it.req : 0;
-  const int64_t t = it.start + token;
+  const int64_t t = it.start + it.token0 + local;
   f32x4_t v = acc * inv;
   if (a.gate != nullptr) {
     const bf16x4_t g4 = *reinterpret_cast<const bf16x4_t*>(a.gate + b * a.gs[0] + head * a.gs[1] + t * a.gs[2] + d);
@@ -329,6 +334,7 @@ __device__ __forceinline__ bool open_job(const PagedArgs& a, int lane, Job* j) {
   it.row0 = uniform(it.row0), it.rows = uniform(it.rows), it.start = uniform(it.start), it.n_new = uniform(it.n_new);
   it.len = uniform(it.len), it.tiles = uniform(it.tiles), it.base = uniform(it.base);
   it.n_rtiles = uniform(it.n_rtiles), it.n_ranges = uniform(it.n_ranges);
+  it.token0 = uniform(it.token0), it.rem0 = uniform(it.rem0);
   j->it = it;
   j->kend = uniform(keys_of_tile<S::kRows>(a, it));
   const int nt_all = (j->kend + S::kKeys - 1) / S::kKeys;
@@ -428,10 +434,37 @@ __device__ __forceinline__ float sum8(bf16x8_t p, float x) {
   return x;
 }
 
-// Half-word i (uniform) of four words.
-__device__ __forceinline__ uint32_t half_of(uint32_t a, uint32_t b, uint32_t c, uint32_t d, int i) {
-  const uint32_t w = i < 2 ? a : i < 4 ? b : i < 6 ? c : d;
-  return (i & 1) ? w >> 16 : w & 0xffffu;
+// Infinities and NaN ("odd" values) among V's operands: are there any, the operand without them, element i
+// (uniform) of one, and o + p x for the odd ones of four values x that a row sees (p is not 0).
+__device__ __forceinline__ bool any_odd(bf16x8_t v) {
+  typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
+  const u32x4_t w = __builtin_bit_cast(u32x4_t, v);
+  bool odd = false;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) odd |= (w[i] & 0x7f80u) == 0x7f80u || (w[i] & 0x7f800000u) == 0x7f800000u;
+  return odd;
+}
+__device__ __forceinline__ bf16x8_t without_odd(bf16x8_t v) {
+  typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
+  u32x4_t w = __builtin_bit_cast(u32x4_t, v);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if ((w[i] & 0x7f80u) == 0x7f80u) w[i] &= 0xffff0000u;
+    if ((w[i] & 0x7f800000u) == 0x7f800000u) w[i] &= 0xffffu;
+  }
+  return __builtin_bit_cast(bf16x8_t, w);
+}
+__device__ __forceinline__ float element(bf16x8_t v, int i) {
+  typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
+  const u32x4_t w = __builtin_bit_cast(u32x4_t, v);
+  const uint32_t pair = i < 2 ? w[0] : i < 4 ? w[1] : i < 6 ? w[2] : w[3];
+  return fd_bf16_to_f32((i & 1) ? pair >> 16 : pair & 0xffffu);
+}
+__device__ __forceinline__ f32x4_t add_odd(f32x4_t o, f32x4_t x, float p) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (!(fabsf(x[e]) < __builtin_inff()) && p != 0.0f) o[e] += p * x[e];
+  return o;
 }
 
 // One byte per lane, zero-extended, to a word of LDS at lds + 4 * lane.
@@ -521,16 +554,16 @@ __global__ __launch_bounds__(S::kThreads, S::kPerCu) void paged_gqa_few_kernel(P
   bf16x8_t qf[NR][kKk];
 #pragma unroll
   for (int n = 0; n < NR; ++n) {
-    const int p = min(it.row0 + n * 16 + li, it.rows - 1);  // rows behind the last one repeat it and are not stored
-    const int token = p / a.group;
+    const int row = min(n * 16 + li, it.rows - it.row0 - 1);  // rows behind the last one repeat it and are not stored
+    const int local = token_of(a, it, row), token = it.token0 + local;
     pos[n] = it.len - it.n_new + token;
     const int b = a.cu == nullptr ? it.req : 0;
-    const int head = it.head * a.group + (p - token * a.group);
+    const int head = it.head * a.group + (it.rem0 + row - local * a.group);
     const uint16_t* qp = a.q + b * a.qs[0] + head * a.qs[1] + static_cast<int64_t>(it.start + token) * a.qs[2] + grp * 8;
 #pragma unroll
     for (int kk = 0; kk < kKk; ++kk) qf[n][kk] = *reinterpret_cast<const bf16x8_t*>(qp + kk * 32);
   }
-  const int pos_min = uniform(it.len - it.n_new + it.row0 / a.group);
+  const int pos_min = it.len - it.n_new + it.token0;
   const bool absent = any_absent<S>(a, job, table, lane);
 
   f32x4_t o[NR][kNdb];
@@ -638,64 +671,60 @@ __global__ __launch_bounds__(S::kThreads, S::kPerCu) void paged_gqa_few_kernel(P
 
   auto p_v = [&](int j) {
     const unsigned char* const st = stage0 + (j & (NS - 1)) * S::kStageBytes + S::kBlockBytes;
-    // a block with masked keys: their values must not reach a row as 0 * NaN or 0 * inf
-    const bool guard = first + j * S::kKeys + 31 > pos_min || absent;
+    bf16x8_t vf[kNdb];  // V[key 8 grp + i][16 db + li]
 #pragma unroll
     for (int db = 0; db < kNdb; ++db) {
-      bf16x8_t vf;  // V[key 8 grp + i][16 db + li]
       if constexpr (FP8) {
         typedef int v2i_t __attribute__((ext_vector_type(2)));
         typedef __attribute__((address_space(3))) v2i_t lds_v2i_t;
         const int row = 8 * grp + (li >> 1);
         const v2i_t w = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
             (lds_v2i_t*)(st + row * RBY + (db ^ few_swz_v<RBY, true>(row)) * 16 + 8 * (li & 1)));
-        vf = codes_to_bf16(static_cast<uint32_t>(w[0]), static_cast<uint32_t>(w[1]));
+        vf[db] = codes_to_bf16(static_cast<uint32_t>(w[0]), static_cast<uint32_t>(w[1]));
       } else {
         const int row = 8 * grp + (li >> 2);
         const unsigned char* vp = st + row * RBY + ((2 * db + ((li & 3) >> 1)) ^ few_swz_v<RBY, false>(row)) * 16 + 8 * (li & 1);
         const v4i16_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16_t*)vp);
         const v4i16_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16_t*)(vp + 4 * RBY));
         const short __attribute__((ext_vector_type(8))) vv = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-        vf = __builtin_bit_cast(bf16x8_t, vv);
+        vf[db] = __builtin_bit_cast(bf16x8_t, vv);
       }
-      if (guard) {
-        typedef short i16x8_t __attribute__((ext_vector_type(8)));
-        i16x8_t e = __builtin_bit_cast(i16x8_t, vf);
-        bool odd = false;
+    }
+    // a block with masked keys: their values must not reach a row as 0 * NaN or 0 * inf
+    if (first + j * S::kKeys + 31 > pos_min || absent) {
+      bool odd = false;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) odd |= (e[i] & 0x7f80) == 0x7f80;
-        if (__builtin_amdgcn_ballot_w64(odd) != 0) {
-          // infinities and NaN leave the product and are added by hand to the rows that see them
-          typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
-          const u32x4_t ew = __builtin_bit_cast(u32x4_t, vf);
+      for (int db = 0; db < kNdb; ++db) odd |= any_odd(vf[db]);
+      if (__builtin_amdgcn_ballot_w64(odd) != 0) {
+        // Infinities and NaN leave the product and are added by hand to the rows that see them: o[n][db][r]
+        // is feature 16 db + 4 grp + r of this lane's row.
+#pragma unroll
+        for (int db = 0; db < kNdb; ++db) vf[db] = without_odd(vf[db]);
 #pragma unroll 1
-          for (int i = 0; i < 8; ++i) {
-            const uint32_t bits = half_of(ew[0], ew[1], ew[2], ew[3], i);
-            const float x = (bits & 0x7f80u) == 0x7f80u ? fd_bf16_to_f32(bits) : 0.0f;
+        for (int key = 0; key < 32; ++key) {
+          float ph[NR];
 #pragma unroll
-            for (int n = 0; n < NR; ++n) {
-              const u32x4_t pw = __builtin_bit_cast(u32x4_t, pb[n]);
-              const float pi = fd_bf16_to_f32(half_of(pw[0], pw[1], pw[2], pw[3], i));
-#pragma unroll 1
-              for (int g = 0; g < 4; ++g) {
-                const float pg = __shfl(pi, 16 * g + li);  // this lane's row, key 8 g + i
+          for (int n = 0; n < NR; ++n) ph[n] = __shfl(element(pb[n], key & 7), 16 * (key >> 3) + li);
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                  const float xd = __shfl(x, 16 * g + 4 * grp + r);  // feature of o[n][db][r]
-                  if (xd != 0.0f && pg != 0.0f) o[n][db][r] += pg * xd;
-                }
-              }
+          for (int db = 0; db < kNdb; ++db) {
+            f32x4_t x;
+            if constexpr (FP8) {
+              const uint32_t w = *reinterpret_cast<const uint32_t*>(st + key * RBY + (db ^ few_swz_v<RBY, true>(key)) * 16 + 4 * grp);
+              x = __builtin_convertvector(__builtin_shufflevector(codes_to_bf16(w, w), bf16x8_t{}, 0, 1, 2, 3), f32x4_t);
+            } else {
+              x = __builtin_convertvector(*reinterpret_cast<const bf16x4_t*>(
+                  st + key * RBY + ((2 * db + (grp >> 1)) ^ few_swz_v<RBY, false>(key)) * 16 + 8 * (grp & 1)), f32x4_t);
             }
-          }
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
-            if ((e[i] & 0x7f80) == 0x7f80) e[i] = 0;
-          vf = __builtin_bit_cast(bf16x8_t, e);
+            for (int n = 0; n < NR; ++n) o[n][db] = add_odd(o[n][db], x, ph[n]);
+          }
         }
       }
-#pragma unroll
-      for (int n = 0; n < NR; ++n) o[n][db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pb[n], o[n][db], 0, 0, 0);
     }
+#pragma unroll
+    for (int db = 0; db < kNdb; ++db)
+#pragma unroll
+      for (int n = 0; n < NR; ++n) o[n][db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf[db], pb[n], o[n][db], 0, 0, 0);
   };
 
   // ---- the loop: copies in the queue, oldest first, at block j's scores: K(j) V(j) .. K(j + NS - 1) V(j + NS - 1)
@@ -790,11 +819,11 @@ __global__ __launch_bounds__(S::kThreads) void paged_gqa_piece_kernel(PagedArgs 
   bf16x8_t qf[NB][kSteps];
 #pragma unroll
   for (int n = 0; n < NB; ++n) {
-    const int p = min(it.row0 + (rw * NB + n) * 32 + col, it.rows - 1);  // rows behind the last repeat it, not stored
-    const int token = p / a.group;
+    const int row = min((rw * NB + n) * 32 + col, it.rows - it.row0 - 1);  // rows behind the last repeat it, not stored
+    const int local = token_of(a, it, row), token = it.token0 + local;
     pos[n] = it.len - it.n_new + token;
     const int b = a.cu == nullptr ? it.req : 0;
-    const int head = it.head * a.group + (p - token * a.group);
+    const int head = it.head * a.group + (it.rem0 + row - local * a.group);
     const uint16_t* qp = a.q + b * a.qs[0] + head * a.qs[1] + static_cast<int64_t>(it.start + token) * a.qs[2] + half * 8;
 #pragma unroll
     for (int kk = 0; kk < kSteps; ++kk) qf[n][kk] = *reinterpret_cast<const bf16x8_t*>(qp + kk * 16);
@@ -803,7 +832,7 @@ __global__ __launch_bounds__(S::kThreads) void paged_gqa_piece_kernel(PagedArgs 
   const int page_mask = (1 << a.c.shift) - 1;
   const bool absent = any_absent<S>(a, job, table, lane);
   // tiles [0, n_full) of the job are seen whole by every row of the workgroup
-  const int pos_first = uniform(it.len - it.n_new + it.row0 / a.group);
+  const int pos_first = it.len - it.n_new + it.token0;
   const int n_full = uniform(absent ? 0 : max(0, min(nt, (pos_first + 1) / S::kKeys - t0)));
 
   // ---- staging.  The kMoveRows rows of a copy (or load) lie on one page: its address is a scalar base plus
@@ -1199,23 +1228,15 @@ __global__ __launch_bounds__(S::kThreads) void paged_gqa_piece_kernel(PagedArgs 
       const int j = i / kNdb, db = i % kNdb;
       read_v(buf, i);
       bf16x8_t vf = v_operand(i);  // V[key 16 j + 8 half + e][32 db + col]
-      typedef short i16x8_t __attribute__((ext_vector_type(8)));
-      typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
-      i16x8_t e = __builtin_bit_cast(i16x8_t, vf);
-      bool odd = false;
-#pragma unroll
-      for (int u = 0; u < 8; ++u) odd |= (e[u] & 0x7f80) == 0x7f80;
-      if (__builtin_amdgcn_ballot_w64(odd) != 0) {
+      if (__builtin_amdgcn_ballot_w64(any_odd(vf)) != 0) {
         // infinities and NaN leave the product (0 times one is NaN) and are added by hand to the rows that see them
-        const u32x4_t ew = __builtin_bit_cast(u32x4_t, vf);
 #pragma unroll 1
         for (int u = 0; u < 8; ++u) {
-          const uint32_t bits = half_of(ew[0], ew[1], ew[2], ew[3], u);
-          const float x = (bits & 0x7f80u) == 0x7f80u ? fd_bf16_to_f32(bits) : 0.0f;
+          const float v = element(vf, u);
+          const float x = fabsf(v) < __builtin_inff() ? 0.0f : v;
 #pragma unroll
           for (int n = 0; n < NB; ++n) {
-            const u32x4_t pw = __builtin_bit_cast(u32x4_t, pb[n][j]);
-            const float pu = fd_bf16_to_f32(half_of(pw[0], pw[1], pw[2], pw[3], u));
+            const float pu = element(pb[n][j], u);
 #pragma unroll 1
             for (int h = 0; h < 2; ++h) {
               const float ph = __shfl(pu, h * 32 + col);  // this lane's row, key 16 j + 8 h + u
@@ -1227,10 +1248,7 @@ __global__ __launch_bounds__(S::kThreads) void paged_gqa_piece_kernel(PagedArgs 
             }
           }
         }
-#pragma unroll
-        for (int u = 0; u < 8; ++u)
-          if ((e[u] & 0x7f80) == 0x7f80) e[u] = 0;
-        vf = __builtin_bit_cast(bf16x8_t, e);
+        vf = without_odd(vf);
       }
 #pragma unroll
       for (int n = 0; n < NB; ++n) o[n][db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pb[n][j], o[n][db], 0, 0, 0);
@@ -1330,14 +1348,18 @@ struct Plan {
   bool may_split;
 };
 
-Plan plan_of(int64_t requests, int64_t tokens, int group, int kv_heads, int head_dim, int64_t max_keys, int max_seqlen) {
+// (E4M3 or not changes what a CU runs at once only, and never to more: bfloat16's workspace holds both.)
+Plan plan_of(int64_t requests, int64_t tokens, int group, int kv_heads, int head_dim, int64_t max_keys, int max_seqlen,
+             bool fp8) {
   Plan p;
   const int64_t rows = static_cast<int64_t>(max_seqlen) * group;
   p.few = rows <= 16 ? 1 : rows <= 32 ? 2 : 0;
   p.rows = p.few ? 16 * p.few : PieceOf<64, false>::kRows;
   p.keys = p.few ? Few<64, false, 1>::kKeys
                  : head_dim == 64 ? PieceOf<64, false>::kKeys : head_dim == 128 ? PieceOf<128, false>::kKeys : PieceOf<256, false>::kKeys;
-  p.slots = kCus * (p.few ? 2 : 1);
+  // Pieces with 64 features: 249 registers and 70 KiB of LDS, two workgroups per CU (2048 tokens on 6144 keys, 16/4
+  // heads: 103 us with ranges for two, 114 for one); with E4M3 267 registers and one (137 us; 150 with ranges for two).
+  p.slots = kCus * (p.few || (head_dim == 64 && !fp8) ? 2 : 1);
   p.min_tiles = 256 / p.keys;
   // a request's last row tile may be partly empty, its last key range too
   p.rtiles = kv_heads * (tokens * group / p.rows + requests);
@@ -1373,6 +1395,7 @@ int check_sizes(const char* what, int batch, int q_heads, int kv_heads, int seq_
   FD_REQUIRE(batch >= 0 && seq_len >= 0 && q_heads >= 1 && kv_heads >= 1 && q_heads % kv_heads == 0 && n_seqs >= 0,
              FD_ERR_INVALID_ARGUMENT, "%s: sizes must be >= 0 and q_heads a multiple of kv_heads >= 1", what);
   FD_REQUIRE(n_seqs == 0 || batch == 1, FD_ERR_INVALID_ARGUMENT, "%s: cu_seqlens requires batch == 1", what);
+  FD_REQUIRE(q_heads / kv_heads <= 2048, FD_ERR_UNSUPPORTED, "%s: at most 2048 query heads per key head", what);
   FD_REQUIRE(max_seqlen >= 0 && max_seqlen <= seq_len, FD_ERR_INVALID_ARGUMENT,
              "%s: max_seqlen must be in [0, seq_len]", what);
   FD_REQUIRE(static_cast<int64_t>(batch) * seq_len * q_heads < (1LL << 30), FD_ERR_UNSUPPORTED,
@@ -1390,7 +1413,7 @@ extern "C" int64_t fd_paged_gqa_workspace_bytes(int batch, int q_heads, int kv_h
              "%s: head_dim must be 64, 128 or 256 (got %d)", what, head_dim);
   FD_REQUIRE(page_size >= 1 && max_pages >= 1, FD_ERR_INVALID_ARGUMENT, "%s: page_size and max_pages must be >= 1", what);
   return plan_of(n_seqs > 0 ? n_seqs : batch, static_cast<int64_t>(batch) * seq_len, q_heads / kv_heads, kv_heads,
-                 head_dim, static_cast<int64_t>(max_pages) * page_size, max_seqlen).bytes;
+                 head_dim, static_cast<int64_t>(max_pages) * page_size, max_seqlen, false).bytes;
 }
 
 extern "C" int fd_paged_gqa_fwd(const void* q, const fd_paged_cache* cache, const void* gate, void* out,
@@ -1413,8 +1436,9 @@ extern "C" int fd_paged_gqa_fwd(const void* q, const fd_paged_cache* cache, cons
              FD_ERR_ALIGNMENT, "%s: rows must be contiguous and 16-byte aligned", what);
   const int requests = n_seqs > 0 ? n_seqs : batch;
   if (requests == 0 || seq_len == 0) return FD_OK;
+  const bool fp8 = cache->dtype == FD_DTYPE_E4M3;
   const Plan p = plan_of(requests, static_cast<int64_t>(batch) * seq_len, q_heads / cache->kv_heads, cache->kv_heads,
-                         cache->head_dim, static_cast<int64_t>(cache->max_pages) * cache->page_size, max_seqlen);
+                         cache->head_dim, static_cast<int64_t>(cache->max_pages) * cache->page_size, max_seqlen, fp8);
   FD_REQUIRE(p.items < (1LL << 30), FD_ERR_UNSUPPORTED, "%s: problem too large", what);
   FD_REQUIRE(p.bytes == 0 || (workspace && fd_aligned16(workspace) && workspace_bytes >= p.bytes),
              FD_ERR_INVALID_ARGUMENT, "%s: the workspace must be 16-byte aligned and hold %lld bytes", what,
@@ -1432,14 +1456,14 @@ extern "C" int fd_paged_gqa_fwd(const void* q, const fd_paged_cache* cache, cons
   a.seq_len = seq_len;
   a.group = q_heads / cache->kv_heads;
   a.kv_heads = cache->kv_heads;
-  a.slots = p.slots;
+  a.group_magic = ((1u << 24) + a.group - 1) / a.group;
+  a.slots_log2 = __builtin_ctz(static_cast<unsigned>(p.slots));
   a.min_tiles = p.min_tiles;
   a.overhead = p.few ? 2 : 4;
   a.max_items = static_cast<int>(p.items);
   a.scale_log2 = scale * 1.4426950408889634f;
   a.range_tiles = p.may_split ? static_cast<int32_t*>(workspace) : nullptr;
   a.part = p.may_split ? static_cast<float*>(workspace) + kHeaderBytes / 4 : nullptr;
-  const bool fp8 = cache->dtype == FD_DTYPE_E4M3;
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (cache->head_dim == 64) launch_dim<64>(a, p, fp8, s);
   else if (cache->head_dim == 128) launch_dim<128>(a, p, fp8, s);

@@ -63,6 +63,8 @@ def paged_gqa_attention(
     _, kv_heads, page_size, cache_dim = k_cache.shape
     if kv_heads < 1 or q_heads % kv_heads or dim != cache_dim:
         raise ValueError("Q must have the cache's head dimension and a multiple of its heads")
+    if q_heads // kv_heads > 2048:
+        raise ValueError("at most 2048 query heads per key head")
     if batch * seq_len * q_heads >= 1 << 30:
         raise ValueError("B * T * Hq must be below 2^30")
     if scale is None:

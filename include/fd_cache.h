@@ -108,7 +108,7 @@ FD_API int fd_paged_kv_read(const fd_paged_cache* cache, void* k_out, void* v_ou
  * are rounded to bf16 before the P V product, the denominator sums the rounded ones.
  *
  *   q, out  [batch, q_heads, seq_len, head_dim] bf16, strides {b, h, t, d}; query head h reads key
- *           head h / (q_heads / kv_heads)
+ *           head h / (q_heads / kv_heads); at most 2048 query heads per key head
  *   gate    NULL, or logically like out: out = attention * sigmoid(gate), rounded to bf16 once
  *   cu_seqlens, n_seqs  as in fd_paged_kv_write; rows of out behind the last request are left as
  *           they were

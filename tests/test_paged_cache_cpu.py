@@ -133,6 +133,17 @@ def test_tensors_that_do_not_fit_are_refused():
         paged_gqa_attention(x.expand(2, -1, -1, -1), k, k, table, lens, cu_seqlens=torch.zeros(3, dtype=torch.int32))
 
 
+def test_more_query_heads_per_key_head_than_a_row_count_holds_are_refused():
+    from fastdecisions_amd.paged_gqa_kernel import paged_gqa_attention
+    lib = _cache_lib.lib()
+    assert lib.fd_paged_gqa_workspace_bytes(1, 2048, 1, 1, 64, 16, 64, 0, 1) > 0
+    assert lib.fd_paged_gqa_workspace_bytes(1, 2049, 1, 1, 64, 16, 64, 0, 1) == _lib.FD_ERR_UNSUPPORTED
+    k = torch.zeros((4, 1, 16, 64), dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="2048 query heads"):
+        paged_gqa_attention(torch.zeros((1, 2049, 1, 64), dtype=torch.bfloat16), k, k,
+                            torch.zeros((1, 2), dtype=torch.int32), torch.ones(1, dtype=torch.int32))
+
+
 def test_state_operators_refuse_bad_arguments():
     lib = _cache_lib.lib()
     inv, align, uns = _lib.FD_ERR_INVALID_ARGUMENT, _lib.FD_ERR_ALIGNMENT, _lib.FD_ERR_UNSUPPORTED

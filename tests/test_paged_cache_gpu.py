@@ -101,6 +101,19 @@ def test_either_kernel_takes_any_lengths(dim, few):
     check_attention(c, q, out, lens, new)
 
 
+@pytest.mark.parametrize("group,hkv", [(1, 2), (5, 2), (7, 1), (13, 1), (31, 1), (33, 1), (127, 1), (129, 1), (1000, 1),
+                                       (2048, 1)])
+def test_groups_of_every_kind(group, hkv):
+    """Query heads per key head that divide no tile: rows change their token inside one, or a token fills many."""
+    new, cached = [1, 3, 10], [300, 0, 90]
+    lens = [a + b for a, b in zip(cached, new)]
+    announce(f"paged attention, {group} query heads per key head")
+    c = make_pages(lens, 16, hkv, 64, False, seed=16)
+    q = make_q(new, group * hkv, 64, 17)
+    out = run_attention(c, q, lens, new)
+    check_attention(c, q, out, lens, new)
+
+
 @pytest.mark.parametrize("n", [1, 40])
 def test_many_requests(n):
     """More requests than lanes of a wavefront, ragged, the longest last."""
