@@ -23,6 +23,7 @@
 // permuted so that a lane's scores are those of the 8 consecutive keys whose
 // probabilities it must supply to P V: P never leaves registers, and V^T comes
 // from transposing LDS reads.
+#include <algorithm>
 #include <type_traits>
 
 #include "gqa_tile.h"
@@ -69,8 +70,7 @@ struct Piece {
   static constexpr int CR = D / 8;                      // 16-byte chunks of a staged (bf16) row
   static constexpr int kTileBytes = kKeys * CR * 16;    // K or V
   static constexpr int kStages = 4;
-  static constexpr int kRowFloats = D + 4;              // epilogue rows, padded
-  static constexpr int kEpilogueBytes = KS * kRows * (kRowFloats + 2) * 4;
+  static constexpr int kEpilogueBytes = KS == 1 ? 0 : kWaves * 64 * (D / 2 + 2) * 4;  // a row block of every wavefront
   static constexpr int kLoopBytes = 2 * kStages * kTileBytes;
   static constexpr int kSmemBytes = kLoopBytes > kEpilogueBytes ? kLoopBytes : kEpilogueBytes;
   // 1 KiB copies of a bf16 K (or V) tile per wavefront, and the rows of each
@@ -1255,28 +1255,110 @@ __global__ __launch_bounds__(S::kThreads) void paged_gqa_piece_kernel(PagedArgs 
     }
   }
 
-  // ---- join the key parts through LDS, row by row, then store the rows or leave the item's part
-  __syncthreads();  // the stages are free
-  float* const rowsf = reinterpret_cast<float*>(smem);
-  float* const ml = rowsf + S::KS * S::kRows * S::kRowFloats;
+  // ---- the key parts joined: with two of them each keeps the row block of its own number and gives the other one
+  // away through LDS, in registers' order.  Then the rows leave from registers, 8 features (of 16) of a row per lane.
+  // (Through LDS row by row, 16 rounds of a few dependent reads each, it took 5 us of every item.)
+  f32x16_t acc[kNdb];
+  float m = m_run[0], l = half_sum(l_run[0]);
+  int n_own = 0;
+  if constexpr (S::KS == 2) {
+    static_assert(NB == 2, "a row block for each key part");
+    n_own = kp;
+    __syncthreads();  // the stages are free
+    float* const gave = reinterpret_cast<float*>(smem) + lane * 4;
+    float* const gave_ml = reinterpret_cast<float*>(smem) + S::kWaves * 64 * (D / 2) + lane * 2;
+    const float l1 = half_sum(l_run[1]);
+    const float m_give = kp ? m : m_run[1], l_give = kp ? l : l1;
+    m = kp ? m_run[1] : m;
+    l = kp ? l1 : l;
 #pragma unroll
-  for (int n = 0; n < NB; ++n) {
-    const int at = kp * S::kRows + (rw * NB + n) * 32 + col;
-    float* dst = rowsf + at * S::kRowFloats;
+    for (int db = 0; db < kNdb; ++db) {
 #pragma unroll
-    for (int db = 0; db < kNdb; ++db)
+      for (int r4 = 0; r4 < 4; ++r4) {
+        f32x4_t x;
 #pragma unroll
-      for (int r4 = 0; r4 < 4; ++r4)
-        *reinterpret_cast<f32x4_t*>(dst + db * 32 + r4 * 8 + half * 4) =
-            f32x4_t{o[n][db][r4 * 4], o[n][db][r4 * 4 + 1], o[n][db][r4 * 4 + 2], o[n][db][r4 * 4 + 3]};
-    const float l = half_sum(l_run[n]);
-    if (half == 0) {
-      ml[at * 2] = m_run[n];
-      ml[at * 2 + 1] = l;
+        for (int e = 0; e < 4; ++e) {
+          x[e] = kp ? o[0][db][4 * r4 + e] : o[1][db][4 * r4 + e];
+          acc[db][4 * r4 + e] = kp ? o[1][db][4 * r4 + e] : o[0][db][4 * r4 + e];
+        }
+        *reinterpret_cast<f32x4_t*>(gave + (wave * (D / 8) + db * 4 + r4) * 256) = x;
+      }
+    }
+    gave_ml[wave * 128] = m_give;
+    gave_ml[wave * 128 + 1] = l_give;
+    __syncthreads();
+    const int other = wave ^ S::RW;  // the other key part of these rows
+    const float m2 = gave_ml[other * 128], l2 = gave_ml[other * 128 + 1];
+    const float top = fmaxf(m, m2), sub = top == -__builtin_inff() ? 0.0f : top;
+    const float w = __builtin_amdgcn_exp2f(m - sub), w2 = __builtin_amdgcn_exp2f(m2 - sub);
+    m = top;
+    l = l * w + l2 * w2;
+#pragma unroll
+    for (int db = 0; db < kNdb; ++db) {
+#pragma unroll
+      for (int r4 = 0; r4 < 4; ++r4) {
+        const f32x4_t x = *reinterpret_cast<const f32x4_t*>(gave + (other * (D / 8) + db * 4 + r4) * 256);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[db][4 * r4 + e] = acc[db][4 * r4 + e] * w + x[e] * w2;
+      }
+    }
+  } else {
+    static_assert(S::KS == 1 && NB == 1, "nothing to join");
+#pragma unroll
+    for (int db = 0; db < kNdb; ++db) acc[db] = o[0][db];
+  }
+  // features 32 db + 16 j + 4 half + 0..3 and the same + 8: the halves exchange theirs for 8 in a row, from 8 half on
+#pragma unroll
+  for (int db = 0; db < kNdb; ++db) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(acc[db][8 * j + e]), __float_as_uint(acc[db][8 * j + 4 + e]), false, false);
+        acc[db][8 * j + e] = __uint_as_float(r[0]);
+        acc[db][8 * j + 4 + e] = __uint_as_float(r[1]);
+      }
     }
   }
-  __syncthreads();
-  close_job<S, S::KS>(a, job, rowsf, ml);
+  const int row = (rw * NB + n_own) * 32 + col;
+  if (row >= it.rows - it.row0) return;
+  if (job.split) {
+    float* const at = a.part + job.slot * part_floats<S::kRows>(D);
+    if (half == 0) {
+      at[S::kRows * D + row * 2] = m;
+      at[S::kRows * D + row * 2 + 1] = l;
+    }
+#pragma unroll
+    for (int i = 0; i < 2 * kNdb; ++i) {
+      f32x4_t* const dst = reinterpret_cast<f32x4_t*>(at + row * D + 16 * i + 8 * half);
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const f32x16_t& x = acc[i / 2];
+        const int e = 8 * (i % 2) + 4 * u;
+        dst[u] = f32x4_t{x[e], x[e + 1], x[e + 2], x[e + 3]};
+      }
+    }
+    return;
+  }
+  const int local = token_of(a, it, row);
+  const int head_q = it.head * a.group + (it.rem0 + row - local * a.group);
+  const int b = a.cu == nullptr ? it.req : 0;
+  const int64_t tok = it.start + it.token0 + local;
+  uint16_t* const dst = a.o + b * a.os[0] + head_q * a.os[1] + tok * a.os[2] + 8 * half;
+  const uint16_t* const gate = a.gate == nullptr ? nullptr : a.gate + b * a.gs[0] + head_q * a.gs[1] + tok * a.gs[2] + 8 * half;
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+  for (int i = 0; i < 2 * kNdb; ++i) {
+    f32x8_t v;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = acc[i / 2][8 * (i % 2) + e] * inv;
+    if (gate != nullptr) {
+      const f32x8_t g = __builtin_convertvector(*reinterpret_cast<const bf16x8_t*>(gate + 16 * i), f32x8_t);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = v[e] / (1.0f + __expf(-g[e]));
+    }
+    *reinterpret_cast<bf16x8_t*>(dst + 16 * i) = __builtin_convertvector(v, bf16x8_t);
+  }
 }
 
 // Joins the key ranges of every split row tile and stores its rows, kJoinRows of them per workgroup.
@@ -1363,7 +1445,8 @@ Plan plan_of(int64_t requests, int64_t tokens, int group, int kv_heads, int head
   p.min_tiles = 256 / p.keys;
   // a request's last row tile may be partly empty, its last key range too
   p.rtiles = kv_heads * (tokens * group / p.rows + requests);
-  p.items = kMaxRounds * p.slots + p.rtiles;
+  // best_range gives at most kMaxRounds * slots items, or splits nothing; a share alone may add a range per row tile
+  p.items = requests <= 64 ? std::max<int64_t>(kMaxRounds * p.slots, p.rtiles) : kMaxRounds * p.slots + p.rtiles;
   p.may_split = max_keys > static_cast<int64_t>(p.min_tiles) * p.keys;
   p.bytes = p.may_split ? kHeaderBytes + p.items * p.rows * (head_dim + 2) * 4 : 0;
   return p;
