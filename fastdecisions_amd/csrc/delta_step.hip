@@ -14,6 +14,10 @@
 // (64 KiB each way per request and head); for few requests the latency of its
 // loads.  The chunked rule moves it too and adds work that only pays from tens
 // of tokens on.
+//
+// Measured (16 heads): one token of one request 4.4 us, of 64 requests 22.7 us, 5.9 TB/s of state (134 MB,
+// in part from the last-level cache; a large copy here: 5.1).  A further token of a request costs 1.25 us:
+// its chain of products and cross-lane adds.
 #include "../../include/fd_cache.h"
 #include "state_slot.h"
 

@@ -8,16 +8,15 @@
 //
 //   few rows   16 or 32 rows, 4 wavefronts that each take every fourth block of
 //              32 keys into LDS of their own: no barrier in the loop, the cache
-//              streams through at the rate of the memory.  Single tokens.
-//   pieces     128 rows, wavefronts share the staged key tiles.  Long suffixes.
+//              streams through at the rate of the memory.  Up to 64 rows.
+//   pieces     128 rows, wavefronts share the staged key tiles.  Suffixes.
 //
 // Key ranges are sized on the device: the lengths are there, and a grid sized by
 // the longest possible request would be mostly empty.  Every workgroup sums the
 // row tiles times key tiles of all requests and cuts every request into ranges
-// of c tiles, c = total / workers, so items are alike whatever the mix of
-// lengths; the host only bounds their number (workers + row tiles).  Items of a
-// split row tile leave (o, max, denominator) in the workspace and
-// paged_gqa_join_kernel joins them.
+// of c tiles (best_range), so items are alike whatever the mix of lengths; the
+// host only bounds their number.  Items of a split row tile leave (o, max,
+// denominator) in the workspace and paged_gqa_join_kernel joins them.
 //
 // In both, scores are computed transposed (S^T = K Q^T on MFMA), with the K rows
 // permuted so that a lane's scores are those of the 8 consecutive keys whose
@@ -144,8 +143,8 @@ __device__ __forceinline__ int tiles_over(int x, int c) {
 // The key tiles of a range, for up to 64 requests of rt row tiles and kt key tiles (a lane each) and
 // `work` tile pairs in all heads.  A range of c tiles gives sum rt ceil(kt / c) heads items; the smallest
 // c whose items fit m times the workgroups that run at once takes about m (c + overhead) tiles of time,
-// and the better of m = 1 .. kMaxRounds is taken (a few items more than workgroups would cost a whole
-// round: six suffixes, 344 items of 35 tiles on 256 CUs, 107 us, 232 of 42: see the figures below).
+// and the better of m = 1 .. kMaxRounds is taken: a few items more than workgroups would cost a whole
+// round (six suffixes of 30 to 400 tokens: 344 items of 35 tiles on 256 CUs 107 us, 232 of 42 tiles 76).
 constexpr int kMaxRounds = 2;
 static_assert(kMaxRounds == 2, "m << slots_log2 and >> (slots_log2 + m - 1) are the same for m = 1 and 2");
 __device__ __forceinline__ int best_range(const PagedArgs& a, int rt, int kt, int64_t work) {
@@ -477,6 +476,9 @@ __device__ __forceinline__ void byte_to_lds(const uint8_t* p, uint32_t lds) {
 // are (codes are converted where they are read, scales multiply scores and probabilities), K and V
 // of kStages blocks each, the next K leaving as soon as a block's scores have read theirs, the next
 // V as soon as P V has.
+// Measured (16 / 4 heads x 128, pages of 64, kernel and join): 64 requests of 8192 keys 195 us, 5.5 TB/s of
+// keys and values (a large copy here: 5.1), E4M3 107 us, 5.0 TB/s; of 256 to 8192 keys 79 and 47 us; one
+// request of 8192 keys 16 us, of 200 keys 8 us, latency: arguments, lengths, page, keys, scores, store.
 template <class S>
 __global__ __launch_bounds__(S::kThreads, S::kPerCu) void paged_gqa_few_kernel(PagedArgs a) {
   constexpr int D = S::D, NR = S::NR, RBY = S::kRowBytes, kKk = D / 32, kNdb = D / 16, NS = S::kStages;
@@ -797,6 +799,14 @@ __device__ __forceinline__ void pieces(int m, F f) {
 // so that the softmax's VALU and exp work runs under both halves of the MFMAs and every operand is
 // read a phase before it is used.  Four LDS stages: bf16 tiles are copied three steps ahead (asm copies,
 // counted by hand), codes are loaded into registers three steps ahead and stored as bf16 two ahead.
+//
+// Measured, 2048 new tokens on 6144 cached ones: 16 / 4 heads x 128 features 149 us, 806 TFLOP/s (14336 cached
+// 268 us, 960; a large library product here: 1370), x 64 104 us, 8 / 2 x 256 148 us, 810; E4M3 189, 127 and
+// 175.  2048 tokens alone: 46 us.  A workgroup spends 1.6 us on finding its item, 3.4 until its first tiles
+// and Q are there, 1.15 per whole tile of 64 keys, 1.3 on the last one, 2 to 3.4 on the masked ones, 2.7 on
+// its rows.  In the loop the matrix cores are busy for a third of the time: a single wavefront per SIMD
+// issues MFMAs, softmax and LDS reads in turn, and 128 rows leave no registers for a second one.  LDS is not
+// the bound: E4M3's 8% of cycles lost to bank conflicts could be removed without any gain.
 template <class S>
 __global__ __launch_bounds__(S::kThreads) void paged_gqa_piece_kernel(PagedArgs a) {
   constexpr int D = S::D, NB = S::NB, CR = S::CR, kNdb = D / 32, kSteps = D / 16, kAhead = 4;
@@ -1361,7 +1371,8 @@ __global__ __launch_bounds__(S::kThreads) void paged_gqa_piece_kernel(PagedArgs 
   }
 }
 
-// Joins the key ranges of every split row tile and stores its rows, kJoinRows of them per workgroup.
+// Joins the key ranges of every split row tile and stores its rows, kJoinRows of them per workgroup.  Bound by
+// the fp32 parts it reads: 2048 tokens x 8 heads x 256 features in two ranges, 34 MB in 11 us; a few rows, 4.5 us.
 constexpr int kJoinRows = 16;
 
 template <class S>
@@ -1420,6 +1431,9 @@ __global__ __launch_bounds__(256) void paged_gqa_join_kernel(PagedArgs a) {
 template <int D, bool FP8>
 using PieceOf = std::conditional_t<D == 256, Piece<D, FP8, 4, 1, 1>, Piece<D, FP8, 2, 2, 2>>;
 
+static_assert(Few<64, false, 1>::kPerCu == 2 && Few<64, true, 1>::kPerCu == 2 && Few<128, true, 1>::kPerCu == 2 &&
+              Few<256, true, 1>::kPerCu == 2 && Few<64, false, 2>::kPerCu == 2 && Few<64, true, 2>::kPerCu == 2 &&
+              Few<128, true, 2>::kPerCu == 2 && Few<256, true, 2>::kPerCu == 1, "plan_of's workgroups per CU");
 constexpr int kHeaderBytes = 256;  // of the workspace: range_tiles
 
 // The kernel of a call, and its items, row tiles and workspace, whatever the lengths turn out to be.
@@ -1430,18 +1444,28 @@ struct Plan {
   bool may_split;
 };
 
-// (E4M3 or not changes what a CU runs at once only, and never to more: bfloat16's workspace holds both.)
 Plan plan_of(int64_t requests, int64_t tokens, int group, int kv_heads, int head_dim, int64_t max_keys, int max_seqlen,
              bool fp8) {
   Plan p;
   const int64_t rows = static_cast<int64_t>(max_seqlen) * group;
-  p.few = rows <= 16 ? 1 : rows <= 32 ? 2 : 0;
+  // Measured with 16 rows, 32 rows and pieces (us; 16/4 heads x 128 unless noted, 64 requests on 2048 keys):
+  //   rows  32: 46, 52, 51; 8/2 x 256 49, 59, 58; E4M3 34, 37, 59      -> two tiles of 16 rows
+  //   rows  64: 69, 49, 52; 8/2 x 256 81, 57, 61; E4M3 59, 45, 59      -> two of 32, but 256 features with E4M3, whose
+  //             46, 53, 62                                              kernel for 32 rows fills a CU alone: four of 16
+  //   rows  96: 92, 72, 53; 8/2 x 256 119, 104, 66; E4M3 84, 68, 60    -> pieces, unless the call is so small that
+  //             one request of 4096 keys 19, 19, 24                     latency counts, up to 128 rows in all
+  const int64_t all_rows = tokens * group;
+  p.few = rows <= 32 ? 1 : rows > 64 && (all_rows > 128 || max_keys > 16384) ? 0 : head_dim == 256 && fp8 ? 1 : 2;
   p.rows = p.few ? 16 * p.few : PieceOf<64, false>::kRows;
   p.keys = p.few ? Few<64, false, 1>::kKeys
                  : head_dim == 64 ? PieceOf<64, false>::kKeys : head_dim == 128 ? PieceOf<128, false>::kKeys : PieceOf<256, false>::kKeys;
-  // Pieces with 64 features: 249 registers and 70 KiB of LDS, two workgroups per CU (2048 tokens on 6144 keys, 16/4
-  // heads: 103 us with ranges for two, 114 for one); with E4M3 267 registers and one (137 us; 150 with ranges for two).
-  p.slots = kCus * (p.few || (head_dim == 64 && !fp8) ? 2 : 1);
+  // Workgroups per CU.  Few rows: by LDS (Few::kPerCu).  Pieces with 64 features: 249 registers and 64 KiB of LDS, two
+  // (2048 tokens on 6144 keys, 16/4 heads: 103 us with ranges for two, 114 for one); with E4M3 267 registers and one
+  // (137 us; 150 with ranges for two).
+  const int per_cu = p.few == 1   ? (head_dim == 256 && !fp8 ? Few<256, false, 1>::kPerCu : Few<128, false, 1>::kPerCu)
+                     : p.few == 2 ? (head_dim == 256 ? Few<256, false, 2>::kPerCu : Few<128, false, 2>::kPerCu)
+                                  : (head_dim == 64 && !fp8 ? 2 : 1);
+  p.slots = kCus * per_cu;
   p.min_tiles = 256 / p.keys;
   // a request's last row tile may be partly empty, its last key range too
   p.rtiles = kv_heads * (tokens * group / p.rows + requests);
@@ -1495,8 +1519,11 @@ extern "C" int64_t fd_paged_gqa_workspace_bytes(int batch, int q_heads, int kv_h
   FD_REQUIRE(head_dim == 64 || head_dim == 128 || head_dim == 256, FD_ERR_UNSUPPORTED,
              "%s: head_dim must be 64, 128 or 256 (got %d)", what, head_dim);
   FD_REQUIRE(page_size >= 1 && max_pages >= 1, FD_ERR_INVALID_ARGUMENT, "%s: page_size and max_pages must be >= 1", what);
-  return plan_of(n_seqs > 0 ? n_seqs : batch, static_cast<int64_t>(batch) * seq_len, q_heads / kv_heads, kv_heads,
-                 head_dim, static_cast<int64_t>(max_pages) * page_size, max_seqlen, false).bytes;
+  auto bytes = [&](bool fp8) {
+    return plan_of(n_seqs > 0 ? n_seqs : batch, static_cast<int64_t>(batch) * seq_len, q_heads / kv_heads, kv_heads,
+                   head_dim, static_cast<int64_t>(max_pages) * page_size, max_seqlen, fp8).bytes;
+  };
+  return std::max(bytes(false), bytes(true));
 }
 
 extern "C" int fd_paged_gqa_fwd(const void* q, const fd_paged_cache* cache, const void* gate, void* out,

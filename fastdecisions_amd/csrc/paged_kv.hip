@@ -10,6 +10,10 @@
 // no logarithm and no division.  x 2^-E is exact in fp32 (or below a code's
 // smallest step), so the one rounding is the conversion's; floating codes lose
 // nothing to a scale that is not the tightest, except a binade of subnormals.
+//
+// Measured (4 heads x 128): 64 tokens 3.5 us, the launch; prompts of 24 MB (bf16 in, E4M3 out)
+// 10.4 us, 2.3 TB/s, and 37 MB read back (E4M3 in, bf16 out) 13.1 us, 2.8 TB/s: a few microseconds of
+// launch and of the page table's, then the pages' latencies besides the bytes' 4.6 and 7.2.
 #include <initializer_list>
 #include <type_traits>
 

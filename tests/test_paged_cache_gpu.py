@@ -175,6 +175,27 @@ def test_nothing_masked_reaches_a_row(dim, n, fp8):
     assert not torch.isfinite(out[:, :, first:]).any() if n > 1 else True
 
 
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("n", [7, 12])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_nothing_masked_reaches_a_row_of_middling_requests(dim, n, fp8):
+    """The same with 28 and 48 rows of a key head: two tiles of the few-rows kernels."""
+    test_nothing_masked_reaches_a_row(dim, n, fp8)
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("hq,hkv,dim", [(16, 4, 128), (8, 2, 256), (16, 4, 64)])
+@pytest.mark.parametrize("new", [[8] * 5, [9, 16, 1, 0, 12], [32], [33], [16, 17]])
+def test_requests_of_a_few_tokens(new, hq, hkv, dim, fp8):
+    """Rows of a key head around every kernel's bounds (32, 64, 128 in all)."""
+    announce(f"paged attention, {new} new, {hq}/{hkv} x {dim}, fp8 {fp8}")
+    lens = [n + c for n, c in zip(new, [1500, 0, 700, 33, 2100])]
+    c = make_pages(lens, 32, hkv, dim, fp8, seed=18)
+    q = make_q(new, hq, dim, 19)
+    out = run_attention(c, q, lens, new)
+    check_attention(c, q, out, lens, new)
+
+
 def test_a_seen_infinity_reaches_its_feature_alone():
     """An infinite value of a key that a row sees, next to rows that do not see it."""
     announce("paged attention, a seen infinity")
