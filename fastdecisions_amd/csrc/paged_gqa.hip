@@ -477,8 +477,8 @@ __device__ __forceinline__ void byte_to_lds(const uint8_t* p, uint32_t lds) {
 // of kStages blocks each, the next K leaving as soon as a block's scores have read theirs, the next
 // V as soon as P V has.
 // Measured (16 / 4 heads x 128, pages of 64, kernel and join): 64 requests of 8192 keys 195 us, 5.5 TB/s of
-// keys and values (a large copy here: 5.1), E4M3 107 us, 5.0 TB/s; of 256 to 8192 keys 79 and 47 us; one
-// request of 8192 keys 16 us, of 200 keys 8 us, latency: arguments, lengths, page, keys, scores, store.
+// keys and values (a large copy here: 5.1), E4M3 107 us, 5.0 TB/s; of 256 to 8192 keys 79 and 46 us; one
+// request of 8192 keys 13 us, of 200 keys 8 us, latency: arguments, lengths, page, keys, scores, store.
 template <class S>
 __global__ __launch_bounds__(S::kThreads, S::kPerCu) void paged_gqa_few_kernel(PagedArgs a) {
   constexpr int D = S::D, NR = S::NR, RBY = S::kRowBytes, kKk = D / 32, kNdb = D / 16, NS = S::kStages;
@@ -1371,13 +1371,16 @@ __global__ __launch_bounds__(S::kThreads) void paged_gqa_piece_kernel(PagedArgs 
   }
 }
 
-// Joins the key ranges of every split row tile and stores its rows, kJoinRows of them per workgroup.  Bound by
-// the fp32 parts it reads: 2048 tokens x 8 heads x 256 features in two ranges, 34 MB in 11 us; a few rows, 4.5 us.
-constexpr int kJoinRows = 16;
-
-template <class S>
+// Joins the key ranges of every split row tile and stores its rows, ROWS of them per workgroup.  16, many row tiles:
+// bound by the fp32 parts it reads: 2048 tokens x 8 heads x 256 features in two ranges, 34 MB in 11 us.  2 or 4, few
+// row tiles: there are many ranges then, read in turn they would cost a memory latency per four of them; the threads
+// that the rows leave over take ranges of their own, joined through LDS.
+template <class S, int ROWS>
 __global__ __launch_bounds__(256) void paged_gqa_join_kernel(PagedArgs a) {
   constexpr int D = S::D;
+  constexpr int kLanes = D / 4;  // of a row
+  constexpr int kRowsAtOnce = ROWS < 256 / kLanes ? ROWS : 256 / kLanes;
+  constexpr int kGroups = 256 / kLanes / kRowsAtOnce;  // of ranges
   Item it;
   const int b = blockIdx.x;
   if (!find_item<S::kRows, S::kKeys, true>(a, threadIdx.x & 63, [&](int) { return b; }, &it)) return;
@@ -1386,16 +1389,17 @@ __global__ __launch_bounds__(256) void paged_gqa_join_kernel(PagedArgs a) {
   if (ranges <= 1) return;  // its one item has stored the rows
   const int slot = it.base + it.head * it.n_ranges * it.n_rtiles + it.rtile;
   if (slot < 0 || slot + (ranges - 1) * static_cast<int64_t>(it.n_rtiles) >= a.max_items) return;
-  const int row_end = min(min(S::kRows, it.rows - it.row0), static_cast<int>(blockIdx.y + 1) * kJoinRows);
+  const int row_end = min(min(S::kRows, it.rows - it.row0), static_cast<int>(blockIdx.y + 1) * ROWS);
   const int64_t step = it.n_rtiles * part_floats<S::kRows>(D);  // from one range's part to the next one's
   const float* const part = a.part + slot * part_floats<S::kRows>(D);
-  constexpr int kLanes = D / 4;  // of a row
-  for (int row = blockIdx.y * kJoinRows + threadIdx.x / kLanes; row < row_end; row += 256 / kLanes) {
-    const int d = (threadIdx.x % kLanes) * 4;
+  const int d = (threadIdx.x % kLanes) * 4;
+  const int own = threadIdx.x / kLanes % kRowsAtOnce, group = threadIdx.x / kLanes / kRowsAtOnce;
+  for (int row0 = blockIdx.y * ROWS; row0 < row_end; row0 += kRowsAtOnce) {
+    const int row = min(row0 + own, row_end - 1);
     // four ranges at a time: their loads are in flight together
     float m = -__builtin_inff(), l = 0.0f;
     f32x4_t acc = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int s0 = 0; s0 < ranges; s0 += 4) {
+    for (int s0 = 4 * group; s0 < ranges; s0 += 4 * kGroups) {
       float ms[4], ls[4];
       f32x4_t os[4];
 #pragma unroll
@@ -1423,7 +1427,24 @@ __global__ __launch_bounds__(256) void paged_gqa_join_kernel(PagedArgs a) {
       }
       m = top;
     }
-    store4(a, it, row, d, acc, l == 0.0f ? 0.0f : 1.0f / l);
+    if constexpr (kGroups > 1) {
+      static_assert(ROWS == kRowsAtOnce, "one round of rows: LDS is used once");
+      __shared__ float ml[kGroups][kRowsAtOnce][2];
+      __shared__ f32x4_t os[kGroups][kRowsAtOnce][kLanes];
+      os[group][own][d / 4] = acc;
+      if (d == 0) ml[group][own][0] = m, ml[group][own][1] = l;
+      __syncthreads();
+      if (group != 0) return;
+#pragma unroll
+      for (int g = 1; g < kGroups; ++g) {
+        const float mg = ml[g][own][0], top = fmaxf(m, mg), sub = top == -__builtin_inff() ? 0.0f : top;
+        const float w = __builtin_amdgcn_exp2f(m - sub), wg = __builtin_amdgcn_exp2f(mg - sub);
+        l = l * w + ml[g][own][1] * wg;
+        acc = acc * w + os[g][own][d / 4] * wg;
+        m = top;
+      }
+    }
+    if (row0 + own < row_end) store4(a, it, row, d, acc, l == 0.0f ? 0.0f : 1.0f / l);
   }
 }
 
@@ -1480,9 +1501,19 @@ template <class S, typename K>
 void launch(K kernel, const PagedArgs& a, const Plan& p, hipStream_t s) {
   const int64_t blocks = (p.items + kNumXcd - 1) / kNumXcd * kNumXcd;
   hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(S::kThreads), 0, s, a);
-  if (p.may_split)
-    hipLaunchKernelGGL((paged_gqa_join_kernel<S>), dim3(static_cast<unsigned>(p.rtiles), (S::kRows + kJoinRows - 1) / kJoinRows),
-                       dim3(256), 0, s, a);
+  if (!p.may_split) return;
+  auto join = [&](auto kernel, int rows) {
+    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(p.rtiles), S::kRows / rows), dim3(256), 0, s, a);
+  };
+  // Two rows per workgroup while a CU gets at most 4 of them, four while it gets 4 (128 features) or 8 (256).  Whole
+  // calls with 16, 4 and 2 rows (us): one request of 4 tokens on 4096 keys, 16/4 x 128, 16.9, -, 12.4, 8/2 x 256 25.0, -,
+  // 16.4; two of 64 tokens on 8192 keys 34.7, 31.8, -; four on 4096, 8/2 x 256, 40.6, 34.3, -.  More row tiles: 64
+  // requests of 4 tokens, 16/4 x 128, 50.7, -, 54.7; four of 100 tokens 38.4, 39.9, -.
+  if (p.rtiles * (S::kRows / 2) <= 4 * kCus) return join(paged_gqa_join_kernel<S, 2>, 2);
+  if constexpr (S::D > 64) {
+    if (p.rtiles * (S::kRows / 4) <= S::D / 32 * kCus) return join(paged_gqa_join_kernel<S, 4>, 4);
+  }
+  join(paged_gqa_join_kernel<S, 16>, 16);
 }
 
 template <int D, bool FP8>
