@@ -250,6 +250,7 @@ __device__ __forceinline__ bool find_item(const PagedArgs& a, int lane, Want wan
       const int l = __builtin_ctzll(past);
       it->req = r0 + l;
       const int k = at - (before + at_lane(incl, l) - at_lane(mine, l));  // within the request
+      if (k < 0) return false;  // sums past 31 bits: only of an offset table that is not ascending
       it->base = base + at_lane(incl_all, l) - at_lane(all, l);
       it->n_rtiles = at_lane(rt, l);
       it->n_ranges = at_lane(ranges, l);

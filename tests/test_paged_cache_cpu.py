@@ -24,8 +24,11 @@ FAKE = 1 << 20  # 16-byte aligned, never dereferenced: validation fails first
 def kernels():
     """The hazards that the other library's sources are checked for, in this one's."""
     request = type("Request", (), {"param": "paged_gqa.hip"})
-    return test_isa_cpu.kernels.__wrapped__(request) if hasattr(test_isa_cpu.kernels, "__wrapped__") else \
-        test_isa_cpu.kernels.__pytest_wrapped__.obj(request)
+    get = test_isa_cpu.kernels
+    get = get.__wrapped__ if hasattr(get, "__wrapped__") else get.__pytest_wrapped__.obj
+    with pytest.MonkeyPatch.context() as m:
+        m.setattr(_build, "DEVICE_FLAGS", _build.DEVICE_FLAGS + _build.EXTRA_FLAGS["paged_gqa.hip"])
+        return get(request)
 
 
 def declared():
