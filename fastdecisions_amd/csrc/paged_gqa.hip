@@ -69,7 +69,7 @@ struct Piece {
   static constexpr int CR = D / 8;                      // 16-byte chunks of a staged (bf16) row
   static constexpr int kTileBytes = kKeys * CR * 16;    // K or V
   static constexpr int kStages = 4;
-  static constexpr int kEpilogueBytes = KS == 1 ? 0 : kWaves * 64 * (D / 2 + 2) * 4;  // a row block of every wavefront
+  static constexpr int kEpilogueBytes = KS == 1 ? 0 : kWaves * 64 * (NB * D / 4 + 2) * 4;  // what the key parts give each other
   static constexpr int kLoopBytes = 2 * kStages * kTileBytes;
   static constexpr int kSmemBytes = kLoopBytes > kEpilogueBytes ? kLoopBytes : kEpilogueBytes;
   // 1 KiB copies of a bf16 K (or V) tile per wavefront, and the rows of each
@@ -785,10 +785,13 @@ __device__ __forceinline__ void pieces(int m, F f) {
   }
 }
 
-// A wavefront owns NB blocks of 32 rows and every KS-th block of 32 keys.  With two row blocks an
-// operand read from LDS feeds two MFMAs: with one, the 4 SIMDs' operand reads (1 KiB per 32-cycle
-// MFMA each) alone would take all of LDS's 128 bytes per cycle.  One wavefront per SIMD: 128 rows
-// of 128 features are 128 registers of O^T and 64 of Q.
+// A wavefront owns NB blocks of 32 rows and every KS-th block of 32 keys.  A block of 128 features is 64 registers of
+// O^T and 32 of Q.  Two blocks per wavefront, four wavefronts: an operand read from LDS feeds two MFMAs, one wavefront
+// per SIMD.  One block, eight wavefronts: two per SIMD fill each other's waits, each operand read feeds one MFMA (1 KiB
+// per 32-cycle MFMA on 4 SIMDs is all of LDS's 128 bytes per cycle, at a half-busy matrix core half of it).  Measured at
+// 128 features, four and eight wavefronts: 2048 tokens on 6144 keys 149 and 141 us, E4M3 189 and 163, on 14336 267 and
+// 263, 2048 alone 46.1 and 42.3.  256 features (128 + 64 registers of a block) leave room for one wavefront per SIMD; at
+// 64 the four of a workgroup leave room for a second workgroup.
 //
 // Tiles that all rows see whole run in a pipelined loop without masks; the rest (the new tokens' own
 // tiles, and everything of a request with absent pages) in a plain one.  A pipelined step t has two
@@ -801,13 +804,12 @@ __device__ __forceinline__ void pieces(int m, F f) {
 // read a phase before it is used.  Four LDS stages: bf16 tiles are copied three steps ahead (asm copies,
 // counted by hand), codes are loaded into registers three steps ahead and stored as bf16 two ahead.
 //
-// Measured, 2048 new tokens on 6144 cached ones: 16 / 4 heads x 128 features 149 us, 806 TFLOP/s (14336 cached
-// 268 us, 960; a large library product here: 1370), x 64 104 us, 8 / 2 x 256 148 us, 810; E4M3 189, 127 and
-// 175.  2048 tokens alone: 46 us.  A workgroup spends 1.6 us on finding its item, 3.4 until its first tiles
-// and Q are there, 1.15 per whole tile of 64 keys, 1.3 on the last one, 2 to 3.4 on the masked ones, 2.7 on
-// its rows.  In the loop the matrix cores are busy for a third of the time: a single wavefront per SIMD
-// issues MFMAs, softmax and LDS reads in turn, and 128 rows leave no registers for a second one.  LDS is not
-// the bound: E4M3's 8% of cycles lost to bank conflicts could be removed without any gain.
+// Measured, 2048 new tokens on 6144 cached ones: 16 / 4 heads x 128 features 141 us, 850 TFLOP/s (14336 cached
+// 263 us, 978; a large library product here: 1370), x 64 104 us, 8 / 2 x 256 148 us, 810; E4M3 163, 127 and
+// 175.  2048 tokens alone: 42 us.  A workgroup spends 1.6 us on finding its item, 3.4 until its first tiles
+// and Q are there, 1.1 per whole tile of 64 keys, 1.3 on the last one, 2 to 3.4 on the masked ones, 2.7 on
+// its rows.  In the loop MFMA, VALU, and LDS reads are each busy for a third to a half of the time, with a
+// barrier per tile.  LDS conflicts are not the bound: E4M3's 8% of cycles could be removed without any gain.
 template <class S>
 __global__ __launch_bounds__(S::kThreads) void paged_gqa_piece_kernel(PagedArgs a) {
   constexpr int D = S::D, NB = S::NB, CR = S::CR, kNdb = D / 32, kSteps = D / 16, kAhead = 4;
@@ -1266,49 +1268,56 @@ __global__ __launch_bounds__(S::kThreads) void paged_gqa_piece_kernel(PagedArgs 
     }
   }
 
-  // ---- the key parts joined: with two of them each keeps the row block of its own number and gives the other one
-  // away through LDS, in registers' order.  Then the rows leave from registers, 8 features (of 16) of a row per lane.
-  // (Through LDS row by row, 16 rounds of a few dependent reads each, it took 5 us of every item.)
-  f32x16_t acc[kNdb];
+  // ---- the key parts joined: with two of them each keeps half (of two row blocks one, of one block half its features)
+  // and gives the other one away through LDS, in registers' order.  Then the rows leave from registers, 8 features (of
+  // 16) of a row per lane.  (Through LDS row by row, 16 rounds of a few dependent reads each, it took 5 us of every item.)
+  constexpr int kOwn = S::KS == 2 && NB == 1 ? kNdb / 2 : kNdb;  // blocks of 32 features that this wavefront stores
+  f32x16_t acc[kOwn];
   float m = m_run[0], l = half_sum(l_run[0]);
-  int n_own = 0;
+  int n_own = 0, d_own = 0;
   if constexpr (S::KS == 2) {
-    static_assert(NB == 2, "a row block for each key part");
-    n_own = kp;
+    n_own = NB == 2 ? kp : 0;
+    d_own = NB == 2 ? 0 : kp * (D / 2);
     __syncthreads();  // the stages are free
+    constexpr int kGave = kOwn * 4;
     float* const gave = reinterpret_cast<float*>(smem) + lane * 4;
-    float* const gave_ml = reinterpret_cast<float*>(smem) + S::kWaves * 64 * (D / 2) + lane * 2;
-    const float l1 = half_sum(l_run[1]);
-    const float m_give = kp ? m : m_run[1], l_give = kp ? l : l1;
-    m = kp ? m_run[1] : m;
-    l = kp ? l1 : l;
+    float* const gave_ml = reinterpret_cast<float*>(smem) + S::kWaves * 256 * kGave + lane * 2;
+    float m_give = m, l_give = l;
+    if constexpr (NB == 2) {
+      const float l1 = half_sum(l_run[1]);
+      m_give = kp ? m : m_run[1], l_give = kp ? l : l1;
+      m = kp ? m_run[1] : m;
+      l = kp ? l1 : l;
+    }
 #pragma unroll
-    for (int db = 0; db < kNdb; ++db) {
+    for (int db = 0; db < kOwn; ++db) {
 #pragma unroll
       for (int r4 = 0; r4 < 4; ++r4) {
         f32x4_t x;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          x[e] = kp ? o[0][db][4 * r4 + e] : o[1][db][4 * r4 + e];
-          acc[db][4 * r4 + e] = kp ? o[1][db][4 * r4 + e] : o[0][db][4 * r4 + e];
+          const float p0 = o[0][db][4 * r4 + e];
+          const float p1 = NB == 2 ? o[NB - 1][db][4 * r4 + e] : o[0][(db + kOwn) % kNdb][4 * r4 + e];
+          x[e] = kp ? p0 : p1;
+          acc[db][4 * r4 + e] = kp ? p1 : p0;
         }
-        *reinterpret_cast<f32x4_t*>(gave + (wave * (D / 8) + db * 4 + r4) * 256) = x;
+        *reinterpret_cast<f32x4_t*>(gave + (wave * kGave + db * 4 + r4) * 256) = x;
       }
     }
     gave_ml[wave * 128] = m_give;
     gave_ml[wave * 128 + 1] = l_give;
     __syncthreads();
-    const int other = wave ^ S::RW;  // the other key part of these rows
+    const int other = kp ? wave - S::RW : wave + S::RW;  // the other key part of these rows
     const float m2 = gave_ml[other * 128], l2 = gave_ml[other * 128 + 1];
     const float top = fmaxf(m, m2), sub = top == -__builtin_inff() ? 0.0f : top;
     const float w = __builtin_amdgcn_exp2f(m - sub), w2 = __builtin_amdgcn_exp2f(m2 - sub);
     m = top;
     l = l * w + l2 * w2;
 #pragma unroll
-    for (int db = 0; db < kNdb; ++db) {
+    for (int db = 0; db < kOwn; ++db) {
 #pragma unroll
       for (int r4 = 0; r4 < 4; ++r4) {
-        const f32x4_t x = *reinterpret_cast<const f32x4_t*>(gave + (other * (D / 8) + db * 4 + r4) * 256);
+        const f32x4_t x = *reinterpret_cast<const f32x4_t*>(gave + (other * kGave + db * 4 + r4) * 256);
 #pragma unroll
         for (int e = 0; e < 4; ++e) acc[db][4 * r4 + e] = acc[db][4 * r4 + e] * w + x[e] * w2;
       }
@@ -1320,7 +1329,7 @@ __global__ __launch_bounds__(S::kThreads) void paged_gqa_piece_kernel(PagedArgs 
   }
   // features 32 db + 16 j + 4 half + 0..3 and the same + 8: the halves exchange theirs for 8 in a row, from 8 half on
 #pragma unroll
-  for (int db = 0; db < kNdb; ++db) {
+  for (int db = 0; db < kOwn; ++db) {
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
 #pragma unroll
@@ -1335,13 +1344,13 @@ __global__ __launch_bounds__(S::kThreads) void paged_gqa_piece_kernel(PagedArgs 
   if (row >= it.rows - it.row0) return;
   if (job.split) {
     float* const at = a.part + job.slot * part_floats<S::kRows>(D);
-    if (half == 0) {
+    if (half == 0 && d_own == 0) {
       at[S::kRows * D + row * 2] = m;
       at[S::kRows * D + row * 2 + 1] = l;
     }
 #pragma unroll
-    for (int i = 0; i < 2 * kNdb; ++i) {
-      f32x4_t* const dst = reinterpret_cast<f32x4_t*>(at + row * D + 16 * i + 8 * half);
+    for (int i = 0; i < 2 * kOwn; ++i) {
+      f32x4_t* const dst = reinterpret_cast<f32x4_t*>(at + row * D + d_own + 16 * i + 8 * half);
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         const f32x16_t& x = acc[i / 2];
@@ -1355,11 +1364,11 @@ __global__ __launch_bounds__(S::kThreads) void paged_gqa_piece_kernel(PagedArgs 
   const int head_q = it.head * a.group + (it.rem0 + row - local * a.group);
   const int b = a.cu == nullptr ? it.req : 0;
   const int64_t tok = it.start + it.token0 + local;
-  uint16_t* const dst = a.o + b * a.os[0] + head_q * a.os[1] + tok * a.os[2] + 8 * half;
-  const uint16_t* const gate = a.gate == nullptr ? nullptr : a.gate + b * a.gs[0] + head_q * a.gs[1] + tok * a.gs[2] + 8 * half;
+  uint16_t* const dst = a.o + b * a.os[0] + head_q * a.os[1] + tok * a.os[2] + d_own + 8 * half;
+  const uint16_t* const gate = a.gate == nullptr ? nullptr : a.gate + b * a.gs[0] + head_q * a.gs[1] + tok * a.gs[2] + d_own + 8 * half;
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
-  for (int i = 0; i < 2 * kNdb; ++i) {
+  for (int i = 0; i < 2 * kOwn; ++i) {
     f32x8_t v;
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = acc[i / 2][8 * (i % 2) + e] * inv;
@@ -1449,9 +1458,10 @@ __global__ __launch_bounds__(256) void paged_gqa_join_kernel(PagedArgs a) {
   }
 }
 
-// 128 rows: two row blocks per wavefront up to 128 features; at 256 one (registers)
+// 128 rows (see the kernel): 4 wavefronts, at 128 features 8
 template <int D, bool FP8>
-using PieceOf = std::conditional_t<D == 256, Piece<D, FP8, 4, 1, 1>, Piece<D, FP8, 2, 2, 2>>;
+using PieceOf = std::conditional_t<D == 256, Piece<D, FP8, 4, 1, 1>,
+                                   std::conditional_t<D == 128, Piece<D, FP8, 4, 1, 2>, Piece<D, FP8, 2, 2, 2>>>;
 
 static_assert(Few<64, false, 1>::kPerCu == 2 && Few<64, true, 1>::kPerCu == 2 && Few<128, true, 1>::kPerCu == 2 &&
               Few<256, true, 1>::kPerCu == 2 && Few<64, false, 2>::kPerCu == 2 && Few<64, true, 2>::kPerCu == 2 &&
