@@ -48,23 +48,25 @@ def _check_rows(query, key, value, g, beta, cu_seqlens):
         raise ValueError("value must be on CUDA")
     if query.ndim != 4 or key.ndim != 4 or value.ndim != 4:
         raise ValueError("Expected query/key [B, T, Hk, Dk] and value [B, T, Hv, Dv]")
-    B, T, Hk, Dk = key.shape
-    Hv, Dv = value.shape[2], value.shape[3]
-    if query.shape != key.shape or value.shape[:2] != (B, T):
+    B, T, Hk, Dk = shape = key.shape
+    Bv, Tv, Hv, Dv = value.shape
+    if query.shape != shape or Bv != B or Tv != T:
         raise ValueError("query and key must match, and value must share their [B, T]")
     if Dk != 128 or Dv != 128:
         raise ValueError("head dims must be 128")
     if Hv % Hk:
         raise ValueError(f"value heads ({Hv}) must be a multiple of key heads ({Hk})")
+    device, bf16 = value.get_device(), torch.bfloat16  # an index: comparing it costs a third of comparing devices
     for name, t in (("query", query), ("key", key), ("value", value)):
-        if t.dtype != torch.bfloat16 or not t.is_contiguous() or t.device != value.device:
+        if t.dtype != bf16 or not t.is_contiguous() or t.get_device() != device:
             raise ValueError(f"{name} must be contiguous BF16 on value's device")
-    if g.shape != (B, T, Hv) or g.dtype != torch.float32 or not g.is_contiguous() or g.device != value.device:
+    gates = (B, T, Hv)
+    if g.shape != gates or g.dtype != torch.float32 or not g.is_contiguous() or g.get_device() != device:
         raise ValueError(f"g must be a contiguous float32 tensor [{B}, {T}, {Hv}] on value's device")
-    if (beta.shape != (B, T, Hv) or beta.dtype not in (torch.bfloat16, torch.float32) or not beta.is_contiguous()
-            or beta.device != value.device):
+    if (beta.shape != gates or (beta.dtype != bf16 and beta.dtype != torch.float32) or not beta.is_contiguous()
+            or beta.get_device() != device):
         raise ValueError(f"beta must be a contiguous BF16 or float32 tensor [{B}, {T}, {Hv}] on value's device")
-    if any(t.data_ptr() % 16 for t in (query, key, value)):
+    if (query.data_ptr() | key.data_ptr() | value.data_ptr()) & 15:
         raise ValueError("query, key and value must be aligned to 16 bytes")
 
     n_seqs = 0
