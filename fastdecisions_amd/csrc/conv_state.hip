@@ -265,7 +265,7 @@ extern "C" int fd_packed_conv_state(const void* x, int64_t x_row_stride, const v
   a.n_runs = body ? static_cast<int>((rows + kRun - 1) / kRun) : 0;
   const int64_t heads = (static_cast<int64_t>(requests) * a.n_col + kNumXcd - 1) / kNumXcd * kNumXcd;
   const int64_t bodies = (static_cast<int64_t>(a.n_runs) * a.n_col + kNumXcd - 1) / kNumXcd * kNumXcd;
-  FD_REQUIRE(heads + bodies < (1LL << 31), FD_ERR_UNSUPPORTED, "%s: grid too large", what);
+  FD_REQUIRE(heads + bodies < (1LL << 32) / kThreads, FD_ERR_UNSUPPORTED, "%s: grid too large", what);
   a.head_blocks = static_cast<int>(heads);
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (width == 2) launch<2>(a, activation == FD_ACT_SILU, heads + bodies, s);

@@ -194,7 +194,7 @@ extern "C" int fd_gated_delta_step(const void* q, const void* k, const void* v, 
              "%s: the state needs a row for every request", what);
   const int64_t rows = static_cast<int64_t>(batch) * seq_len;
   const int64_t blocks = static_cast<int64_t>(requests) * v_heads * (kD / kCols);
-  FD_REQUIRE(rows < (1LL << 31) && blocks < (1LL << 31), FD_ERR_UNSUPPORTED, "%s: problem too large", what);
+  FD_REQUIRE(rows < (1LL << 31) && blocks < (1LL << 32) / 64, FD_ERR_UNSUPPORTED, "%s: problem too large", what);
   if (blocks == 0) return FD_OK;
   const StepArgs a{static_cast<const uint16_t*>(q), static_cast<const uint16_t*>(k), static_cast<const uint16_t*>(v), g,
                    beta, static_cast<uint16_t*>(out), state, state_out, state_indices, cu_seqlens,

@@ -84,18 +84,6 @@ __device__ __forceinline__ int request_keys(const PagedView& c, int r) {
   return min(max(c.lens[r], 0), c.max_pages << c.shift);
 }
 
-// The request of packed row t (the last one that starts at or before it), or -1
-// for a row behind the last request.
-__device__ __forceinline__ int request_of(const int32_t* cu, int n_seqs, int t) {
-  int lo = 0, hi = n_seqs;  // cu[lo] <= t < cu[hi], where the table is well formed
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (cu[mid] <= t) lo = mid;
-    else hi = mid;
-  }
-  return cu[lo] <= t && t < cu[lo + 1] ? lo : -1;
-}
-
 // Scale byte -> 2^(byte - 127).
 __device__ __forceinline__ float scale_of(uint32_t byte) { return __uint_as_float(byte << 23); }
 

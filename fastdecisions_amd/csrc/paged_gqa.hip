@@ -1591,7 +1591,7 @@ extern "C" int fd_paged_gqa_fwd(const void* q, const fd_paged_cache* cache, cons
   const bool fp8 = cache->dtype == FD_DTYPE_E4M3;
   const Plan p = plan_of(requests, static_cast<int64_t>(batch) * seq_len, q_heads / cache->kv_heads, cache->kv_heads,
                          cache->head_dim, static_cast<int64_t>(cache->max_pages) * cache->page_size, max_seqlen, fp8);
-  FD_REQUIRE(p.items < (1LL << 30), FD_ERR_UNSUPPORTED, "%s: problem too large", what);
+  FD_REQUIRE(p.items < (1LL << 32) / 512 - kNumXcd, FD_ERR_UNSUPPORTED, "%s: problem too large", what);
   FD_REQUIRE(p.bytes == 0 || (workspace && fd_aligned16(workspace) && workspace_bytes >= p.bytes),
              FD_ERR_INVALID_ARGUMENT, "%s: the workspace must be 16-byte aligned and hold %lld bytes", what,
              static_cast<long long>(p.bytes));

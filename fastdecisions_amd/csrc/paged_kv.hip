@@ -11,9 +11,10 @@
 // smallest step), so the one rounding is the conversion's; floating codes lose
 // nothing to a scale that is not the tightest, except a binade of subnormals.
 //
-// Measured (4 heads x 128): 64 tokens 3.5 us, the launch; prompts of 24 MB (bf16 in, E4M3 out)
-// 10.4 us, 2.3 TB/s, and 37 MB read back (E4M3 in, bf16 out) 13.1 us, 2.8 TB/s: a few microseconds of
-// launch and of the page table's, then the pages' latencies besides the bytes' 4.6 and 7.2.
+// Measured (4 heads x 128): 64 tokens 3.3 us, the launch; prompts of 24 MB (bf16 in, E4M3 out) 10.2 us,
+// 2.3 TB/s, 37 MB read back (E4M3 in, bf16 out) 9.4 to 13 us (in or out of the last-level cache): a few microseconds of
+// launch and of the page table's, then the pages' latencies besides the bytes' 4.6 and 7.2.  Long calls
+// reach 4.8 TB/s.
 #include <initializer_list>
 #include <type_traits>
 
@@ -23,6 +24,12 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr float kE4m3Max = 448.0f;
+// A thread takes several rows, their chains of loads side by side, once there is more than a round (write) or a few
+// rounds (read) of workgroups: 1024 of a side (K, V) run at once.  Measured with 1, 2, 4 rows (us, 4 heads x 128 bf16):
+// write 1.2, 5 and 48 thousand tokens 4.0, 4.1, 4.1; 9.6, 9.3, 10.0; 39, 40, 41, E4M3 40, 38, 41; read 12 and 96
+// thousand 9.3, 9.4, 9.7; 120, 105, 81 (4.8 TB/s), E4M3 121, 108, 83.
+constexpr int kAtOnce = 1024;
+constexpr int kRows = 2, kManyRows = 4;  // beyond kAtOnce workgroups; of a read beyond four times as many
 
 struct WriteArgs {
   const uint16_t* x[2];       // k, v
@@ -56,73 +63,107 @@ __device__ __forceinline__ float to_code_range(float x, float inv) {
   return y != y ? y : fminf(fmaxf(y, -kE4m3Max), kE4m3Max);
 }
 
-template <int D, bool FP8>
+// The requests of U packed rows (the last one that starts at or before each; -1 for a row behind the last request),
+// searched side by side: their loads are in flight together.
+template <int U>
+__device__ __forceinline__ void requests_of(const int32_t* cu, int n_seqs, const int (&t)[U], int (&r)[U]) {
+  int hi[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) r[u] = 0, hi[u] = n_seqs;
+  for (int width = n_seqs; width > 1; width = (width + 1) >> 1) {
+    int at[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) at[u] = cu[(r[u] + hi[u]) >> 1];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int mid = (r[u] + hi[u]) >> 1;
+      if (hi[u] - r[u] > 1) (at[u] <= t[u] ? r[u] : hi[u]) = mid;
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+    if (!(cu[r[u]] <= t[u] && t[u] < cu[r[u] + 1])) r[u] = -1;
+}
+
+// U rows per thread, kThreads / kLanes apart, a stage of all of them at a time: rows, requests, pages, stores.
+template <int D, bool FP8, int U>
 __global__ __launch_bounds__(kThreads) void paged_kv_write_kernel(WriteArgs a) {
-  constexpr int kLanes = D / 8;  // lanes of a row
+  constexpr int kLanes = D / 8, kSide = kThreads / kLanes;  // lanes of a row; rows of a workgroup side by side
   const int side = blockIdx.y;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * (kThreads / kLanes) + threadIdx.x / kLanes;
   const int li = threadIdx.x % kLanes;
-  const int64_t token = row / a.kv_heads;
-  const int head = static_cast<int>(row - token * a.kv_heads);
+  const uint16_t* const x_side = side == 0 ? a.x[0] : a.x[1];
+  const int64_t xb = side == 0 ? a.xs[0][0] : a.xs[1][0], xh = side == 0 ? a.xs[0][1] : a.xs[1][1],
+                xt = side == 0 ? a.xs[0][2] : a.xs[1][2];
   const int64_t tokens = static_cast<int64_t>(a.batch) * a.seq_len;
-  bool live = token < tokens;
-  int b = 0, t = 0, r = 0, start = 0, end = 0;
-  if (live) {
-    if (a.cu == nullptr) {
-      r = b = static_cast<int>(token / a.seq_len);
-      t = static_cast<int>(token - static_cast<int64_t>(b) * a.seq_len);
+  int head[U], t[U], r[U], pos[U], page[U];
+  uint4 w[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int64_t row = (static_cast<int64_t>(blockIdx.x) * U + u) * kSide + threadIdx.x / kLanes;
+    const int64_t token = row / a.kv_heads;
+    head[u] = static_cast<int>(row - token * a.kv_heads);
+    const int b = a.cu == nullptr ? static_cast<int>(token / a.seq_len) : 0;
+    t[u] = static_cast<int>(token - static_cast<int64_t>(b) * a.seq_len);
+    r[u] = token < tokens ? b : -1;
+    w[u] = {0, 0, 0, 0};
+    if (token < tokens) w[u] = *reinterpret_cast<const uint4*>(x_side + b * xb + head[u] * xh + t[u] * xt + li * 8);
+  }
+  if (a.cu != nullptr) {
+    int found[U];
+    requests_of<U>(a.cu, a.n_seqs, t, found);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (r[u] >= 0) r[u] = found[u];
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    int start, end;
+    request_rows(a.cu, max(r[u], 0), a.seq_len, &start, &end);
+    const int len = request_keys(a.c, max(r[u], 0));
+    pos[u] = len - (end - start) + (t[u] - start);
+    if (r[u] < 0 || pos[u] >= len) pos[u] = -1;
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+    page[u] = pos[u] >= 0 ? a.c.table[r[u] * a.c.table_stride + (pos[u] >> a.c.shift)] : -1;
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const bool live = static_cast<unsigned>(page[u]) < static_cast<unsigned>(a.c.n_pages);
+    const int at = pos[u] & ((1 << a.c.shift) - 1);
+    unsigned char* dst = (side == 0 ? a.c.k : a.c.v) + page[u] * a.c.page + head[u] * a.c.head + at * a.c.row;
+    if constexpr (!FP8) {
+      if (live) *reinterpret_cast<uint4*>(dst + li * 16) = w[u];
     } else {
-      t = static_cast<int>(token);
-      r = request_of(a.cu, a.n_seqs, t);
-      live = r >= 0;
-    }
-  }
-  uint4 w = {0, 0, 0, 0};
-  int pos = 0, page = -1;
-  if (live) {
-    const uint16_t* x = side == 0 ? a.x[0] : a.x[1];
-    const int64_t xb = side == 0 ? a.xs[0][0] : a.xs[1][0], xh = side == 0 ? a.xs[0][1] : a.xs[1][1],
-                  xt = side == 0 ? a.xs[0][2] : a.xs[1][2];
-    w = *reinterpret_cast<const uint4*>(x + b * xb + head * xh + t * xt + li * 8);
-    request_rows(a.cu, r, a.seq_len, &start, &end);
-    const int len = request_keys(a.c, r);
-    pos = len - (end - start) + (t - start);
-    if (pos >= 0 && pos < len) page = a.c.table[r * a.c.table_stride + (pos >> a.c.shift)];
-  }
-  live = static_cast<unsigned>(page) < static_cast<unsigned>(a.c.n_pages);
-  const int at = pos & ((1 << a.c.shift) - 1);
-  unsigned char* dst = (side == 0 ? a.c.k : a.c.v) + page * a.c.page + head * a.c.head + at * a.c.row;
-  if constexpr (!FP8) {
-    if (live) *reinterpret_cast<uint4*>(dst + li * 16) = w;
-  } else {
-    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-    float x[8], top = 0.0f;
+      const uint32_t h[4] = {w[u].x, w[u].y, w[u].z, w[u].w};
+      float x[8], top = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      x[2 * i] = fd_lo(u[i]);
-      x[2 * i + 1] = fd_hi(u[i]);
-    }
+      for (int i = 0; i < 4; ++i) {
+        x[2 * i] = fd_lo(h[i]);
+        x[2 * i + 1] = fd_hi(h[i]);
+      }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float m = fabsf(x[i]);
-      top = fmaxf(top, m < __builtin_inff() ? m : 0.0f);  // finite values only
-    }
-    top = group_max<kLanes>(top);  // every lane of the wavefront takes part
-    const int byte = scale_byte(top);
-    const float inv = __uint_as_float(static_cast<uint32_t>(254 - byte) << 23);  // 2^-E
-    float y[8];
+      for (int i = 0; i < 8; ++i) {
+        const float m = fabsf(x[i]);
+        top = fmaxf(top, m < __builtin_inff() ? m : 0.0f);  // finite values only
+      }
+      top = group_max<kLanes>(top);  // every lane of the wavefront takes part
+      const int byte = scale_byte(top);
+      const float inv = __uint_as_float(static_cast<uint32_t>(254 - byte) << 23);  // 2^-E
+      float y[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = to_code_range(x[i], inv);
-    uint2 code;
-    int lo = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
-    lo = __builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], lo, true);
-    int hi = __builtin_amdgcn_cvt_pk_fp8_f32(y[4], y[5], 0, false);
-    hi = __builtin_amdgcn_cvt_pk_fp8_f32(y[6], y[7], hi, true);
-    code.x = static_cast<uint32_t>(lo);
-    code.y = static_cast<uint32_t>(hi);
-    if (live) {
-      *reinterpret_cast<uint2*>(dst + li * 8) = code;
-      if (li == 0) (side == 0 ? a.c.k_scale : a.c.v_scale)[page * a.c.s_page + head * a.c.s_head + at] = static_cast<uint8_t>(byte);
+      for (int i = 0; i < 8; ++i) y[i] = to_code_range(x[i], inv);
+      uint2 code;
+      int lo = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
+      lo = __builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], lo, true);
+      int hi = __builtin_amdgcn_cvt_pk_fp8_f32(y[4], y[5], 0, false);
+      hi = __builtin_amdgcn_cvt_pk_fp8_f32(y[6], y[7], hi, true);
+      code.x = static_cast<uint32_t>(lo);
+      code.y = static_cast<uint32_t>(hi);
+      if (live) {
+        *reinterpret_cast<uint2*>(dst + li * 8) = code;
+        if (li == 0)
+          (side == 0 ? a.c.k_scale : a.c.v_scale)[page[u] * a.c.s_page + head[u] * a.c.s_head + at] = static_cast<uint8_t>(byte);
+      }
     }
   }
 }
@@ -136,41 +177,66 @@ struct ReadArgs {
   int total;
 };
 
-template <int D, bool FP8>
+template <int D, bool FP8, int U>
 __global__ __launch_bounds__(kThreads) void paged_kv_read_kernel(ReadArgs a) {
-  constexpr int kLanes = D / 8;
+  constexpr int kLanes = D / 8, kSide = kThreads / kLanes;
   const int side = blockIdx.y;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * (kThreads / kLanes) + threadIdx.x / kLanes;
   const int li = threadIdx.x % kLanes;
-  const int64_t t = row / a.kv_heads;
-  const int head = static_cast<int>(row - t * a.kv_heads);
-  if (t >= a.total) return;
-  const int r = request_of(a.cu, a.n_seqs, static_cast<int>(t));
-  if (r < 0) return;
-  const int key = static_cast<int>(t) - max(a.cu[r], 0);
-  const int slot = key >> a.c.shift, at = key & ((1 << a.c.shift) - 1);
-  const int page = slot < a.c.max_pages ? a.c.table[r * a.c.table_stride + slot] : -1;
-  uint4 w = {0, 0, 0, 0};
-  if (static_cast<unsigned>(page) < static_cast<unsigned>(a.c.n_pages)) {
-    const unsigned char* src = (side == 0 ? a.c.k : a.c.v) + page * a.c.page + head * a.c.head + at * a.c.row;
-    if constexpr (!FP8) {
-      w = *reinterpret_cast<const uint4*>(src + li * 16);
-    } else {
-      const uint2 code = *reinterpret_cast<const uint2*>(src + li * 8);
-      const float s = scale_of((side == 0 ? a.c.k_scale : a.c.v_scale)[page * a.c.s_page + head * a.c.s_head + at]);
-      typedef float f32x2_t __attribute__((ext_vector_type(2)));
-      const f32x2_t f0 = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(code.x), false);
-      const f32x2_t f1 = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(code.x), true);
-      const f32x2_t f2 = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(code.y), false);
-      const f32x2_t f3 = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(code.y), true);
-      w.x = fd_pack2(f0[0] * s, f0[1] * s);
-      w.y = fd_pack2(f1[0] * s, f1[1] * s);
-      w.z = fd_pack2(f2[0] * s, f2[1] * s);
-      w.w = fd_pack2(f3[0] * s, f3[1] * s);
+  int head[U], t[U], r[U], key[U], page[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int64_t row = (static_cast<int64_t>(blockIdx.x) * U + u) * kSide + threadIdx.x / kLanes;
+    const int64_t token = row / a.kv_heads;
+    head[u] = static_cast<int>(row - token * a.kv_heads);
+    t[u] = token < a.total ? static_cast<int>(token) : -1;
+  }
+  requests_of<U>(a.cu, a.n_seqs, t, r);
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    if (t[u] < 0) r[u] = -1;
+    key[u] = t[u] - max(a.cu[max(r[u], 0)], 0);
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int slot = key[u] >> a.c.shift;
+    page[u] = r[u] >= 0 && slot < a.c.max_pages ? a.c.table[r[u] * a.c.table_stride + slot] : -1;
+  }
+  uint4 w[U];
+  uint8_t byte[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int at = key[u] & ((1 << a.c.shift) - 1);
+    w[u] = {0, 0, 0, 0};
+    byte[u] = 0;
+    if (static_cast<unsigned>(page[u]) < static_cast<unsigned>(a.c.n_pages)) {
+      const unsigned char* src = (side == 0 ? a.c.k : a.c.v) + page[u] * a.c.page + head[u] * a.c.head + at * a.c.row;
+      if constexpr (!FP8) {
+        w[u] = *reinterpret_cast<const uint4*>(src + li * 16);
+      } else {
+        const uint2 code = *reinterpret_cast<const uint2*>(src + li * 8);
+        w[u].x = code.x, w[u].y = code.y;
+        byte[u] = (side == 0 ? a.c.k_scale : a.c.v_scale)[page[u] * a.c.s_page + head[u] * a.c.s_head + at];
+      }
     }
   }
-  uint16_t* out = side == 0 ? a.out[0] + head * a.os[0][0] + t * a.os[0][1] : a.out[1] + head * a.os[1][0] + t * a.os[1][1];
-  *reinterpret_cast<uint4*>(out + li * 8) = w;
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    if (r[u] < 0) continue;
+    if constexpr (FP8) {  // codes of no page are zeros, whatever their scale
+      const float s = scale_of(byte[u]);
+      typedef float f32x2_t __attribute__((ext_vector_type(2)));
+      const f32x2_t f0 = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(w[u].x), false);
+      const f32x2_t f1 = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(w[u].x), true);
+      const f32x2_t f2 = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(w[u].y), false);
+      const f32x2_t f3 = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(w[u].y), true);
+      w[u].x = fd_pack2(f0[0] * s, f0[1] * s);
+      w[u].y = fd_pack2(f1[0] * s, f1[1] * s);
+      w[u].z = fd_pack2(f2[0] * s, f2[1] * s);
+      w[u].w = fd_pack2(f3[0] * s, f3[1] * s);
+    }
+    uint16_t* out = side == 0 ? a.out[0] + head[u] * a.os[0][0] + t[u] * a.os[0][1] : a.out[1] + head[u] * a.os[1][0] + t[u] * a.os[1][1];
+    *reinterpret_cast<uint4*>(out + li * 8) = w[u];
+  }
 }
 
 template <typename F>
@@ -210,16 +276,17 @@ extern "C" int fd_paged_kv_write(const void* k, const void* v, const int64_t k_s
   const int64_t rows = static_cast<int64_t>(batch) * seq_len * cache->kv_heads;
   const int per = kThreads / (cache->head_dim / 8);
   const int64_t blocks = (rows + per - 1) / per;
-  FD_REQUIRE(blocks < (1LL << 31), FD_ERR_UNSUPPORTED, "%s: too many rows", what);
+  FD_REQUIRE(blocks < (1LL << 32) / kThreads, FD_ERR_UNSUPPORTED, "%s: too many rows", what);
   if (blocks == 0) return FD_OK;
   const bool fp8 = cache->dtype == FD_DTYPE_E4M3;
   by_head_dim(cache->head_dim, [&](auto d) {
     constexpr int D = decltype(d)::value;
-    const dim3 grid(static_cast<unsigned>(blocks), 2);
-    if (fp8)
-      hipLaunchKernelGGL((paged_kv_write_kernel<D, true>), grid, dim3(kThreads), 0, static_cast<hipStream_t>(stream), a);
-    else
-      hipLaunchKernelGGL((paged_kv_write_kernel<D, false>), grid, dim3(kThreads), 0, static_cast<hipStream_t>(stream), a);
+    auto go = [&](auto kernel, int rows) {
+      const dim3 grid(static_cast<unsigned>((blocks + rows - 1) / rows), 2);
+      hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, static_cast<hipStream_t>(stream), a);
+    };
+    if (blocks <= kAtOnce) fp8 ? go(paged_kv_write_kernel<D, true, 1>, 1) : go(paged_kv_write_kernel<D, false, 1>, 1);
+    else fp8 ? go(paged_kv_write_kernel<D, true, kRows>, kRows) : go(paged_kv_write_kernel<D, false, kRows>, kRows);
   });
   return fd_check_launch(what);
 }
@@ -249,16 +316,18 @@ extern "C" int fd_paged_kv_read(const fd_paged_cache* cache, void* k_out, void* 
   a.total = static_cast<int>(total);
   const int per = kThreads / (cache->head_dim / 8);
   const int64_t blocks = (total * cache->kv_heads + per - 1) / per;
-  FD_REQUIRE(blocks < (1LL << 31), FD_ERR_UNSUPPORTED, "%s: too many rows", what);
+  FD_REQUIRE(blocks < (1LL << 32) / kThreads, FD_ERR_UNSUPPORTED, "%s: too many rows", what);
   if (blocks == 0) return FD_OK;
   const bool fp8 = cache->dtype == FD_DTYPE_E4M3;
   by_head_dim(cache->head_dim, [&](auto d) {
     constexpr int D = decltype(d)::value;
-    const dim3 grid(static_cast<unsigned>(blocks), 2);
-    if (fp8)
-      hipLaunchKernelGGL((paged_kv_read_kernel<D, true>), grid, dim3(kThreads), 0, static_cast<hipStream_t>(stream), a);
-    else
-      hipLaunchKernelGGL((paged_kv_read_kernel<D, false>), grid, dim3(kThreads), 0, static_cast<hipStream_t>(stream), a);
+    auto go = [&](auto kernel, int rows) {
+      const dim3 grid(static_cast<unsigned>((blocks + rows - 1) / rows), 2);
+      hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, static_cast<hipStream_t>(stream), a);
+    };
+    if (blocks <= kAtOnce) fp8 ? go(paged_kv_read_kernel<D, true, 1>, 1) : go(paged_kv_read_kernel<D, false, 1>, 1);
+    else if (blocks <= 4 * kAtOnce) fp8 ? go(paged_kv_read_kernel<D, true, kRows>, kRows) : go(paged_kv_read_kernel<D, false, kRows>, kRows);
+    else fp8 ? go(paged_kv_read_kernel<D, true, kManyRows>, kManyRows) : go(paged_kv_read_kernel<D, false, kManyRows>, kManyRows);
   });
   return fd_check_launch(what);
 }

@@ -136,6 +136,18 @@ def test_tensors_that_do_not_fit_are_refused():
         paged_gqa_attention(x.expand(2, -1, -1, -1), k, k, table, lens, cu_seqlens=torch.zeros(3, dtype=torch.int32))
 
 
+def test_calls_larger_than_a_grid_are_refused():
+    """A grid dimension's threads fit 32 bits."""
+    lib, c, uns = _cache_lib.lib(), cache(), _lib.FD_ERR_UNSUPPORTED
+    s4, s2 = (ctypes.c_int64 * 4)(512, 128, 512, 1), (ctypes.c_int64 * 2)(128, 512)
+    assert lib.fd_paged_kv_read(ctypes.byref(c), FAKE, FAKE, s2, s2, 1 << 30, FAKE, 1, None) == uns
+    assert lib.fd_paged_kv_write(FAKE, FAKE, s4, s4, ctypes.byref(c), 1 << 15, 1 << 15, None, 0, None) == uns
+    assert lib.fd_gated_delta_step(FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, None, None, 0, None, 1 << 22, 1, 16, 16, 128, 128,
+                                   0.1, _lib.FD_DTYPE_BF16, 0, None, 0, None) == uns
+    assert lib.fd_packed_conv_state(FAKE, 6144, FAKE, None, FAKE, FAKE, 1 << 26, None, FAKE, FAKE, FAKE, 1 << 26, 1, 2048,
+                                    2048, 4, None, 0, _lib.FD_ACT_SILU, None) == uns
+
+
 def test_more_query_heads_per_key_head_than_a_row_count_holds_are_refused():
     from fastdecisions_amd.paged_gqa_kernel import paged_gqa_attention
     lib = _cache_lib.lib()

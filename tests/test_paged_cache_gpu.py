@@ -447,6 +447,34 @@ def test_read_back(heads, dim, page, fp8):
     assert (out[total:] == 3.0).all()
 
 
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_long_calls(dim, fp8):
+    """Calls in which a thread writes and reads several rows: bits as of the short calls' one, packed requests of
+    every length, a request without tokens among them, a last workgroup that is not full."""
+    from fastdecisions_amd.paged_kv_kernel import paged_kv_read, paged_kv_write
+    heads, page = 1024 // dim, 32
+    new = [7000, 1, 0, 33, 6001, 4200]
+    cached = [20, 511, 9, 0, 250, 1]
+    lens = [a + b for a, b in zip(cached, new)]
+    announce(f"paged write and read, long calls {heads} x {dim}, fp8 {fp8}")
+    c = make_pages(lens, page, heads, dim, fp8, seed=24)
+    k, v = (new_rows(new, heads, dim, 25 + i, True) for i in range(2))
+    at = starts(new)
+    paged_kv_write(k, v, c["k"], c["v"], c["table"], ints(lens), cu_seqlens=ints(at), **scales(c))
+    all_at = starts(lens)
+    got = paged_kv_read(c["k"], c["v"], c["table"], ints(all_at), all_at[-1], **scales(c))
+    for name, x, out in zip(("k", "v"), (k, v), got):
+        for r, n in enumerate(new):
+            want, there = rows(c, name, r, lens[r])
+            assert there.all() and torch.equal(out[0, :, all_at[r]:all_at[r + 1]], want.to(torch.bfloat16)), (name, r)
+            mine = x[0, :, at[r]:at[r + 1]]
+            if fp8:
+                codes, scale = e4m3(mine.double())
+                mine = (codes * pow2(scale)[..., None]).to(torch.bfloat16)
+            assert torch.equal(out[0, :, all_at[r] + cached[r]:all_at[r + 1]], mine), (name, r)
+
+
 def test_written_then_attended_then_read():
     """A run as a program makes it: a prompt in pieces and then tokens one by one, quantised, equal to
     attention over everything at once."""
