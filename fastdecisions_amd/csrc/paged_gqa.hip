@@ -176,6 +176,18 @@ __device__ __forceinline__ int best_range(const PagedArgs& a, int rt, int kt, in
   return best;
 }
 
+// Row tile at place j of n of a key range, of which XCDs take runs of `per` items: the later tiles see more keys, so
+// they go first, and where a range's tiles fill q runs, run s takes every q-th of them (one half of the tiles in a row
+// would be three quarters of the work).  Prompts without a prefix, 16/4 heads x 128: 6000 tokens 240 -> 197 us, 16384
+// 1440 -> 1103 (1000 TFLOP/s); at most one tile per CU the same.
+__device__ __forceinline__ int spread(int j, int n, int per) {
+  const int q = min(max((n + per / 2) / per, 1), n), whole = n / q, more = n - whole * q;  // the first `more` runs have one more
+  const int late = j - more * (whole + 1);
+  const int s = late < 0 ? j / (whole + 1) : more + late / whole;
+  const int i = late < 0 ? j - s * (whole + 1) : late - (s - more) * whole;
+  return n - 1 - (i * q + s);
+}
+
 // Finds work item `want(total items)` (JOIN: row tile, whatever its ranges).  One wavefront
 // looks at 64 requests at a time; false if there is no such item.  Beyond 64 requests ranges are a round's share.
 template <int ROWS, int KEYS, bool JOIN, typename Want>
@@ -259,6 +271,7 @@ __device__ __forceinline__ bool find_item(const PagedArgs& a, int lane, Want wan
       it->len = at_lane(len, l);
       it->tiles = max(tiles_over(at_lane(kt, l), it->n_ranges), 1);  // a request's ranges are alike
       it->rtile = k % it->n_rtiles;  // row tiles of a key range one after the other: they share its keys
+      if constexpr (!JOIN && ROWS >= 128) it->rtile = spread(it->rtile, it->n_rtiles, (total + kNumXcd - 1) / kNumXcd);
       const int hr = k / it->n_rtiles;
       it->range = JOIN ? 0 : hr % it->n_ranges;
       it->head = JOIN ? hr : hr / it->n_ranges;
@@ -804,11 +817,11 @@ __device__ __forceinline__ void pieces(int m, F f) {
 // read a phase before it is used.  Four LDS stages: bf16 tiles are copied three steps ahead (asm copies,
 // counted by hand), codes are loaded into registers three steps ahead and stored as bf16 two ahead.
 //
-// Measured, 2048 new tokens on 6144 cached ones: 16 / 4 heads x 128 features 141 us, 850 TFLOP/s (14336 cached
-// 263 us, 978; a large library product here: 1370), x 64 104 us, 8 / 2 x 256 148 us, 810; E4M3 163, 127 and
-// 175.  2048 tokens alone: 42 us.  A workgroup spends 1.6 us on finding its item, 3.4 until its first tiles
-// and Q are there, 1.1 per whole tile of 64 keys, 1.3 on the last one, 2 to 3.4 on the masked ones, 2.7 on
-// its rows.  In the loop MFMA, VALU, and LDS reads are each busy for a third to a half of the time, with a
+// Measured, 2048 new tokens on 6144 cached ones: 16 / 4 heads x 128 features 142 us, 845 TFLOP/s (14336 cached
+// 263 us, 978; a large library product here: 1370), x 64 104 us, 8 / 2 x 256 148 us, 810; E4M3 164, 127 and
+// 175.  2048 tokens alone: 42 to 46 us.  A workgroup (128 features) spends 1.8 us on finding its item, 3.4 to 3.9 until
+// its first tiles and Q are there, 1.05 per whole tile of 64 keys, 0.7 on the last one, 1.9 to 3 on the masked ones, 1.9
+// on its rows.  In the loop MFMA, VALU, and LDS reads are each busy for a third to a half of the time, with a
 // barrier per tile.  LDS conflicts are not the bound: E4M3's 8% of cycles could be removed without any gain.
 template <class S>
 __global__ __launch_bounds__(S::kThreads) void paged_gqa_piece_kernel(PagedArgs a) {

@@ -87,6 +87,17 @@ def test_packed_suffixes(hq, hkv, dim, page, gated, fp8):
     check_attention(c, q, out, lens, new, gate=gate)
 
 
+@pytest.mark.parametrize("hq,hkv,dim", [(16, 4, 64), (3, 1, 128), (4, 2, 256)])
+@pytest.mark.parametrize("new", [[5000], [2900, 33, 700, 1], [1333, 1400, 1500]])
+def test_prompts_of_many_row_tiles(new, hq, hkv, dim):
+    """Row tiles that fill several rounds of workgroups and are dealt to the XCDs: every one once."""
+    announce(f"paged attention, prompts {new}, {hq}/{hkv} x {dim}")
+    c = make_pages(new, 64, hkv, dim, False, seed=26)
+    q = make_q(new, hq, dim, 27)
+    out = run_attention(c, q, new, new)
+    check_attention(c, q, out, new, new)
+
+
 @pytest.mark.parametrize("few", [True, False])
 @pytest.mark.parametrize("dim", [64, 128, 256])
 def test_either_kernel_takes_any_lengths(dim, few):
