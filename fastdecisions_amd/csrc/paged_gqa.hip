@@ -1494,18 +1494,18 @@ Plan plan_of(int64_t requests, int64_t tokens, int group, int kv_heads, int head
   Plan p;
   const int64_t rows = static_cast<int64_t>(max_seqlen) * group;
   // Measured with 16 rows, 32 rows and pieces (us; 16/4 heads x 128 unless noted, 64 requests on 2048 keys):
-  //   rows  32: 46, 52, 51; 8/2 x 256 49, 59, 58; E4M3 34, 37, 59      -> two tiles of 16 rows
-  //   rows  64: 69, 49, 52; 8/2 x 256 81, 57, 61; E4M3 59, 45, 59      -> two of 32, but 256 features with E4M3, whose
-  //             46, 53, 62                                              kernel for 32 rows fills a CU alone: four of 16
-  //   rows  96: 92, 72, 53; 8/2 x 256 119, 104, 66; E4M3 84, 68, 60    -> pieces, unless the call is so small that
-  //             one request of 4096 keys 19, 19, 24                     latency counts, up to 128 rows in all
+  //   rows 32: 46, 52, 51; 8/2 x 256 49, 60, 59; E4M3 35, 38, 55: two tiles of 16 rows
+  //   rows 64: 68, 49, 52; 8/2 x 256 82, 57, 61; E4M3 62, 47, 52: two of 32; 8/2 x 256 with E4M3 46, 53, 61, whose kernel
+  //            for 32 rows fills a CU alone: four of 16
+  //   rows 96: 98, 72, 53; 8/2 x 256 120, 104, 66; E4M3 84, 69, 53: pieces, unless the call is so small that latency
+  //            counts, up to 128 rows in all (one request of 4096 keys 19, 19, 24)
   const int64_t all_rows = tokens * group;
   p.few = rows <= 32 ? 1 : rows > 64 && (all_rows > 128 || max_keys > 16384) ? 0 : head_dim == 256 && fp8 ? 1 : 2;
   p.rows = p.few ? 16 * p.few : PieceOf<64, false>::kRows;
   p.keys = p.few ? Few<64, false, 1>::kKeys
                  : head_dim == 64 ? PieceOf<64, false>::kKeys : head_dim == 128 ? PieceOf<128, false>::kKeys : PieceOf<256, false>::kKeys;
-  // Workgroups per CU.  Few rows: by LDS (Few::kPerCu).  Pieces with 64 features: 249 registers and 64 KiB of LDS, two
-  // (2048 tokens on 6144 keys, 16/4 heads: 103 us with ranges for two, 114 for one); with E4M3 267 registers and one
+  // Workgroups per CU.  Few rows: by LDS (Few::kPerCu).  Pieces with 64 features: 245 registers and 64 KiB of LDS, two
+  // (2048 tokens on 6144 keys, 16/4 heads: 103 us with ranges for two, 114 for one); with E4M3 265 registers and one
   // (137 us; 150 with ranges for two).
   const int per_cu = p.few == 1   ? (head_dim == 256 && !fp8 ? Few<256, false, 1>::kPerCu : Few<128, false, 1>::kPerCu)
                      : p.few == 2 ? (head_dim == 256 ? Few<256, false, 2>::kPerCu : Few<128, false, 2>::kPerCu)
