@@ -173,6 +173,8 @@ def paged_kv_read(
     strides = (total * heads * dim, dim, heads * dim, 1)
     k = torch.empty_strided((1, heads, total, dim), strides, device=k_cache.device, dtype=_BF16)
     v = torch.empty_like(k)
+    if total == 0:
+        return k, v
     at = _cache_lib.pack2(dim, heads * dim)
     _cache_lib.check("fd_paged_kv_read", _cache_lib.lib().fd_paged_kv_read(
         cache, k.data_ptr(), v.data_ptr(), at, at, total, cu_ptr, n_seqs, _cache_lib.raw_stream(device)))

@@ -184,6 +184,17 @@ def test_what_the_cached_forward_refuses(models):
         plain(prompts[1][:, :10] % TINY.vocab_size, cache=small.step([small.open()], [10]))
 
 
+@torch.no_grad()
+def test_an_empty_request_reads_as_no_rows():
+    from fastdecisions_amd.decider_cache import DeciderCache
+    from fastdecisions_amd.model import TINY
+    announce("decider cache, an empty request")
+    cache = DeciderCache(TINY, requests=2, tokens=64)
+    layer = next(iter(cache._attention))
+    k, v = cache.read(cache.open(), layer)
+    assert k.shape == v.shape == (1, TINY.num_key_value_heads, 0, TINY.head_dim)
+
+
 def test_ops_trace():
     """opcheck of the cache operators' ops: schema (what they mutate), fakes, AOT dispatch."""
     import fastdecisions_amd.cached_ops as ops

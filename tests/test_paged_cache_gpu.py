@@ -509,3 +509,39 @@ def test_written_then_attended_then_read():
     for got, x in ((dk, k), (dv, v)):
         codes, scale = e4m3(x[0].double())
         assert torch.equal(got[0].double(), codes * pow2(scale)[..., None])
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+def test_a_run_on_another_stream(fp8):
+    """Write, attend and read on a stream of the caller's, with work of the default stream going on: the bits of
+    the same run on the default stream."""
+    from fastdecisions_amd.paged_kv_kernel import paged_kv_read, paged_kv_write
+    announce(f"paged cache, a run on another stream, fp8 {fp8}")
+    new, lens = [70, 1, 300], [900, 2000, 300]
+
+    def run():
+        c = make_pages(lens, 32, 4, 128, fp8, seed=28)
+        k, v = (new_rows(new, 4, 128, 29 + i, True) for i in range(2))
+        q = make_q(new, 16, 128, 31)
+        paged_kv_write(k, v, c["k"], c["v"], c["table"], ints(lens), cu_seqlens=ints(starts(new)), **scales(c))
+        out = run_attention(c, q, lens, new)
+        return [out, *paged_kv_read(c["k"], c["v"], c["table"], ints(starts(lens)), sum(lens), **scales(c))]
+    want = run()
+    side, busy = torch.cuda.Stream(), torch.zeros(1 << 26, device="cuda")
+    side.wait_stream(torch.cuda.current_stream())
+    for _ in range(20):
+        busy.add_(1.0)
+    with torch.cuda.stream(side):
+        got = run()
+    torch.cuda.current_stream().wait_stream(side)
+    for a, b in zip(got, want):
+        assert torch.equal(a.view(torch.int16), b.view(torch.int16))
+
+
+def test_reading_nothing():
+    """A request without keys: empty tensors, the pool untouched."""
+    from fastdecisions_amd.paged_kv_kernel import paged_kv_read
+    announce("paged read, no rows")
+    c = make_pages([40], 16, 2, 64, False, seed=32)
+    k, v = paged_kv_read(c["k"], c["v"], c["table"], ints([0, 0]), 0)
+    assert k.shape == v.shape == (1, 2, 0, 64) and k.dtype == torch.bfloat16
