@@ -128,6 +128,8 @@ def paged_kv_write(
     if len(shape) != 4 or k_cache.ndim != 4 or value.shape != shape:
         raise ValueError("key and value must be [B, Hkv, T, D] of one shape")
     batch, heads, seq_len, dim = shape
+    if batch < 1 or seq_len < 1:
+        raise ValueError("Batch and sequence length must be positive")
     if heads != k_cache.shape[1] or dim != k_cache.shape[3]:
         raise ValueError("key and value must have the cache's heads and head dimension")
     if cache_lens is None:

@@ -136,6 +136,14 @@ def test_tensors_that_do_not_fit_are_refused():
         paged_gqa_attention(x.expand(2, -1, -1, -1), k, k, table, lens, cu_seqlens=torch.zeros(3, dtype=torch.int32))
 
 
+def test_a_write_of_no_tokens_is_refused():
+    from fastdecisions_amd.paged_kv_kernel import paged_kv_write
+    k = torch.zeros((4, 2, 16, 64), dtype=torch.bfloat16)
+    x = torch.zeros((1, 2, 0, 64), dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="must be positive"):
+        paged_kv_write(x, x, k, k, torch.zeros((1, 2), dtype=torch.int32), torch.ones(1, dtype=torch.int32))
+
+
 def test_calls_larger_than_a_grid_are_refused():
     """A grid dimension's threads fit 32 bits."""
     lib, c, uns = _cache_lib.lib(), cache(), _lib.FD_ERR_UNSUPPORTED
