@@ -236,3 +236,18 @@ def cached_layers_ready(core) -> bool:
                 and linear.conv1d.bias is None and linear.activation == "silu" and 2 <= linear.conv_kernel_size <= 4):
             return False
     return True
+
+
+def check_cached_call(layer, hidden_states, **others) -> None:
+    """Refuse what a layer's forward over a ``CacheStep`` does not compute: gradients, dropout, other devices and
+    types, and masks or caches (``others``) beside the step."""
+    if torch.is_grad_enabled():
+        raise RuntimeError("The cached forward is for inference: call it without gradients (torch.no_grad() or "
+                           "torch.inference_mode())")
+    if layer.training and getattr(layer, "attention_dropout", 0.0):
+        raise RuntimeError("The cached forward has no dropout: call it in eval mode")
+    if not hidden_states.is_cuda or hidden_states.dtype != torch.bfloat16:
+        raise ValueError("The cached forward takes BF16 hidden states on the GPU")
+    for name, value in others.items():
+        if value is not None:
+            raise ValueError(f"{name} has no meaning beside fd_cache: a step's tokens see everything their requests hold")

@@ -175,8 +175,10 @@ def candidate_forward(self, hidden_states, position_embeddings, attention_mask=N
     mask is applied in-kernel, so the kernel runs only when ``attention_mask`` adds
     nothing to it (``plain_causal``); any other mask (padding, segments, a bias)
     runs the original forward, which applies it.  With ``fd_cache`` (a ``CacheStep``) the tokens continue
-    requests of a ``DeciderCache``."""
+    requests of a ``DeciderCache``; nothing else runs such a call, so what the kernels do not do is refused."""
     if kwargs.get("fd_cache") is not None:
+        from .decider_cache import check_cached_call
+        check_cached_call(self, hidden_states, past_key_values=past_key_values, attention_mask=attention_mask)
         return _cached_forward(self, hidden_states, position_embeddings, kwargs["fd_cache"])
     if (past_key_values is not None or self.training or torch.is_grad_enabled()
             or not hidden_states.is_cuda or hidden_states.dtype != torch.bfloat16

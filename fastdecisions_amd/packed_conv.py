@@ -166,6 +166,8 @@ def _cached_forward(self, hidden_states, step):
 
 def _forward(self, hidden_states, cache_params=None, attention_mask=None, **kwargs):
     if kwargs.get("fd_cache") is not None:  # tokens that continue requests of a DeciderCache
+        from .decider_cache import check_cached_call
+        check_cached_call(self, hidden_states, cache_params=cache_params, attention_mask=attention_mask)
         return _cached_forward(self, hidden_states, kwargs["fd_cache"])
     # The original method owns caches, training and other geometries (ref: src/decider/packed_conv.py:25-38).
     if (cache_params is not None or self.training or torch.is_grad_enabled()
