@@ -3,14 +3,15 @@
 They wrap ``paged_kv_write``, ``paged_kv_read`` (``paged_kv_kernel``), ``paged_gqa_attention``
 (``paged_gqa_kernel``), ``prep_qkv_state`` (``packed_conv_kernel``) and
 ``recurrent_gated_delta_rule`` (``gated_delta_kernel``) in the forms the cached layers call;
-caches and states are updated in place and declared so."""
+caches and states are updated in place and declared so.  ``gated_delta_rule_states`` is the chunked
+rule (``chunk_gated_delta_rule``) from and to states that the caller gathers and scatters."""
 from __future__ import annotations
 
 from typing import Optional
 
 import torch
 
-from .gated_delta_kernel import recurrent_gated_delta_rule
+from .gated_delta_kernel import chunk_gated_delta_rule, recurrent_gated_delta_rule
 from .packed_conv_kernel import prep_qkv_state
 from .paged_gqa_kernel import paged_gqa_attention
 from .paged_kv_kernel import paged_kv_read, paged_kv_write
@@ -83,3 +84,17 @@ def gated_delta_step_op(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: to
 @gated_delta_step_op.register_fake
 def _gated_delta_step_fake(q, k, v, g, beta, state, cu_seqlens, state_indices):
     return v.new_empty(v.shape)
+
+
+@torch.library.custom_op("fastdecisions_cache::gated_delta_rule_states", mutates_args=(), device_types="cuda")
+def gated_delta_rule_states_op(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tensor, beta: torch.Tensor,
+                               initial_state: torch.Tensor,
+                               cu_seqlens: Optional[torch.Tensor]) -> tuple[torch.Tensor, torch.Tensor]:
+    """The chunked rule with q and k normalised: (out, final states)."""
+    return chunk_gated_delta_rule(q, k, v, g, beta, initial_state=initial_state, output_final_state=True,
+                                  use_qk_l2norm_in_kernel=True, cu_seqlens=cu_seqlens)
+
+
+@gated_delta_rule_states_op.register_fake
+def _gated_delta_rule_states_fake(q, k, v, g, beta, initial_state, cu_seqlens):
+    return v.new_empty(v.shape), initial_state.new_empty(initial_state.shape, dtype=torch.float32)
