@@ -44,6 +44,7 @@ class CacheStep:
     page_table: torch.Tensor      # int32 [n, max_pages]
     positions: torch.Tensor       # int32 [1, total]
     buffer: torch.Tensor = field(repr=False)
+    held: list[list[int]] = field(repr=False)  # the requests' pages; another request of a number has another list
 
     @property
     def max_new(self) -> int:
@@ -60,8 +61,15 @@ class CacheStep:
 
     def again(self) -> "CacheStep":
         """The next step of the same requests with as many new tokens each, in the same device tensors."""
+        self._check()
         self.buffer.copy_(self.cache._reserve(self.slots, self.new))
         return self
+
+    def _check(self) -> None:
+        """Refuse a step whose requests are not those it was made for: its pages may be another request's by now."""
+        for slot, pages in zip(self.slots, self.held):
+            if self.cache._pages.get(slot) is not pages:
+                raise ValueError(f"Request {slot} of the step was closed")
 
 
 class DeciderCache:
@@ -162,7 +170,8 @@ class DeciderCache:
         buffer = self._reserve(slots, new).to(self.device)
         n, total = len(slots), sum(new)
         cu, lens, idx, table, pos = buffer.split([n + 1, n, n, n * self.max_pages, total])
-        return CacheStep(self, slots, new, cu, lens, idx, table.view(n, self.max_pages), pos.view(1, total), buffer)
+        return CacheStep(self, slots, new, cu, lens, idx, table.view(n, self.max_pages), pos.view(1, total), buffer,
+                         [self._pages[slot] for slot in slots])
 
     def _check(self, slots) -> None:
         for slot in slots:

@@ -106,6 +106,8 @@ class DeciderModel(nn.Module):
             from .persistent_residual_rms import chain_ready
             if cu_seqlens is not None or ids.shape != cache.positions.shape:
                 raise ValueError(f"A step's ids are [1, {cache.positions.shape[1]}], without cu_seqlens")
+            if not torch.compiler.is_compiling():  # (a trace would be tied to the requests' numbers)
+                cache._check()
             if not (chain_ready(core, h) and cached_layers_ready(core)):
                 raise RuntimeError("The cached forward needs every HIP kernel (install_hip_kernels(model)), bf16 "
                                    "weights on the GPU and no gradients")
