@@ -19,7 +19,11 @@ Use (``model`` with every HIP kernel installed, inference mode)::
     step = cache.step(forks, lengths)                                   # one packed row [1, sum(lengths)]
     logits = model(packed_ids, cache=step)
 
-A step reserves its pages and counts its tokens when it is made; run each step once, in order.
+A step reserves its pages and counts its tokens when it is made; run each step once, in order, or
+take it back with ``CacheStep.cancel``: the rows of a step that is never run are whatever its pages
+held before.  A forward that refuses its step leaves it waiting, and its requests take no other step
+and no fork before it is run or cancelled; one that fails on the way leaves requests whose layers
+hold different tokens, which can only be closed.
 ``CacheStep.again`` makes the next step of the same shape in the same device tensors, so a
 captured forward over a step can be replayed token after token.
 """
@@ -45,6 +49,12 @@ class CacheStep:
     positions: torch.Tensor       # int32 [1, total]
     buffer: torch.Tensor = field(repr=False)
     held: list[list[int]] = field(repr=False)  # the requests' pages; another request of a number has another list
+    ends: list[int]               # tokens of each request, the new ones included
+    live: bool = True             # neither taken back nor failed
+    begun: bool = False           # a forward over it has reached the layers
+    ran: bool = False             # a forward over it has run
+    captured: bool = False        # a forward over it is in a graph: its runs are replays, which are not seen here
+    waiting: bool = False         # a forward over it was refused
 
     @property
     def max_new(self) -> int:
@@ -63,13 +73,67 @@ class CacheStep:
         """The next step of the same requests with as many new tokens each, in the same device tensors."""
         self._check()
         self.buffer.copy_(self.cache._reserve(self.slots, self.new))
+        self.ends = [self.cache._lens[slot] for slot in self.slots]
+        self.live, self.ran = True, False
         return self
+
+    def cancel(self) -> None:
+        """Take back a step that has not run and is the last one of its requests, which then are as before it."""
+        if not self.live:
+            raise RuntimeError("The step was cancelled already, or has failed")
+        if self.ran:
+            raise RuntimeError("The step has run: the states of its requests hold its tokens")
+        mine = [i for i, slot in enumerate(self.slots) if self.cache._pages.get(slot) is self.held[i]]  # not closed since
+        if any(self.cache._lens[self.slots[i]] != self.ends[i] for i in mine):
+            raise RuntimeError("Only the last step of its requests can be cancelled")
+        self.cache._release([self.slots[i] for i in mine], [self.new[i] for i in mine])
+        self.live = False
+        self._settle()
 
     def _check(self) -> None:
         """Refuse a step whose requests are not those it was made for: its pages may be another request's by now."""
         for slot, pages in zip(self.slots, self.held):
             if self.cache._pages.get(slot) is not pages:
                 raise ValueError(f"Request {slot} of the step was closed")
+
+    # ---- what a forward over the step tells it
+
+    def _start(self) -> None:
+        self._check()
+        if not self.live:
+            raise RuntimeError("The step was cancelled or has failed; make another one")
+        self.cache._check(self.slots, self)
+
+    def _done(self) -> None:
+        if not torch.compiler.is_compiling() and self._capturing():
+            self.captured = True
+        else:
+            self.ran = True
+        if self.waiting:
+            self._settle()
+
+    def _failed(self) -> None:
+        """After an error of a forward.  Before the layers nothing was computed; while a graph is captured nothing runs."""
+        if not self.live or any(self.cache._pages.get(slot) is not pages for slot, pages in zip(self.slots, self.held)):
+            return
+        if self.begun:
+            if not self._capturing():
+                self.cache._lost.update(self.slots)
+                self.live = False
+        elif not (self.ran or self.captured):
+            self.waiting = True
+            for slot in self.slots:
+                self.cache._waiting.setdefault(slot, self)
+
+    def _capturing(self) -> bool:
+        return self.positions.is_cuda and torch.cuda.is_current_stream_capturing()
+
+    def _settle(self) -> None:
+        """No longer waiting."""
+        self.waiting = False
+        for slot in self.slots:
+            if self.cache._waiting.get(slot) is self:
+                del self.cache._waiting[slot]
 
 
 class DeciderCache:
@@ -109,6 +173,8 @@ class DeciderCache:
         self._users = [0] * self.n_pages              # requests that hold a page
         self._pages: dict[int, list[int]] = {}        # of an open request
         self._lens: dict[int, int] = {}
+        self._waiting: dict[int, CacheStep] = {}      # the refused step of an open request
+        self._lost: set[int] = set()                  # open requests that a failed forward left half computed
 
     # ---- requests
 
@@ -148,16 +214,15 @@ class DeciderCache:
 
     def close(self, slot: int) -> None:
         """End a request; pages nobody else holds become free."""
-        self._check([slot])
-        for page in self._pages.pop(slot):
-            self._users[page] -= 1
-            if self._users[page] == 0:
-                self._free_pages.append(page)
+        self._check_open([slot])
+        self._give(self._pages.pop(slot))
         del self._lens[slot]
+        self._lost.discard(slot)
+        self._waiting.pop(slot, None)
         self._free_slots.append(slot)
 
     def length(self, slot: int) -> int:
-        self._check([slot])
+        self._check_open([slot])
         return self._lens[slot]
 
     # ---- steps
@@ -171,17 +236,40 @@ class DeciderCache:
         n, total = len(slots), sum(new)
         cu, lens, idx, table, pos = buffer.split([n + 1, n, n, n * self.max_pages, total])
         return CacheStep(self, slots, new, cu, lens, idx, table.view(n, self.max_pages), pos.view(1, total), buffer,
-                         [self._pages[slot] for slot in slots])
+                         [self._pages[slot] for slot in slots], [self._lens[slot] for slot in slots])
 
-    def _check(self, slots) -> None:
+    def _check_open(self, slots) -> None:
         for slot in slots:
             if slot not in self._lens:
                 raise ValueError(f"{slot} is no open request of the cache")
+
+    def _check(self, slots, step=None) -> None:
+        """Refuse requests that are not open, or hold tokens that no forward (but one over ``step``) has computed."""
+        self._check_open(slots)
+        for slot in slots:
+            if slot in self._lost:
+                raise RuntimeError(f"A forward over request {slot} failed on the way; it can only be closed")
+            if self._waiting.get(slot, step) is not step:
+                raise RuntimeError(f"A step of request {slot} was refused and has not run: run it or cancel it")
 
     def _take(self) -> int:
         page = self._free_pages.pop()
         self._users[page] = 1
         return page
+
+    def _give(self, pages) -> None:
+        for page in pages:
+            self._users[page] -= 1
+            if self._users[page] == 0:
+                self._free_pages.append(page)
+
+    def _release(self, slots, new) -> None:
+        """Undo ``_reserve`` of the requests' last tokens."""
+        for slot, n in zip(slots, new):
+            self._lens[slot] -= n
+            pages = -(-self._lens[slot] // self.page_size)
+            self._give(self._pages[slot][pages:])
+            del self._pages[slot][pages:]
 
     def _reserve(self, slots, new) -> torch.Tensor:
         """Pages for the new tokens; the step's device tensors as one host tensor."""

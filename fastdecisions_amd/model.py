@@ -97,6 +97,18 @@ class DeciderModel(nn.Module):
         (device int32), ``segments`` (host (start, end) pairs) and ``max_seqlen``.
         With ``cache`` (a ``CacheStep`` of a ``DeciderCache``) ids [1, total] are the step's new
         tokens, which continue its requests; it needs every HIP kernel installed."""
+        if cache is None:
+            return self._hidden(ids, cu_seqlens, segments, max_seqlen, final_norm)
+        cache.begun = False
+        try:
+            h = self._hidden(ids, cu_seqlens, segments, max_seqlen, final_norm, cache)
+        except BaseException:
+            cache._failed()
+            raise
+        cache._done()
+        return h
+
+    def _hidden(self, ids, cu_seqlens, segments, max_seqlen, final_norm, cache=None):
         core = self.core
         h = core.embed_tokens(ids)
         B, T = ids.shape
@@ -107,7 +119,7 @@ class DeciderModel(nn.Module):
             if cu_seqlens is not None or ids.shape != cache.positions.shape:
                 raise ValueError(f"A step's ids are [1, {cache.positions.shape[1]}], without cu_seqlens")
             if not torch.compiler.is_compiling():  # (a trace would be tied to the requests' numbers)
-                cache._check()
+                cache._start()
             if not (chain_ready(core, h) and cached_layers_ready(core)):
                 raise RuntimeError("The cached forward needs every HIP kernel (install_hip_kernels(model)), bf16 "
                                    "weights on the GPU and no gradients")
@@ -123,6 +135,8 @@ class DeciderModel(nn.Module):
                           max_length_k=int(max_seqlen), fd_segments=tuple(segments))
         pe = core.rotary_emb(h, pos)
         layers = core.layers[: self.config.num_hidden_layers]
+        if cache is not None:
+            cache.begun = True
         from .persistent_residual_rms import chain_ready, fused_add_rms_norm_op
         if len(layers) and chain_ready(core, h):
             # every layer patched: each MLP residual add runs inside the next RMSNorm kernel

@@ -42,3 +42,43 @@ def test_the_op_of_the_rule_between_states():
                           (r(1, 70, 16, 128), r(1, 70, 16, 128), r(1, 70, 16, 128), g, beta,
                            torch.randn((3, 16, 128, 128), device="cuda"), cu),
                           test_utils=("test_schema", "test_faketensor", "test_aot_dispatch_dynamic"))
+
+
+@torch.no_grad()
+def test_refused_and_failed_forwards(monkeypatch):
+    """A refused step runs afterwards as if nothing had been; after one that failed on the way its request can
+    only be closed, and the others go on."""
+    from fastdecisions_amd.decider_cache import DeciderCache
+    from fastdecisions_amd.model import TINY, build_decider, install_hip_kernels, synthetic_ids
+    announce("refused and failed cached forwards")
+    model = build_decider(TINY, seed=3)
+    install_hip_kernels(model)
+    ids = synthetic_ids(1, 60, TINY.vocab_size, seed=1)
+    caches = [DeciderCache(TINY, requests=2, tokens=200) for _ in range(2)]
+    slots = [[c.open(), c.open()] for c in caches]
+    for c, s in zip(caches, slots):
+        model(ids[:, :40], cache=c.step(s, [30, 10]))
+    clean, c = caches
+    want = model(ids[:, 40:50], cache=clean.step(slots[0][:1], [10]))
+    step = c.step(slots[1][:1], [10])
+    with pytest.raises(ValueError, match="ids"):
+        model(ids[:, 40:51], cache=step)
+    assert torch.equal(model(ids[:, 40:50], cache=step), want) and not c._waiting
+    with torch.enable_grad(), pytest.raises(RuntimeError, match="no gradients"):
+        model(ids[:, 50:51], cache=c.step(slots[1][:1], [1]))
+    c._waiting[slots[1][0]].cancel()
+
+    def broken(*args, **kwargs):
+        raise RuntimeError("out of memory, say")
+    with monkeypatch.context() as m:
+        m.setattr(model.core.layers[2].mlp, "forward", broken)
+        with pytest.raises(RuntimeError, match="say"):
+            model(ids[:, 50:55], cache=c.step(slots[1][:1], [5]))
+    with pytest.raises(RuntimeError, match="only be closed"):
+        c.step(slots[1][:1], [1])
+    c.close(slots[1][0])
+    want = model(ids[:, 50:53], cache=clean.step(slots[0][1:], [3]))
+    assert torch.equal(model(ids[:, 50:53], cache=c.step(slots[1][1:], [3])), want)
+    fresh = model(ids[:, :7], cache=c.step([c.open()], [7]))
+    clean.close(slots[0][0])
+    assert torch.equal(fresh, model(ids[:, :7], cache=clean.step([clean.open()], [7])))

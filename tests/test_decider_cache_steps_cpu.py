@@ -37,3 +37,92 @@ def test_a_step_of_a_closed_request(model):
             use()
     assert c.length(other) == 5 and c.length(b) == 3
     assert taken.again() is taken and c.length(other) == 10
+
+
+def state_of(c):
+    return (dict(c._lens), {s: list(p) for s, p in c._pages.items()}, sorted(c._free_pages), list(c._users))
+
+
+@torch.no_grad()
+def test_a_refused_forward_leaves_its_step_waiting(model):
+    """Its tokens were counted and never computed: whatever continues the request would attend over what its new
+    pages held before."""
+    c = make()
+    a, b = c.open(), c.open()
+    c.step([a], [20])
+    before = state_of(c)
+    step = c.step([a, b], [30, 5])
+    with pytest.raises(ValueError, match="ids"):
+        model(ids(34), cache=step)
+    for use in (lambda: c.step([a], [1]), lambda: c.step([b], [1]), lambda: c.fork(a), step.again, lambda: c.read(b, 3)):
+        with pytest.raises(RuntimeError, match="run it or cancel it"):
+            use()
+    with pytest.raises(RuntimeError, match="install_hip_kernels"):  # it may be tried again
+        model(ids(35), cache=step)
+    step.cancel()
+    assert state_of(c) == before and not c._waiting
+    with pytest.raises(RuntimeError, match="make another"):
+        model(ids(35), cache=step)
+    assert c.length(a) == 20 and c.length(b) == 0
+    c.step([a], [1])
+    c.fork(b)
+    assert step.again() is step and c.length(a) == 51 and step.positions[0, :30].tolist() == list(range(21, 51))
+
+
+@torch.no_grad()
+def test_an_earlier_refused_step_holds_back_the_later_one(model):
+    c = make()
+    a = c.open()
+    first, second = c.step([a], [3]), c.step([a], [2])
+    with pytest.raises(ValueError):
+        model(ids(9), cache=first)
+    with pytest.raises(RuntimeError, match="run it or cancel it"):
+        model(ids(2), cache=second)
+    with pytest.raises(RuntimeError, match="Only the last"):
+        first.cancel()
+    second.cancel()
+    first.cancel()
+    assert c.length(a) == 0 and len(c._free_pages) == c.n_pages
+
+
+@torch.no_grad()
+def test_a_forward_that_fails_on_the_way(model):
+    """Some layers hold the step's tokens, others do not: nothing may continue the request."""
+    c = make()
+    a, b = c.open(), c.open()
+    step, other = c.step([a], [3]), c.step([b], [4])
+    step.begun = True
+    step._failed()                                         # an error behind the first layer
+    for use in (lambda: c.step([a], [1]), lambda: c.fork(a), step.again, lambda: c.read(a, 3)):
+        with pytest.raises(RuntimeError, match="only be closed"):
+            use()
+    with pytest.raises(RuntimeError, match="failed"):
+        step.cancel()
+    c.close(a)
+    a = c.open()
+    c.step([a], [1])
+    other.cancel()
+    assert c.length(b) == 0
+
+
+@torch.no_grad()
+def test_what_has_run_stays(model):
+    """A refused repetition of a step takes nothing back."""
+    c = make()
+    a = c.open()
+    step = c.step([a], [3])
+    step._done()                                           # as after a forward
+    with pytest.raises(ValueError):
+        model(ids(4), cache=step)
+    with pytest.raises(RuntimeError, match="has run"):
+        step.cancel()
+    assert c.length(a) == 3
+    step.again()
+    step.cancel()
+    assert c.length(a) == 3
+    both = c.step([a, c.open()], [2, 2])
+    with pytest.raises(ValueError):
+        model(ids(1), cache=both)
+    c.close(a)                                             # the other request is still held by the step
+    both.cancel()
+    assert len(c._free_pages) == c.n_pages and not c._waiting
