@@ -72,7 +72,12 @@ class CacheStep:
     def again(self) -> "CacheStep":
         """The next step of the same requests with as many new tokens each, in the same device tensors."""
         self._check()
-        self.buffer.copy_(self.cache._reserve(self.slots, self.new))
+        sizes = self.cache._reserve(self.slots, self.new)
+        try:
+            self.buffer.copy_(sizes)
+        except BaseException:
+            self.cache._release(self.slots, self.new)
+            raise
         self.ends = [self.cache._lens[slot] for slot in self.slots]
         self.live, self.ran = True, False
         return self
@@ -232,7 +237,12 @@ class DeciderCache:
         slots, new = list(slots), [int(n) for n in new]
         if len(slots) != len(new) or not slots or min(new) < 1:
             raise ValueError("A step takes one or more requests and a positive number of new tokens of each")
-        buffer = self._reserve(slots, new).to(self.device)
+        sizes = self._reserve(slots, new)
+        try:
+            buffer = sizes.to(self.device)
+        except BaseException:  # out of memory
+            self._release(slots, new)
+            raise
         n, total = len(slots), sum(new)
         cu, lens, idx, table, pos = buffer.split([n + 1, n, n, n * self.max_pages, total])
         return CacheStep(self, slots, new, cu, lens, idx, table.view(n, self.max_pages), pos.view(1, total), buffer,
@@ -268,7 +278,7 @@ class DeciderCache:
         for slot, n in zip(slots, new):
             self._lens[slot] -= n
             pages = -(-self._lens[slot] // self.page_size)
-            self._give(self._pages[slot][pages:])
+            self._give(self._pages[slot][pages:][::-1])
             del self._pages[slot][pages:]
 
     def _reserve(self, slots, new) -> torch.Tensor:

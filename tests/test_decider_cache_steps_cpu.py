@@ -126,3 +126,21 @@ def test_what_has_run_stays(model):
     c.close(a)                                             # the other request is still held by the step
     both.cancel()
     assert len(c._free_pages) == c.n_pages and not c._waiting
+
+
+@pytest.mark.parametrize("where", ["to", "copy_"])
+def test_a_step_that_finds_no_memory(where, monkeypatch):
+    """The tokens of a step that was never handed out would be counted for good."""
+    c = make()
+    a = c.open()
+    step = c.step([a], [20])
+    before = state_of(c)
+
+    def full(*args, **kwargs):
+        raise RuntimeError("out of memory")
+    with monkeypatch.context() as m:
+        m.setattr(torch.Tensor, where, full)
+        with pytest.raises(RuntimeError, match="out of memory"):
+            c.step([a], [40]) if where == "to" else step.again()
+    assert state_of(c) == before
+    assert step.again().positions.tolist() == [list(range(20, 40))]
