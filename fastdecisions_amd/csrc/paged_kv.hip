@@ -24,6 +24,9 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr float kE4m3Max = 448.0f;
+// The scale byte of rows whose largest value lies above 1.75 2^127.  From 248 2^120 on their values round to the code of
+// 256, which is 2^128 and no bf16 number: it is read as 255 2^120, the largest one, no further from the value.
+constexpr int kTopByte = 247;
 // A thread takes several rows, their chains of loads side by side, once there is more than a round (write) or a few
 // rounds (read) of workgroups: 1024 of a side (K, V) run at once.  Measured with 1, 2, 4 rows (us, 4 heads x 128 bf16):
 // write 1.2, 5 and 48 thousand tokens 4.0, 4.1, 4.1; 9.6, 9.3, 10.0; 39, 40, 41, E4M3 40, 38, 41; read 12 and 96
@@ -225,10 +228,15 @@ __global__ __launch_bounds__(kThreads) void paged_kv_read_kernel(ReadArgs a) {
     if constexpr (FP8) {  // codes of no page are zeros, whatever their scale
       const float s = scale_of(byte[u]);
       typedef float f32x2_t __attribute__((ext_vector_type(2)));
-      const f32x2_t f0 = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(w[u].x), false);
-      const f32x2_t f1 = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(w[u].x), true);
-      const f32x2_t f2 = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(w[u].y), false);
-      const f32x2_t f3 = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(w[u].y), true);
+      f32x2_t f0 = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(w[u].x), false);
+      f32x2_t f1 = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(w[u].x), true);
+      f32x2_t f2 = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(w[u].y), false);
+      f32x2_t f3 = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(w[u].y), true);
+      if (byte[u] == kTopByte) {
+        for (f32x2_t* const f : {&f0, &f1, &f2, &f3})
+#pragma unroll
+          for (int e = 0; e < 2; ++e) (*f)[e] = fabsf((*f)[e]) == 256.0f ? copysignf(255.0f, (*f)[e]) : (*f)[e];
+      }
       w[u].x = fd_pack2(f0[0] * s, f0[1] * s);
       w[u].y = fd_pack2(f1[0] * s, f1[1] * s);
       w[u].z = fd_pack2(f2[0] * s, f2[1] * s);

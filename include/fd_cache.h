@@ -95,7 +95,8 @@ FD_API int fd_paged_kv_write(const void* k, const void* v, const int64_t k_strid
  * The first cu_seqlens[r + 1] - cu_seqlens[r] keys and values of every request r as dense bf16 rows
  * [cu_seqlens[r], cu_seqlens[r + 1]) of k_out and v_out [kv_heads, total, head_dim] (strides {h, t};
  * d contiguous).  Keys past the page table or on no page are zeros; rows behind the last request are
- * left as they were.  cache_lens is not used.
+ * left as they were.  cache_lens is not used.  A cached value of 2^128 (values from 248 * 2^120 on are
+ * held as one in E4M3) is read as bf16's largest, 255 * 2^120.
  */
 FD_API int fd_paged_kv_read(const fd_paged_cache* cache, void* k_out, void* v_out, const int64_t k_strides[2],
                             const int64_t v_strides[2], int64_t total, const int32_t* cu_seqlens, int n_seqs,
