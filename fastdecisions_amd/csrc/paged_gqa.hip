@@ -92,7 +92,7 @@ struct PagedArgs {
   int n_req, seq_len, group, kv_heads;
   uint32_t group_magic;         // ceil(2^24 / group)
   int slots_log2, min_tiles, overhead;  // workgroups that run at once; tiles of a range at least, and that one costs besides
-  int max_items;                // items the grid and the workspace hold
+  int part_items;               // items whose parts the workspace holds
   float scale_log2;
   int32_t* range_tiles;         // the key tiles of a range, for the joining kernel; null where nothing can be split
   float* part;                  // per item: rows x D of o, then rows x 2 of (max, denominator)
@@ -355,9 +355,9 @@ __device__ __forceinline__ bool open_job(const PagedArgs& a, int lane, Job* j) {
   if (it.range > 0 && j->t0 >= nt_all) return false;
   j->nt = min(it.tiles, nt_all - j->t0);  // 0 where no key is visible at all
   j->split = nt_all > it.tiles;
-  // where a part goes; the workspace has a place for every item of a well-formed offset table
+  // where a part goes; the workspace has a place for every part of a well-formed offset table
   j->slot = it.base + (it.head * it.n_ranges + it.range) * it.n_rtiles + it.rtile;
-  return j->slot >= 0 && j->slot < a.max_items;
+  return !j->split || (j->slot >= 0 && j->slot < a.part_items);
 }
 
 // Is any key of the job's tiles on no page?
@@ -1411,7 +1411,7 @@ __global__ __launch_bounds__(256) void paged_gqa_join_kernel(PagedArgs a) {
   const int ranges = (nt_all + it.tiles - 1) / it.tiles;
   if (ranges <= 1) return;  // its one item has stored the rows
   const int slot = it.base + it.head * it.n_ranges * it.n_rtiles + it.rtile;
-  if (slot < 0 || slot + (ranges - 1) * static_cast<int64_t>(it.n_rtiles) >= a.max_items) return;
+  if (slot < 0 || slot + (ranges - 1) * static_cast<int64_t>(it.n_rtiles) >= a.part_items) return;
   const int row_end = min(min(S::kRows, it.rows - it.row0), static_cast<int>(blockIdx.y + 1) * ROWS);
   const int64_t step = it.n_rtiles * part_floats<S::kRows>(D);  // from one range's part to the next one's
   const float* const part = a.part + slot * part_floats<S::kRows>(D);
@@ -1485,7 +1485,7 @@ constexpr int kHeaderBytes = 256;  // of the workspace: range_tiles
 struct Plan {
   int few;  // blocks of 16 rows of the few-rows kernel, 0: pieces
   int rows, keys, slots, min_tiles;
-  int64_t items, rtiles, bytes;
+  int64_t items, part_items, rtiles, bytes;
   bool may_split;
 };
 
@@ -1517,7 +1517,10 @@ Plan plan_of(int64_t requests, int64_t tokens, int group, int kv_heads, int head
   // best_range gives at most kMaxRounds * slots items, or splits nothing; a share alone may add a range per row tile
   p.items = requests <= 64 ? std::max<int64_t>(kMaxRounds * p.slots, p.rtiles) : kMaxRounds * p.slots + p.rtiles;
   p.may_split = max_keys > static_cast<int64_t>(p.min_tiles) * p.keys;
-  p.bytes = p.may_split ? kHeaderBytes + p.items * p.rows * (head_dim + 2) * 4 : 0;
+  // best_range splits only where all items fit its rounds: the row tiles of long pieces need no place for parts
+  // (131072 tokens, 16/4 heads x 128: 34 MB, 1.09 GB with one for every row tile)
+  p.part_items = requests <= 64 ? kMaxRounds * p.slots : p.items;
+  p.bytes = p.may_split ? kHeaderBytes + p.part_items * p.rows * (head_dim + 2) * 4 : 0;
   return p;
 }
 
@@ -1625,7 +1628,7 @@ extern "C" int fd_paged_gqa_fwd(const void* q, const fd_paged_cache* cache, cons
   a.slots_log2 = __builtin_ctz(static_cast<unsigned>(p.slots));
   a.min_tiles = p.min_tiles;
   a.overhead = p.few ? 2 : 4;
-  a.max_items = static_cast<int>(p.items);
+  a.part_items = static_cast<int>(p.part_items);
   a.scale_log2 = scale * 1.4426950408889634f;
   a.range_tiles = p.may_split ? static_cast<int32_t*>(workspace) : nullptr;
   a.part = p.may_split ? static_cast<float*>(workspace) + kHeaderBytes / 4 : nullptr;

@@ -34,3 +34,16 @@ def test_packed_requests_beyond_64(hq, hkv, dim, top, fp8):
     gate = make_q(new, hq, dim, 32)
     out = run_attention(c, q, lens, new, gate=gate)
     check_attention(c, q, out, lens, new, gate=gate)
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("hq,hkv,dim", [(64, 4, 128), (64, 8, 256), (128, 4, 64)])
+@pytest.mark.parametrize("new,cached", [([1100], [200]), ([1, 1100, 30, 0], [5000, 0, 2000, 77])])
+def test_more_row_tiles_than_places_for_parts(new, cached, hq, hkv, dim, fp8):
+    """More row tiles than two rounds of workgroups: nothing is split, and no tile needs a place in the workspace."""
+    announce(f"paged attention, {new} tokens x {hq}/{hkv} x {dim}, fp8 {fp8}")
+    lens = [n + c for n, c in zip(new, cached)]
+    c = make_pages(lens, 64, hkv, dim, fp8, seed=33)
+    q = make_q(new, hq, dim, 34)
+    out = run_attention(c, q, lens, new)
+    check_attention(c, q, out, lens, new)
