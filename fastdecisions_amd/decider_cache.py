@@ -165,6 +165,7 @@ class DeciderCache:
         kv = (len(attention), self.n_pages, shape.num_key_value_heads, page_size, shape.head_dim)
         self.k = torch.zeros(kv, dtype=kv_dtype, device=self.device)
         self.v = torch.zeros_like(self.k)
+        self.device = self.k.device                   # with its index: steps go there whatever device is current
         self.k_scale = self.v_scale = None
         if kv_dtype == torch.float8_e4m3fn:
             self.k_scale = torch.full(kv[:4], 127, dtype=torch.uint8, device=self.device)

@@ -82,3 +82,12 @@ def test_refused_and_failed_forwards(monkeypatch):
     fresh = model(ids[:, :7], cache=c.step([c.open()], [7]))
     clean.close(slots[0][0])
     assert torch.equal(fresh, model(ids[:, :7], cache=clean.step([clean.open()], [7])))
+
+
+def test_a_cache_stays_on_its_device():
+    """Made on the current device, its later steps go there whichever device is current then."""
+    from fastdecisions_amd.decider_cache import DeciderCache
+    from fastdecisions_amd.model import TINY
+    cache = DeciderCache(TINY, requests=1, tokens=64)
+    assert cache.device == cache.k.device and cache.device.index is not None
+    assert cache.step([cache.open()], [3]).buffer.device == cache.k.device
