@@ -26,6 +26,14 @@ and no fork before it is run or cancelled; one that fails on the way leaves requ
 hold different tokens, which can only be closed.
 ``CacheStep.again`` makes the next step of the same shape in the same device tensors, so a
 captured forward over a step can be replayed token after token.
+
+Streams: a cache's calls change its tensors (``open`` clears states, ``fork`` copies pages and states,
+``step`` and ``again`` write the step's tensors) and its host records at once: ``close`` gives pages and
+states to whoever opens next, also while a forward that reads them is still queued.  So make all calls,
+forwards and replays on one stream, or order the streams yourself: the stream of a later call waits
+(``Stream.wait_stream``) for the one of every forward and replay before it, over any request, and
+``again`` for the one that still reads its step.  Requests in disjoint steps may run on two streams
+at once as long as none of the calls above is made between them without that order.  A cache is not for two threads.
 """
 from __future__ import annotations
 

@@ -91,3 +91,32 @@ def test_a_cache_stays_on_its_device():
     cache = DeciderCache(TINY, requests=1, tokens=64)
     assert cache.device == cache.k.device and cache.device.index is not None
     assert cache.step([cache.open()], [3]).buffer.device == cache.k.device
+
+
+@torch.no_grad()
+def test_two_streams_in_order():
+    """A request closed behind a queued forward on one stream, its pages taken by another one on a second stream
+    that waits for the first: both as on one stream."""
+    from fastdecisions_amd.decider_cache import DeciderCache
+    from fastdecisions_amd.model import TINY, build_decider, install_hip_kernels, synthetic_ids
+    announce("one cache, two streams")
+    model = build_decider(TINY, seed=3)
+    install_hip_kernels(model)
+    ids = synthetic_ids(1, 90, TINY.vocab_size, seed=1)
+    runs = []
+    for streams in ([torch.cuda.current_stream()] * 2, [torch.cuda.Stream(), torch.cuda.Stream()]):
+        cache = DeciderCache(TINY, requests=1, tokens=50, page_size=16)
+        out, last = [], torch.cuda.current_stream()
+        for i in range(6):
+            stream = streams[i % 2]
+            stream.wait_stream(last)
+            with torch.cuda.stream(stream):
+                slot = cache.open()
+                for part in ((0, 40), (40, 41)):
+                    n = part[1] - part[0]
+                    out.append(model(ids[:, i + part[0]:i + part[1]], cache=cache.step([slot], [n])))
+                cache.close(slot)
+            last = stream
+        torch.cuda.synchronize()
+        runs.append(out)
+    assert all(torch.equal(a, b) for a, b in zip(*runs))
