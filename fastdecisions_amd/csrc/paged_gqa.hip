@@ -22,6 +22,15 @@
 // permuted so that a lane's scores are those of the 8 consecutive keys whose
 // probabilities it must supply to P V: P never leaves registers, and V^T comes
 // from transposing LDS reads.
+//
+// The matrix product takes P in bf16.  Few rows, bound by the cache's bytes, take
+// it in two parts (two_bf16), so that nothing but the output is rounded: errors
+// against 64 bits as with P in fp32 (0.00164 of the output, the output's own
+// rounding; one part 0.0020), for 0 to 4 % of the time with single tokens, up to 9 %
+// with 17 to 64 rows.  Pieces, bound by the MFMAs' and the softmax's issue, take one
+// part, as the uncached attention does: with two, 2048 tokens on 6144 keys take 139
+// us (64 features, 103 with one), 192 (128, 143) and 191 (256, 148).  Their
+// denominator sums the rounded p.
 #include <algorithm>
 #include <type_traits>
 
@@ -447,6 +456,17 @@ __device__ __forceinline__ float sum8(bf16x8_t p, float x) {
   return x;
 }
 
+// p >= 0 as the sum of two bf16 up to 2^-16 of it.  The first is below p wherever p is not 0, so that the second is
+// not 0 there either: a seen infinity times the two parts is one infinity, never NaN.
+__device__ __forceinline__ void two_bf16(f32x8_t p, bf16x8_t* hi, bf16x8_t* lo) {
+  f32x8_t first;
+#pragma unroll
+  for (int e = 0; e < 8; ++e)
+    first[e] = __uint_as_float(__builtin_elementwise_sub_sat(__float_as_uint(p[e]), 1u) & 0xffff0000u);
+  *hi = __builtin_convertvector(first, bf16x8_t);
+  *lo = __builtin_convertvector(p - first, bf16x8_t);
+}
+
 // Infinities and NaN ("odd" values) among V's operands: are there any, the operand without them, element i
 // (uniform) of one, and o + p x for the odd ones of four values x that a row sees (p is not 0).
 __device__ __forceinline__ bool any_odd(bf16x8_t v) {
@@ -485,14 +505,14 @@ __device__ __forceinline__ void byte_to_lds(const uint8_t* p, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_ubyte %0, off" ::"v"(p), "s"(lds) : "memory", "m0");
 }
 
-// A block of 32 keys costs a wavefront 16 (NR) MFMAs of 16x16x32 and, at the memory's rate, several
+// A block of 32 keys costs a wavefront 24 (NR) MFMAs of 16x16x32 and, at the memory's rate, several
 // times as long to arrive, so what counts is that copies are always in flight: rows go to LDS as they
 // are (codes are converted where they are read, scales multiply scores and probabilities), K and V
 // of kStages blocks each, the next K leaving as soon as a block's scores have read theirs, the next
 // V as soon as P V has.
 // Measured (16 / 4 heads x 128, pages of 64, kernel and join): 64 requests of 8192 keys 195 us, 5.5 TB/s of
-// keys and values (a large copy here: 5.1), E4M3 107 us, 5.0 TB/s; of 256 to 8192 keys 79 and 46 us; one
-// request of 8192 keys 13 us, of 200 keys 8 us, latency: arguments, lengths, page, keys, scores, store.
+// keys and values (a large copy here: 5.1), E4M3 109 us, 5.0 TB/s; of 256 to 8192 keys 80 and 48 us; one
+// request of 8192 keys 14 us, of 200 keys 8 us, latency: arguments, lengths, page, keys, scores, store.
 template <class S>
 __global__ __launch_bounds__(S::kThreads, S::kPerCu) void paged_gqa_few_kernel(PagedArgs a) {
   constexpr int D = S::D, NR = S::NR, RBY = S::kRowBytes, kKk = D / 32, kNdb = D / 16, NS = S::kStages;
@@ -591,7 +611,7 @@ __global__ __launch_bounds__(S::kThreads, S::kPerCu) void paged_gqa_few_kernel(P
 #pragma unroll
     for (int db = 0; db < kNdb; ++db) o[n][db] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
   }
-  bf16x8_t pb[NR];
+  bf16x8_t pb[NR], pl[NR];  // probabilities, in two parts
 
   auto scores = [&](int j) {
     const unsigned char* const st = stage0 + (j & (NS - 1)) * S::kStageBytes;
@@ -670,18 +690,15 @@ __global__ __launch_bounds__(S::kThreads, S::kPerCu) void paged_gqa_few_kernel(P
       f32x8_t pv;
 #pragma unroll
       for (int e = 0; e < 8; ++e) pv[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[e], a.scale_log2, -m_sub));
-      pb[n] = __builtin_convertvector(pv, bf16x8_t);
-      // the denominator takes the rounded p: its error then cancels where a few keys carry the row
-      f32x8_t pr = __builtin_convertvector(pb[n], f32x8_t);
       float psum = 0.0f;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) psum += pr[e];
+      for (int e = 0; e < 8; ++e) psum += pv[e];
       l_run[n] = l_run[n] * alpha + psum;
-      if constexpr (FP8) {  // V's scales go to P: a power of two changes no rounding
+      if constexpr (FP8) {  // V's scales go to P
 #pragma unroll
-        for (int e = 0; e < 8; ++e) pr[e] = masked && pr[e] == 0.0f ? 0.0f : pr[e] * vs[e];
-        pb[n] = __builtin_convertvector(pr, bf16x8_t);
+        for (int e = 0; e < 8; ++e) pv[e] = masked && pv[e] == 0.0f ? 0.0f : pv[e] * vs[e];
       }
+      two_bf16(pv, &pb[n], &pl[n]);
     }
   };
 
@@ -720,7 +737,7 @@ __global__ __launch_bounds__(S::kThreads, S::kPerCu) void paged_gqa_few_kernel(P
         for (int key = 0; key < 32; ++key) {
           float ph[NR];
 #pragma unroll
-          for (int n = 0; n < NR; ++n) ph[n] = __shfl(element(pb[n], key & 7), 16 * (key >> 3) + li);
+          for (int n = 0; n < NR; ++n) ph[n] = __shfl(element(pb[n], key & 7) + element(pl[n], key & 7), 16 * (key >> 3) + li);
 #pragma unroll
           for (int db = 0; db < kNdb; ++db) {
             f32x4_t x;
@@ -740,7 +757,10 @@ __global__ __launch_bounds__(S::kThreads, S::kPerCu) void paged_gqa_few_kernel(P
 #pragma unroll
     for (int db = 0; db < kNdb; ++db)
 #pragma unroll
-      for (int n = 0; n < NR; ++n) o[n][db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf[db], pb[n], o[n][db], 0, 0, 0);
+      for (int n = 0; n < NR; ++n) {
+        o[n][db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf[db], pb[n], o[n][db], 0, 0, 0);
+        o[n][db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf[db], pl[n], o[n][db], 0, 0, 0);
+      }
   };
 
   // ---- the loop: copies in the queue, oldest first, at block j's scores: K(j) V(j) .. K(j + NS - 1) V(j + NS - 1)
@@ -1494,10 +1514,10 @@ Plan plan_of(int64_t requests, int64_t tokens, int group, int kv_heads, int head
   Plan p;
   const int64_t rows = static_cast<int64_t>(max_seqlen) * group;
   // Measured with 16 rows, 32 rows and pieces (us; 16/4 heads x 128 unless noted, 64 requests on 2048 keys):
-  //   rows 32: 46, 52, 51; 8/2 x 256 49, 60, 59; E4M3 35, 38, 55: two tiles of 16 rows
-  //   rows 64: 68, 49, 52; 8/2 x 256 82, 57, 61; E4M3 62, 47, 52: two of 32; 8/2 x 256 with E4M3 46, 53, 61, whose kernel
-  //            for 32 rows fills a CU alone: four of 16
-  //   rows 96: 98, 72, 53; 8/2 x 256 120, 104, 66; E4M3 84, 69, 53: pieces, unless the call is so small that latency
+  //   rows 32: 47, 52, 51; 8/2 x 256 49, 60, 59; E4M3 39, 40, 54: two tiles of 16 rows
+  //   rows 64: 73, 51, 52; 8/2 x 256 84, 60, 61; E4M3 66, 51, 52: two of 32; 8/2 x 256 with E4M3, whose kernel for 32
+  //            rows fills a CU alone: four of 16 (50; pieces 60)
+  //   rows 96: 103, 78, 54; 8/2 x 256 123, 112, 70; E4M3 88, 75, 53: pieces, unless the call is so small that latency
   //            counts, up to 128 rows in all (one request of 4096 keys 19, 19, 24)
   const int64_t all_rows = tokens * group;
   p.few = rows <= 32 ? 1 : rows > 64 && (all_rows > 128 || max_keys > 16384) ? 0 : head_dim == 256 && fp8 ? 1 : 2;

@@ -105,8 +105,11 @@ FD_API int fd_paged_kv_read(const fd_paged_cache* cache, void* k_out, void* v_ou
 /*
  * Causal grouped-query attention of the new tokens of every request over its paged cache, which
  * holds their own keys and values already (fd_paged_kv_write).  New token i of n of request r sees
- * the keys 0 .. cache_lens[r] - n + i; a row that sees no key is zeros.  fp32 softmax; probabilities
- * are rounded to bf16 before the P V product, the denominator sums the rounded ones.
+ * the keys 0 .. cache_lens[r] - n + i; a row that sees no key is zeros.  fp32 softmax.  The P V product
+ * takes each probability as the sum of two bf16 (good to 2^-16 of it) in the kernels for few rows, as one
+ * bf16 in the one for pieces, whose denominator sums the rounded ones.  Pieces: more than 64 rows (tokens
+ * times query heads of a key head) in the longest request, unless a key head has at most 128 rows in all
+ * and the page table is at most 16384 keys wide.
  *
  *   q, out  [batch, q_heads, seq_len, head_dim] bf16, strides {b, h, t, d}; query head h reads key
  *           head h / (q_heads / kv_heads); at most 2048 query heads per key head
