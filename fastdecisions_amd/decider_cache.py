@@ -99,6 +99,9 @@ class CacheStep:
         mine = [i for i, slot in enumerate(self.slots) if self.cache._pages.get(slot) is self.held[i]]  # not closed since
         if any(self.cache._lens[self.slots[i]] != self.ends[i] for i in mine):
             raise RuntimeError("Only the last step of its requests can be cancelled")
+        first = [(self.ends[i] - self.new[i]) // self.cache.page_size for i in mine]  # page of the step's first token
+        if any(self.cache._users[page] > 1 for i, at in zip(mine, first) for page in self.held[i][at:]):
+            raise RuntimeError("A fork of one of its requests holds tokens of the step")
         self.cache._release([self.slots[i] for i in mine], [self.new[i] for i in mine])
         self.live = False
         self._settle()

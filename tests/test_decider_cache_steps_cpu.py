@@ -144,3 +144,21 @@ def test_a_step_that_finds_no_memory(where, monkeypatch):
             c.step([a], [40]) if where == "to" else step.again()
     assert state_of(c) == before
     assert step.again().positions.tolist() == [list(range(20, 40))]
+
+
+def test_a_forked_step_is_not_taken_back():
+    """The request would write its next tokens into a page that the fork reads."""
+    c = make()
+    a = c.open()
+    c.step([a], [20])
+    step = c.step([a], [30])
+    b = c.fork(a)
+    with pytest.raises(RuntimeError, match="fork"):
+        step.cancel()
+    c.close(b)
+    step.cancel()
+    assert c.length(a) == 20 and len(c._pages[a]) == 2
+    b = c.fork(a)                                          # one whole page shared, 20 tokens in both
+    step = c.step([a], [30])
+    step.cancel()
+    assert c.length(a) == c.length(b) == 20 and c._pages[a][0] == c._pages[b][0]
