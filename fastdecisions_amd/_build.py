@@ -27,8 +27,9 @@ SOURCES = ["fd_abi.cpp", "add_rmsnorm.hip", "packed_conv.hip", "gqa_fwd.hip", "g
 
 CACHE_SOURCES = ["cache_abi.cpp", "paged_kv.hip", "paged_gqa.hip", "delta_step.hip", "conv_state.hip"]
 
-# Accumulators of a kernel with more than 256 registers in either half of the register file: without
-# it the compiler puts them all in the accumulation half and copies scores over for every softmax.
+# MFMA accumulators in ordinary registers: without it the compiler puts them all in the accumulation half of the
+# register file and copies scores over for every softmax.  (At 128 features, where eight wavefronts leave 256 registers
+# and Q takes its part of the accumulation half, some operands are copied between the halves all the same.)
 EXTRA_FLAGS = {"paged_gqa.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
 
 COMMON_FLAGS = [

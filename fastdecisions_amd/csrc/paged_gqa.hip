@@ -8,7 +8,8 @@
 //
 //   few rows   16 or 32 rows, 4 wavefronts that each take every fourth block of
 //              32 keys into LDS of their own: no barrier in the loop, the cache
-//              streams through at the rate of the memory.  Up to 64 rows.
+//              streams through at the rate of the memory.  Up to 64 rows, small
+//              calls up to 128 (plan_of).
 //   pieces     128 rows, wavefronts share the staged key tiles.  Suffixes.
 //
 // Key ranges are sized on the device: the lengths are there, and a grid sized by
@@ -511,7 +512,7 @@ __device__ __forceinline__ void byte_to_lds(const uint8_t* p, uint32_t lds) {
 // of kStages blocks each, the next K leaving as soon as a block's scores have read theirs, the next
 // V as soon as P V has.
 // Measured (16 / 4 heads x 128, pages of 64, kernel and join): 64 requests of 8192 keys 195 us, 5.5 TB/s of
-// keys and values (a large copy here: 5.1), E4M3 109 us, 5.0 TB/s; of 256 to 8192 keys 80 and 48 us; one
+// keys and values (a large copy here: 5.1), E4M3 108 us, 5.0 TB/s; of 256 to 8192 keys 80 and 48 us; one
 // request of 8192 keys 14 us, of 200 keys 8 us, latency: arguments, lengths, page, keys, scores, store.
 template <class S>
 __global__ __launch_bounds__(S::kThreads, S::kPerCu) void paged_gqa_few_kernel(PagedArgs a) {

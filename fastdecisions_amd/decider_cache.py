@@ -156,7 +156,8 @@ class DeciderCache:
     def __init__(self, shape: DeciderShape, *, requests: int, tokens: int, max_tokens: int | None = None,
                  page_size: int = 64, kv_dtype: torch.dtype = torch.bfloat16, device="cuda"):
         """``tokens``: cached tokens of all requests together (rounded up to pages, plus one partly filled
-        page per request); ``max_tokens``: of one request (default ``tokens``)."""
+        page per request); ``max_tokens``: of one request (default ``tokens``), the width of the page tables.  A
+        step writes its requests' tables whole: 64 of 3125 pages cost it 5.2 ms of host time, of 128 pages 0.33 ms."""
         if requests < 1 or tokens < 1:
             raise ValueError("requests and tokens must be positive")
         if page_size not in (16, 32, 64, 128, 256):

@@ -122,6 +122,8 @@ FD_API int fd_paged_kv_read(const fd_paged_cache* cache, void* k_out, void* v_ou
  *           over workgroups, whose parts a second launch joins, both on `stream`: calls that may
  *           overlap need workspaces of their own
  * A row's last bits depend on how the call splits its keys, which follows from all requests' lengths.
+ * Scores are fp32 sums, and p v is summed in fp32 before it is divided by the denominator, with a p of up to
+ * 2^8: values from 2^120 / (keys seen) on may overflow where the quotient would not.
  * Masked or absent keys never reach a row, not even as NaN or infinities.
  */
 FD_API int fd_paged_gqa_fwd(const void* q, const fd_paged_cache* cache, const void* gate, void* out,
