@@ -86,13 +86,16 @@ def _gated_delta_step_fake(q, k, v, g, beta, state, cu_seqlens, state_indices):
     return v.new_empty(v.shape)
 
 
-@torch.library.custom_op("fastdecisions_cache::gated_delta_rule_states", mutates_args=(), device_types="cuda")
-def gated_delta_rule_states_op(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tensor, beta: torch.Tensor,
-                               initial_state: torch.Tensor,
-                               cu_seqlens: Optional[torch.Tensor]) -> tuple[torch.Tensor, torch.Tensor]:
+def gated_delta_rule_states(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tensor, beta: torch.Tensor,
+                            initial_state: torch.Tensor,
+                            cu_seqlens: Optional[torch.Tensor]) -> tuple[torch.Tensor, torch.Tensor]:
     """The chunked rule with q and k normalised: (out, final states)."""
     return chunk_gated_delta_rule(q, k, v, g, beta, initial_state=initial_state, output_final_state=True,
                                   use_qk_l2norm_in_kernel=True, cu_seqlens=cu_seqlens)
+
+
+gated_delta_rule_states_op = torch.library.custom_op("fastdecisions_cache::gated_delta_rule_states",
+                                                     gated_delta_rule_states, mutates_args=(), device_types="cuda")
 
 
 @gated_delta_rule_states_op.register_fake
