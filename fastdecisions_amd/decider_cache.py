@@ -44,7 +44,7 @@ import torch
 from .model import DeciderShape
 
 
-@dataclass
+@dataclass(eq=False)
 class CacheStep:
     """New tokens of some requests, packed into one row: what the cached layers need of them."""
     cache: "DeciderCache"
@@ -138,8 +138,13 @@ class CacheStep:
                 self.live = False
         elif not (self.ran or self.captured):
             self.waiting = True
-            for slot in self.slots:
-                self.cache._waiting.setdefault(slot, self)
+            for slot, end in zip(self.slots, self.ends):
+                steps = self.cache._waiting.setdefault(slot, [])
+                if self not in steps:  # in the order of their tokens
+                    steps.insert(sum(step._end(slot) < end for step in steps), self)
+
+    def _end(self, slot) -> int:
+        return self.ends[self.slots.index(slot)]
 
     def _capturing(self) -> bool:
         return self.positions.is_cuda and torch.cuda.is_current_stream_capturing()
@@ -148,8 +153,11 @@ class CacheStep:
         """No longer waiting."""
         self.waiting = False
         for slot in self.slots:
-            if self.cache._waiting.get(slot) is self:
-                del self.cache._waiting[slot]
+            steps = self.cache._waiting.get(slot, [])
+            if self in steps:
+                steps.remove(self)
+                if not steps:
+                    del self.cache._waiting[slot]
 
 
 class DeciderCache:
@@ -191,7 +199,7 @@ class DeciderCache:
         self._users = [0] * self.n_pages              # requests that hold a page
         self._pages: dict[int, list[int]] = {}        # of an open request
         self._lens: dict[int, int] = {}
-        self._waiting: dict[int, CacheStep] = {}      # the refused step of an open request
+        self._waiting: dict[int, list[CacheStep]] = {}  # the refused steps of an open request, in order
         self._lost: set[int] = set()                  # open requests that a failed forward left half computed
 
     # ---- requests
@@ -267,12 +275,12 @@ class DeciderCache:
                 raise ValueError(f"{slot} is no open request of the cache")
 
     def _check(self, slots, step=None) -> None:
-        """Refuse requests that are not open, or hold tokens that no forward (but one over ``step``) has computed."""
+        """Refuse requests that are not open, or that hold tokens (before those of ``step``) no forward has computed."""
         self._check_open(slots)
         for slot in slots:
             if slot in self._lost:
                 raise RuntimeError(f"A forward over request {slot} failed on the way; it can only be closed")
-            if self._waiting.get(slot, step) is not step:
+            if slot in self._waiting and (step is None or self._waiting[slot][0]._end(slot) < step._end(slot)):
                 raise RuntimeError(f"A step of request {slot} was refused and has not run: run it or cancel it")
 
     def _take(self) -> int:

@@ -66,7 +66,7 @@ def test_refused_and_failed_forwards(monkeypatch):
     assert torch.equal(model(ids[:, 40:50], cache=step), want) and not c._waiting
     with torch.enable_grad(), pytest.raises(RuntimeError, match="no gradients"):
         model(ids[:, 50:51], cache=c.step(slots[1][:1], [1]))
-    c._waiting[slots[1][0]].cancel()
+    c._waiting[slots[1][0]][0].cancel()
 
     def broken(*args, **kwargs):
         raise RuntimeError("out of memory, say")

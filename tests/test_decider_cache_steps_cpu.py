@@ -162,3 +162,28 @@ def test_a_forked_step_is_not_taken_back():
     step = c.step([a], [30])
     step.cancel()
     assert c.length(a) == c.length(b) == 20 and c._pages[a][0] == c._pages[b][0]
+
+
+@torch.no_grad()
+def test_refused_steps_wait_in_order(model):
+    """The second of two refused steps still waits when the first has run."""
+    c = make()
+    a, b = c.open(), c.open()
+    first, second = c.step([a], [3]), c.step([a, b], [2, 1])
+    for step in (second, first, second):
+        with pytest.raises(ValueError, match="ids"):
+            model(ids(9), cache=step)
+    with pytest.raises(RuntimeError, match="run it or cancel it"):
+        model(ids(3), cache=second)
+    first._done()                                          # as after a forward
+    with pytest.raises(RuntimeError, match="run it or cancel it"):
+        c.step([a], [1])
+    with pytest.raises(RuntimeError, match="install_hip_kernels"):  # it is its turn
+        model(ids(3), cache=second)
+    second.cancel()
+    assert c.length(a) == 3 and c.length(b) == 0 and not c._waiting
+    first, second = c.step([a], [1]), c.step([a], [2])
+    with pytest.raises(ValueError, match="ids"):
+        model(ids(9), cache=second)
+    with pytest.raises(RuntimeError, match="install_hip_kernels"):  # a refused later step holds nothing back before it
+        model(ids(1), cache=first)
