@@ -16,6 +16,7 @@ from . import _lib
 LIB_PATH = Path(os.environ.get("FD_CACHE_LIB", Path(__file__).resolve().parent / "libfd_cache.so"))
 
 FD_DTYPE_E4M3 = 2
+FD_DTYPE_E2M1 = 3
 
 # Strides and the cache struct are handed over as packed bytes (c_void_p takes them): building ctypes
 # arrays and structures field by field costs microseconds a call, as much as a small launch.

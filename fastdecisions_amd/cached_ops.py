@@ -14,7 +14,7 @@ import torch
 from .gated_delta_kernel import chunk_gated_delta_rule, recurrent_gated_delta_rule
 from .packed_conv_kernel import prep_qkv_state
 from .paged_gqa_kernel import paged_gqa_attention
-from .paged_kv_kernel import paged_kv_read, paged_kv_write
+from .paged_kv_kernel import cache_dim, paged_kv_read, paged_kv_write
 
 
 @torch.library.custom_op("fastdecisions_cache::paged_kv_write", mutates_args=("k_cache", "v_cache", "k_scale", "v_scale"),
@@ -40,7 +40,7 @@ def paged_kv_read_op(k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: t
 
 @paged_kv_read_op.register_fake
 def _paged_kv_read_fake(k_cache, v_cache, page_table, cu_seqlens, total, k_scale, v_scale):
-    _, h, _, d = k_cache.shape
+    h, d = k_cache.shape[1], cache_dim(k_cache)
     return tuple(k_cache.new_empty((1, total, h, d), dtype=torch.bfloat16).transpose(1, 2) for _ in range(2))
 
 

@@ -44,34 +44,39 @@ constexpr int kNumXcd = 8;
 constexpr int kCus = 256;  // a power of two (slots_log2)
 
 // Few rows: NR blocks of 16 rows; every wavefront stages blocks of 32 keys of its own.
-template <int D_, bool FP8_, int NR_>
+template <int D_, Format F_, int NR_>
 struct Few {
   static constexpr int D = D_, NR = NR_;
-  static constexpr bool FP8 = FP8_;
+  static constexpr Format F = F_;
+  static constexpr bool FP8 = F == kE4m3, FP4 = F == kE2m1;
   static constexpr int kWaves = 4;
   static constexpr int kThreads = 64 * kWaves;
   static constexpr int kRows = 16 * NR;
   static constexpr int kKeys = 32 * kWaves;             // keys of a tile: a block of each wavefront
-  static constexpr int kRowBytes = FP8 ? D : 2 * D;     // of a cached row, staged as it is
+  static constexpr int kRowBytes = FP4 ? D / 2 : FP8 ? D : 2 * D;  // of a cached row, staged as it is
   static constexpr int kBlockBytes = 32 * kRowBytes;    // K or V of a block
-  static constexpr int kScaleBytes = FP8 ? 256 : 0;     // 32 K scales and 32 V scales, a word each
+  // 32 K scales and 32 V scales, a word each; of E2M1 the D / 32 bytes of 32 rows of each, at least a word a row
+  static constexpr int kScaleCopies = FP8 ? 1 : FP4 ? (D == 256 ? 2 : 1) : 0;
+  static constexpr int kScaleBytes = 256 * kScaleCopies;
   static constexpr int kStageBytes = 2 * kBlockBytes + kScaleBytes;
-  static constexpr int kStages = kBlockBytes >= 8192 ? 1 : 8192 / kBlockBytes;
+  static constexpr int kStages = kBlockBytes >= 8192 ? 1 : kBlockBytes <= 2048 ? 4 : 8192 / kBlockBytes;
+  static constexpr int kDecoded = FP4 ? 2048 : 0;       // 32 features of a V block as bf16
   static constexpr int kCopies = kBlockBytes / 1024;    // copy instructions of a block's K (or V)
   static constexpr int kCopyRows = 1024 / kRowBytes;
-  static constexpr int kKGroup = kCopies + (FP8 ? 1 : 0);  // with the scales
+  static constexpr int kKGroup = kCopies + kScaleCopies;
   static constexpr int kRowFloats = D + 4;
   static constexpr int kEpilogueBytes = kWaves * kRows * (kRowFloats + 2) * 4;
-  static constexpr int kLoopBytes = kWaves * kStages * kStageBytes;
+  static constexpr int kLoopBytes = kWaves * (kStages * kStageBytes + kDecoded);
   static constexpr int kSmemBytes = kLoopBytes > kEpilogueBytes ? kLoopBytes : kEpilogueBytes;
   static constexpr int kPerCu = kSmemBytes > 80 * 1024 ? 1 : 2;  // workgroups that a CU's LDS holds
 };
 
 // Pieces: RW row wavefronts of NB blocks of 32 rows, times KS key parts of a tile.
-template <int D_, bool FP8_, int RW_, int NB_, int KS_>
+template <int D_, Format F_, int RW_, int NB_, int KS_>
 struct Piece {
   static constexpr int D = D_, RW = RW_, NB = NB_, KS = KS_;
-  static constexpr bool FP8 = FP8_;
+  static constexpr Format F = F_;
+  static constexpr bool CODES = F != kBf16;
   static constexpr int kWaves = RW * KS;
   static constexpr int kThreads = 64 * kWaves;
   static constexpr int kRows = 32 * RW * NB;
@@ -85,7 +90,7 @@ struct Piece {
   // 1 KiB copies of a bf16 K (or V) tile per wavefront, and the rows of each
   static constexpr int kCopies = kTileBytes / 1024 / kWaves;
   static constexpr int kCopyRows = 1024 / (2 * D);
-  // loads of 16 codes per lane of an E4M3 tile per wavefront, and their rows
+  // loads of 16 codes per lane of a tile per wavefront, and their rows
   static constexpr int kLoads = kKeys * D / 1024 / kWaves;
   static constexpr int kLoadRows = 1024 / D;
   static_assert(kCopies >= 1 && kLoads >= 1, "a tile gives every wavefront a whole copy");
@@ -426,14 +431,15 @@ __device__ __forceinline__ int sigma16(int a, int m) { return 8 * (m >> 2) + 4 *
 // together lie in different banks: 16 permuted rows at one chunk for K; for V the 4 (bf16, chunk
 // pairs) or 8 (codes) rows of a transposing read and the next lane group's.
 template <int ROW_BYTES>
-constexpr int kRowShift = ROW_BYTES >= 256 ? 0 : ROW_BYTES == 128 ? 1 : 2;
+constexpr int kRowShift = ROW_BYTES >= 256 ? 0 : ROW_BYTES == 128 ? 1 : ROW_BYTES == 64 ? 2 : 3;
 template <int ROW_BYTES>
 __device__ __forceinline__ int few_swz_k(int row) {
   return ((row & 3) | ((row >> 3) & 3) << 2) >> kRowShift<ROW_BYTES>;
 }
-template <int ROW_BYTES, bool FP8>
+template <int ROW_BYTES, Format F>
 __device__ __forceinline__ int few_swz_v(int row) {
-  if constexpr (FP8) return ((row & 7) | ((row >> 3) & 1) << 3) >> kRowShift<ROW_BYTES>;
+  if constexpr (F == kE2m1) return (row >> 2) & (ROW_BYTES / 16 < 4 ? 1 : 3);
+  else if constexpr (F == kE4m3) return ((row & 7) | ((row >> 3) & 1) << 3) >> kRowShift<ROW_BYTES>;
   else return 2 * (((row & 3) | ((row >> 3) & 1) << 2) >> kRowShift<ROW_BYTES>);
 }
 
@@ -506,6 +512,17 @@ __device__ __forceinline__ void byte_to_lds(const uint8_t* p, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_ubyte %0, off" ::"v"(p), "s"(lds) : "memory", "m0");
 }
 
+// Two bytes (zero-extended), four or sixteen per lane, likewise, each lane's from an address of its own.
+__device__ __forceinline__ void short_to_lds(const uint8_t* p, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_ushort %0, off" ::"v"(p), "s"(lds) : "memory", "m0");
+}
+__device__ __forceinline__ void word_to_lds(const uint8_t* p, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(p), "s"(lds) : "memory", "m0");
+}
+__device__ __forceinline__ void lane_to_lds(const unsigned char* p, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(p), "s"(lds) : "memory", "m0");
+}
+
 // A block of 32 keys costs a wavefront 24 (NR) MFMAs of 16x16x32 and, at the memory's rate, several
 // times as long to arrive, so what counts is that copies are always in flight: rows go to LDS as they
 // are (codes are converted where they are read, scales multiply scores and probabilities), K and V
@@ -517,7 +534,7 @@ __device__ __forceinline__ void byte_to_lds(const uint8_t* p, uint32_t lds) {
 template <class S>
 __global__ __launch_bounds__(S::kThreads, S::kPerCu) void paged_gqa_few_kernel(PagedArgs a) {
   constexpr int D = S::D, NR = S::NR, RBY = S::kRowBytes, kKk = D / 32, kNdb = D / 16, NS = S::kStages;
-  constexpr bool FP8 = S::FP8;
+  constexpr bool FP8 = S::FP8, FP4 = S::FP4;
   __shared__ __attribute__((aligned(1024))) unsigned char smem[S::kSmemBytes];
   const int tid = threadIdx.x;
   const int lane = tid & 63;
@@ -559,10 +576,13 @@ __global__ __launch_bounds__(S::kThreads, S::kPerCu) void paged_gqa_few_kernel(P
 #pragma unroll
     for (int i = 0; i < S::kCopies; ++i) {
       const int row = i * S::kCopyRows + lane / kChunks;
-      const int chunk = (lane % kChunks) ^ (v ? few_swz_v<RBY, FP8>(row) : few_swz_k<RBY>(row));
+      const int chunk = (lane % kChunks) ^ (v ? few_swz_v<RBY, S::F>(row) : few_swz_k<RBY>(row));
       const int key = min(kb0 + row, kend - 1) & page_mask;
-      copy_to_lds(head_base[v] + pg.p[i * S::kCopyRows / 16] * a.c.page,
-                  static_cast<uint32_t>(key * static_cast<int>(a.c.row) + chunk * 16), lds + static_cast<uint32_t>(i * 1024));
+      const uint32_t at = static_cast<uint32_t>(key * static_cast<int>(a.c.row) + chunk * 16);
+      if constexpr (S::kCopyRows > 16)  // rows of both pages
+        lane_to_lds(head_base[v] + (row < 16 ? pg.p[0] : pg.p[1]) * a.c.page + at, lds + static_cast<uint32_t>(i * 1024));
+      else
+        copy_to_lds(head_base[v] + pg.p[i * S::kCopyRows / 16] * a.c.page, at, lds + static_cast<uint32_t>(i * 1024));
     }
   };
   auto copy_k = [&](const Pages& pg, int j) {
@@ -573,6 +593,20 @@ __global__ __launch_bounds__(S::kThreads, S::kPerCu) void paged_gqa_few_kernel(P
       const int page = row < 16 ? pg.p[0] : pg.p[1];
       byte_to_lds((lane < 32 ? a.c.k_scale : a.c.v_scale) + page * a.c.s_page + it.head * a.c.s_head + key,
                   lds0 + static_cast<uint32_t>((j & (NS - 1)) * S::kStageBytes + 2 * S::kBlockBytes));
+    }
+    if constexpr (FP4) {  // a row's scales in one word per lane, of 256 features in two
+#pragma unroll
+      for (int i = 0; i < S::kScaleCopies; ++i) {
+        const int row = D == 256 ? lane >> 1 : lane & 31;
+        const bool of_k = D == 256 ? i == 0 : lane < 32;
+        const int key = min(first + j * S::kKeys + row, kend - 1) & page_mask;
+        const int page = row < 16 ? pg.p[0] : pg.p[1];
+        const uint8_t* const p = (of_k ? a.c.k_scale : a.c.v_scale) + page * a.c.s_page + it.head * a.c.s_head +
+                                 key * (D / kScaleBlock) + (D == 256 ? 4 * (lane & 1) : 0);
+        const uint32_t lds = lds0 + static_cast<uint32_t>((j & (NS - 1)) * S::kStageBytes + 2 * S::kBlockBytes + i * 256);
+        if constexpr (D == 64) short_to_lds(p, lds);
+        else word_to_lds(p, lds);
+      }
     }
   };
   auto copy_v = [&](const Pages& pg, int j) { copy_side(pg, j, 1); };
@@ -596,9 +630,12 @@ __global__ __launch_bounds__(S::kThreads, S::kPerCu) void paged_gqa_few_kernel(P
     pos[n] = it.len - it.n_new + token;
     const int b = a.cu == nullptr ? it.req : 0;
     const int head = it.head * a.group + (it.rem0 + row - local * a.group);
-    const uint16_t* qp = a.q + b * a.qs[0] + head * a.qs[1] + static_cast<int64_t>(it.start + token) * a.qs[2] + grp * 8;
+    const uint16_t* qp = a.q + b * a.qs[0] + head * a.qs[1] + static_cast<int64_t>(it.start + token) * a.qs[2];
+    // the features of a product's step are any 32, the same ones of Q and K: of E2M1 a lane takes D / 4 in a row, so that
+    // its codes of a key are one read with few scales
 #pragma unroll
-    for (int kk = 0; kk < kKk; ++kk) qf[n][kk] = *reinterpret_cast<const bf16x8_t*>(qp + kk * 32);
+    for (int kk = 0; kk < kKk; ++kk)
+      qf[n][kk] = *reinterpret_cast<const bf16x8_t*>(qp + (FP4 ? grp * (D / 4) + kk * 8 : kk * 32 + grp * 8));
   }
   const int pos_min = it.len - it.n_new + it.token0;
   const bool absent = any_absent<S>(a, job, table, lane);
@@ -624,10 +661,29 @@ __global__ __launch_bounds__(S::kThreads, S::kPerCu) void paged_gqa_few_kernel(P
     for (int h = 0; h < 2; ++h) {
       const int row = sigma16(h, li);
       const int swz = few_swz_k<RBY>(row);
+      uint32_t codes[kKk];  // E2M1: this lane's D / 4 of the key
+      float scales[D == 256 ? 2 : 1];
+      if constexpr (FP4) {
+        const uint8_t* const sc = st + 2 * S::kBlockBytes;
+        if constexpr (D == 64) {
+          const uint2 w = *reinterpret_cast<const uint2*>(st + row * RBY + ((grp >> 1) ^ swz) * 16 + 8 * (grp & 1));
+          codes[0] = w.x, codes[1] = w.y;
+          scales[0] = scale_of(sc[row * 4 + (grp >> 1)]);
+        } else {
+#pragma unroll
+          for (int c = 0; c < D / 128; ++c) {
+            const uint4 w = *reinterpret_cast<const uint4*>(st + row * RBY + ((grp * (D / 128) + c) ^ swz) * 16);
+            codes[4 * c] = w.x, codes[4 * c + 1] = w.y, codes[4 * c + 2] = w.z, codes[4 * c + 3] = w.w;
+            scales[c] = scale_of(sc[row * (D / kScaleBlock) + grp * (D / 128) + c]);
+          }
+        }
+      }
 #pragma unroll
       for (int kk = 0; kk < kKk; ++kk) {
         bf16x8_t kf;
-        if constexpr (FP8) {
+        if constexpr (FP4) {
+          kf = e2m1_to_bf16(codes[kk], scales[kk / 4]);
+        } else if constexpr (FP8) {
           const uint2 w = *reinterpret_cast<const uint2*>(st + row * RBY + ((2 * kk + (grp >> 1)) ^ swz) * 16 + 8 * (grp & 1));
           kf = codes_to_bf16(w.x, w.y);
         } else {
@@ -713,11 +769,11 @@ __global__ __launch_bounds__(S::kThreads, S::kPerCu) void paged_gqa_few_kernel(P
         typedef __attribute__((address_space(3))) v2i_t lds_v2i_t;
         const int row = 8 * grp + (li >> 1);
         const v2i_t w = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
-            (lds_v2i_t*)(st + row * RBY + (db ^ few_swz_v<RBY, true>(row)) * 16 + 8 * (li & 1)));
+            (lds_v2i_t*)(st + row * RBY + (db ^ few_swz_v<RBY, kE4m3>(row)) * 16 + 8 * (li & 1)));
         vf[db] = codes_to_bf16(static_cast<uint32_t>(w[0]), static_cast<uint32_t>(w[1]));
       } else {
         const int row = 8 * grp + (li >> 2);
-        const unsigned char* vp = st + row * RBY + ((2 * db + ((li & 3) >> 1)) ^ few_swz_v<RBY, false>(row)) * 16 + 8 * (li & 1);
+        const unsigned char* vp = st + row * RBY + ((2 * db + ((li & 3) >> 1)) ^ few_swz_v<RBY, kBf16>(row)) * 16 + 8 * (li & 1);
         const v4i16_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16_t*)vp);
         const v4i16_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16_t*)(vp + 4 * RBY));
         const short __attribute__((ext_vector_type(8))) vv = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
@@ -743,11 +799,11 @@ __global__ __launch_bounds__(S::kThreads, S::kPerCu) void paged_gqa_few_kernel(P
           for (int db = 0; db < kNdb; ++db) {
             f32x4_t x;
             if constexpr (FP8) {
-              const uint32_t w = *reinterpret_cast<const uint32_t*>(st + key * RBY + (db ^ few_swz_v<RBY, true>(key)) * 16 + 4 * grp);
+              const uint32_t w = *reinterpret_cast<const uint32_t*>(st + key * RBY + (db ^ few_swz_v<RBY, kE4m3>(key)) * 16 + 4 * grp);
               x = __builtin_convertvector(__builtin_shufflevector(codes_to_bf16(w, w), bf16x8_t{}, 0, 1, 2, 3), f32x4_t);
             } else {
               x = __builtin_convertvector(*reinterpret_cast<const bf16x4_t*>(
-                  st + key * RBY + ((2 * db + (grp >> 1)) ^ few_swz_v<RBY, false>(key)) * 16 + 8 * (grp & 1)), f32x4_t);
+                  st + key * RBY + ((2 * db + (grp >> 1)) ^ few_swz_v<RBY, kBf16>(key)) * 16 + 8 * (grp & 1)), f32x4_t);
             }
 #pragma unroll
             for (int n = 0; n < NR; ++n) o[n][db] = add_odd(o[n][db], x, ph[n]);
@@ -762,6 +818,59 @@ __global__ __launch_bounds__(S::kThreads, S::kPerCu) void paged_gqa_few_kernel(P
         o[n][db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf[db], pb[n], o[n][db], 0, 0, 0);
         o[n][db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf[db], pl[n], o[n][db], 0, 0, 0);
       }
+  };
+
+  // E2M1: 32 features of V at a time become bf16 in LDS of the wavefront (a lane: half a row of them, one scale), from
+  // where the transposing reads take them; their features' products follow.
+  auto p_v_codes = [&](int j) {
+    const unsigned char* const st = stage0 + (j & (NS - 1)) * S::kStageBytes + S::kBlockBytes;
+    const uint8_t* const sc = st + S::kBlockBytes + (D == 256 ? 256 : 128);
+    unsigned char* const bf = smem + S::kWaves * NS * S::kStageBytes + wave * S::kDecoded;
+    const bool masked = first + j * S::kKeys + 31 > pos_min || absent;
+    const int row = lane >> 1, half = lane & 1;
+    auto chunk_of = [](int r, int c) { return c ^ (((r >> 3) & 1) << 1); };  // physical chunk of row r: lane groups' rows apart
+#pragma unroll
+    for (int c = 0; c < D / kScaleBlock; ++c) {
+      const uint2 w = *reinterpret_cast<const uint2*>(st + row * RBY + (c ^ few_swz_v<RBY, kE2m1>(row)) * 16 + 8 * half);
+      const float scale = scale_of(sc[row * (D == 64 ? 4 : D / kScaleBlock) + c]);
+      *reinterpret_cast<bf16x8_t*>(bf + row * 64 + chunk_of(row, 2 * half) * 16) = e2m1_to_bf16(w.x, scale);
+      *reinterpret_cast<bf16x8_t*>(bf + row * 64 + chunk_of(row, 2 * half + 1) * 16) = e2m1_to_bf16(w.y, scale);
+      bf16x8_t vf[2];  // V[key 8 grp + i][32 c + 16 u + li]
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int r = 8 * grp + (li >> 2);
+        const unsigned char* vp = bf + r * 64 + chunk_of(r, 2 * u + ((li & 3) >> 1)) * 16 + 8 * (li & 1);
+        const v4i16_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16_t*)vp);
+        const v4i16_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16_t*)(vp + 4 * 64));
+        const short __attribute__((ext_vector_type(8))) vv = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+        vf[u] = __builtin_bit_cast(bf16x8_t, vv);
+      }
+      if (masked && (__builtin_amdgcn_ballot_w64(any_odd(vf[0])) | __builtin_amdgcn_ballot_w64(any_odd(vf[1]))) != 0) {
+        // blocks of NaN leave the product and are added by hand to the rows that see them
+#pragma unroll
+        for (int u = 0; u < 2; ++u) vf[u] = without_odd(vf[u]);
+#pragma unroll 1
+        for (int key = 0; key < 32; ++key) {
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const f32x4_t x = __builtin_convertvector(*reinterpret_cast<const bf16x4_t*>(
+                bf + key * 64 + chunk_of(key, 2 * u + (grp >> 1)) * 16 + 8 * (grp & 1)), f32x4_t);
+#pragma unroll
+            for (int n = 0; n < NR; ++n) {
+              const float ph = __shfl(element(pb[n], key & 7) + element(pl[n], key & 7), 16 * (key >> 3) + li);
+              o[n][2 * c + u] = add_odd(o[n][2 * c + u], x, ph);
+            }
+          }
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int n = 0; n < NR; ++n) {
+          o[n][2 * c + u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf[u], pb[n], o[n][2 * c + u], 0, 0, 0);
+          o[n][2 * c + u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf[u], pl[n], o[n][2 * c + u], 0, 0, 0);
+        }
+    }
   };
 
   // ---- the loop: copies in the queue, oldest first, at block j's scores: K(j) V(j) .. K(j + NS - 1) V(j + NS - 1)
@@ -779,7 +888,8 @@ __global__ __launch_bounds__(S::kThreads, S::kPerCu) void paged_gqa_few_kernel(P
     } else {
       wait_copies<0>();
     }
-    p_v(j);
+    if constexpr (FP4) p_v_codes(j);
+    else p_v(j);
     wait_lds_reads();
     if (more) copy_v(next, j + NS);
     next = pages_of(j + NS + 1);
@@ -847,7 +957,8 @@ __device__ __forceinline__ void pieces(int m, F f) {
 template <class S>
 __global__ __launch_bounds__(S::kThreads) void paged_gqa_piece_kernel(PagedArgs a) {
   constexpr int D = S::D, NB = S::NB, CR = S::CR, kNdb = D / 32, kSteps = D / 16, kAhead = 4;
-  constexpr bool FP8 = S::FP8;
+  constexpr bool CODES = S::CODES;
+  constexpr int kScales = S::F == kE2m1 ? D / kScaleBlock : 1;  // scale bytes of a row
   __shared__ __attribute__((aligned(1024))) unsigned char smem[S::kSmemBytes];
   const int tid = threadIdx.x;
   const int lane = tid & 63;
@@ -888,10 +999,11 @@ __global__ __launch_bounds__(S::kThreads) void paged_gqa_piece_kernel(PagedArgs 
   const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_void_t*)smem));
   unsigned char* const k_lds = smem;
   unsigned char* const v_lds = smem + S::kStages * S::kTileBytes;
-  constexpr int kMoves = FP8 ? S::kLoads : S::kCopies;  // per wavefront and side
-  constexpr int kMoveRows = FP8 ? S::kLoadRows : S::kCopyRows;
-  constexpr int kLanesRow = 64 / kMoveRows;             // lanes of a row, 16 bytes each
-  const int lrow = lane / kLanesRow;
+  constexpr int kMoves = CODES ? S::kLoads : S::kCopies;  // per wavefront and side
+  constexpr int kMoveRows = CODES ? S::kLoadRows : S::kCopyRows;
+  constexpr int kLanesRow = 64 / kMoveRows;             // lanes of a row, 16 bytes each (of E2M1: 8)
+  using Word = std::conditional_t<S::F == kE2m1, uint2, uint4>;  // 16 codes
+  const int lrow = lane / kLanesRow, lcol = lane % kLanesRow;
   struct Pages {
     int p[kMoves];
   };
@@ -938,23 +1050,27 @@ __global__ __launch_bounds__(S::kThreads) void paged_gqa_piece_kernel(PagedArgs 
       for (int v = 0; v < 2; ++v) copy_piece(whole_c, pg, t, buf, i, v);
   };
   struct Codes {
-    uint4 w[FP8 ? 2 * S::kLoads : 1];
-    uint32_t s[FP8 ? 2 * S::kLoads : 1];
+    Word w[CODES ? 2 * S::kLoads : 1];
+    uint32_t s[CODES ? 2 * S::kLoads : 1];
   };
   auto load_piece = [&](auto whole_c, const Pages& pg, int t, Codes& x, int i, int v) {
     const uint32_t row = static_cast<uint32_t>(lane_row(whole_c, t, i));
     const int first = first_row(whole_c, t, i);
-    x.w[2 * i + v] = *reinterpret_cast<const uint4*>(head_base[v] + move_offset(pg.p[i], first) + (row * row_bytes + (lane % kLanesRow) * 16));
-    x.s[2 * i + v] = (scale_base[v] + static_cast<uint64_t>(static_cast<uint32_t>(a.c.s_page)) * static_cast<uint32_t>(pg.p[i]) + first)[row];
+    x.w[2 * i + v] = *reinterpret_cast<const Word*>(head_base[v] + move_offset(pg.p[i], first) + (row * row_bytes + lcol * static_cast<int>(sizeof(Word))));
+    x.s[2 * i + v] = (scale_base[v] + static_cast<uint64_t>(static_cast<uint32_t>(a.c.s_page)) * static_cast<uint32_t>(pg.p[i]) + first * kScales)
+        [row * kScales + (kScales > 1 ? lcol / 2 : 0)];
   };
   auto store_piece = [&](const Codes& x, int buf, int i, int v) {
     const int row = move_row(i) + lrow;
     const float s = scale_of(x.s[2 * i + v]);
     unsigned char* const dst = (v ? v_lds : k_lds) + buf * S::kTileBytes + row * CR * 16;
     const int swz = v ? swz_v<CR>(row) : swz_k<CR>(row);
-    const uint4 w = x.w[2 * i + v];
-    *reinterpret_cast<bf16x8_t*>(dst + (((lane % kLanesRow) * 2) ^ swz) * 16) = codes_to_bf16(w.x, w.y, s);
-    *reinterpret_cast<bf16x8_t*>(dst + (((lane % kLanesRow) * 2 + 1) ^ swz) * 16) = codes_to_bf16(w.z, w.w, s);
+    const Word w = x.w[2 * i + v];
+    bf16x8_t lo, hi;
+    if constexpr (S::F == kE2m1) lo = e2m1_to_bf16(w.x, s), hi = e2m1_to_bf16(w.y, s);
+    else lo = codes_to_bf16(w.x, w.y, s), hi = codes_to_bf16(w.z, w.w, s);
+    *reinterpret_cast<bf16x8_t*>(dst + ((lcol * 2) ^ swz) * 16) = lo;
+    *reinterpret_cast<bf16x8_t*>(dst + ((lcol * 2 + 1) ^ swz) * 16) = hi;
   };
   auto load_tile = [&](auto whole_c, const Pages& pg, int t, Codes& x) {
 #pragma unroll
@@ -1075,7 +1191,7 @@ __global__ __launch_bounds__(S::kThreads) void paged_gqa_piece_kernel(PagedArgs 
   // before the pipelined loop's last step.
   constexpr int kAheadTiles = 3;
   auto ahead = [&]() {
-    if constexpr (FP8) {
+    if constexpr (CODES) {
       if (n_full < nt) load_tile(part, pages_of(part, n_full), n_full, codes);
     } else {
 #pragma unroll
@@ -1087,7 +1203,7 @@ __global__ __launch_bounds__(S::kThreads) void paged_gqa_piece_kernel(PagedArgs 
     f32x16_t sA[NB], sB[NB];
     Pages next;
     // Prologue: tiles 0 and 1 landed (Q too), tile 2 on its way; scores of tile 0 and the head of its softmax.
-    if constexpr (!FP8) {
+    if constexpr (!CODES) {
       copy_tile(whole, pages_of(whole, 0), 0, 0);
       if (n_full > 1) copy_tile(whole, pages_of(whole, 1), 1, 1);
       next = pages_of(whole, 2);
@@ -1133,7 +1249,7 @@ __global__ __launch_bounds__(S::kThreads) void paged_gqa_piece_kernel(PagedArgs 
       // the matrix core works
       constexpr int kMoveEvery = NB * kSteps / (2 * kMoves);
       auto move_piece = [&](int u) {
-        if constexpr (FP8) {
+        if constexpr (CODES) {
           if (t + 2 < n_full) store_piece(codes, (BUF + 2) & 3, u / 2, u % 2);
           if (issued) load_piece(whole, next, t + 3, codes, u / 2, u % 2);
         } else {
@@ -1176,7 +1292,7 @@ __global__ __launch_bounds__(S::kThreads) void paged_gqa_piece_kernel(PagedArgs 
       }
       rescale();  // by tile t's alpha: phase B moves it on to tile t + 1
       if constexpr (!LAST) {
-        if constexpr (!FP8) {
+        if constexpr (!CODES) {
           if (issued) wait_copies<2 * S::kCopies>();  // all but this step's: tile t + 2 has landed
           else wait_copies<0>();
         }
@@ -1226,8 +1342,8 @@ __global__ __launch_bounds__(S::kThreads) void paged_gqa_piece_kernel(PagedArgs 
 #pragma unroll 1
   for (int t = n_full; t < nt; ++t) {
     const bool early = t < n_full + kAheadTiles;  // copied ahead
-    const int buf = FP8 || early ? t & 3 : 0;
-    if constexpr (FP8) {
+    const int buf = CODES || early ? t & 3 : 0;
+    if constexpr (CODES) {
       store_tile(codes, buf);  // (the stages being read are those of tiles t - 1 and earlier)
       if (t + 1 < nt) load_tile(part, pages_of(part, t + 1), t + 1, codes);
       __syncthreads();
@@ -1493,13 +1609,15 @@ __global__ __launch_bounds__(256) void paged_gqa_join_kernel(PagedArgs a) {
 }
 
 // 128 rows (see the kernel): 4 wavefronts, at 128 features 8
-template <int D, bool FP8>
-using PieceOf = std::conditional_t<D == 256, Piece<D, FP8, 4, 1, 1>,
-                                   std::conditional_t<D == 128, Piece<D, FP8, 4, 1, 2>, Piece<D, FP8, 2, 2, 2>>>;
+template <int D, Format F>
+using PieceOf = std::conditional_t<D == 256, Piece<D, F, 4, 1, 1>,
+                                   std::conditional_t<D == 128, Piece<D, F, 4, 1, 2>, Piece<D, F, 2, 2, 2>>>;
 
-static_assert(Few<64, false, 1>::kPerCu == 2 && Few<64, true, 1>::kPerCu == 2 && Few<128, true, 1>::kPerCu == 2 &&
-              Few<256, true, 1>::kPerCu == 2 && Few<64, false, 2>::kPerCu == 2 && Few<64, true, 2>::kPerCu == 2 &&
-              Few<128, true, 2>::kPerCu == 2 && Few<256, true, 2>::kPerCu == 1, "plan_of's workgroups per CU");
+template <Format F>
+constexpr bool kCodesPerCu = Few<64, F, 1>::kPerCu == 2 && Few<128, F, 1>::kPerCu == 2 && Few<256, F, 1>::kPerCu == 2 &&
+                             Few<64, F, 2>::kPerCu == 2 && Few<128, F, 2>::kPerCu == 2 && Few<256, F, 2>::kPerCu == 1;
+static_assert(Few<64, kBf16, 1>::kPerCu == 2 && Few<64, kBf16, 2>::kPerCu == 2 && kCodesPerCu<kE4m3> && kCodesPerCu<kE2m1>,
+              "plan_of's workgroups per CU");
 constexpr int kHeaderBytes = 256;  // of the workspace: range_tiles
 
 // The kernel of a call, and its items, row tiles and workspace, whatever the lengths turn out to be.
@@ -1511,7 +1629,8 @@ struct Plan {
 };
 
 Plan plan_of(int64_t requests, int64_t tokens, int group, int kv_heads, int head_dim, int64_t max_keys, int max_seqlen,
-             bool fp8) {
+             Format format) {
+  const bool codes = format != kBf16;
   Plan p;
   const int64_t rows = static_cast<int64_t>(max_seqlen) * group;
   // Measured with 16 rows, 32 rows and pieces (us; 16/4 heads x 128 unless noted, 64 requests on 2048 keys):
@@ -1521,16 +1640,16 @@ Plan plan_of(int64_t requests, int64_t tokens, int group, int kv_heads, int head
   //   rows 96: 103, 78, 54; 8/2 x 256 123, 112, 70; E4M3 88, 75, 53: pieces, unless the call is so small that latency
   //            counts, up to 128 rows in all (one request of 4096 keys 19, 19, 24)
   const int64_t all_rows = tokens * group;
-  p.few = rows <= 32 ? 1 : rows > 64 && (all_rows > 128 || max_keys > 16384) ? 0 : head_dim == 256 && fp8 ? 1 : 2;
-  p.rows = p.few ? 16 * p.few : PieceOf<64, false>::kRows;
-  p.keys = p.few ? Few<64, false, 1>::kKeys
-                 : head_dim == 64 ? PieceOf<64, false>::kKeys : head_dim == 128 ? PieceOf<128, false>::kKeys : PieceOf<256, false>::kKeys;
+  p.few = rows <= 32 ? 1 : rows > 64 && (all_rows > 128 || max_keys > 16384) ? 0 : head_dim == 256 && codes ? 1 : 2;
+  p.rows = p.few ? 16 * p.few : PieceOf<64, kBf16>::kRows;
+  p.keys = p.few ? Few<64, kBf16, 1>::kKeys
+                 : head_dim == 64 ? PieceOf<64, kBf16>::kKeys : head_dim == 128 ? PieceOf<128, kBf16>::kKeys : PieceOf<256, kBf16>::kKeys;
   // Workgroups per CU.  Few rows: by LDS (Few::kPerCu).  Pieces with 64 features: 245 registers and 64 KiB of LDS, two
   // (2048 tokens on 6144 keys, 16/4 heads: 103 us with ranges for two, 114 for one); with E4M3 265 registers and one
   // (137 us; 150 with ranges for two).
-  const int per_cu = p.few == 1   ? (head_dim == 256 && !fp8 ? Few<256, false, 1>::kPerCu : Few<128, false, 1>::kPerCu)
-                     : p.few == 2 ? (head_dim == 256 ? Few<256, false, 2>::kPerCu : Few<128, false, 2>::kPerCu)
-                                  : (head_dim == 64 && !fp8 ? 2 : 1);
+  const int per_cu = p.few == 1   ? (head_dim == 256 && !codes ? Few<256, kBf16, 1>::kPerCu : Few<128, kBf16, 1>::kPerCu)
+                     : p.few == 2 ? (head_dim == 256 ? Few<256, kBf16, 2>::kPerCu : Few<128, kBf16, 2>::kPerCu)
+                                  : (head_dim == 64 && !codes ? 2 : 1);
   p.slots = kCus * per_cu;
   p.min_tiles = 256 / p.keys;
   // a request's last row tile may be partly empty, its last key range too
@@ -1564,17 +1683,11 @@ void launch(K kernel, const PagedArgs& a, const Plan& p, hipStream_t s) {
   join(paged_gqa_join_kernel<S, 16>, 16);
 }
 
-template <int D, bool FP8>
+template <int D, Format F>
 void launch_as(const PagedArgs& a, const Plan& p, hipStream_t s) {
-  if (p.few == 1) launch<Few<D, false, 1>>(paged_gqa_few_kernel<Few<D, FP8, 1>>, a, p, s);
-  else if (p.few == 2) launch<Few<D, false, 2>>(paged_gqa_few_kernel<Few<D, FP8, 2>>, a, p, s);
-  else launch<PieceOf<D, false>>(paged_gqa_piece_kernel<PieceOf<D, FP8>>, a, p, s);
-}
-
-template <int D>
-void launch_dim(const PagedArgs& a, const Plan& p, bool fp8, hipStream_t s) {
-  if (fp8) launch_as<D, true>(a, p, s);
-  else launch_as<D, false>(a, p, s);
+  if (p.few == 1) launch<Few<D, kBf16, 1>>(paged_gqa_few_kernel<Few<D, F, 1>>, a, p, s);
+  else if (p.few == 2) launch<Few<D, kBf16, 2>>(paged_gqa_few_kernel<Few<D, F, 2>>, a, p, s);
+  else launch<PieceOf<D, kBf16>>(paged_gqa_piece_kernel<PieceOf<D, F>>, a, p, s);
 }
 
 int check_sizes(const char* what, int batch, int q_heads, int kv_heads, int seq_len, int n_seqs, int max_seqlen) {
@@ -1598,11 +1711,11 @@ extern "C" int64_t fd_paged_gqa_workspace_bytes(int batch, int q_heads, int kv_h
   FD_REQUIRE(head_dim == 64 || head_dim == 128 || head_dim == 256, FD_ERR_UNSUPPORTED,
              "%s: head_dim must be 64, 128 or 256 (got %d)", what, head_dim);
   FD_REQUIRE(page_size >= 1 && max_pages >= 1, FD_ERR_INVALID_ARGUMENT, "%s: page_size and max_pages must be >= 1", what);
-  auto bytes = [&](bool fp8) {
+  auto bytes = [&](Format format) {
     return plan_of(n_seqs > 0 ? n_seqs : batch, static_cast<int64_t>(batch) * seq_len, q_heads / kv_heads, kv_heads,
-                   head_dim, static_cast<int64_t>(max_pages) * page_size, max_seqlen, fp8).bytes;
+                   head_dim, static_cast<int64_t>(max_pages) * page_size, max_seqlen, format).bytes;
   };
-  return std::max(bytes(false), bytes(true));
+  return std::max({bytes(kBf16), bytes(kE4m3), bytes(kE2m1)});
 }
 
 extern "C" int fd_paged_gqa_fwd(const void* q, const fd_paged_cache* cache, const void* gate, void* out,
@@ -1625,9 +1738,8 @@ extern "C" int fd_paged_gqa_fwd(const void* q, const fd_paged_cache* cache, cons
              FD_ERR_ALIGNMENT, "%s: rows must be contiguous and 16-byte aligned", what);
   const int requests = n_seqs > 0 ? n_seqs : batch;
   if (requests == 0 || seq_len == 0) return FD_OK;
-  const bool fp8 = cache->dtype == FD_DTYPE_E4M3;
   const Plan p = plan_of(requests, static_cast<int64_t>(batch) * seq_len, q_heads / cache->kv_heads, cache->kv_heads,
-                         cache->head_dim, static_cast<int64_t>(cache->max_pages) * cache->page_size, max_seqlen, fp8);
+                         cache->head_dim, static_cast<int64_t>(cache->max_pages) * cache->page_size, max_seqlen, format_of(cache));
   FD_REQUIRE(p.items < (1LL << 32) / 512 - kNumXcd, FD_ERR_UNSUPPORTED, "%s: problem too large", what);
   FD_REQUIRE(p.bytes == 0 || (workspace && fd_aligned16(workspace) && workspace_bytes >= p.bytes),
              FD_ERR_INVALID_ARGUMENT, "%s: the workspace must be 16-byte aligned and hold %lld bytes", what,
@@ -1654,8 +1766,6 @@ extern "C" int fd_paged_gqa_fwd(const void* q, const fd_paged_cache* cache, cons
   a.range_tiles = p.may_split ? static_cast<int32_t*>(workspace) : nullptr;
   a.part = p.may_split ? static_cast<float*>(workspace) + kHeaderBytes / 4 : nullptr;
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (cache->head_dim == 64) launch_dim<64>(a, p, fp8, s);
-  else if (cache->head_dim == 128) launch_dim<128>(a, p, fp8, s);
-  else launch_dim<256>(a, p, fp8, s);
+  by_kind(cache, [&](auto d, auto f) { launch_as<decltype(d)::value, decltype(f)::value>(a, p, s); });
   return fd_check_launch(what);
 }

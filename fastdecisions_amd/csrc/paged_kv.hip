@@ -27,6 +27,8 @@ constexpr float kE4m3Max = 448.0f;
 // The scale byte of rows whose largest value lies above 1.75 2^127.  From 248 2^120 on their values round to the code of
 // 256, which is 2^128 and no bf16 number: it is read as 255 2^120, the largest one, no further from the value.
 constexpr int kTopByte = 247;
+// The same of E2M1: above 1.5 2^127.  Their codes end at 3, since 4 2^126 is no bf16 number either.
+constexpr int kTopByteE2m1 = 253;
 // A thread takes several rows, their chains of loads side by side, once there is more than a round (write) or a few
 // rounds (read) of workgroups: 1024 of a side (K, V) run at once.  Measured with 1, 2, 4 rows (us, 4 heads x 128 bf16):
 // write 1.2, 5 and 48 thousand tokens 4.0, 4.1, 4.1; 9.6, 9.3, 10.0; 39, 40, 41, E4M3 40, 38, 41; read 12 and 96
@@ -60,6 +62,14 @@ __device__ __forceinline__ int scale_byte(float a) {
   return max(e, 1);
 }
 
+// The same with 6 = 1.5 2^2 in the place of 448.
+__device__ __forceinline__ int scale_byte_e2m1(float a) {
+  const uint32_t u = __float_as_uint(a);
+  if (u == 0) return 127;
+  const int e = static_cast<int>(u >> 23) - 2 + ((u & 0x7fffffu) > 0x400000u ? 1 : 0);
+  return max(e, 1);
+}
+
 // x / 2^E for a code: infinities become the largest code, NaN stays.
 __device__ __forceinline__ float to_code_range(float x, float inv) {
   const float y = x * inv;
@@ -89,9 +99,10 @@ __device__ __forceinline__ void requests_of(const int32_t* cu, int n_seqs, const
 }
 
 // U rows per thread, kThreads / kLanes apart, a stage of all of them at a time: rows, requests, pages, stores.
-template <int D, bool FP8, int U>
+template <int D, Format F, int U>
 __global__ __launch_bounds__(kThreads) void paged_kv_write_kernel(WriteArgs a) {
   constexpr int kLanes = D / 8, kSide = kThreads / kLanes;  // lanes of a row; rows of a workgroup side by side
+  constexpr int kPer = D / kScaleBlock;             // E2M1 scales of a row
   const int side = blockIdx.y;
   const int li = threadIdx.x % kLanes;
   const uint16_t* const x_side = side == 0 ? a.x[0] : a.x[1];
@@ -134,7 +145,7 @@ __global__ __launch_bounds__(kThreads) void paged_kv_write_kernel(WriteArgs a) {
     const bool live = static_cast<unsigned>(page[u]) < static_cast<unsigned>(a.c.n_pages);
     const int at = pos[u] & ((1 << a.c.shift) - 1);
     unsigned char* dst = (side == 0 ? a.c.k : a.c.v) + page[u] * a.c.page + head[u] * a.c.head + at * a.c.row;
-    if constexpr (!FP8) {
+    if constexpr (F == kBf16) {
       if (live) *reinterpret_cast<uint4*>(dst + li * 16) = w[u];
     } else {
       const uint32_t h[4] = {w[u].x, w[u].y, w[u].z, w[u].w};
@@ -148,6 +159,30 @@ __global__ __launch_bounds__(kThreads) void paged_kv_write_kernel(WriteArgs a) {
       for (int i = 0; i < 8; ++i) {
         const float m = fabsf(x[i]);
         top = fmaxf(top, m < __builtin_inff() ? m : 0.0f);  // finite values only
+      }
+      if constexpr (F == kE2m1) {
+        top = fd_xor_max<2>(fd_xor_max<1>(top));  // of the block's four lanes
+        bool nan = false;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) nan |= x[i] != x[i];
+        const uint64_t nans = __builtin_amdgcn_ballot_w64(nan);
+        const bool any_nan = ((nans >> (threadIdx.x & 60)) & 15) != 0;
+        const int byte = scale_byte_e2m1(top);
+        const float inv = __uint_as_float(static_cast<uint32_t>(254 - byte) << 23);  // 2^-E
+        const float most = byte == kTopByteE2m1 ? 3.0f : 6.0f;
+        uint32_t code = 0;
+        auto y = [&](int i) { return fminf(fmaxf(x[i] * inv, -most), most); };  // (a NaN's block has no values)
+        code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, y(0), y(1), 1.0f, 0);
+        code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, y(2), y(3), 1.0f, 1);
+        code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, y(4), y(5), 1.0f, 2);
+        code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, y(6), y(7), 1.0f, 3);
+        if (live) {
+          *reinterpret_cast<uint32_t*>(dst + li * 4) = code;
+          if ((li & 3) == 0)
+            (side == 0 ? a.c.k_scale : a.c.v_scale)[page[u] * a.c.s_page + head[u] * a.c.s_head + at * kPer + li / 4] =
+                static_cast<uint8_t>(any_nan ? 255 : byte);
+        }
+        continue;
       }
       top = group_max<kLanes>(top);  // every lane of the wavefront takes part
       const int byte = scale_byte(top);
@@ -180,7 +215,7 @@ struct ReadArgs {
   int total;
 };
 
-template <int D, bool FP8, int U>
+template <int D, Format F, int U>
 __global__ __launch_bounds__(kThreads) void paged_kv_read_kernel(ReadArgs a) {
   constexpr int kLanes = D / 8, kSide = kThreads / kLanes;
   const int side = blockIdx.y;
@@ -204,6 +239,7 @@ __global__ __launch_bounds__(kThreads) void paged_kv_read_kernel(ReadArgs a) {
     const int slot = key[u] >> a.c.shift;
     page[u] = r[u] >= 0 && slot < a.c.max_pages ? a.c.table[r[u] * a.c.table_stride + slot] : -1;
   }
+  constexpr int kPer = D / kScaleBlock;  // E2M1 scales of a row
   uint4 w[U];
   uint8_t byte[U];
 #pragma unroll
@@ -213,8 +249,11 @@ __global__ __launch_bounds__(kThreads) void paged_kv_read_kernel(ReadArgs a) {
     byte[u] = 0;
     if (static_cast<unsigned>(page[u]) < static_cast<unsigned>(a.c.n_pages)) {
       const unsigned char* src = (side == 0 ? a.c.k : a.c.v) + page[u] * a.c.page + head[u] * a.c.head + at * a.c.row;
-      if constexpr (!FP8) {
+      if constexpr (F == kBf16) {
         w[u] = *reinterpret_cast<const uint4*>(src + li * 16);
+      } else if constexpr (F == kE2m1) {
+        w[u].x = *reinterpret_cast<const uint32_t*>(src + li * 4);
+        byte[u] = (side == 0 ? a.c.k_scale : a.c.v_scale)[page[u] * a.c.s_page + head[u] * a.c.s_head + at * kPer + li / 4];
       } else {
         const uint2 code = *reinterpret_cast<const uint2*>(src + li * 8);
         w[u].x = code.x, w[u].y = code.y;
@@ -225,7 +264,9 @@ __global__ __launch_bounds__(kThreads) void paged_kv_read_kernel(ReadArgs a) {
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     if (r[u] < 0) continue;
-    if constexpr (FP8) {  // codes of no page are zeros, whatever their scale
+    if constexpr (F == kE2m1) {  // codes of no page are zeros, and their scale is finite
+      w[u] = __builtin_bit_cast(uint4, e2m1_to_bf16(w[u].x, scale_of(byte[u])));
+    } else if constexpr (F == kE4m3) {  // codes of no page are zeros, whatever their scale
       const float s = scale_of(byte[u]);
       typedef float f32x2_t __attribute__((ext_vector_type(2)));
       f32x2_t f0 = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(w[u].x), false);
@@ -245,13 +286,6 @@ __global__ __launch_bounds__(kThreads) void paged_kv_read_kernel(ReadArgs a) {
     uint16_t* out = side == 0 ? a.out[0] + head[u] * a.os[0][0] + t[u] * a.os[0][1] : a.out[1] + head[u] * a.os[1][0] + t[u] * a.os[1][1];
     *reinterpret_cast<uint4*>(out + li * 8) = w[u];
   }
-}
-
-template <typename F>
-void by_head_dim(int head_dim, F&& launch) {
-  if (head_dim == 64) launch(std::integral_constant<int, 64>{});
-  else if (head_dim == 128) launch(std::integral_constant<int, 128>{});
-  else launch(std::integral_constant<int, 256>{});
 }
 
 }  // namespace
@@ -286,15 +320,15 @@ extern "C" int fd_paged_kv_write(const void* k, const void* v, const int64_t k_s
   const int64_t blocks = (rows + per - 1) / per;
   FD_REQUIRE(blocks < (1LL << 32) / kThreads, FD_ERR_UNSUPPORTED, "%s: too many rows", what);
   if (blocks == 0) return FD_OK;
-  const bool fp8 = cache->dtype == FD_DTYPE_E4M3;
-  by_head_dim(cache->head_dim, [&](auto d) {
+  by_kind(cache, [&](auto d, auto f) {
     constexpr int D = decltype(d)::value;
+    constexpr Format F = decltype(f)::value;
     auto go = [&](auto kernel, int rows) {
       const dim3 grid(static_cast<unsigned>((blocks + rows - 1) / rows), 2);
       hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, static_cast<hipStream_t>(stream), a);
     };
-    if (blocks <= kAtOnce) fp8 ? go(paged_kv_write_kernel<D, true, 1>, 1) : go(paged_kv_write_kernel<D, false, 1>, 1);
-    else fp8 ? go(paged_kv_write_kernel<D, true, kRows>, kRows) : go(paged_kv_write_kernel<D, false, kRows>, kRows);
+    if (blocks <= kAtOnce) go(paged_kv_write_kernel<D, F, 1>, 1);
+    else go(paged_kv_write_kernel<D, F, kRows>, kRows);
   });
   return fd_check_launch(what);
 }
@@ -326,16 +360,16 @@ extern "C" int fd_paged_kv_read(const fd_paged_cache* cache, void* k_out, void* 
   const int64_t blocks = (total * cache->kv_heads + per - 1) / per;
   FD_REQUIRE(blocks < (1LL << 32) / kThreads, FD_ERR_UNSUPPORTED, "%s: too many rows", what);
   if (blocks == 0) return FD_OK;
-  const bool fp8 = cache->dtype == FD_DTYPE_E4M3;
-  by_head_dim(cache->head_dim, [&](auto d) {
+  by_kind(cache, [&](auto d, auto f) {
     constexpr int D = decltype(d)::value;
+    constexpr Format F = decltype(f)::value;
     auto go = [&](auto kernel, int rows) {
       const dim3 grid(static_cast<unsigned>((blocks + rows - 1) / rows), 2);
       hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, static_cast<hipStream_t>(stream), a);
     };
-    if (blocks <= kAtOnce) fp8 ? go(paged_kv_read_kernel<D, true, 1>, 1) : go(paged_kv_read_kernel<D, false, 1>, 1);
-    else if (blocks <= 4 * kAtOnce) fp8 ? go(paged_kv_read_kernel<D, true, kRows>, kRows) : go(paged_kv_read_kernel<D, false, kRows>, kRows);
-    else fp8 ? go(paged_kv_read_kernel<D, true, kManyRows>, kManyRows) : go(paged_kv_read_kernel<D, false, kManyRows>, kManyRows);
+    if (blocks <= kAtOnce) go(paged_kv_read_kernel<D, F, 1>, 1);
+    else if (blocks <= 4 * kAtOnce) go(paged_kv_read_kernel<D, F, kRows>, kRows);
+    else go(paged_kv_read_kernel<D, F, kManyRows>, kManyRows);
   });
   return fd_check_launch(what);
 }

@@ -6,9 +6,11 @@ pages that requests hold through a page table:
 
 * ``k_cache``, ``v_cache`` — logical ``[n_pages, Hkv, page_size, D]`` (any strides with a
   contiguous feature dimension, the same for both), bf16 or ``torch.float8_e4m3fn``; D 64, 128 or 256,
-  page_size a power of two in [16, 256];
+  page_size a power of two in [16, 256].  In 4 bits: ``torch.float4_e2m1fn_x2``
+  ``[n_pages, Hkv, page_size, D / 2]``, two features a byte, the even one in the low bits;
 * ``k_scale``, ``v_scale`` — for an e4m3 cache, uint8 ``[n_pages, Hkv, page_size]``: byte b
-  stands for 2^(b - 127), and a cached value is its code times that;
+  stands for 2^(b - 127), and a cached value is its code times that.  For a 4-bit cache uint8
+  ``[n_pages, Hkv, page_size, D / 32]``, one for 32 features (255: they are NaN);
 * ``page_table`` — int32 ``[requests, max_pages]``; key j of request r is row
   ``j % page_size`` of page ``page_table[r, j // page_size]``.  An entry outside
   ``[0, n_pages)`` (as -1) is no page: its keys are not written, read as zeros and are
@@ -31,7 +33,15 @@ from . import _cache_lib, _lib
 
 HEAD_DIMS = (64, 128, 256)
 PAGE_SIZES = (16, 32, 64, 128, 256)
-_BF16, _E4M3, _INT32, _UINT8 = torch.bfloat16, torch.float8_e4m3fn, torch.int32, torch.uint8
+SCALE_BLOCK = 32  # features of a 4-bit row that share a scale
+_BF16, _E4M3, _E2M1 = torch.bfloat16, torch.float8_e4m3fn, torch.float4_e2m1fn_x2
+_INT32, _UINT8 = torch.int32, torch.uint8
+_DTYPES = {_BF16: _lib.FD_DTYPE_BF16, _E4M3: _cache_lib.FD_DTYPE_E4M3, _E2M1: _cache_lib.FD_DTYPE_E2M1}
+
+
+def cache_dim(k_cache: torch.Tensor) -> int:
+    """Features of a cache's rows."""
+    return k_cache.shape[-1] * (2 if k_cache.dtype == _E2M1 else 1)
 
 
 def check_cache(k_cache, v_cache, page_table, cache_lens, k_scale, v_scale, requests) -> bytes:
@@ -39,36 +49,43 @@ def check_cache(k_cache, v_cache, page_table, cache_lens, k_scale, v_scale, requ
     shape = k_cache.shape
     if len(shape) != 4 or v_cache.shape != shape:
         raise ValueError("k_cache and v_cache must be [n_pages, Hkv, page_size, D] of one shape")
-    n_pages, heads, page_size, dim = shape
+    n_pages, heads, page_size, _ = shape
     device = k_cache.get_device()
     if device < 0 or v_cache.get_device() != device:
         raise ValueError("The caches must share a CUDA device")
     dtype = k_cache.dtype
-    if (dtype != _BF16 and dtype != _E4M3) or v_cache.dtype != dtype:
-        raise ValueError("The caches must both be BF16 or float8_e4m3fn")
+    if dtype not in _DTYPES or v_cache.dtype != dtype:
+        raise ValueError("The caches must both be BF16, float8_e4m3fn or float4_e2m1fn_x2")
+    dim = cache_dim(k_cache)
     if dim not in HEAD_DIMS:
         raise ValueError("The cache's head dimension must be 64, 128 or 256")
     if page_size not in PAGE_SIZES:
         raise ValueError("page_size must be a power of two in [16, 256]")
     if n_pages < 1 or heads < 1:
         raise ValueError("The cache needs at least one page and one head")
-    fp8 = dtype == _E4M3
+    codes = dtype != _BF16
     k_ptr, v_ptr = k_cache.data_ptr(), v_cache.data_ptr()
     strides = k_cache.stride()
     if v_cache.stride() != strides:
         raise ValueError("k_cache and v_cache must have the same strides")
     sp, sh, sr, sd = strides
-    if sd != 1 or (k_ptr | v_ptr) % 16 or (sp | sh | sr) % (16 if fp8 else 8) or sr >= 1 << 20:
+    if sd != 1 or (k_ptr | v_ptr) % 16 or (sp | sh | sr) % (16 if codes else 8) or sr >= 1 << 20:
         raise ValueError("Cache rows must be contiguous and 16-byte aligned")
     ks = vs = ssp = ssh = 0
-    if fp8:
+    if codes:
+        blocks = (dim // SCALE_BLOCK,) if dtype == _E2M1 else ()
+        per = blocks[0] if blocks else 1  # scale bytes of a row
         for t in (k_scale, v_scale):
-            if (t is None or t.shape != shape[:3] or t.dtype != _UINT8 or t.get_device() != device or t.stride(2) != 1):
-                raise ValueError("An e4m3 cache needs k_scale and v_scale: uint8 [n_pages, Hkv, page_size] on its device")
+            if (t is None or t.shape != (*shape[:3], *blocks) or t.dtype != _UINT8 or t.get_device() != device
+                    or t.stride()[2:] != ((per, 1) if blocks else (1,)) or t.data_ptr() % per):
+                raise ValueError("An e4m3 cache needs k_scale and v_scale: uint8 [n_pages, Hkv, page_size] on its device; "
+                                 "a 4-bit one uint8 [n_pages, Hkv, page_size, D / 32], rows contiguous and aligned")
         ks, vs = k_scale.data_ptr(), v_scale.data_ptr()
         if v_scale.stride() != k_scale.stride():
             raise ValueError("k_scale and v_scale must have the same strides")
-        ssp, ssh, _ = k_scale.stride()
+        ssp, ssh = k_scale.stride()[:2]
+        if (ssp | ssh) % per:
+            raise ValueError("The scales of a 4-bit cache must be aligned to a row's D / 32 bytes")
     elif k_scale is not None or v_scale is not None:
         raise ValueError("A BF16 cache has no scales")
     max_pages = page_table.shape[-1]
@@ -86,7 +103,7 @@ def check_cache(k_cache, v_cache, page_table, cache_lens, k_scale, v_scale, requ
         lens = cache_lens.data_ptr()
     return _cache_lib.pack_cache(k_ptr, v_ptr, ks, vs, sp, sh, sr, sp, sh, sr, ssp, ssh, ssp, ssh, page_table.data_ptr(),
                                  table_stride[0], lens, n_pages, page_size, max_pages, heads, dim,
-                                 _cache_lib.FD_DTYPE_E4M3 if fp8 else _lib.FD_DTYPE_BF16)
+                                 _DTYPES[dtype])
 
 
 def check_cu_seqlens(cu_seqlens, batch, device) -> tuple[int | None, int]:
@@ -130,7 +147,7 @@ def paged_kv_write(
     batch, heads, seq_len, dim = shape
     if batch < 1 or seq_len < 1:
         raise ValueError("Batch and sequence length must be positive")
-    if heads != k_cache.shape[1] or dim != k_cache.shape[3]:
+    if heads != k_cache.shape[1] or dim != cache_dim(k_cache):
         raise ValueError("key and value must have the cache's heads and head dimension")
     if cache_lens is None:
         raise ValueError("cache_lens is required")
@@ -171,7 +188,7 @@ def paged_kv_read(
     if _cache_lib.current_device() != device:
         with torch.cuda.device(device):
             return paged_kv_read(k_cache, v_cache, page_table, cu_seqlens, total, k_scale=k_scale, v_scale=v_scale)
-    _, heads, _, dim = k_cache.shape
+    heads, dim = k_cache.shape[1], cache_dim(k_cache)
     strides = (total * heads * dim, dim, heads * dim, 1)
     k = torch.empty_strided((1, heads, total, dim), strides, device=k_cache.device, dtype=_BF16)
     v = torch.empty_like(k)

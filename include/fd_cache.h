@@ -26,8 +26,10 @@ extern "C" {
 
 #define FD_CACHE_ABI_VERSION 1
 
-/* Cache element type besides FD_DTYPE_BF16: OCP 8-bit floats with 4 exponent and 3 mantissa bits. */
+/* Cache element types besides FD_DTYPE_BF16: OCP 8-bit floats with 4 exponent and 3 mantissa bits. */
 #define FD_DTYPE_E4M3 2
+/* OCP 4-bit floats with 2 exponent bits and 1 mantissa bit, two a byte (the even feature in the low bits). */
+#define FD_DTYPE_E2M1 3
 
 FD_API int fd_cache_abi_version(void);
 
@@ -37,11 +39,14 @@ FD_API const char* fd_cache_last_error(void);
 /*
  * A paged key/value cache and the requests' view of it.
  *
- *   k, v      [n_pages, kv_heads, page_size, head_dim] of dtype (FD_DTYPE_BF16 or FD_DTYPE_E4M3);
- *             strides {page, head, row} in elements, head_dim contiguous; those of k and v the same
+ *   k, v      [n_pages, kv_heads, page_size, head_dim] of dtype (FD_DTYPE_BF16, FD_DTYPE_E4M3 or
+ *             FD_DTYPE_E2M1); strides {page, head, row} in elements (E2M1: in bytes), head_dim contiguous;
+ *             those of k and v the same
  *   k_scale, v_scale  with FD_DTYPE_E4M3: [n_pages, kv_heads, page_size] bytes, strides {page, head},
  *             rows contiguous; byte b stands for the scale 2^(b - 127), b in [1, 254], and a cached
- *             value is its code times that scale.  NULL with FD_DTYPE_BF16
+ *             value is its code times that scale.  With FD_DTYPE_E2M1: [n_pages, kv_heads, page_size,
+ *             head_dim / 32] bytes, one for 32 features, rows contiguous and aligned to their bytes; b in
+ *             [0, 254], 255 makes its 32 values NaN (E8M0).  NULL with FD_DTYPE_BF16
  *   page_table  [requests, max_pages] int32 on the device, rows table_stride elements apart: key j of
  *             request r is row j % page_size of page page_table[r][j / page_size].  An entry outside
  *             [0, n_pages) is no page: its keys are not there (not written, read as zeros, not visible)
@@ -85,6 +90,9 @@ typedef struct fd_paged_cache {
  * row's finite values (E >= -126; 2^0 for a row of zeros), the code is x / 2^E rounded to nearest
  * even; an infinity becomes +-448 * 2^E, a NaN stays NaN.  Powers of two keep the division and the way
  * back exact, so a value is off by at most half a step of its code.
+ * FD_DTYPE_E2M1: the same per 32 features with 6 in the place of 448; values from 3 * 2^126 on are held as
+ * 3 * 2^126 (the next code's 2^128 is no bf16 number); an infinity becomes +-6 * 2^E (+-3 * 2^126 where E
+ * is 126), and a NaN makes its 32 values NaN.
  * A page that two requests of a call write must not be shared between them at the same rows.
  */
 FD_API int fd_paged_kv_write(const void* k, const void* v, const int64_t k_strides[4], const int64_t v_strides[4],
