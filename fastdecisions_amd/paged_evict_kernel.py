@@ -1,0 +1,108 @@
+"""Which cached keys matter, on the gfx950 HIP kernel ``fd_paged_key_weights``.
+
+``paged_key_weights`` adds to each cached key the attention weight that a call's new tokens give it:
+the sum over the tokens and over the query heads of a key head of their softmax probabilities, in
+fp32.  It takes what ``paged_gqa_attention`` takes, after ``paged_kv_write`` of the same tokens:
+
+* ``weights`` — fp32 ``[rows, Hkv, width]``, keys contiguous, ``width`` at least
+  ``max_pages * page_size``; key j of request r is ``weights[row_indices[r], h, j]`` (int32, default
+  row r).  It belongs to a request, not to a page: requests that share pages weigh them apart.  An
+  index outside the rows, or named by an earlier request of the call, adds nothing;
+* ``last`` — only the last ``last`` new tokens of each request count (default: all).
+
+The cache's layout is described in ``paged_kv_kernel``.
+"""
+from __future__ import annotations
+
+from functools import lru_cache
+
+import torch
+
+from . import _cache_lib
+from .paged_kv_kernel import cache_dim, check_cache, check_cu_seqlens, check_rows
+
+
+@lru_cache(maxsize=4096)
+def workspace_bytes(batch: int, q_heads: int, kv_heads: int, seq_len: int, n_seqs: int, max_seqlen: int, last: int) -> int:
+    """Device workspace of a call of these sizes (``fd_paged_key_weights_workspace_bytes``)."""
+    nbytes = _cache_lib.lib().fd_paged_key_weights_workspace_bytes(batch, q_heads, kv_heads, seq_len, n_seqs, max_seqlen, last)
+    _cache_lib.check("fd_paged_key_weights_workspace_bytes", nbytes)
+    return nbytes
+
+
+def check_weights(name, weights, heads, width, device) -> None:
+    if (weights.ndim != 3 or weights.dtype != torch.float32 or weights.get_device() != device or weights.shape[1] != heads
+            or weights.shape[2] < width or weights.stride(2) != 1):
+        raise ValueError(f"{name} must be FP32 [rows, {heads}, at least {width}] on the cache's device, its keys contiguous")
+
+
+def check_row_indices(row_indices, requests, rows, device) -> int | None:
+    if row_indices is None:
+        if rows < requests:
+            raise ValueError(f"Without row_indices the weights need a row for each of the {requests} requests")
+        return None
+    if (row_indices.shape != (requests,) or row_indices.dtype != torch.int32 or row_indices.get_device() != device
+            or not row_indices.is_contiguous()):
+        raise ValueError(f"row_indices must be a contiguous int32 vector [{requests}] on the cache's device")
+    return row_indices.data_ptr()
+
+
+def paged_key_weights(
+    q: torch.Tensor,
+    k_cache: torch.Tensor,
+    page_table: torch.Tensor,
+    cache_lens: torch.Tensor,
+    weights: torch.Tensor,
+    *,
+    k_scale: torch.Tensor | None = None,
+    scale: float | None = None,
+    cu_seqlens: torch.Tensor | None = None,
+    max_seqlen: int | None = None,
+    last: int | None = None,
+    row_indices: torch.Tensor | None = None,
+) -> None:
+    shape = q.shape
+    if len(shape) != 4:
+        raise ValueError("Q must be four-dimensional")
+    batch, q_heads, seq_len, dim = shape
+    if min(batch, q_heads, seq_len) < 1:
+        raise ValueError("Batch, head counts and sequence length must be positive")
+    if k_cache.ndim != 4:
+        raise ValueError("k_cache must be [n_pages, Hkv, page_size, D]")
+    _, kv_heads, page_size, _ = k_cache.shape
+    if kv_heads < 1 or q_heads % kv_heads or dim != cache_dim(k_cache):
+        raise ValueError("Q must have the cache's head dimension and a multiple of its heads")
+    if q_heads // kv_heads > 2048:
+        raise ValueError("at most 2048 query heads per key head")
+    if batch * seq_len * q_heads >= 1 << 30:
+        raise ValueError("B * T * Hq must be below 2^30")
+    if scale is None:
+        scale = dim ** -0.5
+    elif not 0.0 < scale < 1e30:
+        raise ValueError("scale must be positive")
+    if cache_lens is None:
+        raise ValueError("cache_lens is required")
+    if last is not None and not 1 <= int(last) < 1 << 31:
+        raise ValueError("last must be a positive number of tokens")
+    device = k_cache.get_device()
+    cu_ptr, n_seqs = check_cu_seqlens(cu_seqlens, batch, device)
+    if max_seqlen is None or n_seqs == 0:
+        max_seqlen = seq_len
+    elif not 0 <= int(max_seqlen) <= seq_len:
+        raise ValueError("max_seqlen must lie in [0, T]")
+    requests = n_seqs or batch
+    cache = check_cache(k_cache, k_cache, page_table, cache_lens, k_scale, k_scale, requests)
+    check_weights("weights", weights, kv_heads, page_table.shape[1] * page_size, device)
+    index = check_row_indices(row_indices, requests, weights.shape[0], device)
+    q_ptr, q_strides = check_rows("Q", q, shape, device)
+    if _cache_lib.current_device() != device:
+        with torch.cuda.device(device):
+            return paged_key_weights(q, k_cache, page_table, cache_lens, weights, k_scale=k_scale, scale=scale,
+                                     cu_seqlens=cu_seqlens, max_seqlen=max_seqlen, last=last, row_indices=row_indices)
+    sizes = (batch, q_heads, kv_heads, seq_len, n_seqs, int(max_seqlen), int(last or 0))
+    nbytes = workspace_bytes(*sizes)
+    work = torch.empty(nbytes, device=q.device, dtype=torch.uint8)
+    _cache_lib.check("fd_paged_key_weights", _cache_lib.lib().fd_paged_key_weights(
+        q_ptr, cache, weights.data_ptr(), q_strides, _cache_lib.pack2(*weights.stride()[:2]), weights.shape[0], index, batch,
+        q_heads, seq_len, float(scale), int(last or 0), cu_ptr, n_seqs, int(max_seqlen), work.data_ptr(), nbytes,
+        _cache_lib.raw_stream(device)))

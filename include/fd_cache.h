@@ -5,6 +5,7 @@
  *   fd_paged_kv_write     keys and values of new tokens into a paged cache (bf16, or e4m3 quantised on the way)
  *   fd_paged_kv_read      the pages back as dense bf16 keys and values
  *   fd_paged_gqa_fwd      causal grouped-query attention of the new tokens over the paged cache
+ *   fd_paged_key_weights  the attention weight that every cached key draws from the new tokens
  *   fd_gated_delta_step   the gated delta rule token by token, from and into its fp32 state
  *   fd_packed_conv_state  the packed causal conv + activation continued from its state
  *
@@ -142,6 +143,30 @@ FD_API int fd_paged_gqa_fwd(const void* q, const fd_paged_cache* cache, const vo
 /* Workspace of fd_paged_gqa_fwd for these sizes, or a negative FD_ERR_* code. */
 FD_API int64_t fd_paged_gqa_workspace_bytes(int batch, int q_heads, int kv_heads, int seq_len, int head_dim,
                                             int page_size, int max_pages, int n_seqs, int max_seqlen);
+
+/*
+ * The attention weight that cached keys draw from new tokens, added to what they have drawn:
+ *   weights[row(r)][h][j] += sum of softmax(scale q K^T)[.., j] over the new tokens of request r and the query heads of
+ * key head h, for the keys j that the tokens see (as in fd_paged_gqa_fwd: causal, on a page; v of the cache is not read
+ * and may be k).  fp32 throughout, in an order that the sizes fix.
+ *
+ *   q       as in fd_paged_gqa_fwd
+ *   weights [weight_rows, kv_heads, >= max_pages * page_size] fp32, strides {row, head} in elements, keys contiguous
+ *   row_indices  device int32[requests]: request r's row of weights; NULL: row r.  An index outside [0, weight_rows), or
+ *           one that an earlier request of the call names already, is no row: nothing is added for that request
+ *   last    the last `last` new tokens of each request count; 0: all of them
+ *   cu_seqlens, n_seqs, max_seqlen  as in fd_paged_gqa_fwd
+ *   workspace  fd_paged_key_weights_workspace_bytes(...) bytes, 16-byte aligned; calls that may overlap need their own
+ * Keys that no token sees keep their weight; a key that is NaN makes the weights of a row's keys NaN, as a softmax does.
+ */
+FD_API int fd_paged_key_weights(const void* q, const fd_paged_cache* cache, float* weights, const int64_t q_strides[4],
+                                const int64_t weight_strides[2], int weight_rows, const int32_t* row_indices, int batch,
+                                int q_heads, int seq_len, float scale, int last, const int32_t* cu_seqlens, int n_seqs,
+                                int max_seqlen, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Workspace of fd_paged_key_weights for these sizes, or a negative FD_ERR_* code. */
+FD_API int64_t fd_paged_key_weights_workspace_bytes(int batch, int q_heads, int kv_heads, int seq_len, int n_seqs,
+                                                    int max_seqlen, int last);
 
 /*
  * The gated delta rule of the Gated-DeltaNet layers token by token (transformers'

@@ -1,0 +1,140 @@
+"""Attention weight per cached key on the GPU against its definition in float64."""
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from cache_reference import make_pages, rows
+from e2m1_reference import make_pages4, rows4
+from helpers import announce
+from test_paged_cache_gpu import ints, make_q, starts
+
+pytestmark = pytest.mark.gpu
+
+FORMATS = ["bf16", "e4m3", "e2m1"]
+# fp32 throughout.  Per probability, relative: a score's sum of up to 256 exact products in fp32 (256 half steps of
+# sum |q k|, up to 60 in log2 units here: the absolute error of the exponent, times ln 2), the exponent's own rounding
+# (two, of up to 60), exp2 and the division (a few half steps); then sums of up to 2^14 positive numbers in tiles
+# of 16 to 32 and the tiles in turn.  Sums of roundings in their worst case would be larger; what is added is random
+# in sign, so a few standard deviations are taken: 2^-24 * (60 * sqrt(256) + 2 * 60 + sqrt(2^14)) < 2^-24 * 1300.
+RELATIVE = 2.0 ** -24 * 1300
+
+
+def make(held, lens, page, heads, dim, seed):
+    if held == "e2m1":
+        return make_pages4(lens, page, heads, dim, seed), rows4
+    return make_pages(lens, page, heads, dim, held == "e4m3", seed), rows
+
+
+def want_weights(c, get, q, w, lens, new, index, last=None, packed=True, scale=None):
+    """float64 sums on top of w [rows, heads, width]."""
+    w = w.double().clone()
+    scale = q.shape[-1] ** -0.5 if scale is None else scale
+    at = starts(new)
+    for r, n in enumerate(new):
+        length = lens[r]
+        if not 0 <= index[r] < w.shape[0] or index[r] in index[:r] or n == 0 or length == 0:
+            continue
+        x = (q[0, :, at[r]:at[r + 1]] if packed else q[r]).double()
+        k, there = get(c, "k", r, length)
+        group = x.shape[0] // k.shape[0]
+        pos = length - n + torch.arange(n, device="cuda")
+        seen = (torch.arange(length, device="cuda") <= pos[:, None]) & there
+        for h in range(x.shape[0]):
+            s = torch.where(seen, (x[h] @ k[h // group].T) * scale, -math.inf)
+            top = s.amax(-1, keepdim=True)
+            p = torch.where(seen, torch.exp(s - torch.where(top == -math.inf, 0.0, top)), 0.0)
+            total = p.sum(-1, keepdim=True)
+            p = torch.where(total > 0, p / total, 0.0)
+            w[index[r], h // group, :length] += p[max(0, n - (last or n)):].sum(0)
+    return w
+
+
+def check(held, new, cached, hq, hkv, dim, page, seed, *, packed=True, last=None, index=None, absent=(), max_seqlen=None,
+          scale=None):
+    from fastdecisions_amd.paged_evict_kernel import paged_key_weights
+    lens = [a + b for a, b in zip(cached, new)]
+    c, get = make(held, lens, page, hkv, dim, seed)
+    for r, at in absent:
+        c["table"][r, at] = -1
+    q = make_q(new, hq, dim, seed + 1, packed=packed)
+    width = c["table"].shape[1] * page
+    gen = torch.Generator(device="cuda").manual_seed(seed + 2)
+    w = torch.rand((len(new) + 2, hkv, width + 5), generator=gen, device="cuda") * 1e-3
+    index = list(range(len(new))) if index is None else index
+    want = want_weights(c, get, q, w, lens, new, index, last, packed, scale)
+    kw = dict(cu_seqlens=ints(starts(new)), max_seqlen=max(new) if max_seqlen is None else max_seqlen) if packed else {}
+    got = w.clone()
+    paged_key_weights(q, c["k"], c["table"], ints(lens), got, k_scale=c["ks"], last=last, row_indices=ints(index), scale=scale, **kw)
+    again = w.clone()
+    paged_key_weights(q, c["k"], c["table"], ints(lens), again, k_scale=c["ks"], last=last, row_indices=ints(index), scale=scale, **kw)
+    assert torch.equal(got, again)          # nothing is added in an order of its own
+    same = want == w.double()
+    assert torch.equal(got[same], w[same])  # what no token sees keeps its weight
+    off = ((got.double() - want).abs() / want).max().item()
+    assert off <= RELATIVE, f"off by {off:.3g} relative"
+
+
+@pytest.mark.parametrize("held", FORMATS)
+@pytest.mark.parametrize("hq,hkv,dim,page", [(16, 4, 128, 16), (8, 2, 256, 64), (16, 4, 64, 256), (3, 3, 128, 16),
+                                             (40, 1, 64, 32)])
+def test_single_tokens(hq, hkv, dim, page, held):
+    lens = [1, 2, 31, 32, 33, 127, 128, 129, 255, 257, 1000, 2049, 0, 4111]
+    announce(f"key weights, single tokens {hq}/{hkv} x {dim}, page {page}, {held}")
+    check(held, [1] * len(lens), [n - 1 for n in lens], hq, hkv, dim, page, dim + page, packed=False)
+
+
+@pytest.mark.parametrize("held", FORMATS)
+@pytest.mark.parametrize("last", [None, 1, 33])
+@pytest.mark.parametrize("hq,hkv,dim,page", [(16, 4, 128, 16), (8, 2, 256, 32), (6, 1, 64, 128), (5, 5, 128, 16)])
+def test_packed_suffixes(hq, hkv, dim, page, last, held):
+    announce(f"key weights, packed suffixes {hq}/{hkv} x {dim}, page {page}, last {last}, {held}")
+    check(held, [40, 1, 0, 7, 133, 300, 64], [500, 1000, 77, 0, 1, 2500, 64], hq, hkv, dim, page, dim, last=last)
+
+
+@pytest.mark.parametrize("rows", [1, 300])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_either_kernel_takes_any_lengths(dim, rows):
+    announce(f"key weights x {dim}, the kernels for {rows} tokens")
+    check("bf16", [300, 1, 30, 70], [700, 900, 0, 60], 4, 2, dim, 16, 5, max_seqlen=rows)
+
+
+@pytest.mark.parametrize("new", [[3100], [1333, 1400, 1500]])
+def test_prompts(new):
+    announce(f"key weights, prompts {new}")
+    check("e4m3", new, [0] * len(new), 16, 4, 128, 64, 26)
+
+
+@pytest.mark.parametrize("n", [1, 40])
+def test_many_requests(n):
+    announce(f"key weights, 150 requests of {n}")
+    check("e2m1", [n] * 150, [(i * 37) % 300 for i in range(149)] + [6000], 8, 2, 64, 16, 6, packed=False)
+
+
+@pytest.mark.parametrize("n", [1, 50])
+def test_absent_pages(n):
+    announce(f"key weights, absent pages, {n} new")
+    check("bf16", [n] * 3, [300, 500, 16], 8, 2, 128, 16, 7, packed=False, absent=[(0, 2), (0, 3), (1, 0), (2, 0), (2, 1)])
+
+
+@pytest.mark.parametrize("n", [1, 50])
+def test_rows_of_the_pool(n):
+    """Rows in any order; one named twice is the first request's, one outside the pool nobody's."""
+    announce(f"key weights, row indices, {n} new")
+    check("e2m1", [n] * 5, [100, 200, 30, 4, 77], 8, 2, 64, 16, 8, packed=False, index=[4, 2, 4, -1, 7])
+
+
+def test_far_scores():
+    """Scores of some hundreds: probabilities that are one or nothing."""
+    announce("key weights, scale 4")
+    from fastdecisions_amd.paged_evict_kernel import paged_key_weights
+    c, get = make("bf16", [900], 16, 2, 64, 9)
+    q = make_q([20], 8, 64, 10)
+    w = torch.zeros((1, 2, c["table"].shape[1] * 16), device="cuda")
+    want = want_weights(c, get, q, w, [900], [20], [0], scale=4.0)
+    paged_key_weights(q, c["k"], c["table"], ints([900]), w, cu_seqlens=ints([0, 20]), scale=4.0)
+    # scores up to about 400: the exponent is off by up to 2^-24 * 400 * (sqrt(64) + 2)
+    assert ((w.double() - want).abs() <= 2.0 ** -24 * 4000 * want + 1e-30).all()
+    assert torch.isfinite(w).all() and abs(w.sum().item() - 20 * 8) < 0.01
