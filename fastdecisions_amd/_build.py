@@ -25,7 +25,7 @@ OFFLOAD_ARCH = "gfx950"
 
 SOURCES = ["fd_abi.cpp", "add_rmsnorm.hip", "packed_conv.hip", "gqa_fwd.hip", "gated_delta.hip", "gate_transform.hip", "attn_prologue.hip", "slot_readout.hip", "gated_norm.hip", "hbm_copy.hip"]
 
-CACHE_SOURCES = ["cache_abi.cpp", "paged_kv.hip", "paged_gqa.hip", "paged_weights.hip", "delta_step.hip", "conv_state.hip"]
+CACHE_SOURCES = ["cache_abi.cpp", "paged_kv.hip", "paged_gqa.hip", "paged_weights.hip", "paged_evict.hip", "delta_step.hip", "conv_state.hip"]
 
 # MFMA accumulators in ordinary registers: without it the compiler puts them all in the accumulation half of the
 # register file and copies scores over for every softmax.  (At 128 features, where eight wavefronts leave 256 registers

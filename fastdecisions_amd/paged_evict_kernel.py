@@ -1,4 +1,5 @@
-"""Which cached keys matter, on the gfx950 HIP kernel ``fd_paged_key_weights``.
+"""Which cached keys matter, and a cache without the others, on the gfx950 HIP kernels ``fd_paged_key_weights`` and
+``fd_paged_kv_evict``.
 
 ``paged_key_weights`` adds to each cached key the attention weight that a call's new tokens give it:
 the sum over the tokens and over the query heads of a key head of their softmax probabilities, in
@@ -9,6 +10,19 @@ fp32.  It takes what ``paged_gqa_attention`` takes, after ``paged_kv_write`` of 
   row r).  It belongs to a request, not to a page: requests that share pages weigh them apart.  An
   index outside the rows, or named by an earlier request of the call, adds nothing;
 * ``last`` — only the last ``last`` new tokens of each request count (default: all).
+
+``paged_kv_evict`` cuts every request to at most ``keep`` keys: its ``recent`` last ones and, per key
+head, those of largest weight among the others (of equal weights the lowest; NaN below everything).
+Their rows and scales move, in their order, to the pages of ``new_table`` (int32 ``[requests, n]``,
+``n * page_size >= keep``), which must be none of those that hold the call's requests; the old pages are
+left as they were.  A request of no more than ``keep`` keys moves whole.  Keys are rotated by their
+positions before they are cached, so a request goes on where it stood: its next tokens' positions count
+all the tokens that it has seen, ``cache_lens`` those that it holds.
+
+* returns ``(kept, new_lens)``: int32 ``[requests, Hkv, keep]``, the old place of every kept key (-1
+  behind the last), and int32 ``[requests]``, ``min(cache_lens, keep)``;
+* ``weights_out`` (default ``weights`` itself) — the kept keys' weights in the first places of their rows,
+  zeros from there to ``cache_lens``.
 
 The cache's layout is described in ``paged_kv_kernel``.
 """
@@ -106,3 +120,60 @@ def paged_key_weights(
         q_ptr, cache, weights.data_ptr(), q_strides, _cache_lib.pack2(*weights.stride()[:2]), weights.shape[0], index, batch,
         q_heads, seq_len, float(scale), int(last or 0), cu_ptr, n_seqs, int(max_seqlen), work.data_ptr(), nbytes,
         _cache_lib.raw_stream(device)))
+
+
+def paged_kv_evict(
+    k_cache: torch.Tensor,
+    v_cache: torch.Tensor,
+    page_table: torch.Tensor,
+    cache_lens: torch.Tensor,
+    weights: torch.Tensor,
+    new_table: torch.Tensor,
+    keep: int,
+    *,
+    recent: int = 0,
+    k_scale: torch.Tensor | None = None,
+    v_scale: torch.Tensor | None = None,
+    weights_out: torch.Tensor | None = None,
+    row_indices: torch.Tensor | None = None,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    if k_cache.ndim != 4:
+        raise ValueError("k_cache and v_cache must be [n_pages, Hkv, page_size, D] of one shape")
+    if page_table.ndim != 2 or page_table.shape[0] < 1:
+        raise ValueError("page_table must be int32 [requests, max_pages], of one request or more")
+    if cache_lens is None:
+        raise ValueError("cache_lens is required")
+    keep, recent = int(keep), int(recent)
+    if not 1 <= keep < 1 << 27 or not 0 <= recent <= keep:
+        raise ValueError("keep must be positive and recent in [0, keep]")
+    requests, max_pages = page_table.shape
+    _, heads, page_size, _ = k_cache.shape
+    device = k_cache.get_device()
+    cache = check_cache(k_cache, v_cache, page_table, cache_lens, k_scale, v_scale, requests)
+    check_weights("weights", weights, heads, max_pages * page_size, device)
+    if weights_out is None:
+        weights_out = weights
+    elif weights_out is not weights:
+        check_weights("weights_out", weights_out, heads, max_pages * page_size, device)
+        if weights_out.shape != weights.shape or weights_out.stride() != weights.stride():
+            raise ValueError("weights and weights_out must have one shape and the same strides")
+        gap = abs(weights.data_ptr() - weights_out.data_ptr()) // 4
+        if 0 < gap <= sum((n - 1) * s for n, s in zip(weights.shape, weights.stride())):
+            raise ValueError("weights and weights_out must be the same memory or not overlap")
+    if (new_table.ndim != 2 or new_table.shape[0] != requests or new_table.dtype != torch.int32
+            or new_table.get_device() != device or new_table.stride(1) != 1 or new_table.shape[1] * page_size < keep):
+        raise ValueError(f"new_table must be int32 [{requests}, n] on the cache's device, its rows contiguous, and hold {keep} keys")
+    if requests * heads * keep >= 1 << 31:
+        raise ValueError("requests * Hkv * keep must be below 2^31")
+    index = check_row_indices(row_indices, requests, weights.shape[0], device)
+    if _cache_lib.current_device() != device:
+        with torch.cuda.device(device):
+            return paged_kv_evict(k_cache, v_cache, page_table, cache_lens, weights, new_table, keep, recent=recent,
+                                  k_scale=k_scale, v_scale=v_scale, weights_out=weights_out, row_indices=row_indices)
+    kept = torch.empty((requests, heads, keep), device=k_cache.device, dtype=torch.int32)
+    new_lens = torch.empty(requests, device=k_cache.device, dtype=torch.int32)
+    _cache_lib.check("fd_paged_kv_evict", _cache_lib.lib().fd_paged_kv_evict(
+        cache, weights.data_ptr(), weights_out.data_ptr(), _cache_lib.pack2(*weights.stride()[:2]), weights.shape[0], index,
+        new_table.data_ptr(), new_table.stride(0), new_table.shape[1], requests, keep, recent, kept.data_ptr(),
+        new_lens.data_ptr(), _cache_lib.raw_stream(device)))
+    return kept, new_lens

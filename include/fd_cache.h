@@ -6,6 +6,7 @@
  *   fd_paged_kv_read      the pages back as dense bf16 keys and values
  *   fd_paged_gqa_fwd      causal grouped-query attention of the new tokens over the paged cache
  *   fd_paged_key_weights  the attention weight that every cached key draws from the new tokens
+ *   fd_paged_kv_evict     the keys of largest weight and the most recent ones, moved to pages of their own
  *   fd_gated_delta_step   the gated delta rule token by token, from and into its fp32 state
  *   fd_packed_conv_state  the packed causal conv + activation continued from its state
  *
@@ -167,6 +168,27 @@ FD_API int fd_paged_key_weights(const void* q, const fd_paged_cache* cache, floa
 /* Workspace of fd_paged_key_weights for these sizes, or a negative FD_ERR_* code. */
 FD_API int64_t fd_paged_key_weights_workspace_bytes(int batch, int q_heads, int kv_heads, int seq_len, int n_seqs,
                                                     int max_seqlen, int last);
+
+/*
+ * Cuts every request to at most `keep` keys: its `recent` last ones and, per key head, those of largest weight among the
+ * others (of equal weights the lowest key; NaN below everything).  The kept keys' rows and scales move in their order to
+ * the pages of new_table, their weights to the front of their row.
+ *
+ *   weights, weights_out  [weight_rows, kv_heads, >= max_pages * page_size] fp32 of the same strides {row, head}, keys
+ *           contiguous; the same memory, or without overlap.  weights_out[..][0 .. n - 1] are the kept keys' weights,
+ *           n = min(cache_lens, keep), and [n, cache_lens) are 0
+ *   row_indices  as in fd_paged_key_weights; a request without a row counts as one of equal weights
+ *   new_table  [requests, new_max_pages] int32, rows new_table_stride apart, new_max_pages * page_size >= keep.  Its
+ *           pages must not be among those that the call's page table names for keys of any request.  Entries outside
+ *           [0, n_pages) are no pages: their keys are not written.  Kept keys on no page become zeros
+ *   kept    [requests, kv_heads, keep] int32, contiguous: the old place of every kept key, -1 behind the last one
+ *   new_lens  [requests] int32: min(cache_lens, keep)
+ * The old pages are left as they were.
+ */
+FD_API int fd_paged_kv_evict(const fd_paged_cache* cache, const float* weights, float* weights_out,
+                             const int64_t weight_strides[2], int weight_rows, const int32_t* row_indices,
+                             const int32_t* new_table, int64_t new_table_stride, int new_max_pages, int requests,
+                             int keep, int recent, int32_t* kept, int32_t* new_lens, void* stream);
 
 /*
  * The gated delta rule of the Gated-DeltaNet layers token by token (transformers'
