@@ -1,19 +1,8 @@
-// Tile conventions shared by the attention kernels: operand types, the key
-// permutation and chunk swizzles of the LDS tiles, lane-half reductions and the
-// copy to LDS.
+// Tile conventions shared by the attention kernels: the key
+// permutation and chunk swizzles of the LDS tiles and the copy to LDS.
 #pragma once
 
-#include "fd_common.h"
-
-typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
-typedef float f32x16_t __attribute__((ext_vector_type(16)));
-typedef float f32x8_t __attribute__((ext_vector_type(8)));
-typedef float f32x4_t __attribute__((ext_vector_type(4)));
-typedef __bf16 bf16x4_t __attribute__((ext_vector_type(4)));
-
-typedef __attribute__((address_space(3))) void lds_void_t;
-typedef short v4i16_t __attribute__((ext_vector_type(4)));
-typedef __attribute__((address_space(3))) v4i16_t lds_v4i16_t;
+#include "mfma_types.h"
 
 namespace {
 
@@ -38,19 +27,6 @@ __device__ __forceinline__ int swz_v(int row) {
   // 16+ chunks per row: xor with 4*(row & 3) puts the 4 rows x 4 chunks that
   // 32 lanes of a transposing read touch on 16 distinct chunks (all banks).
   return CR >= 16 ? 4 * (row & 3) : (2 * (row & 3)) & (CR - 1);
-}
-
-// Max / sum of a value over lanes l and l^32 (the two lane halves hold the two
-// 16-key halves of one query's scores).  v_permlane32_swap with the value in
-// both operands leaves this lane's value in one result and its partner's in
-// the other, so max and sum of the pair need no lane-index select.
-__device__ __forceinline__ float half_max(float v) {
-  auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
-}
-__device__ __forceinline__ float half_sum(float v) {
-  auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
 // Copies 16 bytes per lane from `base` (uniform) + `off` to 1 KiB of LDS at

@@ -619,6 +619,7 @@ __global__ __launch_bounds__(S::kThreads, S::kPerCu) void paged_gqa_few_kernel(P
     for (int db = 0; db < kNdb; ++db) o[n][db] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
   }
   bf16x8_t pb[NR], pl[NR];  // probabilities, in two parts
+  uint32_t v_scales[D == 256 ? 2 : 1];  // E2M1: of V's row lane / 2, read before the next K's scales take their place
 
   auto scores = [&](int j) {
     const unsigned char* const st = stage0 + (j & (NS - 1)) * S::kStageBytes;
@@ -661,6 +662,11 @@ __global__ __launch_bounds__(S::kThreads, S::kPerCu) void paged_gqa_few_kernel(P
 #pragma unroll
         for (int n = 0; n < NR; ++n) s[n][h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[n][kk], s[n][h], 0, 0, 0);
       }
+    }
+    if constexpr (FP4) {
+#pragma unroll
+      for (int c = 0; c < (D == 256 ? 2 : 1); ++c)
+        v_scales[c] = reinterpret_cast<const uint32_t*>(st + 2 * S::kBlockBytes + (D == 256 ? 256 : 128))[(lane >> 1) * (D == 256 ? 2 : 1) + c];
     }
     float ks[8], vs[8];
     if constexpr (FP8) {
@@ -793,7 +799,6 @@ __global__ __launch_bounds__(S::kThreads, S::kPerCu) void paged_gqa_few_kernel(P
   // where the transposing reads take them; their features' products follow.
   auto p_v_codes = [&](int j) {
     const unsigned char* const st = stage0 + (j & (NS - 1)) * S::kStageBytes + S::kBlockBytes;
-    const uint8_t* const sc = st + S::kBlockBytes + (D == 256 ? 256 : 128);
     unsigned char* const bf = smem + S::kWaves * NS * S::kStageBytes + wave * S::kDecoded;
     const bool masked = first + j * S::kKeys + 31 > pos_min || absent;
     const int row = lane >> 1, half = lane & 1;
@@ -801,7 +806,7 @@ __global__ __launch_bounds__(S::kThreads, S::kPerCu) void paged_gqa_few_kernel(P
 #pragma unroll
     for (int c = 0; c < D / kScaleBlock; ++c) {
       const uint2 w = *reinterpret_cast<const uint2*>(st + row * RBY + (c ^ few_swz_v<RBY, kE2m1>(row)) * 16 + 8 * half);
-      const float scale = scale_of(sc[row * (D == 64 ? 4 : D / kScaleBlock) + c]);
+      const float scale = scale_of(v_scales[c / 4] >> (8 * (c % 4)) & 255u);
       *reinterpret_cast<bf16x8_t*>(bf + row * 64 + chunk_of(row, 2 * half) * 16) = e2m1_to_bf16(w.x, scale);
       *reinterpret_cast<bf16x8_t*>(bf + row * 64 + chunk_of(row, 2 * half + 1) * 16) = e2m1_to_bf16(w.y, scale);
       bf16x8_t vf[2];  // V[key 8 grp + i][32 c + 16 u + li]

@@ -13,7 +13,7 @@
 #include <algorithm>
 #include <type_traits>
 
-#include "gqa_tile.h"
+#include "mfma_types.h"
 #include "paged_common.h"
 #include "state_slot.h"
 #include "wave_tools.h"

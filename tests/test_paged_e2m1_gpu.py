@@ -89,6 +89,17 @@ def test_many_requests(n):
     check(c, q, run_attention(c, q, lens, [n] * 150, packed=False), lens, [n] * 150, packed=False)
 
 
+@pytest.mark.parametrize("n", [1, 9])
+@pytest.mark.parametrize("hq,hkv,dim", [(16, 4, 64), (16, 4, 128), (8, 2, 256)])
+def test_long_caches(hq, hkv, dim, n):
+    """So many keys that a wavefront takes many blocks of them, each staged where an earlier one lay."""
+    lens = [4000 + 517 * i for i in range(16)] + [9] * 60 + [70000]
+    announce(f"4-bit attention, long caches, {n} new, {hq}/{hkv} x {dim}")
+    c = make_pages4(lens, 64, hkv, dim, seed=8)
+    q = make_q([n] * len(lens), hq, dim, 9, packed=False)
+    check(c, q, run_attention(c, q, lens, [n] * len(lens), packed=False), lens, [n] * len(lens), packed=False)
+
+
 @pytest.mark.parametrize("n", [1, 50])
 @pytest.mark.parametrize("dim", [64, 128, 256])
 def test_absent_pages_and_nan_behind_the_keys(dim, n):
