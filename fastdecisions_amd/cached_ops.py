@@ -1,7 +1,7 @@
 """Torch ops of the cache operators (``fastdecisions_cache::``): one node each under ``torch.compile``, capturable in a HIP graph.
 
 They wrap ``paged_kv_write``, ``paged_kv_read`` (``paged_kv_kernel``), ``paged_gqa_attention``
-(``paged_gqa_kernel``), ``prep_qkv_state`` (``packed_conv_kernel``) and
+(``paged_gqa_kernel``), ``paged_key_weights`` and ``paged_kv_evict`` (``paged_evict_kernel``), ``prep_qkv_state`` (``packed_conv_kernel``) and
 ``recurrent_gated_delta_rule`` (``gated_delta_kernel``) in the forms the cached layers call;
 caches and states are updated in place and declared so.  ``gated_delta_rule_states`` is the chunked
 rule (``chunk_gated_delta_rule``) from and to states that the caller gathers and scatters."""
@@ -13,6 +13,7 @@ import torch
 
 from .gated_delta_kernel import chunk_gated_delta_rule, recurrent_gated_delta_rule
 from .packed_conv_kernel import prep_qkv_state
+from .paged_evict_kernel import paged_key_weights, paged_kv_evict
 from .paged_gqa_kernel import paged_gqa_attention
 from .paged_kv_kernel import cache_dim, paged_kv_read, paged_kv_write
 
@@ -56,6 +57,37 @@ def paged_gqa_op(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, 
 def _paged_gqa_fake(q, k_cache, v_cache, page_table, cache_lens, k_scale, v_scale, gate, cu_seqlens, max_seqlen):
     b, h, t, d = q.shape
     return q.new_empty((b, t, h, d)).permute(0, 2, 1, 3)
+
+
+@torch.library.custom_op("fastdecisions_cache::paged_key_weights", mutates_args=("weights",), device_types="cuda")
+def paged_key_weights_op(q: torch.Tensor, k_cache: torch.Tensor, page_table: torch.Tensor, cache_lens: torch.Tensor,
+                         weights: torch.Tensor, k_scale: Optional[torch.Tensor], cu_seqlens: Optional[torch.Tensor],
+                         max_seqlen: int, last: Optional[int], row_indices: Optional[torch.Tensor]) -> None:
+    paged_key_weights(q, k_cache, page_table, cache_lens, weights, k_scale=k_scale, cu_seqlens=cu_seqlens,
+                      max_seqlen=max_seqlen, last=last, row_indices=row_indices)
+
+
+@paged_key_weights_op.register_fake
+def _paged_key_weights_fake(q, k_cache, page_table, cache_lens, weights, k_scale, cu_seqlens, max_seqlen, last, row_indices):
+    return None
+
+
+@torch.library.custom_op("fastdecisions_cache::paged_kv_evict",
+                         mutates_args=("k_cache", "v_cache", "weights", "k_scale", "v_scale"), device_types="cuda")
+def paged_kv_evict_op(k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor, cache_lens: torch.Tensor,
+                      weights: torch.Tensor, new_table: torch.Tensor, keep: int, recent: int, k_scale: Optional[torch.Tensor],
+                      v_scale: Optional[torch.Tensor],
+                      row_indices: Optional[torch.Tensor]) -> tuple[torch.Tensor, torch.Tensor]:
+    """The weights are moved in place."""
+    return paged_kv_evict(k_cache, v_cache, page_table, cache_lens, weights, new_table, keep, recent=recent, k_scale=k_scale,
+                          v_scale=v_scale, row_indices=row_indices)
+
+
+@paged_kv_evict_op.register_fake
+def _paged_kv_evict_fake(k_cache, v_cache, page_table, cache_lens, weights, new_table, keep, recent, k_scale, v_scale,
+                         row_indices):
+    requests = page_table.shape[0]
+    return (page_table.new_empty((requests, k_cache.shape[1], keep)), page_table.new_empty((requests,)))
 
 
 @torch.library.custom_op("fastdecisions_cache::packed_conv_state", mutates_args=("conv_state",), device_types="cuda")

@@ -4,8 +4,8 @@ The reference computes a shared prefix once and forks its cache per question (ke
 conv state, recurrent state; ref: src/decider/shared_prefix.py:157-200).  ``DeciderCache`` holds
 the caches of up to ``requests`` requests of one model:
 
-* attention layers — a pool of pages of keys and values, bf16 or e4m3 with a power-of-two scale
-  per token and head (``paged_kv_kernel``); a request holds pages, not a range, so a fork shares
+* attention layers — a pool of pages of keys and values, bf16, e4m3 with a power-of-two scale
+  per token and head, or 4-bit with one per 32 features (``paged_kv_kernel``); a request holds pages, not a range, so a fork shares
   its parent's whole pages and copies the last, partly filled one;
 * Gated-DeltaNet layers — the conv's last inputs and the fp32 state of the delta rule, a row of a
   pool per request.
@@ -24,11 +24,17 @@ take it back with ``CacheStep.cancel``: the rows of a step that is never run are
 held before.  A forward that refuses its step leaves it waiting, and its requests take no other step
 and no fork before it is run or cancelled; one that fails on the way leaves requests whose layers
 hold different tokens, which can only be closed.
+With ``key_weights=True`` the attention layers also sum the attention weight that each cached key has drawn
+(``paged_evict_kernel``; of every step's tokens, or of its ``observe`` last ones per request), and ``evict`` cuts
+requests to the keys that drew most and the most recent ones: a prefix of thousands of tokens, cut once, is
+forked as before.  A request's next tokens have the positions behind all the tokens that it has seen
+(``position``), however few it holds (``length``).
+
 ``CacheStep.again`` makes the next step of the same shape in the same device tensors, so a
 captured forward over a step can be replayed token after token.
 
 Streams: a cache's calls change its tensors (``open`` clears states, ``fork`` copies pages and states,
-``step`` and ``again`` write the step's tensors) and its host records at once: ``close`` gives pages and
+``evict`` moves keys, ``step`` and ``again`` write the step's tensors) and its host records at once: ``close`` and ``evict`` give pages and
 states to whoever opens next, also while a forward that reads them is still queued.  So make all calls,
 forwards and replays on one stream, or order the streams yourself: the stream of a later call waits
 (``Stream.wait_stream``) for the one of every forward and replay before it, over any request, and
@@ -42,6 +48,7 @@ from dataclasses import dataclass, field
 import torch
 
 from .model import DeciderShape
+from .paged_kv_kernel import SCALE_BLOCK
 
 
 @dataclass(eq=False)
@@ -110,7 +117,7 @@ class CacheStep:
         """Refuse a step whose requests are not those it was made for: its pages may be another request's by now."""
         for slot, pages in zip(self.slots, self.held):
             if self.cache._pages.get(slot) is not pages:
-                raise ValueError(f"Request {slot} of the step was closed")
+                raise ValueError(f"Request {slot} of the step was closed, or keys of it were evicted")
 
     # ---- what a forward over the step tells it
 
@@ -162,16 +169,22 @@ class CacheStep:
 
 class DeciderCache:
     def __init__(self, shape: DeciderShape, *, requests: int, tokens: int, max_tokens: int | None = None,
-                 page_size: int = 64, kv_dtype: torch.dtype = torch.bfloat16, device="cuda"):
+                 page_size: int = 64, kv_dtype: torch.dtype = torch.bfloat16, key_weights: bool = False,
+                 observe: int | None = None, device="cuda"):
         """``tokens``: cached tokens of all requests together (rounded up to pages, plus one partly filled
         page per request); ``max_tokens``: of one request (default ``tokens``), the width of the page tables.  A
-        step writes its requests' tables whole: 64 of 3125 pages cost it 5.2 ms of host time, of 128 pages 0.33 ms."""
+        step writes its requests' tables whole: 64 of 3125 pages cost it 5.2 ms of host time, of 128 pages 0.33 ms.
+        ``key_weights``: sum the attention weight of every cached key, for ``evict`` (4 bytes per attention layer,
+        request, head and token of ``max_tokens``); ``observe``: of the last ``observe`` tokens of a step's requests
+        (default: all)."""
         if requests < 1 or tokens < 1:
             raise ValueError("requests and tokens must be positive")
         if page_size not in (16, 32, 64, 128, 256):
             raise ValueError("page_size must be a power of two in [16, 256]")
-        if kv_dtype not in (torch.bfloat16, torch.float8_e4m3fn):
-            raise ValueError("kv_dtype must be bfloat16 or float8_e4m3fn")
+        if kv_dtype not in (torch.bfloat16, torch.float8_e4m3fn, torch.float4_e2m1fn_x2):
+            raise ValueError("kv_dtype must be bfloat16, float8_e4m3fn or float4_e2m1fn_x2")
+        if observe is not None and (observe < 1 or not key_weights):
+            raise ValueError("observe must be positive and needs key_weights")
         max_tokens = tokens if max_tokens is None else max_tokens
         self.shape, self.page_size, self.kv_dtype, self.device = shape, page_size, kv_dtype, torch.device(device)
         self.requests = requests
@@ -183,13 +196,21 @@ class DeciderCache:
         self._attention = {layer: i for i, layer in enumerate(attention)}
         self._linear = {layer: i for i, layer in enumerate(linear)}
         kv = (len(attention), self.n_pages, shape.num_key_value_heads, page_size, shape.head_dim)
-        self.k = torch.zeros(kv, dtype=kv_dtype, device=self.device)
-        self.v = torch.zeros_like(self.k)
+        codes4 = kv_dtype == torch.float4_e2m1fn_x2  # two features a byte, a scale per 32 of them
+        pool = lambda: (torch.zeros((*kv[:4], kv[4] // 2), dtype=torch.uint8, device=self.device).view(kv_dtype) if codes4
+                        else torch.zeros(kv, dtype=kv_dtype, device=self.device))
+        self.k, self.v = pool(), pool()
         self.device = self.k.device                   # with its index: steps go there whatever device is current
         self.k_scale = self.v_scale = None
-        if kv_dtype == torch.float8_e4m3fn:
-            self.k_scale = torch.full(kv[:4], 127, dtype=torch.uint8, device=self.device)
+        if kv_dtype != torch.bfloat16:
+            scales = (*kv[:4], kv[4] // SCALE_BLOCK) if codes4 else kv[:4]
+            self.k_scale = torch.full(scales, 127, dtype=torch.uint8, device=self.device)
             self.v_scale = self.k_scale.clone()
+        self.observe = observe
+        self.weights = None
+        if key_weights:
+            self.weights = torch.zeros((len(attention), requests, shape.num_key_value_heads, self.max_pages * page_size),
+                                       dtype=torch.float32, device=self.device)
         heads, dim = shape.linear_num_heads, shape.linear_head_dim
         self.conv = torch.zeros((len(linear), requests, shape.conv_kernel - 1, 3 * heads * dim), dtype=torch.bfloat16,
                                 device=self.device)
@@ -198,7 +219,8 @@ class DeciderCache:
         self._free_pages = list(range(self.n_pages))[::-1]
         self._users = [0] * self.n_pages              # requests that hold a page
         self._pages: dict[int, list[int]] = {}        # of an open request
-        self._lens: dict[int, int] = {}
+        self._lens: dict[int, int] = {}               # keys it holds
+        self._seen: dict[int, int] = {}               # tokens it has seen: the position of its next one
         self._waiting: dict[int, list[CacheStep]] = {}  # the refused steps of an open request, in order
         self._lost: set[int] = set()                  # open requests that a failed forward left half computed
 
@@ -211,7 +233,9 @@ class DeciderCache:
         slot = self._free_slots.pop()
         self.conv[:, slot].zero_()
         self.delta[:, slot].zero_()
-        self._pages[slot], self._lens[slot] = [], 0
+        if self.weights is not None:
+            self.weights[:, slot].zero_()
+        self._pages[slot], self._lens[slot], self._seen[slot] = [], 0, 0
         return slot
 
     def fork(self, parent: int) -> int:
@@ -235,21 +259,72 @@ class DeciderCache:
             own = own + [page]
         self.conv[:, slot] = self.conv[:, parent]
         self.delta[:, slot] = self.delta[:, parent]
-        self._pages[slot], self._lens[slot] = list(own), n
+        if self.weights is not None:
+            self.weights[:, slot] = self.weights[:, parent]
+        self._pages[slot], self._lens[slot], self._seen[slot] = list(own), n, self._seen[parent]
         return slot
 
     def close(self, slot: int) -> None:
         """End a request; pages nobody else holds become free."""
         self._check_open([slot])
         self._give(self._pages.pop(slot))
-        del self._lens[slot]
+        del self._lens[slot], self._seen[slot]
         self._lost.discard(slot)
         self._waiting.pop(slot, None)
         self._free_slots.append(slot)
 
     def length(self, slot: int) -> int:
+        """Keys that a request holds."""
         self._check_open([slot])
         return self._lens[slot]
+
+    def position(self, slot: int) -> int:
+        """Tokens that a request has seen: the position of its next one."""
+        self._check_open([slot])
+        return self._seen[slot]
+
+    def evict(self, slots: list[int], keep: int, *, recent: int = 0) -> None:
+        """Cut requests to ``keep`` keys: in every attention layer and key head the ``recent`` last ones and of the others
+        those that drew most attention.  A request that holds no more stays as it is.  The kept keys move to free pages
+        (``keep`` tokens of each request, before the old ones become free; requests may be cut one by one); pages that
+        forks share stay theirs.  Steps made before are refused afterwards: run or cancel them first."""
+        from .cached_ops import paged_kv_evict_op
+        slots, keep, recent = list(slots), int(keep), int(recent)
+        if self.weights is None:
+            raise RuntimeError("The cache has no key weights: make it with key_weights=True")
+        if keep < 1 or not 0 <= recent <= keep:
+            raise ValueError("keep must be positive and recent in [0, keep]")
+        self._check(slots)
+        if len(set(slots)) != len(slots):
+            raise ValueError("A request appears once in an eviction")
+        cut = [slot for slot in slots if self._lens[slot] > keep]
+        if not cut:
+            return
+        need = -(-keep // self.page_size)
+        if need * len(cut) > len(self._free_pages):
+            raise RuntimeError(f"The cache has {len(self._free_pages)} free pages, the eviction needs {need * len(cut)}")
+        n = len(cut)
+        old = max(len(self._pages[slot]) for slot in cut)
+        tables = [self._pages[slot] + [-1] * (old - len(self._pages[slot])) for slot in cut]
+        new = [[self._take() for _ in range(need)] for _ in cut]
+        begun = False
+        try:
+            sizes = torch.tensor([*sum(tables, []), *sum(new, []), *(self._lens[slot] for slot in cut), *cut], dtype=torch.int32)
+            table, new_table, lens, rows = sizes.to(self.device).split([n * old, n * need, n, n])
+            for layer in self._attention:
+                k, v, k_scale, v_scale = self.attention_layer(layer)
+                begun = True
+                paged_kv_evict_op(k, v, table.view(n, old), lens, self.key_weights(layer), new_table.view(n, need), keep, recent,
+                                  k_scale, v_scale, rows)
+        except BaseException:
+            for pages in new:
+                self._give(pages)
+            if begun:  # some layers' weights have moved, others' have not
+                self._lost.update(cut)
+            raise
+        for slot, pages in zip(cut, new):
+            self._give(self._pages[slot])
+            self._pages[slot], self._lens[slot] = pages, keep
 
     # ---- steps
 
@@ -298,6 +373,7 @@ class DeciderCache:
         """Undo ``_reserve`` of the requests' last tokens."""
         for slot, n in zip(slots, new):
             self._lens[slot] -= n
+            self._seen[slot] -= n
             pages = -(-self._lens[slot] // self.page_size)
             self._give(self._pages[slot][pages:][::-1])
             del self._pages[slot][pages:]
@@ -317,13 +393,13 @@ class DeciderCache:
             raise RuntimeError(f"The cache has {len(self._free_pages)} free pages, the step needs {sum(need)}")
         cu, lens, table, pos = [0], [], [], []
         for slot, n, pages in zip(slots, new, need):
-            held = self._lens[slot]
+            held, seen = self._lens[slot], self._seen[slot]
             self._pages[slot] += [self._take() for _ in range(pages)]
-            self._lens[slot] = held + n
+            self._lens[slot], self._seen[slot] = held + n, seen + n
             cu.append(cu[-1] + n)
             lens.append(held + n)
             table += self._pages[slot] + [-1] * (self.max_pages - len(self._pages[slot]))
-            pos += range(held, held + n)
+            pos += range(seen, seen + n)
         return torch.tensor(cu + lens + list(slots) + table + pos, dtype=torch.int32)
 
     # ---- what the layers see
@@ -333,6 +409,11 @@ class DeciderCache:
         i = self._attention[layer]
         scales = (None, None) if self.k_scale is None else (self.k_scale[i], self.v_scale[i])
         return self.k[i], self.v[i], *scales
+
+    def key_weights(self, layer: int):
+        """Attention weight that an attention layer's cached keys have drawn, [requests, Hkv, max_tokens] (None without
+        ``key_weights``)."""
+        return None if self.weights is None else self.weights[self._attention[layer]]
 
     def linear_layer(self, layer: int):
         """(conv state pool, delta state pool) of a Gated-DeltaNet layer."""

@@ -119,7 +119,7 @@ def _fused_forward(self, hidden_states, position_embeddings, cu_seqlens, max_seq
 def _cached_forward(self, hidden_states, position_embeddings, step):
     """The attention layer over a paged cache: ``hidden_states`` [1, total, hidden] are the step's new tokens,
     whose keys and values are written before the attention reads everything their requests hold."""
-    from .cached_ops import paged_gqa_op, paged_kv_write_op
+    from .cached_ops import paged_gqa_op, paged_key_weights_op, paged_kv_write_op
     shape = hidden_states.shape[:-1]
     d = self.head_dim
     if hasattr(self, "_fd_qkv_weight"):
@@ -143,6 +143,10 @@ def _cached_forward(self, hidden_states, position_embeddings, step):
         q, k = (t.contiguous() for t in apply_rotary_pos_emb(q, k, *position_embeddings))
     k_cache, v_cache, k_scale, v_scale = step.cache.attention_layer(self.layer_idx)
     paged_kv_write_op(k, v, k_cache, v_cache, step.page_table, step.cache_lens, k_scale, v_scale, step.cu_seqlens)
+    weights = step.cache.key_weights(self.layer_idx)
+    if weights is not None:
+        paged_key_weights_op(q, k_cache, step.page_table, step.cache_lens, weights, k_scale, step.cu_seqlens, step.max_new,
+                             step.cache.observe, step.state_indices)
     out = paged_gqa_op(q, k_cache, v_cache, step.page_table, step.cache_lens, k_scale, v_scale,
                        qg[..., d:].transpose(1, 2), step.cu_seqlens, step.max_new)
     return self.o_proj(out.transpose(1, 2).reshape(*shape, -1)), None
