@@ -32,21 +32,32 @@ struct WeightArgs {
   float* w;
   int64_t w_row, w_head;
   int n_req, seq_len, group, kv_heads, last, w_rows;
-  int target;                   // items that the row stats are cut into, about
-  int part_items;
+  uint32_t group_magic;         // ceil(2^24 / group)
   float scale_log2;
+  int stats_items, sums_items;  // items that each kernel cuts its work into, about
+  int part_items;               // items of the row stats whose places the workspace holds
   float* part;                  // per item of the row stats: its rows' (m, l)
+  float* sums;                  // per item of the key sums of a request cut into row ranges: its keys' sums
 };
 
-// Row stats: RW row wavefronts of NB blocks of 32 rows, times 4 / RW key parts of a tile.
-template <int RW_, int NB_>
+// Row stats: RW row wavefronts of NB blocks of 32 rows, times 4 / RW key parts of a tile; a ring of kRing tiles.
+template <int D_, int RW_, int NB_>
 struct Stats {
-  static constexpr int RW = RW_, NB = NB_, KW = kWaves / RW;
+  static constexpr int D = D_, RW = RW_, NB = NB_, KW = kWaves / RW;
   static constexpr int kRows = 32 * RW * NB;
-  static constexpr int kKeys = KW == 1 ? 64 : 32 * KW;
+  static constexpr int kSubs = KW > 1 || D == 256 ? 1 : D == 128 ? 2 : 4;  // blocks of 32 keys of a wavefront and tile
+  static constexpr int kKeys = 32 * KW * kSubs;
+  static constexpr int kTileBytes = kKeys * D * 2;
+  static constexpr int kRing = kTileBytes >= 32768 ? 2 : 3;
 };
-using Few = Stats<1, 1>;
-using Many = Stats<4, 2>;
+template <int D>
+using Few = Stats<D, 1, 1>;
+template <int D>
+using Many = Stats<D, 4, 2>;
+
+// Key sums: every wavefront holds 64 keys; rows stream by in tiles of 32 through a ring of four.
+constexpr int kSumKeys = 64 * kWaves, kSumRows = 32, kSumRing = 4;
+constexpr int kInfoRows = 1024;  // rows whose maxima and denominators are in LDS at a time
 
 // One request's part of the call: the rows that count, and the keys.
 struct Req {
@@ -64,33 +75,27 @@ __device__ __forceinline__ Req request(const WeightArgs& a, int r) {
   return x;
 }
 
-// ceil(x / n) for x >= 0, and of products past 31 bits.
-__device__ __forceinline__ int over(int64_t x, int n) { return static_cast<int>((x + n - 1) / n); }
+__device__ __forceinline__ int over(int x, int n) { return static_cast<int>((static_cast<uint32_t>(x) + n - 1) / static_cast<uint32_t>(n)); }
 
-template <typename T>
-__device__ __forceinline__ T wave_total(T v) {
+__device__ __forceinline__ int64_t wave_total(int64_t v) {
 #pragma unroll
   for (int m = 1; m < 64; m <<= 1) v += __shfl_xor(v, m);
   return v;
 }
 
-// Key tiles of a range of the row stats: all (row tile, key tile) pairs in about `target` items.
-template <class S>
-__device__ __forceinline__ int range_tiles(const WeightArgs& a, int lane) {
+// The share of one item when all key heads' pairs of tiles (pairs(request) of each) are cut into about `items`.
+template <typename Pairs>
+__device__ __forceinline__ int share_of(const WeightArgs& a, int lane, int items, int least, Pairs pairs) {
   int64_t work = 0;
-  for (int r0 = 0; r0 < a.n_req; r0 += 64) {
-    const Req x = request(a, r0 + lane);
-    work += static_cast<int64_t>(over(static_cast<int64_t>(x.n_new) * a.group, S::kRows)) * over(x.len, S::kKeys);
-  }
+  for (int r0 = 0; r0 < a.n_req; r0 += 64) work += pairs(request(a, r0 + lane));
   work = wave_total(work) * a.kv_heads;
-  const int64_t share = (work + a.target - 1) / a.target;
-  return static_cast<int>(min(max(share, static_cast<int64_t>(256 / S::kKeys)), static_cast<int64_t>(1 << 22)));
+  return uniform(static_cast<int>(min(max((work + items - 1) / items, static_cast<int64_t>(least)), static_cast<int64_t>(1 << 25))));
 }
 
 // Request that holds item `at` when request r has count(r) items: false if none does; *base: items before it.
 template <typename Count>
-__device__ __forceinline__ bool find_request(const WeightArgs& a, int lane, int64_t at, Count count, int* req, int64_t* base) {
-  int64_t before = 0;
+__device__ __forceinline__ bool find_request(const WeightArgs& a, int lane, int at, Count count, int* req, int* base) {
+  int before = 0;
   for (int r0 = 0; r0 < a.n_req; r0 += 64) {
     const int mine = r0 + lane < a.n_req ? count(request(a, r0 + lane)) : 0;
     const int incl = wave_scan(mine);
@@ -99,148 +104,204 @@ __device__ __forceinline__ bool find_request(const WeightArgs& a, int lane, int6
       const int l = __builtin_ctzll(past);
       *req = uniform(r0 + l);
       *base = before + __builtin_amdgcn_readlane(incl, l) - __builtin_amdgcn_readlane(mine, l);
-      return true;
+      return at >= *base;  // sums past 31 bits: only of an offset table that is not ascending
     }
     before += __builtin_amdgcn_readlane(incl, 63);
   }
   return false;
 }
 
-// Eight cached values (chunk `chunk` of key `key` of a request) as bf16.
-template <int D, Format F>
-struct Chunk {
-  std::conditional_t<F == kBf16, uint4, std::conditional_t<F == kE4m3, uint2, uint32_t>> w;
-  uint8_t scale;
-};
-template <int D, Format F>
-__device__ __forceinline__ Chunk<D, F> load_chunk(const WeightArgs& a, const int32_t* table, int head, int key, int chunk) {
-  Chunk<D, F> x;
-  const int slot = table[key >> a.c.shift];
-  const int page = static_cast<unsigned>(slot) < static_cast<unsigned>(a.c.n_pages) ? slot : 0;
-  const int at = key & ((1 << a.c.shift) - 1);
-  const unsigned char* p = a.c.k + page * a.c.page + head * a.c.head + at * a.c.row;
-  x.w = reinterpret_cast<const decltype(x.w)*>(p)[chunk];
-  x.scale = 0;
-  if constexpr (F != kBf16) {
-    constexpr int per = F == kE2m1 ? D / kScaleBlock : 1;
-    x.scale = a.c.k_scale[page * a.c.s_page + head * a.c.s_head + at * per + (F == kE2m1 ? chunk / 4 : 0)];
-  }
-  return x;
+// Items of the requests before `req`.
+template <typename Count>
+__device__ __forceinline__ int items_before(const WeightArgs& a, int lane, int req, Count count) {
+  int n = 0;
+  for (int r0 = 0; r0 < req; r0 += 64) n += __builtin_amdgcn_readlane(wave_scan(r0 + lane < req ? count(request(a, r0 + lane)) : 0), 63);
+  return n;
 }
-template <int D, Format F>
-__device__ __forceinline__ bf16x8_t decoded(const Chunk<D, F>& x) {
+
+// How the row stats cut a request.
+template <class S>
+struct Cut {
+  int c;  // key tiles of a range
+  __device__ __forceinline__ Cut(const WeightArgs& a, int lane)
+      : c(share_of(a, lane, a.stats_items, 256 / S::kKeys, [&](const Req& x) {
+          return static_cast<int64_t>(over(x.n_new * a.group, S::kRows)) * over(x.len, S::kKeys);
+        })) {}
+  __device__ __forceinline__ int rtiles(const WeightArgs& a, const Req& x) const { return over(x.n_new * a.group, S::kRows); }
+  __device__ __forceinline__ int ranges(const Req& x) const { return max(over(over(x.len, S::kKeys), c), 1); }
+  __device__ __forceinline__ int items(const WeightArgs& a, const Req& x) const { return rtiles(a, x) * ranges(x) * a.kv_heads; }
+};
+
+// 16 bytes of codes (or bf16) of a cached row, as bf16 in pieces of eight.
+template <Format F>
+constexpr int kWordChunks = F == kBf16 ? 1 : F == kE4m3 ? 2 : 4;
+template <Format F>
+__device__ __forceinline__ void decode(const uint4& w, float s, bf16x8_t (&out)[kWordChunks<F>]) {
   if constexpr (F == kBf16) {
-    return __builtin_bit_cast(bf16x8_t, x.w);
+    out[0] = __builtin_bit_cast(bf16x8_t, w);
   } else if constexpr (F == kE2m1) {
-    return e2m1_to_bf16(x.w, scale_of(x.scale));
+    out[0] = e2m1_to_bf16(w.x, s), out[1] = e2m1_to_bf16(w.y, s), out[2] = e2m1_to_bf16(w.z, s), out[3] = e2m1_to_bf16(w.w, s);
   } else {
-    const float s = scale_of(x.scale);
-    const auto p0 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x.w.x, s, false), p1 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x.w.x, s, true);
-    const auto p2 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x.w.y, s, false), p3 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x.w.y, s, true);
-    return bf16x8_t{p0[0], p0[1], p1[0], p1[1], p2[0], p2[1], p3[0], p3[1]};
+    auto eight = [&](uint32_t lo, uint32_t hi) {
+      const auto p0 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, s, false), p1 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, s, true);
+      const auto p2 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, s, false), p3 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, s, true);
+      return bf16x8_t{p0[0], p0[1], p1[0], p1[1], p2[0], p2[1], p3[0], p3[1]};
+    };
+    out[0] = eight(w.x, w.y), out[1] = eight(w.z, w.w);
   }
 }
 
-// Place of chunk c of row `row` in a staged tile: 8 rows in a row at one chunk lie on 8 chunks.
-template <int D>
-__device__ __forceinline__ int place(int row, int c) { return (row * (D / 8) + (c ^ (row & 7))) * 16; }
-
-// Row `row` of a request's head: its token, its query head's address, and the last key that it sees.
-struct Row {
-  const uint16_t* q;
-  int pos;
-};
-__device__ __forceinline__ Row row_of(const WeightArgs& a, const Req& x, int req, int head, int row) {
-  const int token = row / a.group;
-  const int b = a.cu == nullptr ? req : 0;
-  return {a.q + b * a.qs[0] + static_cast<int64_t>(head * a.group + row - token * a.group) * a.qs[1] +
-              static_cast<int64_t>(x.start + token) * a.qs[2],
-          x.len - x.n_new + token};
+__device__ __forceinline__ int valid_page(const WeightArgs& a, int page) {  // page 0 for none: such keys are masked
+  return static_cast<unsigned>(page) < static_cast<unsigned>(a.c.n_pages) ? page : 0;
+}
+__device__ __forceinline__ bool on_a_page(const WeightArgs& a, const int32_t* table, int key) {
+  return static_cast<unsigned>(table[key >> a.c.shift]) < static_cast<unsigned>(a.c.n_pages);
+}
+template <Format F, int D>
+__device__ __forceinline__ const uint8_t* scales_of(const WeightArgs& a, int page, int head, int at) {
+  return a.c.k_scale + page * a.c.s_page + head * a.c.s_head + at * (F == kE2m1 ? D / kScaleBlock : 1);
 }
 
-// Keys that any of a request's rows [row0, row1] sees.
+// A product's step kk takes any 16 features, the same ones of both operands: lane half h those of chunk h D/16 + kk, so
+// that a lane's share of a row lies in a row.  Staged rows: 8 rows in a row at one chunk lie on 8 chunks.
+template <int D>
+__device__ __forceinline__ int chunk_of(int kk, int half) { return half * (D / 16) + kk; }
+template <int D>
+__device__ __forceinline__ int place(int row, int chunk) { return (row * (D / 8) + (chunk ^ (row & 7))) * 16; }
+
+// Address of a request's row (token, query head of the key head), tokens counted from its first counted one.
+__device__ __forceinline__ const uint16_t* q_row(const WeightArgs& a, const Req& x, int req, int head, int token, int g) {
+  return a.q + (a.cu == nullptr ? req : 0) * a.qs[0] + static_cast<int64_t>(head * a.group + g) * a.qs[1] +
+         static_cast<int64_t>(x.start + token) * a.qs[2];
+}
+
+// Keys that a request's rows up to row1 see.
 __device__ __forceinline__ int seen_by(const WeightArgs& a, const Req& x, int row1) {
   return max(0, min(x.len, x.len - x.n_new + row1 / a.group + 1));
 }
 
-__device__ __forceinline__ bool on_a_page(const WeightArgs& a, const int32_t* table, int key) {
-  return static_cast<unsigned>(table[key >> a.c.shift]) < static_cast<unsigned>(a.c.n_pages);
+__device__ __forceinline__ void lane_to_lds(const void* p, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(p), "s"(lds) : "memory", "m0");
+}
+template <int N>
+__device__ __forceinline__ void wait_copies() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ uint32_t lds_address(const void* p) {
+  return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) void*)p));
 }
 
 template <int D, Format F, class S>
 __global__ __launch_bounds__(kThreads) void row_stats_kernel(WeightArgs a) {
-  constexpr int CR = D / 8, kSteps = D / 16, NB = S::NB, kMoves = S::kKeys * CR / kThreads;
-  __shared__ __attribute__((aligned(16))) unsigned char smem[2 * S::kKeys * CR * 16];
+  constexpr int kSteps = D / 16, NB = S::NB, R = S::kRing;
+  constexpr int kRowBytes = F == kBf16 ? 2 * D : F == kE4m3 ? D : D / 2;
+  constexpr int kMoves = S::kKeys * kRowBytes / 16 / kThreads;      // 16-byte moves of a thread and tile
+  constexpr int kLanes = kRowBytes / 16, kMoveRows = 64 / kLanes;  // lanes of a row, rows of a wavefront's move
+  static_assert(kMoves >= 1, "a tile gives every thread a move");
+  __shared__ __attribute__((aligned(1024))) unsigned char smem[R * S::kTileBytes];
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
   const int rw = wave % S::RW, kw = wave / S::RW, col = lane & 31, half = lane >> 5;
-  const int c = uniform(range_tiles<S>(a, lane));
-  auto tiles = [&](const Req& x) { return over(static_cast<int64_t>(x.n_new) * a.group, S::kRows); };
-  auto ranges = [&](const Req& x) { return max(over(over(x.len, S::kKeys), c), 1); };
-  for (int64_t item = blockIdx.x;; item += gridDim.x) {
-    int req;
-    int64_t base;
-    if (!find_request(a, lane, item, [&](const Req& x) { return tiles(x) * ranges(x) * a.kv_heads; }, &req, &base)) return;
-    const Req x = request(a, req);
-    const int n_rt = uniform(tiles(x)), n_ranges = uniform(ranges(x)), k = uniform(static_cast<int>(item - base));
-    const int rtile = k % n_rt, hr = k / n_rt, range = hr % n_ranges, head = hr / n_ranges;
+  const uint32_t lds0 = lds_address(smem);
+  const Cut<S> cut(a, lane);
+  for (int item = blockIdx.x; item < a.part_items; item += gridDim.x) {
+    int req, base;
+    if (!find_request(a, lane, item, [&](const Req& x) { return cut.items(a, x); }, &req, &base)) return;
+    Req x = request(a, req);
+    x.start = uniform(x.start), x.n_new = uniform(x.n_new), x.len = uniform(x.len);
+    const int n_rt = uniform(cut.rtiles(a, x)), n_ranges = uniform(cut.ranges(x)), k = uniform(item - base);
+    const int rtile = uniform(k % n_rt), hr = uniform(k / n_rt), range = uniform(hr % n_ranges), head = uniform(hr / n_ranges);
     const int row0 = rtile * S::kRows, rows = x.n_new * a.group;
     const int kend = uniform(seen_by(a, x, min(row0 + S::kRows, rows) - 1));
-    const int key0 = range * c * S::kKeys;
-    const int nt = uniform(min(c, over(max(kend - key0, 0), S::kKeys)));
-    if (item >= a.part_items || (range > 0 && nt == 0)) continue;
+    const int key0 = range * cut.c * S::kKeys;
+    const int nt = uniform(min(cut.c, over(max(kend - key0, 0), S::kKeys)));
+    if (range > 0 && nt == 0) continue;
     const int32_t* const table = a.c.table + req * a.c.table_stride;
     bool bad = false;
     for (int i = (key0 >> a.c.shift) + lane; i <= ((min(key0 + nt * S::kKeys, kend) - 1) >> a.c.shift); i += 64)
       bad |= static_cast<unsigned>(table[i]) >= static_cast<unsigned>(a.c.n_pages);
     const bool absent = __builtin_amdgcn_ballot_w64(bad) != 0;
 
-    int pos[NB];
-    bf16x8_t qf[NB][kSteps];
-#pragma unroll
-    for (int n = 0; n < NB; ++n) {
-      const Row r = row_of(a, x, req, head, min(row0 + (rw * NB + n) * 32 + col, rows - 1));
-      pos[n] = r.pos;
-#pragma unroll
-      for (int kk = 0; kk < kSteps; ++kk) qf[n][kk] = *reinterpret_cast<const bf16x8_t*>(r.q + kk * 16 + half * 8);
-    }
-    const int pos_min = x.len - x.n_new + min(row0 + rw * NB * 32, rows - 1) / a.group;
-    float m_run[NB], l_run[NB];
-#pragma unroll
-    for (int n = 0; n < NB; ++n) m_run[n] = -__builtin_inff(), l_run[n] = 0.0f;
-
-    Chunk<D, F> in[kMoves];
-    auto load = [&](int t) {
+    // ---- tiles: bf16 rows are copied to LDS as they are, codes pass through registers.  Keys past kend repeat the last
+    // one (the mask discards them).  A move's rows lie on one page, 32 of them on two.
+    const unsigned char* const base_k = a.c.k + head * a.c.head;
+    const int mask = (1 << a.c.shift) - 1, lrow = lane / kLanes, word = lane % kLanes;
+    uint4 in[F == kBf16 ? 1 : kMoves];
+    uint8_t in_scale[F == kBf16 ? 1 : kMoves];
+    auto move = [&](int t) {
 #pragma unroll
       for (int i = 0; i < kMoves; ++i) {
-        const int at = i * kThreads + tid;
-        in[i] = load_chunk<D, F>(a, table, head, min(key0 + t * S::kKeys + at / CR, kend - 1), at % CR);
+        const int row = (i * kWaves + wave) * kMoveRows, first = key0 + t * S::kKeys + row;
+        int page = valid_page(a, scalar_load(table, uniform(min(first, kend - 1)) >> a.c.shift));
+        if constexpr (kMoveRows > 16) {
+          const int second = valid_page(a, scalar_load(table, uniform(min(first + 16, kend - 1)) >> a.c.shift));
+          page = lrow < 16 ? page : second;
+        }
+        const int at = min(first + lrow, kend - 1) & mask;
+        const unsigned char* const p = base_k + page * a.c.page + at * a.c.row;
+        if constexpr (F == kBf16) {
+          lane_to_lds(p + (word ^ ((row + lrow) & 7)) * 16, lds0 + static_cast<uint32_t>((t % R) * S::kTileBytes + (i * kWaves + wave) * 1024));
+        } else {
+          in[i] = reinterpret_cast<const uint4*>(p)[word];
+          in_scale[i] = scales_of<F, D>(a, page, head, at)[F == kE2m1 ? word : 0];
+        }
       }
     };
     auto store = [&](int t) {
+      if constexpr (F != kBf16) {
 #pragma unroll
-      for (int i = 0; i < kMoves; ++i) {
-        const int at = i * kThreads + tid;
-        *reinterpret_cast<bf16x8_t*>(smem + (t & 1) * S::kKeys * CR * 16 + place<D>(at / CR, at % CR)) = decoded<D, F>(in[i]);
+        for (int i = 0; i < kMoves; ++i) {
+          bf16x8_t y[kWordChunks<F>];
+          decode<F>(in[i], scale_of(in_scale[i]), y);
+#pragma unroll
+          for (int u = 0; u < kWordChunks<F>; ++u)
+            *reinterpret_cast<bf16x8_t*>(smem + (t % R) * S::kTileBytes + place<D>((i * kWaves + wave) * kMoveRows + lrow, word * kWordChunks<F> + u)) = y[u];
+        }
       }
     };
     __syncthreads();  // the item before has read its tiles
     if (nt > 0) {
-      load(0);
-      store(0);
+      move(0);
+      if constexpr (F != kBf16) store(0);
+      if (nt > 1) move(1);
     }
-    __syncthreads();
-    for (int t = 0; t < nt; ++t) {
-      if (t + 1 < nt) load(t + 1);
-      const unsigned char* const tile = smem + (t & 1) * S::kKeys * CR * 16;
+
+    int pos[NB];
+    bf16x8_t qf[NB][kSteps];
 #pragma unroll
-      for (int sub = 0; sub < S::kKeys / 32 / S::KW; ++sub) {
-        const int first = (S::KW == 1 ? sub : kw) * 32, kb0 = key0 + t * S::kKeys + first;
+    for (int n = 0; n < NB; ++n) {
+      const int row = min(row0 + (rw * NB + n) * 32 + col, rows - 1), token = row / a.group;
+      const uint16_t* const q = q_row(a, x, req, head, token, row - token * a.group);
+      pos[n] = x.len - x.n_new + token;
+#pragma unroll
+      for (int kk = 0; kk < kSteps; ++kk) qf[n][kk] = *reinterpret_cast<const bf16x8_t*>(q + chunk_of<D>(kk, half) * 8);
+    }
+    const int pos_min = uniform(x.len - x.n_new + min(row0 + rw * NB * 32, rows - 1) / a.group);
+    float m_run[NB], l_run[NB];
+#pragma unroll
+    for (int n = 0; n < NB; ++n) m_run[n] = -__builtin_inff(), l_run[n] = 0.0f;
+
+    for (int t = 0; t < nt; ++t) {
+      if constexpr (F == kBf16) {
+        if (R > 2 && t + 1 < nt) wait_copies<kMoves>();  // tile t has landed, tile t + 1 may be on its way
+        else wait_copies<0>();
+        __syncthreads();  // and the tile before is read, whose stage is the next copy's
+        if (R > 2 && t + 2 < nt) move(t + 2);
+        if (R == 2 && t > 0 && t + 1 < nt) move(t + 1);
+      } else {
+        __syncthreads();  // tile t is stored, the one before is read
+        if (t + 1 < nt) store(t + 1);
+        if (t + 2 < nt) move(t + 2);
+      }
+      const unsigned char* const tile = smem + (t % R) * S::kTileBytes;
+#pragma unroll
+      for (int sub = 0; sub < S::kSubs; ++sub) {
+        const int first = (kw * S::kSubs + sub) * 32, kb0 = key0 + t * S::kKeys + first;
         f32x16_t s[NB];
 #pragma unroll
         for (int n = 0; n < NB; ++n) s[n] = f32x16_t{};
 #pragma unroll
         for (int kk = 0; kk < kSteps; ++kk) {
-          const bf16x8_t kf = *reinterpret_cast<const bf16x8_t*>(tile + place<D>(first + col, 2 * kk + half));
+          const bf16x8_t kf = *reinterpret_cast<const bf16x8_t*>(tile + place<D>(first + col, chunk_of<D>(kk, half)));
 #pragma unroll
           for (int n = 0; n < NB; ++n) s[n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qf[n][kk], s[n], 0, 0, 0);
         }
@@ -272,15 +333,15 @@ __global__ __launch_bounds__(kThreads) void row_stats_kernel(WeightArgs a) {
           l_run[n] += sum;
         }
       }
-      if (t + 1 < nt) store(t + 1);
-      __syncthreads();
     }
 
-    float* const part = a.part + item * (2 * S::kRows);
+    float* const part = a.part + static_cast<int64_t>(item) * (2 * S::kRows);
+    if constexpr (S::KW > 1) __syncthreads();  // the tiles are read
 #pragma unroll
     for (int n = 0; n < NB; ++n) {
       float m = m_run[n], l = half_sum(l_run[n]);
       if constexpr (S::KW > 1) {  // the key parts of these rows
+        static_assert(NB == 1, "LDS is used once");
         float* const ml = reinterpret_cast<float*>(smem);
         if (half == 0) ml[(wave * 32 + col) * 2] = m, ml[(wave * 32 + col) * 2 + 1] = l;
         __syncthreads();
@@ -303,144 +364,214 @@ __global__ __launch_bounds__(kThreads) void row_stats_kernel(WeightArgs a) {
   }
 }
 
-// Key sums: every wavefront holds 32 keys in registers; rows stream by in tiles of 32.
+// How the key sums cut a request: tiles of kSumKeys keys times ranges of c row tiles.
+struct SumCut {
+  int c;
+  __device__ __forceinline__ SumCut(const WeightArgs& a, int lane)
+      : c(share_of(a, lane, a.sums_items, 4, [&](const Req& x) {
+          return static_cast<int64_t>(over(x.n_new * a.group, kSumRows)) * over(x.len, kSumKeys);
+        })) {}
+  __device__ __forceinline__ int ktiles(const WeightArgs& a, const Req& x) const { return x.n_new > 0 ? over(x.len, kSumKeys) * a.kv_heads : 0; }
+  __device__ __forceinline__ int ranges(const WeightArgs& a, const Req& x) const { return max(over(over(x.n_new * a.group, kSumRows), c), 1); }
+  __device__ __forceinline__ int items(const WeightArgs& a, const Req& x) const { return ktiles(a, x) * ranges(a, x); }
+  // of requests that are cut into row ranges: their items' sums have places in the workspace, below 2 sums_items
+  __device__ __forceinline__ int places(const WeightArgs& a, const Req& x) const { return ranges(a, x) > 1 ? items(a, x) : 0; }
+  __device__ __forceinline__ int joins(const WeightArgs& a, const Req& x) const { return ranges(a, x) > 1 ? ktiles(a, x) : 0; }
+};
+// First row of a request that sees key `key` (of its counted rows).
+__device__ __forceinline__ int first_row(const WeightArgs& a, const Req& x, int key) {
+  return max(0, min(key - (x.len - x.n_new), x.n_new)) * a.group;
+}
+
 template <int D, Format F, class S>
 __global__ __launch_bounds__(kThreads) void key_sums_kernel(WeightArgs a) {
-  constexpr int CR = D / 8, kSteps = D / 16, kKeys = 32 * kWaves, kRows = 32;
-  constexpr int kTile = kRows * CR * 16, kMoves = kRows * CR / kThreads;
-  static_assert(kMoves >= 1 && kKeys * CR * 16 >= 2 * kTile, "LDS holds the keys first, then two tiles of rows");
-  __shared__ __attribute__((aligned(16))) unsigned char smem[kKeys * CR * 16];
-  __shared__ __attribute__((aligned(16))) float row_m[2][kRows], row_inv[2][kRows];
-  __shared__ __attribute__((aligned(16))) int row_pos[2][kRows];
+  constexpr int CR = D / 8, kSteps = D / 16, kTile = kSumRows * CR * 16, kCopies = kTile / 1024 / kWaves;
+  constexpr int kRowBytes = F == kBf16 ? 2 * D : F == kE4m3 ? D : D / 2, kWords = kRowBytes / 32;  // of a lane's half row
+  static_assert(kCopies >= 1, "a tile gives every wavefront a copy");
+  __shared__ __attribute__((aligned(1024))) unsigned char smem[kSumRing * kTile];
+  __shared__ __attribute__((aligned(16))) float row_m[kInfoRows], row_inv[kInfoRows];
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
   const int col = lane & 31, half = lane >> 5;
-  const int c = uniform(range_tiles<S>(a, lane));
-  auto tiles = [&](const Req& x) { return over(static_cast<int64_t>(x.n_new) * a.group, S::kRows); };
-  auto ranges = [&](const Req& x) { return max(over(over(x.len, S::kKeys), c), 1); };
-  for (int64_t item = blockIdx.x;; item += gridDim.x) {
-    int req;
-    int64_t base;
-    auto count = [&](const Req& x) { return x.n_new > 0 ? over(x.len, kKeys) * a.kv_heads : 0; };
-    if (!find_request(a, lane, item, count, &req, &base)) return;
-    const Req x = request(a, req);
-    const int k = uniform(static_cast<int>(item - base)), n_kt = uniform(over(x.len, kKeys));
-    const int head = k / n_kt, key0 = (k % n_kt) * kKeys;
+  const uint32_t lds0 = lds_address(smem);
+  const Cut<S> stats(a, lane);
+  const SumCut cut(a, lane);
+  for (int item = blockIdx.x;; item += gridDim.x) {
+    int req, base;
+    if (!find_request(a, lane, item, [&](const Req& x) { return cut.items(a, x); }, &req, &base)) return;
+    Req x = request(a, req);
+    x.start = uniform(x.start), x.n_new = uniform(x.n_new), x.len = uniform(x.len);
+    const int n_ranges = uniform(cut.ranges(a, x)), k = uniform(item - base), n_kt = uniform(over(x.len, kSumKeys));
+    const int range = uniform(k % n_ranges), hk = uniform(k / n_ranges), kt = uniform(hk % n_kt), head = uniform(hk / n_kt);
+    const int key0 = kt * kSumKeys, rows = x.n_new * a.group;
+    const int t0 = uniform(max(first_row(a, x, key0) / kSumRows, range * cut.c));
+    const int t1 = uniform(min(over(rows, kSumRows), (range + 1) * cut.c));
+    if (t0 >= t1) continue;  // none of these rows sees the keys
     const int slot = uniform(owned_slot(a.index, req, a.w_rows, lane));
     if (slot < 0) continue;
     const int32_t* const table = a.c.table + req * a.c.table_stride;
-    // first item of the request in the row stats
-    int64_t stats = 0;
-    for (int r0 = 0; r0 < req; r0 += 64) {
-      const Req y = request(a, r0 + lane);
-      stats += r0 + lane < req ? static_cast<int64_t>(tiles(y)) * ranges(y) * a.kv_heads : 0;
-    }
-    stats = wave_total(stats);
-    const int n_rt = tiles(x), n_ranges = ranges(x), rows = x.n_new * a.group;
+    const int first_stats = uniform(items_before(a, lane, req, [&](const Req& y) { return stats.items(a, y); }));
+    const int n_rt = uniform(stats.rtiles(a, x)), stats_ranges = uniform(stats.ranges(x));
 
-    // ---- the keys, through LDS into registers
+    // ---- rows: tile t's are copied to stage t % kSumRing; rows behind the last one repeat it (the mask discards them)
+    const int step_tokens = uniform(kSumRows / a.group), step_rem = kSumRows - step_tokens * a.group;
+    int copy_token = uniform(t0 * kSumRows / a.group), copy_rem = t0 * kSumRows - copy_token * a.group;  // of the next copy
+    auto token_in = [&](int rem, int r) { return static_cast<int>((static_cast<uint32_t>(rem + r) * a.group_magic) >> 24); };
+    auto copy = [&](int t) {
+#pragma unroll
+      for (int i = 0; i < kCopies; ++i) {
+        const int at = (i * kWaves + wave) * 64 + lane, r = at / CR, row = min(r, rows - 1 - t * kSumRows);
+        const int token = token_in(copy_rem, row);
+        lane_to_lds(q_row(a, x, req, head, copy_token + token, copy_rem + row - token * a.group) + ((at % CR) ^ (r & 7)) * 8,
+                    lds0 + static_cast<uint32_t>((t % kSumRing) * kTile + (i * kWaves + wave) * 1024));
+      }
+      copy_token += step_tokens, copy_rem += step_rem;
+      if (copy_rem >= a.group) copy_token += 1, copy_rem -= a.group;
+    };
     __syncthreads();  // the item before has read its tiles
 #pragma unroll
-    for (int i = 0; i < kKeys * CR / kThreads; ++i) {
-      const int at = i * kThreads + tid;
-      const auto in = load_chunk<D, F>(a, table, head, min(key0 + at / CR, x.len - 1), at % CR);
-      *reinterpret_cast<bf16x8_t*>(smem + place<D>(at / CR, at % CR)) = decoded<D, F>(in);
-    }
-    __syncthreads();
-    bf16x8_t kf[kSteps];
-#pragma unroll
-    for (int kk = 0; kk < kSteps; ++kk) kf[kk] = *reinterpret_cast<const bf16x8_t*>(smem + place<D>(wave * 32 + col, 2 * kk + half));
-    __syncthreads();
-    const int key = key0 + wave * 32 + col;
+    for (int u = 0; u < kSumRing - 1; ++u)
+      if (t0 + u < t1) copy(t0 + u);
 
-    // ---- the rows that see the first key, tile by tile
-    const int first = max(0, min(key0 - (x.len - x.n_new), x.n_new)) * a.group / kRows, nt = over(rows, kRows);
-    bf16x8_t in[kMoves];
-    float in_m = 0.0f, in_inv = 0.0f;
-    int in_pos = -1;
-    auto load = [&](int t) {
+    // ---- this lane's keys
+    bf16x8_t kf[2][kSteps];
+    int key[2];
 #pragma unroll
-      for (int i = 0; i < kMoves; ++i) {
-        const int at = i * kThreads + tid;
-        in[i] = *reinterpret_cast<const bf16x8_t*>(row_of(a, x, req, head, min(t * kRows + at / CR, rows - 1)).q + at % CR * 8);
-      }
-      if (tid < kRows) {  // the row's maximum and denominator over all ranges
-        const int row = t * kRows + tid, rtile = min(row, rows - 1) / S::kRows;
-        const int kend = seen_by(a, x, min((rtile + 1) * S::kRows, rows) - 1);
-        const int n = max(1, over(over(kend, S::kKeys), c));
-        const int64_t slot0 = stats + static_cast<int64_t>(head) * n_ranges * n_rt + rtile;
-        const float* const p = a.part + slot0 * (2 * S::kRows) + (min(row, rows - 1) - rtile * S::kRows) * 2;
-        // (every part has its place but those of an offset table that is not ascending)
-        const bool held = slot0 >= 0 && slot0 + static_cast<int64_t>(n - 1) * n_rt < a.part_items;
-        float m = -__builtin_inff(), l = 0.0f;
-        for (int i = 0; i < (held ? n : 0); ++i) {
-          const float m2 = p[static_cast<int64_t>(i) * n_rt * (2 * S::kRows)], l2 = p[static_cast<int64_t>(i) * n_rt * (2 * S::kRows) + 1];
-          const float top = fmaxf(m, m2), sub = top == -__builtin_inff() ? 0.0f : top;
-          l = l * __builtin_amdgcn_exp2f(m - sub) + l2 * __builtin_amdgcn_exp2f(m2 - sub);
-          m = top;
-        }
-        in_m = m == -__builtin_inff() ? 0.0f : m;
-        in_inv = l == 0.0f ? 0.0f : 1.0f / l;
-        in_pos = row < rows ? x.len - x.n_new + row / a.group : -1;
-      }
-    };
-    auto store = [&](int t) {
+    for (int n = 0; n < 2; ++n) {
+      key[n] = key0 + wave * 64 + n * 32 + col;
+      const int held = min(key[n], x.len - 1), page = valid_page(a, table[held >> a.c.shift]), at = held & ((1 << a.c.shift) - 1);
+      const uint4* const p = reinterpret_cast<const uint4*>(a.c.k + page * a.c.page + head * a.c.head + at * a.c.row) + half * kWords;
 #pragma unroll
-      for (int i = 0; i < kMoves; ++i) {
-        const int at = i * kThreads + tid;
-        *reinterpret_cast<bf16x8_t*>(smem + (t & 1) * kTile + place<D>(at / CR, at % CR)) = in[i];
+      for (int i = 0; i < kWords; ++i) {
+        float scale = 1.0f;
+        if constexpr (F != kBf16) scale = scale_of(scales_of<F, D>(a, page, head, at)[F == kE2m1 ? half * kWords + i : 0]);
+        bf16x8_t y[kWordChunks<F>];
+        decode<F>(p[i], scale, y);
+#pragma unroll
+        for (int u = 0; u < kWordChunks<F>; ++u) kf[n][i * kWordChunks<F> + u] = y[u];
       }
-      if (tid < kRows) row_m[t & 1][tid] = in_m, row_inv[t & 1][tid] = in_inv, row_pos[t & 1][tid] = in_pos;
-    };
-    float sum = 0.0f;
-    if (first < nt) {
-      load(first);
-      store(first);
     }
-    __syncthreads();
-    for (int t = first; t < nt; ++t) {
-      if (t + 1 < nt) load(t + 1);
-      f32x16_t s = f32x16_t{};
+
+    float sum[2] = {0.0f, 0.0f};
+    int info0 = -1;  // first row of those in row_m
+    int token0 = uniform(t0 * kSumRows / a.group), rem0 = t0 * kSumRows - token0 * a.group;  // of tile t's first row
+    for (int t = t0; t < t1; ++t) {
+      const int row0 = t * kSumRows;
+      if (info0 < 0 || row0 >= info0 + kInfoRows) {
+        __syncthreads();  // the rows before are done with theirs
+        info0 = row0;
+        for (int i = tid; i < min(kInfoRows, t1 * kSumRows - info0); i += kThreads) {
+          // the row's maximum and denominator over all ranges
+          const int row = min(info0 + i, rows - 1), rtile = row / S::kRows;
+          const int kend = seen_by(a, x, min((rtile + 1) * S::kRows, rows) - 1);
+          const int n = max(1, over(over(kend, S::kKeys), stats.c));
+          const int at = first_stats + head * stats_ranges * n_rt + rtile;
+          const float* const p = a.part + static_cast<int64_t>(at) * (2 * S::kRows) + (row - rtile * S::kRows) * 2;
+          // (every part has its place but those of an offset table that is not ascending)
+          const bool held = at >= 0 && at + static_cast<int64_t>(n - 1) * n_rt < a.part_items;
+          float m = -__builtin_inff(), l = 0.0f;
+          for (int v = 0; v < (held ? n : 0); ++v) {
+            const float2 y = *reinterpret_cast<const float2*>(p + static_cast<int64_t>(v) * n_rt * (2 * S::kRows));
+            const float top = fmaxf(m, y.x), sub = top == -__builtin_inff() ? 0.0f : top;
+            l = l * __builtin_amdgcn_exp2f(m - sub) + y.y * __builtin_amdgcn_exp2f(y.x - sub);
+            m = top;
+          }
+          row_m[i] = m == -__builtin_inff() ? 0.0f : m;
+          row_inv[i] = l == 0.0f ? 0.0f : 1.0f / l;
+        }
+      }
+      if (t + 2 < t1) wait_copies<2 * kCopies>();  // tile t has landed
+      else wait_copies<0>();
+      __syncthreads();
+      if (t + kSumRing - 1 < t1) copy(t + kSumRing - 1);
+      const unsigned char* const tile = smem + (t % kSumRing) * kTile;
+      f32x16_t s[2] = {f32x16_t{}, f32x16_t{}};
 #pragma unroll
       for (int kk = 0; kk < kSteps; ++kk) {
-        const bf16x8_t qf = *reinterpret_cast<const bf16x8_t*>(smem + (t & 1) * kTile + place<D>(col, 2 * kk + half));
-        s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(qf, kf[kk], s, 0, 0, 0);
+        const bf16x8_t qf = *reinterpret_cast<const bf16x8_t*>(tile + place<D>(col, chunk_of<D>(kk, half)));
+#pragma unroll
+        for (int n = 0; n < 2; ++n) s[n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(qf, kf[n][kk], s[n], 0, 0, 0);
       }
-      float tile_sum = 0.0f;
+      const int limit = x.len - x.n_new + token0;  // last key that the tile's first row sees
+      const bool masked = limit < key0 + wave * 64 + 63 || row0 + kSumRows > rows;
+      float tile_sum[2] = {0.0f, 0.0f};
 #pragma unroll
       for (int r4 = 0; r4 < 4; ++r4) {
         const int row = 8 * r4 + 4 * half;
-        const f32x4_t m = *reinterpret_cast<const f32x4_t*>(&row_m[t & 1][row]), inv = *reinterpret_cast<const f32x4_t*>(&row_inv[t & 1][row]);
-        const int4 pos = *reinterpret_cast<const int4*>(&row_pos[t & 1][row]);
-        const int ps[4] = {pos.x, pos.y, pos.z, pos.w};
+        const f32x4_t m = *reinterpret_cast<const f32x4_t*>(&row_m[row0 - info0 + row]);
+        const f32x4_t inv = *reinterpret_cast<const f32x4_t*>(&row_inv[row0 - info0 + row]);
+        float p[2][4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * r4 + e], a.scale_log2, -m[e])) * inv[e];
-          tile_sum += key <= ps[e] ? p : 0.0f;
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) p[n][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][4 * r4 + e], a.scale_log2, -m[e])) * inv[e];
+        if (masked) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int last = row0 + row + e < rows ? limit + token_in(rem0, row + e) : -1;
+#pragma unroll
+            for (int n = 0; n < 2; ++n) p[n][e] = key[n] <= last ? p[n][e] : 0.0f;
+          }
         }
+#pragma unroll
+        for (int n = 0; n < 2; ++n) tile_sum[n] += (p[n][0] + p[n][1]) + (p[n][2] + p[n][3]);
       }
-      sum += tile_sum;
-      if (t + 1 < nt) store(t + 1);
-      __syncthreads();
+#pragma unroll
+      for (int n = 0; n < 2; ++n) sum[n] += tile_sum[n];
+      token0 += step_tokens, rem0 += step_rem;
+      if (rem0 >= a.group) token0 += 1, rem0 -= a.group;
     }
-    sum = half_sum(sum);
-    if (half == 0 && key < x.len && on_a_page(a, table, key)) a.w[slot * a.w_row + head * a.w_head + key] += sum;
+    int at = 0;
+    if (n_ranges > 1) at = uniform(items_before(a, lane, req, [&](const Req& y) { return cut.places(a, y); })) + k;
+    if (at < 0 || at >= 2 * a.sums_items) continue;  // only of an offset table that is not ascending
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+      const float y = half_sum(sum[n]);
+      if (half != 0) continue;
+      if (n_ranges > 1) a.sums[static_cast<int64_t>(at) * kSumKeys + wave * 64 + n * 32 + col] = y;
+      else if (key[n] < x.len && on_a_page(a, table, key[n])) a.w[slot * a.w_row + head * a.w_head + key[n]] += y;
+    }
+  }
+}
+
+// The row ranges' sums of every key tile of the requests that are cut into such, added range by range.
+__global__ __launch_bounds__(kSumKeys) void key_sums_join_kernel(WeightArgs a) {
+  const int lane = threadIdx.x & 63;
+  const SumCut cut(a, lane);
+  for (int item = blockIdx.x;; item += gridDim.x) {
+    int req, base;
+    if (!find_request(a, lane, item, [&](const Req& x) { return cut.joins(a, x); }, &req, &base)) return;
+    const Req x = request(a, req);
+    const int n_ranges = uniform(cut.ranges(a, x)), k = uniform(item - base), n_kt = uniform(over(x.len, kSumKeys));
+    const int kt = k % n_kt, head = k / n_kt, key = kt * kSumKeys + static_cast<int>(threadIdx.x);
+    const int slot = uniform(owned_slot(a.index, req, a.w_rows, lane));
+    if (slot < 0) continue;
+    const int at = uniform(items_before(a, lane, req, [&](const Req& y) { return cut.places(a, y); })) + k * n_ranges;
+    if (at < 0 || at + n_ranges > 2 * a.sums_items) continue;
+    float sum = 0.0f;  // from the first range on whose rows see the tile
+    for (int v = first_row(a, x, kt * kSumKeys) / kSumRows / cut.c; v < n_ranges; ++v)
+      sum += a.sums[static_cast<int64_t>(at + v) * kSumKeys + threadIdx.x];
+    if (key < x.len && on_a_page(a, a.c.table + req * a.c.table_stride, key)) a.w[slot * a.w_row + head * a.w_head + key] += sum;
   }
 }
 
 // The kernels of a call, and its items and workspace, whatever the lengths turn out to be.
 struct Plan {
-  bool few;
-  int target;
-  int64_t items, bytes;
+  bool few, may_cut;
+  int stats_items, sums_items;
+  int64_t part_items, part_bytes, bytes;
 };
 Plan plan_of(int64_t requests, int64_t tokens, int group, int kv_heads, int max_rows) {
   Plan p;
   p.few = max_rows <= 64;
-  const int rows = p.few ? Few::kRows : Many::kRows;
-  p.target = 1024;
+  const int rows = p.few ? Few<64>::kRows : Many<64>::kRows;
+  p.stats_items = 1024;
+  p.sums_items = 1024;
   // a share alone may add a range per row tile
-  p.items = p.target + kv_heads * (tokens * group / rows + requests);
-  p.bytes = p.items * rows * 8;
+  p.part_items = p.stats_items + kv_heads * (tokens * group / rows + requests);
+  p.part_bytes = (p.part_items * rows * 8 + 15) / 16 * 16;
+  // a range of row tiles is four at least, and a request without more is never cut
+  p.may_cut = tokens * group > 4 * kSumRows;
+  p.bytes = p.part_bytes + (p.may_cut ? 2LL * p.sums_items * kSumKeys * 4 : 0);
   return p;
 }
 
@@ -488,6 +619,7 @@ extern "C" int fd_paged_key_weights(const void* q, const fd_paged_cache* cache, 
   const int group = q_heads / cache->kv_heads, top = last > 0 ? std::min(last, max_seqlen) : max_seqlen;
   const Plan p = plan_of(requests, static_cast<int64_t>(batch) * seq_len, group, cache->kv_heads,
                          static_cast<int>(std::min<int64_t>(static_cast<int64_t>(top) * group, 1 << 30)));
+  FD_REQUIRE(p.part_items < (1LL << 31), FD_ERR_UNSUPPORTED, "%s: problem too large", what);
   FD_REQUIRE(workspace && fd_aligned16(workspace) && workspace_bytes >= p.bytes, FD_ERR_INVALID_ARGUMENT,
              "%s: the workspace must be 16-byte aligned and hold %lld bytes", what, static_cast<long long>(p.bytes));
   a.q = static_cast<const uint16_t*>(q);
@@ -503,22 +635,32 @@ extern "C" int fd_paged_key_weights(const void* q, const fd_paged_cache* cache, 
   a.kv_heads = cache->kv_heads;
   a.last = last > 0 ? last : seq_len;
   a.w_rows = weight_rows;
-  a.target = p.target;
-  a.part_items = static_cast<int>(std::min<int64_t>(p.items, 0x7fffffff));
+  a.group_magic = ((1u << 24) + group - 1) / group;
+  a.stats_items = p.stats_items;
+  a.sums_items = p.sums_items;
+  a.part_items = static_cast<int>(p.part_items);
   a.scale_log2 = scale * 1.4426950408889634f;
   a.part = static_cast<float*>(workspace);
+  a.sums = reinterpret_cast<float*>(static_cast<char*>(workspace) + p.part_bytes);
   hipStream_t s = static_cast<hipStream_t>(stream);
+  // workgroups: no more than the sizes can make items
+  const int64_t key_tiles = static_cast<int64_t>(requests) * cache->kv_heads *
+                            ((static_cast<int64_t>(cache->max_pages) * cache->page_size + kSumKeys - 1) / kSumKeys);
+  const int64_t row_tiles = (static_cast<int64_t>(batch) * seq_len * group + kSumRows - 1) / kSumRows;
+  const unsigned stats_grid = static_cast<unsigned>(std::min<int64_t>(p.part_items, 2048));
+  const unsigned sums_grid = static_cast<unsigned>(std::min<int64_t>(key_tiles * std::max<int64_t>(row_tiles / 4, 1), 2048));
+  const unsigned join_grid = static_cast<unsigned>(std::min<int64_t>(key_tiles, p.sums_items));
   by_kind(cache, [&](auto d, auto f) {
     constexpr int D = decltype(d)::value;
     constexpr Format F = decltype(f)::value;
     auto go = [&](auto kind) {
       using S = decltype(kind);
-      const dim3 grid(static_cast<unsigned>(std::min<int64_t>(p.items, 2048)));
-      hipLaunchKernelGGL((row_stats_kernel<D, F, S>), grid, dim3(kThreads), 0, s, a);
-      hipLaunchKernelGGL((key_sums_kernel<D, F, S>), dim3(2048), dim3(kThreads), 0, s, a);
+      hipLaunchKernelGGL((row_stats_kernel<D, F, S>), dim3(stats_grid), dim3(kThreads), 0, s, a);
+      hipLaunchKernelGGL((key_sums_kernel<D, F, S>), dim3(sums_grid), dim3(kThreads), 0, s, a);
     };
-    if (p.few) go(Few{});
-    else go(Many{});
+    if (p.few) go(Few<D>{});
+    else go(Many<D>{});
   });
+  if (p.may_cut) hipLaunchKernelGGL(key_sums_join_kernel, dim3(join_grid), dim3(kSumKeys), 0, s, a);
   return fd_check_launch(what);
 }
