@@ -37,6 +37,7 @@ struct WeightArgs {
   int stats_items, sums_items;  // items that each kernel cuts its work into, about
   int part_items;               // items of the row stats whose places the workspace holds
   float* part;                  // per item of the row stats: its rows' (m, l)
+  float* stats;                 // [heads, tokens of the call x group]: (m, 1 / l) of every row over all its keys
   float* sums;                  // per item of the key sums of a request cut into row ranges: its keys' sums
 };
 
@@ -173,6 +174,15 @@ __device__ __forceinline__ int place(int row, int chunk) { return (row * (D / 8)
 __device__ __forceinline__ const uint16_t* q_row(const WeightArgs& a, const Req& x, int req, int head, int token, int g) {
   return a.q + (a.cu == nullptr ? req : 0) * a.qs[0] + static_cast<int64_t>(head * a.group + g) * a.qs[1] +
          static_cast<int64_t>(x.start + token) * a.qs[2];
+}
+
+// Place of a request's row among the call's rows (m, 1 / l); inside them whatever the offset table holds.
+__device__ __forceinline__ int64_t stat_row(const WeightArgs& a, const Req& x, int req, int head) {
+  const int64_t tokens = a.cu == nullptr ? static_cast<int64_t>(a.n_req) * a.seq_len : a.seq_len;
+  return (head * tokens + (a.cu == nullptr ? static_cast<int64_t>(req) * a.seq_len : 0) + x.start) * a.group;
+}
+__device__ __forceinline__ float2 stat_of(float m, float l) {
+  return {m == -__builtin_inff() ? 0.0f : m, l == 0.0f ? 0.0f : 1.0f / l};
 }
 
 // Keys that a request's rows up to row1 see.
@@ -317,19 +327,23 @@ __global__ __launch_bounds__(kThreads) void row_stats_kernel(WeightArgs a) {
         }
 #pragma unroll
         for (int n = 0; n < NB; ++n) {
-          float mx = s[n][0];
-#pragma unroll
-          for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[n][r]);
-          mx = half_max(mx) * a.scale_log2;
-          if (__builtin_amdgcn_ballot_w64(mx > m_run[n] + 8.0f) != 0) {
-            const float m_new = fmaxf(m_run[n], mx);
-            l_run[n] *= m_new == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(m_run[n] - m_new);
-            m_run[n] = m_new;
-          }
-          const float m_sub = m_run[n] == -__builtin_inff() ? 0.0f : m_run[n];
+          // A row's maximum may lag: its exponentials are summed as they are while they stay far from fp32's end, which
+          // their sum shows.  Only a row's first keys, and keys 2^64 above its maximum, take the maximum first.
           float sum = 0.0f;
 #pragma unroll
-          for (int r = 0; r < 16; ++r) sum += __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][r], a.scale_log2, -m_sub));
+          for (int r = 0; r < 16; ++r) sum += __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][r], a.scale_log2, -m_run[n]));
+          if (__builtin_amdgcn_ballot_w64(!(sum < 0x1p64f)) != 0) {
+            float mx = s[n][0];
+#pragma unroll
+            for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[n][r]);
+            mx = half_max(mx) * a.scale_log2;
+            const float m_new = fmaxf(m_run[n], mx), m_sub = m_new == -__builtin_inff() ? 0.0f : m_new;
+            l_run[n] *= m_new == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(m_run[n] - m_new);
+            m_run[n] = m_new;
+            sum = 0.0f;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) sum += __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][r], a.scale_log2, -m_sub));
+          }
           l_run[n] += sum;
         }
       }
@@ -355,12 +369,51 @@ __global__ __launch_bounds__(kThreads) void row_stats_kernel(WeightArgs a) {
           }
         }
       }
-      if (half == 0 && (S::KW == 1 || wave == 0)) {
-        const int row = (rw * NB + n) * 32 + col;
+      const int row = (rw * NB + n) * 32 + col;
+      if (half != 0 || (S::KW > 1 && wave != 0) || row0 + row >= rows) continue;
+      if (n_ranges == 1) {
+        reinterpret_cast<float2*>(a.stats)[stat_row(a, x, req, head) + row0 + row] = stat_of(m, l);
+      } else {
         part[row * 2] = m;
         part[row * 2 + 1] = l;
       }
     }
+  }
+}
+
+// (m, 1 / l) of the rows whose keys were cut into ranges, one row tile per workgroup.
+template <class S>
+constexpr int kJoinThreads = S::kRows < 64 ? 64 : S::kRows;  // whole wavefronts
+template <class S>
+__global__ __launch_bounds__(kJoinThreads<S>) void row_stats_join_kernel(WeightArgs a) {
+  const int lane = threadIdx.x & 63;
+  const Cut<S> cut(a, lane);
+  for (int item = blockIdx.x;; item += gridDim.x) {
+    int req, base;
+    if (!find_request(a, lane, item, [&](const Req& x) { return cut.ranges(x) > 1 ? cut.rtiles(a, x) * a.kv_heads : 0; }, &req, &base)) return;
+    const Req x = request(a, req);
+    const int n_rt = uniform(cut.rtiles(a, x)), n_ranges = uniform(cut.ranges(x)), k = uniform(item - base);
+    const int rtile = k % n_rt, head = k / n_rt, row0 = rtile * S::kRows, rows = x.n_new * a.group;
+    const int first = uniform(items_before(a, lane, req, [&](const Req& y) { return cut.items(a, y); })) + head * n_ranges * n_rt + rtile;
+    const int n = over(over(seen_by(a, x, min(row0 + S::kRows, rows) - 1), S::kKeys), cut.c);  // ranges that a row sees
+    if (first < 0 || first + static_cast<int64_t>(n_ranges - 1) * n_rt >= a.part_items) continue;  // only of an offset table that is not ascending
+    const int row = threadIdx.x;
+    if (row >= S::kRows) continue;
+    const float2* const p = reinterpret_cast<const float2*>(a.part) + static_cast<int64_t>(first) * S::kRows + row;
+    float m = -__builtin_inff(), l = 0.0f;
+    for (int v0 = 0; v0 < n; v0 += 4) {  // four loads in flight
+      float2 y[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) y[u] = p[static_cast<int64_t>(min(v0 + u, n - 1)) * n_rt * S::kRows];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        if (v0 + u >= n) continue;
+        const float top = fmaxf(m, y[u].x), sub = top == -__builtin_inff() ? 0.0f : top;
+        l = l * __builtin_amdgcn_exp2f(m - sub) + y[u].y * __builtin_amdgcn_exp2f(y[u].x - sub);
+        m = top;
+      }
+    }
+    if (row0 + row < rows) reinterpret_cast<float2*>(a.stats)[stat_row(a, x, req, head) + row0 + row] = stat_of(m, l);
   }
 }
 
@@ -383,7 +436,7 @@ __device__ __forceinline__ int first_row(const WeightArgs& a, const Req& x, int 
   return max(0, min(key - (x.len - x.n_new), x.n_new)) * a.group;
 }
 
-template <int D, Format F, class S>
+template <int D, Format F>
 __global__ __launch_bounds__(kThreads) void key_sums_kernel(WeightArgs a) {
   constexpr int CR = D / 8, kSteps = D / 16, kTile = kSumRows * CR * 16, kCopies = kTile / 1024 / kWaves;
   constexpr int kRowBytes = F == kBf16 ? 2 * D : F == kE4m3 ? D : D / 2, kWords = kRowBytes / 32;  // of a lane's half row
@@ -393,7 +446,6 @@ __global__ __launch_bounds__(kThreads) void key_sums_kernel(WeightArgs a) {
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
   const int col = lane & 31, half = lane >> 5;
   const uint32_t lds0 = lds_address(smem);
-  const Cut<S> stats(a, lane);
   const SumCut cut(a, lane);
   for (int item = blockIdx.x;; item += gridDim.x) {
     int req, base;
@@ -409,8 +461,7 @@ __global__ __launch_bounds__(kThreads) void key_sums_kernel(WeightArgs a) {
     const int slot = uniform(owned_slot(a.index, req, a.w_rows, lane));
     if (slot < 0) continue;
     const int32_t* const table = a.c.table + req * a.c.table_stride;
-    const int first_stats = uniform(items_before(a, lane, req, [&](const Req& y) { return stats.items(a, y); }));
-    const int n_rt = uniform(stats.rtiles(a, x)), stats_ranges = uniform(stats.ranges(x));
+    const float2* const stats = reinterpret_cast<const float2*>(a.stats) + stat_row(a, x, req, head);
 
     // ---- rows: tile t's are copied to stage t % kSumRing; rows behind the last one repeat it (the mask discards them)
     const int step_tokens = uniform(kSumRows / a.group), step_rem = kSumRows - step_tokens * a.group;
@@ -459,24 +510,12 @@ __global__ __launch_bounds__(kThreads) void key_sums_kernel(WeightArgs a) {
       if (info0 < 0 || row0 >= info0 + kInfoRows) {
         __syncthreads();  // the rows before are done with theirs
         info0 = row0;
-        for (int i = tid; i < min(kInfoRows, t1 * kSumRows - info0); i += kThreads) {
-          // the row's maximum and denominator over all ranges
-          const int row = min(info0 + i, rows - 1), rtile = row / S::kRows;
-          const int kend = seen_by(a, x, min((rtile + 1) * S::kRows, rows) - 1);
-          const int n = max(1, over(over(kend, S::kKeys), stats.c));
-          const int at = first_stats + head * stats_ranges * n_rt + rtile;
-          const float* const p = a.part + static_cast<int64_t>(at) * (2 * S::kRows) + (row - rtile * S::kRows) * 2;
-          // (every part has its place but those of an offset table that is not ascending)
-          const bool held = at >= 0 && at + static_cast<int64_t>(n - 1) * n_rt < a.part_items;
-          float m = -__builtin_inff(), l = 0.0f;
-          for (int v = 0; v < (held ? n : 0); ++v) {
-            const float2 y = *reinterpret_cast<const float2*>(p + static_cast<int64_t>(v) * n_rt * (2 * S::kRows));
-            const float top = fmaxf(m, y.x), sub = top == -__builtin_inff() ? 0.0f : top;
-            l = l * __builtin_amdgcn_exp2f(m - sub) + y.y * __builtin_amdgcn_exp2f(y.x - sub);
-            m = top;
-          }
-          row_m[i] = m == -__builtin_inff() ? 0.0f : m;
-          row_inv[i] = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+        for (int u = 0; u < kInfoRows / kThreads; ++u) {
+          const int i = u * kThreads + tid;
+          const float2 y = stats[min(info0 + i, rows - 1)];
+          row_m[i] = y.x;
+          row_inv[i] = y.y;
         }
       }
       if (t + 2 < t1) wait_copies<2 * kCopies>();  // tile t has landed
@@ -503,7 +542,7 @@ __global__ __launch_bounds__(kThreads) void key_sums_kernel(WeightArgs a) {
 #pragma unroll
         for (int n = 0; n < 2; ++n)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) p[n][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][4 * r4 + e], a.scale_log2, -m[e])) * inv[e];
+          for (int e = 0; e < 4; ++e) p[n][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][4 * r4 + e], a.scale_log2, -m[e]));
         if (masked) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
@@ -513,7 +552,9 @@ __global__ __launch_bounds__(kThreads) void key_sums_kernel(WeightArgs a) {
           }
         }
 #pragma unroll
-        for (int n = 0; n < 2; ++n) tile_sum[n] += (p[n][0] + p[n][1]) + (p[n][2] + p[n][3]);
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) tile_sum[n] = __builtin_fmaf(p[n][e], inv[e], tile_sum[n]);
       }
 #pragma unroll
       for (int n = 0; n < 2; ++n) sum[n] += tile_sum[n];
@@ -558,7 +599,7 @@ __global__ __launch_bounds__(kSumKeys) void key_sums_join_kernel(WeightArgs a) {
 struct Plan {
   bool few, may_cut;
   int stats_items, sums_items;
-  int64_t part_items, part_bytes, bytes;
+  int64_t part_items, part_bytes, stats_bytes, bytes;
 };
 Plan plan_of(int64_t requests, int64_t tokens, int group, int kv_heads, int max_rows) {
   Plan p;
@@ -571,7 +612,8 @@ Plan plan_of(int64_t requests, int64_t tokens, int group, int kv_heads, int max_
   p.part_bytes = (p.part_items * rows * 8 + 15) / 16 * 16;
   // a range of row tiles is four at least, and a request without more is never cut
   p.may_cut = tokens * group > 4 * kSumRows;
-  p.bytes = p.part_bytes + (p.may_cut ? 2LL * p.sums_items * kSumKeys * 4 : 0);
+  p.stats_bytes = (kv_heads * tokens * group * 8 + 15) / 16 * 16;
+  p.bytes = p.part_bytes + p.stats_bytes + (p.may_cut ? 2LL * p.sums_items * kSumKeys * 4 : 0);
   return p;
 }
 
@@ -641,7 +683,8 @@ extern "C" int fd_paged_key_weights(const void* q, const fd_paged_cache* cache, 
   a.part_items = static_cast<int>(p.part_items);
   a.scale_log2 = scale * 1.4426950408889634f;
   a.part = static_cast<float*>(workspace);
-  a.sums = reinterpret_cast<float*>(static_cast<char*>(workspace) + p.part_bytes);
+  a.stats = reinterpret_cast<float*>(static_cast<char*>(workspace) + p.part_bytes);
+  a.sums = reinterpret_cast<float*>(static_cast<char*>(workspace) + p.part_bytes + p.stats_bytes);
   hipStream_t s = static_cast<hipStream_t>(stream);
   // workgroups: no more than the sizes can make items
   const int64_t key_tiles = static_cast<int64_t>(requests) * cache->kv_heads *
@@ -656,7 +699,8 @@ extern "C" int fd_paged_key_weights(const void* q, const fd_paged_cache* cache, 
     auto go = [&](auto kind) {
       using S = decltype(kind);
       hipLaunchKernelGGL((row_stats_kernel<D, F, S>), dim3(stats_grid), dim3(kThreads), 0, s, a);
-      hipLaunchKernelGGL((key_sums_kernel<D, F, S>), dim3(sums_grid), dim3(kThreads), 0, s, a);
+      hipLaunchKernelGGL((row_stats_join_kernel<S>), dim3(static_cast<unsigned>(std::min<int64_t>(p.part_items - p.stats_items, 1024))), dim3(kJoinThreads<S>), 0, s, a);
+      hipLaunchKernelGGL((key_sums_kernel<D, F>), dim3(sums_grid), dim3(kThreads), 0, s, a);
     };
     if (p.few) go(Few<D>{});
     else go(Many<D>{});
