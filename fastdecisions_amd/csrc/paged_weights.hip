@@ -49,15 +49,18 @@ struct Stats {
   static constexpr int kSubs = KW > 1 || D == 256 ? 1 : D == 128 ? 2 : 4;  // blocks of 32 keys of a wavefront and tile
   static constexpr int kKeys = 32 * KW * kSubs;
   static constexpr int kTileBytes = kKeys * D * 2;
-  static constexpr int kRing = kTileBytes >= 32768 ? 2 : 3;
+  static constexpr int kRing = 4;
+  // how far ahead of its products a tile is there: its first operands are read a block of keys before
+  static constexpr int kEarly = kSubs == 1 ? 1 : 0;
+  static constexpr int kPerCu = kRing * kTileBytes > 80 * 1024 ? 1 : 2;
 };
 template <int D>
 using Few = Stats<D, 1, 1>;
 template <int D>
 using Many = Stats<D, 4, 2>;
 
-// Key sums: every wavefront holds 64 keys; rows stream by in tiles of 32 through a ring of four.
-constexpr int kSumKeys = 64 * kWaves, kSumRows = 32, kSumRing = 4;
+// Key sums: every wavefront holds 64 keys; rows stream by in tiles of 32 through a ring of eight.
+constexpr int kSumKeys = 64 * kWaves, kSumRows = 32, kSumRing = 8;
 constexpr int kInfoRows = 1024;  // rows whose maxima and denominators are in LDS at a time
 
 // One request's part of the call: the rows that count, and the keys.
@@ -197,12 +200,20 @@ template <int N>
 __device__ __forceinline__ void wait_copies() {
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
+// The compiler's own loads of these end here: a wait of its own for them inside the loops would be one for the copies.
+template <int N, int M>
+__device__ __forceinline__ void loaded(bf16x8_t (&x)[N][M]) {
+#pragma unroll
+  for (int n = 0; n < N; ++n)
+#pragma unroll
+    for (int m = 0; m < M; ++m) asm volatile("" : "+v"(x[n][m]));
+}
 __device__ __forceinline__ uint32_t lds_address(const void* p) {
   return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) void*)p));
 }
 
 template <int D, Format F, class S>
-__global__ __launch_bounds__(kThreads) void row_stats_kernel(WeightArgs a) {
+__global__ __launch_bounds__(kThreads, S::kPerCu) void row_stats_kernel(WeightArgs a) {
   constexpr int kSteps = D / 16, NB = S::NB, R = S::kRing;
   constexpr int kRowBytes = F == kBf16 ? 2 * D : F == kE4m3 ? D : D / 2;
   constexpr int kMoves = S::kKeys * kRowBytes / 16 / kThreads;      // 16-byte moves of a thread and tile
@@ -268,11 +279,33 @@ __global__ __launch_bounds__(kThreads) void row_stats_kernel(WeightArgs a) {
         }
       }
     };
+    // Tile t + 1 (+ kEarly) is there for every wavefront, and tile t - 1 is read, whose stage is the next move's.
+    constexpr int E = S::kEarly;
+    auto advance = [&](int t) {
+      if constexpr (F == kBf16) {
+        if (E == 0 && t + 2 < nt) wait_copies<kMoves>();
+        else wait_copies<0>();
+        __syncthreads();
+        if (t + 3 < nt) move(t + 3);
+      } else {
+        __syncthreads();
+        if (t + 2 + E < nt) store(t + 2 + E);
+        if (t + 3 + E < nt) move(t + 3 + E);
+      }
+    };
     __syncthreads();  // the item before has read its tiles
-    if (nt > 0) {
-      move(0);
-      if constexpr (F != kBf16) store(0);
-      if (nt > 1) move(1);
+    if constexpr (F == kBf16) {
+#pragma unroll
+      for (int u = 0; u < 3; ++u)
+        if (u < nt) move(u);
+    } else {
+#pragma unroll
+      for (int u = 0; u < 2 + E; ++u) {
+        if (u >= nt) continue;
+        move(u);
+        store(u);
+      }
+      if (nt > 2 + E) move(2 + E);
     }
 
     int pos[NB];
@@ -285,67 +318,150 @@ __global__ __launch_bounds__(kThreads) void row_stats_kernel(WeightArgs a) {
 #pragma unroll
       for (int kk = 0; kk < kSteps; ++kk) qf[n][kk] = *reinterpret_cast<const bf16x8_t*>(q + chunk_of<D>(kk, half) * 8);
     }
-    const int pos_min = uniform(x.len - x.n_new + min(row0 + rw * NB * 32, rows - 1) / a.group);
+    loaded(qf);
     float m_run[NB], l_run[NB];
 #pragma unroll
     for (int n = 0; n < NB; ++n) m_run[n] = -__builtin_inff(), l_run[n] = 0.0f;
 
-    for (int t = 0; t < nt; ++t) {
-      if constexpr (F == kBf16) {
-        if (R > 2 && t + 1 < nt) wait_copies<kMoves>();  // tile t has landed, tile t + 1 may be on its way
-        else wait_copies<0>();
-        __syncthreads();  // and the tile before is read, whose stage is the next copy's
-        if (R > 2 && t + 2 < nt) move(t + 2);
-        if (R == 2 && t > 0 && t + 1 < nt) move(t + 1);
-      } else {
-        __syncthreads();  // tile t is stored, the one before is read
-        if (t + 1 < nt) store(t + 1);
-        if (t + 2 < nt) move(t + 2);
+    // ---- blocks of 32 keys, S::kSubs per tile
+    constexpr int kAhead = 4, kSlots = NB * kSteps, kScores = 16 * NB, kPer = kScores >= kSlots ? kScores / kSlots : 1;
+    static_assert(kScores % kSlots == 0 || kSlots % kScores == 0, "scores per product");
+    auto operand = [&](int block, int kk) {
+      const unsigned char* const tile = smem + ((block / S::kSubs) & (R - 1)) * S::kTileBytes;
+      return *reinterpret_cast<const bf16x8_t*>(tile + place<D>((kw * S::kSubs + block % S::kSubs) * 32 + col, chunk_of<D>(kk, half)));
+    };
+    f32x4_t sums[NB];  // four side by side: a chain of 16 additions would take as long as the block's products
+    float m_sub[NB];
+    auto begin = [&]() {
+#pragma unroll
+      for (int n = 0; n < NB; ++n) sums[n] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f}, m_sub[n] = m_run[n];
+    };
+    auto score = [&](int i, const f32x16_t (&s)[NB]) {
+      const int n = i % NB, r = i / NB;
+      float y = sums[n][r & 3] + __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][r], a.scale_log2, -m_sub[n]));
+      asm volatile("" : "+v"(y));  // computed here, not sunk towards the block's end
+      sums[n][r & 3] = y;
+    };
+    // A row's maximum may lag: its exponentials are summed as they are while they stay far from fp32's end, which their sum
+    // shows.  Only a row's first keys, and keys 2^64 above its maximum, take the maximum first.
+    auto finish = [&](const f32x16_t (&s)[NB]) {
+#pragma unroll
+      for (int n = 0; n < NB; ++n) {
+        float sum = (sums[n][0] + sums[n][1]) + (sums[n][2] + sums[n][3]);
+        if (__builtin_amdgcn_ballot_w64(!(sum < 0x1p64f)) != 0) {
+          float mx = s[n][0];
+#pragma unroll
+          for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[n][r]);
+          mx = half_max(mx) * a.scale_log2;
+          const float m_new = fmaxf(m_run[n], mx), sub = m_new == -__builtin_inff() ? 0.0f : m_new;
+          l_run[n] *= m_new == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(m_run[n] - m_new);
+          m_run[n] = m_new;
+          sum = 0.0f;
+#pragma unroll
+          for (int r = 0; r < 16; ++r) sum += __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][r], a.scale_log2, -sub));
+        }
+        l_run[n] += sum;
       }
-      const unsigned char* const tile = smem + (t % R) * S::kTileBytes;
+    };
+    auto softmax = [&](const f32x16_t (&s)[NB]) {
+      begin();
 #pragma unroll
+      for (int i = 0; i < kScores; ++i) score(i, s);
+      finish(s);
+    };
+    auto products = [&](int block, f32x16_t (&s)[NB]) {
+#pragma unroll
+      for (int n = 0; n < NB; ++n) s[n] = f32x16_t{};
+#pragma unroll
+      for (int kk = 0; kk < kSteps; ++kk) {
+        const bf16x8_t kf = operand(block, kk);
+#pragma unroll
+        for (int n = 0; n < NB; ++n) s[n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qf[n][kk], s[n], 0, 0, 0);
+      }
+    };
+    if (F == kBf16) wait_copies<0>();
+    __syncthreads();
+    // tiles [0, n_full) are seen whole by every row
+    const int pos_first = x.len - x.n_new + row0 / a.group;
+    const int n_full = uniform(absent ? 0 : max(0, min(nt, (pos_first + 1 - key0) / S::kKeys)));
+    if (n_full > 0) {
+      // Products of a block between the exponentials of the one before: wavefronts of a SIMD would run the same phase side by
+      // side, one unit idle at a time.
+      f32x16_t sA[NB], sB[NB];
+      bf16x8_t kf[kAhead];
+      products(0, sA);
+#pragma unroll
+      for (int kk = 0; kk < kAhead; ++kk) kf[kk] = operand(1, kk);  // (of a last block: unused)
+      auto step = [&](int block, f32x16_t (&sc)[NB], f32x16_t (&sn)[NB]) {  // softmax of `block`, products of the next one
+        begin();
+#pragma unroll
+        for (int n = 0; n < NB; ++n) sn[n] = f32x16_t{};
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int slot = 0; slot < kSlots; ++slot) {
+          const int kk = slot / NB, n = slot % NB;
+#pragma unroll
+          for (int i = 0; i < kPer; ++i)
+            if (kScores >= kSlots || slot % (kSlots / kScores) == 0) score(kScores >= kSlots ? slot * kPer + i : slot / (kSlots / kScores), sc);
+          sn[n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[kk % kAhead], qf[n][kk], sn[n], 0, 0, 0);
+          if (n == NB - 1) kf[kk % kAhead] = kk + kAhead < kSteps ? operand(block + 1, kk + kAhead) : operand(block + 2, kk + kAhead - kSteps);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        finish(sc);
+      };
+      if constexpr (S::kSubs > 1) {
+#pragma unroll 1
+        for (int t = 0; t + 1 < n_full; ++t) {
+          advance(t);
+#pragma unroll
+          for (int sub = 0; sub < S::kSubs; sub += 2) {
+            step(t * S::kSubs + sub, sA, sB);
+            step(t * S::kSubs + sub + 1, sB, sA);
+          }
+        }
+        advance(n_full - 1);
+#pragma unroll
+        for (int sub = 0; sub < S::kSubs; sub += 2) {
+          step((n_full - 1) * S::kSubs + sub, sA, sB);
+          if (sub + 2 < S::kSubs) step((n_full - 1) * S::kSubs + sub + 1, sB, sA);
+        }
+        softmax(sB);
+      } else {
+        int t = 0;
+#pragma unroll 1
+        for (; t + 2 < n_full; t += 2) {
+          advance(t);
+          step(t, sA, sB);
+          advance(t + 1);
+          step(t + 1, sB, sA);
+        }
+        if (t + 1 < n_full) {
+          advance(t);
+          step(t, sA, sB);
+#pragma unroll
+          for (int n = 0; n < NB; ++n) sA[n] = sB[n];
+        }
+        advance(n_full - 1);
+        softmax(sA);
+      }
+    }
+#pragma unroll 1
+    for (int t = n_full; t < nt; ++t) {
+      advance(t);
+#pragma unroll 1
       for (int sub = 0; sub < S::kSubs; ++sub) {
-        const int first = (kw * S::kSubs + sub) * 32, kb0 = key0 + t * S::kKeys + first;
+        const int kb0 = key0 + t * S::kKeys + (kw * S::kSubs + sub) * 32;
         f32x16_t s[NB];
+        products(t * S::kSubs + sub, s);
 #pragma unroll
-        for (int n = 0; n < NB; ++n) s[n] = f32x16_t{};
+        for (int r = 0; r < 16; ++r) {
+          const int key = kb0 + 8 * (r >> 2) + 4 * half + (r & 3);
+          const bool there = !absent || on_a_page(a, table, max(min(key, kend - 1), 0));
 #pragma unroll
-        for (int kk = 0; kk < kSteps; ++kk) {
-          const bf16x8_t kf = *reinterpret_cast<const bf16x8_t*>(tile + place<D>(first + col, chunk_of<D>(kk, half)));
-#pragma unroll
-          for (int n = 0; n < NB; ++n) s[n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qf[n][kk], s[n], 0, 0, 0);
+          for (int n = 0; n < NB; ++n)
+            if (key > pos[n] || !there) s[n][r] = -__builtin_inff();
         }
-        if (kb0 + 31 > pos_min || absent) {
-#pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const int key = kb0 + 8 * (r >> 2) + 4 * half + (r & 3);
-            const bool there = !absent || on_a_page(a, table, max(min(key, kend - 1), 0));
-#pragma unroll
-            for (int n = 0; n < NB; ++n)
-              if (key > pos[n] || !there) s[n][r] = -__builtin_inff();
-          }
-        }
-#pragma unroll
-        for (int n = 0; n < NB; ++n) {
-          // A row's maximum may lag: its exponentials are summed as they are while they stay far from fp32's end, which
-          // their sum shows.  Only a row's first keys, and keys 2^64 above its maximum, take the maximum first.
-          float sum = 0.0f;
-#pragma unroll
-          for (int r = 0; r < 16; ++r) sum += __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][r], a.scale_log2, -m_run[n]));
-          if (__builtin_amdgcn_ballot_w64(!(sum < 0x1p64f)) != 0) {
-            float mx = s[n][0];
-#pragma unroll
-            for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[n][r]);
-            mx = half_max(mx) * a.scale_log2;
-            const float m_new = fmaxf(m_run[n], mx), m_sub = m_new == -__builtin_inff() ? 0.0f : m_new;
-            l_run[n] *= m_new == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(m_run[n] - m_new);
-            m_run[n] = m_new;
-            sum = 0.0f;
-#pragma unroll
-            for (int r = 0; r < 16; ++r) sum += __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][r], a.scale_log2, -m_sub));
-          }
-          l_run[n] += sum;
-        }
+        softmax(s);
       }
     }
 
@@ -437,7 +553,7 @@ __device__ __forceinline__ int first_row(const WeightArgs& a, const Req& x, int 
 }
 
 template <int D, Format F>
-__global__ __launch_bounds__(kThreads) void key_sums_kernel(WeightArgs a) {
+__global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void key_sums_kernel(WeightArgs a) {
   constexpr int CR = D / 8, kSteps = D / 16, kTile = kSumRows * CR * 16, kCopies = kTile / 1024 / kWaves;
   constexpr int kRowBytes = F == kBf16 ? 2 * D : F == kE4m3 ? D : D / 2, kWords = kRowBytes / 32;  // of a lane's half row
   static_assert(kCopies >= 1, "a tile gives every wavefront a copy");
@@ -463,7 +579,7 @@ __global__ __launch_bounds__(kThreads) void key_sums_kernel(WeightArgs a) {
     const int32_t* const table = a.c.table + req * a.c.table_stride;
     const float2* const stats = reinterpret_cast<const float2*>(a.stats) + stat_row(a, x, req, head);
 
-    // ---- rows: tile t's are copied to stage t % kSumRing; rows behind the last one repeat it (the mask discards them)
+    // ---- rows: tile t's to stage t % kSumRing; rows behind the last one repeat it (the mask discards them)
     const int step_tokens = uniform(kSumRows / a.group), step_rem = kSumRows - step_tokens * a.group;
     int copy_token = uniform(t0 * kSumRows / a.group), copy_rem = t0 * kSumRows - copy_token * a.group;  // of the next copy
     auto token_in = [&](int rem, int r) { return static_cast<int>((static_cast<uint32_t>(rem + r) * a.group_magic) >> 24); };
@@ -473,7 +589,7 @@ __global__ __launch_bounds__(kThreads) void key_sums_kernel(WeightArgs a) {
         const int at = (i * kWaves + wave) * 64 + lane, r = at / CR, row = min(r, rows - 1 - t * kSumRows);
         const int token = token_in(copy_rem, row);
         lane_to_lds(q_row(a, x, req, head, copy_token + token, copy_rem + row - token * a.group) + ((at % CR) ^ (r & 7)) * 8,
-                    lds0 + static_cast<uint32_t>((t % kSumRing) * kTile + (i * kWaves + wave) * 1024));
+                    lds0 + static_cast<uint32_t>((t & (kSumRing - 1)) * kTile + (i * kWaves + wave) * 1024));
       }
       copy_token += step_tokens, copy_rem += step_rem;
       if (copy_rem >= a.group) copy_token += 1, copy_rem -= a.group;
@@ -502,65 +618,141 @@ __global__ __launch_bounds__(kThreads) void key_sums_kernel(WeightArgs a) {
       }
     }
 
+    loaded(kf);
     float sum[2] = {0.0f, 0.0f};
     int info0 = -1;  // first row of those in row_m
-    int token0 = uniform(t0 * kSumRows / a.group), rem0 = t0 * kSumRows - token0 * a.group;  // of tile t's first row
-    for (int t = t0; t < t1; ++t) {
-      const int row0 = t * kSumRows;
-      if (info0 < 0 || row0 >= info0 + kInfoRows) {
-        __syncthreads();  // the rows before are done with theirs
-        info0 = row0;
+    auto info = [&](int row0) {
+      if (info0 >= 0 && row0 < info0 + kInfoRows) return;
+      __syncthreads();  // the rows before are done with theirs
+      info0 = row0;
 #pragma unroll
-        for (int u = 0; u < kInfoRows / kThreads; ++u) {
-          const int i = u * kThreads + tid;
-          const float2 y = stats[min(info0 + i, rows - 1)];
-          row_m[i] = y.x;
-          row_inv[i] = y.y;
-        }
+      for (int u = 0; u < kInfoRows / kThreads; ++u) {
+        const int i = u * kThreads + tid;
+        const float2 y = stats[min(info0 + i, rows - 1)];
+        row_m[i] = y.x;
+        row_inv[i] = y.y;
       }
-      if (t + 2 < t1) wait_copies<2 * kCopies>();  // tile t has landed
+      __syncthreads();
+    };
+    auto operand = [&](int t, int kk) {
+      return *reinterpret_cast<const bf16x8_t*>(smem + (t & (kSumRing - 1)) * kTile + place<D>(col, chunk_of<D>(kk, half)));
+    };
+    // Tile t + 2 has landed for every wavefront (tile t + 1 at its first operands' reads), and tile t - 1 is read, whose
+    // stage is the next copy's.
+    auto advance = [&](int t) {
+      if (t + 6 < t1) wait_copies<4 * kCopies>();
+      else if (t + 4 < t1) wait_copies<2 * kCopies>();
       else wait_copies<0>();
       __syncthreads();
       if (t + kSumRing - 1 < t1) copy(t + kSumRing - 1);
-      const unsigned char* const tile = smem + (t % kSumRing) * kTile;
-      f32x16_t s[2] = {f32x16_t{}, f32x16_t{}};
+    };
+    // Scores one by one: exp(score - m) / l of row 8 r4 + 4 half + e and key block n, into four sums per block side by
+    // side (a chain of 16 additions would take as long as the tile's products).
+    f32x4_t tile_sum[2], mv[2], iv[2];
+    const float *m_at = row_m, *inv_at = row_inv;
+    auto score = [&](int i, const f32x16_t (&s)[2], auto last_of) {
+      const int r4 = i / 8, e = (i / 2) % 4, n = i % 2;
+      if (i % 8 == 0 && r4 < 3) {
+        mv[(r4 + 1) & 1] = *static_cast<const f32x4_t*>(__builtin_assume_aligned(m_at + 8 * (r4 + 1), 16));
+        iv[(r4 + 1) & 1] = *static_cast<const f32x4_t*>(__builtin_assume_aligned(inv_at + 8 * (r4 + 1), 16));
+      }
+      float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][4 * r4 + e], a.scale_log2, -mv[r4 & 1][e]));
+      p = last_of(8 * r4 + 4 * half + e, n) ? p : 0.0f;
+      float y = __builtin_fmaf(p, iv[r4 & 1][e], tile_sum[n][e]);
+      asm volatile("" : "+v"(y));  // computed here, not sunk towards the tile's end
+      tile_sum[n][e] = y;
+    };
+    auto begin = [&](int t) {
+      m_at = row_m + (t * kSumRows - info0) + 4 * half;
+      inv_at = row_inv + (t * kSumRows - info0) + 4 * half;
+      mv[0] = *static_cast<const f32x4_t*>(__builtin_assume_aligned(m_at, 16));
+      iv[0] = *static_cast<const f32x4_t*>(__builtin_assume_aligned(inv_at, 16));
+      tile_sum[0] = tile_sum[1] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    };
+    auto finish = [&]() {
+#pragma unroll
+      for (int n = 0; n < 2; ++n) sum[n] += (tile_sum[n][0] + tile_sum[n][1]) + (tile_sum[n][2] + tile_sum[n][3]);
+    };
+    auto always = [](int, int) { return true; };
+    auto products = [&](int t, f32x16_t (&s)[2]) {
+      s[0] = s[1] = f32x16_t{};
 #pragma unroll
       for (int kk = 0; kk < kSteps; ++kk) {
-        const bf16x8_t qf = *reinterpret_cast<const bf16x8_t*>(tile + place<D>(col, chunk_of<D>(kk, half)));
+        const bf16x8_t qf = operand(t, kk);
 #pragma unroll
         for (int n = 0; n < 2; ++n) s[n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(qf, kf[n][kk], s[n], 0, 0, 0);
       }
-      const int limit = x.len - x.n_new + token0;  // last key that the tile's first row sees
-      const bool masked = limit < key0 + wave * 64 + 63 || row0 + kSumRows > rows;
-      float tile_sum[2] = {0.0f, 0.0f};
+    };
+    // A tile with rows that do not see every key, or rows behind the last one.
+    auto masked_tile = [&](int t) {
+      f32x16_t s[2];
+      advance(t);
+      info(t * kSumRows);
+      products(t, s);
+      const int row0 = t * kSumRows, token0 = row0 / a.group, rem0 = row0 - token0 * a.group;
+      int last = -1;  // key that the row sees
+      begin(t);
 #pragma unroll
-      for (int r4 = 0; r4 < 4; ++r4) {
-        const int row = 8 * r4 + 4 * half;
-        const f32x4_t m = *reinterpret_cast<const f32x4_t*>(&row_m[row0 - info0 + row]);
-        const f32x4_t inv = *reinterpret_cast<const f32x4_t*>(&row_inv[row0 - info0 + row]);
-        float p[2][4];
+      for (int i = 0; i < 32; ++i)
+        score(i, s, [&](int r, int n) {
+          if (n == 0) last = row0 + r < rows ? x.len - x.n_new + token0 + token_in(rem0, r) : -1;
+          return key[n] <= last;
+        });
+      finish();
+    };
+    wait_copies<0>();
+    __syncthreads();
+    // tiles [t0, whole) are masked, tiles [whole, whole_end) are not, the last one again where its rows end within
+    const int whole = uniform(min(max(over(first_row(a, x, min(key0 + kSumKeys, x.len) - 1), kSumRows), t0), t1));
+    const int whole_end = uniform(max(whole, min(t1, rows / kSumRows)));
+#pragma unroll 1
+    for (int t = t0; t < whole; ++t) masked_tile(t);
+    if (whole < whole_end) {
+      // Products of tile t + 1 between the exponentials of tile t: two wavefronts of a SIMD would run the same phase side by
+      // side, one unit idle at a time.
+      constexpr int kAhead = 4, kSlots = 2 * kSteps, kPer = 32 / kSlots;
+      static_assert(32 % kSlots == 0, "scores per product");
+      f32x16_t sA[2], sB[2];
+      bf16x8_t qf[kAhead];
+      products(whole, sA);
 #pragma unroll
-        for (int n = 0; n < 2; ++n)
+      for (int kk = 0; kk < kAhead; ++kk) qf[kk] = operand(whole + 1, kk);  // (behind the last tile: unused)
+      auto step = [&](int t, f32x16_t (&sc)[2], f32x16_t (&sn)[2]) {
+        advance(t);
+        info(t * kSumRows);
+        begin(t);
+        sn[0] = sn[1] = f32x16_t{};
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) p[n][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][4 * r4 + e], a.scale_log2, -m[e]));
-        if (masked) {
+        for (int slot = 0; slot < kSlots; ++slot) {
+          const int kk = slot / 2, n = slot % 2;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int last = row0 + row + e < rows ? limit + token_in(rem0, row + e) : -1;
-#pragma unroll
-            for (int n = 0; n < 2; ++n) p[n][e] = key[n] <= last ? p[n][e] : 0.0f;
-          }
+          for (int i = 0; i < kPer; ++i) score(slot * kPer + i, sc, always);
+          sn[n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(qf[kk % kAhead], kf[n][kk], sn[n], 0, 0, 0);
+          if (n == 1) qf[kk % kAhead] = kk + kAhead < kSteps ? operand(t + 1, kk + kAhead) : operand(t + 2, kk + kAhead - kSteps);
+          __builtin_amdgcn_sched_barrier(0);
         }
-#pragma unroll
-        for (int n = 0; n < 2; ++n)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) tile_sum[n] = __builtin_fmaf(p[n][e], inv[e], tile_sum[n]);
+        finish();
+      };
+      int t = whole;
+#pragma unroll 1
+      for (; t + 2 < whole_end; t += 2) {
+        step(t, sA, sB);
+        step(t + 1, sB, sA);
       }
+      if (t + 1 < whole_end) {
+        step(t, sA, sB);
+        sA[0] = sB[0], sA[1] = sB[1];
+      }
+      advance(whole_end - 1);
+      info((whole_end - 1) * kSumRows);
+      begin(whole_end - 1);
 #pragma unroll
-      for (int n = 0; n < 2; ++n) sum[n] += tile_sum[n];
-      token0 += step_tokens, rem0 += step_rem;
-      if (rem0 >= a.group) token0 += 1, rem0 -= a.group;
+      for (int i = 0; i < 32; ++i) score(i, sA, always);
+      finish();
     }
+#pragma unroll 1
+    for (int t = whole_end; t < t1; ++t) masked_tile(t);
     int at = 0;
     if (n_ranges > 1) at = uniform(items_before(a, lane, req, [&](const Req& y) { return cut.places(a, y); })) + k;
     if (at < 0 || at >= 2 * a.sums_items) continue;  // only of an offset table that is not ascending
