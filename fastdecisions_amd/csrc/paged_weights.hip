@@ -22,6 +22,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWaves = 4;
+constexpr int kCus = 256;
 
 struct WeightArgs {
   PagedView c;                  // K alone
@@ -34,30 +35,26 @@ struct WeightArgs {
   int n_req, seq_len, group, kv_heads, last, w_rows;
   uint32_t group_magic;         // ceil(2^24 / group)
   float scale_log2;
-  int stats_items, sums_items;  // items that each kernel cuts its work into, about
+  int stats_items, sums_items;  // items that each kernel cuts its work into at most, but for one per tile that stays
+  int slots;                    // workgroups that run at once
   int part_items;               // items of the row stats whose places the workspace holds
   float* part;                  // per item of the row stats: its rows' (m, l)
   float* stats;                 // [heads, tokens of the call x group]: (m, 1 / l) of every row over all its keys
   float* sums;                  // per item of the key sums of a request cut into row ranges: its keys' sums
 };
 
-// Row stats: RW row wavefronts of NB blocks of 32 rows, times 4 / RW key parts of a tile; a ring of kRing tiles.
-template <int D_, int RW_, int NB_>
+// Row stats: a wavefront holds two blocks of 32 rows; keys stream by through a ring of tiles.
+template <int D_>
 struct Stats {
-  static constexpr int D = D_, RW = RW_, NB = NB_, KW = kWaves / RW;
-  static constexpr int kRows = 32 * RW * NB;
-  static constexpr int kSubs = KW > 1 || D == 256 ? 1 : D == 128 ? 2 : 4;  // blocks of 32 keys of a wavefront and tile
-  static constexpr int kKeys = 32 * KW * kSubs;
+  static constexpr int D = D_, NB = 2;
+  static constexpr int kRows = 32 * NB * kWaves;
+  static constexpr int kSubs = D == 256 ? 1 : D == 128 ? 2 : 4;  // blocks of 32 keys of a tile
+  static constexpr int kKeys = 32 * kSubs;
   static constexpr int kTileBytes = kKeys * D * 2;
   static constexpr int kRing = 4;
   // how far ahead of its products a tile is there: its first operands are read a block of keys before
   static constexpr int kEarly = kSubs == 1 ? 1 : 0;
-  static constexpr int kPerCu = kRing * kTileBytes > 80 * 1024 ? 1 : 2;
 };
-template <int D>
-using Few = Stats<D, 1, 1>;
-template <int D>
-using Many = Stats<D, 4, 2>;
 
 // Key sums: every wavefront holds 64 keys; rows stream by in tiles of 32 through a ring of eight.
 constexpr int kSumKeys = 64 * kWaves, kSumRows = 32, kSumRing = 8;
@@ -87,13 +84,38 @@ __device__ __forceinline__ int64_t wave_total(int64_t v) {
   return v;
 }
 
-// The share of one item when all key heads' pairs of tiles (pairs(request) of each) are cut into about `items`.
-template <typename Pairs>
-__device__ __forceinline__ int share_of(const WeightArgs& a, int lane, int items, int least, Pairs pairs) {
-  int64_t work = 0;
-  for (int r0 = 0; r0 < a.n_req; r0 += 64) work += pairs(request(a, r0 + lane));
-  work = wave_total(work) * a.kv_heads;
-  return uniform(static_cast<int>(min(max((work + items - 1) / items, static_cast<int64_t>(least)), static_cast<int64_t>(1 << 25))));
+// What a kernel's cut needs of a request: pairs of tiles of a key head, those of them that are seen (about), and the tiles
+// of the operand that stays, each of which wastes half a range or so.
+struct Size {
+  int64_t pairs;
+  float seen, stays;
+};
+// Streamed tiles of an item.  Items that just fill m rounds of the workgroups that run at once take m (c + overhead) tiles of
+// time, and the best of a few m is taken; a few items more than workgroups would cost a whole round.  `items` bounds them
+// whatever the estimate: no more than that many places (and one per tile that stays) are needed.
+template <typename SizeOf>
+__device__ __forceinline__ int tiles_of_item(const WeightArgs& a, int lane, int items, int least, int overhead, SizeOf size_of) {
+  constexpr int kRounds = 4;
+  Size all{0, 0.0f, 0.0f};
+  for (int r0 = 0; r0 < a.n_req; r0 += 64) {
+    const Req x = request(a, r0 + lane);
+    if (x.n_new == 0) continue;
+    const Size y = size_of(x);
+    all.pairs += y.pairs, all.seen += y.seen, all.stays += y.stays;
+  }
+  const int64_t pairs = wave_total(all.pairs) * a.kv_heads;
+  const float seen = fd_xor_sum_up<64>(all.seen) * static_cast<float>(a.kv_heads);
+  const float stays = fd_xor_sum_up<64>(all.stays) * static_cast<float>(a.kv_heads);
+  float best = 1e9f, cost = 1e30f;  // without room for any cut: whole
+#pragma unroll
+  for (int m = 1; m <= kRounds; ++m) {
+    const float room = static_cast<float>(m * a.slots) - 1.1f * stays;
+    if (room < 1.0f) continue;
+    const float c = ceilf(seen / room), now = static_cast<float>(m) * (c + static_cast<float>(overhead));
+    if (now < cost) best = c, cost = now;
+  }
+  const int64_t floor = max((pairs + items - 1) / items, static_cast<int64_t>(least));
+  return uniform(static_cast<int>(max(min(static_cast<int64_t>(best), static_cast<int64_t>(1 << 25)), min(floor, static_cast<int64_t>(1 << 25)))));
 }
 
 // Request that holds item `at` when request r has count(r) items: false if none does; *base: items before it.
@@ -128,8 +150,10 @@ template <class S>
 struct Cut {
   int c;  // key tiles of a range
   __device__ __forceinline__ Cut(const WeightArgs& a, int lane)
-      : c(share_of(a, lane, a.stats_items, 256 / S::kKeys, [&](const Req& x) {
-          return static_cast<int64_t>(over(x.n_new * a.group, S::kRows)) * over(x.len, S::kKeys);
+      : c(tiles_of_item(a, lane, a.stats_items, 256 / S::kKeys, 4, [&](const Req& x) {
+          const int rt = over(x.n_new * a.group, S::kRows), kt = over(x.len, S::kKeys);
+          const float mean = 0.5f * static_cast<float>(min(x.len, x.len - x.n_new + S::kRows / a.group) + x.len);
+          return Size{static_cast<int64_t>(rt) * kt, static_cast<float>(rt) * (mean / S::kKeys + 0.5f), static_cast<float>(rt)};
         })) {}
   __device__ __forceinline__ int rtiles(const WeightArgs& a, const Req& x) const { return over(x.n_new * a.group, S::kRows); }
   __device__ __forceinline__ int ranges(const Req& x) const { return max(over(over(x.len, S::kKeys), c), 1); }
@@ -212,8 +236,9 @@ __device__ __forceinline__ uint32_t lds_address(const void* p) {
   return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) void*)p));
 }
 
-template <int D, Format F, class S>
-__global__ __launch_bounds__(kThreads, S::kPerCu) void row_stats_kernel(WeightArgs a) {
+template <int D, Format F>
+__global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void row_stats_kernel(WeightArgs a) {
+  using S = Stats<D>;
   constexpr int kSteps = D / 16, NB = S::NB, R = S::kRing;
   constexpr int kRowBytes = F == kBf16 ? 2 * D : F == kE4m3 ? D : D / 2;
   constexpr int kMoves = S::kKeys * kRowBytes / 16 / kThreads;      // 16-byte moves of a thread and tile
@@ -221,7 +246,7 @@ __global__ __launch_bounds__(kThreads, S::kPerCu) void row_stats_kernel(WeightAr
   static_assert(kMoves >= 1, "a tile gives every thread a move");
   __shared__ __attribute__((aligned(1024))) unsigned char smem[R * S::kTileBytes];
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
-  const int rw = wave % S::RW, kw = wave / S::RW, col = lane & 31, half = lane >> 5;
+  const int col = lane & 31, half = lane >> 5;
   const uint32_t lds0 = lds_address(smem);
   const Cut<S> cut(a, lane);
   for (int item = blockIdx.x; item < a.part_items; item += gridDim.x) {
@@ -312,7 +337,7 @@ __global__ __launch_bounds__(kThreads, S::kPerCu) void row_stats_kernel(WeightAr
     bf16x8_t qf[NB][kSteps];
 #pragma unroll
     for (int n = 0; n < NB; ++n) {
-      const int row = min(row0 + (rw * NB + n) * 32 + col, rows - 1), token = row / a.group;
+      const int row = min(row0 + (wave * NB + n) * 32 + col, rows - 1), token = row / a.group;
       const uint16_t* const q = q_row(a, x, req, head, token, row - token * a.group);
       pos[n] = x.len - x.n_new + token;
 #pragma unroll
@@ -328,7 +353,7 @@ __global__ __launch_bounds__(kThreads, S::kPerCu) void row_stats_kernel(WeightAr
     static_assert(kScores % kSlots == 0 || kSlots % kScores == 0, "scores per product");
     auto operand = [&](int block, int kk) {
       const unsigned char* const tile = smem + ((block / S::kSubs) & (R - 1)) * S::kTileBytes;
-      return *reinterpret_cast<const bf16x8_t*>(tile + place<D>((kw * S::kSubs + block % S::kSubs) * 32 + col, chunk_of<D>(kk, half)));
+      return *reinterpret_cast<const bf16x8_t*>(tile + place<D>((block % S::kSubs) * 32 + col, chunk_of<D>(kk, half)));
     };
     f32x4_t sums[NB];  // four side by side: a chain of 16 additions would take as long as the block's products
     float m_sub[NB];
@@ -450,7 +475,7 @@ __global__ __launch_bounds__(kThreads, S::kPerCu) void row_stats_kernel(WeightAr
       advance(t);
 #pragma unroll 1
       for (int sub = 0; sub < S::kSubs; ++sub) {
-        const int kb0 = key0 + t * S::kKeys + (kw * S::kSubs + sub) * 32;
+        const int kb0 = key0 + t * S::kKeys + sub * 32;
         f32x16_t s[NB];
         products(t * S::kSubs + sub, s);
 #pragma unroll
@@ -466,27 +491,11 @@ __global__ __launch_bounds__(kThreads, S::kPerCu) void row_stats_kernel(WeightAr
     }
 
     float* const part = a.part + static_cast<int64_t>(item) * (2 * S::kRows);
-    if constexpr (S::KW > 1) __syncthreads();  // the tiles are read
 #pragma unroll
     for (int n = 0; n < NB; ++n) {
-      float m = m_run[n], l = half_sum(l_run[n]);
-      if constexpr (S::KW > 1) {  // the key parts of these rows
-        static_assert(NB == 1, "LDS is used once");
-        float* const ml = reinterpret_cast<float*>(smem);
-        if (half == 0) ml[(wave * 32 + col) * 2] = m, ml[(wave * 32 + col) * 2 + 1] = l;
-        __syncthreads();
-        if (wave == 0) {
-#pragma unroll
-          for (int v = 1; v < S::KW; ++v) {
-            const float m2 = ml[(v * 32 + col) * 2], l2 = ml[(v * 32 + col) * 2 + 1];
-            const float top = fmaxf(m, m2), sub = top == -__builtin_inff() ? 0.0f : top;
-            l = l * __builtin_amdgcn_exp2f(m - sub) + l2 * __builtin_amdgcn_exp2f(m2 - sub);
-            m = top;
-          }
-        }
-      }
-      const int row = (rw * NB + n) * 32 + col;
-      if (half != 0 || (S::KW > 1 && wave != 0) || row0 + row >= rows) continue;
+      const float m = m_run[n], l = half_sum(l_run[n]);
+      const int row = (wave * NB + n) * 32 + col;
+      if (half != 0 || row0 + row >= rows) continue;
       if (n_ranges == 1) {
         reinterpret_cast<float2*>(a.stats)[stat_row(a, x, req, head) + row0 + row] = stat_of(m, l);
       } else {
@@ -499,9 +508,7 @@ __global__ __launch_bounds__(kThreads, S::kPerCu) void row_stats_kernel(WeightAr
 
 // (m, 1 / l) of the rows whose keys were cut into ranges, one row tile per workgroup.
 template <class S>
-constexpr int kJoinThreads = S::kRows < 64 ? 64 : S::kRows;  // whole wavefronts
-template <class S>
-__global__ __launch_bounds__(kJoinThreads<S>) void row_stats_join_kernel(WeightArgs a) {
+__global__ __launch_bounds__(S::kRows) void row_stats_join_kernel(WeightArgs a) {
   const int lane = threadIdx.x & 63;
   const Cut<S> cut(a, lane);
   for (int item = blockIdx.x;; item += gridDim.x) {
@@ -514,7 +521,6 @@ __global__ __launch_bounds__(kJoinThreads<S>) void row_stats_join_kernel(WeightA
     const int n = over(over(seen_by(a, x, min(row0 + S::kRows, rows) - 1), S::kKeys), cut.c);  // ranges that a row sees
     if (first < 0 || first + static_cast<int64_t>(n_ranges - 1) * n_rt >= a.part_items) continue;  // only of an offset table that is not ascending
     const int row = threadIdx.x;
-    if (row >= S::kRows) continue;
     const float2* const p = reinterpret_cast<const float2*>(a.part) + static_cast<int64_t>(first) * S::kRows + row;
     float m = -__builtin_inff(), l = 0.0f;
     for (int v0 = 0; v0 < n; v0 += 4) {  // four loads in flight
@@ -537,8 +543,10 @@ __global__ __launch_bounds__(kJoinThreads<S>) void row_stats_join_kernel(WeightA
 struct SumCut {
   int c;
   __device__ __forceinline__ SumCut(const WeightArgs& a, int lane)
-      : c(share_of(a, lane, a.sums_items, 4, [&](const Req& x) {
-          return static_cast<int64_t>(over(x.n_new * a.group, kSumRows)) * over(x.len, kSumKeys);
+      : c(tiles_of_item(a, lane, a.sums_items, 4, 9, [&](const Req& x) {
+          const int rt = over(x.n_new * a.group, kSumRows), kt = over(x.len, kSumKeys);
+          const float fresh = 0.5f * static_cast<float>(x.n_new) / kSumKeys;  // half of the new tokens' keys are seen
+          return Size{static_cast<int64_t>(rt) * kt, static_cast<float>(rt) * (static_cast<float>(kt) - fresh), static_cast<float>(kt)};
         })) {}
   __device__ __forceinline__ int ktiles(const WeightArgs& a, const Req& x) const { return x.n_new > 0 ? over(x.len, kSumKeys) * a.kv_heads : 0; }
   __device__ __forceinline__ int ranges(const WeightArgs& a, const Req& x) const { return max(over(over(x.n_new * a.group, kSumRows), c), 1); }
@@ -789,16 +797,16 @@ __global__ __launch_bounds__(kSumKeys) void key_sums_join_kernel(WeightArgs a) {
 
 // The kernels of a call, and its items and workspace, whatever the lengths turn out to be.
 struct Plan {
-  bool few, may_cut;
-  int stats_items, sums_items;
+  bool may_cut;
+  int stats_items, sums_items, slots;
   int64_t part_items, part_bytes, stats_bytes, bytes;
 };
-Plan plan_of(int64_t requests, int64_t tokens, int group, int kv_heads, int max_rows) {
+Plan plan_of(int64_t requests, int64_t tokens, int group, int kv_heads, int head_dim) {
   Plan p;
-  p.few = max_rows <= 64;
-  const int rows = p.few ? Few<64>::kRows : Many<64>::kRows;
-  p.stats_items = 1024;
-  p.sums_items = 1024;
+  constexpr int rows = Stats<64>::kRows;
+  p.slots = kCus * (head_dim == 256 ? 1 : 2);
+  p.stats_items = 2048;
+  p.sums_items = 2048;
   // a share alone may add a range per row tile
   p.part_items = p.stats_items + kv_heads * (tokens * group / rows + requests);
   p.part_bytes = (p.part_items * rows * 8 + 15) / 16 * 16;
@@ -827,9 +835,7 @@ extern "C" int64_t fd_paged_key_weights_workspace_bytes(int batch, int q_heads, 
                                                         int max_seqlen, int last) {
   static const char* what = "fd_paged_key_weights_workspace_bytes";
   if (int rc = check_sizes(what, batch, q_heads, kv_heads, seq_len, n_seqs, max_seqlen, last)) return rc;
-  const int group = q_heads / kv_heads, top = last > 0 ? std::min(last, max_seqlen) : max_seqlen;
-  return plan_of(n_seqs > 0 ? n_seqs : batch, static_cast<int64_t>(batch) * seq_len, group, kv_heads,
-                 static_cast<int>(std::min<int64_t>(static_cast<int64_t>(top) * group, 1 << 30))).bytes;
+  return plan_of(n_seqs > 0 ? n_seqs : batch, static_cast<int64_t>(batch) * seq_len, q_heads / kv_heads, kv_heads, 64).bytes;
 }
 
 extern "C" int fd_paged_key_weights(const void* q, const fd_paged_cache* cache, float* weights, const int64_t q_strides[4],
@@ -850,9 +856,8 @@ extern "C" int fd_paged_key_weights(const void* q, const fd_paged_cache* cache, 
              "%s: the weights need a row for every request", what);
   FD_REQUIRE(weight_strides[0] >= 0 && weight_strides[1] >= 0, FD_ERR_INVALID_ARGUMENT, "%s: weight strides must be >= 0", what);
   if (requests == 0 || seq_len == 0) return FD_OK;
-  const int group = q_heads / cache->kv_heads, top = last > 0 ? std::min(last, max_seqlen) : max_seqlen;
-  const Plan p = plan_of(requests, static_cast<int64_t>(batch) * seq_len, group, cache->kv_heads,
-                         static_cast<int>(std::min<int64_t>(static_cast<int64_t>(top) * group, 1 << 30)));
+  const int group = q_heads / cache->kv_heads;
+  const Plan p = plan_of(requests, static_cast<int64_t>(batch) * seq_len, group, cache->kv_heads, cache->head_dim);
   FD_REQUIRE(p.part_items < (1LL << 31), FD_ERR_UNSUPPORTED, "%s: problem too large", what);
   FD_REQUIRE(workspace && fd_aligned16(workspace) && workspace_bytes >= p.bytes, FD_ERR_INVALID_ARGUMENT,
              "%s: the workspace must be 16-byte aligned and hold %lld bytes", what, static_cast<long long>(p.bytes));
@@ -872,6 +877,7 @@ extern "C" int fd_paged_key_weights(const void* q, const fd_paged_cache* cache, 
   a.group_magic = ((1u << 24) + group - 1) / group;
   a.stats_items = p.stats_items;
   a.sums_items = p.sums_items;
+  a.slots = p.slots;
   a.part_items = static_cast<int>(p.part_items);
   a.scale_log2 = scale * 1.4426950408889634f;
   a.part = static_cast<float*>(workspace);
@@ -888,14 +894,10 @@ extern "C" int fd_paged_key_weights(const void* q, const fd_paged_cache* cache, 
   by_kind(cache, [&](auto d, auto f) {
     constexpr int D = decltype(d)::value;
     constexpr Format F = decltype(f)::value;
-    auto go = [&](auto kind) {
-      using S = decltype(kind);
-      hipLaunchKernelGGL((row_stats_kernel<D, F, S>), dim3(stats_grid), dim3(kThreads), 0, s, a);
-      hipLaunchKernelGGL((row_stats_join_kernel<S>), dim3(static_cast<unsigned>(std::min<int64_t>(p.part_items - p.stats_items, 1024))), dim3(kJoinThreads<S>), 0, s, a);
-      hipLaunchKernelGGL((key_sums_kernel<D, F>), dim3(sums_grid), dim3(kThreads), 0, s, a);
-    };
-    if (p.few) go(Few<D>{});
-    else go(Many<D>{});
+    hipLaunchKernelGGL((row_stats_kernel<D, F>), dim3(stats_grid), dim3(kThreads), 0, s, a);
+    hipLaunchKernelGGL((row_stats_join_kernel<Stats<D>>), dim3(static_cast<unsigned>(std::min<int64_t>(p.part_items - p.stats_items, 1024))),
+                       dim3(Stats<D>::kRows), 0, s, a);
+    hipLaunchKernelGGL((key_sums_kernel<D, F>), dim3(sums_grid), dim3(kThreads), 0, s, a);
   });
   if (p.may_cut) hipLaunchKernelGGL(key_sums_join_kernel, dim3(join_grid), dim3(kSumKeys), 0, s, a);
   return fd_check_launch(what);
