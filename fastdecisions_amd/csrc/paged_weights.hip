@@ -273,26 +273,39 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void row_stats_kernel(W
     const int mask = (1 << a.c.shift) - 1, lrow = lane / kLanes, word = lane % kLanes;
     uint4 in[F == kBf16 ? 1 : kMoves];
     uint8_t in_scale[F == kBf16 ? 1 : kMoves];
-    auto move = [&](int t) {
+    const uint32_t lane_at = static_cast<uint32_t>(lrow) * static_cast<uint32_t>(a.c.row);
+    auto move = [&](int t) __attribute__((always_inline)) {
 #pragma unroll
       for (int i = 0; i < kMoves; ++i) {
         const int row = (i * kWaves + wave) * kMoveRows, first = key0 + t * S::kKeys + row;
-        int page = valid_page(a, scalar_load(table, uniform(min(first, kend - 1)) >> a.c.shift));
+        const int first_key = uniform(min(first, kend - 1));
+        int page = valid_page(a, scalar_load(table, first_key >> a.c.shift)), at;
+        const unsigned char* p;
         if constexpr (kMoveRows > 16) {
           const int second = valid_page(a, scalar_load(table, uniform(min(first + 16, kend - 1)) >> a.c.shift));
-          page = lrow < 16 ? page : second;
+          const int key = min(first + lrow, kend - 1);
+          page = (key >> a.c.shift) == (first_key >> a.c.shift) ? page : second;
+          at = key & mask;
+          p = base_k + page * a.c.page + at * a.c.row;
+        } else {
+          uint32_t lane_row = lane_at;
+          at = (first_key & mask) + lrow;
+          if (first + kMoveRows > kend) {
+            const int live = max(0, min(lrow, kend - 1 - first));
+            lane_row = static_cast<uint32_t>(live) * static_cast<uint32_t>(a.c.row);
+            at += live - lrow;
+          }
+          p = base_k + (page * a.c.page + (first_key & mask) * a.c.row) + lane_row;
         }
-        const int at = min(first + lrow, kend - 1) & mask;
-        const unsigned char* const p = base_k + page * a.c.page + at * a.c.row;
         if constexpr (F == kBf16) {
-          lane_to_lds(p + (word ^ ((row + lrow) & 7)) * 16, lds0 + static_cast<uint32_t>((t % R) * S::kTileBytes + (i * kWaves + wave) * 1024));
+          lane_to_lds(p + (word ^ ((row + lrow) & 7)) * 16, lds0 + static_cast<uint32_t>((t & (R - 1)) * S::kTileBytes + (i * kWaves + wave) * 1024));
         } else {
           in[i] = reinterpret_cast<const uint4*>(p)[word];
           in_scale[i] = scales_of<F, D>(a, page, head, at)[F == kE2m1 ? word : 0];
         }
       }
     };
-    auto store = [&](int t) {
+    auto store = [&](int t) __attribute__((always_inline)) {
       if constexpr (F != kBf16) {
 #pragma unroll
         for (int i = 0; i < kMoves; ++i) {
@@ -300,13 +313,13 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void row_stats_kernel(W
           decode<F>(in[i], scale_of(in_scale[i]), y);
 #pragma unroll
           for (int u = 0; u < kWordChunks<F>; ++u)
-            *reinterpret_cast<bf16x8_t*>(smem + (t % R) * S::kTileBytes + place<D>((i * kWaves + wave) * kMoveRows + lrow, word * kWordChunks<F> + u)) = y[u];
+            *reinterpret_cast<bf16x8_t*>(smem + (t & (R - 1)) * S::kTileBytes + place<D>((i * kWaves + wave) * kMoveRows + lrow, word * kWordChunks<F> + u)) = y[u];
         }
       }
     };
     // Tile t + 1 (+ kEarly) is there for every wavefront, and tile t - 1 is read, whose stage is the next move's.
     constexpr int E = S::kEarly;
-    auto advance = [&](int t) {
+    auto advance = [&](int t) __attribute__((always_inline)) {
       if constexpr (F == kBf16) {
         if (E == 0 && t + 2 < nt) wait_copies<kMoves>();
         else wait_copies<0>();
@@ -351,17 +364,17 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void row_stats_kernel(W
     // ---- blocks of 32 keys, S::kSubs per tile
     constexpr int kAhead = 4, kSlots = NB * kSteps, kScores = 16 * NB, kPer = kScores >= kSlots ? kScores / kSlots : 1;
     static_assert(kScores % kSlots == 0 || kSlots % kScores == 0, "scores per product");
-    auto operand = [&](int block, int kk) {
+    auto operand = [&](int block, int kk) __attribute__((always_inline)) {
       const unsigned char* const tile = smem + ((block / S::kSubs) & (R - 1)) * S::kTileBytes;
       return *reinterpret_cast<const bf16x8_t*>(tile + place<D>((block % S::kSubs) * 32 + col, chunk_of<D>(kk, half)));
     };
     f32x4_t sums[NB];  // four side by side: a chain of 16 additions would take as long as the block's products
     float m_sub[NB];
-    auto begin = [&]() {
+    auto begin = [&]() __attribute__((always_inline)) {
 #pragma unroll
       for (int n = 0; n < NB; ++n) sums[n] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f}, m_sub[n] = m_run[n];
     };
-    auto score = [&](int i, const f32x16_t (&s)[NB]) {
+    auto score = [&](int i, const f32x16_t (&s)[NB]) __attribute__((always_inline)) {
       const int n = i % NB, r = i / NB;
       float y = sums[n][r & 3] + __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][r], a.scale_log2, -m_sub[n]));
       asm volatile("" : "+v"(y));  // computed here, not sunk towards the block's end
@@ -369,7 +382,7 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void row_stats_kernel(W
     };
     // A row's maximum may lag: its exponentials are summed as they are while they stay far from fp32's end, which their sum
     // shows.  Only a row's first keys, and keys 2^64 above its maximum, take the maximum first.
-    auto finish = [&](const f32x16_t (&s)[NB]) {
+    auto finish = [&](const f32x16_t (&s)[NB]) __attribute__((always_inline)) {
 #pragma unroll
       for (int n = 0; n < NB; ++n) {
         float sum = (sums[n][0] + sums[n][1]) + (sums[n][2] + sums[n][3]);
@@ -388,13 +401,13 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void row_stats_kernel(W
         l_run[n] += sum;
       }
     };
-    auto softmax = [&](const f32x16_t (&s)[NB]) {
+    auto softmax = [&](const f32x16_t (&s)[NB]) __attribute__((always_inline)) {
       begin();
 #pragma unroll
       for (int i = 0; i < kScores; ++i) score(i, s);
       finish(s);
     };
-    auto products = [&](int block, f32x16_t (&s)[NB]) {
+    auto products = [&](int block, f32x16_t (&s)[NB]) __attribute__((always_inline)) {
 #pragma unroll
       for (int n = 0; n < NB; ++n) s[n] = f32x16_t{};
 #pragma unroll
@@ -417,7 +430,7 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void row_stats_kernel(W
       products(0, sA);
 #pragma unroll
       for (int kk = 0; kk < kAhead; ++kk) kf[kk] = operand(1, kk);  // (of a last block: unused)
-      auto step = [&](int block, f32x16_t (&sc)[NB], f32x16_t (&sn)[NB]) {  // softmax of `block`, products of the next one
+      auto step = [&](int block, f32x16_t (&sc)[NB], f32x16_t (&sn)[NB]) __attribute__((always_inline)) {  // softmax of `block`, products of the next one
         begin();
 #pragma unroll
         for (int n = 0; n < NB; ++n) sn[n] = f32x16_t{};
@@ -567,6 +580,7 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void key_sums_kernel(We
   static_assert(kCopies >= 1, "a tile gives every wavefront a copy");
   __shared__ __attribute__((aligned(1024))) unsigned char smem[kSumRing * kTile];
   __shared__ __attribute__((aligned(16))) float row_m[kInfoRows], row_inv[kInfoRows];
+  __shared__ __attribute__((aligned(16))) int row_last[kInfoRows];  // key that the row sees last
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
   const int col = lane & 31, half = lane >> 5;
   const uint32_t lds0 = lds_address(smem);
@@ -587,20 +601,32 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void key_sums_kernel(We
     const int32_t* const table = a.c.table + req * a.c.table_stride;
     const float2* const stats = reinterpret_cast<const float2*>(a.stats) + stat_row(a, x, req, head);
 
-    // ---- rows: tile t's to stage t % kSumRing; rows behind the last one repeat it (the mask discards them)
+    // ---- rows: tile t's are copied to stage t % kSumRing, in order; every lane's pointers move on by 32 rows (rows behind the
+    // last one read the first: the mask discards them)
     const int step_tokens = uniform(kSumRows / a.group), step_rem = kSumRows - step_tokens * a.group;
-    int copy_token = uniform(t0 * kSumRows / a.group), copy_rem = t0 * kSumRows - copy_token * a.group;  // of the next copy
-    auto token_in = [&](int rem, int r) { return static_cast<int>((static_cast<uint32_t>(rem + r) * a.group_magic) >> 24); };
-    auto copy = [&](int t) {
+    const uint16_t* const q_first = q_row(a, x, req, head, 0, 0);
+    const int64_t step_bytes = 2 * (step_tokens * a.qs[2] + step_rem * a.qs[1]), wrap_bytes = 2 * (a.qs[2] - a.group * a.qs[1]);
+    int copy_g[kCopies];
+    const char* copy_at[kCopies];
+#pragma unroll
+    for (int i = 0; i < kCopies; ++i) {
+      const int at = (i * kWaves + wave) * 64 + lane, r = at / CR, row = t0 * kSumRows + r, token = row / a.group;
+      copy_g[i] = row - token * a.group;
+      copy_at[i] = reinterpret_cast<const char*>(q_first + token * a.qs[2] + copy_g[i] * a.qs[1] + ((at % CR) ^ (r & 7)) * 8);
+    }
+    auto copy = [&](int t) __attribute__((always_inline)) {
+      const int left = rows - t * kSumRows;
 #pragma unroll
       for (int i = 0; i < kCopies; ++i) {
-        const int at = (i * kWaves + wave) * 64 + lane, r = at / CR, row = min(r, rows - 1 - t * kSumRows);
-        const int token = token_in(copy_rem, row);
-        lane_to_lds(q_row(a, x, req, head, copy_token + token, copy_rem + row - token * a.group) + ((at % CR) ^ (r & 7)) * 8,
-                    lds0 + static_cast<uint32_t>((t & (kSumRing - 1)) * kTile + (i * kWaves + wave) * 1024));
+        const int at = (i * kWaves + wave) * 64 + lane;
+        const char* p = copy_at[i];
+        if (left < kSumRows) p = at / CR < left ? p : reinterpret_cast<const char*>(q_first);
+        lane_to_lds(p, lds0 + static_cast<uint32_t>((t & (kSumRing - 1)) * kTile + (i * kWaves + wave) * 1024));
+        copy_g[i] += step_rem;
+        const bool wrap = copy_g[i] >= a.group;
+        copy_g[i] -= wrap ? a.group : 0;
+        copy_at[i] += step_bytes + (wrap ? wrap_bytes : 0);
       }
-      copy_token += step_tokens, copy_rem += step_rem;
-      if (copy_rem >= a.group) copy_token += 1, copy_rem -= a.group;
     };
     __syncthreads();  // the item before has read its tiles
 #pragma unroll
@@ -629,25 +655,27 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void key_sums_kernel(We
     loaded(kf);
     float sum[2] = {0.0f, 0.0f};
     int info0 = -1;  // first row of those in row_m
-    auto info = [&](int row0) {
+    auto info = [&](int row0) __attribute__((always_inline)) {
       if (info0 >= 0 && row0 < info0 + kInfoRows) return;
       __syncthreads();  // the rows before are done with theirs
       info0 = row0;
 #pragma unroll
       for (int u = 0; u < kInfoRows / kThreads; ++u) {
         const int i = u * kThreads + tid;
-        const float2 y = stats[min(info0 + i, rows - 1)];
+        const int row = info0 + i;
+        const float2 y = stats[min(row, rows - 1)];
         row_m[i] = y.x;
         row_inv[i] = y.y;
+        row_last[i] = row < rows ? x.len - x.n_new + row / a.group : -1;
       }
       __syncthreads();
     };
-    auto operand = [&](int t, int kk) {
+    auto operand = [&](int t, int kk) __attribute__((always_inline)) {
       return *reinterpret_cast<const bf16x8_t*>(smem + (t & (kSumRing - 1)) * kTile + place<D>(col, chunk_of<D>(kk, half)));
     };
     // Tile t + 2 has landed for every wavefront (tile t + 1 at its first operands' reads), and tile t - 1 is read, whose
     // stage is the next copy's.
-    auto advance = [&](int t) {
+    auto advance = [&](int t) __attribute__((always_inline)) {
       if (t + 6 < t1) wait_copies<4 * kCopies>();
       else if (t + 4 < t1) wait_copies<2 * kCopies>();
       else wait_copies<0>();
@@ -657,110 +685,81 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void key_sums_kernel(We
     // Scores one by one: exp(score - m) / l of row 8 r4 + 4 half + e and key block n, into four sums per block side by
     // side (a chain of 16 additions would take as long as the tile's products).
     f32x4_t tile_sum[2], mv[2], iv[2];
-    const float *m_at = row_m, *inv_at = row_inv;
-    auto score = [&](int i, const f32x16_t (&s)[2], auto last_of) {
+    int4 lv[2];
+    int info_at = 0;
+    auto values = [&](auto masked_c, int r4) __attribute__((always_inline)) {
+      const int at = info_at + 8 * r4;
+      mv[r4 & 1] = *static_cast<const f32x4_t*>(__builtin_assume_aligned(row_m + at, 16));
+      iv[r4 & 1] = *static_cast<const f32x4_t*>(__builtin_assume_aligned(row_inv + at, 16));
+      if constexpr (decltype(masked_c)::value) lv[r4 & 1] = *static_cast<const int4*>(__builtin_assume_aligned(row_last + at, 16));
+    };
+    auto score = [&](auto masked_c, int i, const f32x16_t (&s)[2]) __attribute__((always_inline)) {
       const int r4 = i / 8, e = (i / 2) % 4, n = i % 2;
-      if (i % 8 == 0 && r4 < 3) {
-        mv[(r4 + 1) & 1] = *static_cast<const f32x4_t*>(__builtin_assume_aligned(m_at + 8 * (r4 + 1), 16));
-        iv[(r4 + 1) & 1] = *static_cast<const f32x4_t*>(__builtin_assume_aligned(inv_at + 8 * (r4 + 1), 16));
+      if (i % 8 == 0 && r4 < 3) values(masked_c, r4 + 1);
+      float y = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][4 * r4 + e], a.scale_log2, -mv[r4 & 1][e]));
+      if constexpr (decltype(masked_c)::value) {
+        const int4 l = lv[r4 & 1];
+        y = key[n] <= (e == 0 ? l.x : e == 1 ? l.y : e == 2 ? l.z : l.w) ? y : 0.0f;
       }
-      float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][4 * r4 + e], a.scale_log2, -mv[r4 & 1][e]));
-      p = last_of(8 * r4 + 4 * half + e, n) ? p : 0.0f;
-      float y = __builtin_fmaf(p, iv[r4 & 1][e], tile_sum[n][e]);
+      y = __builtin_fmaf(y, iv[r4 & 1][e], tile_sum[n][e]);
       asm volatile("" : "+v"(y));  // computed here, not sunk towards the tile's end
       tile_sum[n][e] = y;
     };
-    auto begin = [&](int t) {
-      m_at = row_m + (t * kSumRows - info0) + 4 * half;
-      inv_at = row_inv + (t * kSumRows - info0) + 4 * half;
-      mv[0] = *static_cast<const f32x4_t*>(__builtin_assume_aligned(m_at, 16));
-      iv[0] = *static_cast<const f32x4_t*>(__builtin_assume_aligned(inv_at, 16));
+    // Products of tile t + 1 between the exponentials of tile t: two wavefronts of a SIMD would run the same phase side by
+    // side, one unit idle at a time.  (Behind the last tile they are of whatever lies in LDS, and unused.)
+    constexpr int kAhead = 4, kSlots = 2 * kSteps, kPer = 32 / kSlots;
+    static_assert(32 % kSlots == 0, "scores per product");
+    f32x16_t sA[2], sB[2];
+    bf16x8_t qf[kAhead];
+    auto step = [&](auto masked_c, int t, f32x16_t (&sc)[2], f32x16_t (&sn)[2]) __attribute__((always_inline)) {
+      advance(t);
+      info(t * kSumRows);
+      info_at = t * kSumRows - info0 + 4 * half;
+      values(masked_c, 0);
       tile_sum[0] = tile_sum[1] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-    };
-    auto finish = [&]() {
+      sn[0] = sn[1] = f32x16_t{};
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int slot = 0; slot < kSlots; ++slot) {
+        const int kk = slot / 2, n = slot % 2;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) score(masked_c, slot * kPer + i, sc);
+        sn[n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(qf[kk % kAhead], kf[n][kk], sn[n], 0, 0, 0);
+        if (n == 1) qf[kk % kAhead] = kk + kAhead < kSteps ? operand(t + 1, kk + kAhead) : operand(t + 2, kk + kAhead - kSteps);
+        __builtin_amdgcn_sched_barrier(0);
+      }
 #pragma unroll
       for (int n = 0; n < 2; ++n) sum[n] += (tile_sum[n][0] + tile_sum[n][1]) + (tile_sum[n][2] + tile_sum[n][3]);
     };
-    auto always = [](int, int) { return true; };
-    auto products = [&](int t, f32x16_t (&s)[2]) {
-      s[0] = s[1] = f32x16_t{};
-#pragma unroll
-      for (int kk = 0; kk < kSteps; ++kk) {
-        const bf16x8_t qf = operand(t, kk);
-#pragma unroll
-        for (int n = 0; n < 2; ++n) s[n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(qf, kf[n][kk], s[n], 0, 0, 0);
+    auto run = [&](auto masked_c, int from, int to) __attribute__((always_inline)) {  // products of tile `from` are in sA, and of tile `to` afterwards
+      int t = from;
+#pragma unroll 1
+      for (; t + 1 < to; t += 2) {
+        step(masked_c, t, sA, sB);
+        step(masked_c, t + 1, sB, sA);
       }
-    };
-    // A tile with rows that do not see every key, or rows behind the last one.
-    auto masked_tile = [&](int t) {
-      f32x16_t s[2];
-      advance(t);
-      info(t * kSumRows);
-      products(t, s);
-      const int row0 = t * kSumRows, token0 = row0 / a.group, rem0 = row0 - token0 * a.group;
-      int last = -1;  // key that the row sees
-      begin(t);
-#pragma unroll
-      for (int i = 0; i < 32; ++i)
-        score(i, s, [&](int r, int n) {
-          if (n == 0) last = row0 + r < rows ? x.len - x.n_new + token0 + token_in(rem0, r) : -1;
-          return key[n] <= last;
-        });
-      finish();
+      if (t < to) {
+        step(masked_c, t, sA, sB);
+        sA[0] = sB[0], sA[1] = sB[1];
+      }
     };
     wait_copies<0>();
     __syncthreads();
-    // tiles [t0, whole) are masked, tiles [whole, whole_end) are not, the last one again where its rows end within
+    sA[0] = sA[1] = f32x16_t{};
+#pragma unroll
+    for (int kk = 0; kk < kSteps; ++kk) {
+      const bf16x8_t y = operand(t0, kk);
+#pragma unroll
+      for (int n = 0; n < 2; ++n) sA[n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(y, kf[n][kk], sA[n], 0, 0, 0);
+    }
+#pragma unroll
+    for (int kk = 0; kk < kAhead; ++kk) qf[kk] = operand(t0 + 1, kk);
+    // tiles [t0, whole) have rows that do not see every key, the last one may have rows behind the request's
     const int whole = uniform(min(max(over(first_row(a, x, min(key0 + kSumKeys, x.len) - 1), kSumRows), t0), t1));
     const int whole_end = uniform(max(whole, min(t1, rows / kSumRows)));
-#pragma unroll 1
-    for (int t = t0; t < whole; ++t) masked_tile(t);
-    if (whole < whole_end) {
-      // Products of tile t + 1 between the exponentials of tile t: two wavefronts of a SIMD would run the same phase side by
-      // side, one unit idle at a time.
-      constexpr int kAhead = 4, kSlots = 2 * kSteps, kPer = 32 / kSlots;
-      static_assert(32 % kSlots == 0, "scores per product");
-      f32x16_t sA[2], sB[2];
-      bf16x8_t qf[kAhead];
-      products(whole, sA);
-#pragma unroll
-      for (int kk = 0; kk < kAhead; ++kk) qf[kk] = operand(whole + 1, kk);  // (behind the last tile: unused)
-      auto step = [&](int t, f32x16_t (&sc)[2], f32x16_t (&sn)[2]) {
-        advance(t);
-        info(t * kSumRows);
-        begin(t);
-        sn[0] = sn[1] = f32x16_t{};
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int slot = 0; slot < kSlots; ++slot) {
-          const int kk = slot / 2, n = slot % 2;
-#pragma unroll
-          for (int i = 0; i < kPer; ++i) score(slot * kPer + i, sc, always);
-          sn[n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(qf[kk % kAhead], kf[n][kk], sn[n], 0, 0, 0);
-          if (n == 1) qf[kk % kAhead] = kk + kAhead < kSteps ? operand(t + 1, kk + kAhead) : operand(t + 2, kk + kAhead - kSteps);
-          __builtin_amdgcn_sched_barrier(0);
-        }
-        finish();
-      };
-      int t = whole;
-#pragma unroll 1
-      for (; t + 2 < whole_end; t += 2) {
-        step(t, sA, sB);
-        step(t + 1, sB, sA);
-      }
-      if (t + 1 < whole_end) {
-        step(t, sA, sB);
-        sA[0] = sB[0], sA[1] = sB[1];
-      }
-      advance(whole_end - 1);
-      info((whole_end - 1) * kSumRows);
-      begin(whole_end - 1);
-#pragma unroll
-      for (int i = 0; i < 32; ++i) score(i, sA, always);
-      finish();
-    }
-#pragma unroll 1
-    for (int t = whole_end; t < t1; ++t) masked_tile(t);
+    run(std::true_type{}, t0, whole);
+    run(std::false_type{}, whole, whole_end);
+    run(std::true_type{}, whole_end, t1);
     int at = 0;
     if (n_ranges > 1) at = uniform(items_before(a, lane, req, [&](const Req& y) { return cut.places(a, y); })) + k;
     if (at < 0 || at >= 2 * a.sums_items) continue;  // only of an offset table that is not ascending
