@@ -157,7 +157,17 @@ struct Cut {
         })) {}
   __device__ __forceinline__ int rtiles(const WeightArgs& a, const Req& x) const { return over(x.n_new * a.group, S::kRows); }
   __device__ __forceinline__ int ranges(const Req& x) const { return max(over(over(x.len, S::kKeys), c), 1); }
-  __device__ __forceinline__ int items(const WeightArgs& a, const Req& x) const { return rtiles(a, x) * ranges(x) * a.kv_heads; }
+  // first row tile with keys in range v: later tokens see more keys
+  __device__ __forceinline__ int rtile0(const WeightArgs& a, const Req& x, int v) const {
+    const int rows = max(v * c * S::kKeys - (x.len - x.n_new), 0) * a.group;  // of the tokens that see none of the range
+    return v == 0 ? 0 : min(rows / S::kRows, rtiles(a, x));
+  }
+  __device__ __forceinline__ int per_head(const WeightArgs& a, const Req& x) const {
+    int n = 0;
+    for (int v = 0; v < ranges(x); ++v) n += rtiles(a, x) - rtile0(a, x, v);
+    return n;
+  }
+  __device__ __forceinline__ int items(const WeightArgs& a, const Req& x) const { return x.n_new > 0 ? per_head(a, x) * a.kv_heads : 0; }
 };
 
 // 16 bytes of codes (or bf16) of a cached row, as bf16 in pieces of eight.
@@ -254,8 +264,17 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void row_stats_kernel(W
     if (!find_request(a, lane, item, [&](const Req& x) { return cut.items(a, x); }, &req, &base)) return;
     Req x = request(a, req);
     x.start = uniform(x.start), x.n_new = uniform(x.n_new), x.len = uniform(x.len);
-    const int n_rt = uniform(cut.rtiles(a, x)), n_ranges = uniform(cut.ranges(x)), k = uniform(item - base);
-    const int rtile = uniform(k % n_rt), hr = uniform(k / n_rt), range = uniform(hr % n_ranges), head = uniform(hr / n_ranges);
+    const int n_rt = uniform(cut.rtiles(a, x)), n_ranges = uniform(cut.ranges(x)), per_head = uniform(cut.per_head(a, x));
+    const int head = uniform((item - base) / per_head);
+    int rtile = item - base - head * per_head, range = 0;  // place within the head, range by range
+    for (;; ++range) {
+      const int first = uniform(cut.rtile0(a, x, range));
+      if (rtile < n_rt - first || range + 1 == n_ranges) {
+        rtile += first;
+        break;
+      }
+      rtile -= n_rt - first;
+    }
     const int row0 = rtile * S::kRows, rows = x.n_new * a.group;
     const int kend = uniform(seen_by(a, x, min(row0 + S::kRows, rows) - 1));
     const int key0 = range * cut.c * S::kKeys;
@@ -530,19 +549,24 @@ __global__ __launch_bounds__(S::kRows) void row_stats_join_kernel(WeightArgs a) 
     const Req x = request(a, req);
     const int n_rt = uniform(cut.rtiles(a, x)), n_ranges = uniform(cut.ranges(x)), k = uniform(item - base);
     const int rtile = k % n_rt, head = k / n_rt, row0 = rtile * S::kRows, rows = x.n_new * a.group;
-    const int first = uniform(items_before(a, lane, req, [&](const Req& y) { return cut.items(a, y); })) + head * n_ranges * n_rt + rtile;
-    const int n = over(over(seen_by(a, x, min(row0 + S::kRows, rows) - 1), S::kKeys), cut.c);  // ranges that a row sees
-    if (first < 0 || first + static_cast<int64_t>(n_ranges - 1) * n_rt >= a.part_items) continue;  // only of an offset table that is not ascending
+    const int place = uniform(items_before(a, lane, req, [&](const Req& y) { return cut.items(a, y); })) + head * uniform(cut.per_head(a, x)) + rtile;
     const int row = threadIdx.x;
-    const float2* const p = reinterpret_cast<const float2*>(a.part) + static_cast<int64_t>(first) * S::kRows + row;
+    const float2* const p = reinterpret_cast<const float2*>(a.part) + row;
     float m = -__builtin_inff(), l = 0.0f;
-    for (int v0 = 0; v0 < n; v0 += 4) {  // four loads in flight
+    int at = place;  // of range v's first row tile, were this one that
+    for (int v0 = 0; v0 < n_ranges; v0 += 4) {  // four loads in flight
       float2 y[4];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) y[u] = p[static_cast<int64_t>(min(v0 + u, n - 1)) * n_rt * S::kRows];
+      for (int u = 0; u < 4; ++u) {
+        const int v = min(v0 + u, n_ranges - 1), first = cut.rtile0(a, x, v), here = at - first;
+        // (every part has its place but those of an offset table that is not ascending)
+        const bool seen = v0 + u < n_ranges && rtile >= first && here >= 0 && here < a.part_items;
+        y[u] = float2{-__builtin_inff(), 0.0f};
+        if (seen) y[u] = p[static_cast<int64_t>(here) * S::kRows];
+        at += n_rt - first;
+      }
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
-        if (v0 + u >= n) continue;
         const float top = fmaxf(m, y[u].x), sub = top == -__builtin_inff() ? 0.0f : top;
         l = l * __builtin_amdgcn_exp2f(m - sub) + y[u].y * __builtin_amdgcn_exp2f(y[u].x - sub);
         m = top;
@@ -563,7 +587,18 @@ struct SumCut {
         })) {}
   __device__ __forceinline__ int ktiles(const WeightArgs& a, const Req& x) const { return x.n_new > 0 ? over(x.len, kSumKeys) * a.kv_heads : 0; }
   __device__ __forceinline__ int ranges(const WeightArgs& a, const Req& x) const { return max(over(over(x.n_new * a.group, kSumRows), c), 1); }
-  __device__ __forceinline__ int items(const WeightArgs& a, const Req& x) const { return ktiles(a, x) * ranges(a, x); }
+  // Ranges are counted from the last one on, which all key tiles have: the first `seen` key tiles have range j.
+  __device__ __forceinline__ int seen(const WeightArgs& a, const Req& x, int n_ranges, int j) const {
+    const int keys = x.len - x.n_new + over((n_ranges - j) * c * kSumRows, a.group);  // that the range's rows and those before see
+    return min(max(over(max(keys, 0), kSumKeys), 0), over(x.len, kSumKeys));
+  }
+  __device__ __forceinline__ int per_head(const WeightArgs& a, const Req& x) const {
+    const int n_ranges = ranges(a, x);
+    int n = 0;
+    for (int j = 0; j < n_ranges; ++j) n += seen(a, x, n_ranges, j);
+    return n;
+  }
+  __device__ __forceinline__ int items(const WeightArgs& a, const Req& x) const { return x.n_new > 0 ? per_head(a, x) * a.kv_heads : 0; }
   // of requests that are cut into row ranges: their items' sums have places in the workspace, below 2 sums_items
   __device__ __forceinline__ int places(const WeightArgs& a, const Req& x) const { return ranges(a, x) > 1 ? items(a, x) : 0; }
   __device__ __forceinline__ int joins(const WeightArgs& a, const Req& x) const { return ranges(a, x) > 1 ? ktiles(a, x) : 0; }
@@ -590,8 +625,15 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void key_sums_kernel(We
     if (!find_request(a, lane, item, [&](const Req& x) { return cut.items(a, x); }, &req, &base)) return;
     Req x = request(a, req);
     x.start = uniform(x.start), x.n_new = uniform(x.n_new), x.len = uniform(x.len);
-    const int n_ranges = uniform(cut.ranges(a, x)), k = uniform(item - base), n_kt = uniform(over(x.len, kSumKeys));
-    const int range = uniform(k % n_ranges), hk = uniform(k / n_ranges), kt = uniform(hk % n_kt), head = uniform(hk / n_kt);
+    const int n_ranges = uniform(cut.ranges(a, x)), k = uniform(item - base), per_head = uniform(cut.per_head(a, x));
+    const int head = uniform(k / per_head);
+    int kt = k - head * per_head, j = 0;  // place within the head, range by range
+    for (;; ++j) {
+      const int n = uniform(cut.seen(a, x, n_ranges, j));
+      if (kt < n || j + 1 == n_ranges) break;
+      kt -= n;
+    }
+    const int range = n_ranges - 1 - j;
     const int key0 = kt * kSumKeys, rows = x.n_new * a.group;
     const int t0 = uniform(max(first_row(a, x, key0) / kSumRows, range * cut.c));
     const int t1 = uniform(min(over(rows, kSumRows), (range + 1) * cut.c));
@@ -622,10 +664,13 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void key_sums_kernel(We
         const char* p = copy_at[i];
         if (left < kSumRows) p = at / CR < left ? p : reinterpret_cast<const char*>(q_first);
         lane_to_lds(p, lds0 + static_cast<uint32_t>((t & (kSumRing - 1)) * kTile + (i * kWaves + wave) * 1024));
-        copy_g[i] += step_rem;
-        const bool wrap = copy_g[i] >= a.group;
-        copy_g[i] -= wrap ? a.group : 0;
-        copy_at[i] += step_bytes + (wrap ? wrap_bytes : 0);
+        copy_at[i] += step_bytes;
+        if (step_rem != 0) {
+          copy_g[i] += step_rem;
+          const bool wrap = copy_g[i] >= a.group;
+          copy_g[i] -= wrap ? a.group : 0;
+          copy_at[i] += wrap ? wrap_bytes : 0;
+        }
       }
     };
     __syncthreads();  // the item before has read its tiles
@@ -785,11 +830,13 @@ __global__ __launch_bounds__(kSumKeys) void key_sums_join_kernel(WeightArgs a) {
     const int kt = k % n_kt, head = k / n_kt, key = kt * kSumKeys + static_cast<int>(threadIdx.x);
     const int slot = uniform(owned_slot(a.index, req, a.w_rows, lane));
     if (slot < 0) continue;
-    const int at = uniform(items_before(a, lane, req, [&](const Req& y) { return cut.places(a, y); })) + k * n_ranges;
-    if (at < 0 || at + n_ranges > 2 * a.sums_items) continue;
-    float sum = 0.0f;  // from the first range on whose rows see the tile
-    for (int v = first_row(a, x, kt * kSumKeys) / kSumRows / cut.c; v < n_ranges; ++v)
-      sum += a.sums[static_cast<int64_t>(at + v) * kSumKeys + threadIdx.x];
+    int at = uniform(items_before(a, lane, req, [&](const Req& y) { return cut.places(a, y); })) + head * uniform(cut.per_head(a, x)) + kt;
+    float sum = 0.0f;
+    for (int j = 0; j < n_ranges; ++j) {
+      const int n = uniform(cut.seen(a, x, n_ranges, j));
+      if (kt < n && at >= 0 && at < 2 * a.sums_items) sum += a.sums[static_cast<int64_t>(at) * kSumKeys + threadIdx.x];
+      at += n;
+    }
     if (key < x.len && on_a_page(a, a.c.table + req * a.c.table_stride, key)) a.w[slot * a.w_row + head * a.w_head + key] += sum;
   }
 }
