@@ -76,6 +76,19 @@ __device__ __forceinline__ Req request(const WeightArgs& a, int r) {
   return x;
 }
 
+// All requests: the first 64 are loaded once, a lane each.
+struct Requests {
+  Req first;
+  __device__ __forceinline__ Requests(const WeightArgs& a, int lane) : first(request(a, lane)) {}
+  __device__ __forceinline__ Req lanes(const WeightArgs& a, int r0, int lane) const { return r0 == 0 ? first : request(a, r0 + lane); }
+  __device__ __forceinline__ Req one(const WeightArgs& a, int r) const {  // r is uniform
+    Req x = first;
+    if (r >= 64) x = request(a, r);
+    const int l = r < 64 ? r : 0;
+    return {__builtin_amdgcn_readlane(x.start, l), __builtin_amdgcn_readlane(x.n_new, l), __builtin_amdgcn_readlane(x.len, l)};
+  }
+};
+
 __device__ __forceinline__ int over(int x, int n) { return static_cast<int>((static_cast<uint32_t>(x) + n - 1) / static_cast<uint32_t>(n)); }
 
 __device__ __forceinline__ int64_t wave_total(int64_t v) {
@@ -94,11 +107,11 @@ struct Size {
 // time, and the best of a few m is taken; a few items more than workgroups would cost a whole round.  `items` bounds them
 // whatever the estimate: no more than that many places (and one per tile that stays) are needed.
 template <typename SizeOf>
-__device__ __forceinline__ int tiles_of_item(const WeightArgs& a, int lane, int items, int least, int overhead, SizeOf size_of) {
+__device__ __forceinline__ int tiles_of_item(const WeightArgs& a, const Requests& all_req, int lane, int items, int least, int overhead, SizeOf size_of) {
   constexpr int kRounds = 4;
   Size all{0, 0.0f, 0.0f};
   for (int r0 = 0; r0 < a.n_req; r0 += 64) {
-    const Req x = request(a, r0 + lane);
+    const Req x = all_req.lanes(a, r0, lane);
     if (x.n_new == 0) continue;
     const Size y = size_of(x);
     all.pairs += y.pairs, all.seen += y.seen, all.stays += y.stays;
@@ -109,7 +122,7 @@ __device__ __forceinline__ int tiles_of_item(const WeightArgs& a, int lane, int 
   float best = 1e9f, cost = 1e30f;  // without room for any cut: whole
 #pragma unroll
   for (int m = 1; m <= kRounds; ++m) {
-    const float room = static_cast<float>(m * a.slots) - 1.1f * stays;
+    const float room = static_cast<float>(m * a.slots) - 0.6f * stays;
     if (room < 1.0f) continue;
     const float c = ceilf(seen / room), now = static_cast<float>(m) * (c + static_cast<float>(overhead));
     if (now < cost) best = c, cost = now;
@@ -120,10 +133,10 @@ __device__ __forceinline__ int tiles_of_item(const WeightArgs& a, int lane, int 
 
 // Request that holds item `at` when request r has count(r) items: false if none does; *base: items before it.
 template <typename Count>
-__device__ __forceinline__ bool find_request(const WeightArgs& a, int lane, int at, Count count, int* req, int* base) {
+__device__ __forceinline__ bool find_request(const WeightArgs& a, const Requests& all, int lane, int at, Count count, int* req, int* base) {
   int before = 0;
   for (int r0 = 0; r0 < a.n_req; r0 += 64) {
-    const int mine = r0 + lane < a.n_req ? count(request(a, r0 + lane)) : 0;
+    const int mine = r0 + lane < a.n_req ? count(all.lanes(a, r0, lane)) : 0;
     const int incl = wave_scan(mine);
     const uint64_t past = __builtin_amdgcn_ballot_w64(before + incl > at);
     if (past != 0) {
@@ -139,22 +152,35 @@ __device__ __forceinline__ bool find_request(const WeightArgs& a, int lane, int 
 
 // Items of the requests before `req`.
 template <typename Count>
-__device__ __forceinline__ int items_before(const WeightArgs& a, int lane, int req, Count count) {
+__device__ __forceinline__ int items_before(const WeightArgs& a, const Requests& all, int lane, int req, Count count) {
   int n = 0;
-  for (int r0 = 0; r0 < req; r0 += 64) n += __builtin_amdgcn_readlane(wave_scan(r0 + lane < req ? count(request(a, r0 + lane)) : 0), 63);
+  for (int r0 = 0; r0 < req; r0 += 64) n += __builtin_amdgcn_readlane(wave_scan(r0 + lane < req ? count(all.lanes(a, r0, lane)) : 0), 63);
   return n;
+}
+
+// The estimate put right: a few items more than whole rounds of workgroups are made fewer.
+template <class C>
+__device__ __forceinline__ void fit(C& cut, const WeightArgs& a, const Requests& all, int lane) {
+  for (int i = 0; i < 4; ++i) {
+    const int n = items_before(a, all, lane, a.n_req, [&](const Req& x) { return cut.items(a, x); });
+    const int more = n & (a.slots - 1);  // of the last round
+    if (n <= a.slots || n > 4 * a.slots || more == 0 || 8 * more > a.slots) break;
+    cut.c += max(cut.c >> 4, 1);
+  }
 }
 
 // How the row stats cut a request.
 template <class S>
 struct Cut {
   int c;  // key tiles of a range
-  __device__ __forceinline__ Cut(const WeightArgs& a, int lane)
-      : c(tiles_of_item(a, lane, a.stats_items, 256 / S::kKeys, 4, [&](const Req& x) {
+  __device__ __forceinline__ Cut(const WeightArgs& a, const Requests& all, int lane)
+      : c(tiles_of_item(a, all, lane, a.stats_items, 256 / S::kKeys, 5, [&](const Req& x) {
           const int rt = over(x.n_new * a.group, S::kRows), kt = over(x.len, S::kKeys);
           const float mean = 0.5f * static_cast<float>(min(x.len, x.len - x.n_new + S::kRows / a.group) + x.len);
           return Size{static_cast<int64_t>(rt) * kt, static_cast<float>(rt) * (mean / S::kKeys + 0.5f), static_cast<float>(rt)};
-        })) {}
+        })) {
+    fit(*this, a, all, lane);
+  }
   __device__ __forceinline__ int rtiles(const WeightArgs& a, const Req& x) const { return over(x.n_new * a.group, S::kRows); }
   __device__ __forceinline__ int ranges(const Req& x) const { return max(over(over(x.len, S::kKeys), c), 1); }
   // first row tile with keys in range v: later tokens see more keys
@@ -258,12 +284,12 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void row_stats_kernel(W
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
   const int col = lane & 31, half = lane >> 5;
   const uint32_t lds0 = lds_address(smem);
-  const Cut<S> cut(a, lane);
+  const Requests all(a, lane);
+  const Cut<S> cut(a, all, lane);
   for (int item = blockIdx.x; item < a.part_items; item += gridDim.x) {
     int req, base;
-    if (!find_request(a, lane, item, [&](const Req& x) { return cut.items(a, x); }, &req, &base)) return;
-    Req x = request(a, req);
-    x.start = uniform(x.start), x.n_new = uniform(x.n_new), x.len = uniform(x.len);
+    if (!find_request(a, all, lane, item, [&](const Req& x) { return cut.items(a, x); }, &req, &base)) return;
+    const Req x = all.one(a, req);
     const int n_rt = uniform(cut.rtiles(a, x)), n_ranges = uniform(cut.ranges(x)), per_head = uniform(cut.per_head(a, x));
     const int head = uniform((item - base) / per_head);
     int rtile = item - base - head * per_head, range = 0;  // place within the head, range by range
@@ -402,10 +428,16 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void row_stats_kernel(W
     // A row's maximum may lag: its exponentials are summed as they are while they stay far from fp32's end, which their sum
     // shows.  Only a row's first keys, and keys 2^64 above its maximum, take the maximum first.
     auto finish = [&](const f32x16_t (&s)[NB]) __attribute__((always_inline)) {
+      float sum[NB];
+      bool far = false;
 #pragma unroll
       for (int n = 0; n < NB; ++n) {
-        float sum = (sums[n][0] + sums[n][1]) + (sums[n][2] + sums[n][3]);
-        if (__builtin_amdgcn_ballot_w64(!(sum < 0x1p64f)) != 0) {
+        sum[n] = (sums[n][0] + sums[n][1]) + (sums[n][2] + sums[n][3]);
+        far |= !(sum[n] < 0x1p64f);
+      }
+      if (__builtin_expect(__builtin_amdgcn_ballot_w64(far) != 0, 0)) {
+#pragma unroll
+        for (int n = 0; n < NB; ++n) {
           float mx = s[n][0];
 #pragma unroll
           for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[n][r]);
@@ -413,12 +445,13 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void row_stats_kernel(W
           const float m_new = fmaxf(m_run[n], mx), sub = m_new == -__builtin_inff() ? 0.0f : m_new;
           l_run[n] *= m_new == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(m_run[n] - m_new);
           m_run[n] = m_new;
-          sum = 0.0f;
+          sum[n] = 0.0f;
 #pragma unroll
-          for (int r = 0; r < 16; ++r) sum += __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][r], a.scale_log2, -sub));
+          for (int r = 0; r < 16; ++r) sum[n] += __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][r], a.scale_log2, -sub));
         }
-        l_run[n] += sum;
       }
+#pragma unroll
+      for (int n = 0; n < NB; ++n) l_run[n] += sum[n];
     };
     auto softmax = [&](const f32x16_t (&s)[NB]) __attribute__((always_inline)) {
       begin();
@@ -542,14 +575,15 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void row_stats_kernel(W
 template <class S>
 __global__ __launch_bounds__(S::kRows) void row_stats_join_kernel(WeightArgs a) {
   const int lane = threadIdx.x & 63;
-  const Cut<S> cut(a, lane);
+  const Requests all(a, lane);
+  const Cut<S> cut(a, all, lane);
   for (int item = blockIdx.x;; item += gridDim.x) {
     int req, base;
-    if (!find_request(a, lane, item, [&](const Req& x) { return cut.ranges(x) > 1 ? cut.rtiles(a, x) * a.kv_heads : 0; }, &req, &base)) return;
-    const Req x = request(a, req);
+    if (!find_request(a, all, lane, item, [&](const Req& x) { return cut.ranges(x) > 1 ? cut.rtiles(a, x) * a.kv_heads : 0; }, &req, &base)) return;
+    const Req x = all.one(a, req);
     const int n_rt = uniform(cut.rtiles(a, x)), n_ranges = uniform(cut.ranges(x)), k = uniform(item - base);
     const int rtile = k % n_rt, head = k / n_rt, row0 = rtile * S::kRows, rows = x.n_new * a.group;
-    const int place = uniform(items_before(a, lane, req, [&](const Req& y) { return cut.items(a, y); })) + head * uniform(cut.per_head(a, x)) + rtile;
+    const int place = uniform(items_before(a, all, lane, req, [&](const Req& y) { return cut.items(a, y); })) + head * uniform(cut.per_head(a, x)) + rtile;
     const int row = threadIdx.x;
     const float2* const p = reinterpret_cast<const float2*>(a.part) + row;
     float m = -__builtin_inff(), l = 0.0f;
@@ -579,12 +613,14 @@ __global__ __launch_bounds__(S::kRows) void row_stats_join_kernel(WeightArgs a) 
 // How the key sums cut a request: tiles of kSumKeys keys times ranges of c row tiles.
 struct SumCut {
   int c;
-  __device__ __forceinline__ SumCut(const WeightArgs& a, int lane)
-      : c(tiles_of_item(a, lane, a.sums_items, 4, 9, [&](const Req& x) {
+  __device__ __forceinline__ SumCut(const WeightArgs& a, const Requests& all, int lane)
+      : c(tiles_of_item(a, all, lane, a.sums_items, 4, 10, [&](const Req& x) {
           const int rt = over(x.n_new * a.group, kSumRows), kt = over(x.len, kSumKeys);
           const float fresh = 0.5f * static_cast<float>(x.n_new) / kSumKeys;  // half of the new tokens' keys are seen
           return Size{static_cast<int64_t>(rt) * kt, static_cast<float>(rt) * (static_cast<float>(kt) - fresh), static_cast<float>(kt)};
-        })) {}
+        })) {
+    fit(*this, a, all, lane);
+  }
   __device__ __forceinline__ int ktiles(const WeightArgs& a, const Req& x) const { return x.n_new > 0 ? over(x.len, kSumKeys) * a.kv_heads : 0; }
   __device__ __forceinline__ int ranges(const WeightArgs& a, const Req& x) const { return max(over(over(x.n_new * a.group, kSumRows), c), 1); }
   // Ranges are counted from the last one on, which all key tiles have: the first `seen` key tiles have range j.
@@ -619,12 +655,12 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void key_sums_kernel(We
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
   const int col = lane & 31, half = lane >> 5;
   const uint32_t lds0 = lds_address(smem);
-  const SumCut cut(a, lane);
+  const Requests all(a, lane);
+  const SumCut cut(a, all, lane);
   for (int item = blockIdx.x;; item += gridDim.x) {
     int req, base;
-    if (!find_request(a, lane, item, [&](const Req& x) { return cut.items(a, x); }, &req, &base)) return;
-    Req x = request(a, req);
-    x.start = uniform(x.start), x.n_new = uniform(x.n_new), x.len = uniform(x.len);
+    if (!find_request(a, all, lane, item, [&](const Req& x) { return cut.items(a, x); }, &req, &base)) return;
+    const Req x = all.one(a, req);
     const int n_ranges = uniform(cut.ranges(a, x)), k = uniform(item - base), per_head = uniform(cut.per_head(a, x));
     const int head = uniform(k / per_head);
     int kt = k - head * per_head, j = 0;  // place within the head, range by range
@@ -806,7 +842,7 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void key_sums_kernel(We
     run(std::false_type{}, whole, whole_end);
     run(std::true_type{}, whole_end, t1);
     int at = 0;
-    if (n_ranges > 1) at = uniform(items_before(a, lane, req, [&](const Req& y) { return cut.places(a, y); })) + k;
+    if (n_ranges > 1) at = uniform(items_before(a, all, lane, req, [&](const Req& y) { return cut.places(a, y); })) + k;
     if (at < 0 || at >= 2 * a.sums_items) continue;  // only of an offset table that is not ascending
 #pragma unroll
     for (int n = 0; n < 2; ++n) {
@@ -821,16 +857,17 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void key_sums_kernel(We
 // The row ranges' sums of every key tile of the requests that are cut into such, added range by range.
 __global__ __launch_bounds__(kSumKeys) void key_sums_join_kernel(WeightArgs a) {
   const int lane = threadIdx.x & 63;
-  const SumCut cut(a, lane);
+  const Requests all(a, lane);
+  const SumCut cut(a, all, lane);
   for (int item = blockIdx.x;; item += gridDim.x) {
     int req, base;
-    if (!find_request(a, lane, item, [&](const Req& x) { return cut.joins(a, x); }, &req, &base)) return;
-    const Req x = request(a, req);
+    if (!find_request(a, all, lane, item, [&](const Req& x) { return cut.joins(a, x); }, &req, &base)) return;
+    const Req x = all.one(a, req);
     const int n_ranges = uniform(cut.ranges(a, x)), k = uniform(item - base), n_kt = uniform(over(x.len, kSumKeys));
     const int kt = k % n_kt, head = k / n_kt, key = kt * kSumKeys + static_cast<int>(threadIdx.x);
     const int slot = uniform(owned_slot(a.index, req, a.w_rows, lane));
     if (slot < 0) continue;
-    int at = uniform(items_before(a, lane, req, [&](const Req& y) { return cut.places(a, y); })) + head * uniform(cut.per_head(a, x)) + kt;
+    int at = uniform(items_before(a, all, lane, req, [&](const Req& y) { return cut.places(a, y); })) + head * uniform(cut.per_head(a, x)) + kt;
     float sum = 0.0f;
     for (int j = 0; j < n_ranges; ++j) {
       const int n = uniform(cut.seen(a, x, n_ranges, j));
