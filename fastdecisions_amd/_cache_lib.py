@@ -43,7 +43,7 @@ SIGNATURES = {
     "fd_paged_gqa_fwd": (_i, [_p, _p, _p, _p, _p, _p, _p, _i, _i, _i, _f, _p, _i, _i, _p, _i64, _p]),
     "fd_paged_gqa_workspace_bytes": (_i64, [_i] * 9),
     "fd_paged_key_weights": (_i, [_p, _p, _p, _p, _p, _i, _p, _i, _i, _i, _f, _i, _p, _i, _i, _p, _i64, _p]),
-    "fd_paged_key_weights_workspace_bytes": (_i64, [_i] * 7),
+    "fd_paged_key_weights_workspace_bytes": (_i64, [_i] * 10),
     "fd_paged_kv_evict": (_i, [_p, _p, _p, _p, _i, _p, _p, _i64, _i, _i, _i, _i, _p, _p, _p]),
     "fd_gated_delta_step": (_i, [_p] * 8 + [_i, _p] + [_i] * 6 + [_f, _i, _i, _p, _i, _p]),
     "fd_packed_conv_state": (_i, [_p, _i64, _p, _p, _p, _p, _i, _p, _p, _p, _p] + [_i] * 5 + [_p, _i, _i, _p]),

@@ -23,6 +23,7 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kWaves = 4;
 constexpr int kCus = 256;
+constexpr int64_t kMostScores = 1LL << 28;  // bytes of kept scores: what the last-level cache may hold
 
 struct WeightArgs {
   PagedView c;                  // K alone
@@ -38,7 +39,10 @@ struct WeightArgs {
   int stats_items, sums_items;  // items that each kernel cuts its work into at most, but for one per tile that stays
   int slots;                    // workgroups that run at once
   int part_items;               // items of the row stats whose places the workspace holds
+  int32_t* cuts;                // what the kernels before have cut by: row stats (or scores), key sums
   float* part;                  // per item of the row stats: its rows' (m, l)
+  float* scores;                // [heads, tokens of the call x group, score_stride], few rows
+  int64_t score_stride;
   float* stats;                 // [heads, tokens of the call x group]: (m, 1 / l) of every row over all its keys
   float* sums;                  // per item of the key sums of a request cut into row ranges: its keys' sums
 };
@@ -180,7 +184,9 @@ struct Cut {
           return Size{static_cast<int64_t>(rt) * kt, static_cast<float>(rt) * (mean / S::kKeys + 0.5f), static_cast<float>(rt)};
         })) {
     fit(*this, a, all, lane);
+    if (blockIdx.x == 0 && threadIdx.x == 0) a.cuts[0] = c;
   }
+  __device__ __forceinline__ explicit Cut(const WeightArgs& a) : c(scalar_load(a.cuts, 0)) {}
   __device__ __forceinline__ int rtiles(const WeightArgs& a, const Req& x) const { return over(x.n_new * a.group, S::kRows); }
   __device__ __forceinline__ int ranges(const Req& x) const { return max(over(over(x.len, S::kKeys), c), 1); }
   // first row tile with keys in range v: later tokens see more keys
@@ -576,7 +582,7 @@ template <class S>
 __global__ __launch_bounds__(S::kRows) void row_stats_join_kernel(WeightArgs a) {
   const int lane = threadIdx.x & 63;
   const Requests all(a, lane);
-  const Cut<S> cut(a, all, lane);
+  const Cut<S> cut(a);
   for (int item = blockIdx.x;; item += gridDim.x) {
     int req, base;
     if (!find_request(a, all, lane, item, [&](const Req& x) { return cut.ranges(x) > 1 ? cut.rtiles(a, x) * a.kv_heads : 0; }, &req, &base)) return;
@@ -620,7 +626,9 @@ struct SumCut {
           return Size{static_cast<int64_t>(rt) * kt, static_cast<float>(rt) * (static_cast<float>(kt) - fresh), static_cast<float>(kt)};
         })) {
     fit(*this, a, all, lane);
+    if (blockIdx.x == 0 && threadIdx.x == 0) a.cuts[1] = c;
   }
+  __device__ __forceinline__ explicit SumCut(const WeightArgs& a) : c(scalar_load(a.cuts, 1)) {}
   __device__ __forceinline__ int ktiles(const WeightArgs& a, const Req& x) const { return x.n_new > 0 ? over(x.len, kSumKeys) * a.kv_heads : 0; }
   __device__ __forceinline__ int ranges(const WeightArgs& a, const Req& x) const { return max(over(over(x.n_new * a.group, kSumRows), c), 1); }
   // Ranges are counted from the last one on, which all key tiles have: the first `seen` key tiles have range j.
@@ -858,7 +866,7 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void key_sums_kernel(We
 __global__ __launch_bounds__(kSumKeys) void key_sums_join_kernel(WeightArgs a) {
   const int lane = threadIdx.x & 63;
   const Requests all(a, lane);
-  const SumCut cut(a, all, lane);
+  const SumCut cut(a);
   for (int item = blockIdx.x;; item += gridDim.x) {
     int req, base;
     if (!find_request(a, all, lane, item, [&](const Req& x) { return cut.joins(a, x); }, &req, &base)) return;
@@ -878,25 +886,246 @@ __global__ __launch_bounds__(kSumKeys) void key_sums_join_kernel(WeightArgs a) {
   }
 }
 
+// ---------------------------------------------------------------- few rows
+
+// How the scores cut a request: tiles of 16 rows times ranges of c tiles of kScoreKeys keys.
+constexpr int kScoreRows = 16, kScoreKeys = 64 * kWaves;
+struct ScoreCut {
+  int c;
+  __device__ __forceinline__ ScoreCut(const WeightArgs& a, const Requests& all, int lane)
+      : c(tiles_of_item(a, all, lane, a.stats_items, 1, 3, [&](const Req& x) {
+          const int rt = rtiles(a, x), kt = over(x.len, kScoreKeys);
+          return Size{static_cast<int64_t>(rt) * kt, static_cast<float>(rt * kt), static_cast<float>(rt)};
+        })) {
+    fit(*this, a, all, lane);
+    if (blockIdx.x == 0 && threadIdx.x == 0) a.cuts[0] = c;
+  }
+  __device__ __forceinline__ explicit ScoreCut(const WeightArgs& a) : c(scalar_load(a.cuts, 0)) {}
+  static __device__ __forceinline__ int rtiles(const WeightArgs& a, const Req& x) { return over(x.n_new * a.group, kScoreRows); }
+  __device__ __forceinline__ int ranges(const Req& x) const { return max(over(over(x.len, kScoreKeys), c), 1); }
+  __device__ __forceinline__ int items(const WeightArgs& a, const Req& x) const { return rtiles(a, x) * ranges(x) * a.kv_heads; }
+};
+
+// Scores of up to 16 rows, kept in the workspace in fp32, and their rows' (m, l) over the item's keys.  Every wavefront
+// takes blocks of 64 keys of its own, loaded straight into the operands' registers a block ahead: a lane's share of a
+// key is D / 4 features in a row (the steps of the product take any 32 features, the same ones of Q).
+template <int D, Format F>
+__global__ __launch_bounds__(kThreads, D == 256 && F == kBf16 ? 1 : 2) void key_scores_kernel(WeightArgs a) {
+  constexpr int kSteps = D / 32, kRowBytes = F == kBf16 ? 2 * D : F == kE4m3 ? D : D / 2;
+  constexpr int kBytes = kRowBytes / 4, kWords = kBytes < 16 ? 1 : kBytes / 16;  // of a lane and key
+  constexpr int kChunks = kBytes < 16 ? 2 : kWordChunks<F>;                      // eights of features in a word
+  constexpr int kScales = F == kE2m1 && D == 256 ? 2 : 1;
+  using Word = std::conditional_t<kBytes < 16, uint2, uint4>;
+  __shared__ float join[kWaves][kScoreRows][2];
+  const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
+  const int li = lane & 15, grp = lane >> 4;
+  const Requests all(a, lane);
+  const ScoreCut cut(a, all, lane);
+  for (int item = blockIdx.x; item < a.part_items; item += gridDim.x) {
+    int req, base;
+    if (!find_request(a, all, lane, item, [&](const Req& x) { return cut.items(a, x); }, &req, &base)) return;
+    const Req x = all.one(a, req);
+    const int n_rt = uniform(cut.rtiles(a, x)), n_ranges = uniform(cut.ranges(x)), k = uniform(item - base);
+    const int rtile = uniform(k % n_rt), hr = uniform(k / n_rt), range = uniform(hr % n_ranges), head = uniform(hr / n_ranges);
+    const int row0 = rtile * kScoreRows, rows = x.n_new * a.group, row = min(row0 + li, rows - 1), token = row / a.group;
+    const int pos = x.len - x.n_new + token, pos_min = uniform(x.len - x.n_new + row0 / a.group);
+    const int32_t* const table = a.c.table + req * a.c.table_stride;
+    const int first = range * cut.c * kScoreKeys + wave * 64, end = min(x.len, (range + 1) * cut.c * kScoreKeys);
+    const int mask = (1 << a.c.shift) - 1;
+    const unsigned char* const base_k = a.c.k + head * a.c.head + grp * kBytes;
+
+    struct Block {
+      Word w[4][kWords];
+      uint32_t s[4];   // E2M1: the bytes of the lane's features, E4M3: of the key
+    };
+    auto page_at = [&](int key) __attribute__((always_inline)) { return scalar_load(table, uniform(max(min(key, x.len - 1), 0)) >> a.c.shift); };
+    auto load = [&](int kb0, Block& b) __attribute__((always_inline)) {  // keys behind the last repeat it (the mask discards them)
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int page = valid_page(a, page_at(kb0 + 16 * u)), at = max(min(kb0 + 16 * u + li, x.len - 1), 0) & mask;
+        const Word* const p = reinterpret_cast<const Word*>(base_k + page * a.c.page + at * a.c.row);
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) b.w[u][i] = p[i];
+        if constexpr (F == kE4m3) b.s[u] = *scales_of<F, D>(a, page, head, at);
+        if constexpr (F == kE2m1) {
+          const uint8_t* const sp = scales_of<F, D>(a, page, head, at) + grp * D / 4 / kScaleBlock;
+          b.s[u] = kScales == 2 ? *reinterpret_cast<const uint16_t*>(sp) : *sp;
+        }
+      }
+    };
+    Block cur, next;
+    if (first < end) load(first, cur);
+    bf16x8_t qf[kSteps];
+    const uint16_t* const q = q_row(a, x, req, head, token, row - token * a.group) + grp * (D / 4);
+#pragma unroll
+    for (int kk = 0; kk < kSteps; ++kk) qf[kk] = *reinterpret_cast<const bf16x8_t*>(q + kk * 8);
+    float* const out = a.scores + (stat_row(a, x, req, head) + row) * a.score_stride + 4 * grp;
+    float m = -__builtin_inff(), l = 0.0f;  // of this lane's keys
+    for (int kb0 = first; kb0 < end; kb0 += kScoreKeys) {
+      if (kb0 + kScoreKeys < end) load(kb0 + kScoreKeys, next);
+      f32x4_t s[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        bf16x8_t kf[kSteps];
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) {
+          if constexpr (kBytes < 16) {
+            kf[0] = e2m1_to_bf16(cur.w[u][i].x, scale_of(cur.s[u]));
+            kf[1] = e2m1_to_bf16(cur.w[u][i].y, scale_of(cur.s[u]));
+          } else {
+            bf16x8_t y[kWordChunks<F>];
+            decode<F>(cur.w[u][i], F == kBf16 ? 1.0f : scale_of(kScales == 2 ? cur.s[u] >> (8 * i) & 255u : cur.s[u]), y);
+#pragma unroll
+            for (int e = 0; e < kChunks; ++e) kf[i * kChunks + e] = y[e];
+          }
+        }
+        s[u] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int kk = 0; kk < kSteps; ++kk) s[u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[kk], qf[kk], s[u], 0, 0, 0);
+      }
+      bool there = true;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) there &= static_cast<unsigned>(page_at(kb0 + 16 * u)) < static_cast<unsigned>(a.c.n_pages);
+      if (kb0 + 63 > pos_min || !there) {
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const bool here = static_cast<unsigned>(page_at(kb0 + 16 * u)) < static_cast<unsigned>(a.c.n_pages);
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (kb0 + 16 * u + 4 * grp + e > pos || !here) s[u][e] = -__builtin_inff();
+        }
+      }
+      // as in the row stats: the maximum is looked for where the sum shows that it is needed
+      auto exp_sum = [&](float sub) __attribute__((always_inline)) {
+        f32x4_t y = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) y[e] += __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][e], a.scale_log2, -sub));
+        return (y[0] + y[1]) + (y[2] + y[3]);
+      };
+      float sum = exp_sum(m);
+      if (__builtin_expect(__builtin_amdgcn_ballot_w64(!(sum < 0x1p64f)) != 0, 0)) {
+        float mx = s[0][0];
+#pragma unroll
+        for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i / 4][i % 4]);
+        const float m_new = fmaxf(m, mx * a.scale_log2), sub = m_new == -__builtin_inff() ? 0.0f : m_new;
+        l *= m_new == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(m - m_new);
+        m = m_new;
+        sum = exp_sum(sub);
+      }
+      l += sum;
+      if (row0 + li < rows) {
+#pragma unroll
+        for (int u = 0; u < 4; ++u) *reinterpret_cast<f32x4_t*>(out + kb0 + 16 * u) = s[u];
+      }
+      cur = next;
+    }
+    // ---- the lane groups' and the wavefronts' keys joined
+    auto join2 = [](float m, float l, float m2, float l2, float* mo, float* lo) __attribute__((always_inline)) {
+      const float top = fmaxf(m, m2), sub = top == -__builtin_inff() ? 0.0f : top;
+      *lo = l * __builtin_amdgcn_exp2f(m - sub) + l2 * __builtin_amdgcn_exp2f(m2 - sub);
+      *mo = top;
+    };
+#pragma unroll
+    for (int d = 16; d < 64; d *= 2) {
+      const float m2 = __shfl_xor(m, d), l2 = __shfl_xor(l, d);
+      join2(m, l, m2, l2, &m, &l);
+    }
+    __syncthreads();  // the item before has read its join
+    if (grp == 0) join[wave][li][0] = m, join[wave][li][1] = l;
+    __syncthreads();
+    if (wave == 0 && grp == 0) {
+#pragma unroll
+      for (int v = 1; v < kWaves; ++v) join2(m, l, join[v][li][0], join[v][li][1], &m, &l);
+      reinterpret_cast<float2*>(a.part)[static_cast<int64_t>(item) * kScoreRows + li] = float2{m, l};
+    }
+  }
+}
+
+// The kept scores' probabilities summed key by key, kAddKeys of a request's head per workgroup.
+constexpr int kAddKeys = 4 * kThreads;
+__global__ __launch_bounds__(kThreads) void key_scores_add_kernel(WeightArgs a) {
+  constexpr int kHold = 256;  // rows whose (m, 1 / l) are in LDS at a time
+  __shared__ float2 stats[kHold];
+  const int lane = threadIdx.x & 63;
+  const Requests all(a, lane);
+  const ScoreCut cut(a);
+  for (int item = blockIdx.x;; item += gridDim.x) {
+    int req, base;
+    if (!find_request(a, all, lane, item, [&](const Req& x) { return x.n_new > 0 ? over(x.len, kAddKeys) * a.kv_heads : 0; }, &req, &base)) return;
+    const Req x = all.one(a, req);
+    const int n_kt = uniform(over(x.len, kAddKeys)), head = uniform((item - base) / n_kt), kt = item - base - head * n_kt;
+    const int slot = uniform(owned_slot(a.index, req, a.w_rows, lane));
+    if (slot < 0) continue;
+    const int first = uniform(items_before(a, all, lane, req, [&](const Req& y) { return cut.items(a, y); }));
+    const int n_rt = uniform(cut.rtiles(a, x)), n_ranges = uniform(cut.ranges(x)), rows = x.n_new * a.group;
+    const int key0 = kt * kAddKeys + static_cast<int>(threadIdx.x);
+    const float* const scores = a.scores + stat_row(a, x, req, head) * a.score_stride;
+    float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int r0 = 0; r0 < rows; r0 += kHold) {
+      __syncthreads();  // the rows before are done with theirs
+      for (int i = threadIdx.x; i < min(kHold, rows - r0); i += kThreads) {
+        const int row = r0 + i, at = first + head * n_ranges * n_rt + row / kScoreRows;
+        const float2* const p = reinterpret_cast<const float2*>(a.part) + static_cast<int64_t>(at) * kScoreRows + row % kScoreRows;
+        // (every part has its place but those of an offset table that is not ascending)
+        const int n = at >= 0 && at + static_cast<int64_t>(n_ranges - 1) * n_rt < a.part_items ? n_ranges : 0;
+        float m = -__builtin_inff(), l = 0.0f;
+        for (int v0 = 0; v0 < n; v0 += 4) {
+          float2 y[4];
+#pragma unroll
+          for (int u = 0; u < 4; ++u) y[u] = p[static_cast<int64_t>(min(v0 + u, n - 1)) * n_rt * kScoreRows];
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            if (v0 + u >= n) continue;
+            const float top = fmaxf(m, y[u].x), sub = top == -__builtin_inff() ? 0.0f : top;
+            l = l * __builtin_amdgcn_exp2f(m - sub) + y[u].y * __builtin_amdgcn_exp2f(y[u].x - sub);
+            m = top;
+          }
+        }
+        stats[i] = stat_of(m, l);
+      }
+      __syncthreads();
+      for (int i = 0; i < min(kHold, rows - r0); ++i) {
+        const float2 y = stats[i];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const int key = min(key0 + u * kThreads, x.len - 1);
+          sum[u] = __builtin_fmaf(__builtin_amdgcn_exp2f(__builtin_fmaf(scores[(r0 + i) * a.score_stride + key], a.scale_log2, -y.x)), y.y, sum[u]);
+        }
+      }
+    }
+    float* const w = a.w + slot * a.w_row + head * a.w_head;
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (key0 + u * kThreads < x.len && sum[u] != 0.0f) w[key0 + u * kThreads] += sum[u];
+  }
+}
+
 // The kernels of a call, and its items and workspace, whatever the lengths turn out to be.
 struct Plan {
-  bool may_cut;
+  bool few, may_cut;
   int stats_items, sums_items, slots;
-  int64_t part_items, part_bytes, stats_bytes, bytes;
+  int64_t score_stride, part_items, part_bytes, stats_bytes, bytes;
 };
-Plan plan_of(int64_t requests, int64_t tokens, int group, int kv_heads, int head_dim) {
+constexpr int kHeaderBytes = 256;  // of the workspace: the cuts
+Plan plan_of(int64_t requests, int64_t tokens, int group, int kv_heads, int head_dim, int64_t max_keys, int64_t max_rows) {
   Plan p;
-  constexpr int rows = Stats<64>::kRows;
-  p.slots = kCus * (head_dim == 256 ? 1 : 2);
+  const int64_t rows_all = kv_heads * tokens * group;
+  p.score_stride = (max_keys + 63) / 64 * 64;
+  const int64_t score_bytes = rows_all * p.score_stride * 4;
+  p.few = max_rows <= kScoreRows && score_bytes <= kMostScores;
+  const int rows = p.few ? kScoreRows : Stats<64>::kRows;
+  p.slots = kCus * (head_dim == 256 && !p.few ? 1 : 2);
   p.stats_items = 2048;
   p.sums_items = 2048;
   // a share alone may add a range per row tile
   p.part_items = p.stats_items + kv_heads * (tokens * group / rows + requests);
   p.part_bytes = (p.part_items * rows * 8 + 15) / 16 * 16;
+  p.stats_bytes = p.few ? score_bytes : (rows_all * 8 + 15) / 16 * 16;
   // a range of row tiles is four at least, and a request without more is never cut
-  p.may_cut = tokens * group > 4 * kSumRows;
-  p.stats_bytes = (kv_heads * tokens * group * 8 + 15) / 16 * 16;
-  p.bytes = p.part_bytes + p.stats_bytes + (p.may_cut ? 2LL * p.sums_items * kSumKeys * 4 : 0);
+  p.may_cut = !p.few && tokens * group > 4 * kSumRows;
+  p.bytes = kHeaderBytes + p.part_bytes + p.stats_bytes + (p.may_cut ? 2LL * p.sums_items * kSumKeys * 4 : 0);
   return p;
 }
 
@@ -914,11 +1143,16 @@ int check_sizes(const char* what, int batch, int q_heads, int kv_heads, int seq_
 
 }  // namespace
 
-extern "C" int64_t fd_paged_key_weights_workspace_bytes(int batch, int q_heads, int kv_heads, int seq_len, int n_seqs,
-                                                        int max_seqlen, int last) {
+extern "C" int64_t fd_paged_key_weights_workspace_bytes(int batch, int q_heads, int kv_heads, int seq_len, int head_dim,
+                                                        int page_size, int max_pages, int n_seqs, int max_seqlen, int last) {
   static const char* what = "fd_paged_key_weights_workspace_bytes";
   if (int rc = check_sizes(what, batch, q_heads, kv_heads, seq_len, n_seqs, max_seqlen, last)) return rc;
-  return plan_of(n_seqs > 0 ? n_seqs : batch, static_cast<int64_t>(batch) * seq_len, q_heads / kv_heads, kv_heads, 64).bytes;
+  FD_REQUIRE(head_dim == 64 || head_dim == 128 || head_dim == 256, FD_ERR_UNSUPPORTED,
+             "%s: head_dim must be 64, 128 or 256 (got %d)", what, head_dim);
+  FD_REQUIRE(page_size >= 1 && max_pages >= 1, FD_ERR_INVALID_ARGUMENT, "%s: page_size and max_pages must be >= 1", what);
+  return plan_of(n_seqs > 0 ? n_seqs : batch, static_cast<int64_t>(batch) * seq_len, q_heads / kv_heads, kv_heads, head_dim,
+                 static_cast<int64_t>(max_pages) * page_size,
+                 static_cast<int64_t>(last > 0 ? std::min(last, max_seqlen) : max_seqlen) * (q_heads / kv_heads)).bytes;
 }
 
 extern "C" int fd_paged_key_weights(const void* q, const fd_paged_cache* cache, float* weights, const int64_t q_strides[4],
@@ -940,7 +1174,9 @@ extern "C" int fd_paged_key_weights(const void* q, const fd_paged_cache* cache, 
   FD_REQUIRE(weight_strides[0] >= 0 && weight_strides[1] >= 0, FD_ERR_INVALID_ARGUMENT, "%s: weight strides must be >= 0", what);
   if (requests == 0 || seq_len == 0) return FD_OK;
   const int group = q_heads / cache->kv_heads;
-  const Plan p = plan_of(requests, static_cast<int64_t>(batch) * seq_len, group, cache->kv_heads, cache->head_dim);
+  const int64_t max_keys = static_cast<int64_t>(cache->max_pages) * cache->page_size;
+  const Plan p = plan_of(requests, static_cast<int64_t>(batch) * seq_len, group, cache->kv_heads, cache->head_dim, max_keys,
+                         static_cast<int64_t>(last > 0 ? std::min(last, max_seqlen) : max_seqlen) * group);
   FD_REQUIRE(p.part_items < (1LL << 31), FD_ERR_UNSUPPORTED, "%s: problem too large", what);
   FD_REQUIRE(workspace && fd_aligned16(workspace) && workspace_bytes >= p.bytes, FD_ERR_INVALID_ARGUMENT,
              "%s: the workspace must be 16-byte aligned and hold %lld bytes", what, static_cast<long long>(p.bytes));
@@ -963,13 +1199,15 @@ extern "C" int fd_paged_key_weights(const void* q, const fd_paged_cache* cache, 
   a.slots = p.slots;
   a.part_items = static_cast<int>(p.part_items);
   a.scale_log2 = scale * 1.4426950408889634f;
-  a.part = static_cast<float*>(workspace);
-  a.stats = reinterpret_cast<float*>(static_cast<char*>(workspace) + p.part_bytes);
-  a.sums = reinterpret_cast<float*>(static_cast<char*>(workspace) + p.part_bytes + p.stats_bytes);
+  char* const work = static_cast<char*>(workspace);
+  a.cuts = reinterpret_cast<int32_t*>(work);
+  a.part = reinterpret_cast<float*>(work + kHeaderBytes);
+  a.scores = a.stats = reinterpret_cast<float*>(work + kHeaderBytes + p.part_bytes);
+  a.score_stride = p.score_stride;
+  a.sums = reinterpret_cast<float*>(work + kHeaderBytes + p.part_bytes + p.stats_bytes);
   hipStream_t s = static_cast<hipStream_t>(stream);
   // workgroups: no more than the sizes can make items
-  const int64_t key_tiles = static_cast<int64_t>(requests) * cache->kv_heads *
-                            ((static_cast<int64_t>(cache->max_pages) * cache->page_size + kSumKeys - 1) / kSumKeys);
+  const int64_t heads = static_cast<int64_t>(requests) * cache->kv_heads, key_tiles = heads * ((max_keys + kSumKeys - 1) / kSumKeys);
   const int64_t row_tiles = (static_cast<int64_t>(batch) * seq_len * group + kSumRows - 1) / kSumRows;
   const unsigned stats_grid = static_cast<unsigned>(std::min<int64_t>(p.part_items, 2048));
   const unsigned sums_grid = static_cast<unsigned>(std::min<int64_t>(key_tiles * std::max<int64_t>(row_tiles / 4, 1), 2048));
@@ -977,11 +1215,19 @@ extern "C" int fd_paged_key_weights(const void* q, const fd_paged_cache* cache, 
   by_kind(cache, [&](auto d, auto f) {
     constexpr int D = decltype(d)::value;
     constexpr Format F = decltype(f)::value;
+    if (p.few) {
+      hipLaunchKernelGGL((key_scores_kernel<D, F>), dim3(stats_grid), dim3(kThreads), 0, s, a);
+      return;
+    }
     hipLaunchKernelGGL((row_stats_kernel<D, F>), dim3(stats_grid), dim3(kThreads), 0, s, a);
     hipLaunchKernelGGL((row_stats_join_kernel<Stats<D>>), dim3(static_cast<unsigned>(std::min<int64_t>(p.part_items - p.stats_items, 1024))),
                        dim3(Stats<D>::kRows), 0, s, a);
     hipLaunchKernelGGL((key_sums_kernel<D, F>), dim3(sums_grid), dim3(kThreads), 0, s, a);
   });
+  if (p.few) {
+    const unsigned grid = static_cast<unsigned>(std::min<int64_t>(heads * ((max_keys + kAddKeys - 1) / kAddKeys), 4096));
+    hipLaunchKernelGGL(key_scores_add_kernel, dim3(grid), dim3(kThreads), 0, s, a);
+  }
   if (p.may_cut) hipLaunchKernelGGL(key_sums_join_kernel, dim3(join_grid), dim3(kSumKeys), 0, s, a);
   return fd_check_launch(what);
 }

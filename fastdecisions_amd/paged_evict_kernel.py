@@ -37,9 +37,11 @@ from .paged_kv_kernel import cache_dim, check_cache, check_cu_seqlens, check_row
 
 
 @lru_cache(maxsize=4096)
-def workspace_bytes(batch: int, q_heads: int, kv_heads: int, seq_len: int, n_seqs: int, max_seqlen: int, last: int) -> int:
+def workspace_bytes(batch: int, q_heads: int, kv_heads: int, seq_len: int, head_dim: int, page_size: int, max_pages: int,
+                    n_seqs: int, max_seqlen: int, last: int) -> int:
     """Device workspace of a call of these sizes (``fd_paged_key_weights_workspace_bytes``)."""
-    nbytes = _cache_lib.lib().fd_paged_key_weights_workspace_bytes(batch, q_heads, kv_heads, seq_len, n_seqs, max_seqlen, last)
+    nbytes = _cache_lib.lib().fd_paged_key_weights_workspace_bytes(batch, q_heads, kv_heads, seq_len, head_dim, page_size,
+                                                                   max_pages, n_seqs, max_seqlen, last)
     _cache_lib.check("fd_paged_key_weights_workspace_bytes", nbytes)
     return nbytes
 
@@ -113,8 +115,8 @@ def paged_key_weights(
         with torch.cuda.device(device):
             return paged_key_weights(q, k_cache, page_table, cache_lens, weights, k_scale=k_scale, scale=scale,
                                      cu_seqlens=cu_seqlens, max_seqlen=max_seqlen, last=last, row_indices=row_indices)
-    sizes = (batch, q_heads, kv_heads, seq_len, n_seqs, int(max_seqlen), int(last or 0))
-    nbytes = workspace_bytes(*sizes)
+    nbytes = workspace_bytes(batch, q_heads, kv_heads, seq_len, dim, page_size, page_table.shape[1], n_seqs, int(max_seqlen),
+                             int(last or 0))
     work = torch.empty(nbytes, device=q.device, dtype=torch.uint8)
     _cache_lib.check("fd_paged_key_weights", _cache_lib.lib().fd_paged_key_weights(
         q_ptr, cache, weights.data_ptr(), q_strides, _cache_lib.pack2(*weights.stride()[:2]), weights.shape[0], index, batch,

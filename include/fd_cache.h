@@ -166,8 +166,8 @@ FD_API int fd_paged_key_weights(const void* q, const fd_paged_cache* cache, floa
                                 int max_seqlen, void* workspace, int64_t workspace_bytes, void* stream);
 
 /* Workspace of fd_paged_key_weights for these sizes, or a negative FD_ERR_* code. */
-FD_API int64_t fd_paged_key_weights_workspace_bytes(int batch, int q_heads, int kv_heads, int seq_len, int n_seqs,
-                                                    int max_seqlen, int last);
+FD_API int64_t fd_paged_key_weights_workspace_bytes(int batch, int q_heads, int kv_heads, int seq_len, int head_dim,
+                                                    int page_size, int max_pages, int n_seqs, int max_seqlen, int last);
 
 /*
  * Cuts every request to at most `keep` keys: its `recent` last ones and, per key head, those of largest weight among the

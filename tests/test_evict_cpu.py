@@ -35,8 +35,11 @@ def test_key_weights_refuse_bad_arguments():
     assert weigh(batch=0) == _lib.FD_OK and weigh(t=0) == _lib.FD_OK
     assert b"fd_paged_key_weights" in lib.fd_cache_last_error()
     size = lib.fd_paged_key_weights_workspace_bytes
-    assert size(1, 16, 3, 1, 0, 1, 0) == INV and size(1, 16, 4, 1, 0, 2, 0) == INV and size(1, 16, 4, 1, 0, 1, -1) == INV
-    assert size(1, 16, 4, 1, 0, 1, 0) > 0
+    assert size(1, 16, 3, 1, 128, 16, 4, 0, 1, 0) == INV and size(1, 16, 4, 1, 128, 16, 4, 0, 2, 0) == INV
+    assert size(1, 16, 4, 1, 128, 16, 4, 0, 1, -1) == INV and size(1, 16, 4, 1, 128, 16, 0, 0, 1, 0) == INV
+    assert size(1, 16, 4, 1, 96, 16, 4, 0, 1, 0) == UNS and size(1, 16, 4, 1, 128, 16, 4, 0, 1, 0) > 0
+    # kept scores stay within a bound, whatever the page table's width
+    assert size(64, 16, 4, 1, 128, 64, 1 << 20, 0, 1, 0) < 1 << 29 and size(1, 16, 4, 131072, 128, 64, 2048, 0, 131072, 0) < 1 << 29
 
 
 def test_evict_refuses_bad_arguments():
