@@ -60,8 +60,10 @@ struct Few {
   static constexpr int kScaleCopies = FP8 ? 1 : FP4 ? (D == 256 ? 2 : 1) : 0;
   static constexpr int kScaleBytes = 256 * kScaleCopies;
   static constexpr int kStageBytes = 2 * kBlockBytes + kScaleBytes;
-  static constexpr int kStages = kBlockBytes >= 8192 ? 1 : kBlockBytes <= 2048 ? 4 : 8192 / kBlockBytes;
-  static constexpr int kDecoded = FP4 ? 2048 : 0;       // 32 features of a V block as bf16
+  // E2M1 blocks leave their stage for registers at once, so half as many do
+  static constexpr int kStages = FP4 ? 4096 / kBlockBytes : kBlockBytes >= 8192 ? 1 : 8192 / kBlockBytes;
+  static constexpr int kWide = D < 128 ? D : 128;       // features of an E2M1 V block that are bf16 in LDS at a time
+  static constexpr int kDecoded = FP4 ? 32 * 2 * kWide : 0;
   static constexpr int kCopies = kBlockBytes / 1024;    // copy instructions of a block's K (or V)
   static constexpr int kCopyRows = 1024 / kRowBytes;
   static constexpr int kKGroup = kCopies + kScaleCopies;
@@ -619,7 +621,42 @@ __global__ __launch_bounds__(S::kThreads, S::kPerCu) void paged_gqa_few_kernel(P
     for (int db = 0; db < kNdb; ++db) o[n][db] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
   }
   bf16x8_t pb[NR], pl[NR];  // probabilities, in two parts
-  uint32_t v_scales[D == 256 ? 2 : 1];  // E2M1: of V's row lane / 2, read before the next K's scales take their place
+// E2M1: a block's codes and scales on their way from LDS: K of this lane's two keys, V of half a row
+  uint32_t k_codes[2][FP4 ? kKk : 1], v_codes[FP4 ? D / 16 : 1], v_scales[D == 256 ? 2 : 1];
+  float k_scales[2][D == 256 ? 2 : 1];
+  auto take = [&](int j) {
+    const unsigned char* const st = stage0 + (j & (NS - 1)) * S::kStageBytes;
+    const unsigned char* const sc = st + 2 * S::kBlockBytes;
+    auto words = [](const unsigned char* p, uint32_t* to) {
+      const uint4 w = *reinterpret_cast<const uint4*>(p);
+      to[0] = w.x, to[1] = w.y, to[2] = w.z, to[3] = w.w;
+    };
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int row = sigma16(h, li), swz = few_swz_k<RBY>(row);
+      if constexpr (D == 64) {
+        const uint2 w = *reinterpret_cast<const uint2*>(st + row * RBY + ((grp >> 1) ^ swz) * 16 + 8 * (grp & 1));
+        k_codes[h][0] = w.x, k_codes[h][1] = w.y;
+        k_scales[h][0] = scale_of(sc[row * 4 + (grp >> 1)]);
+      } else {
+#pragma unroll
+        for (int c = 0; c < D / 128; ++c) {
+          words(st + row * RBY + ((grp * (D / 128) + c) ^ swz) * 16, &k_codes[h][4 * c]);
+          k_scales[h][c] = scale_of(sc[row * (D / kScaleBlock) + grp * (D / 128) + c]);
+        }
+      }
+    }
+    // V: of every S::kWide features of row lane / 2 the lane takes half, in 16-byte chunks
+    const int row = lane >> 1, half = lane & 1, swz = few_swz_v<RBY, kE2m1>(row);
+#pragma unroll
+    for (int c = 0; c < D / 64; ++c) {
+      constexpr int kHalf = S::kWide / 64;  // chunks of a lane in S::kWide features
+      words(st + S::kBlockBytes + row * RBY + (((c / kHalf) * 2 * kHalf + half * kHalf + c % kHalf) ^ swz) * 16, &v_codes[4 * c]);
+    }
+#pragma unroll
+    for (int c = 0; c < (D == 256 ? 2 : 1); ++c)
+      v_scales[c] = reinterpret_cast<const uint32_t*>(sc + (D == 256 ? 256 : 128))[row * (D == 256 ? 2 : 1) + c];
+  };
 
   auto scores = [&](int j) {
     const unsigned char* const st = stage0 + (j & (NS - 1)) * S::kStageBytes;
@@ -631,28 +668,11 @@ __global__ __launch_bounds__(S::kThreads, S::kPerCu) void paged_gqa_few_kernel(P
     for (int h = 0; h < 2; ++h) {
       const int row = sigma16(h, li);
       const int swz = few_swz_k<RBY>(row);
-      uint32_t codes[kKk];  // E2M1: this lane's D / 4 of the key
-      float scales[D == 256 ? 2 : 1];
-      if constexpr (FP4) {
-        const uint8_t* const sc = st + 2 * S::kBlockBytes;
-        if constexpr (D == 64) {
-          const uint2 w = *reinterpret_cast<const uint2*>(st + row * RBY + ((grp >> 1) ^ swz) * 16 + 8 * (grp & 1));
-          codes[0] = w.x, codes[1] = w.y;
-          scales[0] = scale_of(sc[row * 4 + (grp >> 1)]);
-        } else {
-#pragma unroll
-          for (int c = 0; c < D / 128; ++c) {
-            const uint4 w = *reinterpret_cast<const uint4*>(st + row * RBY + ((grp * (D / 128) + c) ^ swz) * 16);
-            codes[4 * c] = w.x, codes[4 * c + 1] = w.y, codes[4 * c + 2] = w.z, codes[4 * c + 3] = w.w;
-            scales[c] = scale_of(sc[row * (D / kScaleBlock) + grp * (D / 128) + c]);
-          }
-        }
-      }
 #pragma unroll
       for (int kk = 0; kk < kKk; ++kk) {
         bf16x8_t kf;
         if constexpr (FP4) {
-          kf = e2m1_to_bf16(codes[kk], scales[kk / 4]);
+          kf = e2m1_to_bf16(k_codes[h][kk], k_scales[h][kk / 4]);
         } else if constexpr (FP8) {
           const uint2 w = *reinterpret_cast<const uint2*>(st + row * RBY + ((2 * kk + (grp >> 1)) ^ swz) * 16 + 8 * (grp & 1));
           kf = codes_to_bf16(w.x, w.y);
@@ -662,11 +682,6 @@ __global__ __launch_bounds__(S::kThreads, S::kPerCu) void paged_gqa_few_kernel(P
 #pragma unroll
         for (int n = 0; n < NR; ++n) s[n][h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[n][kk], s[n][h], 0, 0, 0);
       }
-    }
-    if constexpr (FP4) {
-#pragma unroll
-      for (int c = 0; c < (D == 256 ? 2 : 1); ++c)
-        v_scales[c] = reinterpret_cast<const uint32_t*>(st + 2 * S::kBlockBytes + (D == 256 ? 256 : 128))[(lane >> 1) * (D == 256 ? 2 : 1) + c];
     }
     float ks[8], vs[8];
     if constexpr (FP8) {
@@ -795,56 +810,62 @@ __global__ __launch_bounds__(S::kThreads, S::kPerCu) void paged_gqa_few_kernel(P
       }
   };
 
-  // E2M1: 32 features of V at a time become bf16 in LDS of the wavefront (a lane: half a row of them, one scale), from
-  // where the transposing reads take them; their features' products follow.
-  auto p_v_codes = [&](int j) {
-    const unsigned char* const st = stage0 + (j & (NS - 1)) * S::kStageBytes + S::kBlockBytes;
-    unsigned char* const bf = smem + S::kWaves * NS * S::kStageBytes + wave * S::kDecoded;
-    const bool masked = first + j * S::kKeys + 31 > pos_min || absent;
-    const int row = lane >> 1, half = lane & 1;
-    auto chunk_of = [](int r, int c) { return c ^ (((r >> 3) & 1) << 1); };  // physical chunk of row r: lane groups' rows apart
+  // E2M1: V becomes bf16 in LDS of the wavefront, S::kWide features at a time, from where the transposing reads take it.
+  constexpr int VBY = 2 * S::kWide;  // bytes of a row there
+  unsigned char* const wide = smem + S::kWaves * NS * S::kStageBytes + wave * S::kDecoded;
+  auto widen_v = [&](int part) {
+    const int row = lane >> 1, half = lane & 1, swz = few_swz_v<VBY, kBf16>(row);
+    constexpr int kEights = S::kWide / 16;  // of a lane
 #pragma unroll
-    for (int c = 0; c < D / kScaleBlock; ++c) {
-      const uint2 w = *reinterpret_cast<const uint2*>(st + row * RBY + (c ^ few_swz_v<RBY, kE2m1>(row)) * 16 + 8 * half);
-      const float scale = scale_of(v_scales[c / 4] >> (8 * (c % 4)) & 255u);
-      *reinterpret_cast<bf16x8_t*>(bf + row * 64 + chunk_of(row, 2 * half) * 16) = e2m1_to_bf16(w.x, scale);
-      *reinterpret_cast<bf16x8_t*>(bf + row * 64 + chunk_of(row, 2 * half + 1) * 16) = e2m1_to_bf16(w.y, scale);
-      bf16x8_t vf[2];  // V[key 8 grp + i][32 c + 16 u + li]
+    for (int c = 0; c < kEights; ++c) {
+      const int block = part * (S::kWide / kScaleBlock) + c / 4;  // scale of half 0; half 1's lies S::kWide / 64 further
+      const uint32_t word = v_scales[block / 4] >> (half * (S::kWide / 64) * 8);
+      const float scale = scale_of(word >> (8 * (block % 4)) & 255u);
+      *reinterpret_cast<bf16x8_t*>(wide + row * VBY + ((half * kEights + c) ^ swz) * 16) = e2m1_to_bf16(v_codes[part * kEights + c], scale);
+    }
+  };
+  auto p_v_wide = [&](int j, int part) {
+    constexpr int kDb = S::kWide / 16;
+    bf16x8_t vf[kDb];  // V[key 8 grp + i][S::kWide part + 16 db + li]
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const int r = 8 * grp + (li >> 2);
-        const unsigned char* vp = bf + r * 64 + chunk_of(r, 2 * u + ((li & 3) >> 1)) * 16 + 8 * (li & 1);
-        const v4i16_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16_t*)vp);
-        const v4i16_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16_t*)(vp + 4 * 64));
-        const short __attribute__((ext_vector_type(8))) vv = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-        vf[u] = __builtin_bit_cast(bf16x8_t, vv);
-      }
-      if (masked && (__builtin_amdgcn_ballot_w64(any_odd(vf[0])) | __builtin_amdgcn_ballot_w64(any_odd(vf[1]))) != 0) {
-        // blocks of NaN leave the product and are added by hand to the rows that see them
+    for (int db = 0; db < kDb; ++db) {
+      const int row = 8 * grp + (li >> 2);
+      const unsigned char* vp = wide + row * VBY + ((2 * db + ((li & 3) >> 1)) ^ few_swz_v<VBY, kBf16>(row)) * 16 + 8 * (li & 1);
+      const v4i16_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16_t*)vp);
+      const v4i16_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16_t*)(vp + 4 * VBY));
+      const short __attribute__((ext_vector_type(8))) vv = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+      vf[db] = __builtin_bit_cast(bf16x8_t, vv);
+    }
+    if (first + j * S::kKeys + 31 > pos_min || absent) {
+      bool odd = false;
 #pragma unroll
-        for (int u = 0; u < 2; ++u) vf[u] = without_odd(vf[u]);
+      for (int db = 0; db < kDb; ++db) odd |= any_odd(vf[db]);
+      if (__builtin_amdgcn_ballot_w64(odd) != 0) {  // blocks of NaN: as in p_v
+#pragma unroll
+        for (int db = 0; db < kDb; ++db) vf[db] = without_odd(vf[db]);
 #pragma unroll 1
         for (int key = 0; key < 32; ++key) {
+          float ph[NR];
 #pragma unroll
-          for (int u = 0; u < 2; ++u) {
+          for (int n = 0; n < NR; ++n) ph[n] = __shfl(element(pb[n], key & 7) + element(pl[n], key & 7), 16 * (key >> 3) + li);
+#pragma unroll
+          for (int db = 0; db < kDb; ++db) {
             const f32x4_t x = __builtin_convertvector(*reinterpret_cast<const bf16x4_t*>(
-                bf + key * 64 + chunk_of(key, 2 * u + (grp >> 1)) * 16 + 8 * (grp & 1)), f32x4_t);
+                wide + key * VBY + ((2 * db + (grp >> 1)) ^ few_swz_v<VBY, kBf16>(key)) * 16 + 8 * (grp & 1)), f32x4_t);
 #pragma unroll
-            for (int n = 0; n < NR; ++n) {
-              const float ph = __shfl(element(pb[n], key & 7) + element(pl[n], key & 7), 16 * (key >> 3) + li);
-              o[n][2 * c + u] = add_odd(o[n][2 * c + u], x, ph);
-            }
+            for (int n = 0; n < NR; ++n) o[n][part * kDb + db] = add_odd(o[n][part * kDb + db], x, ph[n]);
           }
         }
       }
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int n = 0; n < NR; ++n) {
-          o[n][2 * c + u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf[u], pb[n], o[n][2 * c + u], 0, 0, 0);
-          o[n][2 * c + u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf[u], pl[n], o[n][2 * c + u], 0, 0, 0);
-        }
     }
+#pragma unroll
+    for (int db = 0; db < kDb; ++db)
+#pragma unroll
+      for (int n = 0; n < NR; ++n) {
+        f32x4_t& y = o[n][part * kDb + db];
+        y = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf[db], pb[n], y, 0, 0, 0);
+        y = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf[db], pl[n], y, 0, 0, 0);
+      }
   };
 
   // ---- the loop: copies in the queue, oldest first, at block j's scores: K(j) V(j) .. K(j + NS - 1) V(j + NS - 1)
@@ -852,6 +873,27 @@ __global__ __launch_bounds__(S::kThreads, S::kPerCu) void paged_gqa_few_kernel(P
   Pages next = pages_of(NS);
   for (int j = 0; j < mine; ++j) {
     const bool more = j + NS < mine;
+    if constexpr (FP4) {
+      // the block leaves its stage for registers, and the stage's next copies leave before any of its work
+      if (more || j + NS == mine) wait_copies<(NS - 1) * kBoth>();
+      else wait_copies<0>();
+      take(j);
+      wait_lds_reads();
+      if (more) {
+        copy_k(next, j + NS);
+        copy_v(next, j + NS);
+      }
+      next = pages_of(j + NS + 1);
+      widen_v(0);
+      scores(j);
+      p_v_wide(j, 0);
+#pragma unroll
+      for (int part = 1; part < D / S::kWide; ++part) {
+        widen_v(part);
+        p_v_wide(j, part);
+      }
+      continue;
+    }
     if (more || j + NS == mine) wait_copies<S::kCopies + (NS - 1) * kBoth>();  // K(j) has landed
     else wait_copies<0>();
     scores(j);
@@ -862,8 +904,7 @@ __global__ __launch_bounds__(S::kThreads, S::kPerCu) void paged_gqa_few_kernel(P
     } else {
       wait_copies<0>();
     }
-    if constexpr (FP4) p_v_codes(j);
-    else p_v(j);
+    p_v(j);
     wait_lds_reads();
     if (more) copy_v(next, j + NS);
     next = pages_of(j + NS + 1);

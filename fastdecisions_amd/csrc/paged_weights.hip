@@ -1209,8 +1209,8 @@ extern "C" int fd_paged_key_weights(const void* q, const fd_paged_cache* cache, 
   // workgroups: no more than the sizes can make items
   const int64_t heads = static_cast<int64_t>(requests) * cache->kv_heads, key_tiles = heads * ((max_keys + kSumKeys - 1) / kSumKeys);
   const int64_t row_tiles = (static_cast<int64_t>(batch) * seq_len * group + kSumRows - 1) / kSumRows;
-  const unsigned stats_grid = static_cast<unsigned>(std::min<int64_t>(p.part_items, 2048));
-  const unsigned sums_grid = static_cast<unsigned>(std::min<int64_t>(key_tiles * std::max<int64_t>(row_tiles / 4, 1), 2048));
+  const unsigned stats_grid = static_cast<unsigned>(std::min<int64_t>(p.part_items, 2 * p.slots));
+  const unsigned sums_grid = static_cast<unsigned>(std::min<int64_t>(key_tiles * std::max<int64_t>(row_tiles / 4, 1), 2 * p.slots));
   const unsigned join_grid = static_cast<unsigned>(std::min<int64_t>(key_tiles, p.sums_items));
   by_kind(cache, [&](auto d, auto f) {
     constexpr int D = decltype(d)::value;
