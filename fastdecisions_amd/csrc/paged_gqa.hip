@@ -621,7 +621,7 @@ __global__ __launch_bounds__(S::kThreads, S::kPerCu) void paged_gqa_few_kernel(P
     for (int db = 0; db < kNdb; ++db) o[n][db] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
   }
   bf16x8_t pb[NR], pl[NR];  // probabilities, in two parts
-// E2M1: a block's codes and scales on their way from LDS: K of this lane's two keys, V of half a row
+  // E2M1: a block's codes and scales on their way from LDS: K of this lane's two keys, V of half a row
   uint32_t k_codes[2][FP4 ? kKk : 1], v_codes[FP4 ? D / 16 : 1], v_scales[D == 256 ? 2 : 1];
   float k_scales[2][D == 256 ? 2 : 1];
   auto take = [&](int j) {

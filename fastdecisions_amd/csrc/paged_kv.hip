@@ -1,8 +1,8 @@
 // Writing and reading a paged key/value cache, gfx950.
 //
 // Streaming kernels, bound by HBM (and by the launch for a few tokens).  head_dim
-// / 8 lanes own one (token, head) row of K or V, 16 bytes of bf16 each, so a
-// wavefront moves 1 KiB in one instruction; blockIdx.y picks K or V.
+// / 8 lanes (E2M1: / 16) own one (token, head) row of K or V, 16 bytes of bf16 each
+// (32), so a wavefront moves 1 KiB in one instruction; blockIdx.y picks K or V.
 //
 // Quantising (E4M3): a row's scale is the smallest power of two 2^E with
 // max|x| <= 448 2^E.  With A = max|x| = m 2^k, m in [1, 2), and 448 = 1.75 2^8 that
@@ -98,10 +98,14 @@ __device__ __forceinline__ void requests_of(const int32_t* cu, int n_seqs, const
     if (!(cu[r[u]] <= t[u] && t[u] < cu[r[u] + 1])) r[u] = -1;
 }
 
+// Features of a row per lane: 16 bytes of bf16; with E2M1 twice as many, whose codes are 8 bytes.
+template <Format F>
+constexpr int kLane = F == kE2m1 ? 16 : 8;
+
 // U rows per thread, kThreads / kLanes apart, a stage of all of them at a time: rows, requests, pages, stores.
 template <int D, Format F, int U>
 __global__ __launch_bounds__(kThreads) void paged_kv_write_kernel(WriteArgs a) {
-  constexpr int kLanes = D / 8, kSide = kThreads / kLanes;  // lanes of a row; rows of a workgroup side by side
+  constexpr int kLanes = D / kLane<F>, kVecs = kLane<F> / 8, kSide = kThreads / kLanes;  // lanes of a row; rows of a workgroup side by side
   constexpr int kPer = D / kScaleBlock;             // E2M1 scales of a row
   const int side = blockIdx.y;
   const int li = threadIdx.x % kLanes;
@@ -110,7 +114,7 @@ __global__ __launch_bounds__(kThreads) void paged_kv_write_kernel(WriteArgs a) {
                 xt = side == 0 ? a.xs[0][2] : a.xs[1][2];
   const int64_t tokens = static_cast<int64_t>(a.batch) * a.seq_len;
   int head[U], t[U], r[U], pos[U], page[U];
-  uint4 w[U];
+  uint4 w[U][kVecs];
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     const int64_t row = (static_cast<int64_t>(blockIdx.x) * U + u) * kSide + threadIdx.x / kLanes;
@@ -119,8 +123,11 @@ __global__ __launch_bounds__(kThreads) void paged_kv_write_kernel(WriteArgs a) {
     const int b = a.cu == nullptr ? static_cast<int>(token / a.seq_len) : 0;
     t[u] = static_cast<int>(token - static_cast<int64_t>(b) * a.seq_len);
     r[u] = token < tokens ? b : -1;
-    w[u] = {0, 0, 0, 0};
-    if (token < tokens) w[u] = *reinterpret_cast<const uint4*>(x_side + b * xb + head[u] * xh + t[u] * xt + li * 8);
+#pragma unroll
+    for (int i = 0; i < kVecs; ++i) {
+      w[u][i] = {0, 0, 0, 0};
+      if (token < tokens) w[u][i] = *reinterpret_cast<const uint4*>(x_side + b * xb + head[u] * xh + t[u] * xt + (li * kVecs + i) * 8);
+    }
   }
   if (a.cu != nullptr) {
     int found[U];
@@ -146,40 +153,46 @@ __global__ __launch_bounds__(kThreads) void paged_kv_write_kernel(WriteArgs a) {
     const int at = pos[u] & ((1 << a.c.shift) - 1);
     unsigned char* dst = (side == 0 ? a.c.k : a.c.v) + page[u] * a.c.page + head[u] * a.c.head + at * a.c.row;
     if constexpr (F == kBf16) {
-      if (live) *reinterpret_cast<uint4*>(dst + li * 16) = w[u];
+      if (live) *reinterpret_cast<uint4*>(dst + li * 16) = w[u][0];
     } else {
-      const uint32_t h[4] = {w[u].x, w[u].y, w[u].z, w[u].w};
-      float x[8], top = 0.0f;
+      float x[kLane<F>], top = 0.0f;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        x[2 * i] = fd_lo(h[i]);
-        x[2 * i + 1] = fd_hi(h[i]);
+      for (int i = 0; i < kVecs; ++i) {
+        const uint32_t h[4] = {w[u][i].x, w[u][i].y, w[u][i].z, w[u][i].w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          x[8 * i + 2 * e] = fd_lo(h[e]);
+          x[8 * i + 2 * e + 1] = fd_hi(h[e]);
+        }
       }
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
+      for (int i = 0; i < kLane<F>; ++i) {
         const float m = fabsf(x[i]);
         top = fmaxf(top, m < __builtin_inff() ? m : 0.0f);  // finite values only
       }
       if constexpr (F == kE2m1) {
-        top = fd_xor_max<2>(fd_xor_max<1>(top));  // of the block's four lanes
+        top = fd_xor_max<1>(top);  // of the block's two lanes
         bool nan = false;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) nan |= x[i] != x[i];
+        for (int i = 0; i < 16; ++i) nan |= x[i] != x[i];
         const uint64_t nans = __builtin_amdgcn_ballot_w64(nan);
-        const bool any_nan = ((nans >> (threadIdx.x & 60)) & 15) != 0;
+        const bool any_nan = ((nans >> (threadIdx.x & 62)) & 3) != 0;
         const int byte = scale_byte_e2m1(top);
         const float inv = __uint_as_float(static_cast<uint32_t>(254 - byte) << 23);  // 2^-E
         const float most = byte == kTopByteE2m1 ? 3.0f : 6.0f;
-        uint32_t code = 0;
         auto y = [&](int i) { return fminf(fmaxf(x[i] * inv, -most), most); };  // (a NaN's block has no values)
-        code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, y(0), y(1), 1.0f, 0);
-        code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, y(2), y(3), 1.0f, 1);
-        code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, y(4), y(5), 1.0f, 2);
-        code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, y(6), y(7), 1.0f, 3);
+        auto eight = [&](int i) {
+          uint32_t code = 0;
+          code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, y(i), y(i + 1), 1.0f, 0);
+          code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, y(i + 2), y(i + 3), 1.0f, 1);
+          code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, y(i + 4), y(i + 5), 1.0f, 2);
+          return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, y(i + 6), y(i + 7), 1.0f, 3);
+        };
+        const uint2 code = {eight(0), eight(8)};
         if (live) {
-          *reinterpret_cast<uint32_t*>(dst + li * 4) = code;
-          if ((li & 3) == 0)
-            (side == 0 ? a.c.k_scale : a.c.v_scale)[page[u] * a.c.s_page + head[u] * a.c.s_head + at * kPer + li / 4] =
+          *reinterpret_cast<uint2*>(dst + li * 8) = code;
+          if ((li & 1) == 0)
+            (side == 0 ? a.c.k_scale : a.c.v_scale)[page[u] * a.c.s_page + head[u] * a.c.s_head + at * kPer + li / 2] =
                 static_cast<uint8_t>(any_nan ? 255 : byte);
         }
         continue;
@@ -217,7 +230,7 @@ struct ReadArgs {
 
 template <int D, Format F, int U>
 __global__ __launch_bounds__(kThreads) void paged_kv_read_kernel(ReadArgs a) {
-  constexpr int kLanes = D / 8, kSide = kThreads / kLanes;
+  constexpr int kLanes = D / kLane<F>, kVecs = kLane<F> / 8, kSide = kThreads / kLanes;
   const int side = blockIdx.y;
   const int li = threadIdx.x % kLanes;
   int head[U], t[U], r[U], key[U], page[U];
@@ -240,23 +253,25 @@ __global__ __launch_bounds__(kThreads) void paged_kv_read_kernel(ReadArgs a) {
     page[u] = r[u] >= 0 && slot < a.c.max_pages ? a.c.table[r[u] * a.c.table_stride + slot] : -1;
   }
   constexpr int kPer = D / kScaleBlock;  // E2M1 scales of a row
-  uint4 w[U];
+  uint4 w[U][kVecs];
   uint8_t byte[U];
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     const int at = key[u] & ((1 << a.c.shift) - 1);
-    w[u] = {0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < kVecs; ++i) w[u][i] = {0, 0, 0, 0};
     byte[u] = 0;
     if (static_cast<unsigned>(page[u]) < static_cast<unsigned>(a.c.n_pages)) {
       const unsigned char* src = (side == 0 ? a.c.k : a.c.v) + page[u] * a.c.page + head[u] * a.c.head + at * a.c.row;
       if constexpr (F == kBf16) {
-        w[u] = *reinterpret_cast<const uint4*>(src + li * 16);
+        w[u][0] = *reinterpret_cast<const uint4*>(src + li * 16);
       } else if constexpr (F == kE2m1) {
-        w[u].x = *reinterpret_cast<const uint32_t*>(src + li * 4);
-        byte[u] = (side == 0 ? a.c.k_scale : a.c.v_scale)[page[u] * a.c.s_page + head[u] * a.c.s_head + at * kPer + li / 4];
+        const uint2 code = *reinterpret_cast<const uint2*>(src + li * 8);
+        w[u][0].x = code.x, w[u][0].y = code.y;
+        byte[u] = (side == 0 ? a.c.k_scale : a.c.v_scale)[page[u] * a.c.s_page + head[u] * a.c.s_head + at * kPer + li / 2];
       } else {
         const uint2 code = *reinterpret_cast<const uint2*>(src + li * 8);
-        w[u].x = code.x, w[u].y = code.y;
+        w[u][0].x = code.x, w[u][0].y = code.y;
         byte[u] = (side == 0 ? a.c.k_scale : a.c.v_scale)[page[u] * a.c.s_page + head[u] * a.c.s_head + at];
       }
     }
@@ -265,26 +280,29 @@ __global__ __launch_bounds__(kThreads) void paged_kv_read_kernel(ReadArgs a) {
   for (int u = 0; u < U; ++u) {
     if (r[u] < 0) continue;
     if constexpr (F == kE2m1) {  // codes of no page are zeros, and their scale is finite
-      w[u] = __builtin_bit_cast(uint4, e2m1_to_bf16(w[u].x, scale_of(byte[u])));
+      const uint2 code = {w[u][0].x, w[u][0].y};
+      w[u][0] = __builtin_bit_cast(uint4, e2m1_to_bf16(code.x, scale_of(byte[u])));
+      w[u][kVecs - 1] = __builtin_bit_cast(uint4, e2m1_to_bf16(code.y, scale_of(byte[u])));
     } else if constexpr (F == kE4m3) {  // codes of no page are zeros, whatever their scale
       const float s = scale_of(byte[u]);
       typedef float f32x2_t __attribute__((ext_vector_type(2)));
-      f32x2_t f0 = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(w[u].x), false);
-      f32x2_t f1 = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(w[u].x), true);
-      f32x2_t f2 = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(w[u].y), false);
-      f32x2_t f3 = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(w[u].y), true);
+      f32x2_t f0 = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(w[u][0].x), false);
+      f32x2_t f1 = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(w[u][0].x), true);
+      f32x2_t f2 = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(w[u][0].y), false);
+      f32x2_t f3 = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(w[u][0].y), true);
       if (byte[u] == kTopByte) {
         for (f32x2_t* const f : {&f0, &f1, &f2, &f3})
 #pragma unroll
           for (int e = 0; e < 2; ++e) (*f)[e] = fabsf((*f)[e]) == 256.0f ? copysignf(255.0f, (*f)[e]) : (*f)[e];
       }
-      w[u].x = fd_pack2(f0[0] * s, f0[1] * s);
-      w[u].y = fd_pack2(f1[0] * s, f1[1] * s);
-      w[u].z = fd_pack2(f2[0] * s, f2[1] * s);
-      w[u].w = fd_pack2(f3[0] * s, f3[1] * s);
+      w[u][0].x = fd_pack2(f0[0] * s, f0[1] * s);
+      w[u][0].y = fd_pack2(f1[0] * s, f1[1] * s);
+      w[u][0].z = fd_pack2(f2[0] * s, f2[1] * s);
+      w[u][0].w = fd_pack2(f3[0] * s, f3[1] * s);
     }
     uint16_t* out = side == 0 ? a.out[0] + head[u] * a.os[0][0] + t[u] * a.os[0][1] : a.out[1] + head[u] * a.os[1][0] + t[u] * a.os[1][1];
-    *reinterpret_cast<uint4*>(out + li * 8) = w[u];
+#pragma unroll
+    for (int i = 0; i < kVecs; ++i) *reinterpret_cast<uint4*>(out + (li * kVecs + i) * 8) = w[u][i];
   }
 }
 
@@ -316,7 +334,7 @@ extern "C" int fd_paged_kv_write(const void* k, const void* v, const int64_t k_s
   a.seq_len = seq_len;
   a.kv_heads = cache->kv_heads;
   const int64_t rows = static_cast<int64_t>(batch) * seq_len * cache->kv_heads;
-  const int per = kThreads / (cache->head_dim / 8);
+  const int per = kThreads / (cache->head_dim / (cache->dtype == FD_DTYPE_E2M1 ? kLane<kE2m1> : kLane<kBf16>));
   const int64_t blocks = (rows + per - 1) / per;
   FD_REQUIRE(blocks < (1LL << 32) / kThreads, FD_ERR_UNSUPPORTED, "%s: too many rows", what);
   if (blocks == 0) return FD_OK;
@@ -356,7 +374,7 @@ extern "C" int fd_paged_kv_read(const fd_paged_cache* cache, void* k_out, void* 
   a.n_seqs = n_seqs;
   a.kv_heads = cache->kv_heads;
   a.total = static_cast<int>(total);
-  const int per = kThreads / (cache->head_dim / 8);
+  const int per = kThreads / (cache->head_dim / (cache->dtype == FD_DTYPE_E2M1 ? kLane<kE2m1> : kLane<kBf16>));
   const int64_t blocks = (total * cache->kv_heads + per - 1) / per;
   FD_REQUIRE(blocks < (1LL << 32) / kThreads, FD_ERR_UNSUPPORTED, "%s: too many rows", what);
   if (blocks == 0) return FD_OK;
