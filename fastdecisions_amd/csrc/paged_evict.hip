@@ -11,12 +11,15 @@
 
 #include "paged_common.h"
 #include "state_slot.h"
+#include "wave_tools.h"
 
 namespace {
 
 constexpr int kSelectThreads = 1024, kSelectWaves = kSelectThreads / 64;
 constexpr int kBins = 2048;
-constexpr int kPer = 4;  // consecutive keys of a thread in the last pass
+constexpr int kPer = 4;                            // consecutive keys of a thread and chunk
+constexpr int kChunk = kSelectThreads * kPer;
+constexpr int kHeld = 4;                           // chunks whose weights stay in registers: all of up to 16384 keys
 constexpr int kMoveThreads = 256;
 
 struct EvictArgs {
@@ -42,7 +45,7 @@ __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(EvictArgs 
   __shared__ int bins[kBins];
   __shared__ int wave_sums[2][kSelectWaves];
   __shared__ int found[2];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
   const int req = blockIdx.x / a.heads, head = blockIdx.x % a.heads;
   const int len = request_keys(a.c, req), left = min(len, a.keep), recent = min(a.recent, left);
   const int fixed = len - recent, need = left - recent;  // `need` of the keys [0, fixed) stay, and all behind them
@@ -52,6 +55,34 @@ __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(EvictArgs 
   int32_t* const kept = a.kept + static_cast<int64_t>(blockIdx.x) * a.keep;
   auto weight = [&](int j) { return w == nullptr ? 0.0f : w[j]; };  // a request without weights: the first keys stay
   if (tid == 0 && head == 0) a.new_lens[req] = left;
+
+  // The row's weights are loaded once where they fit, else in every pass.  (four keys of a thread lie in a row)
+  const bool held = len <= kHeld * kChunk;
+  float x[kHeld][kPer];
+  auto load = [&](int j0, float (&y)[kPer]) {
+#pragma unroll
+    for (int u = 0; u < kPer; ++u) {
+      const int j = j0 + tid * kPer + u;
+      y[u] = j < len ? weight(j) : 0.0f;
+    }
+  };
+  if (held) {
+#pragma unroll
+    for (int c = 0; c < kHeld; ++c) load(c * kChunk, x[c]);
+  }
+  auto each = [&](int end, auto use) {  // use(first key, weights) of the chunks of [0, end)
+    if (held) {
+#pragma unroll
+      for (int c = 0; c < kHeld; ++c)
+        if (c * kChunk < end) use(c * kChunk, x[c]);
+    } else {
+      for (int j0 = 0; j0 < end; j0 += kChunk) {
+        float y[kPer];
+        load(j0, y);
+        use(j0, y);
+      }
+    }
+  };
 
   // ---- the weight at the border: its leading bits, and how many keys of those bits stay
   uint32_t border = 0;
@@ -63,22 +94,23 @@ __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(EvictArgs 
       const int shift = shifts[pass], width = pass < 2 ? 11 : 10;
       for (int i = tid; i < kBins; i += kSelectThreads) bins[i] = 0;
       __syncthreads();
-      for (int j = tid; j < fixed; j += kSelectThreads) {
-        const uint32_t key = order_of(weight(j));
-        if (pass == 0 || key >> (shift + width) == border >> (shift + width)) atomicAdd(&bins[(key >> shift) & ((1 << width) - 1)], 1);
-      }
+      each(fixed, [&](int j0, const float (&y)[kPer]) {
+#pragma unroll
+        for (int u = 0; u < kPer; ++u) {
+          const uint32_t key = order_of(y[u]);
+          if (j0 + tid * kPer + u < fixed && (pass == 0 || key >> (shift + width) == border >> (shift + width)))
+            atomicAdd(&bins[(key >> shift) & ((1 << width) - 1)], 1);
+        }
+      });
       __syncthreads();
       // two bins per thread, largest first: the bin where the running count reaches `room`
       const int b0 = kBins - 1 - 2 * tid, c0 = bins[b0], c1 = bins[b0 - 1];
-      int incl = c0 + c1;
-#pragma unroll
-      for (int d = 1; d < 64; d <<= 1) {
-        const int up = __shfl_up(incl, d);
-        if (lane >= d) incl += up;
-      }
-      if (lane == 63) wave_sums[0][wave] = incl;
+      const int incl_wave = wave_scan(c0 + c1);
+      if (lane == 63) wave_sums[pass & 1][wave] = incl_wave;
       __syncthreads();
-      for (int v = 0; v < wave; ++v) incl += wave_sums[0][v];
+      // (16 wavefronts: lane v of each holds the sum of wavefront v)
+      const int sums = wave_scan(lane < kSelectWaves ? wave_sums[pass & 1][lane] : 0);
+      const int incl = incl_wave + (wave == 0 ? 0 : __builtin_amdgcn_readlane(sums, max(wave - 1, 0)));
       const int before = incl - c0 - c1;
       if (before < room && room <= incl) {
         const bool first = room <= before + c0;
@@ -88,55 +120,43 @@ __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(EvictArgs 
       __syncthreads();
       border |= static_cast<uint32_t>(found[0]) << shift;
       room = found[1];
-      __syncthreads();  // found and the bins are read
     }
   }
   const bool all = need >= fixed;
 
   // ---- the keys that stay, in their order
   int above = 0, equal = 0;  // of the keys before this chunk
-  for (int j0 = 0; j0 < len; j0 += kSelectThreads * kPer) {
-    float x[kPer];
+  __syncthreads();           // the sums are read
+  each(len, [&](int j0, const float (&y)[kPer]) {
     bool is_above[kPer], is_equal[kPer];
-    int sums = 0;  // keys above in the low half, at the border in the high one
+    int mine = 0;  // keys above in the low half, at the border in the high one
 #pragma unroll
     for (int u = 0; u < kPer; ++u) {
       const int j = j0 + tid * kPer + u;
-      x[u] = j < len ? weight(j) : 0.0f;
-      const uint32_t key = order_of(x[u]);
+      const uint32_t key = order_of(y[u]);
       is_above[u] = j < len && (j >= fixed || all || (need > 0 && key > border));
       is_equal[u] = !is_above[u] && j < fixed && need > 0 && key == border;
-      sums += (is_above[u] ? 1 : 0) + (is_equal[u] ? 1 << 16 : 0);
+      mine += (is_above[u] ? 1 : 0) + (is_equal[u] ? 1 << 16 : 0);
     }
-    int incl = sums;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int up = __shfl_up(incl, d);
-      if (lane >= d) incl += up;
-    }
-    if (lane == 63) wave_sums[(j0 / (kSelectThreads * kPer)) & 1][wave] = incl;
+    const int incl = wave_scan(mine), parity = (j0 / kChunk) & 1;
+    if (lane == 63) wave_sums[parity][wave] = incl;
     __syncthreads();  // every weight of the chunk is read, too
-    int total = 0, before = incl - sums;
-    for (int v = 0; v < kSelectWaves; ++v) {
-      const int s = wave_sums[(j0 / (kSelectThreads * kPer)) & 1][v];
-      if (v < wave) before += s;
-      total += s;
-    }
+    const int sums = wave_scan(lane < kSelectWaves ? wave_sums[parity][lane] : 0), total = __builtin_amdgcn_readlane(sums, 63);
+    const int before = incl - mine + (wave == 0 ? 0 : __builtin_amdgcn_readlane(sums, max(wave - 1, 0)));
     int n_above = above + (before & 0xffff), n_equal = equal + (before >> 16);
 #pragma unroll
     for (int u = 0; u < kPer; ++u) {
-      const int j = j0 + tid * kPer + u;
       if (is_above[u] || (is_equal[u] && n_equal < room)) {
         const int place = n_above + min(n_equal, room);
-        kept[place] = j;
-        if (w_out != nullptr) w_out[place] = x[u];
+        kept[place] = j0 + tid * kPer + u;
+        if (w_out != nullptr) w_out[place] = y[u];
       }
       n_above += is_above[u] ? 1 : 0;
       n_equal += is_equal[u] ? 1 : 0;
     }
     above += total & 0xffff;
     equal += total >> 16;
-  }
+  });
   __syncthreads();  // weights that move into [0, left) are read
   for (int i = left + tid; i < a.keep; i += kSelectThreads) kept[i] = -1;
   if (w_out != nullptr)
