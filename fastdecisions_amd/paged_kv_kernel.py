@@ -73,19 +73,22 @@ def check_cache(k_cache, v_cache, page_table, cache_lens, k_scale, v_scale, requ
         raise ValueError("Cache rows must be contiguous and 16-byte aligned")
     ks = vs = ssp = ssh = 0
     if codes:
-        blocks = (dim // SCALE_BLOCK,) if dtype == _E2M1 else ()
-        per = blocks[0] if blocks else 1  # scale bytes of a row
-        for t in (k_scale, v_scale):
-            if (t is None or t.shape != (*shape[:3], *blocks) or t.dtype != _UINT8 or t.get_device() != device
-                    or t.stride()[2:] != ((per, 1) if blocks else (1,)) or t.data_ptr() % per):
-                raise ValueError("An e4m3 cache needs k_scale and v_scale: uint8 [n_pages, Hkv, page_size] on its device; "
-                                 "a 4-bit one uint8 [n_pages, Hkv, page_size, D / 32], rows contiguous and aligned")
+        if dtype == _E2M1:
+            per = dim // SCALE_BLOCK  # scale bytes of a row
+            want = (n_pages, heads, page_size, per)
+        else:
+            per, want = 1, (n_pages, heads, page_size)
+        if (k_scale is None or v_scale is None or k_scale.shape != want or v_scale.shape != want or k_scale.dtype != _UINT8
+                or v_scale.dtype != _UINT8 or k_scale.get_device() != device or v_scale.get_device() != device):
+            raise ValueError("An e4m3 cache needs k_scale and v_scale: uint8 [n_pages, Hkv, page_size] on its device; a 4-bit "
+                             "one uint8 [n_pages, Hkv, page_size, D / 32]")
         ks, vs = k_scale.data_ptr(), v_scale.data_ptr()
-        if v_scale.stride() != k_scale.stride():
+        scale_strides = k_scale.stride()
+        if v_scale.stride() != scale_strides:
             raise ValueError("k_scale and v_scale must have the same strides")
-        ssp, ssh = k_scale.stride()[:2]
-        if (ssp | ssh) % per:
-            raise ValueError("The scales of a 4-bit cache must be aligned to a row's D / 32 bytes")
+        ssp, ssh, sst = scale_strides[:3]
+        if sst != per or scale_strides[-1] != 1 or (ssp | ssh | ks | vs) % per:
+            raise ValueError("Scale rows must be contiguous, and those of a 4-bit cache aligned to their D / 32 bytes")
     elif k_scale is not None or v_scale is not None:
         raise ValueError("A BF16 cache has no scales")
     max_pages = page_table.shape[-1]
