@@ -227,7 +227,7 @@ extern "C" int fd_paged_kv_evict(const fd_paged_cache* cache, const float* weigh
              "%s: the weights need a row for every request", what);
   FD_REQUIRE(weight_strides[0] >= 0 && weight_strides[1] >= 0, FD_ERR_INVALID_ARGUMENT, "%s: weight strides must be >= 0", what);
   const int64_t select = static_cast<int64_t>(requests) * cache->kv_heads, rows = select * keep;
-  FD_REQUIRE(select < (1LL << 32) / kSelectThreads && rows < (1LL << 31), FD_ERR_UNSUPPORTED, "%s: problem too large", what);
+  FD_REQUIRE(select < (1LL << 32) / kSelectThreads && rows < (1LL << 27), FD_ERR_UNSUPPORTED, "%s: problem too large", what);
   if (requests == 0) return FD_OK;
   a.w = weights;
   a.w_out = weights_out;

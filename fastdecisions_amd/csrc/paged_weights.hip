@@ -23,6 +23,7 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kWaves = 4;
 constexpr int kCus = 256;
+constexpr int kMostKeys = 1 << 27, kMostRows = 1 << 30;  // of a request
 constexpr int64_t kMostScores = 1LL << 28;  // bytes of kept scores: what the last-level cache may hold
 
 struct WeightArgs {
@@ -34,7 +35,6 @@ struct WeightArgs {
   float* w;
   int64_t w_row, w_head;
   int n_req, seq_len, group, kv_heads, last, w_rows;
-  uint32_t group_magic;         // ceil(2^24 / group)
   float scale_log2;
   int stats_items, sums_items;  // items that each kernel cuts its work into at most, but for one per tile that stays
   int slots;                    // workgroups that run at once
@@ -109,9 +109,10 @@ struct Size {
 };
 // Streamed tiles of an item.  Items that just fill m rounds of the workgroups that run at once take m (c + overhead) tiles of
 // time, and the best of a few m is taken; a few items more than workgroups would cost a whole round.  `items` bounds them
-// whatever the estimate: no more than that many places (and one per tile that stays) are needed.
+// whatever the estimate: no more than that many places (and one per tile that stays) are needed.  `most`: what holds any
+// request whole.
 template <typename SizeOf>
-__device__ __forceinline__ int tiles_of_item(const WeightArgs& a, const Requests& all_req, int lane, int items, int least, int overhead, SizeOf size_of) {
+__device__ __forceinline__ int tiles_of_item(const WeightArgs& a, const Requests& all_req, int lane, int items, int least, int most, int overhead, SizeOf size_of) {
   constexpr int kRounds = 4;
   Size all{0, 0.0f, 0.0f};
   for (int r0 = 0; r0 < a.n_req; r0 += 64) {
@@ -132,7 +133,7 @@ __device__ __forceinline__ int tiles_of_item(const WeightArgs& a, const Requests
     if (now < cost) best = c, cost = now;
   }
   const int64_t floor = max((pairs + items - 1) / items, static_cast<int64_t>(least));
-  return uniform(static_cast<int>(max(min(static_cast<int64_t>(best), static_cast<int64_t>(1 << 25)), min(floor, static_cast<int64_t>(1 << 25)))));
+  return uniform(static_cast<int>(max(min(static_cast<int64_t>(best), static_cast<int64_t>(most)), min(floor, static_cast<int64_t>(most)))));
 }
 
 // Request that holds item `at` when request r has count(r) items: false if none does; *base: items before it.
@@ -178,7 +179,7 @@ template <class S>
 struct Cut {
   int c;  // key tiles of a range
   __device__ __forceinline__ Cut(const WeightArgs& a, const Requests& all, int lane)
-      : c(tiles_of_item(a, all, lane, a.stats_items, 256 / S::kKeys, 5, [&](const Req& x) {
+      : c(tiles_of_item(a, all, lane, a.stats_items, 256 / S::kKeys, kMostKeys / S::kKeys, 5, [&](const Req& x) {
           const int rt = over(x.n_new * a.group, S::kRows), kt = over(x.len, S::kKeys);
           const float mean = 0.5f * static_cast<float>(min(x.len, x.len - x.n_new + S::kRows / a.group) + x.len);
           return Size{static_cast<int64_t>(rt) * kt, static_cast<float>(rt) * (mean / S::kKeys + 0.5f), static_cast<float>(rt)};
@@ -620,7 +621,7 @@ __global__ __launch_bounds__(S::kRows) void row_stats_join_kernel(WeightArgs a) 
 struct SumCut {
   int c;
   __device__ __forceinline__ SumCut(const WeightArgs& a, const Requests& all, int lane)
-      : c(tiles_of_item(a, all, lane, a.sums_items, 4, 10, [&](const Req& x) {
+      : c(tiles_of_item(a, all, lane, a.sums_items, 4, kMostRows / kSumRows, 10, [&](const Req& x) {
           const int rt = over(x.n_new * a.group, kSumRows), kt = over(x.len, kSumKeys);
           const float fresh = 0.5f * static_cast<float>(x.n_new) / kSumKeys;  // half of the new tokens' keys are seen
           return Size{static_cast<int64_t>(rt) * kt, static_cast<float>(rt) * (static_cast<float>(kt) - fresh), static_cast<float>(kt)};
@@ -786,11 +787,11 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void key_sums_kernel(We
       const int r4 = i / 8, e = (i / 2) % 4, n = i % 2;
       if (i % 8 == 0 && r4 < 3) values(masked_c, r4 + 1);
       float y = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][4 * r4 + e], a.scale_log2, -mv[r4 & 1][e]));
-      if constexpr (decltype(masked_c)::value) {
-        const int4 l = lv[r4 & 1];
-        y = key[n] <= (e == 0 ? l.x : e == 1 ? l.y : e == 2 ? l.z : l.w) ? y : 0.0f;
-      }
       y = __builtin_fmaf(y, iv[r4 & 1][e], tile_sum[n][e]);
+      if constexpr (decltype(masked_c)::value) {  // (a row of NaN is none of a key that it does not see)
+        const int4 l = lv[r4 & 1];
+        y = key[n] <= (e == 0 ? l.x : e == 1 ? l.y : e == 2 ? l.z : l.w) ? y : tile_sum[n][e];
+      }
       asm volatile("" : "+v"(y));  // computed here, not sunk towards the tile's end
       tile_sum[n][e] = y;
     };
@@ -893,7 +894,7 @@ constexpr int kScoreRows = 16, kScoreKeys = 64 * kWaves;
 struct ScoreCut {
   int c;
   __device__ __forceinline__ ScoreCut(const WeightArgs& a, const Requests& all, int lane)
-      : c(tiles_of_item(a, all, lane, a.stats_items, 1, 3, [&](const Req& x) {
+      : c(tiles_of_item(a, all, lane, a.stats_items, 1, kMostKeys / kScoreKeys, 3, [&](const Req& x) {
           const int rt = rtiles(a, x), kt = over(x.len, kScoreKeys);
           return Size{static_cast<int64_t>(rt) * kt, static_cast<float>(rt * kt), static_cast<float>(rt)};
         })) {
@@ -1091,7 +1092,9 @@ __global__ __launch_bounds__(kThreads) void key_scores_add_kernel(WeightArgs a) 
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
           const int key = min(key0 + u * kThreads, x.len - 1);
-          sum[u] = __builtin_fmaf(__builtin_amdgcn_exp2f(__builtin_fmaf(scores[(r0 + i) * a.score_stride + key], a.scale_log2, -y.x)), y.y, sum[u]);
+          const float s = scores[(r0 + i) * a.score_stride + key];  // -inf: not seen (also where the row is NaN)
+          const float p = __builtin_fmaf(__builtin_amdgcn_exp2f(__builtin_fmaf(s, a.scale_log2, -y.x)), y.y, sum[u]);
+          sum[u] = s == -__builtin_inff() ? sum[u] : p;
         }
       }
     }
@@ -1193,7 +1196,6 @@ extern "C" int fd_paged_key_weights(const void* q, const fd_paged_cache* cache, 
   a.kv_heads = cache->kv_heads;
   a.last = last > 0 ? last : seq_len;
   a.w_rows = weight_rows;
-  a.group_magic = ((1u << 24) + group - 1) / group;
   a.stats_items = p.stats_items;
   a.sums_items = p.sums_items;
   a.slots = p.slots;

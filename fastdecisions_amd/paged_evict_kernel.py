@@ -50,6 +50,9 @@ def check_weights(name, weights, heads, width, device) -> None:
     if (weights.ndim != 3 or weights.dtype != torch.float32 or weights.get_device() != device or weights.shape[1] != heads
             or weights.shape[2] < width or weights.stride(2) != 1):
         raise ValueError(f"{name} must be FP32 [rows, {heads}, at least {width}] on the cache's device, its keys contiguous")
+    (row, head, _), (rows, _, keys) = weights.stride(), weights.shape
+    if (rows > 1 and row < keys) or (heads > 1 and head < keys) or (rows > 1 and heads > 1 and row < heads * head and head < rows * row):
+        raise ValueError(f"{name} must not hold two of its elements in the same memory")
 
 
 def check_row_indices(row_indices, requests, rows, device) -> int | None:
@@ -165,8 +168,8 @@ def paged_kv_evict(
     if (new_table.ndim != 2 or new_table.shape[0] != requests or new_table.dtype != torch.int32
             or new_table.get_device() != device or new_table.stride(1) != 1 or new_table.shape[1] * page_size < keep):
         raise ValueError(f"new_table must be int32 [{requests}, n] on the cache's device, its rows contiguous, and hold {keep} keys")
-    if requests * heads * keep >= 1 << 31:
-        raise ValueError("requests * Hkv * keep must be below 2^31")
+    if requests * heads * keep >= 1 << 27:
+        raise ValueError("requests * Hkv * keep must be below 2^27")
     index = check_row_indices(row_indices, requests, weights.shape[0], device)
     if _cache_lib.current_device() != device:
         with torch.cuda.device(device):

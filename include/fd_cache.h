@@ -152,7 +152,8 @@ FD_API int64_t fd_paged_gqa_workspace_bytes(int batch, int q_heads, int kv_heads
  * and may be k).  fp32 throughout, in an order that the sizes fix.
  *
  *   q       as in fd_paged_gqa_fwd
- *   weights [weight_rows, kv_heads, >= max_pages * page_size] fp32, strides {row, head} in elements, keys contiguous
+ *   weights [weight_rows, kv_heads, >= max_pages * page_size] fp32, strides {row, head} in elements, keys contiguous;
+ *           no two of its elements the same memory
  *   row_indices  device int32[requests]: request r's row of weights; NULL: row r.  An index outside [0, weight_rows), or
  *           one that an earlier request of the call names already, is no row: nothing is added for that request
  *   last    the last `last` new tokens of each request count; 0: all of them
@@ -183,7 +184,7 @@ FD_API int64_t fd_paged_key_weights_workspace_bytes(int batch, int q_heads, int 
  *           [0, n_pages) are no pages: their keys are not written.  Kept keys on no page become zeros
  *   kept    [requests, kv_heads, keep] int32, contiguous: the old place of every kept key, -1 behind the last one
  *   new_lens  [requests] int32: min(cache_lens, keep)
- * The old pages are left as they were.
+ * The old pages are left as they were.  Limit: requests * kv_heads * keep below 2^27.
  */
 FD_API int fd_paged_kv_evict(const fd_paged_cache* cache, const float* weights, float* weights_out,
                              const int64_t weight_strides[2], int weight_rows, const int32_t* row_indices,

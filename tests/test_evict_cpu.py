@@ -87,6 +87,11 @@ def test_tensors_that_do_not_fit_are_refused():
     for bad in (w[:, :1], w.double(), w[:, :, :31], w[0], w.transpose(1, 2).contiguous().transpose(1, 2)):
         with pytest.raises(ValueError, match="at least 32"):
             check_weights("w", bad, 2, 32, -1)
+    for same in (torch.zeros((1, 2, 32)).expand(3, -1, -1), torch.zeros((1, 1, 32)).expand(-1, 2, -1),
+                 torch.zeros(200).as_strided((2, 2, 32), (40, 32, 1))):
+        with pytest.raises(ValueError, match="same memory"):
+            check_weights("w", same, 2, 32, -1)
+    check_weights("w", torch.zeros((2, 3, 32)).transpose(0, 1), 2, 32, -1)
     assert check_row_indices(None, 2, 2, -1) is None
     for idx, n in ((None, 3), (torch.zeros(2, dtype=torch.int32), 3), (torch.zeros(3, dtype=torch.int64), 3),
                    (torch.zeros(6, dtype=torch.int32)[::2], 3)):

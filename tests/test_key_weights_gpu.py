@@ -138,3 +138,82 @@ def test_far_scores():
     # scores up to about 400: the exponent is off by up to 2^-24 * 400 * (sqrt(64) + 2)
     assert ((w.double() - want).abs() <= 2.0 ** -24 * 4000 * want + 1e-30).all()
     assert torch.isfinite(w).all() and abs(w.sum().item() - 20 * 8) < 0.01
+
+
+@pytest.mark.parametrize("n", [1, 6, 40])
+def test_fewer_keys_than_tokens(n):
+    """Requests whose lengths say that some of their tokens see nothing, or that they hold nothing."""
+    announce(f"key weights, fewer keys than tokens, {n} new")
+    check("bf16", [n] * 5, [-n, -n + 1, -(n // 2), 3, 700], 8, 2, 64, 16, 11, packed=False)
+
+
+def test_thousands_of_requests():
+    """More row tiles than any number of rounds: no request is cut, and all are whole."""
+    announce("key weights, 2300 requests")
+    check("e2m1", [1] * 2300, [(i * 37) % 90 for i in range(2300)], 4, 4, 64, 16, 12, packed=False)
+    check("bf16", [20] * 700, [(i * 37) % 90 for i in range(700)], 4, 4, 64, 16, 13, packed=False)
+
+
+@pytest.mark.parametrize("n", [1, 4, 90])
+def test_a_key_that_is_nan(n):
+    """The rows that see it are NaN and with them the weights of every key that they see; no other key's."""
+    from fastdecisions_amd.paged_evict_kernel import paged_key_weights
+    announce(f"key weights, a key that is NaN, {n} new")
+    length = 300 + n
+    c, get = make("bf16", [length], 16, 2, 64, 14)
+    q = make_q([n], 4, 64, 15)
+    w = torch.zeros((1, 2, c["table"].shape[1] * 16), device="cuda")
+    for key, first in ((100, 0), (300 + n // 2, n // 2)):  # seen by all tokens, by the later half
+        k, got = c["k"].clone(), w.clone()
+        k[c["table"][0, key // 16].long(), 1, key % 16, 5] = float("nan")
+        paged_key_weights(q, k, c["table"], ints([length]), got, cu_seqlens=ints([0, n]))
+        assert torch.isfinite(got[0, 0]).all()
+        assert torch.isnan(got[0, 1, :length]).all()      # the last token sees them all
+        last = torch.full((1, 2, w.shape[2]), 0.0, device="cuda")
+        before = n // 2
+        if first and before:
+            paged_key_weights(q[:, :, :before], k, c["table"], ints([300 + before]), last, cu_seqlens=ints([0, before]))
+            assert torch.isfinite(last).all()
+    # a token that is NaN itself weighs the keys up to its own, and none behind it
+    if n > 1:
+        odd, got = q.clone(), w.clone()
+        odd[0, 1, n // 2, 3] = float("nan")               # a query head of key head 0
+        paged_key_weights(odd, c["k"], c["table"], ints([length]), got, cu_seqlens=ints([0, n]))
+        assert torch.isfinite(got[0, 1]).all()
+        assert torch.isnan(got[0, 0, :300 + n // 2 + 1]).all() and torch.isfinite(got[0, 0, 300 + n // 2 + 1:]).all()
+
+
+def test_in_a_graph_as_requests_grow():
+    """Weights and eviction captured once and replayed with other lengths, weights and tables: the eager results."""
+    from fastdecisions_amd.paged_evict_kernel import paged_key_weights, paged_kv_evict
+    announce("key weights and eviction in a graph")
+    for n, held in ((1, "e2m1"), (60, "bf16")):
+        c, _ = make(held, [900, 700, 160], 16, 2, 64, 16)  # the last one's pages become the new ones
+        table, new_table = c["table"][:2].contiguous(), c["table"][2, :10].reshape(2, 5).contiguous()
+        q = make_q([n] * 2, 8, 64, 17, packed=False)
+        lens = ints([500, 300])
+        w, out = (torch.zeros((2, 2, table.shape[1] * 16), device="cuda") for _ in range(2))
+
+        def step(lens, w, out):
+            paged_key_weights(q, c["k"], table, lens, w, k_scale=c["ks"])
+            return paged_kv_evict(c["k"], c["v"], table, lens, w, new_table, 70, recent=9, k_scale=c["ks"], v_scale=c["vs"],
+                                  weights_out=out)
+
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step(lens, w, out)
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            kept, left = step(lens, w, out)
+        for i in range(4):
+            lens.copy_(ints([500 + 100 * i, 60 + 200 * i]))
+            w.zero_()
+            out.zero_()
+            graph.replay()
+            got = [t.clone() for t in (kept, left, w, out)] + [c[x].view(torch.uint8).clone() for x in "kv"]
+            w2, out2 = torch.zeros_like(w), torch.zeros_like(out)
+            want = [*step(lens, w2, out2), w2, out2] + [c[x].view(torch.uint8) for x in "kv"]
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(got, want)), (n, i)
