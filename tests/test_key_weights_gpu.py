@@ -217,3 +217,42 @@ def test_in_a_graph_as_requests_grow():
             want = [*step(lens, w2, out2), w2, out2] + [c[x].view(torch.uint8) for x in "kv"]
             torch.cuda.synchronize()
             assert all(torch.equal(a, b) for a, b in zip(got, want)), (n, i)
+
+
+@pytest.mark.parametrize("n", [1, 2, 77])
+@pytest.mark.parametrize("hq,hkv", [(14, 2), (10, 2), (129, 1), (2048, 1)])
+def test_groups_that_divide_no_tile(hq, hkv, n):
+    announce(f"key weights, {hq}/{hkv} heads, {n} new")
+    check("bf16", [n] * 2, [300, 1000 - n], hq, hkv, 64, 16, 18, packed=False, last=40)
+
+
+def test_two_streams_at_once():
+    """Calls side by side on streams of their own, weights of other strides: each as it is alone."""
+    from fastdecisions_amd.paged_evict_kernel import paged_key_weights, paged_kv_evict
+    announce("key weights and eviction on two streams")
+    jobs = []
+    for i, (held, n) in enumerate((("e2m1", 1), ("bf16", 130))):
+        c, _ = make(held, [2100, 1800, 160], 16, 2, 64, 20 + i)
+        table, new_table = c["table"][:2].contiguous(), c["table"][2, :10].reshape(2, 5).contiguous()
+        q, lens = make_q([n] * 2, 8, 64, 30 + i, packed=False), ints([2100, 1800])
+        store = lambda: torch.zeros((2, 2, 2200), device="cuda").transpose(0, 1)  # heads in front
+
+        def run(w, out, c=c, table=table, new_table=new_table, q=q, lens=lens):
+            paged_key_weights(q, c["k"], table, lens, w, k_scale=c["ks"])
+            return *paged_kv_evict(c["k"], c["v"], table, lens, w, new_table, 80, recent=9, k_scale=c["ks"], v_scale=c["vs"],
+                                   weights_out=out), w, out, c["k"].view(torch.uint8), c["v"].view(torch.uint8)
+        jobs.append((run, store))
+    want = [[t.clone() for t in run(store(), store())] for run, store in jobs]
+    streams = [torch.cuda.Stream() for _ in jobs]
+    made = [(store(), store()) for _, store in jobs]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(3):
+        got.clear()
+        for (run, _), stream, (w, out) in zip(jobs, streams, made):
+            with torch.cuda.stream(stream):
+                w.zero_(), out.zero_()
+                got.append(run(w, out))
+    torch.cuda.synchronize()
+    for a, b in zip(got, want):
+        assert all(torch.equal(x, y) for x, y in zip(a, b))
