@@ -911,7 +911,9 @@ struct ScoreCut {
 // takes blocks of 64 keys of its own, loaded straight into the operands' registers a block ahead: a lane's share of a
 // key is D / 4 features in a row (the steps of the product take any 32 features, the same ones of Q).
 template <int D, Format F>
-__global__ __launch_bounds__(kThreads, D == 256 && F == kBf16 ? 1 : 2) void key_scores_kernel(WeightArgs a) {
+constexpr int kScoreGroups = D == 256 && F == kBf16 ? 1 : D == 256 || (D == 128 && F == kBf16) ? 2 : 4;  // of a CU
+template <int D, Format F>
+__global__ __launch_bounds__(kThreads, (kScoreGroups<D, F>)) void key_scores_kernel(WeightArgs a) {
   constexpr int kSteps = D / 32, kRowBytes = F == kBf16 ? 2 * D : F == kE4m3 ? D : D / 2;
   constexpr int kBytes = kRowBytes / 4, kWords = kBytes < 16 ? 1 : kBytes / 16;  // of a lane and key
   constexpr int kChunks = kBytes < 16 ? 2 : kWordChunks<F>;                      // eights of features in a word
@@ -1048,6 +1050,7 @@ __global__ __launch_bounds__(kThreads, D == 256 && F == kBf16 ? 1 : 2) void key_
 constexpr int kAddKeys = 4 * kThreads;
 __global__ __launch_bounds__(kThreads) void key_scores_add_kernel(WeightArgs a) {
   constexpr int kHold = 256;  // rows whose (m, 1 / l) are in LDS at a time
+  constexpr int kAhead = 4;   // rows whose scores are asked for before those are joined
   __shared__ float2 stats[kHold];
   const int lane = threadIdx.x & 63;
   const Requests all(a, lane);
@@ -1063,45 +1066,61 @@ __global__ __launch_bounds__(kThreads) void key_scores_add_kernel(WeightArgs a) 
     const int n_rt = uniform(cut.rtiles(a, x)), n_ranges = uniform(cut.ranges(x)), rows = x.n_new * a.group;
     const int key0 = kt * kAddKeys + static_cast<int>(threadIdx.x);
     const float* const scores = a.scores + stat_row(a, x, req, head) * a.score_stride;
-    float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    float* const w = a.w + slot * a.w_row + head * a.w_head;
+    float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f}, ahead[kAhead][4], old[4];
+    int keys[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      keys[u] = min(key0 + u * kThreads, x.len - 1);
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) ahead[i][u] = scores[min(i, rows - 1) * a.score_stride + keys[u]];
+      old[u] = w[keys[u]];
+    }
+    auto add = [&](const float2& y, const float (&s)[4]) __attribute__((always_inline)) {
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {  // -inf: not seen (also where the row is NaN)
+        const float p = __builtin_fmaf(__builtin_amdgcn_exp2f(__builtin_fmaf(s[u], a.scale_log2, -y.x)), y.y, sum[u]);
+        sum[u] = s[u] == -__builtin_inff() ? sum[u] : p;
+      }
+    };
     for (int r0 = 0; r0 < rows; r0 += kHold) {
       __syncthreads();  // the rows before are done with theirs
-      for (int i = threadIdx.x; i < min(kHold, rows - r0); i += kThreads) {
-        const int row = r0 + i, at = first + head * n_ranges * n_rt + row / kScoreRows;
+      // 16 lanes share a row's ranges
+      for (int i = static_cast<int>(threadIdx.x) / 16; i < min(kHold, rows - r0); i += kThreads / 16) {
+        const int row = r0 + i, at = first + head * n_ranges * n_rt + row / kScoreRows, mine = threadIdx.x % 16;
         const float2* const p = reinterpret_cast<const float2*>(a.part) + static_cast<int64_t>(at) * kScoreRows + row % kScoreRows;
         // (every part has its place but those of an offset table that is not ascending)
         const int n = at >= 0 && at + static_cast<int64_t>(n_ranges - 1) * n_rt < a.part_items ? n_ranges : 0;
         float m = -__builtin_inff(), l = 0.0f;
-        for (int v0 = 0; v0 < n; v0 += 4) {
-          float2 y[4];
-#pragma unroll
-          for (int u = 0; u < 4; ++u) y[u] = p[static_cast<int64_t>(min(v0 + u, n - 1)) * n_rt * kScoreRows];
-#pragma unroll
-          for (int u = 0; u < 4; ++u) {
-            if (v0 + u >= n) continue;
-            const float top = fmaxf(m, y[u].x), sub = top == -__builtin_inff() ? 0.0f : top;
-            l = l * __builtin_amdgcn_exp2f(m - sub) + y[u].y * __builtin_amdgcn_exp2f(y[u].x - sub);
-            m = top;
-          }
+        auto join = [&](float m2, float l2) __attribute__((always_inline)) {
+          const float top = fmaxf(m, m2), sub = top == -__builtin_inff() ? 0.0f : top;
+          l = l * __builtin_amdgcn_exp2f(m - sub) + l2 * __builtin_amdgcn_exp2f(m2 - sub);
+          m = top;
+        };
+        for (int v = mine; v < n; v += 16) {
+          const float2 y = p[static_cast<int64_t>(v) * n_rt * kScoreRows];
+          join(y.x, y.y);
         }
-        stats[i] = stat_of(m, l);
+#pragma unroll
+        for (int d = 1; d < 16; d *= 2) join(__shfl_xor(m, d), __shfl_xor(l, d));
+        if (mine == 0) stats[i] = stat_of(m, l);
       }
       __syncthreads();
-      for (int i = 0; i < min(kHold, rows - r0); ++i) {
-        const float2 y = stats[i];
+      if (r0 == 0) {
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const int key = min(key0 + u * kThreads, x.len - 1);
-          const float s = scores[(r0 + i) * a.score_stride + key];  // -inf: not seen (also where the row is NaN)
-          const float p = __builtin_fmaf(__builtin_amdgcn_exp2f(__builtin_fmaf(s, a.scale_log2, -y.x)), y.y, sum[u]);
-          sum[u] = s == -__builtin_inff() ? sum[u] : p;
-        }
+        for (int i = 0; i < kAhead; ++i)
+          if (i < rows) add(stats[i], ahead[i]);
+      }
+      for (int i = r0 == 0 ? kAhead : 0; i < min(kHold, rows - r0); ++i) {
+        float s[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) s[u] = scores[(r0 + i) * a.score_stride + keys[u]];
+        add(stats[i], s);
       }
     }
-    float* const w = a.w + slot * a.w_row + head * a.w_head;
 #pragma unroll
     for (int u = 0; u < 4; ++u)
-      if (key0 + u * kThreads < x.len && sum[u] != 0.0f) w[key0 + u * kThreads] += sum[u];
+      if (key0 + u * kThreads < x.len && sum[u] != 0.0f) w[keys[u]] = old[u] + sum[u];
   }
 }
 
@@ -1218,7 +1237,8 @@ extern "C" int fd_paged_key_weights(const void* q, const fd_paged_cache* cache, 
     constexpr int D = decltype(d)::value;
     constexpr Format F = decltype(f)::value;
     if (p.few) {
-      hipLaunchKernelGGL((key_scores_kernel<D, F>), dim3(stats_grid), dim3(kThreads), 0, s, a);
+      a.slots = kCus * kScoreGroups<D, F>;
+      hipLaunchKernelGGL((key_scores_kernel<D, F>), dim3(static_cast<unsigned>(std::min<int64_t>(p.part_items, 2 * a.slots))), dim3(kThreads), 0, s, a);
       return;
     }
     hipLaunchKernelGGL((row_stats_kernel<D, F>), dim3(stats_grid), dim3(kThreads), 0, s, a);
