@@ -909,7 +909,8 @@ struct ScoreCut {
 
 // Scores of up to 16 rows, kept in the workspace in fp32, and their rows' (m, l) over the item's keys.  Every wavefront
 // takes blocks of 64 keys of its own, loaded straight into the operands' registers a block ahead: a lane's share of a
-// key is D / 4 features in a row (the steps of the product take any 32 features, the same ones of Q).
+// key is every fourth word of 16 bytes (the steps of the product take any 32 features, the same ones of Q), so that
+// four lanes read 64 bytes in a row.
 template <int D, Format F>
 constexpr int kScoreGroups = D == 256 && F == kBf16 ? 1 : D == 256 || (D == 128 && F == kBf16) ? 2 : 4;  // of a CU
 template <int D, Format F>
@@ -935,7 +936,7 @@ __global__ __launch_bounds__(kThreads, (kScoreGroups<D, F>)) void key_scores_ker
     const int32_t* const table = a.c.table + req * a.c.table_stride;
     const int first = range * cut.c * kScoreKeys + wave * 64, end = min(x.len, (range + 1) * cut.c * kScoreKeys);
     const int mask = (1 << a.c.shift) - 1;
-    const unsigned char* const base_k = a.c.k + head * a.c.head + grp * kBytes;
+    const unsigned char* const base_k = a.c.k + head * a.c.head + grp * sizeof(Word);
 
     struct Block {
       Word w[4][kWords];
@@ -948,20 +949,20 @@ __global__ __launch_bounds__(kThreads, (kScoreGroups<D, F>)) void key_scores_ker
         const int page = valid_page(a, page_at(kb0 + 16 * u)), at = max(min(kb0 + 16 * u + li, x.len - 1), 0) & mask;
         const Word* const p = reinterpret_cast<const Word*>(base_k + page * a.c.page + at * a.c.row);
 #pragma unroll
-        for (int i = 0; i < kWords; ++i) b.w[u][i] = p[i];
+        for (int i = 0; i < kWords; ++i) b.w[u][i] = p[4 * i];
         if constexpr (F == kE4m3) b.s[u] = *scales_of<F, D>(a, page, head, at);
         if constexpr (F == kE2m1) {
-          const uint8_t* const sp = scales_of<F, D>(a, page, head, at) + grp * D / 4 / kScaleBlock;
-          b.s[u] = kScales == 2 ? *reinterpret_cast<const uint16_t*>(sp) : *sp;
+          const uint8_t* const sp = scales_of<F, D>(a, page, head, at);
+          b.s[u] = kScales == 2 ? sp[grp] | sp[4 + grp] << 8 : sp[kBytes < 16 ? grp / 2 : grp];
         }
       }
     };
     Block cur, next;
     if (first < end) load(first, cur);
     bf16x8_t qf[kSteps];
-    const uint16_t* const q = q_row(a, x, req, head, token, row - token * a.group) + grp * (D / 4);
+    const uint16_t* const q = q_row(a, x, req, head, token, row - token * a.group) + grp * (8 * kChunks);
 #pragma unroll
-    for (int kk = 0; kk < kSteps; ++kk) qf[kk] = *reinterpret_cast<const bf16x8_t*>(q + kk * 8);
+    for (int kk = 0; kk < kSteps; ++kk) qf[kk] = *reinterpret_cast<const bf16x8_t*>(q + (kk / kChunks * 4 * kChunks + kk % kChunks) * 8);
     float* const out = a.scores + (stat_row(a, x, req, head) + row) * a.score_stride + 4 * grp;
     float m = -__builtin_inff(), l = 0.0f;  // of this lane's keys
     for (int kb0 = first; kb0 < end; kb0 += kScoreKeys) {
