@@ -5,7 +5,12 @@
 //           11, 11 and 10 bits of the weights in an order-preserving integer form, then one pass that numbers the keys
 //           that stay in their order (a key above the weight, and as many at it as there is room for, lowest first) and
 //           moves their weights
-//   move    rows and scales of the kept keys, a lane per 16 bytes; streaming
+//   move    rows and scales of the kept keys, a lane per 16 bytes, two rows each; streaming
+//
+// Select is bound by the latency of one workgroup (12 requests x 4 heads: 48 of 256 CUs): weights of up to 16384 keys are
+// loaded once and stay in registers (from memory in every pass: 21 us for 1500 to 16384 keys, now 15; 700 keys 7.8), 3
+// passes of LDS atomics over 2048 bins, and a barrier per 4096 keys when they are numbered.  A cut of a head over several
+// workgroups would need a launch per pass, 3 to 4 us each.  Move: 50 MB in 10.4 us, 4.8 TB/s.
 #include <algorithm>
 #include <type_traits>
 

@@ -32,7 +32,9 @@ constexpr int kTopByteE2m1 = 253;
 // A thread takes several rows, their chains of loads side by side, once there is more than a round (write) or a few
 // rounds (read) of workgroups: 1024 of a side (K, V) run at once.  Measured with 1, 2, 4 rows (us, 4 heads x 128 bf16):
 // write 1.2, 5 and 48 thousand tokens 4.0, 4.1, 4.1; 9.6, 9.3, 10.0; 39, 40, 41, E4M3 40, 38, 41; read 12 and 96
-// thousand 9.3, 9.4, 9.7; 120, 105, 81 (4.8 TB/s), E4M3 121, 108, 83.
+// thousand 9.3, 9.4, 9.7; 120, 105, 81 (4.8 TB/s), E4M3 121, 108, 83.  E2M1, prompts of 10.5 thousand tokens: written
+// in 11.4 us (27 MB, 2.4 TB/s), read in 9.7 (2.8 TB/s); with 8 features a lane as in the other formats 13.5 and 12.0,
+// since a lane's codes are 4 bytes then.
 constexpr int kAtOnce = 1024;
 constexpr int kRows = 2, kManyRows = 4;  // beyond kAtOnce workgroups; of a read beyond four times as many
 

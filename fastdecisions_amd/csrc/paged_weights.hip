@@ -3,13 +3,38 @@
 //   w[r, h, j] += sum over rows p of head h of exp(s_pj - m_p) / l_p,   s = scale q_p . k_j
 //
 // with m_p, l_p a row's maximum and denominator over the keys that it sees.  A sum over rows needs every row's
-// denominator first, so there are two kernels, each one product Q K^T with one exponential per score:
+// denominator first.
 //
-//   row stats   m and l of every row over ranges of keys (S^T = K Q^T: a lane's scores are of one row)
-//   key sums    the rows' probabilities summed key by key (S = Q K^T: a lane's scores are of one key)
+// Many rows: two kernels, each one product Q K^T with one exponential per score, the operand that stays in registers and
+// the other one through a ring of tiles in LDS:
 //
-// In both the operand that stays is in registers and the other one streams through LDS.  Everything is added in an
-// order that the sizes fix: no atomics.
+//   row stats   m and l of every row over ranges of keys (S^T = K Q^T: a lane's scores are of one row); 256 rows of a
+//               workgroup, ranges joined by a launch of their own
+//   key sums    the rows' probabilities summed key by key (S = Q K^T: a lane's scores are of one key); 256 keys of a
+//               workgroup, cut into ranges of rows, joined likewise
+//
+// The wavefronts of a SIMD fall into step, so a loop of products and then exponentials leaves one unit idle at a time:
+// the products of a block are written between the exponentials of the one before, slot by slot, held there by
+// scheduling barriers.  A slot (one 32x32x16 product, 2 scores of exponential and sums) takes about 41 cycles of a SIMD,
+// the product alone 32; a row's maximum is looked for only where a block's sum shows that it is needed.  2900 tokens on
+// 2048 keys, 16/4 heads x 128 (41.6 GFLOP a product): 67.5 + 4.7 + 74.5 + 6.4 us of kernels, 135 a call; without the ring
+// and the ranges of rows 870, with maxima of every block 195, with products first and exponentials after them 177.  Beyond
+// the loops: 7 to 9 us until the first product (finding the item, Q or K into registers, three tiles), and ranges that
+// end before the longest one.
+//
+// Few rows (up to 16 of a key head in a request, kMostScores): K is read once.
+//
+//   scores      S^T in fp32 into the workspace and the rows' (m, l) over the item's keys; streaming, no LDS
+//   scores add  the ranges joined, exp(s - m) / l summed over the rows; w read and written
+//
+// bound by K's bytes and, for short calls, by the chain from lengths to items to pages (3.5 us).  A token each of 64
+// requests of 256 to 8192 keys (4 bits, 16/4 x 128, 37 MB): 15.7 + 6.4 us; by the two kernels above 94.  64 x 8192 keys:
+// bf16 144 us (3.7 TB/s of K alone, the scores are 67 MB more), 4 bits 48.
+//
+// Items: workgroups do not start alike when their times differ, and a few more than the card holds at once cost a whole
+// round, so every workgroup sums up the requests (a lane each), picks the range that makes the items fill whole rounds
+// (tiles_of_item, fit) and finds its own; only items that exist are counted.  Everything is added in an order that the
+// sizes fix: no atomics.
 #include <algorithm>
 #include <type_traits>
 

@@ -14,8 +14,8 @@ fp32.  It takes what ``paged_gqa_attention`` takes, after ``paged_kv_write`` of 
 ``paged_kv_evict`` cuts every request to at most ``keep`` keys: its ``recent`` last ones and, per key
 head, those of largest weight among the others (of equal weights the lowest; NaN below everything).
 Their rows and scales move, in their order, to the pages of ``new_table`` (int32 ``[requests, n]``,
-``n * page_size >= keep``), which must be none of those that hold the call's requests; the old pages are
-left as they were.  A request of no more than ``keep`` keys moves whole.  Keys are rotated by their
+``n * page_size >= keep``), which must be distinct and none of those that hold the call's requests; the old
+pages are left as they were.  A request without a row of weights counts as one of equal weights.  A request of no more than ``keep`` keys moves whole.  Keys are rotated by their
 positions before they are cached, so a request goes on where it stood: its next tokens' positions count
 all the tokens that it has seen, ``cache_lens`` those that it holds.
 

@@ -180,7 +180,7 @@ FD_API int64_t fd_paged_key_weights_workspace_bytes(int batch, int q_heads, int 
  *           n = min(cache_lens, keep), and [n, cache_lens) are 0
  *   row_indices  as in fd_paged_key_weights; a request without a row counts as one of equal weights
  *   new_table  [requests, new_max_pages] int32, rows new_table_stride apart, new_max_pages * page_size >= keep.  Its
- *           pages must not be among those that the call's page table names for keys of any request.  Entries outside
+ *           pages must be distinct and not among those that the call's page table names for keys of any request.  Entries outside
  *           [0, n_pages) are no pages: their keys are not written.  Kept keys on no page become zeros
  *   kept    [requests, kv_heads, keep] int32, contiguous: the old place of every kept key, -1 behind the last one
  *   new_lens  [requests] int32: min(cache_lens, keep)
