@@ -84,7 +84,7 @@ def paged_key_weights(
     if len(shape) != 4:
         raise ValueError("Q must be four-dimensional")
     batch, q_heads, seq_len, dim = shape
-    if min(batch, q_heads, seq_len) < 1:
+    if batch < 1 or q_heads < 1 or seq_len < 1:
         raise ValueError("Batch, head counts and sequence length must be positive")
     if k_cache.ndim != 4:
         raise ValueError("k_cache must be [n_pages, Hkv, page_size, D]")

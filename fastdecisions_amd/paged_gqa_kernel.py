@@ -25,7 +25,7 @@ from functools import lru_cache
 import torch
 
 from . import _cache_lib
-from .paged_kv_kernel import cache_dim, check_cache, check_cu_seqlens, check_rows
+from .paged_kv_kernel import E2M1, check_cache, check_cu_seqlens, check_rows
 
 
 @lru_cache(maxsize=4096)
@@ -56,12 +56,13 @@ def paged_gqa_attention(
     if len(shape) != 4:
         raise ValueError("Q must be four-dimensional")
     batch, q_heads, seq_len, dim = shape
-    if min(batch, q_heads, seq_len) < 1:
+    if batch < 1 or q_heads < 1 or seq_len < 1:
         raise ValueError("Batch, head counts and sequence length must be positive")
-    if k_cache.ndim != 4:
+    cache_shape = k_cache.shape
+    if len(cache_shape) != 4:
         raise ValueError("k_cache and v_cache must be [n_pages, Hkv, page_size, D] of one shape")
-    _, kv_heads, page_size, _ = k_cache.shape
-    if kv_heads < 1 or q_heads % kv_heads or dim != cache_dim(k_cache):
+    _, kv_heads, page_size, held = cache_shape
+    if kv_heads < 1 or q_heads % kv_heads or dim != (2 * held if k_cache.dtype is E2M1 else held):
         raise ValueError("Q must have the cache's head dimension and a multiple of its heads")
     if q_heads // kv_heads > 2048:
         raise ValueError("at most 2048 query heads per key head")

@@ -34,14 +34,13 @@ from . import _cache_lib, _lib
 HEAD_DIMS = (64, 128, 256)
 PAGE_SIZES = (16, 32, 64, 128, 256)
 SCALE_BLOCK = 32  # features of a 4-bit row that share a scale
-_BF16, _E4M3, _E2M1 = torch.bfloat16, torch.float8_e4m3fn, torch.float4_e2m1fn_x2
+_BF16, _E4M3, E2M1 = torch.bfloat16, torch.float8_e4m3fn, torch.float4_e2m1fn_x2
 _INT32, _UINT8 = torch.int32, torch.uint8
-_DTYPES = {_BF16: _lib.FD_DTYPE_BF16, _E4M3: _cache_lib.FD_DTYPE_E4M3, _E2M1: _cache_lib.FD_DTYPE_E2M1}
 
 
 def cache_dim(k_cache: torch.Tensor) -> int:
     """Features of a cache's rows."""
-    return k_cache.shape[-1] * (2 if k_cache.dtype == _E2M1 else 1)
+    return k_cache.shape[-1] * 2 if k_cache.dtype is E2M1 else k_cache.shape[-1]
 
 
 def check_cache(k_cache, v_cache, page_table, cache_lens, k_scale, v_scale, requests) -> bytes:
@@ -49,21 +48,22 @@ def check_cache(k_cache, v_cache, page_table, cache_lens, k_scale, v_scale, requ
     shape = k_cache.shape
     if len(shape) != 4 or v_cache.shape != shape:
         raise ValueError("k_cache and v_cache must be [n_pages, Hkv, page_size, D] of one shape")
-    n_pages, heads, page_size, _ = shape
+    n_pages, heads, page_size, dim = shape
     device = k_cache.get_device()
     if device < 0 or v_cache.get_device() != device:
         raise ValueError("The caches must share a CUDA device")
     dtype = k_cache.dtype
-    if dtype not in _DTYPES or v_cache.dtype != dtype:
+    if (dtype is not _BF16 and dtype is not _E4M3 and dtype is not E2M1) or v_cache.dtype is not dtype:
         raise ValueError("The caches must both be BF16, float8_e4m3fn or float4_e2m1fn_x2")
-    dim = cache_dim(k_cache)
+    if dtype is E2M1:
+        dim *= 2
     if dim not in HEAD_DIMS:
         raise ValueError("The cache's head dimension must be 64, 128 or 256")
     if page_size not in PAGE_SIZES:
         raise ValueError("page_size must be a power of two in [16, 256]")
     if n_pages < 1 or heads < 1:
         raise ValueError("The cache needs at least one page and one head")
-    codes = dtype != _BF16
+    codes = dtype is not _BF16
     k_ptr, v_ptr = k_cache.data_ptr(), v_cache.data_ptr()
     strides = k_cache.stride()
     if v_cache.stride() != strides:
@@ -72,14 +72,15 @@ def check_cache(k_cache, v_cache, page_table, cache_lens, k_scale, v_scale, requ
     if sd != 1 or (k_ptr | v_ptr) % 16 or (sp | sh | sr) % (16 if codes else 8) or sr >= 1 << 20:
         raise ValueError("Cache rows must be contiguous and 16-byte aligned")
     ks = vs = ssp = ssh = 0
+    code = _lib.FD_DTYPE_BF16
     if codes:
-        if dtype == _E2M1:
-            per = dim // SCALE_BLOCK  # scale bytes of a row
+        if dtype is E2M1:
+            code, per = _cache_lib.FD_DTYPE_E2M1, dim // SCALE_BLOCK  # scale bytes of a row
             want = (n_pages, heads, page_size, per)
         else:
-            per, want = 1, (n_pages, heads, page_size)
-        if (k_scale is None or v_scale is None or k_scale.shape != want or v_scale.shape != want or k_scale.dtype != _UINT8
-                or v_scale.dtype != _UINT8 or k_scale.get_device() != device or v_scale.get_device() != device):
+            code, per, want = _cache_lib.FD_DTYPE_E4M3, 1, (n_pages, heads, page_size)
+        if (k_scale is None or v_scale is None or k_scale.shape != want or v_scale.shape != want or k_scale.dtype is not _UINT8
+                or v_scale.dtype is not _UINT8 or k_scale.get_device() != device or v_scale.get_device() != device):
             raise ValueError("An e4m3 cache needs k_scale and v_scale: uint8 [n_pages, Hkv, page_size] on its device; a 4-bit "
                              "one uint8 [n_pages, Hkv, page_size, D / 32]")
         ks, vs = k_scale.data_ptr(), v_scale.data_ptr()
@@ -91,22 +92,21 @@ def check_cache(k_cache, v_cache, page_table, cache_lens, k_scale, v_scale, requ
             raise ValueError("Scale rows must be contiguous, and those of a 4-bit cache aligned to their D / 32 bytes")
     elif k_scale is not None or v_scale is not None:
         raise ValueError("A BF16 cache has no scales")
-    max_pages = page_table.shape[-1]
-    table_stride = page_table.stride()
-    if (page_table.shape != (requests, max_pages) or max_pages < 1 or page_table.dtype != _INT32
+    table_shape, table_stride = page_table.shape, page_table.stride()
+    max_pages = table_shape[-1]
+    if (table_shape != (requests, max_pages) or max_pages < 1 or page_table.dtype is not _INT32
             or page_table.get_device() != device or table_stride[1] != 1):
         raise ValueError(f"page_table must be int32 [{requests}, max_pages] on the cache's device, its rows contiguous")
     if max_pages * page_size >= 1 << 27:
         raise ValueError("A request holds fewer than 2^27 keys")
     lens = 0
     if cache_lens is not None:
-        if (cache_lens.shape != (requests,) or cache_lens.dtype != _INT32 or cache_lens.get_device() != device
+        if (cache_lens.shape != (requests,) or cache_lens.dtype is not _INT32 or cache_lens.get_device() != device
                 or not cache_lens.is_contiguous()):
             raise ValueError(f"cache_lens must be a contiguous int32 vector [{requests}] on the cache's device")
         lens = cache_lens.data_ptr()
     return _cache_lib.pack_cache(k_ptr, v_ptr, ks, vs, sp, sh, sr, sp, sh, sr, ssp, ssh, ssp, ssh, page_table.data_ptr(),
-                                 table_stride[0], lens, n_pages, page_size, max_pages, heads, dim,
-                                 _DTYPES[dtype])
+                                 table_stride[0], lens, n_pages, page_size, max_pages, heads, dim, code)
 
 
 def check_cu_seqlens(cu_seqlens, batch, device) -> tuple[int | None, int]:
@@ -115,15 +115,16 @@ def check_cu_seqlens(cu_seqlens, batch, device) -> tuple[int | None, int]:
         return None, 0
     if batch != 1:
         raise ValueError("cu_seqlens requires batch size 1 (packed requests)")
-    if (cu_seqlens.ndim != 1 or cu_seqlens.dtype != _INT32 or cu_seqlens.get_device() != device
-            or cu_seqlens.numel() < 2 or not cu_seqlens.is_contiguous()):
+    shape = cu_seqlens.shape
+    if (len(shape) != 1 or cu_seqlens.dtype is not _INT32 or cu_seqlens.get_device() != device
+            or shape[0] < 2 or not cu_seqlens.is_contiguous()):
         raise ValueError("cu_seqlens must be a contiguous int32 vector [n_seqs + 1] on the cache's device")
-    return cu_seqlens.data_ptr(), cu_seqlens.numel() - 1
+    return cu_seqlens.data_ptr(), shape[0] - 1
 
 
 def check_rows(name: str, t: torch.Tensor, shape, device: int) -> tuple[int, bytes]:
     """(pointer, packed strides) of a bf16 tensor of rows."""
-    if t.shape != shape or t.dtype != _BF16 or t.get_device() != device:
+    if t.shape != shape or t.dtype is not _BF16 or t.get_device() != device:
         raise ValueError(f"{name} must be BF16 {list(shape)} on the cache's device")
     strides, ptr = t.stride(), t.data_ptr()
     sb, sh, st, sd = strides
