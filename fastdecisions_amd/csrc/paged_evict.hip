@@ -1,15 +1,16 @@
 // Eviction from a paged cache, gfx950: of every request the `recent` last keys and, per key head, those of largest
 // weight stay, `keep` in all, and move in their order to pages of their own.
 //
-//   select  one workgroup per (request, head): the weight of the last key that stays by three counting passes over
-//           11, 11 and 10 bits of the weights in an order-preserving integer form, then one pass that numbers the keys
-//           that stay in their order (a key above the weight, and as many at it as there is room for, lowest first) and
-//           moves their weights
+//   select  one workgroup per (request, head): the weight of the last key that stays by up to three counting passes
+//           over 11, 11 and 10 bits of the weights in an order-preserving integer form (fewer where all keys of a count
+//           stay), then one pass that numbers the keys that stay in their order (a key above the weight, and as many at
+//           it as there is room for, lowest first) and moves their weights
 //   move    rows and scales of the kept keys, a lane per 16 bytes, two rows each; streaming
 //
 // Select is bound by the latency of one workgroup (12 requests x 4 heads: 48 of 256 CUs): weights of up to 16384 keys are
-// loaded once and stay in registers (from memory in every pass: 21 us for 1500 to 16384 keys, now 15; 700 keys 7.8), 3
-// passes of LDS atomics over 2048 bins, and a barrier per 4096 keys when they are numbered.  A cut of a head over several
+// loaded once and stay in registers (from memory in every pass: 21 us for 1500 to 10411 keys, now 14 to 15; 700 keys
+// 7.0, with three passes always 7.8), then passes of LDS atomics over 2048 bins, and a barrier per 4096 keys when they are
+// numbered.  A cut of a head over several
 // workgroups would need a launch per pass, 3 to 4 us each.  Move: 50 MB in 10.4 us, 4.8 TB/s.
 #include <algorithm>
 #include <type_traits>
@@ -49,7 +50,7 @@ __device__ __forceinline__ uint32_t order_of(float w) {
 __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(EvictArgs a) {
   __shared__ int bins[kBins];
   __shared__ int wave_sums[2][kSelectWaves];
-  __shared__ int found[2];
+  __shared__ int found[3];
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
   const int req = blockIdx.x / a.heads, head = blockIdx.x % a.heads;
   const int len = request_keys(a.c, req), left = min(len, a.keep), recent = min(a.recent, left);
@@ -91,7 +92,7 @@ __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(EvictArgs 
 
   // ---- the weight at the border: its leading bits, and how many keys of those bits stay
   uint32_t border = 0;
-  int room = need;
+  int room = need, bits = 0;  // of a weight below the leading ones
   if (need > 0 && need < fixed) {
     const int shifts[3] = {21, 10, 0};
 #pragma unroll 1
@@ -121,10 +122,13 @@ __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(EvictArgs 
         const bool first = room <= before + c0;
         found[0] = first ? b0 : b0 - 1;
         found[1] = room - before - (first ? 0 : c0);
+        found[2] = first ? c0 : c1;
       }
       __syncthreads();
       border |= static_cast<uint32_t>(found[0]) << shift;
       room = found[1];
+      bits = shift;
+      if (room == found[2]) break;  // all of these bits stay: what follows them does not matter
     }
   }
   const bool all = need >= fixed;
@@ -138,9 +142,9 @@ __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(EvictArgs 
 #pragma unroll
     for (int u = 0; u < kPer; ++u) {
       const int j = j0 + tid * kPer + u;
-      const uint32_t key = order_of(y[u]);
-      is_above[u] = j < len && (j >= fixed || all || (need > 0 && key > border));
-      is_equal[u] = !is_above[u] && j < fixed && need > 0 && key == border;
+      const uint32_t key = order_of(y[u]) >> bits, last = border >> bits;
+      is_above[u] = j < len && (j >= fixed || all || (need > 0 && key > last));
+      is_equal[u] = !is_above[u] && j < fixed && need > 0 && key == last;
       mine += (is_above[u] ? 1 : 0) + (is_equal[u] ? 1 << 16 : 0);
     }
     const int incl = wave_scan(mine), parity = (j0 / kChunk) & 1;
