@@ -46,13 +46,16 @@ def workspace_bytes(batch: int, q_heads: int, kv_heads: int, seq_len: int, head_
     return nbytes
 
 
-def check_weights(name, weights, heads, width, device) -> None:
-    if (weights.ndim != 3 or weights.dtype != torch.float32 or weights.get_device() != device or weights.shape[1] != heads
-            or weights.shape[2] < width or weights.stride(2) != 1):
+def check_weights(name, weights, heads, width, device) -> tuple[int, bytes]:
+    """(rows, packed strides) of the weights."""
+    shape, strides = weights.shape, weights.stride()
+    if (len(shape) != 3 or weights.dtype is not torch.float32 or weights.get_device() != device or shape[1] != heads
+            or shape[2] < width or strides[2] != 1):
         raise ValueError(f"{name} must be FP32 [rows, {heads}, at least {width}] on the cache's device, its keys contiguous")
-    (row, head, _), (rows, _, keys) = weights.stride(), weights.shape
+    (row, head, _), (rows, _, keys) = strides, shape
     if (rows > 1 and row < keys) or (heads > 1 and head < keys) or (rows > 1 and heads > 1 and row < heads * head and head < rows * row):
         raise ValueError(f"{name} must not hold two of its elements in the same memory")
+    return rows, _cache_lib.pack2(row, head)
 
 
 def check_row_indices(row_indices, requests, rows, device) -> int | None:
@@ -111,18 +114,19 @@ def paged_key_weights(
         raise ValueError("max_seqlen must lie in [0, T]")
     requests = n_seqs or batch
     cache = check_cache(k_cache, k_cache, page_table, cache_lens, k_scale, k_scale, requests)
-    check_weights("weights", weights, kv_heads, page_table.shape[1] * page_size, device)
-    index = check_row_indices(row_indices, requests, weights.shape[0], device)
+    max_pages = page_table.shape[1]
+    rows, w_strides = check_weights("weights", weights, kv_heads, max_pages * page_size, device)
+    index = check_row_indices(row_indices, requests, rows, device)
     q_ptr, q_strides = check_rows("Q", q, shape, device)
     if _cache_lib.current_device() != device:
         with torch.cuda.device(device):
             return paged_key_weights(q, k_cache, page_table, cache_lens, weights, k_scale=k_scale, scale=scale,
                                      cu_seqlens=cu_seqlens, max_seqlen=max_seqlen, last=last, row_indices=row_indices)
-    nbytes = workspace_bytes(batch, q_heads, kv_heads, seq_len, dim, page_size, page_table.shape[1], n_seqs, int(max_seqlen),
+    nbytes = workspace_bytes(batch, q_heads, kv_heads, seq_len, dim, page_size, max_pages, n_seqs, int(max_seqlen),
                              int(last or 0))
-    work = torch.empty(nbytes, device=q.device, dtype=torch.uint8)
+    work = q.new_empty((nbytes + 1) // 2)
     _cache_lib.check("fd_paged_key_weights", _cache_lib.lib().fd_paged_key_weights(
-        q_ptr, cache, weights.data_ptr(), q_strides, _cache_lib.pack2(*weights.stride()[:2]), weights.shape[0], index, batch,
+        q_ptr, cache, weights.data_ptr(), q_strides, w_strides, rows, index, batch,
         q_heads, seq_len, float(scale), int(last or 0), cu_ptr, n_seqs, int(max_seqlen), work.data_ptr(), nbytes,
         _cache_lib.raw_stream(device)))
 
@@ -155,7 +159,7 @@ def paged_kv_evict(
     _, heads, page_size, _ = k_cache.shape
     device = k_cache.get_device()
     cache = check_cache(k_cache, v_cache, page_table, cache_lens, k_scale, v_scale, requests)
-    check_weights("weights", weights, heads, max_pages * page_size, device)
+    rows, w_strides = check_weights("weights", weights, heads, max_pages * page_size, device)
     if weights_out is None:
         weights_out = weights
     elif weights_out is not weights:
@@ -165,20 +169,20 @@ def paged_kv_evict(
         gap = abs(weights.data_ptr() - weights_out.data_ptr()) // 4
         if 0 < gap <= sum((n - 1) * s for n, s in zip(weights.shape, weights.stride())):
             raise ValueError("weights and weights_out must be the same memory or not overlap")
-    if (new_table.ndim != 2 or new_table.shape[0] != requests or new_table.dtype != torch.int32
-            or new_table.get_device() != device or new_table.stride(1) != 1 or new_table.shape[1] * page_size < keep):
+    new_shape, new_strides = new_table.shape, new_table.stride()
+    if (len(new_shape) != 2 or new_shape[0] != requests or new_table.dtype is not torch.int32
+            or new_table.get_device() != device or new_strides[1] != 1 or new_shape[1] * page_size < keep):
         raise ValueError(f"new_table must be int32 [{requests}, n] on the cache's device, its rows contiguous, and hold {keep} keys")
     if requests * heads * keep >= 1 << 27:
         raise ValueError("requests * Hkv * keep must be below 2^27")
-    index = check_row_indices(row_indices, requests, weights.shape[0], device)
+    index = check_row_indices(row_indices, requests, rows, device)
     if _cache_lib.current_device() != device:
         with torch.cuda.device(device):
             return paged_kv_evict(k_cache, v_cache, page_table, cache_lens, weights, new_table, keep, recent=recent,
                                   k_scale=k_scale, v_scale=v_scale, weights_out=weights_out, row_indices=row_indices)
-    kept = torch.empty((requests, heads, keep), device=k_cache.device, dtype=torch.int32)
-    new_lens = torch.empty(requests, device=k_cache.device, dtype=torch.int32)
+    kept, new_lens = page_table.new_empty((requests, heads, keep)), page_table.new_empty(requests)
     _cache_lib.check("fd_paged_kv_evict", _cache_lib.lib().fd_paged_kv_evict(
-        cache, weights.data_ptr(), weights_out.data_ptr(), _cache_lib.pack2(*weights.stride()[:2]), weights.shape[0], index,
-        new_table.data_ptr(), new_table.stride(0), new_table.shape[1], requests, keep, recent, kept.data_ptr(),
+        cache, weights.data_ptr(), weights_out.data_ptr(), w_strides, rows, index,
+        new_table.data_ptr(), new_strides[0], new_shape[1], requests, keep, recent, kept.data_ptr(),
         new_lens.data_ptr(), _cache_lib.raw_stream(device)))
     return kept, new_lens

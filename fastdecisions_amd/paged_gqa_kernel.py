@@ -88,10 +88,10 @@ def paged_gqa_attention(
             return paged_gqa_attention(q, k_cache, v_cache, page_table, cache_lens, k_scale=k_scale, v_scale=v_scale,
                                        scale=scale, cu_seqlens=cu_seqlens, max_seqlen=max_seqlen, gate=gate)
     strides = (seq_len * q_heads * dim, dim, q_heads * dim, 1)
-    out = torch.empty_strided(shape, strides, device=q.device, dtype=q.dtype)
+    out = q.new_empty_strided(shape, strides)
     nbytes = workspace_bytes(batch, q_heads, kv_heads, seq_len, dim, page_size, page_table.shape[1], n_seqs,
                              int(max_seqlen))
-    work = torch.empty(nbytes, device=q.device, dtype=torch.uint8) if nbytes > 0 else None
+    work = q.new_empty((nbytes + 1) // 2) if nbytes > 0 else None
     _cache_lib.check("fd_paged_gqa_fwd", _cache_lib.lib().fd_paged_gqa_fwd(
         q_ptr, cache, g_ptr, out.data_ptr(), q_strides, g_strides, _cache_lib.pack4(*strides), batch, q_heads, seq_len,
         float(scale), cu_ptr, n_seqs, int(max_seqlen), None if work is None else work.data_ptr(), nbytes,

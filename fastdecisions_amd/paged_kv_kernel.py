@@ -194,7 +194,7 @@ def paged_kv_read(
             return paged_kv_read(k_cache, v_cache, page_table, cu_seqlens, total, k_scale=k_scale, v_scale=v_scale)
     heads, dim = k_cache.shape[1], cache_dim(k_cache)
     strides = (total * heads * dim, dim, heads * dim, 1)
-    k = torch.empty_strided((1, heads, total, dim), strides, device=k_cache.device, dtype=_BF16)
+    k = k_cache.new_empty_strided((1, heads, total, dim), strides, dtype=_BF16)
     v = torch.empty_like(k)
     if total == 0:
         return k, v
