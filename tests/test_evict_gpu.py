@@ -127,3 +127,10 @@ def test_many_requests(held):
 def test_a_long_request():
     announce("evict, 150000 keys")
     check("e2m1", [150001, 70000], 9001, 333, 1, 64, 256, 6)
+
+
+def test_long_requests_in_place():
+    """Beyond the weights that stay in registers, their moves overtake no load; equal weights at the border."""
+    announce("evict in place, 16384 to 70000 keys")
+    check("e2m1", [70000, 16385, 16384, 40000], 1000, 50, 2, 64, 64, 7, weights=some_equal, in_place=True)
+    check("bf16", [33000, 20000], 18000, 0, 1, 64, 256, 8, in_place=True)
