@@ -28,7 +28,8 @@ With ``key_weights=True`` the attention layers also sum the attention weight tha
 (``paged_evict_kernel``; of every step's tokens, or of its ``observe`` last ones per request), and ``evict`` cuts
 requests to the keys that drew most and the most recent ones: a prefix of thousands of tokens, cut once, is
 forked as before.  A request's next tokens have the positions behind all the tokens that it has seen
-(``position``), however few it holds (``length``).
+(``position``), however few it holds (``length``).  ``evict`` refuses requests with a step, still held by its maker,
+that has not run: its keys' rows are whatever their pages held before.
 
 ``CacheStep.again`` makes the next step of the same shape in the same device tensors, so a
 captured forward over a step can be replayed token after token.
@@ -44,6 +45,7 @@ at once as long as none of the calls above is made between them without that ord
 from __future__ import annotations
 
 from dataclasses import dataclass, field
+from weakref import WeakSet
 
 import torch
 
@@ -64,12 +66,14 @@ class CacheStep:
     positions: torch.Tensor       # int32 [1, total]
     buffer: torch.Tensor = field(repr=False)
     held: list[list[int]] = field(repr=False)  # the requests' pages; another request of a number has another list
+    opened: list[int] = field(repr=False)      # which requests of the cache they are, counted as they were opened
     ends: list[int]               # tokens of each request, the new ones included
     live: bool = True             # neither taken back nor failed
     begun: bool = False           # a forward over it has reached the layers
     ran: bool = False             # a forward over it has run
     captured: bool = False        # a forward over it is in a graph: its runs are replays, which are not seen here
     waiting: bool = False         # a forward over it was refused
+    written: bool = False         # an attention layer was called with it, by the model or by itself
 
     @property
     def max_new(self) -> int:
@@ -94,11 +98,13 @@ class CacheStep:
             self.cache._release(self.slots, self.new)
             raise
         self.ends = [self.cache._lens[slot] for slot in self.slots]
+        self.written &= not self.ran  # (calls of single layers leave no other sign)
         self.live, self.ran = True, False
         return self
 
     def cancel(self) -> None:
-        """Take back a step that has not run and is the last one of its requests, which then are as before it."""
+        """Take back a step that has not run and is the last one of its requests, which then are as before it.  Requests
+        whose keys were evicted since hold some that are never computed: they can only be closed."""
         if not self.live:
             raise RuntimeError("The step was cancelled already, or has failed")
         if self.ran:
@@ -110,6 +116,8 @@ class CacheStep:
         if any(self.cache._users[page] > 1 for i, at in zip(mine, first) for page in self.held[i][at:]):
             raise RuntimeError("A fork of one of its requests holds tokens of the step")
         self.cache._release([self.slots[i] for i in mine], [self.new[i] for i in mine])
+        self.cache._lost.update(slot for i, slot in enumerate(self.slots)
+                                if i not in mine and self.cache._opened.get(slot) == self.opened[i])
         self.live = False
         self._settle()
 
@@ -143,6 +151,8 @@ class CacheStep:
             if not self._capturing():
                 self.cache._lost.update(self.slots)
                 self.live = False
+            else:
+                self.written = False
         elif not (self.ran or self.captured):
             self.waiting = True
             for slot, end in zip(self.slots, self.ends):
@@ -152,6 +162,11 @@ class CacheStep:
 
     def _end(self, slot) -> int:
         return self.ends[self.slots.index(slot)]
+
+    def _pending(self) -> bool:
+        """No forward has run over it or is in a graph, and one may come.  (None does over a cache in host memory: its steps
+        keep the books alone.)"""
+        return self.live and not (self.ran or self.captured or self.written) and self.positions.is_cuda
 
     def _capturing(self) -> bool:
         return self.positions.is_cuda and torch.cuda.is_current_stream_capturing()
@@ -221,6 +236,9 @@ class DeciderCache:
         self._pages: dict[int, list[int]] = {}        # of an open request
         self._lens: dict[int, int] = {}               # keys it holds
         self._seen: dict[int, int] = {}               # tokens it has seen: the position of its next one
+        self._opened: dict[int, int] = {}             # open requests, counted as they were opened
+        self._steps: WeakSet[CacheStep] = WeakSet()   # those that somebody holds
+        self._opens = 0
         self._waiting: dict[int, list[CacheStep]] = {}  # the refused steps of an open request, in order
         self._lost: set[int] = set()                  # open requests that a failed forward left half computed
 
@@ -235,7 +253,7 @@ class DeciderCache:
         self.delta[:, slot].zero_()
         if self.weights is not None:
             self.weights[:, slot].zero_()
-        self._pages[slot], self._lens[slot], self._seen[slot] = [], 0, 0
+        self._enter(slot, [], 0, 0)
         return slot
 
     def fork(self, parent: int) -> int:
@@ -261,14 +279,18 @@ class DeciderCache:
         self.delta[:, slot] = self.delta[:, parent]
         if self.weights is not None:
             self.weights[:, slot] = self.weights[:, parent]
-        self._pages[slot], self._lens[slot], self._seen[slot] = list(own), n, self._seen[parent]
+        self._enter(slot, list(own), n, self._seen[parent])
         return slot
+
+    def _enter(self, slot, pages, length, seen) -> None:
+        self._pages[slot], self._lens[slot], self._seen[slot], self._opened[slot] = pages, length, seen, self._opens
+        self._opens += 1
 
     def close(self, slot: int) -> None:
         """End a request; pages nobody else holds become free."""
         self._check_open([slot])
         self._give(self._pages.pop(slot))
-        del self._lens[slot], self._seen[slot]
+        del self._lens[slot], self._seen[slot], self._opened[slot]
         self._lost.discard(slot)
         self._waiting.pop(slot, None)
         self._free_slots.append(slot)
@@ -287,7 +309,8 @@ class DeciderCache:
         """Cut requests to ``keep`` keys: in every attention layer and key head the ``recent`` last ones and of the others
         those that drew most attention.  A request that holds no more stays as it is.  The kept keys move to free pages
         (``keep`` tokens of each request, before the old ones become free; requests may be cut one by one); pages that
-        forks share stay theirs.  Steps made before are refused afterwards: run or cancel them first."""
+        forks share stay theirs.  Steps made before are refused afterwards, and so must be the replays of captured ones; a
+        step that has not run is run or cancelled first."""
         from .cached_ops import paged_kv_evict_op
         slots, keep, recent = list(slots), int(keep), int(recent)
         if self.weights is None:
@@ -300,6 +323,10 @@ class DeciderCache:
         cut = [slot for slot in slots if self._lens[slot] > keep]
         if not cut:
             return
+        for step in self._steps:
+            for slot, pages in zip(step.slots, step.held):
+                if slot in cut and self._pages[slot] is pages and step._pending():
+                    raise RuntimeError(f"A step of request {slot} has not run: run it or cancel it before its keys are evicted")
         need = -(-keep // self.page_size)
         if need * len(cut) > len(self._free_pages):
             raise RuntimeError(f"The cache has {len(self._free_pages)} free pages, the eviction needs {need * len(cut)}")
@@ -341,8 +368,11 @@ class DeciderCache:
             raise
         n, total = len(slots), sum(new)
         cu, lens, idx, table, pos = buffer.split([n + 1, n, n, n * self.max_pages, total])
-        return CacheStep(self, slots, new, cu, lens, idx, table.view(n, self.max_pages), pos.view(1, total), buffer,
-                         [self._pages[slot] for slot in slots], [self._lens[slot] for slot in slots])
+        step = CacheStep(self, slots, new, cu, lens, idx, table.view(n, self.max_pages), pos.view(1, total), buffer,
+                         [self._pages[slot] for slot in slots], [self._opened[slot] for slot in slots],
+                         [self._lens[slot] for slot in slots])
+        self._steps.add(step)
+        return step
 
     def _check_open(self, slots) -> None:
         for slot in slots:

@@ -143,6 +143,7 @@ def _cached_forward(self, hidden_states, position_embeddings, step):
         q, k = (t.contiguous() for t in apply_rotary_pos_emb(q, k, *position_embeddings))
     k_cache, v_cache, k_scale, v_scale = step.cache.attention_layer(self.layer_idx)
     paged_kv_write_op(k, v, k_cache, v_cache, step.page_table, step.cache_lens, k_scale, v_scale, step.cu_seqlens)
+    step.written = True
     weights = step.cache.key_weights(self.layer_idx)
     if weights is not None:
         paged_key_weights_op(q, k_cache, step.page_table, step.cache_lens, weights, k_scale, step.cu_seqlens, step.max_new,
