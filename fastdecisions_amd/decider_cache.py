@@ -327,6 +327,8 @@ class DeciderCache:
             for slot, pages in zip(step.slots, step.held):
                 if slot in cut and self._pages[slot] is pages and step._pending():
                     raise RuntimeError(f"A step of request {slot} has not run: run it or cancel it before its keys are evicted")
+        if len(cut) * self.shape.num_key_value_heads * keep >= 1 << 27:  # (refused by the first layer, it would cost the requests)
+            raise ValueError("requests * Hkv * keep must be below 2^27: cut fewer requests at once")
         need = -(-keep // self.page_size)
         if need * len(cut) > len(self._free_pages):
             raise RuntimeError(f"The cache has {len(self._free_pages)} free pages, the eviction needs {need * len(cut)}")

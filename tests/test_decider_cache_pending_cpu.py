@@ -98,3 +98,18 @@ def test_a_failed_step_holds_back_nothing_else(calls):  # noqa: F811
     c._lost.add(a)
     c.evict([b], 20)
     assert c.length(b) == 20
+
+
+def test_more_kept_keys_than_an_eviction_moves():
+    """Refused before anything has moved, where the kernels' entry point refuses it too: the requests stay as they are."""
+    from fastdecisions_amd.decider_cache import DeciderCache
+    from fastdecisions_amd.model import TINY
+    keep = (1 << 26) // TINY.num_key_value_heads
+    c = DeciderCache(TINY, requests=2, tokens=4 * keep + 1024, max_tokens=keep + 1, page_size=256, key_weights=True, device="meta")
+    slots = [c.open(), c.open()]
+    for s in slots:
+        c._pages[s], c._lens[s], c._seen[s] = [c._take() for _ in range(keep // 256 + 1)], keep + 1, keep + 1
+    free = len(c._free_pages)
+    with pytest.raises(ValueError, match=r"below 2\^27"):
+        c.evict(slots, keep)
+    assert not c._lost and len(c._free_pages) == free and c.length(slots[0]) == keep + 1
