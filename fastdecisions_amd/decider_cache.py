@@ -28,8 +28,8 @@ With ``key_weights=True`` the attention layers also sum the attention weight tha
 (``paged_evict_kernel``; of every step's tokens, or of its ``observe`` last ones per request), and ``evict`` cuts
 requests to the keys that drew most and the most recent ones: a prefix of thousands of tokens, cut once, is
 forked as before.  A request's next tokens have the positions behind all the tokens that it has seen
-(``position``), however few it holds (``length``).  ``evict`` refuses requests with a step, still held by its maker,
-that has not run: its keys' rows are whatever their pages held before.
+(``position``), however few it holds (``length``).  ``evict`` refuses requests with a step that has not run: its
+keys' rows are whatever their pages held before.
 
 ``CacheStep.again`` makes the next step of the same shape in the same device tensors, so a
 captured forward over a step can be replayed token after token.
@@ -168,6 +168,10 @@ class CacheStep:
         keep the books alone.)"""
         return self.live and not (self.ran or self.captured or self.written) and self.positions.is_cuda
 
+    def __del__(self):
+        if self._pending():
+            self.cache._dropped.update(zip(self.slots, self.opened))
+
     def _capturing(self) -> bool:
         return self.positions.is_cuda and torch.cuda.is_current_stream_capturing()
 
@@ -238,6 +242,7 @@ class DeciderCache:
         self._seen: dict[int, int] = {}               # tokens it has seen: the position of its next one
         self._opened: dict[int, int] = {}             # open requests, counted as they were opened
         self._steps: WeakSet[CacheStep] = WeakSet()   # those that somebody holds
+        self._dropped: dict[int, int] = {}            # requests (as in _opened) whose step was dropped before it had run
         self._opens = 0
         self._waiting: dict[int, list[CacheStep]] = {}  # the refused steps of an open request, in order
         self._lost: set[int] = set()                  # open requests that a failed forward left half computed
@@ -323,6 +328,9 @@ class DeciderCache:
         cut = [slot for slot in slots if self._lens[slot] > keep]
         if not cut:
             return
+        for slot in cut:
+            if self._dropped.get(slot) == self._opened[slot]:
+                raise RuntimeError(f"A step of request {slot} was dropped before it had run: its keys cannot be chosen from")
         for step in self._steps:
             for slot, pages in zip(step.slots, step.held):
                 if slot in cut and self._pages[slot] is pages and step._pending():

@@ -113,3 +113,26 @@ def test_more_kept_keys_than_an_eviction_moves():
     with pytest.raises(ValueError, match=r"below 2\^27"):
         c.evict(slots, keep)
     assert not c._lost and len(c._free_pages) == free and c.length(slots[0]) == keep + 1
+
+
+def test_a_dropped_step_holds_back_an_eviction(calls):  # noqa: F811
+    """Nobody can run it or take it back any more, as after an error between a step and its forward."""
+    c = make()
+    a, b = c.open(), c.open()
+    c.step([a, b], [5, 30])
+    step = on_a_gpu(c.step([a], [50]))
+    del step
+    with pytest.raises(RuntimeError, match="dropped before it had run"):
+        c.evict([b, a], 10)
+    assert not calls
+    c.evict([b], 10)
+    c.close(a)
+    assert c.open() == a
+    c.step([a], [50])
+    c.evict([a], 10)                                       # another request
+    for end in ("ran", "live"):                            # run or taken back, then dropped
+        step = on_a_gpu(c.step([a], [3]))
+        setattr(step, end, end == "ran")
+        del step
+        c.evict([a], 10)
+    assert c.length(a) == 10
