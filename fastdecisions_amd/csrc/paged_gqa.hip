@@ -34,10 +34,13 @@
 // denominator sums the rounded p.
 //
 // e2m1 pages: v_cvt_scalef32_pk_bf16_fp4 takes codes times a block's scale to bf16,
-// exactly.  Few rows copy codes to LDS as they are; V's leave it at once, transposed
-// by nibbles, and are widened in registers: 256 to 8192 keys of 64 requests (97 MB)
-// 33 us and 4.8 for the join, 64 x 8192 keys 65 us (4.4 TB/s; e4m3 106, bf16 187).
-// The decoding, 4.4 cycles per 2 values and SIMD, then costs as much as the bytes.
+// exactly.  Few rows copy codes to LDS as they are, and a block's leave it for
+// registers at once, so that the next copies may follow.  K is widened there; V is
+// widened into LDS of the wavefront as bf16, 32 keys of up to 128 features at a time
+// (8 KiB), and read by the 16-bit transposing reads that bf16 pages take: 256 to 8192
+// keys of 64 requests (97 MB) 33 us and 4.8 for the join, 64 x 8192 keys 65 us (4.4
+// TB/s; e4m3 106, bf16 187).  The decoding, 4.4 cycles per 2 values and SIMD, and V's
+// way through LDS then cost as much as the bytes.
 // Pieces decode into their bf16 stages: 2048 tokens on 6144 keys 157 us (128
 // features; e4m3 159, bf16 139) and 174 (256; 175, 147).
 #include <algorithm>

@@ -27,6 +27,10 @@
 //   scores      S^T in fp32 into the workspace and the rows' (m, l) over the item's keys; streaming, no LDS
 //   scores add  the ranges joined, exp(s - m) / l summed over the rows; w read and written
 //
+// The scores' rows are as wide as the page table, which is all that the host knows of the lengths.  A table so wide that they
+// would pass kMostScores takes the two kernels above: a token each of 64 requests of 256 to 8192 keys behind up to 1024 pages
+// of 64 takes 40, 27 and 22 us a call (bf16, e4m3, 4 bits), behind 1025 pages 108, 105 and 98.
+//
 // bound by K's bytes and, for short calls, by the chain from lengths to items to pages (3.5 us).  A token each of 64
 // requests of 256 to 8192 keys (4 bits, 16/4 x 128, 37 MB): 15.7 + 6.4 us; by the two kernels above 94.  64 x 8192 keys:
 // bf16 144 us (3.7 TB/s of K alone, the scores are 67 MB more), 4 bits 48.
@@ -49,7 +53,7 @@ constexpr int kThreads = 256;
 constexpr int kWaves = 4;
 constexpr int kCus = 256;
 constexpr int kMostKeys = 1 << 27, kMostRows = 1 << 30;  // of a request
-constexpr int64_t kMostScores = 1LL << 28;  // bytes of kept scores: what the last-level cache may hold
+constexpr int64_t kMostScores = 1LL << 28;  // bytes of kept scores at the page table's width: what the last-level cache may hold
 
 struct WeightArgs {
   PagedView c;                  // K alone

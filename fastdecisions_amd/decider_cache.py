@@ -193,9 +193,12 @@ class DeciderCache:
         """``tokens``: cached tokens of all requests together (rounded up to pages, plus one partly filled
         page per request); ``max_tokens``: of one request (default ``tokens``), the width of the page tables.  A
         step writes its requests' tables whole: 64 of 3125 pages cost it 5.2 ms of host time, of 128 pages 0.33 ms.
-        ``key_weights``: sum the attention weight of every cached key, for ``evict`` (4 bytes per attention layer,
-        request, head and token of ``max_tokens``); ``observe``: of the last ``observe`` tokens of a step's requests
-        (default: all)."""
+        ``key_weights``: sum the attention weight of every cached key, for ``evict``.  The sums take 4 bytes per attention
+        layer, request, key head and token of ``max_tokens``, whatever the requests hold: 64 requests of up to 200,000
+        tokens (7 layers, 4 heads) 1.4 GB, twice their 4-bit pages; of up to 8192 59 MB.  Give ``max_tokens``: tokens one by
+        one are weighed fastest while query heads * requests of a step * ``max_tokens`` stay within 2^26 (64 requests of 256
+        to 8192 keys in 4 bits: 22 us a layer, beyond that 98).  ``observe``: of the last ``observe`` tokens of a step's
+        requests (default: all)."""
         if requests < 1 or tokens < 1:
             raise ValueError("requests and tokens must be positive")
         if page_size not in (16, 32, 64, 128, 256):

@@ -134,7 +134,8 @@ FD_API int fd_paged_kv_read(const fd_paged_cache* cache, void* k_out, void* v_ou
  * A row's last bits depend on how the call splits its keys, which follows from all requests' lengths.
  * Scores are fp32 sums, and p v is summed in fp32 before it is divided by the denominator, with a p of up to
  * 2^8: values from 2^120 / (keys seen) on may overflow where the quotient would not.
- * Masked or absent keys never reach a row, not even as NaN or infinities.
+ * Masked or absent keys never reach a row, not even as NaN or infinities.  An E4M3 value of 2^128 (fd_paged_kv_read) is
+ * infinite to the kernel for pieces.
  */
 FD_API int fd_paged_gqa_fwd(const void* q, const fd_paged_cache* cache, const void* gate, void* out,
                             const int64_t q_strides[4], const int64_t gate_strides[4], const int64_t out_strides[4],
@@ -158,8 +159,12 @@ FD_API int64_t fd_paged_gqa_workspace_bytes(int batch, int q_heads, int kv_heads
  *           one that an earlier request of the call names already, is no row: nothing is added for that request
  *   last    the last `last` new tokens of each request count; 0: all of them
  *   cu_seqlens, n_seqs, max_seqlen  as in fd_paged_gqa_fwd
- *   workspace  fd_paged_key_weights_workspace_bytes(...) bytes, 16-byte aligned; calls that may overlap need their own
+ *   workspace  fd_paged_key_weights_workspace_bytes(...) bytes, 16-byte aligned; calls that may overlap need their own.
+ *           With up to 16 rows (tokens times query heads of a key head) in the longest request it holds their scores, 4 bytes
+ *           for each of max_pages * page_size keys, up to 2^28 bytes in all; beyond that a call takes the kernels for more
+ *           rows, up to five times as long
  * Keys that no token sees keep their weight; a key that is NaN makes the weights of a row's keys NaN, as a softmax does.
+ * Scores that overflow fp32 do so too, and E4M3 values of 2^128 (fd_paged_kv_read) are infinite here.
  */
 FD_API int fd_paged_key_weights(const void* q, const fd_paged_cache* cache, float* weights, const int64_t q_strides[4],
                                 const int64_t weight_strides[2], int weight_rows, const int32_t* row_indices, int batch,
